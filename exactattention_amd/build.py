@@ -6,12 +6,12 @@ import os
 import subprocess
 import sys
 
-SOURCES = ["ea_hip.hip", "ea_decode.hip", "ea_mrow.hip", "ea_prefill.hip", "ea_exact_host.cpp", "ea_csr.cpp"]
+SOURCES = ["ea_hip.hip", "ea_decode.hip", "ea_mrow.hip", "ea_prefill.hip", "ea_step.hip", "ea_exact_host.cpp", "ea_csr.cpp"]
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libexactattn_hip.so")
 
-# -packed-fp32-ops: never emit packed fp32 VALU ops (their forms have misbehaved on this pool).
+# -packed-fp32-ops: never emit packed fp32 VALU ops (some of their forms have given wrong results).
 # -fno-gpu-flush-denormals-to-zero: bf16 subnormals convert exactly through fp32.
 # -amdgpu-mfma-vgpr-form=1: MFMA operands and accumulators in VGPRs; the prefill kernel's int32
 #  accumulators are also read by VALU folds, and the AGPR file then serves as cheap spill space

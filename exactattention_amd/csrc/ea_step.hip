@@ -1,0 +1,434 @@
+// What a serving step does before its attention call (gfx950): the step plan (block-table growth,
+// slots, positions and visible lengths from the requests' lengths) and the rotary positions of q and k
+// with the write into the paged cache. No reference counterpart: the reference's demo leaves its cache
+// and its positions to transformers (scripts/spec_decode_demo.py:116-125).
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "../../include/exactattn_hip.h"
+
+namespace {
+
+int herr(hipError_t e) { return e == hipSuccess ? 0 : -100 - (int)e; }
+
+// ------------------------------------------------------------------------------------------------
+// Step plan. Sequence b holds L_b keys in held_b = ceil(L_b / P) pages and takes c_b more:
+//   cu_b = sum of c before b, need_b = ceil((L_b + c_b) / P) - held_b, np_b = sum of need before b
+//   page i of the new ones of b is free[num_free - 1 - np_b - i] (a stack, its top first)
+//   token j of b, at flat index cu_b + j: position L_b + j, its page from the table when it has one
+//   there already, else from the stack; its pool row is page P + position % P
+// What bounds it is latency: 24 bytes a token leave it and a step of 100,000 tokens writes 3 MB. So it
+// is one launch: every block scans the sequences by itself (12 bytes each, from the L2 after the
+// first) and then takes its share of the tokens, pages and padded rows; no block reads what another
+// one writes (new pages come from the stack, not from the table), so no block waits for another.
+// Every input is checked by each block alike: a step that does not fit leaves the table alone and
+// reports why.
+// ------------------------------------------------------------------------------------------------
+constexpr int SP_THREADS = 1024;
+constexpr int SP_MAX_SEQS = 8192;
+constexpr int SP_MAX_ROWS = 65536;
+
+struct PlanSmem {
+    int64_t part[2][SP_THREADS / 64];
+    int status;
+};
+
+// inclusive sums over the block of two values per thread
+__device__ __forceinline__ void block_scan2(PlanSmem& S, int64_t& a, int64_t& b) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int64_t x = __shfl_up(a, o, 64), y = __shfl_up(b, o, 64);
+        if (lane >= o) {
+            a += x;
+            b += y;
+        }
+    }
+    if (lane == 63) {
+        S.part[0][w] = a;
+        S.part[1][w] = b;
+    }
+    __syncthreads();
+    for (int i = 0; i < w; ++i) {
+        a += S.part[0][i];
+        b += S.part[1][i];
+    }
+}
+
+// the last b in [0, n) with x[b] <= i: x ascends from x[0] = 0, x[n] > i
+__device__ __forceinline__ int find_seq(const int* x, int n, int i) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int m = (lo + hi) >> 1;
+        if (x[m] <= i) lo = m;
+        else hi = m;
+    }
+    return lo;
+}
+
+__global__ void __launch_bounds__(SP_THREADS) ea_step_plan_kernel(ea_step_plan A, int pshift) {
+    extern __shared__ __align__(16) int smem[];
+    __shared__ PlanSmem S;
+    const int tid = threadIdx.x, B = A.num_seqs, P = A.page_size;
+    int* const cu = smem;                       // B + 1
+    int* const np = smem + B + 1;               // B + 1
+    uint32_t* const seen = (uint32_t*)(smem + 2 * B + 2);  // a bit per table row
+    const int words = (A.table_rows + 31) / 32;
+    for (int i = tid; i < words; i += SP_THREADS) seen[i] = 0;
+    if (tid == 0) S.status = 0;
+    __syncthreads();
+    const int64_t room = min((int64_t)A.table_width << pshift, (int64_t)A.max_seq_len);
+    const int per = (B + SP_THREADS - 1) / SP_THREADS;
+    const int b0 = min(tid * per, B), b1 = min(b0 + per, B);
+    int bad = 0;
+    int64_t st = 0, sp = 0;
+    for (int b = b0; b < b1; ++b) {
+        const int64_t L = A.seq_len[b], c = A.counts[b];
+        const int s = A.slots ? A.slots[b] : b;
+        if (L < 0 || c < 0 || s < 0 || s >= A.table_rows) {
+            bad |= EA_PLAN_BAD_INPUT;
+            continue;
+        }
+        if (atomicOr(&seen[s >> 5], 1u << (s & 31)) >> (s & 31) & 1) bad |= EA_PLAN_BAD_INPUT;
+        if (L + c > room) bad |= EA_PLAN_TOO_LONG;
+        if (A.kv_len && c > A.pad_tokens) bad |= EA_PLAN_TOO_MANY;
+        st += c;
+        sp += ((L + c + P - 1) >> pshift) - ((L + P - 1) >> pshift);
+    }
+    int64_t at = st, ap = sp;
+    block_scan2(S, at, ap);
+    __syncthreads();  // part is read before the totals below reuse nothing of it
+    const int nf = *A.num_free;
+    if (tid == SP_THREADS - 1) {
+        if (at > A.max_tokens) bad |= EA_PLAN_TOO_MANY;
+        if (nf < 0 || nf > A.free_capacity) bad |= EA_PLAN_BAD_INPUT;
+        else if (ap > nf) bad |= EA_PLAN_NO_PAGES;
+    }
+    if (bad) atomicOr(&S.status, bad);
+    at -= st;
+    ap -= sp;
+    __syncthreads();
+    const int status = S.status;
+    if (!status) {
+        // sums below 2^31 from here on: at most max_tokens tokens, at most free_capacity pages
+        for (int b = b0; b < b1; ++b) {
+            const int L = A.seq_len[b], c = A.counts[b];
+            cu[b] = (int)at;
+            np[b] = (int)ap;
+            at += c;
+            ap += (((int64_t)L + c + P - 1) >> pshift) - (((int64_t)L + P - 1) >> pshift);
+        }
+        if (tid == SP_THREADS - 1) {
+            cu[B] = (int)at;
+            np[B] = (int)ap;
+        }
+    }
+    __syncthreads();
+    const int total = status ? 0 : cu[B], news = status ? 0 : np[B];
+    const int64_t g0 = (int64_t)blockIdx.x * SP_THREADS + tid, gs = (int64_t)gridDim.x * SP_THREADS;
+    if (g0 == 0) {
+        *A.status = status;
+        *A.new_num_free = nf - news;
+    }
+    for (int64_t b = g0; b < B; b += gs) A.new_seq_len[b] = A.seq_len[b] + (status ? 0 : cu[b + 1] - cu[b]);
+    for (int64_t i = g0; i < A.max_tokens; i += gs) {
+        int64_t dst = -1, qr = -1;
+        int pos = -1, b = -1;
+        if (i < total) {
+            b = find_seq(cu, B, (int)i);
+            const int L = A.seq_len[b], held = (int)(((int64_t)L + P - 1) >> pshift);
+            pos = L + ((int)i - cu[b]);
+            const int idx = pos >> pshift;
+            const int page = idx < held ? A.block_table[(int64_t)(A.slots ? A.slots[b] : b) * A.table_width + idx]
+                                        : A.free_pages[nf - 1 - (np[b] + idx - held)];
+            dst = ((int64_t)page << pshift) + (pos & (P - 1));
+            qr = (int64_t)b * A.pad_tokens + ((int)i - cu[b]);
+        }
+        A.dst_rows[i] = dst;
+        if (A.positions) A.positions[i] = pos;
+        if (A.seq_of) A.seq_of[i] = b;
+        if (A.q_rows) A.q_rows[i] = qr;
+    }
+    for (int64_t i = g0; i < news; i += gs) {
+        const int b = find_seq(np, B, (int)i);
+        const int held = (int)(((int64_t)A.seq_len[b] + P - 1) >> pshift);
+        A.block_table[(int64_t)(A.slots ? A.slots[b] : b) * A.table_width + held + ((int)i - np[b])] =
+            A.free_pages[nf - 1 - i];
+    }
+    if (A.kv_len) {
+        const int64_t n = (int64_t)B * A.pad_tokens;
+        for (int64_t i = g0; i < n; i += gs) {
+            const int b = (int)(i / A.pad_tokens), j = (int)(i - (int64_t)b * A.pad_tokens);
+            A.kv_len[i] = !status && j < cu[b + 1] - cu[b] ? A.seq_len[b] + j + 1 : 0;
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Rotary positions. Pair i of a head, (x, y) = elements (i, i + R/2) or (2i, 2i + 1), turns by the angle
+// theta = (position on axis(i)) * w_i:  (x cos - y sin, y cos + x sin) * scale, by -theta when inverse,
+// which is the transposed rotation and so the gradient's. Elements past R pass unchanged.
+// The angle is taken in half turns in fp64 (a position of 2^20 at frequency 1 still has an error below
+// 2^-32 of a turn) and the rotation in fp64 too, rounded once to the output type: 8 fp64 operations a pair cost
+// less than the pair's 8 bytes of traffic, so the exact form is free here.
+// What bounds it is memory: every element is read once and written once. A block takes whole tokens, so
+// the sines of a token are computed once for all its heads (LDS), and q, k and v of a token go in one
+// launch, k and v straight to their pool rows.
+// ------------------------------------------------------------------------------------------------
+constexpr int RT_THREADS = 256;
+constexpr int RT_MAX_PAIRS = 128;  // rot_dim at most 256
+
+// RN of a double to bf16 bits, one rounding: the fp32 value decides except where it is itself the
+// midpoint of two bf16 values and inexact; there the double's side of it does
+__device__ __forceinline__ uint32_t f64_bf16(double x) {
+    const float f = (float)x;
+    uint32_t b = __float_as_uint(f);
+    if ((b & 0x7FFFFFFFu) > 0x7F800000u) return (b >> 16) | 0x40u;
+    if ((b & 0xFFFFu) == 0x8000u) {
+        const double a = fabs(x), d = (double)fabsf(f);
+        b += (a > d ? 1u : 0u) - (a < d ? 1u : 0u);
+    }
+    return (b + 0x7FFFu + ((b >> 16) & 1u)) >> 16;
+}
+__device__ __forceinline__ uint32_t f32_bf16(float f) {
+    const uint32_t b = __float_as_uint(f);
+    if ((b & 0x7FFFFFFFu) > 0x7F800000u) return (b >> 16) | 0x40u;
+    return (b + 0x7FFFu + ((b >> 16) & 1u)) >> 16;
+}
+
+// V consecutive elements of type bf16 (FP32 = 0) or fp32, as doubles
+template <int V, bool FP32>
+struct Chunk {
+    uint32_t r[FP32 ? V : (V + 1) / 2];
+    __device__ __forceinline__ void load(const void* p, int64_t at) {
+        if constexpr (V == 8) {
+            const uint4* s = (const uint4*)((const char*)p + at * (FP32 ? 4 : 2));
+#pragma unroll
+            for (int i = 0; i < (FP32 ? 2 : 1); ++i) {
+                const uint4 x = s[i];
+                r[4 * i] = x.x;
+                r[4 * i + 1] = x.y;
+                r[4 * i + 2] = x.z;
+                r[4 * i + 3] = x.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                if constexpr (FP32) r[i] = ((const uint32_t*)p)[at + i];
+                else if (i & 1) r[i >> 1] |= (uint32_t)((const uint16_t*)p)[at + i] << 16;
+                else r[i >> 1] = ((const uint16_t*)p)[at + i];
+            }
+        }
+    }
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (FP32) return __uint_as_float(r[i]);
+        else return __uint_as_float(i & 1 ? r[i >> 1] & 0xFFFF0000u : r[i >> 1] << 16);
+    }
+    __device__ __forceinline__ void put(int i, double x) {
+        if constexpr (FP32) r[i] = __float_as_uint((float)x);
+        else if (i & 1) r[i >> 1] |= f64_bf16(x) << 16;
+        else r[i >> 1] = f64_bf16(x);
+    }
+    __device__ __forceinline__ void store(void* p, int64_t at) const {
+        if constexpr (V == 8) {
+            uint4* s = (uint4*)((char*)p + at * (FP32 ? 4 : 2));
+#pragma unroll
+            for (int i = 0; i < (FP32 ? 2 : 1); ++i) s[i] = make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                if constexpr (FP32) ((uint32_t*)p)[at + i] = r[i];
+                else ((uint16_t*)p)[at + i] = (uint16_t)(i & 1 ? r[i >> 1] >> 16 : r[i >> 1]);
+            }
+        }
+    }
+};
+
+// V elements from src to dst, another type or the same
+template <int V, bool IN32, bool OUT32>
+__device__ __forceinline__ void copy_chunk(const void* src, int64_t s, void* dst, int64_t d) {
+    Chunk<V, IN32> a;
+    a.load(src, s);
+    if constexpr (IN32 == OUT32) {
+        a.store(dst, d);
+    } else {
+        Chunk<V, OUT32> o;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const uint32_t h = f32_bf16(a.get(i));  // fp32 to bf16 only
+            if (i & 1) o.r[i >> 1] |= h << 16;
+            else o.r[i >> 1] = h;
+        }
+        o.store(dst, d);
+    }
+}
+
+// V = 8: 16-byte accesses throughout (the host has checked strides and alignment); V = 1 (pairs of
+// halves) or 2 (adjacent pairs): any stride
+template <int V, bool IN32, bool OUT32, bool ADJ>
+__global__ void __launch_bounds__(RT_THREADS) ea_rotary_kernel(ea_rotary A, int tpb) {
+    extern __shared__ __align__(16) double2 cs[];  // tpb x pairs of (cos, sin) * scale
+    const int h = A.rot_dim / 2, tid = threadIdx.x;
+    const int64_t t0 = (int64_t)blockIdx.x * tpb;
+    const int nt = (int)min((int64_t)tpb, A.num_tokens - t0);
+    for (int i = tid; i < nt * h; i += RT_THREADS) {
+        const int tk = i / h, p = i - tk * h;
+        const int axis = A.axis_of_pair ? A.axis_of_pair[p] : 0;
+        const double pos = (double)((int64_t)A.positions[axis * A.pos_axis_stride + t0 + tk] + A.pos_offset);
+        const double w = A.half_turns[p];
+        // pos w mod 2 half turns: the product's rounding error comes back by the FMA
+        const double x = pos * w, e = __fma_rn(pos, w, -x);
+        double sn, cn;
+        sincospi((x - 2.0 * rint(0.5 * x)) + e, &sn, &cn);
+        cs[i] = make_double2(cn * (double)A.scale, (A.inverse ? -sn : sn) * (double)A.scale);
+    }
+    __syncthreads();
+    const int d = A.head_dim;
+    const int pu = ADJ ? A.rot_dim / V : h / V;  // units of a head that turn, and its other ones
+    const int uh = pu + (d - A.rot_dim) / V, uv = d / V;
+    const int uq = A.num_q_heads * uh, uk = A.num_kv_heads * uh, ua = uq + uk + (A.v ? A.num_kv_heads * uv : 0);
+    for (int u = tid; u < nt * ua; u += RT_THREADS) {
+        const int tk = u / ua;
+        int r = u - tk * ua;
+        const int64_t t = t0 + tk;
+        const int64_t drow = A.dst_rows ? A.dst_rows[t] : t;
+        if (r >= uq + uk) {  // v
+            r -= uq + uk;
+            const int hd = r / uv, c = (r - hd * uv) * V;
+            if (drow < 0 || drow >= A.pool_rows) continue;
+            copy_chunk<V, IN32, OUT32>(A.v, t * A.v_tok_stride + hd * A.v_head_stride + c, A.v_out,
+                                       drow * A.vo_tok_stride + hd * A.vo_head_stride + c);
+            continue;
+        }
+        const bool isk = r >= uq;
+        if (isk) r -= uq;
+        const int hd = r / uh, c = r - hd * uh;
+        const int64_t orow = isk ? drow : (A.q_rows ? A.q_rows[t] : t);
+        if (orow < 0 || orow >= (isk ? A.pool_rows : A.q_out_rows)) continue;
+        const void* src = isk ? A.k : A.q;
+        void* dst = isk ? A.k_out : A.q_out;
+        const int64_t s = isk ? t * A.k_tok_stride + hd * A.k_head_stride : t * A.q_tok_stride + hd * A.q_head_stride;
+        const int64_t o = isk ? orow * A.ko_tok_stride + hd * A.ko_head_stride : orow * A.qo_tok_stride + hd * A.qo_head_stride;
+        if (c >= pu) {  // past the rotated dims
+            const int e = A.rot_dim + (c - pu) * V;
+            copy_chunk<V, IN32, OUT32>(src, s + e, dst, o + e);
+            continue;
+        }
+        const double2* z = cs + tk * h;
+        Chunk<V, IN32> a;
+        Chunk<V, OUT32> x;
+        if constexpr (ADJ) {
+            a.load(src, s + c * V);
+#pragma unroll
+            for (int i = 0; i < V; i += 2) {
+                const double2 q = z[(c * V + i) >> 1];
+                const double u0 = a.get(i), u1 = a.get(i + 1);
+                x.put(i, __fma_rn(u0, q.x, -(u1 * q.y)));
+                x.put(i + 1, __fma_rn(u1, q.x, u0 * q.y));
+            }
+            x.store(dst, o + c * V);
+        } else {
+            Chunk<V, IN32> b;
+            Chunk<V, OUT32> y;
+            a.load(src, s + c * V);
+            b.load(src, s + h + c * V);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const double2 q = z[c * V + i];
+                const double u0 = a.get(i), u1 = b.get(i);
+                x.put(i, __fma_rn(u0, q.x, -(u1 * q.y)));
+                y.put(i, __fma_rn(u1, q.x, u0 * q.y));
+            }
+            x.store(dst, o + c * V);
+            y.store(dst, o + h + c * V);
+        }
+    }
+}
+
+template <int V, bool ADJ>
+void rotary_launch(const ea_rotary& A, unsigned grid, size_t lds, int tpb, hipStream_t st) {
+    if (!A.in_fp32) hipLaunchKernelGGL((ea_rotary_kernel<V, false, false, ADJ>), dim3(grid), dim3(RT_THREADS), lds, st, A, tpb);
+    else if (A.out_fp32)
+        hipLaunchKernelGGL((ea_rotary_kernel<V, true, true, ADJ>), dim3(grid), dim3(RT_THREADS), lds, st, A, tpb);
+    else hipLaunchKernelGGL((ea_rotary_kernel<V, true, false, ADJ>), dim3(grid), dim3(RT_THREADS), lds, st, A, tpb);
+}
+
+}  // namespace
+
+extern "C" {
+
+int ea_hip_step_plan(const ea_step_plan* p, ea_stream_t stream) {
+    if (!p || p->num_seqs < 0 || p->num_seqs > SP_MAX_SEQS || p->max_tokens < 0 || p->pad_tokens < 0) return -1;
+    if (p->page_size <= 0 || (p->page_size & (p->page_size - 1))) return -1;
+    if (p->table_rows < 0 || p->table_rows > SP_MAX_ROWS || p->table_width < 0 || p->max_seq_len < 0 || p->free_capacity < 0)
+        return -1;
+    if (!p->num_free || !p->new_num_free || !p->status) return -1;
+    if (p->num_seqs > 0 && (!p->seq_len || !p->counts || !p->new_seq_len || !p->block_table)) return -1;
+    if (p->max_tokens > 0 && !p->dst_rows) return -1;
+    if (p->free_capacity > 0 && !p->free_pages) return -1;
+    if ((p->q_rows || p->kv_len) && p->pad_tokens <= 0) return -1;
+    // the blocks read these while others write those
+    if ((p->num_seqs > 0 && p->new_seq_len == p->seq_len) || p->new_num_free == p->num_free) return -1;
+    int ps = 0;
+    while ((1 << ps) < p->page_size) ++ps;
+    const int64_t work = std::max<int64_t>({p->max_tokens, p->kv_len ? (int64_t)p->num_seqs * p->pad_tokens : 0, p->num_seqs, 1});
+    const unsigned grid = (unsigned)std::min<int64_t>((work + 4 * SP_THREADS - 1) / (4 * SP_THREADS), 256);
+    const size_t lds = ((size_t)2 * p->num_seqs + 2) * 4 + (size_t)(p->table_rows + 31) / 32 * 4;  // at most 74 KB
+    if (lds > 60 * 1024) {  // beside the static part
+        const hipError_t e = hipFuncSetAttribute((const void*)ea_step_plan_kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                 (int)lds);
+        if (e != hipSuccess) return herr(e);
+    }
+    hipLaunchKernelGGL(ea_step_plan_kernel, dim3(grid), dim3(SP_THREADS), lds, (hipStream_t)stream, *p, ps);
+    return herr(hipGetLastError());
+}
+
+int ea_hip_rotary(const ea_rotary* a, ea_stream_t stream) {
+    if (!a || a->num_tokens < 0 || a->num_q_heads < 0 || a->num_kv_heads < 0) return -1;
+    const int d = a->head_dim, R = a->rot_dim, h = R / 2;
+    if (d <= 0 || d > 256 || R <= 0 || R > d || (R & 1) || h > RT_MAX_PAIRS) return -1;
+    if ((a->in_fp32 | 1) != 1 || (a->out_fp32 | 1) != 1 || (a->out_fp32 && !a->in_fp32)) return -2;
+    if (a->num_axes <= 0 || (a->num_axes > 1 && !a->axis_of_pair)) return -1;
+    if (!(a->scale - a->scale == 0.0f)) return -2;
+    if (a->num_tokens == 0 || a->num_q_heads + a->num_kv_heads == 0) return 0;
+    if (!a->positions || !a->half_turns || a->pool_rows < 0 || a->q_out_rows < 0) return -1;
+    if (a->num_q_heads > 0 && (!a->q || !a->q_out)) return -1;
+    if (a->num_kv_heads > 0 && (!a->k || !a->k_out || (a->v && !a->v_out))) return -1;
+    // 16-byte accesses: every row of every tensor starts on one
+    const int64_t in = a->in_fp32 ? 4 : 8, out = a->out_fp32 ? 4 : 8;
+    uintptr_t ptr = 0;
+    int64_t si = 0, so = 0;
+    if (a->num_q_heads > 0) {
+        ptr |= (uintptr_t)a->q | (uintptr_t)a->q_out;
+        si |= a->q_tok_stride | a->q_head_stride;
+        so |= a->qo_tok_stride | a->qo_head_stride;
+    }
+    if (a->num_kv_heads > 0) {
+        ptr |= (uintptr_t)a->k | (uintptr_t)a->k_out;
+        si |= a->k_tok_stride | a->k_head_stride;
+        so |= a->ko_tok_stride | a->ko_head_stride;
+        if (a->v) {
+            ptr |= (uintptr_t)a->v | (uintptr_t)a->v_out;
+            si |= a->v_tok_stride | a->v_head_stride;
+            so |= a->vo_tok_stride | a->vo_head_stride;
+        }
+    }
+    const bool wide = !(ptr & 15) && !(si & (in - 1)) && !(so & (out - 1)) && !(d & 7) && !((a->adjacent ? R : h) & 7);
+    if (!wide && a->adjacent && (d & 1)) return -1;  // the narrow form of adjacent pairs takes two elements at a time
+    const int tpb = a->num_tokens >= 4096 ? 4 : 1;
+    const int64_t grid = ((int64_t)a->num_tokens + tpb - 1) / tpb;
+    const size_t lds = (size_t)tpb * h * 16;
+    const hipStream_t st = (hipStream_t)stream;
+    if (a->adjacent) {
+        if (wide) rotary_launch<8, true>(*a, (unsigned)grid, lds, tpb, st);
+        else rotary_launch<2, true>(*a, (unsigned)grid, lds, tpb, st);
+    } else {
+        if (wide) rotary_launch<8, false>(*a, (unsigned)grid, lds, tpb, st);
+        else rotary_launch<1, false>(*a, (unsigned)grid, lds, tpb, st);
+    }
+    return herr(hipGetLastError());
+}
+
+}  // extern "C"

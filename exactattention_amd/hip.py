@@ -46,6 +46,25 @@ class Options(ctypes.Structure):
                 ("prefill_waves", ctypes.c_int32), ("stats_entries", ctypes.c_int32)]
 
 
+class StepPlanArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("num_seqs", "page_size", "table_rows", "table_width", "max_tokens", "pad_tokens",
+                                               "max_seq_len", "free_capacity")]
+                + [(n, P) for n in ("seq_len", "counts", "slots", "free_pages", "num_free", "block_table", "dst_rows",
+                                    "positions", "seq_of", "q_rows", "kv_len", "new_seq_len", "new_num_free", "status")])
+
+
+class RotaryArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("num_tokens", "num_q_heads", "num_kv_heads", "head_dim", "rot_dim", "num_axes",
+                                               "adjacent", "inverse", "in_fp32", "out_fp32", "pos_offset")]
+                + [("scale", ctypes.c_float)]
+                + [(n, ctypes.c_int64) for n in ("q_tok_stride", "q_head_stride", "k_tok_stride", "k_head_stride",
+                                                 "v_tok_stride", "v_head_stride", "qo_tok_stride", "qo_head_stride",
+                                                 "ko_tok_stride", "ko_head_stride", "vo_tok_stride", "vo_head_stride",
+                                                 "pos_axis_stride", "q_out_rows", "pool_rows")]
+                + [(n, P) for n in ("q", "k", "v", "positions", "half_turns", "axis_of_pair", "q_rows", "dst_rows", "q_out",
+                                    "k_out", "v_out")])
+
+
 # ea_options.kernel (include/exactattn_hip.h EA_KERNEL_*)
 KERNELS = {"auto": 0, "prefill": 1, "decode": 2, "general": 3}
 
@@ -110,6 +129,10 @@ def load():
         lib.ea_hip_kv_append.argtypes = [P, P, ctypes.c_int64, ctypes.c_int64, P, P, P, ctypes.c_int64, P,
                                          ctypes.c_int64, P, P, ctypes.c_int64, P]
         lib.ea_hip_kv_append.restype = ctypes.c_int
+        lib.ea_hip_step_plan.argtypes = [ctypes.POINTER(StepPlanArgs), P]
+        lib.ea_hip_step_plan.restype = ctypes.c_int
+        lib.ea_hip_rotary.argtypes = [ctypes.POINTER(RotaryArgs), P]
+        lib.ea_hip_rotary.restype = ctypes.c_int
         lib.ea_hip_kv_digits_bytes.argtypes = [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]
         lib.ea_hip_kv_digits_bytes.restype = ctypes.c_size_t
         lib.ea_hip_kv_digits_update.argtypes = [ctypes.POINTER(Geometry), ctypes.POINTER(Buffers), P, P,

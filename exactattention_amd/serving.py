@@ -29,6 +29,7 @@ import numpy as np
 
 from . import hip
 from .formats import ExactAttentionDomainError, ExactAttentionUncertifiedError, alpha_bits_for, alpha_fp32_bits
+from .step import Rotary, StepPlan  # noqa: F401
 
 TILE = 64  # keys per digit tile
 

@@ -331,6 +331,90 @@ int ea_hip_kv_digits_update(const ea_geometry* g, const ea_buffers* b, const int
                             const int32_t* key_end, int32_t max_new_keys, void* kv_digits, int32_t tiles_per_seq,
                             ea_stream_t stream);
 
+/* Step plan: where a serving step's new tokens go, from lengths that are on the device. Sequence b of
+ * the step (row slots[b] of the block table; NULL: row b) holds seq_len[b] keys in its first
+ * ceil(seq_len / page_size) pages and takes counts[b] >= 0 more. New pages are taken from the stack
+ * free_pages[0 .. num_free - 1], its last entry first, in the order of the sequences and of each
+ * sequence's pages. In one launch it writes
+ *   block_table   the new pages' entries, in place (other entries are not written)
+ *   dst_rows      per token, the tokens of sequence 0 first: its pool row page * page_size + slot, as
+ *                 ea_hip_kv_append and ea_hip_rotary take it; -1 past the last token
+ *   positions     its position seq_len[b] + j (-1 past the last token); optional
+ *   seq_of        its sequence b (-1 past the last token); optional
+ *   q_rows        its row b * pad_tokens + j among pad_tokens rows per sequence (-1 past the last
+ *                 token), the token rows of an ea_geometry with num_tokens = pad_tokens; optional
+ *   kv_len        num_seqs * pad_tokens visible lengths of those rows: seq_len[b] + j + 1, and 0 for rows
+ *                 without a token (which see nothing); optional
+ *   new_seq_len   seq_len[b] + counts[b];  new_num_free: the pages left on the stack
+ *   status        0, or why the step does not fit (EA_PLAN_* bits); then no entry of the table is
+ *                 written, lengths and stack are reported as they were, dst_rows, positions, seq_of and
+ *                 q_rows are -1 and kv_len is 0
+ * All pointers are device memory; new_seq_len and new_num_free must not be seq_len and num_free. Up to
+ * 8192 sequences and 65536 table rows; a row may appear once. Entries of the first pages and of
+ * free_pages are taken as they are. Enqueue only, capturable. Returns 0, -1 on bad arguments,
+ * -100 - e on a HIP error. No reference counterpart. */
+#define EA_PLAN_NO_PAGES 1  /* the stack holds fewer pages than the step needs */
+#define EA_PLAN_TOO_LONG 2  /* a sequence would pass max_seq_len or its table row */
+#define EA_PLAN_TOO_MANY 4  /* more than max_tokens tokens, or more than pad_tokens of a sequence */
+#define EA_PLAN_BAD_INPUT 8 /* a negative length or count, a row outside the table or twice, num_free */
+typedef struct ea_step_plan {
+    int32_t num_seqs, page_size;       /* page_size a power of two */
+    int32_t table_rows, table_width;   /* block_table [table_rows][table_width] */
+    int32_t max_tokens, pad_tokens;    /* entries of dst_rows ..; rows per sequence of kv_len, q_rows */
+    int32_t max_seq_len, free_capacity; /* entries of free_pages */
+    const int32_t* seq_len;
+    const int32_t* counts;
+    const int32_t* slots;
+    const int32_t* free_pages;
+    const int32_t* num_free;
+    int32_t* block_table;
+    int64_t* dst_rows;
+    int32_t* positions;
+    int32_t* seq_of;
+    int64_t* q_rows;
+    int32_t* kv_len;
+    int32_t* new_seq_len;
+    int32_t* new_num_free;
+    int32_t* status;
+} ea_step_plan;
+int ea_hip_step_plan(const ea_step_plan* p, ea_stream_t stream);
+
+/* Rotary positions of q and k, with k and v written to their rows of the paged cache (or anywhere).
+ * Pair i < rot_dim / 2 of a head is elements (i, i + rot_dim / 2), or (2 i, 2 i + 1) when adjacent; it
+ * turns by theta = pi * half_turns[i] * (positions[axis_of_pair[i]][token] + pos_offset):
+ *   (x, y) -> scale (x cos theta - y sin theta, y cos theta + x sin theta)
+ * with -theta when inverse, which gives the gradient of the rotation. Elements past rot_dim and v pass
+ * unchanged. Everything is computed in fp64 and rounded once to the output type. Inputs are bf16 (or
+ * fp32 with in_fp32), outputs bf16 (or fp32 with out_fp32, which needs in_fp32). Several position axes
+ * (time, height, width) share a head through axis_of_pair (NULL: one axis).
+ *   element c of head g of token t:  q + t q_tok_stride + g q_head_stride + c, k and v alike
+ *   outputs: row r of q_out is q_rows[t] (NULL: t), row r of k_out and v_out is dst_rows[t] (NULL: t);
+ *   rows outside [0, q_out_rows) or [0, pool_rows) are skipped
+ * v may be NULL (k alone). q_out may be q and k_out k where their strides and rows are the same.
+ * half_turns: num pairs fp64, the frequencies divided by pi. head_dim up to 256, rot_dim even. All
+ * pointers are device memory. Enqueue only, capturable. Returns 0, -1 on bad arguments, -2 on a bad type
+ * or scale, -100 - e on a HIP error. No reference counterpart. */
+typedef struct ea_rotary {
+    int32_t num_tokens, num_q_heads, num_kv_heads, head_dim, rot_dim, num_axes;
+    int32_t adjacent, inverse, in_fp32, out_fp32, pos_offset;
+    float scale;
+    int64_t q_tok_stride, q_head_stride, k_tok_stride, k_head_stride, v_tok_stride, v_head_stride;
+    int64_t qo_tok_stride, qo_head_stride, ko_tok_stride, ko_head_stride, vo_tok_stride, vo_head_stride;
+    int64_t pos_axis_stride, q_out_rows, pool_rows;
+    const void* q;
+    const void* k;
+    const void* v;
+    const int32_t* positions;
+    const double* half_turns;
+    const uint8_t* axis_of_pair; /* entries below num_axes */
+    const int64_t* q_rows;
+    const int64_t* dst_rows;
+    void* q_out;
+    void* k_out;
+    void* v_out;
+} ea_rotary;
+int ea_hip_rotary(const ea_rotary* a, ea_stream_t stream);
+
 /* Library version string. */
 const char* ea_hip_version(void);
 
