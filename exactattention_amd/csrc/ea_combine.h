@@ -7,8 +7,11 @@ namespace ea {
 
 // Returns the row's stats events, the same in every lane: bit 0 the row was merged (stats[0]),
 // bit 1 it is flagged (stats[1]), bit 2 only its final rounding failed (stats[7]). The caller
-// adds them up per block. MR: the multi-row kernel wrote the partials.
-template <int PRE, bool MR>
+// adds them up per block. MR: the multi-row kernel wrote the partials. MOD: with score modifications,
+// whose partials may lie any number of binades apart: those 2^-900 below the row's largest change no
+// decision (ea_mod.h; one more unit in the depth), and the multi-row kernel's tiles are counted from each
+// partial's own keys, because its last split takes what is past the others.
+template <int PRE, bool MR, bool MOD = false>
 __device__ inline int combine_row(const Params& P, int64_t row, int lane) {
     constexpr int SLAB = 2 * PRE;  // splits per load round past PRE of them
     const int dv = P.g.head_dim_v;
@@ -125,10 +128,15 @@ __device__ inline int combine_row(const Params& P, int64_t row, int lane) {
     int nterm = 0, far = 0;
     auto add_z = [&](int n, int r, double z) __attribute__((always_inline)) {
         const int dsh = shift_of(n, r);
-        far |= (n > 0 && dsh < -900) ? 1 : 0;
+        if constexpr (!MOD) far |= (n > 0 && dsh < -900) ? 1 : 0;
         const double zs = n > 0 ? ldexp(z, max(dsh, -1000)) : 0.0;
         Z += zs;
-        A += zs * (double)(min((int64_t)n + 4, dcap) + nsb);
+        if constexpr (MOD) {
+            const int64_t cap = MR ? 16 * (((int64_t)n + 63) >> 6) + 6 : INT64_MAX;
+            A += zs * (double)(min((int64_t)n + 4, cap) + nsb + 1);
+        } else {
+            A += zs * (double)(min((int64_t)n + 4, dcap) + nsb);
+        }
         nterm += n > 0 ? n : 0;
     };
     add_z(n0, r0, z0);

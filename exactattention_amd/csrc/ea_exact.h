@@ -22,14 +22,21 @@ struct KeyTrace {
     int64_t* we;
 };
 
+// Score modifications of a row (ea_mod.h): cap c (0: none), its query head's slope, and the distance
+// n - p of each of its n keys.
+struct RowMod {
+    float cap, slope;
+    const int32_t* dist;
+};
+
 // q: d bf16 bit patterns; K: n rows of d, V: n rows of dv (row-major, contiguous); alpha as fp32
 // bits; out: dv bf16 (uint16) or fp32 (uint32) bit patterns, +0 for zero. Returns EAX_OK,
 // EAX_DOMAIN for a NaN/inf input or an fp32 logit overflow (out untouched), or EAX_REFUSED when
 // deciding a rounding would need the exact sums over an exponent spread above 2^20 bits (the
 // reference's own limit, src/exactattn/reference.py:27-30), or EAX_NOMEM when the host heap is
-// exhausted (no exception leaves this function).
+// exhausted (no exception leaves this function). mod: the row's score modifications, if any.
 int exact_row(const uint16_t* q, int d, const uint16_t* K, const uint16_t* V, int64_t n, int dv, uint32_t alpha_bits,
-              int fp32, void* out, const KeyTrace* tr) noexcept;
+              int fp32, void* out, const KeyTrace* tr, const RowMod* mod = nullptr) noexcept;
 
 // RN-even of (a / b) * 2^E with a, b given as 128-bit (hi, lo) words, b > 0, into fp32 (p = 24)
 // or bf16 (p = 8) with gradual underflow. Returns the result's bit pattern (negated when neg) and

@@ -23,6 +23,8 @@
 #include <vector>
 
 #include "ea_exact.h"
+#include "ea_mod.h"
+#include "ea_tables.h"
 
 namespace eax {
 namespace {
@@ -488,8 +490,11 @@ const i128 SPREAD_LIMIT = (i128)1 << 20;
 namespace {
 
 int exact_row_body(const uint16_t* q, int d, const uint16_t* K, const uint16_t* V, int64_t n, int dv,
-                   uint32_t alpha_bits, int fp32, void* out, const KeyTrace* tr) {
+                   uint32_t alpha_bits, int fp32, void* out, const KeyTrace* tr, const RowMod* mod) {
     std::vector<int> qm(d), qe(d);
+    double T1[256];
+    memcpy(T1, EA_T1_BITS, sizeof(T1));
+    const ea::ModCap cap = ea::mod_cap_of(mod ? mod->cap : 0.0f);
     for (int i = 0; i < d; ++i)
         if (!dec_bf16(q[i], &qm[i], &qe[i])) return EAX_DOMAIN;
     for (int64_t j = 0; j < n; ++j) {
@@ -533,6 +538,13 @@ int exact_row_body(const uint16_t* q, int d, const uint16_t* K, const uint16_t* 
             tm = tneg ? -(int32_t)r.Q : (int32_t)r.Q;
             te = (int32_t)r.qe;
             tbits = encode(r, tneg, 1);
+        }
+        if (mod) {
+            if (ea::mod_logit(0, false, cap, mod->slope, mod->dist[j], T1, 0, &tbits)) return EAX_DOMAIN;
+            const int f = (int)((tbits >> 23) & 0xFF);
+            tm = (int32_t)((tbits & 0x7FFFFF) | (f ? 0x800000 : 0));
+            if (tbits >> 31) tm = -tm;
+            te = tm ? (f ? f : 1) - 150 : 0;
         }
         tmv[(size_t)j] = tm;
         tev[(size_t)j] = te;
@@ -677,9 +689,9 @@ int exact_row_body(const uint16_t* q, int d, const uint16_t* K, const uint16_t* 
 }  // namespace
 
 int exact_row(const uint16_t* q, int d, const uint16_t* K, const uint16_t* V, int64_t n, int dv, uint32_t alpha_bits,
-              int fp32, void* out, const KeyTrace* tr) noexcept {
+              int fp32, void* out, const KeyTrace* tr, const RowMod* mod) noexcept {
     try {
-        return exact_row_body(q, d, K, V, n, dv, alpha_bits, fp32, out, tr);
+        return exact_row_body(q, d, K, V, n, dv, alpha_bits, fp32, out, tr, mod);
     } catch (const std::bad_alloc&) {
         return EAX_NOMEM;
     } catch (...) {

@@ -44,11 +44,13 @@ using namespace ea;
 // (unit u, S_u, S_(u+1), share): the unit holding tile g share is the u with
 // S_u <= g share < S_(u+1), so the blocks g in [ceil(S_u / share), ceil(S_(u+1) / share)) start in
 // unit u and each is written by that unit's thread. Blocks past W get u = units. Every entry the
-// decode kernel and the combine read is written here.
-template <int NT>
+// decode kernel and the combine read is written here. MOD: with score modifications a unit's tiles are
+// those of unit_keys, from its first key's on, and the share is also at least the longest unit's over
+// the pieces it may have, instead of dq_min_share: the host knows no more than a hint of the span.
+template <int NT, bool MOD = false>
 __device__ void dq_plan_block(const Params& P) {
     __shared__ int s_scan[2][NT];
-    __shared__ int s_share;
+    __shared__ int s_share, s_most;
     const int tid = threadIdx.x, U = P.dq_units, G = P.dq_blocks;
     int32_t* plan = P.dq_plan;
     int32_t* Su = plan + 2;
@@ -56,12 +58,24 @@ __device__ void dq_plan_block(const Params& P) {
     const int per = (U + NT - 1) / NT;
     const int u0 = min(tid * per, U), u1 = min(u0 + per, U);
     // each thread's units twice: their tile counts, kept in Su, and then the prefix sums over them
-    int sum = 0;
+    int sum = 0, most = 0;
+    if constexpr (MOD) {
+        if (tid == 0) s_most = 0;
+        __syncthreads();
+    }
     for (int u = u0; u < u1; ++u) {
-        const int t = min((unit_kend(P, u / P.nrb, u % P.nrb) + 63) >> 6, P.dq_max_tiles);
+        int t;
+        if constexpr (MOD) {
+            const int2 k = unit_keys(P, u / P.nrb, u % P.nrb);
+            t = min(((k.y + 63) >> 6) - (k.x >> 6), P.dq_max_tiles);
+            most = max(most, t);
+        } else {
+            t = min((unit_kend(P, u / P.nrb, u % P.nrb) + 63) >> 6, P.dq_max_tiles);
+        }
         Su[u] = t;
         sum += t;
     }
+    if constexpr (MOD) atomicMax(&s_most, most);
     // inclusive scan of the chunk sums (Hillis-Steele, ping-pong)
     int cur = 0;
     s_scan[0][tid] = sum;
@@ -74,7 +88,9 @@ __device__ void dq_plan_block(const Params& P) {
     }
     const int W = s_scan[cur][NT - 1];
     if (tid == 0) {
-        const int share = max(max((W + G - 1) / G, P.dq_min_share), 1);
+        // (nsplit slots hold the pieces of a unit: one more than the whole shares it spans)
+        const int least = MOD ? (s_most + P.nsplit - 2) / (P.nsplit - 1) : P.dq_min_share;
+        const int share = max(max((W + G - 1) / G, least), 1);
         s_share = share;
         plan[0] = W;
         plan[1] = share;
@@ -96,9 +112,10 @@ __device__ void dq_plan_block(const Params& P) {
 }
 
 // The equal-share plan alone (the multi-row kernel's steps), and the cleared tier-2 work list.
+template <bool MOD>
 __global__ void __launch_bounds__(1024) ea_plan(Params P) {
     if (threadIdx.x < EA_T2_CNT) P.wl_cnt[threadIdx.x] = 0;
-    dq_plan_block<1024>(P);
+    dq_plan_block<1024, MOD>(P);
 }
 
 __global__ void __launch_bounds__(256) ea_prep(Params P) {
@@ -151,7 +168,9 @@ struct SplitSmem {
     uint32_t vred[4][64];                // 1 KB
 };
 
-template <int RB, bool TIMERS>
+// MOD: with score modifications (ea_mod.h); the key range starts at the block's first visible key, down to
+// a whole tile, and the last split takes every key past the others.
+template <int RB, bool TIMERS, bool MOD = false>
 __global__ void __launch_bounds__(EA_THREADS, 2) ea_split(Params P) {
     uint64_t tclk[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     uint64_t tprev = TIMERS ? __builtin_amdgcn_s_memtime() : 0;
@@ -213,8 +232,25 @@ __global__ void __launch_bounds__(EA_THREADS, 2) ea_split(Params P) {
     }
     const int64_t slen = P.seq_len[b];
     if (kend > slen) kend = slen;
-    const int64_t k0 = (int64_t)split * P.split_len;
-    const int64_t k1 = min(k0 + (int64_t)P.split_len, kend);
+    int64_t k0 = (int64_t)split * P.split_len;
+    int64_t k1 = min(k0 + (int64_t)P.split_len, kend);
+    int64_t kbeg = 0;
+    int my_kvb = 0, my_pos = 0;
+    float my_slope = 0.0f;
+    if constexpr (MOD) {
+        const int2 ks = unit_keys(P, seg, rbk);
+        kbeg = ks.x;
+        kend = ks.y;
+        k0 += tile_floor(ks.x);
+        k1 = split == (int)gridDim.y - 1 ? kend : min(k0 + (int64_t)P.split_len, kend);
+        if (brow_ok) {
+            const int lr = row0 + br;
+            const int64_t tok = b * P.g.num_tokens + lr / P.grp;
+            my_kvb = vis_begin(P, tok, (int)my_kvl);
+            my_pos = mod_pos(P, tok, (int)my_kvl);
+            my_slope = mod_slope(P, hk * P.grp + lr % P.grp);
+        }
+    }
     const int64_t pbase = (int64_t)split * P.rows;
     const int64_t bt_off = P.bt ? (P.bt_off ? P.bt_off[b] : b * (int64_t)P.g.block_table_stride) : 0;
     cint_t* bt4 = (cint_t*)P.bt;
@@ -248,7 +284,7 @@ __global__ void __launch_bounds__(EA_THREADS, 2) ea_split(Params P) {
     u32x4 kst[4];
     auto load_k = [&](int64_t n0) {
         int64_t n = n0 + kt;
-        bool ok = n < k1;
+        bool ok = n < k1 && (!MOD || n >= kbeg);
         int64_t page = b, slot = n;
         if (ok && P.bt) {
             page = P.bt[bt_off + (n >> P.pshift)];
@@ -278,7 +314,7 @@ __global__ void __launch_bounds__(EA_THREADS, 2) ea_split(Params P) {
         for (int kk = 0; kk < 16; ++kk) {
             int64_t n = n0 + 16 * w + kk;  // wave-uniform
             uint32_t val = 0;
-            if (n < k1) {
+            if (n < k1 && (!MOD || n >= kbeg)) {
                 int64_t page = b, slot = n;
                 if (P.bt) {
                     page = bt4[bt_off + (n >> P.pshift)];
@@ -368,7 +404,8 @@ __global__ void __launch_bounds__(EA_THREADS, 2) ea_split(Params P) {
             const int key = 16 * w + bk;
             const int64_t n = n0 + key;
             const int64_t ti = n - my_tb;
-            const bool vis = brow_ok && (n < k1) && (n < my_kvl || (ti >= 0 && ti < 64 && ((my_tm >> ti) & 1)));
+            const bool vis = brow_ok && (n < k1) &&
+                             ((n < my_kvl && (!MOD || n >= my_kvb)) || (ti >= 0 && ti < 64 && ((my_tm >> ti) & 1)));
             const int r = brow_ok ? br : 0;
             double x0 = S.sc[0][r][key], x1 = S.sc[1][r][key], x2 = S.sc[2][r][key], x3 = S.sc[3][r][key];
             bool slow = ((S.fm[0][key] | S.fm[1][key] | S.fm[2][key] | S.fm[3][key]) >> r) & 1;
@@ -406,8 +443,9 @@ __global__ void __launch_bounds__(EA_THREADS, 2) ea_split(Params P) {
             int why = 0;  // 1 score not certified, 2 weight not certified
             if (vis && !rflag) {
                 uint32_t tb = 0;
-                int ls = (ssum == 0.0 && sig == 0.0 && del == 0.0) ? 1
-                         : (isfinite(ssum) ? logit_cert(P.alpha, ssum, sig, del, &tb) : 3);
+                const bool zero = ssum == 0.0 && sig == 0.0 && del == 0.0;
+                int ls = zero ? 1 : (isfinite(ssum) ? logit_cert(P.alpha, ssum, sig, del, &tb) : 3);
+                if constexpr (MOD) ls = mod_logit(ls, zero, P.cap, my_slope, (int)n - my_pos, S.T1, 0, &tb);
                 if (ls == 2 || ls == 3) {
                     why = 1;  // overflow (tier 2 reports the domain error) or undecided
                 } else if (ls == 0) {
@@ -438,15 +476,15 @@ __global__ void __launch_bounds__(EA_THREADS, 2) ea_split(Params P) {
             double sc = 1.0;
             if (Rrun != INT_MIN && Rnew != Rrun) {
                 int dsh = Rrun - Rnew;
-                if (dsh < -900) rflag = 1;
+                if (!MOD && dsh < -900) rflag = 1;
                 sc = ldexp(1.0, max(dsh, -1000));
                 zacc *= sc;
             }
             double om = 0.0;
             if (vis) {
                 int de = E - Rnew;
-                if (de < -1000) rflag = 1;
-                om = ldexp((double)M, max(de, -1000));
+                if (!MOD && de < -1000) rflag = 1;
+                om = MOD && de < -1000 ? 0.0 : ldexp((double)M, max(de, -1000));
             }
             if (rflag) om = 0.0;
             zacc += om;
@@ -532,7 +570,7 @@ __global__ void __launch_bounds__(EA_THREADS, 2) ea_split(Params P) {
         for (int ww = 0; ww < 4; ++ww) {
             int rw = S.wR[ww][r];
             if (rw == INT_MIN || rw == -0x7FFFFFFF) continue;
-            if (rw - R < -900) fl = true;
+            if (!MOD && rw - R < -900) fl = true;
             s += ldexp(red[((ww * EA_MAXRB) + r) * 128 + c], max(rw - R, -1000));
             zs += ldexp(S.wZ[ww][r], max(rw - R, -1000));
             nv += S.wn[ww][r];
@@ -585,14 +623,15 @@ __global__ void __launch_bounds__(EA_THREADS, 2) ea_split(Params P) {
 // row and wants waves in flight instead (PRE 2: 72 registers against 157; 65,536 rows of 64-dim heads,
 // two pieces each, 92 -> 53 us).
 // MR: whether the multi-row kernel wrote the partials; a branch on it cost the decode step 1 us.
-template <int PRE, bool MR>
+// MOD: with score modifications.
+template <int PRE, bool MR, bool MOD = false>
 __global__ void __launch_bounds__(64) ea_combine(Params P) {
     // one row per 64-thread block: the merge is a chain of dependent loads, so it wants as many
     // rows in flight as the machine holds. stats[0] counts the step's rows once; the per-row
     // counters only move for flagged rows (rare), so they never serialise on one address.
     const int64_t row = blockIdx.x;
     if (row == 0 && threadIdx.x == 0 && P.stats) atomicAdd((unsigned long long*)&P.stats[0], (unsigned long long)P.rows);
-    const int ev = combine_row<PRE, MR>(P, row, threadIdx.x);
+    const int ev = combine_row<PRE, MR, MOD>(P, row, threadIdx.x);
     if (threadIdx.x == 0 && P.stats && (ev & 2)) {
         atomicAdd((unsigned long long*)&P.stats[1], 1ull);
         if (ev & 4) atomicAdd((unsigned long long*)&P.stats[7], 1ull);
@@ -688,7 +727,8 @@ struct T2Part {
 // larger base by an arithmetic right shift: floor(a 2^-s) <= a 2^-s < floor(a 2^-s) + lost, so
 // the row's sums stay of the form [acc, acc + lost count] in units of the common base, the form
 // the final rounding takes. With C = 1 the block finishes the row itself. done: EA_T2_BLOCKS
-// counters, 0 at the start, of the rows' finished chunks.
+// counters, 0 at the start, of the rows' finished chunks. MOD: with score modifications.
+template <bool MOD>
 __device__ __forceinline__ void t2_rows(const Params& P, T2Smem& S, int& s_last, int32_t* list, int cnt, int slot_id,
                                         int32_t* done, int32_t* next) {
     const int tid = threadIdx.x;
@@ -717,13 +757,12 @@ __device__ __forceinline__ void t2_rows(const Params& P, T2Smem& S, int& s_last,
         const int t = (int)((row / Hq) % T), hq = (int)(row % Hq);
         const int hk = hq / P.grp;
         const int64_t tok = b * T + t;
-        // the row's visible keys (vis_prefix, vis_tree_bits: the set tier 1 attends); this block
+        // the row's visible keys (row_keys: the set tier 1 attends); this block
         // takes keys [jc0, jc1) of them
-        const int64_t slen = P.seq_len[b];
-        const int64_t L = vis_prefix(P.kv_len[tok], slen);
-        const uint64_t mask =
-            P.tree_mask ? vis_tree_bits(P.tree_mask[tok], (int64_t)P.tree_base[b], L, slen) : 0ull;
-        const int64_t nkeys = L + __popcll(mask);
+        const int kvl = P.kv_len[tok];
+        const RowKeys keys = row_keys(MOD ? vis_begin(P, tok, kvl) : 0, kvl, P.seq_len[b], P.tree_mask ? P.tree_mask[tok] : 0ull,
+                                      P.tree_mask ? P.tree_base[b] : 0);
+        const int64_t nkeys = keys.count();
         const int64_t csz = (nkeys + C - 1) / C;
         const int64_t jc0 = min(nkeys, (int64_t)chunk * csz), jc1 = min(nkeys, jc0 + csz);
         const int64_t nkc = jc1 - jc0;
@@ -755,13 +794,7 @@ __device__ __forceinline__ void t2_rows(const Params& P, T2Smem& S, int& s_last,
                 tq0 = tn;
             }
         };
-        const int64_t tb = P.tree_mask ? P.tree_base[b] : 0;
-        auto key_n = [&](int64_t j) -> int64_t {
-            if (j < L) return j;
-            uint64_t m = mask;
-            for (int64_t cc = j - L; cc > 0; --cc) m &= m - 1;
-            return tb + (__ffsll((long long)m) - 1);
-        };
+        auto key_n = [&](int64_t j) -> int64_t { return keys.key(j); };
         int64_t emax = INT64_MIN;
         // one key per thread, its K row in registers (16-byte loads when rows are aligned)
         const bool k16 = (((uintptr_t)P.k | (uintptr_t)(P.g.k_page_stride * 2) | (uintptr_t)(P.g.k_slot_stride * 2) |
@@ -804,6 +837,7 @@ __device__ __forceinline__ void t2_rows(const Params& P, T2Smem& S, int& s_last,
             }
             int32_t M = 1 << 23;
             int64_t E = -23;
+            uint32_t tlo = 0;  // t's bits; 0 where every product, or alpha, is
             if (lmax != INT_MIN && P.am != 0) {
                 const int base = lmax + 1 - 120;
                 i128 acc = 0;
@@ -824,7 +858,7 @@ __device__ __forceinline__ void t2_rows(const Params& P, T2Smem& S, int& s_last,
                         err += (uint64_t)lost;
                     }
                 }
-                uint32_t tlo = 0, thi = 0;
+                uint32_t thi = 0;
                 const int slo = rn32_prod(P.am, acc, P.ae + base, &tlo);
                 const int shi = err ? rn32_prod(P.am, acc + (i128)err, P.ae + base, &thi) : slo;
                 if (!err) thi = tlo;
@@ -836,6 +870,14 @@ __device__ __forceinline__ void t2_rows(const Params& P, T2Smem& S, int& s_last,
                     myflag = 1;
                     break;
                 }
+            }
+            if constexpr (MOD) {
+                if (mod_logit(0, false, P.cap, mod_slope(P, hq), (int)key_n(jc0 + jr) - mod_pos(P, tok, kvl), S.T1, 0, &tlo)) {
+                    atomicMax(&S.flag, 2);
+                    break;
+                }
+            }
+            if (MOD || (lmax != INT_MIN && P.am != 0)) {
                 int32_t Mi;
                 int32_t Ei;
                 if (weight_f64(tlo, S.T1, S.T2, &Mi, &Ei) == 0) {
@@ -1133,6 +1175,7 @@ __device__ __forceinline__ int t2_left(const Params& P, int nact, int* slot_id) 
 // 4096-key bf16 row after a prefill step 116 -> 35 us; an empty list 4.6 us (3.8 at least)
 // in the trace, as without the pass; 512 blocks cost a C2 step 1.8 us, so bf16 steps, which list few rows,
 // launch 32. The pass itself is 1.5 us slower (64.8 -> 66.3) for the 128-bit path's registers beside it.
+template <bool MOD>
 __global__ void __launch_bounds__(EA_T2_THREADS) ea_tier2(Params P) {
     __shared__ union {
         T2Smem t2;
@@ -1144,24 +1187,25 @@ __global__ void __launch_bounds__(EA_T2_THREADS) ea_tier2(Params P) {
     // every item of a split row is in flight at once (a block each, a partial each, a count per row)
     // and no chunk is shorter than a pass of 128 keys
     const int C = cnt <= EA_T2_ROWS ? min(min(EA_DD_PARTS, (int)gridDim.x) / cnt, (P.t2_keys + EA_DD_KEYS - 1) / EA_DD_KEYS) : 1;
-    dd_rows(P, S.dd, cnt, max(C, 1), (DDPart*)P.ddpart);
+    dd_rows<MOD>(P, S.dd, cnt, max(C, 1), (DDPart*)P.ddpart);
     const int nact = (int)min((int64_t)cnt * max(C, 1), (int64_t)gridDim.x);
     if ((int)blockIdx.x >= nact) return;
     agent_done();  // the list of what is left, and the partials, whose memory the 128-bit path reuses
     __syncthreads();
     if (threadIdx.x == 0) s_left = t2_left(P, nact, &s_slot);
     __syncthreads();
-    if (s_left > 0) t2_rows(P, S.t2, s_last, P.t2left, s_left, s_slot, &P.wl_cnt[EA_T2_CHUNKS], &P.wl_cnt[EA_T2_NEXT]);
+    if (s_left > 0) t2_rows<MOD>(P, S.t2, s_last, P.t2left, s_left, s_slot, &P.wl_cnt[EA_T2_CHUNKS], &P.wl_cnt[EA_T2_NEXT]);
 }
 
 // force_tier2: every row straight to the 128-bit path, over EA_T2_BLOCKS blocks. A kernel of its own:
 // beside the double-double pass the body spills 324 SGPRs instead of 176 (32 rows of 32K keys, that pass
 // included, 6.4 ms against 6.0).
+template <bool MOD>
 __global__ void __launch_bounds__(EA_T2_THREADS) ea_tier2_wide(Params P) {
     __shared__ T2Smem S;
     __shared__ int s_last;
     const int cnt = *P.wl_cnt;
-    if (cnt > 0) t2_rows(P, S, s_last, P.wl, cnt, (int)blockIdx.x, &P.wl_cnt[EA_T2_CHUNKS], nullptr);
+    if (cnt > 0) t2_rows<MOD>(P, S, s_last, P.wl, cnt, (int)blockIdx.x, &P.wl_cnt[EA_T2_CHUNKS], nullptr);
 }
 
 // Lists every row for tier 2 (ea_options.force_tier2); runs after tier 1, so nothing else appends.
@@ -1172,7 +1216,7 @@ __global__ void __launch_bounds__(256) ea_list_all(Params P) {
 }
 
 // The host exact tier's input for one row: its q row, then the K rows and the V rows of its
-// visible keys (the prefix, then the tree keys in bit order: vis_prefix, vis_tree_bits), packed in
+// visible keys (the prefix, then the tree keys in bit order: row_keys), packed in
 // dst as [q d][K nkeys x d][V nkeys x dv], one element per thread.
 __global__ void __launch_bounds__(256) ea_gather_row(Params P, int64_t row, int64_t nkeys, uint16_t* dst) {
     const int d = P.g.head_dim, dv = P.g.head_dim_v, T = P.g.num_tokens, Hq = P.g.num_q_heads;
@@ -1180,10 +1224,9 @@ __global__ void __launch_bounds__(256) ea_gather_row(Params P, int64_t row, int6
     const int t = (int)((row / Hq) % T), hq = (int)(row % Hq);
     const int hk = hq / P.grp;
     const int64_t tok = b * T + t;
-    const int64_t slen = P.seq_len[b];
-    const int64_t L = vis_prefix(P.kv_len[tok], slen);
-    const int64_t tb = P.tree_mask ? P.tree_base[b] : 0;
-    const uint64_t mask = P.tree_mask ? vis_tree_bits(P.tree_mask[tok], tb, L, slen) : 0ull;
+    const int kvl = P.kv_len[tok];
+    const RowKeys keys = row_keys(vis_begin(P, tok, kvl), kvl, P.seq_len[b], P.tree_mask ? P.tree_mask[tok] : 0ull,
+                                  P.tree_mask ? P.tree_base[b] : 0);
     const int64_t total = d + nkeys * (int64_t)(d + dv);
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
         if (i < d) {
@@ -1196,13 +1239,7 @@ __global__ void __launch_bounds__(256) ea_gather_row(Params P, int64_t row, int6
         const int wdt = isv ? dv : d;
         const int64_t j = r / wdt;
         const int e = (int)(r % wdt);
-        int64_t n = j;
-        if (j >= L) {
-            uint64_t m = mask;
-            for (int64_t c = j - L; c > 0; --c) m &= m - 1;
-            n = tb + (__ffsll((long long)m) - 1);
-        }
-        dst[i] = (isv ? P.v : P.k)[kv_off(P, b, n, hk, isv) + e];
+        dst[i] = (isv ? P.v : P.k)[kv_off(P, b, keys.key(j), hk, isv) + e];
     }
 }
 
@@ -1298,6 +1335,18 @@ __global__ void ea_kat_rn32_prod(int64_t n, const int32_t* am, const int64_t* x_
     bits[i] = bb;
 }
 
+__global__ void ea_kat_mod_logit(int64_t n, const uint32_t* t, const int32_t* dist, const float* slope, ModCap cap,
+                                 uint32_t* bits, int32_t* status) {
+    __shared__ double T1[256];
+    T1[threadIdx.x] = u64_as_f64(EA_T1_BITS[threadIdx.x]) * 8388608.0;
+    __syncthreads();
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    uint32_t b = t[i];
+    status[i] = mod_logit(0, false, cap, slope[i], dist[i], T1, 23, &b);
+    bits[i] = b;
+}
+
 __global__ void ea_kat_round_ratio(int64_t n, const uint64_t* ah, const uint64_t* al, const uint64_t* bh,
                                    const uint64_t* bl, const int32_t* E, const int32_t* neg, int32_t fp32, uint32_t* bits,
                                    int32_t* ov) {
@@ -1368,15 +1417,20 @@ size_t align_up(size_t x) { return (x + 255) & ~(size_t)255; }
 // heads, 1 row per segment, the line holds too (of 254 decode geometries on either side of it none is slower than
 // on ea_decode by 3%). Any other
 // head size: always (ea_split takes what the pointers or pages do not allow).
-int mrow_rows(const ea_geometry* g, const ea_options* o, int r_seg) {
+// With score modifications (mods), which ea_decode does not know: every step the prefill kernel leaves.
+int mrow_rows(const ea_geometry* g, const ea_options* o, int r_seg, bool mods) {
     if (o->timers || o->kernel == EA_KERNEL_GENERAL) return 0;
-    if (g->head_dim == 128 && g->head_dim_v == 128) {
+    if (g->head_dim == 128 && g->head_dim_v == 128 && !mods) {
         if (o->kernel == EA_KERNEL_DECODE) return 0;
         int nt = 0, nr = 0;
         const int64_t tiles = (int64_t)g->num_seqs * g->num_kv_heads * (((int64_t)g->max_seq_len + 63) / 64);
         if ((r_seg <= 2 && tiles >= 4096) ||
             ea_prefill_eligible(*g, g->num_q_heads / g->num_kv_heads, o->kernel, &nt, &nr))
             return 0;
+    }
+    if (mods) {
+        int nt = 0, nr = 0;
+        if (ea_prefill_eligible(*g, g->num_q_heads / g->num_kv_heads, o->kernel, &nt, &nr)) return 0;
     }
     return r_seg <= 4 ? 4 : (r_seg <= 8 ? 8 : 16);
 }
@@ -1490,7 +1544,26 @@ size_t lay_out(Plan* pl, const ea_geometry* g, const ea_options* o, bool mrow) {
     return pl->total = std::max(off, align_up(pl->off_dd + EA_DD_PARTS * sizeof(DDPart)));
 }
 
-int make_plan(const ea_geometry* g, const ea_options* o, Plan* pl) {
+// The keys a unit of a step with score modifications is taken to span at most, whole tiles at both ends:
+// the caller's bound, or what the window gives for consecutive tokens, or every key. A hint: it chooses
+// the splits, and the kernels read past it where a unit's range does.
+int mod_span(const ea_geometry* g, const ea_score_mods* m, int maxlen) {
+    int64_t span = maxlen;
+    if (m->window > 0) span = std::min<int64_t>(span, (int64_t)m->window + g->num_tokens - 1);
+    if (m->max_span > 0) span = std::min<int64_t>(span, m->max_span);
+    return (int)std::min<int64_t>(maxlen, span + 63);
+}
+
+// 0, or the code that ea_hip_attention_mods returns for these modifications
+int check_mods(const ea_options* o, const ea_score_mods* m) {
+    if (!m) return 0;
+    if (m->window < 0 || m->max_span < 0 || (o && o->timers)) return -2;
+    const uint32_t c = m->softcap_bits;  // +0: none; else positive, normal and finite
+    const int f = (int)(c >> 23);        // the sign is its top bit
+    return c == 0 || (f > 0 && f < 255) ? 0 : -2;
+}
+
+int make_plan(const ea_geometry* g, const ea_options* o, Plan* pl, const ea_score_mods* m = nullptr) {
     if (!g || !o) return -1;
     if (g->num_seqs < 0 || g->num_tokens <= 0 || g->num_q_heads <= 0 || g->num_kv_heads <= 0) return -1;
     if (g->num_q_heads % g->num_kv_heads) return -1;
@@ -1501,6 +1574,8 @@ int make_plan(const ea_geometry* g, const ea_options* o, Plan* pl) {
     if (o->splits < 0) return -2;
     if (o->kernel < EA_KERNEL_AUTO || o->kernel > EA_KERNEL_GENERAL) return -2;
     if (o->prefill_waves != 0 && o->prefill_waves != 4 && o->prefill_waves != 8) return -2;
+    const int mrc = check_mods(o, m);
+    if (mrc) return mrc;
     pl->grp = g->num_q_heads / g->num_kv_heads;
     pl->r_seg = g->num_tokens * pl->grp;
     pl->nseg = g->num_seqs * g->num_kv_heads;
@@ -1513,6 +1588,7 @@ int make_plan(const ea_geometry* g, const ea_options* o, Plan* pl) {
     pl->dlog = dl;
     const int maxlen = g->max_seq_len > 0 ? g->max_seq_len : 1;
     const int64_t max_tiles = ((int64_t)maxlen + 63) / 64;
+    const int span = m ? mod_span(g, m, maxlen) : maxlen;
     pl->dq_max_tiles = (int)max_tiles;
     pl->t2_keys = maxlen;  // a row's visible keys are distinct and below max_seq_len
     pl->prefill = ea_prefill_eligible(*g, pl->grp, o->kernel, &pl->pf_ntiles, &pl->pf_nrb) ? 1 : 0;
@@ -1523,14 +1599,15 @@ int make_plan(const ea_geometry* g, const ea_options* o, Plan* pl) {
         // fills a CU's LDS): double the splits while the grid is under 256 blocks and every split
         // keeps at least 16 tiles; a caller's split count is taken as given
         int ns = 1;
+        const int nt = (span + 63) / 64;
         if (o->splits > 0) {
             ns = o->splits;
         } else {
-            while ((int64_t)pl->nseg * pl->pf_nrb * ns < 256 && pl->pf_ntiles / (2 * ns) >= 16) ns *= 2;
+            while ((int64_t)pl->nseg * pl->pf_nrb * ns < 256 && nt / (2 * ns) >= 16) ns *= 2;
         }
-        pl->pf_tps = (pl->pf_ntiles + ns - 1) / ns;
+        pl->pf_tps = (nt + ns - 1) / ns;
         if (pl->pf_tps < 1) pl->pf_tps = 1;
-        pl->pf_nsplit = (pl->pf_ntiles + pl->pf_tps - 1) / pl->pf_tps;
+        pl->pf_nsplit = (nt + pl->pf_tps - 1) / pl->pf_tps;
         if (pl->pf_nsplit < 1) pl->pf_nsplit = 1;
     }
     // an equal-share plan over nrb row blocks per segment stays within its 30-bit arithmetic
@@ -1545,18 +1622,18 @@ int make_plan(const ea_geometry* g, const ea_options* o, Plan* pl) {
     // 1, 2 or 4
     Tier1& gen = pl->gen;
     const bool d128 = g->head_dim == 128 && g->head_dim_v == 128;
-    const bool dec_rows = d128 && o->kernel != EA_KERNEL_GENERAL && !o->timers;
+    const bool dec_rows = d128 && o->kernel != EA_KERNEL_GENERAL && !o->timers && !m;
     gen.rb = dec_rows ? std::min(pl->r_seg, 2) : (pl->r_seg >= 3 ? 4 : pl->r_seg);
     gen.nrb = (pl->r_seg + gen.rb - 1) / gen.rb;
-    choose_splits(pl->nseg * (int64_t)gen.nrb, maxlen, o->splits, &gen.nsplit, &gen.split_len);
-    gen.dq = d128 && dq_fits(gen.nrb);
+    choose_splits(pl->nseg * (int64_t)gen.nrb, span, o->splits, &gen.nsplit, &gen.split_len);
+    gen.dq = d128 && !m && dq_fits(gen.nrb);
     Tier1& mr = pl->mr;
-    mr.rb = mrow_rows(g, o, pl->r_seg);
+    mr.rb = mrow_rows(g, o, pl->r_seg, m != nullptr);
     pl->mrow = mr.rb > 0;
     const size_t without = lay_out(pl, g, o, false);
     if (!pl->mrow) return 0;
     mr.nrb = (pl->r_seg + mr.rb - 1) / mr.rb;
-    choose_splits_mrow(*pl, mr, maxlen, g->head_dim_v, o->splits);
+    choose_splits_mrow(*pl, mr, span, g->head_dim_v, o->splits);
     // Row blocks of half the rows while their grid is at most a block per CU: a wave's chain of steps
     // is what such a step waits for, and it is shorter with fewer rows. 16 rows, 16 -> 4 a block: 8
     // segments of 100 keys 32.7 -> 25.8 us a step (29.5 on ea_decode), of 1000 33.2 -> 27.0; one of 16K 58.7
@@ -1566,7 +1643,7 @@ int make_plan(const ea_geometry* g, const ea_options* o, Plan* pl) {
         Tier1 half = mr;
         half.rb = mr.rb / 2;
         half.nrb = (pl->r_seg + half.rb - 1) / half.rb;
-        choose_splits_mrow(*pl, half, maxlen, g->head_dim_v, o->splits);
+        choose_splits_mrow(*pl, half, span, g->head_dim_v, o->splits);
         if ((int64_t)pl->nseg * half.nrb * half.nsplit > 256) break;
         mr = half;
     }
@@ -1578,7 +1655,7 @@ int make_plan(const ea_geometry* g, const ea_options* o, Plan* pl) {
     const Tier1 first = mr;
     while (lay_out(pl, g, o, true) > cap && without <= cap) {
         if (o->splits == 0 && mr.nsplit > 1) {
-            split_tiles(maxlen, mr.nsplit / 2, &mr.nsplit, &mr.split_len);
+            split_tiles(span, mr.nsplit / 2, &mr.nsplit, &mr.split_len);
         } else if (mr.dq) {
             mr = first;
             mr.dq = 0;
@@ -1595,7 +1672,17 @@ int herr(hipError_t e) { return e == hipSuccess ? 0 : -100 - (int)e; }
 int reported_nsplit(const Plan& pl) { return pl.prefill ? pl.pf_nsplit : (pl.mrow ? pl.mr.nsplit : pl.gen.nsplit); }
 
 // The caller's arrays and strides, as far as the choice of kernel and the split kernels read them
-void set_inputs(Params& P, const Plan& pl, const ea_geometry* g, const ea_buffers* bf) {
+void set_inputs(Params& P, const Plan& pl, const ea_geometry* g, const ea_buffers* bf, const ea_score_mods* m = nullptr) {
+    if (m) {
+        float c;
+        memcpy(&c, &m->softcap_bits, 4);
+        P.kv_begin = m->kv_begin;
+        P.q_pos = m->q_pos;
+        P.slopes = m->slopes;
+        P.cap = mod_cap_of(c);
+        P.window = m->window;
+        P.mods = c > 0.0f ? 2 : 1;
+    }
     P.g = *g;
     P.q = bf->q; P.k = bf->k; P.v = bf->v;
     P.seq_len = bf->seq_len; P.kv_len = bf->kv_len; P.bt = bf->block_table; P.bt_off = bf->block_table_offset;
@@ -1613,7 +1700,7 @@ bool choose_split_kernel(Params& P, const Plan& pl) {
     P.nrb = t.nrb;
     P.nsplit = t.nsplit;
     P.split_len = t.split_len;
-    return !P.mrow && t.dq && pl.nseg > 0 && ea_decode_eligible(P);
+    return !P.mrow && !P.mods && t.dq && pl.nseg > 0 && ea_decode_eligible(P);
 }
 
 // The caller's merge order where the combine may follow it: it has exactly the reported number of
@@ -1664,6 +1751,18 @@ int list_all(const Params& P, const ea_options* o, unsigned blocks, hipStream_t 
     return herr(hipGetLastError());
 }
 
+// tier 2 on the listed rows
+void tier2(const Params& P, const ea_options* o, hipStream_t st) {
+    const dim3 grid(o->force_tier2 ? EA_T2_BLOCKS : EA_DD_BLOCKS(P.out_fp32)), blk(EA_T2_THREADS);
+    if (o->force_tier2) {
+        if (P.mods) hipLaunchKernelGGL(ea_tier2_wide<true>, grid, blk, 0, st, P);
+        else hipLaunchKernelGGL(ea_tier2_wide<false>, grid, blk, 0, st, P);
+    } else {
+        if (P.mods) hipLaunchKernelGGL(ea_tier2<true>, grid, blk, 0, st, P);
+        else hipLaunchKernelGGL(ea_tier2<false>, grid, blk, 0, st, P);
+    }
+}
+
 }  // namespace
 
 extern "C" {
@@ -1708,10 +1807,10 @@ int ea_hip_reads_kv_digits(const ea_geometry* g, const ea_options* o, int32_t* r
     return 0;
 }
 
-int ea_hip_attention(const ea_geometry* g, const ea_buffers* bf, const ea_options* o, void* workspace,
-                     size_t workspace_bytes, ea_stream_t stream) {
+static int attention_impl(const ea_geometry* g, const ea_buffers* bf, const ea_options* o, const ea_score_mods* m,
+                          void* workspace, size_t workspace_bytes, ea_stream_t stream) {
     Plan pl;
-    int rc = make_plan(g, o, &pl);
+    int rc = make_plan(g, o, &pl, m);
     if (rc) return rc;
     uint32_t ab = o->alpha_bits;
     // an empty batch reads and writes nothing: no buffer or workspace is needed for it
@@ -1722,7 +1821,7 @@ int ea_hip_attention(const ea_geometry* g, const ea_buffers* bf, const ea_option
     if (((ab >> 23) & 0xFF) == 0xFF) return -3;
     Params P;
     memset(&P, 0, sizeof(P));
-    set_inputs(P, pl, g, bf);
+    set_inputs(P, pl, g, bf, m);
     P.out = bf->out; P.flags = bf->flags; P.stats = o->stats;
     P.stats_x = o->stats && o->stats_entries == EA_STATS ? o->stats + 16 : nullptr;
     P.timers = o->timers;
@@ -1822,10 +1921,7 @@ int ea_hip_attention(const ea_geometry* g, const ea_buffers* bf, const ea_option
         if ((rc = mark(3))) return rc;
         if (o->tier2) {
             if ((rc = list_all(P, o, rb4 * 4 / 256 + 1, st))) return rc;
-            if (o->force_tier2)
-                hipLaunchKernelGGL(ea_tier2_wide, dim3(EA_T2_BLOCKS), dim3(EA_T2_THREADS), 0, st, P);
-            else
-                hipLaunchKernelGGL(ea_tier2, dim3(EA_DD_BLOCKS(P.out_fp32)), dim3(EA_T2_THREADS), 0, st, P);
+            tier2(P, o, st);
             rc = herr(hipGetLastError());
             if (rc) return rc;
         }
@@ -1835,7 +1931,8 @@ int ea_hip_attention(const ea_geometry* g, const ea_buffers* bf, const ea_option
     if (P.mrow) {
         // the multi-row kernel converts its own q rows; the plan is one block's work
         if (P.dq_stream) {
-            hipLaunchKernelGGL(ea_plan, dim3(1), dim3(1024), 0, st, P);
+            if (P.mods) hipLaunchKernelGGL(ea_plan<true>, dim3(1), dim3(1024), 0, st, P);
+            else hipLaunchKernelGGL(ea_plan<false>, dim3(1), dim3(1024), 0, st, P);
             if ((rc = herr(hipGetLastError()))) return rc;
         }
     } else if (!(use_decode && !P.dq_stream)) {
@@ -1847,9 +1944,11 @@ int ea_hip_attention(const ea_geometry* g, const ea_buffers* bf, const ea_option
         static std::once_flag once;
         static hipError_t attr_err = hipSuccess;
         std::call_once(once, [] {
-            const void* fns[6] = {(const void*)ea_split<1, false>, (const void*)ea_split<2, false>,
-                                  (const void*)ea_split<4, false>, (const void*)ea_split<1, true>,
-                                  (const void*)ea_split<2, true>, (const void*)ea_split<4, true>};
+            const void* fns[9] = {(const void*)ea_split<1, false>,       (const void*)ea_split<2, false>,
+                                  (const void*)ea_split<4, false>,       (const void*)ea_split<1, true>,
+                                  (const void*)ea_split<2, true>,        (const void*)ea_split<4, true>,
+                                  (const void*)ea_split<1, false, true>, (const void*)ea_split<2, false, true>,
+                                  (const void*)ea_split<4, false, true>};
             for (const void* f : fns) {
                 hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize,
                                                    (int)sizeof(SplitSmem));
@@ -1866,6 +1965,10 @@ int ea_hip_attention(const ea_geometry* g, const ea_buffers* bf, const ea_option
             if ((rc = ea_launch_mrow(P, st))) return rc;
         } else if (use_decode) {
             if ((rc = ea_launch_decode(P, st))) return rc;
+        } else if (P.mods) {
+            if (P.rb == 1) hipLaunchKernelGGL((ea_split<1, false, true>), grid, blk, lds, st, P);
+            else if (P.rb == 2) hipLaunchKernelGGL((ea_split<2, false, true>), grid, blk, lds, st, P);
+            else hipLaunchKernelGGL((ea_split<4, false, true>), grid, blk, lds, st, P);
         } else if (o->timers) {
             if (P.rb == 1) hipLaunchKernelGGL((ea_split<1, true>), grid, blk, lds, st, P);
             else if (P.rb == 2) hipLaunchKernelGGL((ea_split<2, true>), grid, blk, lds, st, P);
@@ -1881,22 +1984,42 @@ int ea_hip_attention(const ea_geometry* g, const ea_buffers* bf, const ea_option
         return rc;
     }
     if ((rc = mark(2))) return rc;
-    auto* const combine = pl.rows >= 8192 ? (P.mrow ? ea_combine<2, true> : ea_combine<2, false>)
-                                          : (P.mrow ? ea_combine<8, true> : ea_combine<8, false>);
+    auto* combine = pl.rows >= 8192 ? (P.mrow ? ea_combine<2, true> : ea_combine<2, false>)
+                                    : (P.mrow ? ea_combine<8, true> : ea_combine<8, false>);
+    if (P.mods)
+        combine = pl.rows >= 8192 ? (P.mrow ? ea_combine<2, true, true> : ea_combine<2, false, true>)
+                                  : (P.mrow ? ea_combine<8, true, true> : ea_combine<8, false, true>);
     hipLaunchKernelGGL(combine, dim3((unsigned)pl.rows), dim3(64), 0, st, P);
     rc = herr(hipGetLastError());
     if (rc) return rc;
     if ((rc = mark(3))) return rc;
     if (o->tier2) {
         if ((rc = list_all(P, o, rb4 * 4 / 256 + 1, st))) return rc;
-        if (o->force_tier2)
-            hipLaunchKernelGGL(ea_tier2_wide, dim3(EA_T2_BLOCKS), dim3(EA_T2_THREADS), 0, st, P);
-        else
-            hipLaunchKernelGGL(ea_tier2, dim3(EA_DD_BLOCKS(P.out_fp32)), dim3(EA_T2_THREADS), 0, st, P);
+        tier2(P, o, st);
         rc = herr(hipGetLastError());
         if (rc) return rc;
     }
     return mark(4);
+}
+
+int ea_hip_attention(const ea_geometry* g, const ea_buffers* bf, const ea_options* o, void* workspace,
+                     size_t workspace_bytes, ea_stream_t stream) {
+    return attention_impl(g, bf, o, nullptr, workspace, workspace_bytes, stream);
+}
+
+int ea_hip_attention_mods(const ea_geometry* g, const ea_buffers* bf, const ea_options* o, const ea_score_mods* m,
+                          void* workspace, size_t workspace_bytes, ea_stream_t stream) {
+    return attention_impl(g, bf, o, m, workspace, workspace_bytes, stream);
+}
+
+int ea_hip_mods_workspace_size(const ea_geometry* g, const ea_options* o, const ea_score_mods* m, size_t* bytes,
+                               int32_t* nsplit) {
+    Plan pl;
+    int rc = make_plan(g, o, &pl, m);
+    if (rc) return rc;
+    if (bytes) *bytes = pl.total;
+    if (nsplit) *nsplit = reported_nsplit(pl);
+    return 0;
 }
 
 int ea_hip_attention_noalloc(const ea_geometry* g, const ea_buffers* bf, const ea_options* o, ea_stream_t stream) {
@@ -1910,9 +2033,10 @@ int ea_hip_attention_noalloc(const ea_geometry* g, const ea_buffers* bf, const e
     return ea_hip_attention(g, bf, o, ws, (size_t)EA_NOALLOC_SCRATCH_BYTES, stream);
 }
 
-static int exact_rows_impl(const ea_geometry* g, const ea_buffers* bf, const ea_options* o, ea_stream_t stream) {
+static int exact_rows_impl(const ea_geometry* g, const ea_buffers* bf, const ea_options* o, const ea_score_mods* m,
+                           ea_stream_t stream) {
     Plan pl;
-    int rc = make_plan(g, o, &pl);
+    int rc = make_plan(g, o, &pl, m);
     if (rc) return rc;
     if (pl.rows == 0) return ((o->alpha_bits >> 23) & 0xFF) == 0xFF ? -3 : 0;  // an empty batch
     if (!bf || !bf->q || !bf->k || !bf->v || !bf->seq_len || !bf->kv_len || !bf->out || !bf->flags) return -1;
@@ -1929,29 +2053,44 @@ static int exact_rows_impl(const ea_geometry* g, const ea_buffers* bf, const ea_
     if (todo.empty()) return 0;
     Params P;
     memset(&P, 0, sizeof(P));
-    P.g = *g;
-    P.q = bf->q; P.k = bf->k; P.v = bf->v;
-    P.seq_len = bf->seq_len; P.kv_len = bf->kv_len; P.bt = bf->block_table; P.bt_off = bf->block_table_offset;
-    P.tree_mask = bf->tree_mask; P.tree_base = bf->tree_base;
-    P.grp = pl.grp; P.pshift = pl.pshift; P.rows = pl.rows;
+    set_inputs(P, pl, g, bf, m);
     const int d = g->head_dim, dv = g->head_dim_v, T = g->num_tokens, Hq = g->num_q_heads;
-    // visible keys per listed row: the prefix plus the tree keys (vis_prefix, vis_tree_bits)
-    std::vector<int64_t> nk(todo.size());
+    // each listed row's visible keys, and with modifications its slope and position
+    struct Listed {
+        RowKeys keys;
+        float slope;
+        int32_t pos;
+    };
+    std::vector<Listed> rows(todo.size());
     int64_t maxk = 0;
     for (size_t i = 0; i < todo.size(); ++i) {
         const int64_t row = todo[i], b = row / ((int64_t)T * Hq), t = (row / Hq) % T, tok = b * T + t;
-        int32_t L = 0, sl = 0, tb = 0;
-        uint64_t m = 0;
-        if ((e = hipMemcpy(&L, bf->kv_len + tok, 4, hipMemcpyDeviceToHost)) != hipSuccess) return herr(e);
-        if ((e = hipMemcpy(&sl, bf->seq_len + b, 4, hipMemcpyDeviceToHost)) != hipSuccess) return herr(e);
+        int32_t L = 0, sl = 0, tb = 0, begin = 0;
+        uint64_t tm = 0;
+        auto get = [&](void* dst, const void* src, size_t n) {
+            if (e == hipSuccess) e = hipMemcpy(dst, src, n, hipMemcpyDeviceToHost);
+        };
+        get(&L, bf->kv_len + tok, 4);
+        get(&sl, bf->seq_len + b, 4);
         if (bf->tree_mask) {
-            if ((e = hipMemcpy(&m, bf->tree_mask + tok, 8, hipMemcpyDeviceToHost)) != hipSuccess) return herr(e);
-            if ((e = hipMemcpy(&tb, bf->tree_base + b, 4, hipMemcpyDeviceToHost)) != hipSuccess) return herr(e);
+            get(&tm, bf->tree_mask + tok, 8);
+            get(&tb, bf->tree_base + b, 4);
         }
-        const int64_t Lc = vis_prefix(L, sl);
-        nk[i] = Lc + __builtin_popcountll(bf->tree_mask ? vis_tree_bits(m, tb, Lc, sl) : 0ull);
-        maxk = nk[i] > maxk ? nk[i] : maxk;
+        Listed& r = rows[i];
+        r.slope = 0.0f;
+        r.pos = L - 1;
+        if (m) {
+            if (m->kv_begin) get(&begin, m->kv_begin + tok, 4);
+            if (m->q_pos) get(&r.pos, m->q_pos + tok, 4);
+            if (m->slopes) get(&r.slope, m->slopes + row % Hq, 4);
+            begin = std::max(begin, 0);
+            if (m->window > 0 && L > m->window) begin = std::max(begin, L - m->window);
+        }
+        if (e != hipSuccess) return herr(e);
+        r.keys = row_keys(begin, L, sl, tm, tb);
+        maxk = std::max(maxk, r.keys.count());
     }
+    std::vector<int32_t> dist(m ? (size_t)maxk : 0);
     const size_t cap = (size_t)(d + maxk * (int64_t)(d + dv));
     std::vector<uint16_t> host(cap);  // before the device buffer: a throw here leaks nothing
     uint16_t* stage = nullptr;
@@ -1959,7 +2098,7 @@ static int exact_rows_impl(const ea_geometry* g, const ea_buffers* bf, const ea_
     const size_t osz = o->out_fp32 ? 4 : 2;
     int64_t fixed = 0, refused = 0, dom = 0;
     for (size_t i = 0; i < todo.size() && e == hipSuccess; ++i) {
-        const int64_t row = todo[i], n = nk[i];
+        const int64_t row = todo[i], n = rows[i].keys.count();
         const int64_t b = row / ((int64_t)T * Hq), t = (row / Hq) % T, hq = row % Hq;
         const size_t cnt = (size_t)(d + n * (int64_t)(d + dv));
         const unsigned blocks = (unsigned)std::min<size_t>((cnt + 255) / 256, 4096);
@@ -1968,8 +2107,11 @@ static int exact_rows_impl(const ea_geometry* g, const ea_buffers* bf, const ea_
         if ((e = hipMemcpyAsync(host.data(), stage, cnt * 2, hipMemcpyDeviceToHost, st)) != hipSuccess) break;
         if ((e = hipStreamSynchronize(st)) != hipSuccess) break;
         uint8_t res[EA_MAXDV * 4];  // dv bf16 (uint16) or fp32 (uint32) patterns, as exact_row writes them
+        eax::RowMod mod{(float)P.cap.c, rows[i].slope, dist.data()};
+        if (m)
+            for (int64_t j = 0; j < n; ++j) dist[(size_t)j] = (int32_t)(rows[i].keys.key(j) - rows[i].pos);
         const int x = eax::exact_row(host.data(), d, host.data() + d, host.data() + d + n * d, n, dv, o->alpha_bits,
-                                     o->out_fp32, res, nullptr);
+                                     o->out_fp32, res, nullptr, m ? &mod : nullptr);
         if (x == eax::EAX_NOMEM) {
             (void)hipFree(stage);
             return EA_ERR_HOST_MEMORY;
@@ -1997,12 +2139,17 @@ static int exact_rows_impl(const ea_geometry* g, const ea_buffers* bf, const ea_
     return 0;
 }
 
-int ea_hip_exact_rows(const ea_geometry* g, const ea_buffers* bf, const ea_options* o, ea_stream_t stream) {
+int ea_hip_exact_rows_mods(const ea_geometry* g, const ea_buffers* bf, const ea_options* o, const ea_score_mods* m,
+                           ea_stream_t stream) {
     try {
-        return exact_rows_impl(g, bf, o, stream);
+        return exact_rows_impl(g, bf, o, m, stream);
     } catch (...) {  // host vectors: only an exhausted heap throws
         return EA_ERR_HOST_MEMORY;
     }
+}
+
+int ea_hip_exact_rows(const ea_geometry* g, const ea_buffers* bf, const ea_options* o, ea_stream_t stream) {
+    return ea_hip_exact_rows_mods(g, bf, o, nullptr, stream);
 }
 
 int ea_exact_row(const uint16_t* q, int d, const uint16_t* k, const uint16_t* v, int64_t n, int dv,
@@ -2084,6 +2231,15 @@ int ea_hip_kat_weight(int64_t n, const uint32_t* t_bits, int32_t* M, int64_t* E,
     if (n <= 0) return n < 0 ? -1 : 0;
     hipLaunchKernelGGL(ea_kat_weight, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, (hipStream_t)stream, n, t_bits,
                        M, E, status, M2, E2, status2);
+    return herr(hipGetLastError());
+}
+
+int ea_hip_kat_mod_logit(int64_t n, const uint32_t* t_bits, const int32_t* dist, const float* slope, float cap,
+                         uint32_t* bits, int32_t* status, ea_stream_t stream) {
+    if (n < 0 || (n > 0 && (!t_bits || !dist || !slope || !bits || !status))) return -1;
+    if (n == 0) return 0;
+    hipLaunchKernelGGL(ea_kat_mod_logit, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, (hipStream_t)stream, n, t_bits, dist,
+                       slope, mod_cap_of(cap), bits, status);
     return herr(hipGetLastError());
 }
 

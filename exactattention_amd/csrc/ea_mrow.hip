@@ -91,6 +91,12 @@ struct MRowSmem {
     // waiting, so a step's 16 RS more always fit
     int2 list[4][MR_LIST + (mr_two_steps<RS>() ? 32 : 16) * RS];
 };
+// and with score modifications the rows' first prefix keys, positions and slopes
+template <int RS, int DK, int CPL>
+struct MRowModSmem : MRowSmem<RS, DK, CPL> {
+    int kvb[RS], pos[RS];
+    float slope[RS];
+};
 
 // the larger of x and the values 16, 32 and 48 lanes away (lanes l, l ^ 16, l ^ 32, l ^ 48)
 __device__ __forceinline__ int max_x(int v) {
@@ -113,14 +119,17 @@ __device__ __forceinline__ double rot4(double w) {
 
 }  // namespace
 
-template <int RS, int DK, int CPL>
+// MOD: with score modifications (ea_mod.h), 1 without a cap and 2 with one. A unit's key range is then
+// counted from its rows' first visible key, down to a whole tile, and on uniform splits the last split
+// takes every key past the others.
+template <int RS, int DK, int CPL, int MOD = 0>
 __global__ void __launch_bounds__(MR_THREADS, (mr_waves<RS, DK>())) ea_mrow(Params P) {
     constexpr int NS = RS == 16 ? 1 : RS / 4;  // row sets of the 4x4x4 form
     constexpr int NP = RS / 4;                 // pairs per lane and step
     constexpr int NR = RS == 16 ? 1 : NS;      // rows a lane holds in the score layout
     constexpr int NACC = RS / 4;               // row quads of the output layout
     constexpr bool DB = mr_two_steps<RS>();
-    typedef MRowSmem<RS, DK, CPL> Smem;
+    typedef std::conditional_t<MOD != 0, MRowModSmem<RS, DK, CPL>, MRowSmem<RS, DK, CPL>> Smem;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     Smem& S = *reinterpret_cast<Smem*>(smem_raw);
     const int tid = (int)(threadIdx.x + MR_BX * threadIdx.y);
@@ -138,7 +147,7 @@ __global__ void __launch_bounds__(MR_THREADS, (mr_waves<RS, DK>())) ea_mrow(Para
 
     // One piece: keys [kA, kB) of unit `item` (segment, row block), clipped to the unit's visible
     // end, as partial slot `split`.
-    auto piece = [&](const int item, const int split, const int kA, const int kB) __attribute__((always_inline)) {
+    auto piece = [&](const int item, const int split, int kA, int kB) __attribute__((always_inline)) {
         const int lane = tid & 63;
         const int x = lane >> 4, c = lane & 15, blk = c >> 2;
         const int seg = item / P.nrb, rbk = item % P.nrb;
@@ -172,6 +181,7 @@ __global__ void __launch_bounds__(MR_THREADS, (mr_waves<RS, DK>())) ea_mrow(Para
         const int slen = P.seq_len[b];
         const int tb = P.tree_mask ? P.tree_base[b] : 0;
         int kend = 0, kvmin = INT_MAX;
+        int kbeg = INT_MAX, kbmax = 0;  // MOD: the rows' first visible key, their last prefix start
         {
             const int r = lane & (RS - 1);
             const int tok = b * P.g.num_tokens + (row0 + min(r, nrow - 1)) / P.grp;
@@ -179,6 +189,22 @@ __global__ void __launch_bounds__(MR_THREADS, (mr_waves<RS, DK>())) ea_mrow(Para
             const uint64_t tmk = P.tree_mask ? P.tree_mask[tok] : 0ull;
             kend = tmk ? max(kvl, tb + 64 - (int)__clzll(tmk)) : kvl;
             kvmin = kvl;
+            if constexpr (MOD) {
+                const int kvb = vis_begin(P, tok, kvl);
+                kbmax = kvb;
+                if (kvb < min(kvl, slen)) kbeg = kvb;
+                else kend = 0;
+                if (tmk) {
+                    kbeg = min(kbeg, tb + (int)__builtin_ctzll(tmk));
+                    kend = max(kend, tb + 64 - (int)__clzll(tmk));
+                }
+                if (w == 0 && lane < RS) {
+                    S.kvb[r] = kvb;
+                    S.pos[r] = mod_pos(P, tok, kvl);
+                    const int lr = row0 + min(r, nrow - 1);
+                    S.slope[r] = mod_slope(P, hk * P.grp + lr % P.grp);
+                }
+            }
             if (w == 0 && lane < RS) {
                 S.kvl[r] = r < nrow ? kvl : INT_MIN;
                 S.tmk[r] = r < nrow ? tmk : 0ull;
@@ -186,6 +212,13 @@ __global__ void __launch_bounds__(MR_THREADS, (mr_waves<RS, DK>())) ea_mrow(Para
         }
         kend = min(wave_max_dpp(kend), slen);
         kvmin = min(-wave_max_dpp(-kvmin), slen);
+        if constexpr (MOD) {
+            kbeg = -wave_max_dpp(-kbeg);
+            kbmax = wave_max_dpp(kbmax);
+            const int k0 = kend > 0 ? tile_floor(kbeg) : 0;
+            kA += k0;
+            kB += k0;
+        }
         const int k1 = min(kB, kend);
         const int k0w = kA + 16 * w;  // this wave's keys: k0w + 64 it .. + 15
         const int nst = k1 > k0w ? (k1 - k0w + 63) >> 6 : 0;
@@ -202,12 +235,17 @@ __global__ void __launch_bounds__(MR_THREADS, (mr_waves<RS, DK>())) ea_mrow(Para
         const int ss4 = 4 * (int)vss2;
         const int voff = x * (int)vss2 + 2 * CPL * c;
         // 16 consecutive keys starting at a multiple of 16 lie in one page (page size >= 16)
-        auto page_of = [&](int n) __attribute__((always_inline)) { return P.bt ? btb[min(n, k1 - 1) >> pshift] : b; };
+        // (MOD: a tile's keys before kbeg are not loaded, nor their pages looked up)
+        auto page_of = [&](int n) __attribute__((always_inline)) {
+            int m = min(n, k1 - 1);
+            if constexpr (MOD) m = max(m, kbeg);
+            return P.bt ? btb[m >> pshift] : b;
+        };
         auto issue_k = [&](int n0, int pg, u32x4 (&kr)[DK]) __attribute__((always_inline)) {
             const int64_t sl = P.bt ? (n0 & pmask) : n0;
             const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
                 (void*)(kh + (int64_t)pg * kps2 + sl * kss2), (short)0, 0x7FFFFFFF, 0x00020000);
-            const int kd = n0 + c < k1 ? d : 0;
+            const int kd = n0 + c < k1 && (!MOD || n0 + c >= kbeg) ? d : 0;
 #pragma unroll
             for (int j = 0; j < DK; ++j)
                 kr[j] = __builtin_amdgcn_raw_buffer_load_b128(rk, 8 * (4 * j + x) < kd ? koff + 64 * j : EA_OOB, 0, 0);
@@ -219,7 +257,8 @@ __global__ void __launch_bounds__(MR_THREADS, (mr_waves<RS, DK>())) ea_mrow(Para
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int kq = RS == 16 ? i : (blk + i) & 3;  // the lane's key is 4 kq + x
-                const int o = (n0 + 4 * kq + x < k1 && CPL * c < dv) ? voff + kq * ss4 : EA_OOB;
+                const bool in = n0 + 4 * kq + x < k1 && (!MOD || n0 + 4 * kq + x >= kbeg);
+                const int o = (in && CPL * c < dv) ? voff + kq * ss4 : EA_OOB;
                 if constexpr (CPL == 8) {
                     vr[i] = __builtin_amdgcn_raw_buffer_load_b128(rv, o, 0, 0);
                 } else {
@@ -252,6 +291,15 @@ __global__ void __launch_bounds__(MR_THREADS, (mr_waves<RS, DK>())) ea_mrow(Para
             q1a[s] = fabs(alpha) * (66.0 * 0x1p-53 * (1.0 + 0x1p-20)) * S.q1[RS == 16 ? c : (c & 3) + 4 * s];
             R[s] = MR_NONE;
             z[s] = 0.0;
+        }
+        int mpos[NR];
+        float mslope[NR];
+        if constexpr (MOD) {
+#pragma unroll
+            for (int s = 0; s < NR; ++s) {
+                mpos[s] = S.pos[RS == 16 ? c : (c & 3) + 4 * s];
+                mslope[s] = S.slope[RS == 16 ? c : (c & 3) + 4 * s];
+            }
         }
 
         auto step = [&](int n0, int pgn, u32x4 (&kr)[DK], u32x4 (&vr)[4], u32x4 (&kn)[DK], u32x4 (&vn)[4]) __attribute__((always_inline)) {
@@ -328,19 +376,32 @@ __global__ void __launch_bounds__(MR_THREADS, (mr_waves<RS, DK>())) ea_mrow(Para
                 adel[p] = q1a[RS == 16 ? 0 : p] * (double)__int_as_float(__shfl(kmx, key, 64));
                 vism |= ((RS == 16 ? c : (c & 3) + 4 * p) < nrow) ? (1u << p) : 0u;
             }
-            if (n0 + 16 > min(kvmin, k1)) {
+            if (n0 + 16 > min(kvmin, k1) || (MOD && n0 < kbmax)) {
                 vism = 0;
 #pragma unroll
                 for (int p = 0; p < NP; ++p) {
                     const int r = RS == 16 ? c : (c & 3) + 4 * p, n = n0 + (RS == 16 ? 4 * p : 4 * blk) + x, ti = n - tb;
                     const bool in = ((unsigned)ti < 64u) & (((S.tmk[r] >> (ti & 63)) & 1ull) != 0);
-                    vism |= ((n < k1) & ((n < S.kvl[r]) | in)) ? (1u << p) : 0u;
+                    bool pre = n < S.kvl[r];
+                    if constexpr (MOD) pre = pre & (n >= S.kvb[r]);
+                    vism |= ((n < k1) & (pre | in)) ? (1u << p) : 0u;
                 }
             }
             // ---- certified weights
             int M[NP], E[NP];
             bool ok[NP];
-            pf::cert_pairs<NP>(s_, adel, alpha, S.T1, S.T2, M, E, ok);
+            if constexpr (MOD) {
+                float m[NP];
+                int dist[NP];
+#pragma unroll
+                for (int p = 0; p < NP; ++p) {
+                    m[p] = mslope[RS == 16 ? 0 : p];
+                    dist[p] = n0 + (RS == 16 ? 4 * p : 4 * blk) + x - mpos[RS == 16 ? 0 : p];
+                }
+                pf::cert_pairs<NP, MOD>(s_, adel, alpha, S.T1, S.T2, M, E, ok, P.cap, m, dist);
+            } else {
+                pf::cert_pairs<NP>(s_, adel, alpha, S.T1, S.T2, M, E, ok);
+            }
             uint32_t good = 0;
 #pragma unroll
             for (int p = 0; p < NP; ++p) good |= ok[p] ? (1u << p) : 0u;
@@ -382,7 +443,7 @@ __global__ void __launch_bounds__(MR_THREADS, (mr_waves<RS, DK>())) ea_mrow(Para
                     if (m > R[s] + MR_HEAD) {
                         if (R[s] != MR_NONE) {
                             const int dsh = R[s] - m;
-                            if (dsh < -900) rfl |= 1 << s;
+                            if (!MOD && dsh < -900) rfl |= 1 << s;
                             f = ldexp(1.0, max(dsh, -1000));
                             z[s] *= f;
                         }
@@ -408,7 +469,7 @@ __global__ void __launch_bounds__(MR_THREADS, (mr_waves<RS, DK>())) ea_mrow(Para
                 const int s = RS == 16 ? 0 : p;
                 const int de = E[p] - R[s];
                 const bool g = (good >> p) & 1, far = de < -1000;
-                if (g && far) rfl |= 1 << s;
+                if (!MOD && g && far) rfl |= 1 << s;
                 om[p] = (g && !far) ? ldexp((double)M[p], de) : 0.0;
                 z[s] += om[p];
             }
@@ -484,8 +545,10 @@ __global__ void __launch_bounds__(MR_THREADS, (mr_waves<RS, DK>())) ea_mrow(Para
                     int ls = 3;
                     fin = isfinite(ss);
                     if (fin) {
-                        ls = (ss == 0.0 && es == 0.0 && ea == 0.0) ? 1 : logit_cert(alpha, ss, es, ea * 0x1p-44, &tbits);
+                        const bool zero = ss == 0.0 && es == 0.0 && ea == 0.0;
+                        ls = zero ? 1 : logit_cert(alpha, ss, es, ea * 0x1p-44, &tbits);
                         if (ls == 1) tbits = 0;
+                        if constexpr (MOD) ls = mod_logit(ls, zero, P.cap, S.slope[en.x], en.y - S.pos[en.x], S.T1, 23, &tbits);
                     }
                     if (ls == 2 || ls == 3) {
                         why = 1;  // undecided, or an overflow (tier 2 reports the domain error)
@@ -521,7 +584,7 @@ __global__ void __launch_bounds__(MR_THREADS, (mr_waves<RS, DK>())) ea_mrow(Para
                             Rr = __builtin_amdgcn_readlane(R[s], RS == 16 ? r : (r & 3));
                             if (Er + 23 > Rr + MR_HEAD) {
                                 if (Rr != MR_NONE) {
-                                    if (Rr - (Er + 23) < -900) flag_row(r);
+                                    if (!MOD && Rr - (Er + 23) < -900) flag_row(r);
                                     f = ldexp(1.0, max(Rr - (Er + 23), -1000));
                                 }
                                 Rr = Er + 23;
@@ -532,7 +595,7 @@ __global__ void __launch_bounds__(MR_THREADS, (mr_waves<RS, DK>())) ea_mrow(Para
                             }
                         }
                     const int de = Er - Rr;
-                    if (de < -1000) flag_row(r);
+                    if (!MOD && de < -1000) flag_row(r);
                     const double om = de < -1000 ? 0.0 : ldexp((double)Mr, de);
 #pragma unroll
                     for (int s = 0; s < NR; ++s)
@@ -625,7 +688,7 @@ __global__ void __launch_bounds__(MR_THREADS, (mr_waves<RS, DK>())) ea_mrow(Para
             for (int ww = 0; ww < 4; ++ww) Rm = max(Rm, S.wR[ww][r]);
             const int Rw = S.wR[w][r];
             const double f = Rw == MR_NONE ? 1.0 : ldexp(1.0, max(Rw - Rm, -1000));
-            if (Rw != MR_NONE && Rw - Rm < -900) far4 |= 1 << i;
+            if (!MOD && Rw != MR_NONE && Rw - Rm < -900) far4 |= 1 << i;
 #pragma unroll
             for (int e = 0; e < CPL; ++e) {
                 if constexpr (RS == 16) acc[i][e] = acc16[e][i] * f;
@@ -722,6 +785,7 @@ __global__ void __launch_bounds__(MR_THREADS, (mr_waves<RS, DK>())) ea_mrow(Para
         }
         start = (int)blockIdx.y * (P.split_len >> 6);
         end = start + (P.split_len >> 6);
+        if (MOD && blockIdx.y == gridDim.y - 1) end = 1 << 24;  // keys are below 2^30
     }
     for (bool first = true;; first = false) {
         int t0 = start, t1 = end, slot = (int)blockIdx.y;
@@ -747,34 +811,43 @@ __global__ void __launch_bounds__(MR_THREADS, (mr_waves<RS, DK>())) ea_mrow(Para
 
 namespace {
 
-template <int RS>
+// mod: Params::mods of ea_mod.h's variants, 0 the plain kernel
+template <int RS, int MOD>
 const void* mrow_fn(bool small) {
-    return small ? (const void*)ea_mrow<RS, 2, 4> : (const void*)ea_mrow<RS, 4, 8>;
+    return small ? (const void*)ea_mrow<RS, 2, 4, MOD> : (const void*)ea_mrow<RS, 4, 8, MOD>;
 }
 template <int RS>
-size_t mrow_lds(bool small) {
+const void* mrow_fn(bool small, int mod) {
+    return mod == 2 ? mrow_fn<RS, 2>(small) : (mod ? mrow_fn<RS, 1>(small) : mrow_fn<RS, 0>(small));
+}
+template <int RS>
+size_t mrow_lds(bool small, int mod) {
+    if (mod) return small ? sizeof(MRowModSmem<RS, 2, 4>) : sizeof(MRowModSmem<RS, 4, 8>);
     return small ? sizeof(MRowSmem<RS, 2, 4>) : sizeof(MRowSmem<RS, 4, 8>);
 }
 // head sizes up to 64 take half the K chunks and 4 channels per lane
 bool mrow_small(const Params& P) { return P.g.head_dim <= 64 && P.g.head_dim_v <= 64; }
 const void* mrow_fn_for(const Params& P) {
     const bool s = mrow_small(P);
-    return P.rb == 4 ? mrow_fn<4>(s) : (P.rb == 8 ? mrow_fn<8>(s) : mrow_fn<16>(s));
+    return P.rb == 4 ? mrow_fn<4>(s, P.mods) : (P.rb == 8 ? mrow_fn<8>(s, P.mods) : mrow_fn<16>(s, P.mods));
 }
 size_t mrow_lds_for(const Params& P) {
     const bool s = mrow_small(P);
-    return P.rb == 4 ? mrow_lds<4>(s) : (P.rb == 8 ? mrow_lds<8>(s) : mrow_lds<16>(s));
+    return P.rb == 4 ? mrow_lds<4>(s, P.mods) : (P.rb == 8 ? mrow_lds<8>(s, P.mods) : mrow_lds<16>(s, P.mods));
 }
 hipError_t mrow_attrs() {
     static std::once_flag once;
     static hipError_t err = hipSuccess;
     std::call_once(once, [] {
-        const void* fns[6] = {mrow_fn<4>(false), mrow_fn<8>(false), mrow_fn<16>(false),
-                              mrow_fn<4>(true),  mrow_fn<8>(true),  mrow_fn<16>(true)};
-        for (const void* f : fns) {
-            hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(MRowSmem<16, 4, 8>));
-            if (e != hipSuccess) err = e;
-        }
+        for (int mod = 0; mod < 3; ++mod)
+            for (int small = 0; small < 2; ++small) {
+                const void* fns[3] = {mrow_fn<4>(small, mod), mrow_fn<8>(small, mod), mrow_fn<16>(small, mod)};
+                for (const void* f : fns) {
+                    hipError_t e =
+                        hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(MRowModSmem<16, 4, 8>));
+                    if (e != hipSuccess) err = e;
+                }
+            }
     });
     return err;
 }
@@ -798,12 +871,12 @@ int ea::ea_mrow_eligible(const Params& P) {
 int ea::ea_mrow_slots(const Params& P, int* slots) {
     // blocks resident on the current device at once, cached per device and kernel
     static std::mutex mu;
-    static int cache[64][6] = {};
+    static int cache[64][18] = {};
     hipError_t e = mrow_attrs();
     if (e != hipSuccess) return -100 - (int)e;
     int dev = 0;
     if ((e = hipGetDevice(&dev)) != hipSuccess) return -100 - (int)e;
-    const int ki = (P.rb == 4 ? 0 : (P.rb == 8 ? 1 : 2)) + (mrow_small(P) ? 3 : 0);
+    const int ki = (P.rb == 4 ? 0 : (P.rb == 8 ? 1 : 2)) + (mrow_small(P) ? 3 : 0) + 6 * P.mods;
     std::lock_guard<std::mutex> lk(mu);
     if (dev < 0 || dev >= 64) return -1;
     if (!cache[dev][ki]) {

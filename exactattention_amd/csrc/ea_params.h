@@ -5,6 +5,7 @@
 
 #include "../../include/exactattn_hip.h"
 #include "ea_device.h"
+#include "ea_mod.h"
 
 namespace ea {
 
@@ -117,7 +118,25 @@ struct Params {
     // 1: the multi-row split kernel wrote the partials (it keeps no qinfo: the combine looks at the
     // q row itself where a row has no visible key)
     int32_t mrow;
+    // Score modifications (ea_mod.h; the kernels' MOD variants alone read these)
+    const int32_t* kv_begin;  // per token: its first prefix key; NULL: 0
+    const int32_t* q_pos;     // per token: the position distances count from; NULL: kv_len - 1
+    const float* slopes;      // per query head; NULL: no bias
+    ModCap cap;
+    int32_t window;           // > 0: a token's prefix starts at kv_len - window at the earliest
+    int32_t mods;             // the MOD variant: 0 none, 1 key ranges and bias, 2 those and the cap
 };
+
+// Token `tok`'s first prefix key, its prefix ending at kvl
+__device__ __forceinline__ int vis_begin(const Params& P, int64_t tok, int kvl) {
+    int b = P.kv_begin ? max(P.kv_begin[tok], 0) : 0;
+    if (P.window > 0 && kvl > P.window) b = max(b, kvl - P.window);
+    return b;
+}
+__device__ __forceinline__ int mod_pos(const Params& P, int64_t tok, int kvl) { return P.q_pos ? P.q_pos[tok] : kvl - 1; }
+__device__ __forceinline__ float mod_slope(const Params& P, int hq) { return P.slopes ? P.slopes[hq] : 0.0f; }
+// the first key of a unit's tiles: its rows' first visible key, down to a whole tile
+__host__ __device__ inline int tile_floor(int key) { return key & ~63; }
 
 __device__ __forceinline__ int64_t row_index(const Params& P, int64_t b, int t, int hq) {
     return (b * P.g.num_tokens + t) * P.g.num_q_heads + hq;
@@ -143,6 +162,31 @@ __device__ inline int unit_kend(const Params& P, int seg, int rbk) {
         kend = max(kend, e);
     }
     return min(kend, (int)P.seq_len[b]);
+}
+
+// The keys [first, end) a unit's rows see with score modifications: rows that see nothing widen neither
+// end. (0, 0) when no row sees a key.
+__device__ inline int2 unit_keys(const Params& P, int seg, int rbk) {
+    const int b = seg / P.g.num_kv_heads;
+    const int row0 = rbk * P.rb;
+    const int nrow = min(P.rb, P.r_seg - row0);
+    const int tb = P.tree_mask ? P.tree_base[b] : 0, slen = P.seq_len[b];
+    int kbeg = INT_MAX, kend = 0;
+    const int t1 = (row0 + nrow - 1) / P.grp;
+    for (int t = row0 / P.grp; t <= t1; ++t) {
+        const int64_t tok = (int64_t)b * P.g.num_tokens + t;
+        const int e = min(P.kv_len[tok], slen), g = vis_begin(P, tok, P.kv_len[tok]);
+        if (g < e) {
+            kbeg = min(kbeg, g);
+            kend = max(kend, e);
+        }
+        const uint64_t m = P.tree_mask ? P.tree_mask[tok] : 0ull;
+        if (m && tb + (int)__builtin_ctzll(m) < slen) {
+            kbeg = min(kbeg, tb + (int)__builtin_ctzll(m));
+            kend = max(kend, min(tb + 64 - (int)__clzll(m), slen));
+        }
+    }
+    return kend > 0 ? make_int2(kbeg, kend) : make_int2(0, 0);
 }
 
 // global element offset of key n of sequence b, kv head hk (K when isv = 0, V when 1)
@@ -184,6 +228,36 @@ __host__ __device__ inline uint64_t vis_tree_bits(uint64_t mask, int64_t tb, int
 }
 __host__ __device__ inline int64_t vis_prefix(int64_t kv_len, int64_t slen) {
     return kv_len < 0 ? 0 : (kv_len < slen ? kv_len : slen);
+}
+
+// A row's visible keys, listed: the prefix [begin, begin + npre), then the tree keys outside it in
+// bit order. With MOD false begin is 0.
+struct RowKeys {
+    int64_t begin, npre, tb;
+    uint64_t mask;
+    __host__ __device__ int64_t count() const { return npre + __builtin_popcountll(mask); }
+    __host__ __device__ int64_t key(int64_t j) const {
+        if (j < npre) return begin + j;
+        uint64_t m = mask;
+        for (int64_t c = j - npre; c > 0; --c) m &= m - 1;
+        return tb + __builtin_ctzll(m);
+    }
+};
+// kv_begin: the row's first prefix key (vis_begin). Tree keys below it count as tree keys.
+__host__ __device__ inline RowKeys row_keys(int64_t kv_begin, int64_t kv_len, int64_t slen, uint64_t mask, int64_t tb) {
+    RowKeys r;
+    const int64_t L = vis_prefix(kv_len, slen);
+    r.begin = kv_begin < L ? kv_begin : L;
+    r.npre = L - r.begin;
+    r.tb = tb;
+    r.mask = vis_tree_bits(mask, tb, r.begin == 0 || r.npre > 0 ? L : 0, slen);
+    if (r.begin > 0 && r.npre > 0) {
+        // the bits below the prefix too: those of keys under begin
+        const int64_t hi = r.begin - tb;
+        const uint64_t below = hi <= 0 ? 0ull : (hi >= 64 ? ~0ull : ((1ull << hi) - 1));
+        r.mask |= vis_tree_bits(mask, tb, 0, slen) & below;
+    }
+    return r;
 }
 
 // end of the visible key range of a query token

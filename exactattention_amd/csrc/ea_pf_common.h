@@ -68,13 +68,17 @@ __device__ __forceinline__ bool table_weight(uint32_t tbits, const double* T1s, 
 // rows qr, kr (elements rounded at slicing) by TwoSum with a certified logit, the rows read 32
 // elements at a time in 16-byte loads when both are 16-byte aligned (one memory round trip per
 // batch instead of one per element); mode 2: q holds NaN/inf (no score). Returns (status, M, E):
-// 0 w = M 2^E, 2 domain error, 3 score not certified, 4 weight not certified.
+// 0 w = M 2^E, 2 domain error, 3 score not certified, 4 weight not certified. MOD: with the cap C and
+// the bias of slope m at distance dist.
 // ------------------------------------------------------------------------------------------------
+template <int MOD = 0>
 __device__ __forceinline__ int3 pf_cold_pair(int mode, const uint8_t* qrow, int qsw, const uint8_t* krow, int ksw,
                                           const uint16_t* qr, const uint16_t* kr, int32_t am, int eS, double alpha,
-                                          const double* T1s, const double* T2) {
+                                          const double* T1s, const double* T2, const ModCap& C = ModCap{}, float m = 0.0f,
+                                          int dist = 0) {
     uint32_t tbits = 0;
     int ls = 3;
+    bool zero = false;
     if (mode == 0) {
         int D[4][4];
 #pragma unroll
@@ -147,9 +151,11 @@ __device__ __forceinline__ int3 pf_cold_pair(int mode, const uint8_t* qrow, int 
                 ea += fabs(e0);
             }
         }
-        ls = (ss == 0.0 && es == 0.0 && ea == 0.0) ? 1 : logit_cert(alpha, ss, es, ea * 0x1p-44, &tbits);
+        zero = ss == 0.0 && es == 0.0 && ea == 0.0;
+        ls = zero ? 1 : logit_cert(alpha, ss, es, ea * 0x1p-44, &tbits);
         if (ls == 1) tbits = 0;
     }
+    if constexpr (MOD) ls = mod_logit(ls, zero, C, m, dist, T1s, 23, &tbits);
     int32_t M = 0, E = 0;
     if (ls == 2) return make_int3(2, M, E);
     if (ls == 3) return make_int3(3, M, E);
@@ -172,10 +178,14 @@ __device__ __forceinline__ int3 pf_cold_pair(int mode, const uint8_t* qrow, int 
 // unscaled evaluation times a power of two: the same bits); rounded to an integer by adding and
 // subtracting 1.5 * 2^52; certified when |Y - RN(Y)| <= 1/2 - 2^-26 (the fp64 evaluation error
 // is below 2^-26.9). ok[i] false: the exact path decides.
+// MOD 1: with the bias -m[i] |dist[i]|; 2: with the cap before it. A decided t0 is modified as it is; where
+// only |alpha s| <= 2^-25 is known, both ends of that interval are, and must give one weight (the cap only
+// shrinks it).
 // ------------------------------------------------------------------------------------------------
-template <int NP>
+template <int NP, int MOD = 0>
 __device__ __forceinline__ void cert_pairs(const double (&xs)[NP], const double (&adel)[NP], double a, const double* T1s,
-                                           const double* T2, int (&M)[NP], int (&E)[NP], bool (&ok)[NP]) {
+                                           const double* T2, int (&M)[NP], int (&E)[NP], bool (&ok)[NP],
+                                           const ModCap& C = ModCap{}, const float* m = nullptr, const int* dist = nullptr) {
     const double c1 = u64_as_f64(EA_C_BITS[0]) * 0x1p-16, c2 = u64_as_f64(EA_C_BITS[1]) * 0x1p-32,
                  c3 = u64_as_f64(EA_C_BITS[2]) * 0x1p-48;
     double d0[NP];
@@ -195,6 +205,16 @@ __device__ __forceinline__ void cert_pairs(const double (&xs)[NP], const double 
         const bool inner = (__fma_rn(fabs(r), 1.0 + 0x1p-50, adel[i]) < h) & (at >= 0x1p-24) & (at < 0x1p30);
         ok[i] = tiny | inner;
         d0[i] = tiny ? 0.0 : t0;
+        if constexpr (MOD) {
+            float tc = tf;
+            if constexpr (MOD == 2) tc = mod_cap(tf, C, T1s, 23);
+            const float dl = (float)((fabs(p) + fabs(pe) + adel[i]) * (1.0 + 0x1p-20));
+            const float hi = mod_bias(tiny ? dl : tc, m[i], dist[i]), lo = mod_bias(tiny ? -dl : tc, m[i], dist[i]);
+            const float ah = fabsf(hi);
+            const bool one = (ah <= 0x1p-25f) & (fabsf(lo) <= 0x1p-25f);
+            ok[i] = ok[i] & (one | ((hi == lo) & (ah >= 0x1p-24f) & (ah < 0x1p30f)));
+            d0[i] = one | !ok[i] ? 0.0 : (double)hi;
+        }
     }
     double fl[NP], rr[NP];
     int idx[NP];

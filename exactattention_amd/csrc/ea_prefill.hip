@@ -269,6 +269,9 @@ __global__ void __launch_bounds__(256) ea_pf_qslice(Params P) {
 // straight to memory in 16-byte chunks; the V planes (keys interleaved per channel) are
 // assembled in LDS and copied out in 16-byte chunks.
 // ------------------------------------------------------------------------------------------------
+// MOD (score modifications): tiles wholly before the first key that a token of the sequence sees are left
+// out; no row of ea_pf_main reads them.
+template <bool MOD>
 __global__ void __launch_bounds__(256) ea_pf_kvslice(Params P) {
     __shared__ __align__(16) uint8_t s_v[32768];
     __shared__ int s_lc[128];
@@ -289,6 +292,17 @@ __global__ void __launch_bounds__(256) ea_pf_kvslice(Params P) {
     const int Hkv = P.g.num_kv_heads;
     const int64_t b = seg / Hkv;
     const int hk = seg % Hkv;
+    if constexpr (MOD) {
+        int first = INT_MAX;
+        for (int t = tid; t < P.g.num_tokens; t += 256) {
+            const int64_t tok = b * P.g.num_tokens + t;
+            const int g = vis_begin(P, tok, P.kv_len[tok]);
+            if (g < min(P.kv_len[tok], P.seq_len[b])) first = min(first, g);
+            const uint64_t m = P.tree_mask ? P.tree_mask[tok] : 0ull;
+            if (m) first = min(first, P.tree_base[b] + (int)__builtin_ctzll(m));
+        }
+        if (!__syncthreads_or(first < 64 * (tile + 1))) return;
+    }
     uint8_t* T = P.pfkv + ((int64_t)seg * P.pf_ntiles + tile) * EA_PF_TILE_BYTES;
     PfTileMeta* TM = (PfTileMeta*)(T + EA_PF_META_OFF);
     if (tid < 128) s_lc[tid] = 0;
@@ -410,7 +424,9 @@ struct PfPar {
     static constexpr int value = N;
 };
 
-template <int NWB, bool TIMERS>
+// MOD: with score modifications (ea_mod.h), 1 without a cap and 2 with one; a block's tiles then start at
+// its rows' first visible key, and its last key split takes every tile past the others.
+template <int NWB, bool TIMERS, int MOD = 0>
 __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
     // phase clocks (TIMERS build): shader cycles summed over waves into P.timers[i]. Per tile:
     // [14] DMA wait before B1, [0] B1, [1] EV reads and score MFMAs, [2] base move and weight
@@ -453,6 +469,7 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
     uint32_t* const sWD = (uint32_t*)(smem + PF_OFF_WD);  // weight digits [wave][plane 5][2][lane]
     PfX* const sX = (PfX*)(smem + PF_OFF_X);              // pair exchange [wave][lane]
     int& s_kend = *(int*)(smem + PF_OFF_KEND);
+    int& s_kbeg = *(int*)(smem + PF_OFF_KEND + 4);
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rg = w / SPLIT, hh = w % SPLIT;
@@ -473,7 +490,10 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
     // per-lane scratch: fp64 sums of completed epochs, then the final quotients
     double* const scr = P.pfscr + (((int64_t)blockIdx.x * NWB + w) * 64 + lane) * (8 * NCT);
 
-    if (tid == 0) s_kend = 0;
+    if (tid == 0) {
+        s_kend = 0;
+        if constexpr (MOD) s_kbeg = INT_MAX;
+    }
     if (tid < 256) {
         sT1[tid] = u64_as_f64(EA_T1_BITS[tid]) * 8388608.0;  // 2^23: exact
         sT2[tid] = u64_as_f64(EA_T2_BITS[tid]);
@@ -497,10 +517,29 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
     ve = min(ve, slen);
     // keys below kvmin are visible to every row of the wave (and of its partner)
     const int kvmin = wave_min_i(rvalid ? min(kvl, slen) : INT_MAX);
+    int kvb = 0, mpos = 0, kbmax = 0;
+    float mslope = 0.0f;
+    int vb = INT_MAX;
+    if constexpr (MOD) {
+        kvb = vis_begin(P, tok, kvl);
+        mpos = mod_pos(P, tok, kvl);
+        mslope = mod_slope(P, hk * P.grp + lrc % P.grp);
+        kbmax = wave_max_i(rvalid ? kvb : 0);
+        if (kvb < min(kvl, slen)) vb = kvb;
+        else ve = 0;
+        if (tmk) {
+            vb = min(vb, tbase + (int)__builtin_ctzll(tmk));
+            ve = max(ve, min(tbase + 64 - (int)__clzll(tmk), slen));
+        }
+    }
     __syncthreads();  // s_kend initialised
     {
         const int kw = wave_max_i(ve);
         if (lane == 0) atomicMax(&s_kend, kw);
+        if constexpr (MOD) {
+            const int kb0 = wave_min_i(vb);
+            if (lane == 0) atomicMin(&s_kbeg, kb0);
+        }
     }
     // q digits of the block's rows into LDS: [row][plane 4][128 bytes] with rows PF_QROW = 528
     // bytes apart, so the 16 rows a 16-lane group reads start 4 banks apart (132 dwords = 4 mod 64)
@@ -537,7 +576,12 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
     const int kend = s_kend;
     const int ntiles = (kend + 63) >> 6;
     // this block's key split: tiles [t0, t1) of the rows' visible range
-    const int t0 = min(split * P.pf_tps, ntiles), t1 = min(t0 + P.pf_tps, ntiles);
+    int t0 = min(split * P.pf_tps, ntiles), t1 = min(t0 + P.pf_tps, ntiles);
+    if constexpr (MOD) {
+        const int tb0 = min(s_kbeg >> 6, ntiles);
+        t0 = min(tb0 + split * P.pf_tps, ntiles);
+        t1 = split == P.pf_nsplit - 1 ? ntiles : min(t0 + P.pf_tps, ntiles);
+    }
     const int nt = t1 - t0;
     const double* const T1s = sT1;
     const double* const T2 = sT2;
@@ -826,7 +870,7 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
                 }
         }
         uint32_t vism = rvalid ? 0xFFu : 0u;  // bit 4 kk + i: pair visible
-        if (!((it + 1) * 64 <= kvmin)) {
+        if (!((it + 1) * 64 <= kvmin) || (MOD && it * 64 < kbmax)) {
             vism = 0;
 #pragma unroll
             for (int kk = 0; kk < NKT; ++kk)
@@ -835,7 +879,9 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
                     const int n = it * 64 + 16 * (NKT * hh + kk) + 4 * g + i;
                     const int ti = n - tbase;
                     const bool intree = ((unsigned)ti < 64u) & (((tmk >> (ti & 63)) & 1ull) != 0);
-                    vism |= ((n < slen) & ((n < kvl) | intree)) ? (1u << (4 * kk + i)) : 0u;
+                    bool pre = n < kvl;
+                    if constexpr (MOD) pre = pre & (n >= kvb);
+                    vism |= ((n < slen) & (pre | intree)) ? (1u << (4 * kk + i)) : 0u;
                 }
         }
         if (tfl & 16) {
@@ -860,7 +906,18 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
             pv_mfma(Wd, sVp, kk * (NCT / NKT), (kk + 1) * (NCT / NKT));
             int M[4], E[4];
             bool ok[4];
-            cert_pairs<4>(xs[kk], adel[kk], qm.a, T1s, T2, M, E, ok);
+            if constexpr (MOD) {
+                float m4[4];
+                int dist[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    m4[i] = mslope;
+                    dist[i] = it * 64 + 16 * (NKT * hh + kk) + 4 * g + i - mpos;
+                }
+                cert_pairs<4, MOD>(xs[kk], adel[kk], qm.a, T1s, T2, M, E, ok, P.cap, m4, dist);
+            } else {
+                cert_pairs<4>(xs[kk], adel[kk], qm.a, T1s, T2, M, E, ok);
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const bool vis = (vism >> (4 * kk + i)) & 1;
@@ -895,8 +952,8 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
                          (int64_t)(hk * P.grp + lrc % P.grp) * P.g.q_head_stride;
                     kr = P.k + kv_off(P, b, n, hk, 0);
                 }
-                const int3 cw = pf_cold_pair(mode, qlds, 0, (const uint8_t*)Kg + key * 128, key & 7, qr, kr, P.am,
-                                             P.ae + qm.lsb + TMc->lsbk[key], P.alpha, T1s, T2);
+                const int3 cw = pf_cold_pair<MOD>(mode, qlds, 0, (const uint8_t*)Kg + key * 128, key & 7, qr, kr, P.am,
+                                                  P.ae + qm.lsb + TMc->lsbk[key], P.alpha, T1s, T2, P.cap, mslope, n - mpos);
                 const bool live = cw.x == 0;
                 const int32_t M = cw.y, E = cw.z;
                 if (cw.x == 2) dom = 1;
@@ -1328,8 +1385,9 @@ int ea::ea_launch_prefill(const Params& P, hipStream_t st) {
     static std::once_flag once;
     static hipError_t attr_err = hipSuccess;
     std::call_once(once, [] {
-        const void* fns[4] = {(const void*)ea_pf_main<4, false>, (const void*)ea_pf_main<4, true>,
-                              (const void*)ea_pf_main<8, false>, (const void*)ea_pf_main<8, true>};
+        const void* fns[6] = {(const void*)ea_pf_main<4, false>,    (const void*)ea_pf_main<4, true>,
+                              (const void*)ea_pf_main<8, false>,    (const void*)ea_pf_main<8, true>,
+                              (const void*)ea_pf_main<8, false, 1>, (const void*)ea_pf_main<8, false, 2>};
         for (const void* f : fns)
             if (attr_err == hipSuccess)
                 attr_err = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, PF_LDS);
@@ -1340,7 +1398,9 @@ int ea::ea_launch_prefill(const Params& P, hipStream_t st) {
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return -100 - (int)e;
     if (P.nseg > 0 && P.pf_ntiles > 0 && !P.pf_kv_cached) {
-        hipLaunchKernelGGL(ea_pf_kvslice, dim3((unsigned)(P.nseg * P.pf_ntiles)), dim3(256), 0, st, Pc);
+        const dim3 grid((unsigned)(P.nseg * P.pf_ntiles));
+        if (P.mods) hipLaunchKernelGGL(ea_pf_kvslice<true>, grid, dim3(256), 0, st, Pc);
+        else hipLaunchKernelGGL(ea_pf_kvslice<false>, grid, dim3(256), 0, st, Pc);
         e = hipGetLastError();
         if (e != hipSuccess) return -100 - (int)e;
     }
@@ -1350,7 +1410,7 @@ int ea::ea_launch_prefill(const Params& P, hipStream_t st) {
 int ea::ea_launch_kv_digits(const Params& P, hipStream_t st) {
     if (P.nseg <= 0 || P.kvd_span <= 0) return 0;
     Params Pc = P;
-    hipLaunchKernelGGL(ea_pf_kvslice, dim3((unsigned)(P.nseg * P.kvd_span)), dim3(256), 0, st, Pc);
+    hipLaunchKernelGGL(ea_pf_kvslice<false>, dim3((unsigned)(P.nseg * P.kvd_span)), dim3(256), 0, st, Pc);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : -100 - (int)e;
 }
@@ -1359,7 +1419,11 @@ int ea::ea_launch_prefill_main(const Params& P, hipStream_t st) {
     Params Pc = P;
     if (P.nseg > 0 && P.pf_nrb > 0) {
         const dim3 grid((unsigned)(P.nseg * P.pf_nrb * P.pf_nsplit));
-        if (P.pf_waves != 4) {
+        if (P.mods == 2) {
+            hipLaunchKernelGGL((ea_pf_main<8, false, 2>), grid, dim3(512), PF_LDS, st, Pc);
+        } else if (P.mods) {
+            hipLaunchKernelGGL((ea_pf_main<8, false, 1>), grid, dim3(512), PF_LDS, st, Pc);
+        } else if (P.pf_waves != 4) {
             if (P.timers) hipLaunchKernelGGL((ea_pf_main<8, true>), grid, dim3(512), PF_LDS, st, Pc);
             else hipLaunchKernelGGL((ea_pf_main<8, false>), grid, dim3(512), PF_LDS, st, Pc);
         } else {

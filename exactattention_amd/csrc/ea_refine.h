@@ -139,6 +139,9 @@ struct DDSmem {
 // The listed rows, in grid-stride order; C chunks per row (C > 1 only with rows C <= EA_DD_PARTS and
 // rows C <= gridDim.x). parts: EA_DD_PARTS partials. Certified rows get their output and flag 0,
 // rows with a domain error flag 2; the rest are listed in P.t2left, P.wl_cnt[EA_T2_LEFT] of them.
+// MOD: with score modifications; weights 2^-800 below the row's reference, which leave the row undecided
+// otherwise, then count as terms left out, at most 2^-770 each.
+template <bool MOD = false>
 __device__ inline void dd_rows(const Params& P, DDSmem& S, int cnt, int C, DDPart* parts) {
     const int tid = (int)threadIdx.x, lane = tid & 63, wv = tid >> 6;
     const int d = P.g.head_dim, dv = P.g.head_dim_v, Hq = P.g.num_q_heads, T = P.g.num_tokens;
@@ -157,18 +160,15 @@ __device__ inline void dd_rows(const Params& P, DDSmem& S, int cnt, int C, DDPar
         const int64_t b = row / ((int64_t)T * Hq);
         const int t = (int)((row / Hq) % T), hq = (int)(row % Hq), hk = hq / P.grp;
         const int64_t tok = b * T + t;
-        const int64_t slen = P.seq_len[b], L = vis_prefix(P.kv_len[tok], slen);
-        const int64_t tb = P.tree_mask ? P.tree_base[b] : 0;
-        const uint64_t mask = P.tree_mask ? vis_tree_bits(P.tree_mask[tok], tb, L, slen) : 0ull;
-        const int64_t nkeys = L + __popcll(mask);
+        const int kvl = P.kv_len[tok];
+        const RowKeys keys = row_keys(MOD ? vis_begin(P, tok, kvl) : 0, kvl, P.seq_len[b], P.tree_mask ? P.tree_mask[tok] : 0ull,
+                                      P.tree_mask ? P.tree_base[b] : 0);
+        const int mpos = MOD ? mod_pos(P, tok, kvl) : 0;
+        const float mslope = MOD ? mod_slope(P, hq) : 0.0f;
+        const int64_t nkeys = keys.count();
         const int64_t csz = (nkeys + C - 1) / C;
         const int64_t jc0 = min(nkeys, (int64_t)chunk * csz), jc1 = min(nkeys, jc0 + csz);
-        auto key_n = [&](int64_t j) -> int64_t {
-            if (j < L) return j;
-            uint64_t m = mask;
-            for (int64_t cc = j - L; cc > 0; --cc) m &= m - 1;
-            return tb + (__ffsll((long long)m) - 1);
-        };
+        auto key_n = [&](int64_t j) -> int64_t { return keys.key(j); };
         __syncthreads();  // the previous row's LDS reads are done
         if (tid == 0) {
             S.flag = 0;
@@ -257,10 +257,11 @@ __device__ inline void dd_rows(const Params& P, DDSmem& S, int cnt, int C, DDPar
             int32_t M = 0, E = 0;
             if (have && part == 0 && !bad) {
                 uint32_t tbits = 0;
-                const int ls = !isfinite(s) ? 3
-                               : (s == 0.0 && es == 0.0 && ea == 0.0) ? 1 : logit_cert(P.alpha, s, es, ea * 0x1p-44, &tbits);
+                const bool zero = s == 0.0 && es == 0.0 && ea == 0.0;
+                int ls = !isfinite(s) ? 3 : zero ? 1 : logit_cert(P.alpha, s, es, ea * 0x1p-44, &tbits);
                 bool ok = false;
                 if (ls == 1) tbits = 0;
+                if constexpr (MOD) ls = mod_logit(ls, zero, P.cap, mslope, (int)key_n(j) - mpos, S.T1, 23, &tbits);
                 if (ls <= 1) {
                     ok = pf::table_weight(tbits, S.T1, S.T2, &M, &E);
                     if (!ok) {
@@ -285,25 +286,33 @@ __device__ inline void dd_rows(const Params& P, DDSmem& S, int cnt, int C, DDPar
             const int mx = S.mx;
             if (mx > R + 64) {
                 if (R != DD_NONE) {
-                    if (R - mx < -800) mf = max(mf, 1);
+                    if (!MOD && R - mx < -800) mf = max(mf, 1);
                     const double f = ldexp(1.0, max(R - mx, -800));
-                    dd_scale(z, f);
-                    dd_scale(n[0], f);
-                    dd_scale(n[1], f);
+                    if (MOD && R - mx < -800) {
+                        z = DD{0.0, 0.0, 0.0, dd_size(z) * f};
+                        n[0] = DD{0.0, 0.0, 0.0, dd_size(n[0]) * f};
+                        n[1] = DD{0.0, 0.0, 0.0, dd_size(n[1]) * f};
+                    } else {
+                        dd_scale(z, f);
+                        dd_scale(n[0], f);
+                        dd_scale(n[1], f);
+                    }
                 }
                 R = mx;
             }
             if (M) {
                 // products stay normal numbers down to 2^-800 (2^-133 the smallest V element)
-                if (E - R < -800) mf = max(mf, 1);
-                else if (E + 23 - R < DD_WINDOW) z.err += ldexp((double)M, E - R);
+                if (E - R < -800) {
+                    if (MOD) z.err += 0x1p-770;
+                    else mf = max(mf, 1);
+                } else if (E + 23 - R < DD_WINDOW) z.err += ldexp((double)M, E - R);
                 else dd_add(z, ldexp((double)M, E - R));
             }
             // ---- P.V
             double myw = 0.0;
             if (lane < nk) {
                 const int de = S.E[kb + lane] - R;
-                myw = de < -800 ? 0.0 : ldexp((double)S.M[kb + lane], de);
+                myw = de < -800 ? (MOD && S.M[kb + lane] ? 0x1p-770 : 0.0) : ldexp((double)S.M[kb + lane], de);
             }
             bool vbad = false;
 #pragma unroll
@@ -376,7 +385,7 @@ __device__ inline void dd_rows(const Params& P, DDSmem& S, int cnt, int C, DDPar
             for (int k = 0; k < C; ++k) {
                 if (S.pR[k] == DD_NONE) continue;
                 const double f = ldexp(1.0, max(S.pR[k] - R, -800));
-                if (S.pR[k] - R < -800) fl = max(fl, 1);
+                if (!MOD && S.pR[k] - R < -800) fl = max(fl, 1);
                 if (S.pR[k] - R < DD_WINDOW) z.err += dd_size(S.pz[k]) * f;
                 else dd_join(z, S.pz[k], f);
             }

@@ -46,6 +46,11 @@ class Options(ctypes.Structure):
                 ("prefill_waves", ctypes.c_int32), ("stats_entries", ctypes.c_int32)]
 
 
+class ScoreModsArgs(ctypes.Structure):
+    _fields_ = [("kv_begin", P), ("q_pos", P), ("slopes", P), ("softcap_bits", ctypes.c_uint32), ("window", ctypes.c_int32),
+                ("max_span", ctypes.c_int32), ("pad0", ctypes.c_int32)]
+
+
 class StepPlanArgs(ctypes.Structure):
     _fields_ = ([(n, ctypes.c_int32) for n in ("num_seqs", "page_size", "table_rows", "table_width", "max_tokens", "pad_tokens",
                                                "max_seq_len", "free_capacity")]
@@ -129,6 +134,13 @@ def load():
         lib.ea_hip_kv_append.argtypes = [P, P, ctypes.c_int64, ctypes.c_int64, P, P, P, ctypes.c_int64, P,
                                          ctypes.c_int64, P, P, ctypes.c_int64, P]
         lib.ea_hip_kv_append.restype = ctypes.c_int
+        G, B, O, M = (ctypes.POINTER(x) for x in (Geometry, Buffers, Options, ScoreModsArgs))
+        lib.ea_hip_mods_workspace_size.argtypes = [G, O, M, ctypes.POINTER(ctypes.c_size_t), ctypes.POINTER(ctypes.c_int32)]
+        lib.ea_hip_attention_mods.argtypes = [G, B, O, M, P, ctypes.c_size_t, P]
+        lib.ea_hip_exact_rows_mods.argtypes = [G, B, O, M, P]
+        lib.ea_hip_kat_mod_logit.argtypes = [ctypes.c_int64, P, P, P, ctypes.c_float, P, P, P]
+        for f in (lib.ea_hip_mods_workspace_size, lib.ea_hip_attention_mods, lib.ea_hip_exact_rows_mods, lib.ea_hip_kat_mod_logit):
+            f.restype = ctypes.c_int
         lib.ea_hip_step_plan.argtypes = [ctypes.POINTER(StepPlanArgs), P]
         lib.ea_hip_step_plan.restype = ctypes.c_int
         lib.ea_hip_rotary.argtypes = [ctypes.POINTER(RotaryArgs), P]
@@ -162,13 +174,61 @@ def _stream_ptr(torch):
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-def workspace_size(g: dict, splits: int = 0, out_fp32: bool = False, kernel: int = 0) -> tuple[int, int]:
+def workspace_size(g: dict, splits: int = 0, out_fp32: bool = False, kernel: int = 0, mods=None) -> tuple[int, int]:
+    """Bytes and splits of a step; mods: the ScoreModsArgs of one with score modifications."""
     lib = load()
     o = Options(splits=splits, out_fp32=int(out_fp32), tier2=1, kernel=kernel)
     nb, ns = ctypes.c_size_t(0), ctypes.c_int32(0)
-    _check(lib.ea_hip_workspace_size(ctypes.byref(geometry(g)), ctypes.byref(o), ctypes.byref(nb), ctypes.byref(ns)),
-           "ea_hip_workspace_size")
+    if mods is None:
+        _check(lib.ea_hip_workspace_size(ctypes.byref(geometry(g)), ctypes.byref(o), ctypes.byref(nb), ctypes.byref(ns)),
+               "ea_hip_workspace_size")
+    else:
+        _check(lib.ea_hip_mods_workspace_size(ctypes.byref(geometry(g)), ctypes.byref(o), ctypes.byref(mods), ctypes.byref(nb),
+                                              ctypes.byref(ns)), "ea_hip_mods_workspace_size")
     return int(nb.value), int(ns.value)
+
+
+class ScoreMods:
+    """Score modifications of a step (ea_score_mods): which keys of its prefix a token sees, and what
+    happens to its scores before they weigh. Arrays are numpy or torch, one entry per token (B, T):
+
+      kv_begin   its first key (packed documents); window: at most that many keys of its prefix
+      softcap    scores s become c tanh(s / c), c in base-2 logits as alpha is (a cap C in natural units:
+                 C / ln 2); 0: none
+      slopes     (Hq,) fp32: each key's score falls by slope * |key - q_pos|, in base-2 logits; q_pos
+                 defaults to the end of the token's prefix (kv_len - 1)
+      max_span   a bound of the keys between the first and the last that the tokens of one sequence see,
+                 where it is far below the sequence's length (it sizes the grid, never the result)
+    """
+
+    def __init__(self, kv_begin=None, window: int = 0, slopes=None, q_pos=None, softcap: float = 0.0, max_span: int = 0):
+        c = np.float32(softcap)
+        if not np.isfinite(c) or c < 0 or 0 < c < np.finfo(np.float32).tiny:
+            raise ValueError("softcap must be positive, or 0 for none")
+        if not 0 <= int(window) < 1 << 31 or not 0 <= int(max_span) < 1 << 31:
+            raise ValueError("window and max_span must not be negative")
+        self.kv_begin, self.window, self.slopes, self.q_pos = kv_begin, int(window), slopes, q_pos
+        self.softcap_bits, self.max_span = int(c.view(np.uint32)), int(max_span)
+
+    def bind(self, geom: dict, dev):
+        """(ScoreModsArgs for a step of this geometry, the device tensors it points at)."""
+        import torch
+        tok = int(geom["num_seqs"]) * int(geom["num_tokens"])
+
+        def put(x, name, n, dt):
+            if x is None:
+                return None
+            t = x if hasattr(x, "data_ptr") else torch.from_numpy(np.ascontiguousarray(x))
+            if t.numel() != n:
+                raise ValueError(f"{name} must have {n} entries, got {t.numel()}")
+            if t.is_floating_point() != (dt == torch.float32) or t.is_complex() or t.dtype == torch.bool:
+                raise ValueError(f"{name} must hold {'floats' if dt == torch.float32 else 'whole numbers'}")
+            return t.to(device=dev, dtype=dt).contiguous()
+
+        keep = (put(self.kv_begin, "kv_begin", tok, torch.int32), put(self.q_pos, "q_pos", tok, torch.int32),
+                put(self.slopes, "slopes", int(geom["num_q_heads"]), torch.float32))
+        a = ScoreModsArgs(*(None if t is None else t.data_ptr() for t in keep), self.softcap_bits, self.window, self.max_span, 0)
+        return a, keep
 
 
 ROUTES = {1: "prefill", 2: "decode", 3: "general", 4: "multirow"}
@@ -190,7 +250,7 @@ class DeviceProblem:
     Built once; `launch_hip` then runs steps on it with no allocation."""
 
     def __init__(self, prob: dict, out: str = "bf16", splits: int = 0, device: str = "cuda", kernel: str = "auto",
-                 prefill_waves: int = 0):
+                 prefill_waves: int = 0, mods: ScoreMods | None = None):
         import torch
         self.torch = torch
         self.prob = prob
@@ -221,7 +281,8 @@ class DeviceProblem:
         self.rows = rows
         self.out = torch.empty(prob["out_shape"], dtype=torch.int32 if self.out_fp32 else torch.int16, device=dev)
         self.flags = torch.empty(rows, dtype=torch.uint8, device=dev)
-        nb, self.nsplit = workspace_size(self.geom, splits, self.out_fp32, self.kernel)
+        self.mods, self._mods_keep = (None, None) if mods is None else mods.bind(self.geom, dev)
+        nb, self.nsplit = workspace_size(self.geom, splits, self.out_fp32, self.kernel, self.mods)
         self.workspace = torch.empty(max(nb, 256), dtype=torch.uint8, device=dev)
         self.ws_bytes = nb
         self.stats = torch.zeros(len(STATS), dtype=torch.int64, device=dev)
@@ -258,6 +319,10 @@ def launch_hip(dp: DeviceProblem, alpha_bits: int, merge_order=None, tier2: bool
     lib = load()
     o = options(dp, alpha_bits, merge_order, tier2, events, timers, kv_digits, force_tier2)
     b = dp.buffers()
+    if dp.mods is not None:
+        _check(lib.ea_hip_attention_mods(ctypes.byref(dp._geom_c), ctypes.byref(b), ctypes.byref(o), ctypes.byref(dp.mods),
+                                         dp.workspace.data_ptr(), dp.ws_bytes, _stream_ptr(dp.torch)), "ea_hip_attention_mods")
+        return
     _check(lib.ea_hip_attention(ctypes.byref(dp._geom_c), ctypes.byref(b), ctypes.byref(o), dp.workspace.data_ptr(),
                                 dp.ws_bytes, _stream_ptr(dp.torch)), "ea_hip_attention")
 
@@ -268,7 +333,8 @@ def exact_rows(dp: DeviceProblem, alpha_bits: int) -> None:
     lib = load()
     o = options(dp, alpha_bits)
     b = dp.buffers()
-    _check(lib.ea_hip_exact_rows(ctypes.byref(dp._geom_c), ctypes.byref(b), ctypes.byref(o), _stream_ptr(dp.torch)),
+    m = None if dp.mods is None else ctypes.byref(dp.mods)
+    _check(lib.ea_hip_exact_rows_mods(ctypes.byref(dp._geom_c), ctypes.byref(b), ctypes.byref(o), m, _stream_ptr(dp.torch)),
            "ea_hip_exact_rows")
 
 
@@ -310,16 +376,17 @@ def merge_order_tensor(order, nsplit: int, device="cuda"):
 
 def attention_problem(prob: dict, alpha=None, out: str = "bf16", splits: int = 0, merge_order=None,
                       tier2: bool = True, fallback: bool = True, device: str = "cuda", kernel: str = "auto",
-                      force_tier2: bool = False, prefill_waves: int = 0, *, alpha_bits=None):
+                      force_tier2: bool = False, prefill_waves: int = 0, *, alpha_bits=None, mods: ScoreMods | None = None):
     """Run a problem on the GPU. Returns (out bits shaped (B, T, Hq, dv): uint16 for bf16, uint32
     for fp32; flags (rows,) uint8; stats dict). fallback=False returns the device tiers' flags as
     they are. With fallback=True rows the device tiers leave at flag 1 are recomputed by the host
     exact tier (ea_hip_exact_rows, counted in stats["host_exact_rows"]), and flag 2 raises
     ExactAttentionDomainError, as the reference's backends do (src/exactattn/cpu.py:103-108).
-    `alpha` is the fp32 scale as a value; `alpha_bits=` passes its bit pattern instead."""
+    `alpha` is the fp32 scale as a value; `alpha_bits=` passes its bit pattern instead. mods: score
+    modifications (ScoreMods)."""
     import torch
     alpha_bits = alpha_fp32_bits(alpha, alpha_bits)
-    dp = DeviceProblem(prob, out, splits, device, kernel, prefill_waves)
+    dp = DeviceProblem(prob, out, splits, device, kernel, prefill_waves, mods)
     mo = merge_order_tensor(merge_order, dp.nsplit, device) if merge_order is not None else None
     launch_hip(dp, int(alpha_bits), mo, tier2, force_tier2=force_tier2)
     torch.cuda.synchronize()

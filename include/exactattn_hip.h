@@ -209,6 +209,43 @@ int ea_hip_attention_noalloc(const ea_geometry* g, const ea_buffers* b, const ea
  * 1553-1559 and src/exactattn/cpu.py:105-108 (reference.attention_row). */
 int ea_hip_exact_rows(const ea_geometry* g, const ea_buffers* b, const ea_options* o, ea_stream_t stream);
 
+/* Score modifications: attention whose rows see an interval of the prefix (packed documents, sliding
+ * windows, prefixes that every token sees), whose scores are capped, or get a bias that falls with the
+ * distance. Row (b, t, h) attends the keys begin <= n < kv_len[b*T + t], begin the larger of
+ * kv_begin[b*T + t] and kv_len[b*T + t] - window, plus its tree keys, all below seq_len[b]; a row whose interval
+ * is empty and that has no tree key is +0. Pair (row, n) weighs RN24(2^t2), with t = RN32(alpha s),
+ *   t1 = RN32(c tanh(t / c)) for a cap c (in base-2 logits, as alpha: a cap C of the scores in natural units is C / ln 2),
+ *   t2 = RN32(t1 - slopes[h] * |n - q_pos[b*T + t]|), the difference rounded to fp32 and the rest exact.
+ * t1 is the exact value's rounding or, within 2^-14 of a step of a midpoint, its neighbour; it is a fixed
+ * function of t, and so the output's bits are those of this definition whatever the splits, pages and
+ * batch are, as without modifications. A t2 that is not finite is a domain error (flag 2).
+ * Keys (and block-table entries) before the 64-key tile of the first key that a token of the sequence sees are
+ * not read: their pages may hold other sequences' keys by then. */
+typedef struct ea_score_mods {
+    const int32_t* kv_begin; /* optional device array, per token; below 0 counts as 0 */
+    const int32_t* q_pos;    /* optional device array, per token; NULL: kv_len - 1 */
+    const float* slopes;     /* optional device array, per query head, in base-2 logits per key */
+    uint32_t softcap_bits;   /* fp32 bits of c, positive; 0: none */
+    int32_t window;          /* > 0: keys of the prefix a token sees at most; 0: all */
+    int32_t max_span;        /* > 0: a bound of the keys between the first and the last that the tokens of
+                                one sequence see, when it is below max_seq_len; sizes the split grid. A
+                                range past it costs time and changes nothing. 0: max_seq_len, or
+                                window + num_tokens - 1 */
+    int32_t pad0;
+} ea_score_mods;
+
+/* ea_hip_attention, ea_hip_workspace_size and ea_hip_exact_rows with score modifications (m NULL: without).
+ * Same buffers, options, workspace rules and return codes; -2 also for a negative window or max_span, a
+ * softcap that is negative, subnormal or not finite, and o->timers. o->prefill_waves is not read: the
+ * 8-wave block runs. Steps that ea_hip_attention gives the d = 128 decode kernel run on the multi-row kernel.
+ * Reference counterpart: none (the reference's masks are key lists, src/exactattn/cpu.py:70-109). */
+int ea_hip_mods_workspace_size(const ea_geometry* g, const ea_options* o, const ea_score_mods* m, size_t* bytes,
+                               int32_t* nsplit);
+int ea_hip_attention_mods(const ea_geometry* g, const ea_buffers* b, const ea_options* o, const ea_score_mods* m,
+                          void* workspace, size_t workspace_bytes, ea_stream_t stream);
+int ea_hip_exact_rows_mods(const ea_geometry* g, const ea_buffers* b, const ea_options* o, const ea_score_mods* m,
+                           ea_stream_t stream);
+
 /* The host exact tier on one row of host arrays: q (d), k (n x d), v (n x dv) bf16 bits, alpha as
  * fp32 bits -> out (dv bf16 or fp32 bits). t_bits, w_m, w_e (optional, n entries each) receive
  * the per-key logits t = RN32(alpha s) and weights w = RN24(2^t) = w_m 2^w_e. Returns 0, 2 for a
@@ -289,6 +326,10 @@ int ea_hip_kat_round_ratio(int64_t n, const uint64_t* a_hi, const uint64_t* a_lo
                            int32_t* overflow, ea_stream_t stream);
 int ea_hip_kat_certify_quotient(int64_t n, const int64_t* cases, int32_t fp32, uint32_t* bits, int32_t* ok,
                                 ea_stream_t stream);
+/* ea_hip_kat_mod_logit: t2 of the logits t (fp32 bits) at distances dist with per-pair slopes and the cap c
+ * (0: none) -> bits, status (0 ok, 2 not finite). No reference counterpart. */
+int ea_hip_kat_mod_logit(int64_t n, const uint32_t* t_bits, const int32_t* dist, const float* slope, float cap,
+                         uint32_t* bits, int32_t* status, ea_stream_t stream);
 /* ea_hip_kat_rn32_prod: the exact logit RN32(am * X * 2^E), X a signed 128-bit integer given as
  * (x_hi signed, x_lo) words, |am| < 2^24 -> fp32 bits, status (0 ok, 2 overflow). The prefill
  * kernel's cold path and tier 2 round exact scores with it.
