@@ -1681,7 +1681,7 @@ void set_inputs(Params& P, const Plan& pl, const ea_geometry* g, const ea_buffer
         P.slopes = m->slopes;
         P.cap = mod_cap_of(c);
         P.window = m->window;
-        P.mods = c > 0.0f ? 2 : 1;
+        P.mods = c > 0.0f ? 3 : (m->slopes ? 2 : 1);
     }
     P.g = *g;
     P.q = bf->q; P.k = bf->k; P.v = bf->v;
@@ -1753,7 +1753,9 @@ int list_all(const Params& P, const ea_options* o, unsigned blocks, hipStream_t 
 
 // tier 2 on the listed rows
 void tier2(const Params& P, const ea_options* o, hipStream_t st) {
-    const dim3 grid(o->force_tier2 ? EA_T2_BLOCKS : EA_DD_BLOCKS(P.out_fp32)), blk(EA_T2_THREADS);
+    // 512 blocks cost an empty list 2 us, and one of many rows takes a sixteenth of the time on them: steps
+    // that may list many (2500 capped rows of 16 heads with large scores, 826 listed: 3040 -> 250 us)
+    const dim3 grid(o->force_tier2 ? EA_T2_BLOCKS : EA_DD_BLOCKS(P.out_fp32 || P.rows >= 8192)), blk(EA_T2_THREADS);
     if (o->force_tier2) {
         if (P.mods) hipLaunchKernelGGL(ea_tier2_wide<true>, grid, blk, 0, st, P);
         else hipLaunchKernelGGL(ea_tier2_wide<false>, grid, blk, 0, st, P);

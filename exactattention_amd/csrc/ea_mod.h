@@ -24,57 +24,65 @@
 
 #ifdef __HIPCC__
 #include <hip/hip_runtime.h>
-#define EA_HD __host__ __device__ __forceinline__
+#define EA_MOD_HD __host__ __device__ __forceinline__
 #else
-#define EA_HD inline
+#define EA_MOD_HD inline
 #endif
 
 namespace ea {
 
-// The cap's constants: c (0: none), 1 / c and 2 log2(e) / c, each rounded to fp64 on the host
+// The cap's constants: c (0: none) and 512 log2(e) / c, rounded to fp64 on the host
 struct ModCap {
-    double c, ic, k2;
+    double c, k256;
 };
 inline ModCap mod_cap_of(float c) {
-    if (!(c > 0.0f)) return ModCap{0.0, 0.0, 0.0};
-    return ModCap{(double)c, 1.0 / (double)c, 0x1.71547652b82fep+1 / (double)c};
+    if (!(c > 0.0f)) return ModCap{0.0, 0.0};
+    return ModCap{(double)c, 0x1.71547652b82fep+9 / (double)c};
 }
 
-EA_HD uint32_t mod_bits(float x) {
+EA_MOD_HD uint32_t mod_bits(float x) {
     uint32_t u;
     memcpy(&u, &x, 4);
     return u;
 }
-EA_HD float mod_float(uint32_t u) {
+EA_MOD_HD float mod_float(uint32_t u) {
     float x;
     memcpy(&x, &u, 4);
     return x;
 }
 
-// RN32(c tanh(t / c)). tanh(x) = (1 - e) / (1 + e) with e = 2^-y, y = |t| 2 log2(e) / c (64 and above:
-// e is below the rounding of 1 + e); e from the 2^(j/256) table (times 2^tsh) and a quartic in the rest,
-// r < 2^-8 (truncation below 2^-49). 1 - e cancels for small x, whose error 2^-50 / (2 x) stays below
-// 2^-39 down to x = 2^-11; below it x - x^3 / 3 (next term 2^-45 of x).
-EA_HD float mod_cap(float t, const ModCap& C, const double* T1, int tsh) {
-    const double a = fabs((double)t);
-    const double y = fmin(a * C.k2, 64.0);
-    const double N = ceil(y);
-    const double f = (N - y) * 256.0;
-    const double fj = floor(f);
-    const double r = (f - fj) * 0x1p-8;
-    double p = fma(r, 0x1.3b2ab6fba4e77p-7, 0x1.c6b08d704a0c0p-5);
-    p = fma(r, p, 0x1.ebfbdff82c58fp-3);
-    p = fma(r, p, 0x1.62e42fefa39efp-1);
-    p = fma(r, p, 1.0);
-    const double e = ldexp(T1[(int)fj & 255] * p, -(int)N - tsh);
-    const double th = (1.0 - e) / (1.0 + e);
-    const double x = a * C.ic;
-    const double ts = x * fma(x * x, -0x1.5555555555555p-2, 1.0);
-    return copysignf((float)(C.c * (x < 0x1p-11 ? ts : th)), t);
+// n / d for d in [1, 2] and |n| <= 1, correctly rounded: on the device the steps of the IEEE division
+// without its scaling, which numbers of this size do not need (11 instructions -> 8).
+EA_MOD_HD double mod_div(double n, double d) {
+#ifdef __HIP_DEVICE_COMPILE__
+    double y = __builtin_amdgcn_rcp(d);
+    y = fma(fma(-d, y, 1.0), y, y);
+    y = fma(fma(-d, y, 1.0), y, y);
+    const double q = n * y;
+    return fma(fma(-d, q, n), y, q);
+#else
+    return n / d;
+#endif
+}
+
+// RN32(c tanh(t / c)). tanh(x) = -g / (2 + g) with g = 2^-y - 1, y = |t| 2 log2(e) / c (64 and above: 2^-y
+// is below the rounding of g). y = (i + r) / 256 with i whole: g = S P + (S - 1), S = 2^(-i/256) from the
+// 2^(j/256) table (times 2^tsh), P = 2^(-r/256) - 1 a quartic in r (truncation 2^-41 of it). For i = 0
+// S - 1 is 0 and g = P keeps its relative accuracy down to t = 0; for i > 0 S - 1 is exact and above 2^-9.
+EA_MOD_HD float mod_cap(float t, const ModCap& C, const double* T1, int tsh) {
+    const double y = fmin(fabs((double)t) * C.k256, 16384.0);
+    const double fi = floor(y), r = y - fi;
+    const int j = -(int)fi;
+    double P = fma(r, 0x1.3b2ab6fba4e77p-39, -0x1.c6b08d704a0c0p-29);
+    P = fma(r, P, 0x1.ebfbdff82c58fp-19);
+    P = r * fma(r, P, -0x1.62e42fefa39efp-9);
+    const double S = ldexp(T1[j & 255], (j >> 8) - tsh);
+    const double g = fma(S, P, S - 1.0);
+    return copysignf((float)(C.c * mod_div(-g, 2.0 + g)), t);
 }
 
 // RN32(t - m |dist|)
-EA_HD float mod_bias(float t, float m, int32_t dist) {
+EA_MOD_HD float mod_bias(float t, float m, int32_t dist) {
     const uint32_t ad = dist < 0 ? 0u - (uint32_t)dist : (uint32_t)dist;
     return fmaf(-m, (float)ad, t);
 }
@@ -83,7 +91,7 @@ EA_HD float mod_bias(float t, float m, int32_t dist) {
 // 1, |alpha s| <= 2^-25 without its value (0 when zero). Returns 0 and the bits in *tb, 2 for a domain
 // error, 3 when t's value would be needed; other states pass through. A |t| up to 2^-25 gives the
 // weight 1 whatever it is, so two ends that both do are taken as 0.
-EA_HD int mod_logit(int st, bool zero, const ModCap& C, float m, int32_t dist, const double* T1, int tsh, uint32_t* tb) {
+EA_MOD_HD int mod_logit(int st, bool zero, const ModCap& C, float m, int32_t dist, const double* T1, int tsh, uint32_t* tb) {
     if (st > 1) return st;
     if (st == 1 && !zero) {
         const float lo = mod_bias(-0x1p-25f, m, dist), hi = mod_bias(0x1p-25f, m, dist);

@@ -119,7 +119,7 @@ __device__ __forceinline__ double rot4(double w) {
 
 }  // namespace
 
-// MOD: with score modifications (ea_mod.h), 1 without a cap and 2 with one. A unit's key range is then
+// MOD: with score modifications (ea_mod.h): 1 key ranges alone, 2 with a bias, 3 with a cap. A unit's key range is then
 // counted from its rows' first visible key, down to a whole tile, and on uniform splits the last split
 // takes every key past the others.
 template <int RS, int DK, int CPL, int MOD = 0>
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(MR_THREADS, (mr_waves<RS, DK>())) ea_mrow(Para
         }
         int mpos[NR];
         float mslope[NR];
-        if constexpr (MOD) {
+        if constexpr (MOD >= 2) {
 #pragma unroll
             for (int s = 0; s < NR; ++s) {
                 mpos[s] = S.pos[RS == 16 ? c : (c & 3) + 4 * s];
@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(MR_THREADS, (mr_waves<RS, DK>())) ea_mrow(Para
             // ---- certified weights
             int M[NP], E[NP];
             bool ok[NP];
-            if constexpr (MOD) {
+            if constexpr (MOD >= 2) {
                 float m[NP];
                 int dist[NP];
 #pragma unroll
@@ -548,7 +548,7 @@ __global__ void __launch_bounds__(MR_THREADS, (mr_waves<RS, DK>())) ea_mrow(Para
                         const bool zero = ss == 0.0 && es == 0.0 && ea == 0.0;
                         ls = zero ? 1 : logit_cert(alpha, ss, es, ea * 0x1p-44, &tbits);
                         if (ls == 1) tbits = 0;
-                        if constexpr (MOD) ls = mod_logit(ls, zero, P.cap, S.slope[en.x], en.y - S.pos[en.x], S.T1, 23, &tbits);
+                        if constexpr (MOD >= 2) ls = mod_logit(ls, zero, P.cap, S.slope[en.x], en.y - S.pos[en.x], S.T1, 23, &tbits);
                     }
                     if (ls == 2 || ls == 3) {
                         why = 1;  // undecided, or an overflow (tier 2 reports the domain error)
@@ -811,14 +811,15 @@ __global__ void __launch_bounds__(MR_THREADS, (mr_waves<RS, DK>())) ea_mrow(Para
 
 namespace {
 
-// mod: Params::mods of ea_mod.h's variants, 0 the plain kernel
+// MOD: Params::mods, 0 the plain kernel
 template <int RS, int MOD>
 const void* mrow_fn(bool small) {
     return small ? (const void*)ea_mrow<RS, 2, 4, MOD> : (const void*)ea_mrow<RS, 4, 8, MOD>;
 }
 template <int RS>
 const void* mrow_fn(bool small, int mod) {
-    return mod == 2 ? mrow_fn<RS, 2>(small) : (mod ? mrow_fn<RS, 1>(small) : mrow_fn<RS, 0>(small));
+    return mod == 3 ? mrow_fn<RS, 3>(small)
+                    : (mod == 2 ? mrow_fn<RS, 2>(small) : (mod ? mrow_fn<RS, 1>(small) : mrow_fn<RS, 0>(small)));
 }
 template <int RS>
 size_t mrow_lds(bool small, int mod) {
@@ -839,7 +840,7 @@ hipError_t mrow_attrs() {
     static std::once_flag once;
     static hipError_t err = hipSuccess;
     std::call_once(once, [] {
-        for (int mod = 0; mod < 3; ++mod)
+        for (int mod = 0; mod < 4; ++mod)
             for (int small = 0; small < 2; ++small) {
                 const void* fns[3] = {mrow_fn<4>(small, mod), mrow_fn<8>(small, mod), mrow_fn<16>(small, mod)};
                 for (const void* f : fns) {
@@ -871,7 +872,7 @@ int ea::ea_mrow_eligible(const Params& P) {
 int ea::ea_mrow_slots(const Params& P, int* slots) {
     // blocks resident on the current device at once, cached per device and kernel
     static std::mutex mu;
-    static int cache[64][18] = {};
+    static int cache[64][24] = {};
     hipError_t e = mrow_attrs();
     if (e != hipSuccess) return -100 - (int)e;
     int dev = 0;

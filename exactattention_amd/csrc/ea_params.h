@@ -24,7 +24,7 @@ namespace ea {
 #define EA_T2_NEXT (3 + EA_T2_ROWS)
 #define EA_T2_CHUNKS (4 + EA_T2_ROWS)
 #define EA_T2_CNT (EA_T2_CHUNKS + EA_T2_BLOCKS)
-#define EA_DD_BLOCKS(fp32) ((fp32) ? 512 : 32)  // of the double-double pass: two per CU where many rows are listed
+#define EA_DD_BLOCKS(many) ((many) ? 512 : 32)  // of the double-double pass: two per CU where many rows are listed
 
 // ------------------------------------------------------------------------------------------------
 // Kernel parameters
@@ -124,7 +124,7 @@ struct Params {
     const float* slopes;      // per query head; NULL: no bias
     ModCap cap;
     int32_t window;           // > 0: a token's prefix starts at kv_len - window at the earliest
-    int32_t mods;             // the MOD variant: 0 none, 1 key ranges and bias, 2 those and the cap
+    int32_t mods;             // the MOD variant: 0 none, 1 key ranges, 2 those and the bias, 3 and the cap
 };
 
 // Token `tok`'s first prefix key, its prefix ending at kvl

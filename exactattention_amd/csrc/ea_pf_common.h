@@ -178,9 +178,9 @@ __device__ __forceinline__ int3 pf_cold_pair(int mode, const uint8_t* qrow, int 
 // unscaled evaluation times a power of two: the same bits); rounded to an integer by adding and
 // subtracting 1.5 * 2^52; certified when |Y - RN(Y)| <= 1/2 - 2^-26 (the fp64 evaluation error
 // is below 2^-26.9). ok[i] false: the exact path decides.
-// MOD 1: with the bias -m[i] |dist[i]|; 2: with the cap before it. A decided t0 is modified as it is; where
-// only |alpha s| <= 2^-25 is known, both ends of that interval are, and must give one weight (the cap only
-// shrinks it).
+// MOD 2: with the bias -m[i] |dist[i]|; 3: with the cap before it. A decided t0 is modified as it is. Where
+// only |alpha s| <= 2^-25 is known, a pair without a bias weighs 1, and one with a bias is decided when its
+// score is an exact 0.
 // ------------------------------------------------------------------------------------------------
 template <int NP, int MOD = 0>
 __device__ __forceinline__ void cert_pairs(const double (&xs)[NP], const double (&adel)[NP], double a, const double* T1s,
@@ -205,15 +205,14 @@ __device__ __forceinline__ void cert_pairs(const double (&xs)[NP], const double 
         const bool inner = (__fma_rn(fabs(r), 1.0 + 0x1p-50, adel[i]) < h) & (at >= 0x1p-24) & (at < 0x1p30);
         ok[i] = tiny | inner;
         d0[i] = tiny ? 0.0 : t0;
-        if constexpr (MOD) {
+        if constexpr (MOD >= 2) {
             float tc = tf;
-            if constexpr (MOD == 2) tc = mod_cap(tf, C, T1s, 23);
-            const float dl = (float)((fabs(p) + fabs(pe) + adel[i]) * (1.0 + 0x1p-20));
-            const float hi = mod_bias(tiny ? dl : tc, m[i], dist[i]), lo = mod_bias(tiny ? -dl : tc, m[i], dist[i]);
-            const float ah = fabsf(hi);
-            const bool one = (ah <= 0x1p-25f) & (fabsf(lo) <= 0x1p-25f);
-            ok[i] = ok[i] & (one | ((hi == lo) & (ah >= 0x1p-24f) & (ah < 0x1p30f)));
-            d0[i] = one | !ok[i] ? 0.0 : (double)hi;
+            if constexpr (MOD == 3) tc = mod_cap(tf, C, T1s, 23);
+            const float t2 = mod_bias(tiny ? 0.0f : tc, m[i], dist[i]), ah = fabsf(t2);
+            const bool one = ah <= 0x1p-25f;
+            const bool t_known = inner | (tiny & ((m[i] == 0.0f) | ((p == 0.0) & (adel[i] == 0.0))));
+            ok[i] = t_known & (one | ((ah >= 0x1p-24f) & (ah < 0x1p30f)));
+            d0[i] = (ok[i] & !one) ? (double)t2 : 0.0;
         }
     }
     double fl[NP], rr[NP];

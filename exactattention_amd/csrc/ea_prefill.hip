@@ -419,12 +419,17 @@ constexpr int PF_OFF_X = PF_OFF_WD + 10240;  // up to 8 waves x 64 lanes x 16 by
 constexpr int PF_OFF_KEND = PF_OFF_X + 8192;
 constexpr int PF_LDS = PF_OFF_KEND + 16;
 
+// MOD: a row's base leaves its largest weight at 2^23 to 2^24 times 2^PF_MOD_TOP0 of 2^38, with room for
+// larger ones to come; one that has to move shows scores of a wide spread, whose many small weights lose
+// bits below the base, and leaves it at PF_MOD_TOP.
+constexpr int PF_MOD_TOP0 = 11, PF_MOD_TOP = 13;
+
 template <int N>
 struct PfPar {
     static constexpr int value = N;
 };
 
-// MOD: with score modifications (ea_mod.h), 1 without a cap and 2 with one; a block's tiles then start at
+// MOD: with score modifications (ea_mod.h): 1 key ranges alone, 2 with a bias, 3 with a cap; a block's tiles then start at
 // its rows' first visible key, and its last key split takes every tile past the others.
 template <int NWB, bool TIMERS, int MOD = 0>
 __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
@@ -630,6 +635,15 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
     double z = 0.0;  // this wave's keys
     int nv = 0;
     int nfrac = 0;   // this wave's keys of the current epoch whose scaled weight may have a fraction
+    // MOD: instead of their number, the sum of what rounding the scaled weights moved them by in the epoch. Of
+    // large scores most weights lie far below the base, where that is the weight and not a half
+    float dsum = 0.0f;
+    // The row's sum over its 4 lanes, times |X| < 2^30 of a key's V row: two additions here, SPLIT before and
+    // the up to 1024 of each lane lose less than 2^-10 of it
+    auto frac_total = [&](float pair) __attribute__((always_inline)) {
+        pair += __shfl_xor(pair, 16, 64);
+        return (pair + __shfl_xor(pair, 32, 64)) * (0x1p30f * (1.0f + 0x1p-10f));
+    };
     // P.V state (P.V layout): int32 accumulators of digit weights 256^1 .. 256^7, 4 channel tiles
     v4i pacc[NCT][7];
 #pragma unroll
@@ -641,6 +655,10 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
     for (int cc = 0; cc < NCT; ++cc) EVs[cc] = 0.0;
     int ep_tiles = 0;
     bool had_fold = false;  // scr holds the sums of earlier epochs
+    // MOD: the bound of what earlier epochs left out, per row (score layout), and the tiles since the base
+    // last moved for the accumulators' sake
+    float err = 0.0f;
+    int since = 0;
     uint32_t failbits = 0;
 
     // fp64 value of the int32 P.V accumulators of (channel tile cc, row 4 g + i) in units 2^base,
@@ -657,6 +675,50 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
         }
         *en = 6.02 * 0x1p-53 * (ha * 256.0) + EVs[cc] + omit + fr_i;
         return h * 256.0;
+    };
+    // ---- MOD: the epoch's sums back into the accumulators at the new bases nb. Modified scores move the
+    // base often (large scores: 5 times a wave in 20 tiles), and a fold to memory costs 14,000 cycles
+    // there, a round trip per entry. The sum, units 2^base 256, is cut into three parts 24 bits apart, the
+    // slots 256^7, 256^4 and 256^1: |N| <= 2^74 per tile of 64 keys (weights to 2^38, |X| < 2^30), so the top
+    // one stays below 2^30 for 4096 tiles, and with the 2^28 that 256 tiles add below 2^31. The rest is a
+    // rounding of 2^7. What the epoch left out becomes one bound per row, the largest over the wave's channels.
+    auto refold = [&](float ds_pair, int nb) __attribute__((always_inline)) {
+        ++nfold;
+        const float ft = frac_total(ds_pair);
+        dsum = 0.0f;
+        const double omit = (double)ep_tiles * 0x1p20;
+        const int sh = base == INT_MIN ? 0 : max(base - nb, -1100);  // of the row in the score layout
+        int er = 0;  // row j's bound as fp32 bits, in the score layout
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const double fr = (double)__shfl(ft, 4 * g + i, 64);
+            const int dsh = __shfl(sh, 4 * g + i, 64);
+            double e = 0.0;
+#pragma unroll
+            for (int cc = 0; cc < NCT; ++cc) {
+                double en;
+                const double nn = epoch_sum(cc, i, fr, omit, &en);
+                e = fmax(e, en);
+                double v = ldexp(nn, dsh - 8);
+                const double A = rint(v * 0x1p-48);
+                v = __fma_rn(-A, 0x1p48, v);
+                const double B = rint(v * 0x1p-24);
+                v = __fma_rn(-B, 0x1p24, v);
+#pragma unroll
+                for (int k = 0; k < 7; ++k) pacc[cc][k][i] = 0;
+                pacc[cc][6][i] = (int)A;
+                pacc[cc][3][i] = (int)B;
+                pacc[cc][0][i] = (int)rint(v);
+            }
+            const float ef = (float)((ldexp(e, dsh) + 0x1p8) * (1.0 + 0x1p-20));
+            const int em = row16_max(__float_as_int(ef));  // the 16 channels of row 4 g + i; bounds are positive
+            const int mine = __shfl(em, 16 * (j >> 2), 64);
+            er = (j & 3) == i ? mine : er;
+        }
+        err = (ldexpf(err, sh) + __int_as_float(er)) * (1.0f + 0x1p-20f);
+#pragma unroll
+        for (int cc = 0; cc < NCT; ++cc) EVs[cc] = 0.0;
+        ep_tiles = 0;
     };
     // ---- fold the epoch into the per-lane fp64 sums in scr, rescaled to the new bases nb
     auto fold = [&](int nf_pair, int nb) __attribute__((always_inline)) {
@@ -738,16 +800,24 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
     auto rebase_digits = [&](const double (&evp)[NCT]) __attribute__((always_inline)) {
         int gm = cgm;
         int nf_pair = nfrac;  // the row group's keys (all SPLIT waves) of the epoch
+        float ds_pair = dsum;
 #pragma unroll
         for (int o = 1; o < SPLIT; ++o) {
             const PfX x = sX[(rg * SPLIT + (hh + o) % SPLIT) * 64 + lane];
             gm = max(gm, x.a);
-            nf_pair += x.b;
+            if constexpr (MOD) ds_pair += __int_as_float(x.b);
+            else nf_pair += x.b;
         }
         // the base moves when a weight would exceed 2^38 (G - base > 14 for G = E + vlsb)
         const bool need_rb = gm != INT_MIN && (base == INT_MIN || gm > base + 14);
-        const int nb = need_rb ? gm - 10 : base;
-        if (ep_tiles > 0 && (__ballot(need_rb) != 0 || ep_tiles >= 256)) fold(nf_pair, nb);
+        int nb = need_rb ? gm - (!MOD ? 10 : (base == INT_MIN ? PF_MOD_TOP0 : PF_MOD_TOP)) : base;
+        if constexpr (MOD) {
+            if (++since > 4096 && base != INT_MIN) nb = max(nb, base + 8);
+            if (ep_tiles > 0 && (__ballot(nb != base) != 0 || ep_tiles >= 256)) refold(ds_pair, nb);
+            if (since > 4096) since = 0;
+        } else {
+            if (ep_tiles > 0 && (__ballot(need_rb) != 0 || ep_tiles >= 256)) fold(nf_pair, nb);
+        }
 #pragma unroll
         for (int cc = 0; cc < NCT; ++cc) EVs[cc] += evp[cc];
         if (nb != base && base != INT_MIN) z = ldexp(z, max(base - nb, -1100));
@@ -763,8 +833,10 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
                     const double wsc = ldexp(md, sc + cvl[kk][i]);  // <= 2^38
                     z += ldexp(md, sc);                             // md = 0 for masked pairs
                     nv += Mp ? 1 : 0;
-                    nfrac += (Mp && sc + cvl[kk][i] < 0) ? 1 : 0;
-                    const uint64_t yb = f64_as_u64(wsc + PF_C40);
+                    const double yw = wsc + PF_C40;
+                    if constexpr (MOD) dsum += fabsf((float)(wsc - (yw - PF_C40)));
+                    else nfrac += (Mp && sc + cvl[kk][i] < 0) ? 1 : 0;
+                    const uint64_t yb = f64_as_u64(yw);
                     L[i] = (uint32_t)yb;
                     H[i] = (uint32_t)(yb >> 32);
                 }
@@ -906,7 +978,7 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
             pv_mfma(Wd, sVp, kk * (NCT / NKT), (kk + 1) * (NCT / NKT));
             int M[4], E[4];
             bool ok[4];
-            if constexpr (MOD) {
+            if constexpr (MOD >= 2) {
                 float m4[4];
                 int dist[4];
 #pragma unroll
@@ -952,7 +1024,7 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
                          (int64_t)(hk * P.grp + lrc % P.grp) * P.g.q_head_stride;
                     kr = P.k + kv_off(P, b, n, hk, 0);
                 }
-                const int3 cw = pf_cold_pair<MOD>(mode, qlds, 0, (const uint8_t*)Kg + key * 128, key & 7, qr, kr, P.am,
+                const int3 cw = pf_cold_pair<(MOD >= 2)>(mode, qlds, 0, (const uint8_t*)Kg + key * 128, key & 7, qr, kr, P.am,
                                                   P.ae + qm.lsb + TMc->lsbk[key], P.alpha, T1s, T2, P.cap, mslope, n - mpos);
                 const bool live = cw.x == 0;
                 const int32_t M = cw.y, E = cw.z;
@@ -983,7 +1055,7 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
         // row group's exchange after the next B1
         gm = max(gm, __shfl_xor(gm, 16, 64));
         gm = max(gm, __shfl_xor(gm, 32, 64));
-        sX[w * 64 + lane] = PfX{gm, nfrac, 0.0};
+        sX[w * 64 + lane] = PfX{gm, MOD ? __float_as_int(dsum) : nfrac, 0.0};
         cgm = gm;
 #pragma unroll
         for (int kk = 0; kk < NKT; ++kk) {
@@ -1028,21 +1100,31 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
     dom |= __shfl_xor(dom, 32, 64);
     unc |= __shfl_xor(unc, 16, 64);
     unc |= __shfl_xor(unc, 32, 64);
-    sX[w * 64 + lane] = PfX{nv, nfrac | (dom << 24) | (unc << 25), z};
+    // MOD: the flags in the last bits of the sum, rounded up
+    const int fdom = (__float_as_int(dsum) & ~3) + 4;
+    sX[w * 64 + lane] = MOD ? PfX{nv, fdom | dom | (unc << 1), z} : PfX{nv, nfrac | (dom << 24) | (unc << 25), z};
     pf_bar();
     int nf_pair = nfrac;
+    float ds_pair = __int_as_float(fdom);
     {
 #pragma unroll
         for (int o = 1; o < SPLIT; ++o) {
             const PfX x = sX[(rg * SPLIT + (hh + o) % SPLIT) * 64 + lane];
             nv += x.a;
-            nf_pair += x.b & 0xFFFFFF;
-            dom |= (x.b >> 24) & 1;
-            unc |= (x.b >> 25) & 1;
+            if constexpr (MOD) {
+                ds_pair += __int_as_float(x.b & ~3);
+                dom |= x.b & 1;
+                unc |= (x.b >> 1) & 1;
+            } else {
+                nf_pair += x.b & 0xFFFFFF;
+                dom |= (x.b >> 24) & 1;
+                unc |= (x.b >> 25) & 1;
+            }
             z += x.c;
         }
     }
     tick(10);
+    const float ft = MOD ? frac_total(ds_pair) : 0.0f;
     if (P.pf_nsplit > 1) {
         // ---- key splits: this split's (N, bound) per (row, channel) and (base, nv, flags, Z) per
         // row, in units 2^base; ea_pf_combine merges the splits and rounds. Every record a
@@ -1059,12 +1141,13 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
                 if (lri >= P.r_seg) continue;
                 int ti;
                 const int64_t gr = seg_row(P, b, hk, lri, &ti);
-                const double fri = 0x1p29 * (double)__shfl(nf, 4 * g + i, 64);
+                double fri = 0x1p29 * (double)__shfl(nf, 4 * g + i, 64);
+                if constexpr (MOD) fri = (double)__shfl(ft, 4 * g + i, 64) + (double)__shfl(err, 4 * g + i, 64);
 #pragma unroll
                 for (int cc = 0; cc < NCT; ++cc) {
                     double en;
                     double nn = epoch_sum(cc, i, fri, omit, &en);
-                    if (had_fold) {
+                    if (!MOD && had_fold) {
                         const double2 o = *(const double2*)(scr + 2 * (4 * cc + i));
                         nn += o.x;
                         en += o.y;
@@ -1109,7 +1192,8 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
     if (nt > 0) {
         double2 prev[4 * NCT];
 #pragma unroll
-        for (int e = 0; e < 4 * NCT; ++e) prev[e] = had_fold ? *(const double2*)(scr + 2 * e) : make_double2(0.0, 0.0);
+        for (int e = 0; e < 4 * NCT; ++e)
+            prev[e] = !MOD && had_fold ? *(const double2*)(scr + 2 * e) : make_double2(0.0, 0.0);
         int nf = nf_pair + __shfl_xor(nf_pair, 16, 64);
         nf += __shfl_xor(nf, 32, 64);
         double fr[4], Zr[4], eZr[4], rz[4], rze[4];
@@ -1117,6 +1201,7 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             fr[i] = 0x1p29 * (double)__shfl(nf, 4 * g + i, 64);
+            if constexpr (MOD) fr[i] = (double)__shfl(ft, 4 * g + i, 64) + (double)__shfl(err, 4 * g + i, 64);
             Zr[i] = __shfl(z, 4 * g + i, 64);
             const int nvr = __shfl(nv, 4 * g + i, 64);
             eZr[i] = (double)(nvr + 8) * PF_U * Zr[i] + (double)(nvr + 64) * 0x1p-1074;
@@ -1385,9 +1470,10 @@ int ea::ea_launch_prefill(const Params& P, hipStream_t st) {
     static std::once_flag once;
     static hipError_t attr_err = hipSuccess;
     std::call_once(once, [] {
-        const void* fns[6] = {(const void*)ea_pf_main<4, false>,    (const void*)ea_pf_main<4, true>,
+        const void* fns[7] = {(const void*)ea_pf_main<4, false>,    (const void*)ea_pf_main<4, true>,
                               (const void*)ea_pf_main<8, false>,    (const void*)ea_pf_main<8, true>,
-                              (const void*)ea_pf_main<8, false, 1>, (const void*)ea_pf_main<8, false, 2>};
+                              (const void*)ea_pf_main<8, false, 1>, (const void*)ea_pf_main<8, false, 2>,
+                              (const void*)ea_pf_main<8, false, 3>};
         for (const void* f : fns)
             if (attr_err == hipSuccess)
                 attr_err = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, PF_LDS);
@@ -1419,7 +1505,9 @@ int ea::ea_launch_prefill_main(const Params& P, hipStream_t st) {
     Params Pc = P;
     if (P.nseg > 0 && P.pf_nrb > 0) {
         const dim3 grid((unsigned)(P.nseg * P.pf_nrb * P.pf_nsplit));
-        if (P.mods == 2) {
+        if (P.mods == 3) {
+            hipLaunchKernelGGL((ea_pf_main<8, false, 3>), grid, dim3(512), PF_LDS, st, Pc);
+        } else if (P.mods == 2) {
             hipLaunchKernelGGL((ea_pf_main<8, false, 2>), grid, dim3(512), PF_LDS, st, Pc);
         } else if (P.mods) {
             hipLaunchKernelGGL((ea_pf_main<8, false, 1>), grid, dim3(512), PF_LDS, st, Pc);

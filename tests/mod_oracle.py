@@ -28,28 +28,23 @@ def _table():
     return [float(Decimal(2) ** (Decimal(j) / 256)) for j in range(256)]
 
 
-_POLY = [float(LN2 ** k / math.factorial(k)) for k in (4, 3, 2, 1)] + [1.0]
+_POLY = [float((-LN2 / 256) ** k / math.factorial(k)) for k in (4, 3, 2, 1)]
 
 
 def cap32(t: float, c: float) -> float:
     """RN32(c tanh(t / c)) as ea_mod.h computes it; t and c fp32 values."""
     if not c:
         return t
-    a = abs(t)
-    y = min(a * (float(2 / LN2) / c), 64.0)
-    n = math.ceil(y)
-    f = (n - y) * 256.0
-    j = math.floor(f)
-    r = (f - j) / 256.0
+    y = min(abs(t) * (float(512 / LN2) / c), 16384.0)
+    i = math.floor(y)
+    r = y - i
     p = _POLY[0]
     for q in _POLY[1:]:
         p = fma(r, p, q)
-    e = math.ldexp(_table()[j & 255] * p, -n)
-    th = (1.0 - e) / (1.0 + e)
-    x = a * (1.0 / c)
-    if x < 2.0 ** -11:
-        th = x * fma(x * x, -1.0 / 3.0, 1.0)
-    return math.copysign(float(np.float32(c * th)), t)
+    p = r * p
+    s = math.ldexp(_table()[-i & 255], -i >> 8)
+    g = fma(s, p, s - 1.0)
+    return math.copysign(float(np.float32(c * (-g / (2.0 + g)))), t)
 
 
 def tanh_exact(t: float, c: float) -> Decimal:
