@@ -19,150 +19,133 @@ int herr(hipError_t e) { return e == hipSuccess ? 0 : -100 - (int)e; }
 //   page i of the new ones of b is free[num_free - 1 - np_b - i] (a stack, its top first)
 //   token j of b, at flat index cu_b + j: position L_b + j, its page from the table when it has one
 //   there already, else from the stack; its pool row is page P + position % P
-// What bounds it is latency: 24 bytes a token leave it and a step of 100,000 tokens writes 3 MB. So it
-// is one launch: every block scans the sequences by itself (12 bytes each, from the L2 after the
-// first) and then takes its share of the tokens, pages and padded rows; no block reads what another
-// one writes (new pages come from the stack, not from the table), so no block waits for another.
-// Every input is checked by each block alike: a step that does not fit leaves the table alone and
-// reports why.
+// What bounds it is latency: 24 bytes a token leave it, and a step of 125,000 tokens writes 5 MB. So it
+// is one launch of a short chain: every block reads the sequences (12 bytes each), sums them up in LDS by
+// itself, and takes its share of the padded rows (b, j), whose sequence is a division away, without a
+// search. A row with a token writes all that belongs to it, and the table entry too where it opens a
+// page. No block reads what another one writes (new pages come from the stack, not from the table), so
+// none waits for another. Every input is checked by each block alike: a step that does not fit leaves
+// the table alone and reports why.
 // ------------------------------------------------------------------------------------------------
 constexpr int SP_THREADS = 1024;
 constexpr int SP_MAX_SEQS = 8192;
 constexpr int SP_MAX_ROWS = 65536;
 
-struct PlanSmem {
-    int64_t part[2][SP_THREADS / 64];
-    int status;
-};
-
-// inclusive sums over the block of two values per thread
-__device__ __forceinline__ void block_scan2(PlanSmem& S, int64_t& a, int64_t& b) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int64_t x = __shfl_up(a, o, 64), y = __shfl_up(b, o, 64);
-        if (lane >= o) {
-            a += x;
-            b += y;
-        }
-    }
-    if (lane == 63) {
-        S.part[0][w] = a;
-        S.part[1][w] = b;
-    }
-    __syncthreads();
-    for (int i = 0; i < w; ++i) {
-        a += S.part[0][i];
-        b += S.part[1][i];
-    }
-}
-
-// the last b in [0, n) with x[b] <= i: x ascends from x[0] = 0, x[n] > i
-__device__ __forceinline__ int find_seq(const int* x, int n, int i) {
-    int lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const int m = (lo + hi) >> 1;
-        if (x[m] <= i) lo = m;
-        else hi = m;
-    }
-    return lo;
+// inclusive sum over the wave: within each 16 lanes, then across (row broadcasts)
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
+    return x;
 }
 
 __global__ void __launch_bounds__(SP_THREADS) ea_step_plan_kernel(ea_step_plan A, int pshift) {
     extern __shared__ __align__(16) int smem[];
-    __shared__ PlanSmem S;
-    const int tid = threadIdx.x, B = A.num_seqs, P = A.page_size;
-    int* const cu = smem;                       // B + 1
-    int* const np = smem + B + 1;               // B + 1
-    uint32_t* const seen = (uint32_t*)(smem + 2 * B + 2);  // a bit per table row
+    __shared__ int part[2][SP_THREADS / 64];
+    __shared__ int s_status, s_pages;
+    const int tid = threadIdx.x, B = A.num_seqs, P = A.page_size, T = A.pad_tokens;
+    int* const cu = smem;          // B + 1
+    int* const np = cu + B + 1;    // B: counts until the sums are known
+    int* const len = np + B;       // B
+    int* const row = len + B;      // B
+    uint32_t* const seen = (uint32_t*)(row + B);  // a bit per table row
     const int words = (A.table_rows + 31) / 32;
+    const int nf = *A.num_free;
     for (int i = tid; i < words; i += SP_THREADS) seen[i] = 0;
-    if (tid == 0) S.status = 0;
+    if (tid == 0) s_status = 0;
     __syncthreads();
     const int64_t room = min((int64_t)A.table_width << pshift, (int64_t)A.max_seq_len);
     const int per = (B + SP_THREADS - 1) / SP_THREADS;
     const int b0 = min(tid * per, B), b1 = min(b0 + per, B);
-    int bad = 0;
-    int64_t st = 0, sp = 0;
+    auto need_of = [&](int64_t L, int64_t c) { return (int)(((L + c + P - 1) >> pshift) - ((L + P - 1) >> pshift)); };
+    int bad = 0, st = 0, sp = 0;
     for (int b = b0; b < b1; ++b) {
         const int64_t L = A.seq_len[b], c = A.counts[b];
         const int s = A.slots ? A.slots[b] : b;
+        np[b] = 0;
+        len[b] = (int)L;
+        row[b] = s;
         if (L < 0 || c < 0 || s < 0 || s >= A.table_rows) {
             bad |= EA_PLAN_BAD_INPUT;
             continue;
         }
         if (atomicOr(&seen[s >> 5], 1u << (s & 31)) >> (s & 31) & 1) bad |= EA_PLAN_BAD_INPUT;
         if (L + c > room) bad |= EA_PLAN_TOO_LONG;
-        if (A.kv_len && c > A.pad_tokens) bad |= EA_PLAN_TOO_MANY;
-        st += c;
-        sp += ((L + c + P - 1) >> pshift) - ((L + P - 1) >> pshift);
+        if (c > T) {
+            bad |= EA_PLAN_TOO_MANY;
+            continue;
+        }
+        // at most B T tokens, below 2^31, and no more pages than tokens
+        np[b] = (int)c;
+        st += (int)c;
+        sp += need_of(L, c);
     }
-    int64_t at = st, ap = sp;
-    block_scan2(S, at, ap);
-    __syncthreads();  // part is read before the totals below reuse nothing of it
-    const int nf = *A.num_free;
+    int at = wave_scan(st), ap = wave_scan(sp);
+    if ((tid & 63) == 63) {
+        part[0][tid >> 6] = at;
+        part[1][tid >> 6] = ap;
+    }
+    __syncthreads();
+    for (int i = 0; i < tid >> 6; ++i) {
+        at += part[0][i];
+        ap += part[1][i];
+    }
     if (tid == SP_THREADS - 1) {
         if (at > A.max_tokens) bad |= EA_PLAN_TOO_MANY;
         if (nf < 0 || nf > A.free_capacity) bad |= EA_PLAN_BAD_INPUT;
         else if (ap > nf) bad |= EA_PLAN_NO_PAGES;
+        cu[B] = at;
+        s_pages = ap;
     }
-    if (bad) atomicOr(&S.status, bad);
+    if (bad) atomicOr(&s_status, bad);
     at -= st;
     ap -= sp;
-    __syncthreads();
-    const int status = S.status;
-    if (!status) {
-        // sums below 2^31 from here on: at most max_tokens tokens, at most free_capacity pages
-        for (int b = b0; b < b1; ++b) {
-            const int L = A.seq_len[b], c = A.counts[b];
-            cu[b] = (int)at;
-            np[b] = (int)ap;
-            at += c;
-            ap += (((int64_t)L + c + P - 1) >> pshift) - (((int64_t)L + P - 1) >> pshift);
-        }
-        if (tid == SP_THREADS - 1) {
-            cu[B] = (int)at;
-            np[B] = (int)ap;
-        }
+    for (int b = b0; b < b1; ++b) {
+        const int c = np[b], n = need_of(len[b], c);
+        cu[b] = at;
+        np[b] = ap;
+        at += c;
+        ap += n;
     }
     __syncthreads();
-    const int total = status ? 0 : cu[B], news = status ? 0 : np[B];
+    const int status = s_status;
+    const int total = status ? 0 : cu[B];
     const int64_t g0 = (int64_t)blockIdx.x * SP_THREADS + tid, gs = (int64_t)gridDim.x * SP_THREADS;
     if (g0 == 0) {
         *A.status = status;
-        *A.new_num_free = nf - news;
+        *A.new_num_free = nf - (status ? 0 : s_pages);
     }
-    for (int64_t b = g0; b < B; b += gs) A.new_seq_len[b] = A.seq_len[b] + (status ? 0 : cu[b + 1] - cu[b]);
-    for (int64_t i = g0; i < A.max_tokens; i += gs) {
-        int64_t dst = -1, qr = -1;
-        int pos = -1, b = -1;
-        if (i < total) {
-            b = find_seq(cu, B, (int)i);
-            const int L = A.seq_len[b], held = (int)(((int64_t)L + P - 1) >> pshift);
-            pos = L + ((int)i - cu[b]);
-            const int idx = pos >> pshift;
-            const int page = idx < held ? A.block_table[(int64_t)(A.slots ? A.slots[b] : b) * A.table_width + idx]
-                                        : A.free_pages[nf - 1 - (np[b] + idx - held)];
-            dst = ((int64_t)page << pshift) + (pos & (P - 1));
-            qr = (int64_t)b * A.pad_tokens + ((int)i - cu[b]);
+    for (int64_t b = g0; b < B; b += gs) A.new_seq_len[b] = len[b] + (status ? 0 : cu[b + 1] - cu[b]);
+    const int64_t rows = (int64_t)B * T;
+    for (int64_t i = g0; i < rows; i += gs) {
+        const int b = (int)((uint32_t)i / (uint32_t)T), j = (int)i - b * T;
+        const bool live = !status && j < cu[b + 1] - cu[b];
+        const int pos = len[b] + j;
+        if (A.kv_len) A.kv_len[i] = live ? pos + 1 : 0;
+        if (!live) continue;
+        const int held = (int)(((int64_t)len[b] + P - 1) >> pshift), idx = pos >> pshift;
+        int32_t* const entry = A.block_table + (int64_t)row[b] * A.table_width + idx;
+        int page;
+        if (idx < held) {
+            page = *entry;
+        } else {
+            page = A.free_pages[nf - 1 - (np[b] + idx - held)];
+            if ((pos & (P - 1)) == 0) *entry = page;
         }
-        A.dst_rows[i] = dst;
-        if (A.positions) A.positions[i] = pos;
-        if (A.seq_of) A.seq_of[i] = b;
-        if (A.q_rows) A.q_rows[i] = qr;
+        const int t = cu[b] + j;
+        A.dst_rows[t] = ((int64_t)page << pshift) + (pos & (P - 1));
+        if (A.positions) A.positions[t] = pos;
+        if (A.seq_of) A.seq_of[t] = b;
+        if (A.q_rows) A.q_rows[t] = i;
     }
-    for (int64_t i = g0; i < news; i += gs) {
-        const int b = find_seq(np, B, (int)i);
-        const int held = (int)(((int64_t)A.seq_len[b] + P - 1) >> pshift);
-        A.block_table[(int64_t)(A.slots ? A.slots[b] : b) * A.table_width + held + ((int)i - np[b])] =
-            A.free_pages[nf - 1 - i];
-    }
-    if (A.kv_len) {
-        const int64_t n = (int64_t)B * A.pad_tokens;
-        for (int64_t i = g0; i < n; i += gs) {
-            const int b = (int)(i / A.pad_tokens), j = (int)(i - (int64_t)b * A.pad_tokens);
-            A.kv_len[i] = !status && j < cu[b + 1] - cu[b] ? A.seq_len[b] + j + 1 : 0;
-        }
+    for (int64_t t = total + g0; t < A.max_tokens; t += gs) {
+        A.dst_rows[t] = -1;
+        if (A.positions) A.positions[t] = -1;
+        if (A.seq_of) A.seq_of[t] = -1;
+        if (A.q_rows) A.q_rows[t] = -1;
     }
 }
 
@@ -246,13 +229,11 @@ struct Chunk {
     }
 };
 
-// V elements from src to dst, another type or the same
+// V elements to dst, of another type or the same
 template <int V, bool IN32, bool OUT32>
-__device__ __forceinline__ void copy_chunk(const void* src, int64_t s, void* dst, int64_t d) {
-    Chunk<V, IN32> a;
-    a.load(src, s);
+__device__ __forceinline__ void store_as(const Chunk<V, IN32>& a, void* dst, int64_t at) {
     if constexpr (IN32 == OUT32) {
-        a.store(dst, d);
+        a.store(dst, at);
     } else {
         Chunk<V, OUT32> o;
 #pragma unroll
@@ -261,98 +242,119 @@ __device__ __forceinline__ void copy_chunk(const void* src, int64_t s, void* dst
             if (i & 1) o.r[i >> 1] |= h << 16;
             else o.r[i >> 1] = h;
         }
-        o.store(dst, d);
+        o.store(dst, at);
     }
 }
 
 // V = 8: 16-byte accesses throughout (the host has checked strides and alignment); V = 1 (pairs of
-// halves) or 2 (adjacent pairs): any stride
+// halves) or 2 (adjacent pairs): any stride. A unit is V elements, of a pair's both halves where those
+// are apart: unit u of a token is in turn those of its q heads, k heads and v heads. gridDim.y cuts a
+// token's units where there are few tokens. The first unit of a thread is loaded ahead of the sines.
 template <int V, bool IN32, bool OUT32, bool ADJ>
 __global__ void __launch_bounds__(RT_THREADS) ea_rotary_kernel(ea_rotary A, int tpb) {
     extern __shared__ __align__(16) double2 cs[];  // tpb x pairs of (cos, sin) * scale
-    const int h = A.rot_dim / 2, tid = threadIdx.x;
+    const int h = A.rot_dim / 2, d = A.head_dim, tid = threadIdx.x;
     const int64_t t0 = (int64_t)blockIdx.x * tpb;
     const int nt = (int)min((int64_t)tpb, A.num_tokens - t0);
+    const int pu = ADJ ? A.rot_dim / V : h / V;  // units of a head that turn, and its other ones
+    const int uh = pu + (d - A.rot_dim) / V, uv = d / V;
+    const int uq = A.num_q_heads * uh, uk = A.num_kv_heads * uh, ua = uq + uk + (A.v ? A.num_kv_heads * uv : 0);
+    struct Unit {
+        bool live, turn;
+        int c, tk;
+        const void* src;
+        void* dst;
+        int64_t s, o;
+        Chunk<V, IN32> a, b;
+    };
+    auto fetch = [&](int u, Unit& x) __attribute__((always_inline)) {
+        x.tk = u / ua;
+        int r = u - x.tk * ua;
+        const int64_t t = t0 + x.tk;
+        const int64_t drow = r >= uq ? (A.dst_rows ? A.dst_rows[t] : t) : (A.q_rows ? A.q_rows[t] : t);
+        x.live = drow >= 0 && drow < (r >= uq ? A.pool_rows : A.q_out_rows);
+        x.turn = false;
+        if (r >= uq + uk) {
+            r -= uq + uk;
+            const int hd = r / uv;
+            x.src = A.v;
+            x.dst = A.v_out;
+            x.s = t * A.v_tok_stride + hd * A.v_head_stride + (r - hd * uv) * V;
+            x.o = drow * A.vo_tok_stride + hd * A.vo_head_stride + (r - hd * uv) * V;
+        } else {
+            const bool isk = r >= uq;
+            if (isk) r -= uq;
+            const int hd = r / uh, c = r - hd * uh;
+            x.turn = c < pu;
+            x.c = c * V;
+            const int e = x.turn ? c * V : A.rot_dim + (c - pu) * V;
+            x.src = isk ? A.k : A.q;
+            x.dst = isk ? A.k_out : A.q_out;
+            x.s = (isk ? t * A.k_tok_stride + hd * A.k_head_stride : t * A.q_tok_stride + hd * A.q_head_stride) + e;
+            x.o = (isk ? drow * A.ko_tok_stride + hd * A.ko_head_stride : drow * A.qo_tok_stride + hd * A.qo_head_stride) + e;
+        }
+        if (!x.live) return;
+        x.a.load(x.src, x.s);
+        if (!ADJ && x.turn) x.b.load(x.src, x.s + h);
+    };
+    auto finish = [&](Unit& x) __attribute__((always_inline)) {
+        if (!x.live) return;
+        if (!x.turn) {
+            store_as<V, IN32, OUT32>(x.a, x.dst, x.o);
+            return;
+        }
+        const double2* z = cs + x.tk * h;
+        Chunk<V, OUT32> y0, y1;
+        if constexpr (ADJ) {
+#pragma unroll
+            for (int i = 0; i < V; i += 2) {
+                const double2 q = z[(x.c + i) >> 1];
+                const double u0 = x.a.get(i), u1 = x.a.get(i + 1);
+                y0.put(i, __fma_rn(u0, q.x, -(u1 * q.y)));
+                y0.put(i + 1, __fma_rn(u1, q.x, u0 * q.y));
+            }
+            y0.store(x.dst, x.o);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const double2 q = z[x.c + i];
+                const double u0 = x.a.get(i), u1 = x.b.get(i);
+                y0.put(i, __fma_rn(u0, q.x, -(u1 * q.y)));
+                y1.put(i, __fma_rn(u1, q.x, u0 * q.y));
+            }
+            y0.store(x.dst, x.o);
+            y1.store(x.dst, x.o + h);
+        }
+    };
+    const int us = gridDim.y * RT_THREADS, u1 = nt * ua;
+    int u = blockIdx.y * RT_THREADS + tid;
+    Unit x;
+    if (u < u1) fetch(u, x);
     for (int i = tid; i < nt * h; i += RT_THREADS) {
         const int tk = i / h, p = i - tk * h;
         const int axis = A.axis_of_pair ? A.axis_of_pair[p] : 0;
         const double pos = (double)((int64_t)A.positions[axis * A.pos_axis_stride + t0 + tk] + A.pos_offset);
         const double w = A.half_turns[p];
         // pos w mod 2 half turns: the product's rounding error comes back by the FMA
-        const double x = pos * w, e = __fma_rn(pos, w, -x);
+        const double y = pos * w, e = __fma_rn(pos, w, -y);
         double sn, cn;
-        sincospi((x - 2.0 * rint(0.5 * x)) + e, &sn, &cn);
+        sincospi((y - 2.0 * rint(0.5 * y)) + e, &sn, &cn);
         cs[i] = make_double2(cn * (double)A.scale, (A.inverse ? -sn : sn) * (double)A.scale);
     }
     __syncthreads();
-    const int d = A.head_dim;
-    const int pu = ADJ ? A.rot_dim / V : h / V;  // units of a head that turn, and its other ones
-    const int uh = pu + (d - A.rot_dim) / V, uv = d / V;
-    const int uq = A.num_q_heads * uh, uk = A.num_kv_heads * uh, ua = uq + uk + (A.v ? A.num_kv_heads * uv : 0);
-    for (int u = tid; u < nt * ua; u += RT_THREADS) {
-        const int tk = u / ua;
-        int r = u - tk * ua;
-        const int64_t t = t0 + tk;
-        const int64_t drow = A.dst_rows ? A.dst_rows[t] : t;
-        if (r >= uq + uk) {  // v
-            r -= uq + uk;
-            const int hd = r / uv, c = (r - hd * uv) * V;
-            if (drow < 0 || drow >= A.pool_rows) continue;
-            copy_chunk<V, IN32, OUT32>(A.v, t * A.v_tok_stride + hd * A.v_head_stride + c, A.v_out,
-                                       drow * A.vo_tok_stride + hd * A.vo_head_stride + c);
-            continue;
-        }
-        const bool isk = r >= uq;
-        if (isk) r -= uq;
-        const int hd = r / uh, c = r - hd * uh;
-        const int64_t orow = isk ? drow : (A.q_rows ? A.q_rows[t] : t);
-        if (orow < 0 || orow >= (isk ? A.pool_rows : A.q_out_rows)) continue;
-        const void* src = isk ? A.k : A.q;
-        void* dst = isk ? A.k_out : A.q_out;
-        const int64_t s = isk ? t * A.k_tok_stride + hd * A.k_head_stride : t * A.q_tok_stride + hd * A.q_head_stride;
-        const int64_t o = isk ? orow * A.ko_tok_stride + hd * A.ko_head_stride : orow * A.qo_tok_stride + hd * A.qo_head_stride;
-        if (c >= pu) {  // past the rotated dims
-            const int e = A.rot_dim + (c - pu) * V;
-            copy_chunk<V, IN32, OUT32>(src, s + e, dst, o + e);
-            continue;
-        }
-        const double2* z = cs + tk * h;
-        Chunk<V, IN32> a;
-        Chunk<V, OUT32> x;
-        if constexpr (ADJ) {
-            a.load(src, s + c * V);
-#pragma unroll
-            for (int i = 0; i < V; i += 2) {
-                const double2 q = z[(c * V + i) >> 1];
-                const double u0 = a.get(i), u1 = a.get(i + 1);
-                x.put(i, __fma_rn(u0, q.x, -(u1 * q.y)));
-                x.put(i + 1, __fma_rn(u1, q.x, u0 * q.y));
-            }
-            x.store(dst, o + c * V);
-        } else {
-            Chunk<V, IN32> b;
-            Chunk<V, OUT32> y;
-            a.load(src, s + c * V);
-            b.load(src, s + h + c * V);
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const double2 q = z[c * V + i];
-                const double u0 = a.get(i), u1 = b.get(i);
-                x.put(i, __fma_rn(u0, q.x, -(u1 * q.y)));
-                y.put(i, __fma_rn(u1, q.x, u0 * q.y));
-            }
-            x.store(dst, o + c * V);
-            y.store(dst, o + h + c * V);
-        }
+    if (u < u1) finish(x);
+    for (u += us; u < u1; u += us) {
+        fetch(u, x);
+        finish(x);
     }
 }
 
 template <int V, bool ADJ>
-void rotary_launch(const ea_rotary& A, unsigned grid, size_t lds, int tpb, hipStream_t st) {
-    if (!A.in_fp32) hipLaunchKernelGGL((ea_rotary_kernel<V, false, false, ADJ>), dim3(grid), dim3(RT_THREADS), lds, st, A, tpb);
+void rotary_launch(const ea_rotary& A, dim3 grid, size_t lds, int tpb, hipStream_t st) {
+    if (!A.in_fp32) hipLaunchKernelGGL((ea_rotary_kernel<V, false, false, ADJ>), grid, dim3(RT_THREADS), lds, st, A, tpb);
     else if (A.out_fp32)
-        hipLaunchKernelGGL((ea_rotary_kernel<V, true, true, ADJ>), dim3(grid), dim3(RT_THREADS), lds, st, A, tpb);
-    else hipLaunchKernelGGL((ea_rotary_kernel<V, true, false, ADJ>), dim3(grid), dim3(RT_THREADS), lds, st, A, tpb);
+        hipLaunchKernelGGL((ea_rotary_kernel<V, true, true, ADJ>), grid, dim3(RT_THREADS), lds, st, A, tpb);
+    else hipLaunchKernelGGL((ea_rotary_kernel<V, true, false, ADJ>), grid, dim3(RT_THREADS), lds, st, A, tpb);
 }
 
 }  // namespace
@@ -368,14 +370,15 @@ int ea_hip_step_plan(const ea_step_plan* p, ea_stream_t stream) {
     if (p->num_seqs > 0 && (!p->seq_len || !p->counts || !p->new_seq_len || !p->block_table)) return -1;
     if (p->max_tokens > 0 && !p->dst_rows) return -1;
     if (p->free_capacity > 0 && !p->free_pages) return -1;
-    if ((p->q_rows || p->kv_len) && p->pad_tokens <= 0) return -1;
+    if (p->num_seqs > 0 && (p->pad_tokens == 0 || (int64_t)p->num_seqs * p->pad_tokens >= (int64_t)1 << 31)) return -1;
     // the blocks read these while others write those
     if ((p->num_seqs > 0 && p->new_seq_len == p->seq_len) || p->new_num_free == p->num_free) return -1;
     int ps = 0;
     while ((1 << ps) < p->page_size) ++ps;
-    const int64_t work = std::max<int64_t>({p->max_tokens, p->kv_len ? (int64_t)p->num_seqs * p->pad_tokens : 0, p->num_seqs, 1});
-    const unsigned grid = (unsigned)std::min<int64_t>((work + 4 * SP_THREADS - 1) / (4 * SP_THREADS), 256);
-    const size_t lds = ((size_t)2 * p->num_seqs + 2) * 4 + (size_t)(p->table_rows + 31) / 32 * 4;  // at most 74 KB
+    // two rows a thread, up to two blocks a CU
+    const int64_t work = std::max<int64_t>({(int64_t)p->max_tokens, (int64_t)p->num_seqs * p->pad_tokens, 1});
+    const unsigned grid = (unsigned)std::min<int64_t>((work + 2 * SP_THREADS - 1) / (2 * SP_THREADS), 512);
+    const size_t lds = ((size_t)4 * p->num_seqs + 1 + (p->table_rows + 31) / 32) * 4;  // at most 136 KB
     if (lds > 60 * 1024) {  // beside the static part
         const hipError_t e = hipFuncSetAttribute((const void*)ea_step_plan_kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
                                                  (int)lds);
@@ -417,16 +420,21 @@ int ea_hip_rotary(const ea_rotary* a, ea_stream_t stream) {
     }
     const bool wide = !(ptr & 15) && !(si & (in - 1)) && !(so & (out - 1)) && !(d & 7) && !((a->adjacent ? R : h) & 7);
     if (!wide && a->adjacent && (d & 1)) return -1;  // the narrow form of adjacent pairs takes two elements at a time
-    const int tpb = a->num_tokens >= 4096 ? 4 : 1;
-    const int64_t grid = ((int64_t)a->num_tokens + tpb - 1) / tpb;
+    // four tokens a block where there are many (fewer sines waited for), and a block for every 256 units of a
+    // token where they alone would leave CUs idle
+    const int tpb = a->num_tokens >= 4096 ? 4 : 1, v = wide ? 8 : (a->adjacent ? 2 : 1);
+    const int64_t units = (int64_t)(a->num_q_heads + a->num_kv_heads) * ((a->adjacent ? R : h) + d - R) / v +
+                          (a->v ? (int64_t)a->num_kv_heads * d / v : 0);
+    const int64_t slices = a->num_tokens < 256 ? std::min<int64_t>((units + RT_THREADS - 1) / RT_THREADS, 64) : 1;
+    const dim3 grid((unsigned)(((int64_t)a->num_tokens + tpb - 1) / tpb), (unsigned)slices);
     const size_t lds = (size_t)tpb * h * 16;
     const hipStream_t st = (hipStream_t)stream;
     if (a->adjacent) {
-        if (wide) rotary_launch<8, true>(*a, (unsigned)grid, lds, tpb, st);
-        else rotary_launch<2, true>(*a, (unsigned)grid, lds, tpb, st);
+        if (wide) rotary_launch<8, true>(*a, grid, lds, tpb, st);
+        else rotary_launch<2, true>(*a, grid, lds, tpb, st);
     } else {
-        if (wide) rotary_launch<8, false>(*a, (unsigned)grid, lds, tpb, st);
-        else rotary_launch<1, false>(*a, (unsigned)grid, lds, tpb, st);
+        if (wide) rotary_launch<8, false>(*a, grid, lds, tpb, st);
+        else rotary_launch<1, false>(*a, grid, lds, tpb, st);
     }
     return herr(hipGetLastError());
 }

@@ -14,7 +14,6 @@ counterpart: the reference's demo leaves its cache and positions to transformers
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 
@@ -27,22 +26,23 @@ PLAN_STATUS = {1: "out of pages", 2: "a sequence longer than its table row or ma
                8: "a negative length or count, or a table row outside the table or used twice"}
 
 
-def _on(dev):
-    """The device made current for a launch, when it is not already."""
+def _call(fn, args, index: int, what: str) -> None:
+    """One launch on torch's current stream of device `index`, made current when it is not."""
     import torch
-    if torch.cuda.current_device() == dev.index:
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
+    C = torch._C
+    if C._cuda_getDevice() == index:
+        rc = fn(ctypes.byref(args), C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(ctypes.byref(args), C._cuda_getCurrentRawStream(index))
+    if rc:
+        raise ValueError(f"{what}: error code {rc}")
 
 
-def _stream(dev):
-    import torch
-    return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
-
-
-def _vec(t, name, dev, dtype, n=None):
-    if t.dtype != dtype or t.device != dev or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor on {dev}")
+def _vec(t, name, index, dtype, n=None):
+    """The address of a contiguous tensor of this type on this device (of n entries)."""
+    if t.dtype is not dtype or not t.is_cuda or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor on cuda:{index}")
     if n is not None and t.numel() != n:
         raise ValueError(f"{name} must have {n} entries, got {t.numel()}")
     return t.data_ptr()
@@ -65,8 +65,8 @@ class StepPlan:
         import torch
         if num_seqs < 0 or max_tokens < 0 or pad_tokens <= 0:
             raise ValueError("num_seqs and max_tokens must not be negative, pad_tokens positive")
-        if num_seqs > 8192:
-            raise ValueError("at most 8192 sequences")
+        if num_seqs > 8192 or num_seqs * pad_tokens >= 1 << 31 or max_tokens >= 1 << 31:
+            raise ValueError("at most 8192 sequences, and fewer than 2^31 tokens and padded rows")
         dev = torch.empty(0, device=device).device
         if dev.type != "cuda":
             raise ValueError("the step plan runs on the GPU")
@@ -80,6 +80,12 @@ class StepPlan:
         self.seq_len = torch.empty(num_seqs, dtype=i32, device=dev)
         self.num_free = torch.empty(1, dtype=i32, device=dev)
         self.status = torch.empty(1, dtype=i32, device=dev)
+        self._lib, self._i32 = hip.load().ea_hip_step_plan, i32
+        self._fixed = bytes(hip.StepPlanArgs(
+            num_seqs=num_seqs, max_tokens=max_tokens, pad_tokens=pad_tokens, dst_rows=self.dst_rows.data_ptr(),
+            positions=self.positions.data_ptr(), seq_of=self.seq_of.data_ptr(), q_rows=self.q_rows.data_ptr(),
+            kv_len=self.kv_len.data_ptr(), new_seq_len=self.seq_len.data_ptr(), new_num_free=self.num_free.data_ptr(),
+            status=self.status.data_ptr()))
 
     def build(self, seq_len, counts, block_table, free_pages, num_free, page_size: int, *, slots=None,
               max_seq_len: int | None = None) -> None:
@@ -88,8 +94,6 @@ class StepPlan:
         one-entry int32 tensor). max_seq_len: bound of the lengths (None: what a table row holds). The
         outputs must not be passed in as the inputs of the same build: copy them (or use two plans in
         turn)."""
-        import torch
-        i32, dev = torch.int32, self.dev
         if block_table.dim() != 2:
             raise ValueError("block_table must be (rows, width)")
         rows, width = block_table.shape
@@ -97,19 +101,19 @@ class StepPlan:
             raise ValueError("page_size must be a power of two")
         if rows > 65536:
             raise ValueError("at most 65536 block table rows")
-        B = self.num_seqs
-        a = hip.StepPlanArgs(
-            num_seqs=B, page_size=page_size, table_rows=rows, table_width=width, max_tokens=self.max_tokens,
-            pad_tokens=self.pad_tokens, max_seq_len=(1 << 31) - 1 if max_seq_len is None else int(max_seq_len),
-            free_capacity=free_pages.numel(), seq_len=_vec(seq_len, "seq_len", dev, i32, B),
-            counts=_vec(counts, "counts", dev, i32, B), slots=None if slots is None else _vec(slots, "slots", dev, i32, B),
-            free_pages=_vec(free_pages, "free_pages", dev, i32), num_free=_vec(num_free, "num_free", dev, i32, 1),
-            block_table=_vec(block_table, "block_table", dev, i32), dst_rows=self.dst_rows.data_ptr(),
-            positions=self.positions.data_ptr(), seq_of=self.seq_of.data_ptr(), q_rows=self.q_rows.data_ptr(),
-            kv_len=self.kv_len.data_ptr(), new_seq_len=self.seq_len.data_ptr(), new_num_free=self.num_free.data_ptr(),
-            status=self.status.data_ptr())
-        with _on(dev):
-            hip._check(hip.load().ea_hip_step_plan(ctypes.byref(a), _stream(dev)), "ea_hip_step_plan")
+        B, i32, at = self.num_seqs, self._i32, self.dev.index
+        a = hip.StepPlanArgs.from_buffer_copy(self._fixed)
+        a.page_size, a.table_rows, a.table_width = page_size, rows, width
+        a.max_seq_len = 0x7FFFFFFF if max_seq_len is None else int(max_seq_len)
+        a.free_capacity = free_pages.numel()
+        a.seq_len = _vec(seq_len, "seq_len", at, i32, B)
+        a.counts = _vec(counts, "counts", at, i32, B)
+        if slots is not None:
+            a.slots = _vec(slots, "slots", at, i32, B)
+        a.free_pages = _vec(free_pages, "free_pages", at, i32)
+        a.num_free = _vec(num_free, "num_free", at, i32, 1)
+        a.block_table = _vec(block_table, "block_table", at, i32)
+        _call(self._lib, a, at, "ea_hip_step_plan")
 
     def check(self) -> None:
         """Waits for the plan and raises when the step did not fit."""
@@ -151,65 +155,74 @@ class Rotary:
         self.axes = len(sections) if sections is not None else int(ax.max()) + 1
         self.half_turns = torch.from_numpy(f / math.pi).to(self.dev)
         self.axis_of_pair = torch.from_numpy(ax.astype(np.uint8)).to(self.dev)
+        self._lib = hip.load().ea_hip_rotary
+        self._bits, self._f32 = (torch.bfloat16, torch.int16), torch.float32
+        self._fixed = bytes(hip.RotaryArgs(head_dim=head_dim, rot_dim=rot, num_axes=self.axes, adjacent=self.adjacent,
+                                           scale=self.scale, half_turns=self.half_turns.data_ptr(),
+                                           axis_of_pair=self.axis_of_pair.data_ptr()))
 
-    def _tokens(self, x, name, n=None):
-        """Checks a (tokens, heads, head_dim) input and returns it, int16 standing for bf16 bits."""
-        import torch
-        if x.dim() != 3 or x.shape[2] != self.head_dim or (n is not None and x.shape[0] != n):
+    def _tokens(self, x, name, n=None, dtypes=None):
+        """Checks a (tokens, heads, head_dim) tensor, int16 standing for bf16 bits: (tokens, heads, fp32, strides)."""
+        if x.dim() != 3:
+            raise ValueError(f"{name} must be (tokens, heads, {self.head_dim})")
+        m, h, d = x.shape
+        st = x.stride()
+        if d != self.head_dim or (n is not None and m != n):
             raise ValueError(f"{name} must be (tokens, heads, {self.head_dim}), one row per token")
-        if x.dtype not in (torch.bfloat16, torch.int16, torch.float32) or x.device != self.dev:
+        wide = x.dtype is self._f32
+        if not (wide or x.dtype in self._bits) or not x.is_cuda or x.get_device() != self.dev.index:
             raise ValueError(f"{name} must be bf16 (or int16 bit patterns) or fp32 on {self.dev}")
-        if x.numel() and x.stride(2) != 1:
+        if st[2] != 1 and m * h:
             raise ValueError(f"{name} needs a contiguous last dimension")
-        return x
+        return m, h, wide, st
 
-    def _args(self, q, k, v, positions, inverse, pos_offset):
+    def _args(self, q, k, v, positions):
+        """The arguments that the inputs give, checked; (arguments, fp32, tokens, Hq, Hkv)."""
         import torch
-        n = q.shape[0]
-        q, k = self._tokens(q, "q"), self._tokens(k, "k", n)
-        wide = q.dtype == torch.float32
-        if (k.dtype == torch.float32) != wide or (v is not None and (self._tokens(v, "v", n).dtype == torch.float32) != wide):
-            raise ValueError("q, k and v must have one type")
-        if v is not None and v.shape[1] != k.shape[1]:
-            raise ValueError("k and v must have the same heads")
-        if positions.dtype != torch.int32 or positions.device != self.dev:
-            raise ValueError(f"positions must be int32 on {self.dev}")
-        p = positions.unsqueeze(0) if positions.dim() == 1 else positions
-        if p.dim() != 2 or p.shape[1] != n or p.shape[0] < self.axes or (n > 1 and p.stride(1) != 1):
-            raise ValueError(f"positions must be ({self.axes}, {n}) or, for one axis, ({n},), each axis contiguous")
-        a = hip.RotaryArgs(
-            num_tokens=n, num_q_heads=q.shape[1], num_kv_heads=k.shape[1], head_dim=self.head_dim, rot_dim=self.rot_dim,
-            num_axes=self.axes, adjacent=self.adjacent, inverse=int(bool(inverse)), in_fp32=int(wide), pos_offset=int(pos_offset),
-            scale=self.scale, q_tok_stride=q.stride(0), q_head_stride=q.stride(1), k_tok_stride=k.stride(0),
-            k_head_stride=k.stride(1), pos_axis_stride=p.stride(0), q=q.data_ptr(), k=k.data_ptr(), positions=p.data_ptr(),
-            half_turns=self.half_turns.data_ptr(), axis_of_pair=self.axis_of_pair.data_ptr())
+        n, hq, wide, sq = self._tokens(q, "q")
+        _, hk, wk, sk = self._tokens(k, "k", n)
+        a = hip.RotaryArgs.from_buffer_copy(self._fixed)
         if v is not None:
-            a.v, a.v_tok_stride, a.v_head_stride = v.data_ptr(), v.stride(0), v.stride(1)
-        return a
-
-    def _launch(self, a) -> None:
-        with _on(self.dev):
-            hip._check(hip.load().ea_hip_rotary(ctypes.byref(a), _stream(self.dev)), "ea_hip_rotary")
+            _, hv, wv, sv = self._tokens(v, "v", n)
+            if hv != hk:
+                raise ValueError("k and v must have the same heads")
+            wk = wk if wv == wk else None
+            a.v, a.v_tok_stride, a.v_head_stride = v.data_ptr(), sv[0], sv[1]
+        if wk is not wide:
+            raise ValueError("q, k and v must have one type")
+        if positions.dtype is not torch.int32 or not positions.is_cuda or positions.get_device() != self.dev.index:
+            raise ValueError(f"positions must be int32 on {self.dev}")
+        shape, sp = tuple(positions.shape), positions.stride()
+        if shape != (n,) if len(shape) == 1 else (len(shape) != 2 or shape[1] != n or shape[0] < self.axes):
+            raise ValueError(f"positions must be ({self.axes}, {n}) or, for one axis, ({n},)")
+        if (len(shape) == 1 and self.axes > 1) or (n > 1 and sp[-1] != 1):
+            raise ValueError(f"positions must be ({self.axes}, {n}), each axis contiguous")
+        a.num_tokens, a.num_q_heads, a.num_kv_heads, a.in_fp32 = n, hq, hk, wide
+        a.q_tok_stride, a.q_head_stride, a.k_tok_stride, a.k_head_stride = sq[0], sq[1], sk[0], sk[1]
+        a.pos_axis_stride = sp[0] if len(shape) == 2 else 0
+        a.q, a.k, a.positions = q.data_ptr(), k.data_ptr(), positions.data_ptr()
+        return a, wide, n, hq, hk
 
     def rotate(self, q, k, positions, *, inverse: bool = False, q_out=None, k_out=None):
         """q (tokens, Hq, head_dim) and k (tokens, Hkv, head_dim) turned by positions ((tokens,) or (axes,
         tokens) int32), into new tensors of their type or into q_out and k_out (which may be q and k
         themselves). inverse turns back: the gradient of the rotation. Returns (q_out, k_out)."""
         import torch
-        a = self._args(q, k, None, positions, inverse, 0)
-        outs = []
-        for x, o, name in ((q, q_out, "q_out"), (k, k_out, "k_out")):
-            if o is None:
-                o = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            elif o.shape != x.shape or self._tokens(o, name).dtype != x.dtype:
-                raise ValueError(f"{name} must have the input's shape and type")
-            outs.append(o)
-        qo, ko = outs
-        a.out_fp32 = a.in_fp32
-        a.q_out, a.qo_tok_stride, a.qo_head_stride, a.q_out_rows = qo.data_ptr(), qo.stride(0), qo.stride(1), qo.shape[0]
-        a.k_out, a.ko_tok_stride, a.ko_head_stride, a.pool_rows = ko.data_ptr(), ko.stride(0), ko.stride(1), ko.shape[0]
-        self._launch(a)
-        return qo, ko
+        a, wide, n, hq, hk = self._args(q, k, None, positions)
+        if q_out is None:
+            q_out = torch.empty((n, hq, self.head_dim), dtype=q.dtype, device=self.dev)
+        elif q_out.shape != q.shape or q_out.dtype != q.dtype:
+            raise ValueError("q_out must have q's shape and type")
+        if k_out is None:
+            k_out = torch.empty((n, hk, self.head_dim), dtype=k.dtype, device=self.dev)
+        elif k_out.shape != k.shape or k_out.dtype != k.dtype:
+            raise ValueError("k_out must have k's shape and type")
+        so, ko = self._tokens(q_out, "q_out")[3], self._tokens(k_out, "k_out")[3]
+        a.inverse, a.out_fp32, a.q_out_rows, a.pool_rows = bool(inverse), wide, n, n
+        a.q_out, a.qo_tok_stride, a.qo_head_stride = q_out.data_ptr(), so[0], so[1]
+        a.k_out, a.ko_tok_stride, a.ko_head_stride = k_out.data_ptr(), ko[0], ko[1]
+        _call(self._lib, a, self.dev.index, "ea_hip_rotary")
+        return q_out, k_out
 
     def append(self, q, k, v, positions, dst_rows, k_pool, v_pool, *, q_rows=None, q_out=None, pos_offset: int = 0):
         """A step's tokens into the cache: q and k turned by positions (+ pos_offset), k and v (tokens, Hkv,
@@ -218,30 +231,34 @@ class Rotary:
         tensor of q's shape, or to rows q_rows (int64; rows outside are skipped) of q_out (rows, Hq,
         head_dim). Returns it. Rows that no token names are not written; a row may be named once."""
         import torch
-        a = self._args(q, k, v, positions, False, pos_offset)
-        n, i64 = a.num_tokens, torch.int64
+        a, _, n, hq, hk = self._args(q, k, v, positions)
+        at, d, i64 = self.dev.index, self.head_dim, torch.int64
+        shape = k_pool.shape
         for pool, name in ((k_pool, "k_pool"), (v_pool, "v_pool")):
-            if pool.dtype not in (torch.bfloat16, torch.int16) or pool.device != self.dev or not pool.is_contiguous():
+            if pool.dtype not in self._bits or not pool.is_cuda or pool.get_device() != at or not pool.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous bf16 (or int16) tensor on {self.dev}")
-            if pool.dim() != 4 or pool.shape[2:] != k.shape[1:] or pool.shape != k_pool.shape:
-                raise ValueError(f"{name} must be (pages, page_size, {k.shape[1]}, {self.head_dim})")
+            if pool.shape != shape:
+                raise ValueError("k_pool and v_pool must have one shape")
+        if len(shape) != 4 or shape[2] != hk or shape[3] != d:
+            raise ValueError(f"the pools must be (pages, page_size, {hk}, {d})")
         if q_out is None:
             if q_rows is not None:
                 raise ValueError("q_rows needs q_out")
-            q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=self.dev)
-        elif q_out.dtype not in (torch.bfloat16, torch.int16) or self._tokens(q_out, "q_out").shape[1] != q.shape[1]:
-            raise ValueError("q_out must be (rows, Hq, head_dim) bf16 (or int16)")
-        elif q_rows is None and q_out.shape[0] < n:
-            raise ValueError("q_out has fewer rows than there are tokens")
-        a.dst_rows = _vec(dst_rows, "dst_rows", self.dev, i64, n)
+            q_out = torch.empty((n, hq, d), dtype=torch.bfloat16, device=self.dev)
+            rows, so = n, (hq * d, d)
+        else:
+            rows, ho, wide, so = self._tokens(q_out, "q_out")
+            if wide or ho != hq or (q_rows is None and rows < n):
+                raise ValueError("q_out must be (rows, Hq, head_dim) bf16 (or int16), a row per token without q_rows")
+        a.dst_rows = _vec(dst_rows, "dst_rows", at, i64, n)
         if q_rows is not None:
-            a.q_rows = _vec(q_rows, "q_rows", self.dev, i64, n)
-        row = k.shape[1] * self.head_dim
-        a.q_out, a.qo_tok_stride, a.qo_head_stride, a.q_out_rows = q_out.data_ptr(), q_out.stride(0), q_out.stride(1), q_out.shape[0]
-        a.k_out, a.ko_tok_stride, a.ko_head_stride = k_pool.data_ptr(), row, self.head_dim
-        a.v_out, a.vo_tok_stride, a.vo_head_stride = v_pool.data_ptr(), row, self.head_dim
-        a.pool_rows = k_pool.shape[0] * k_pool.shape[1]
-        self._launch(a)
+            a.q_rows = _vec(q_rows, "q_rows", at, i64, n)
+        row = hk * d
+        a.pos_offset, a.q_out_rows, a.pool_rows = pos_offset, rows, shape[0] * shape[1]
+        a.q_out, a.qo_tok_stride, a.qo_head_stride = q_out.data_ptr(), so[0], so[1]
+        a.k_out, a.ko_tok_stride, a.ko_head_stride = k_pool.data_ptr(), row, d
+        a.v_out, a.vo_tok_stride, a.vo_head_stride = v_pool.data_ptr(), row, d
+        _call(self._lib, a, at, "ea_hip_rotary")
         return q_out
 
 
