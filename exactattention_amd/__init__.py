@@ -103,11 +103,12 @@ def attention_hip(q_bits, k_bits, v_bits, alpha=None, kv_len=None, row_ptr=None,
 
 
 def attention_geom(prob: dict, alpha=None, out: str = "bf16", splits: int = 0, merge_order=None,
-                   fallback: bool = True, device: str = "cuda", *, alpha_bits=None):
-    """Serving-geometry problem (exactattention_amd.problem) on the GPU -> (out (B,T,Hq,dv), flags, stats)."""
+                   fallback: bool = True, device: str = "cuda", *, alpha_bits=None, mods=None):
+    """Serving-geometry problem (exactattention_amd.problem) on the GPU -> (out (B,T,Hq,dv), flags, stats).
+    mods: score modifications (hip.ScoreMods): interval masks, a distance bias, capped scores."""
     from .hip import attention_problem
     ab = _alpha_bits(alpha, alpha_bits)
-    res, flags, st = attention_problem(prob, None, out, splits, merge_order, True, fallback, device, alpha_bits=ab)
+    res, flags, st = attention_problem(prob, None, out, splits, merge_order, True, fallback, device, alpha_bits=ab, mods=mods)
     return _finish(res, out), flags, st
 
 

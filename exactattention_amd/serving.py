@@ -194,34 +194,59 @@ class PagedKVCache:
     def _plan_general(self, seqs, counts, k_new, v_new):
         """_plan_append after its checks, for any counts (at least one key in all)."""
         sa = np.asarray(seqs, dtype=np.int64)
+        L, cnt, have, _ = self._grow(seqs, counts)
+        bt_pos, bt_val = [], []  # block-table entries of the new pages
+        for s, h in zip(seqs, have.tolist()):
+            for p in range(h, len(self.pages[s])):
+                bt_pos.append(s * self.max_pages + p)
+                bt_val.append(self.pages[s][p])
+        b_of = np.repeat(np.arange(len(seqs)), cnt)
+        pos = np.arange(int(cnt.sum())) - np.repeat(np.cumsum(cnt) - cnt - L, cnt)
+        idx = self.bt_host[sa[b_of], pos // self.P].astype(np.int64) * self.P + pos % self.P
+        arrays = [idx]
+        if bt_pos:
+            arrays += [np.asarray(bt_pos, dtype=np.int64), np.asarray(bt_val, dtype=np.int32)]
+        return {"k": k_new.contiguous(), "v": v_new.contiguous(), "grown": bool(bt_pos), "arrays": arrays}
+
+    def _grow(self, seqs, counts):
+        """The bookkeeping of an append of counts[i] keys to slot seqs[i]: pages taken, lengths, stale
+        tiles. Returns the lengths before, the counts, the pages each slot had (int64 arrays) and the new
+        pages in the order they were taken."""
         cnt = np.asarray(counts, dtype=np.int64)
-        L = np.asarray(self.length, dtype=np.int64)[sa]
+        L = np.asarray([self.length[s] for s in seqs], dtype=np.int64)
         if np.any(L + cnt > self.max_seq_len):
             raise ValueError("sequence longer than the cache's max_seq_len")
         have = np.asarray([len(self.pages[s]) for s in seqs], dtype=np.int64)
         need = np.maximum(0, (L + cnt + self.P - 1) // self.P - have)
         if int(need.sum()) > len(self.free):
             raise RuntimeError("out of pages")
-        bt_pos, bt_val = [], []  # block-table entries of the new pages
+        taken = []
         for i in np.flatnonzero(need):
             s = seqs[i]
-            self.pages[s].extend(self.free.pop() for _ in range(int(need[i])))
-            self.bt_host[s, :len(self.pages[s])] = self.pages[s]
-            for p in range(int(have[i]), len(self.pages[s])):
-                bt_pos.append(s * self.max_pages + p)
-                bt_val.append(self.pages[s][p])
-        b_of = np.repeat(np.arange(len(seqs)), cnt)
-        pos = np.arange(int(cnt.sum())) - np.repeat(np.cumsum(cnt) - cnt - L, cnt)
-        idx = self.bt_host[sa[b_of], pos // self.P].astype(np.int64) * self.P + pos % self.P
+            new = [self.free.pop() for _ in range(int(need[i]))]
+            self.pages[s].extend(new)
+            self.bt_host[s, int(have[i]):len(self.pages[s])] = new
+            taken += new
         stale, track = self.stale, self.digits is not None
         for s, a, e in zip(seqs, L.tolist(), (L + cnt).tolist()):
             self.length[s] = e
             if track:
                 stale[s] = a if stale[s] is None else min(stale[s], a)
-        arrays = [idx]
-        if bt_pos:
-            arrays += [np.asarray(bt_pos, dtype=np.int64), np.asarray(bt_val, dtype=np.int32)]
-        return {"k": k_new.contiguous(), "v": v_new.contiguous(), "grown": bool(bt_pos), "arrays": arrays}
+        return L, cnt, have, taken
+
+    def _step_plan(self, seqs, counts, *extra, stream=None):
+        """An append of counts[i] keys to slot seqs[i] (checked by the caller), planned on the device: the
+        pages are taken here, and one launch on torch's current stream writes their block-table entries and
+        the tokens' slots, positions, padded rows and visible lengths. Returns the StepPlan and device copies
+        of the arrays `extra`, uploaded with the plan's."""
+        L, cnt, _, taken = self._grow(seqs, counts)
+        # the plan takes pages off the top of a stack: the last entry first
+        up = self.stage.put(L.astype(np.int32), cnt.astype(np.int32), np.asarray(seqs, dtype=np.int32),
+                            np.asarray(taken[::-1], dtype=np.int32), np.asarray([len(taken)], dtype=np.int32), *extra,
+                            stream=stream)
+        plan = StepPlan(len(seqs), int(cnt.sum()), max(1, int(cnt.max())), device=self.dev)
+        plan.build(up[0], up[1], self.block_table, up[3], up[4], self.P, slots=up[2], max_seq_len=self.max_seq_len)
+        return plan, up[5:]
 
     def _plan_one_each(self, seqs, k_new, v_new):
         """_plan_append for one key per sequence (a decode step), in plain integer arithmetic: the
@@ -358,17 +383,40 @@ def _equal_runs(ql, heads=None, head_dim=128, longest=0):
 
 class ExactAttentionBackend:
     """Certified attention over a PagedKVCache. `alpha` is the base-2 logit scale as an fp32
-    value; `alpha_bits=` passes its bit pattern instead."""
+    value; `alpha_bits=` passes its bit pattern instead.
 
-    def __init__(self, cache: PagedKVCache, num_q_heads: int, alpha=None, out: str = "bf16", *, alpha_bits=None):
+    mods: score modifications of every call (hip.ScoreMods with a window, slopes or a softcap; its
+    per-token arrays are the calls' own). A token's distance counts from its own position, the end of
+    its prefix. rotary: rotary positions (Rotary): the calls then take q and k as the projections leave them,
+    turn both by the tokens' positions and write k to the cache on the way."""
+
+    def __init__(self, cache: PagedKVCache, num_q_heads: int, alpha=None, out: str = "bf16", *, alpha_bits=None,
+                 mods: "hip.ScoreMods | None" = None, rotary: Rotary | None = None):
         self.cache, self.Hq, self.out = cache, num_q_heads, out
         self.alpha_bits = alpha_fp32_bits(alpha, alpha_bits)
+        if mods is not None and (mods.kv_begin is not None or mods.q_pos is not None):
+            raise ValueError("kv_begin and q_pos are per token: the backend's calls set them")
+        if rotary is not None and rotary.head_dim != cache.d:
+            raise ValueError("the rotary positions are of another head size")
+        self.mods, self.rotary = mods, rotary
+        self._mods_keep = None
+        if mods is not None:
+            g = dict(num_seqs=0, num_tokens=0, num_q_heads=num_q_heads)
+            self._mods_args, self._mods_keep = mods.bind(g, cache.dev)
         self.ws = None
         self._last = None  # the latest launch: its ea_* arguments and the tensors they point at
         self._geoms = {}   # ea_geometry per (B, T): only max_seq_len changes between launches
 
+    def _step_mods(self, kv_begin=None):
+        """A call's ScoreModsArgs; kv_begin: its tokens' first keys (device int32), in place of the window."""
+        m = hip.ScoreModsArgs.from_buffer_copy(self._mods_args)
+        if kv_begin is not None:
+            m.kv_begin, m.window = kv_begin.data_ptr(), 0
+            m.max_span = self.mods.max_span or (self.mods.window + 64 if self.mods.window else 0)
+        return m
+
     def _launch(self, seqs, qd, kvl, tree_mask=None, tree_base=None, digits_slot=None, staged=None, stream=None,
-                dst=None):
+                dst=None, kv_begin=None):
         """Enqueue one ea_hip_attention call over sequences `seqs` on torch's current stream.
         qd: (B, T, Hq, d) int16 device tensor, row (b, t, h) = token t of sequence seqs[b];
         kvl: (B*T,) int32 device tensor of visible prefix lengths; staged: the device seq_len and
@@ -418,8 +466,13 @@ class ExactAttentionBackend:
             if reads.value:
                 c.flush(stream)  # the stale tiles, re-sliced ahead of the call in stream order
         nb, ns = ctypes.c_size_t(0), ctypes.c_int32(0)
-        hip._check(lib.ea_hip_workspace_size(ctypes.byref(gc), ctypes.byref(o), ctypes.byref(nb), ctypes.byref(ns)),
-                   "ea_hip_workspace_size")
+        m = None if self.mods is None else self._step_mods(kv_begin)
+        if m is None:
+            hip._check(lib.ea_hip_workspace_size(ctypes.byref(gc), ctypes.byref(o), ctypes.byref(nb), ctypes.byref(ns)),
+                       "ea_hip_workspace_size")
+        else:
+            hip._check(lib.ea_hip_mods_workspace_size(ctypes.byref(gc), ctypes.byref(o), ctypes.byref(m), ctypes.byref(nb),
+                                                      ctypes.byref(ns)), "ea_hip_mods_workspace_size")
         if self.ws is None or self.ws.numel() < int(nb.value):
             self.ws = torch.empty(max(int(nb.value), 1 << 20), dtype=torch.uint8, device=c.dev)
         ws = self.ws
@@ -428,27 +481,81 @@ class ExactAttentionBackend:
                         tree_mask=None if tm is None else tm.data_ptr(), tree_base=None if tb is None else tb.data_ptr(),
                         out=out.data_ptr(), flags=flags.data_ptr())
         st = stream if stream is not None else hip._stream_ptr(torch)
-        hip._check(lib.ea_hip_attention(ctypes.byref(gc), ctypes.byref(b), ctypes.byref(o), ws.data_ptr(), int(nb.value),
-                                        st), "ea_hip_attention")
-        self._last = {"args": (gc, b, o), "before": [], "keep": (qd, kvl, seq, off, tm, tb, staged), "out": out, "flags": flags,
-                      "ret": None}
+        if m is None:
+            hip._check(lib.ea_hip_attention(ctypes.byref(gc), ctypes.byref(b), ctypes.byref(o), ws.data_ptr(), int(nb.value),
+                                            st), "ea_hip_attention")
+        else:
+            hip._check(lib.ea_hip_attention_mods(ctypes.byref(gc), ctypes.byref(b), ctypes.byref(o), ctypes.byref(m),
+                                                 ws.data_ptr(), int(nb.value), st), "ea_hip_attention_mods")
+        self._last = {"args": (gc, b, o), "mods": m, "before": [], "keep": (qd, kvl, seq, off, tm, tb, staged, kv_begin), "out": out,
+                      "flags": flags, "ret": None}
         return out, flags
 
     def _exact_tier(self) -> None:
         """The host exact tier on the latest call's launches (ea_hip_exact_rows): waits for torch's current
         stream and recomputes every row left at flag 1 in place (flag 0, or 2 on a domain error)."""
         c = self.cache
+        m = self._last["mods"]
         for gc, b, o in self._last["before"] + [self._last["args"]]:
-            hip._check(hip.load().ea_hip_exact_rows(ctypes.byref(gc), ctypes.byref(b), ctypes.byref(o),
-                                                    hip._stream_ptr(c.torch)), "ea_hip_exact_rows")
+            hip._check(hip.load().ea_hip_exact_rows_mods(ctypes.byref(gc), ctypes.byref(b), ctypes.byref(o),
+                                                         None if m is None else ctypes.byref(m), hip._stream_ptr(c.torch)),
+                       "ea_hip_exact_rows")
 
-    def _run(self, seqs, q, kv_len, tree_mask=None, tree_base=None, digits_slot=None):
+    def _append(self, seqs, counts, q, k, v, positions=None):
+        """The new keys into the cache, counts[i] of slot seqs[i], and the q to attend with: as it is, or with
+        rotary positions turned by `positions` (int32, host or device; None: the tokens' own), as k then is on
+        its way (q None: k alone)."""
+        c = self.cache
+        if self.rotary is None:
+            c.append_batch(seqs, counts, k, v)
+            return q
+        torch = c.torch
+        kd, vd = _dev16(torch, k, c.dev), _dev16(torch, v, c.dev)
+        n = sum(int(x) for x in counts)
+        if len(counts) != len(seqs) or kd.shape[0] != n or vd.shape[0] != n:
+            raise ValueError("one count per sequence slot, and as many keys as they add up to")
+        c._check_slots(seqs)
+        qd = kd[:, :0] if q is None else _dev16(torch, q, c.dev)
+        if n == 0:
+            return qd
+        pos = self._positions(positions, n)
+        self._check_turn(qd, kd, vd, pos)
+        plan, _ = c._step_plan(seqs, counts)
+        return self.rotary.append(qd, kd, vd, plan.positions if pos is None else pos, plan.dst_rows, c.k, c.v)
+
+    def _check_turn(self, q, k, v, pos) -> None:
+        """What Rotary.append would refuse, before the cache's bookkeeping changes."""
+        c, r = self.cache, self.rotary
+        n, hq = r._tokens(q, "query")[:2]
+        if (q.shape[1] and hq != self.Hq) or tuple(k.shape) != (n, c.Hkv, c.d) or tuple(v.shape) != (n, c.Hkv, c.d):
+            raise ValueError(f"query must be (tokens, {self.Hq}, {c.d}), key and value (tokens, {c.Hkv}, {c.d})")
+        if pos is None:
+            pos = c.torch.empty(n, dtype=c.torch.int32, device=c.dev)
+        r._args(q, k, v, pos)
+
+    def _positions(self, positions, n):
+        """A call's positions as an int32 device tensor, None for the tokens' own (one axis)."""
+        r = self.rotary
+        if positions is None:
+            if r is not None and r.axes > 1:
+                raise ValueError(f"positions of {r.axes} axes are needed")
+            return None
+        if r is None:
+            raise ValueError("positions need rotary=")
+        if not hasattr(positions, "data_ptr"):
+            positions = self.cache.torch.from_numpy(np.ascontiguousarray(positions, dtype=np.int32))
+        p = positions.to(self.cache.dev)
+        if p.shape[-1] != n:
+            raise ValueError("one position per token and axis")
+        return p
+
+    def _run(self, seqs, q, kv_len, tree_mask=None, tree_base=None, digits_slot=None, kv_begin=None):
         """_launch, then the result on the host: (out bits (B, T, Hq, d), flags); flag 2 raises."""
         c = self.cache
         torch = c.torch
         qd = _dev16(torch, q, c.dev).contiguous()
-        (kvl,) = c.stage.put(np.asarray(kv_len, dtype=np.int32).reshape(-1))
-        out, flags = self._launch(seqs, qd, kvl, tree_mask, tree_base, digits_slot)
+        up = c.stage.put(*(np.asarray(x, dtype=np.int32).reshape(-1) for x in (kv_len, kv_begin) if x is not None))
+        out, flags = self._launch(seqs, qd, up[0], tree_mask, tree_base, digits_slot, kv_begin=up[1] if len(up) > 1 else None)
         torch.cuda.current_stream().synchronize()  # the launch stream only, not the whole device
         fl = flags.cpu().numpy()
         if np.any(fl == 1):
@@ -460,7 +567,7 @@ class ExactAttentionBackend:
             raise ExactAttentionDomainError("non-finite input or fp32 logit overflow")
         return res, fl
 
-    def forward(self, query, key, value, seqs, query_lens):
+    def forward(self, query, key, value, seqs, query_lens, positions=None):
         """One attention call per layer over a mixed batch, the way vLLM's attention backends are
         called: `query_lens[i]` new tokens of sequence slot `seqs[i]`, flattened in that order
         (query (num_tokens, Hq, d), key/value (num_tokens, Hkv, d), bf16 or int16 device tensors).
@@ -469,7 +576,11 @@ class ExactAttentionBackend:
         current stream, no host synchronisation: returns device (out (num_tokens, Hq, d) bf16/fp32
         bits, flags (num_tokens, Hq) uint8; 0 certified, 1 not certified by the device tiers (the
         row holds +0), 2 domain error). Call check_flags(flags) before the next forward: it
-        finishes flag-1 rows with the host exact tier, in place, and raises on flag 2."""
+        finishes flag-1 rows with the host exact tier, in place, and raises on flag 2.
+
+        With rotary positions, query and key (then bf16, int16 or fp32, any strides over tokens and heads)
+        are turned by `positions` ((num_tokens,) or (axes, num_tokens) int32 device tensor), by default each
+        token's place in its sequence."""
         c = self.cache
         torch = c.torch
         ql = [int(n) for n in query_lens]
@@ -485,24 +596,23 @@ class ExactAttentionBackend:
             return (torch.empty((0, Hq, d), dtype=torch.int32 if self.out == "fp32" else torch.int16, device=c.dev),
                     torch.empty((0, Hq), dtype=torch.uint8, device=c.dev))
         B, T, Hq, d = len(ql), max(ql), query.shape[1], query.shape[2]
+        if self.rotary is not None or positions is not None:
+            return self._forward_planned(query, key, value, list(seqs), ql, self._positions(positions, ntok))
         prefix = [c.length[s] for s in seqs]
-        plan = c._plan_append(seqs, ql, key, value, checked=True)
-        lens = np.asarray([c.length[s] for s in seqs], dtype=np.int32)
-        mine = [lens, np.asarray(seqs, dtype=np.int64) * c.max_pages, np.asarray(seqs, dtype=np.int32)]
         runs = None
         if T > 1:
             if query.dim() == 3 and query.element_size() == 2 and query.device == c.k.device:
                 runs = _equal_runs(ql, Hq, d, max(prefix))
+            if runs is None:
+                return self._forward_planned(query, key, value, list(seqs), ql, None)
+        plan = c._plan_append(seqs, ql, key, value, checked=True)
+        lens = np.asarray([c.length[s] for s in seqs], dtype=np.int32)
+        mine = [lens, np.asarray(seqs, dtype=np.int64) * c.max_pages, np.asarray(seqs, dtype=np.int32)]
+        if T > 1:
             start = np.concatenate([[0], np.cumsum(ql)])
             b_of = np.repeat(np.arange(B), ql)
             j_of = np.arange(ntok) - start[b_of]
-            seen = np.asarray(prefix, dtype=np.int32)[b_of] + j_of + 1
-            if runs is not None:
-                mine.append(seen.astype(np.int32))
-            else:
-                kvl_h = np.zeros(B * T, dtype=np.int32)
-                kvl_h[b_of * T + j_of] = seen
-                mine += [kvl_h, (b_of * T + j_of).astype(np.int64)]
+            mine.append((np.asarray(prefix, dtype=np.int32)[b_of] + j_of + 1).astype(np.int32))
         n_app = len(plan["arrays"])
         ts = torch.cuda.current_stream(c.dev)
         st = ctypes.c_void_p(ts.cuda_stream)
@@ -512,23 +622,48 @@ class ExactAttentionBackend:
         if runs is not None:
             return self._forward_runs(query, list(seqs), ql, runs, staged, dev[n_app + 3], st)
         # one token per sequence sees the whole sequence: its visible length is the sequence's
-        kvl = dev[n_app + 3] if T > 1 else dev[n_app]
-        row = dev[n_app + 4] if T > 1 else None
         q16 = query.view(torch.int16) if query.dtype != torch.int16 else query
-        if T == 1:
-            qd = q16.reshape(B, 1, Hq, d).contiguous()
-        else:
-            qd = torch.zeros((B * T, Hq, d), dtype=torch.int16, device=c.dev)
-            qd.index_copy_(0, row, q16)
-            qd = qd.view(B, T, Hq, d)
+        qd = q16.reshape(B, 1, Hq, d).contiguous()
         slots = list(seqs)
-        out, flags = self._launch(slots, qd, kvl, digits_slot=slots[0], staged=staged, stream=st)
-        self._last["keep"] += (q16, row)
-        if T == 1:
-            ret = (out.view(B, Hq, -1), flags.view(B, Hq))
+        out, flags = self._launch(slots, qd, dev[n_app], digits_slot=slots[0], staged=staged, stream=st)
+        self._last["keep"] += (q16,)
+        ret = (out.view(B, Hq, -1), flags.view(B, Hq))
+        self._last["ret"] = (ret, None, 1)
+        return ret
+
+    def _forward_planned(self, query, key, value, seqs, ql, pos):
+        """forward() on rows padded to the longest chunk, the step planned on the device: the new tokens'
+        slots, rows and visible lengths come from one launch (PagedKVCache._step_plan), and with rotary
+        positions a second one turns q and k and writes q to its padded rows, k and v to the cache."""
+        c, r = self.cache, self.rotary
+        torch = c.torch
+        B, T, Hq, d = len(ql), max(ql), query.shape[1], query.shape[2]
+        if r is None:
+            k16, v16 = _dev16(torch, key, c.dev).contiguous(), _dev16(torch, value, c.dev).contiguous()
+            q16 = query.view(torch.int16) if query.dtype != torch.int16 else query
         else:
+            self._check_turn(query, key, value, pos)
+        ts = torch.cuda.current_stream(c.dev)
+        st = ctypes.c_void_p(ts.cuda_stream)
+        plan, (off, slot) = c._step_plan(seqs, ql, np.asarray(seqs, dtype=np.int64) * c.max_pages,
+                                         np.asarray(seqs, dtype=np.int32), stream=ts)
+        staged = (plan.seq_len, off, slot)
+        ragged = B * T != sum(ql)
+        qd = (torch.zeros if ragged else torch.empty)((B * T, Hq, d), dtype=torch.int16, device=c.dev)
+        if r is None:
+            c._kv_append(k16, v16, plan.dst_rows, sum(ql), None, None, 0, st)
+            qd.index_copy_(0, plan.q_rows, q16)
+        else:
+            r.append(query, key, value, plan.positions if pos is None else pos, plan.dst_rows, c.k, c.v, q_rows=plan.q_rows, q_out=qd)
+        out, flags = self._launch(seqs, qd.view(B, T, Hq, d), plan.kv_len.view(-1), digits_slot=seqs[0], staged=staged, stream=st)
+        self._last["keep"] += (plan,)
+        if ragged:
+            row = plan.q_rows
             ret = (out.view(B * T, Hq, -1).index_select(0, row), flags.view(B * T, Hq).index_select(0, row))
-        self._last["ret"] = (ret, row, T)
+            self._last["ret"] = (ret, row, T)
+        else:
+            ret = (out.view(B * T, Hq, -1), flags.view(B * T, Hq))
+            self._last["ret"] = (ret, None, 1)
         return ret
 
     def _forward_runs(self, query, seqs, ql, runs, staged, kvl, st):
@@ -575,55 +710,86 @@ class ExactAttentionBackend:
         if bool((flags == 2).any().item()):
             raise ExactAttentionDomainError("non-finite input or fp32 logit overflow")
 
-    def prefill(self, s: int, q, k, v):
+    def prefill(self, s: int, q, k, v, positions=None):
         """Append T tokens' K/V to slot s and attend causally: token t sees the prefix and tokens
         0..t of the chunk. q (T, Hq, d), k/v (T, Hkv, d) bf16 bits. Returns (out (T, Hq, d), flags)."""
         c = self.cache
         L = c.length[s]
         T = q.shape[0]
-        c.append(s, k, v)
+        self._positions(positions, T)
+        qr = self._append([s], [len(k)], q, k, v, positions)
         kv_len = (L + 1 + np.arange(T)).reshape(1, T)
-        res, fl = self._run([s], np.asarray(q)[None], kv_len, digits_slot=s)
+        res, fl = self._run([s], _batch(qr, 0), kv_len, digits_slot=s)
         return res[0], fl
 
-    def decode(self, seqs, q, k, v):
+    def decode(self, seqs, q, k, v, positions=None):
         """One new token per sequence: q (B, Hq, d), k/v (B, Hkv, d). Returns (out (B, Hq, d), flags)."""
         c = self.cache
-        for i, s in enumerate(seqs):
-            c.append(s, np.asarray(k)[i:i + 1] if not hasattr(k, "data_ptr") else k[i:i + 1],
-                     np.asarray(v)[i:i + 1] if not hasattr(v, "data_ptr") else v[i:i + 1])
+        self._positions(positions, len(seqs))
+        if self.rotary is None:
+            for i, s in enumerate(seqs):
+                c.append(s, np.asarray(k)[i:i + 1] if not hasattr(k, "data_ptr") else k[i:i + 1],
+                         np.asarray(v)[i:i + 1] if not hasattr(v, "data_ptr") else v[i:i + 1])
+        else:
+            q = self._append(seqs, [1] * len(seqs), q, k, v, positions)
         kv_len = np.array([[c.length[s]] for s in seqs])
-        res, fl = self._run(list(seqs), np.asarray(q)[:, None], kv_len)
+        res, fl = self._run(list(seqs), _batch(q, 1), kv_len)
         return res[:, 0], fl
 
     def verify_tree(self, s: int, q, k, v, parents):
         """Speculative verification: N <= 64 draft nodes, parents[i] < i (-1: the prefix), appended
         after the prefix; node i attends the prefix and its root-to-node path. q (N, Hq, d), k/v
-        (N, Hkv, d). Returns (out (N, Hq, d), flags); keep the accepted path with accept()."""
+        (N, Hkv, d). Returns (out (N, Hq, d), flags); keep the accepted path with accept().
+        A node's position is the prefix's length plus its depth (rotary positions; a window counts the
+        prefix's last keys and the path's). Slopes are refused: distances are between cache slots, which
+        are not the nodes' positions."""
         c = self.cache
         N = q.shape[0]
         if N > 64:
             raise ValueError("at most 64 draft nodes")
+        if self.mods is not None and self.mods.slopes is not None:
+            raise ValueError("tree verification has no distance bias")
         L = c.length[s]
-        c.append(s, k, v)
+        depth = np.zeros(N, dtype=np.int64)
+        for i in range(N):
+            depth[i] = depth[parents[i]] + 1 if parents[i] >= 0 else 0
+        if self.rotary is not None and self.rotary.axes > 1:
+            raise ValueError("tree verification has one position axis")
+        window = self.mods.window if self.mods is not None else 0
         mask = np.zeros((1, N), dtype=np.uint64)
         for i in range(N):
             j, m = i, 0
-            while j >= 0:
+            while j >= 0 and not (window and depth[i] - depth[j] >= window):
                 m |= 1 << j
                 j = parents[j]
             mask[0, i] = m
-        res, fl = self._run([s], np.asarray(q)[None], np.full((1, N), L), tree_mask=mask, tree_base=[L],
-                            digits_slot=s)
+        qr = self._append([s], [len(k)], q, k, v, None if self.rotary is None else L + depth)
+        begin = np.clip(L + depth + 1 - window, 0, L).reshape(1, N) if window else None
+        res, fl = self._run([s], _batch(qr, 0), np.full((1, N), L), tree_mask=mask, tree_base=[L], digits_slot=s,
+                            kv_begin=begin)
         return res[0], fl
 
     def accept(self, s: int, prefix_len: int, path, k, v) -> None:
         """Keep the accepted draft nodes `path` (node indices in draft order) after the prefix:
-        the cache is cut back to the prefix and the path's K/V appended in order."""
+        the cache is cut back to the prefix and the path's K/V appended in order (with rotary positions k as
+        verify_tree took it: it is turned again)."""
         self.cache.truncate(s, prefix_len)
         if len(path):
             idx = np.asarray(path)
-            self.cache.append(s, np.asarray(k)[idx], np.asarray(v)[idx])
+            if self.rotary is None:
+                self.cache.append(s, np.asarray(k)[idx], np.asarray(v)[idx])
+            else:
+                torch = self.cache.torch
+                at = torch.from_numpy(idx.astype(np.int64)).to(self.cache.dev)
+                kk, vv = (_dev16(torch, x, self.cache.dev).index_select(0, at) for x in (k, v))
+                self._append([s], [len(idx)], None, kk, vv)
+
+
+def _batch(q, axis: int):
+    """q with a batch axis put in front (0) or a token axis after the first (1)."""
+    if hasattr(q, "data_ptr"):
+        return q.unsqueeze(axis)
+    return np.expand_dims(np.asarray(q), axis)
 
 
 class DecodeGraph:
@@ -636,6 +802,8 @@ class DecodeGraph:
 
     The caller writes the step's inputs into the static tensors `q` (B, 1, Hq, d), `k` and `v`
     (B, Hkv, d) (int16 views of bf16) before calling step(); the outputs land in `out` and `flags`.
+    The backend's score modifications and rotary positions are part of the graph: q and k are then given
+    unturned, and with several position axes the caller also writes `positions` (axes, B), int32.
     `max_len` bounds every sequence's length while the graph lives: it sizes the split grid (the
     kernel skips the splits past a sequence's end), so a tight bound keeps the grid dense."""
 
@@ -696,11 +864,17 @@ class DecodeGraph:
         self.gc = hip.geometry(g)
         self.o = hip.Options(alpha_bits=backend.alpha_bits, out_fp32=int(fp32), splits=0, tier2=1)
         nb, ns = ctypes.c_size_t(0), ctypes.c_int32(0)
-        hip._check(lib.ea_hip_workspace_size(ctypes.byref(self.gc), ctypes.byref(self.o), ctypes.byref(nb),
-                                             ctypes.byref(ns)), "ea_hip_workspace_size")
+        self.m = None if backend.mods is None else backend._step_mods()
+        hip._check(lib.ea_hip_mods_workspace_size(ctypes.byref(self.gc), ctypes.byref(self.o),
+                                                  None if self.m is None else ctypes.byref(self.m), ctypes.byref(nb),
+                                                  ctypes.byref(ns)), "ea_hip_workspace_size")
         self.ws_bytes = int(nb.value)
         self.ws = torch.empty(max(self.ws_bytes, 256), dtype=torch.uint8, device=dev)
-        self.bufs = hip.Buffers(q=self.q.data_ptr(), k=c.k.data_ptr(), v=c.v.data_ptr(),
+        rot = backend.rotary
+        # with rotary positions the attention reads the turned q; one axis counts from the visible lengths
+        self._qr = torch.empty((B, Hq, d), dtype=torch.int16, device=dev) if rot is not None else self.q
+        self.positions = torch.zeros((rot.axes, B), dtype=torch.int32, device=dev) if rot is not None and rot.axes > 1 else None
+        self.bufs = hip.Buffers(q=self._qr.data_ptr(), k=c.k.data_ptr(), v=c.v.data_ptr(),
                                 seq_len=self.dv["kvl"].data_ptr(), kv_len=self.dv["kvl"].data_ptr(),
                                 block_table=c.block_table.data_ptr(), block_table_offset=self.dv["bt_off"].data_ptr(),
                                 tree_mask=None, tree_base=None, out=self.out.data_ptr(),
@@ -717,9 +891,14 @@ class DecodeGraph:
     def _enqueue(self, stream) -> None:
         c, lib, d = self.c, hip.load(), self.dv
         st = ctypes.c_void_p(stream.cuda_stream)
-        c._kv_append(self.k, self.v, d["idx"], self.B, d["bt_pos"], d["bt_val"], self.B, st)
-        hip._check(lib.ea_hip_attention(ctypes.byref(self.gc), ctypes.byref(self.bufs), ctypes.byref(self.o),
-                                        self.ws.data_ptr(), self.ws_bytes, st), "ea_hip_attention")
+        rot = self.be.rotary
+        c._kv_append(self.k, self.v, d["idx"], self.B if rot is None else 0, d["bt_pos"], d["bt_val"], self.B, st)
+        if rot is not None:
+            pos, off = (d["kvl"], -1) if self.positions is None else (self.positions, 0)
+            rot.append(self.q[:, 0], self.k, self.v, pos, d["idx"], c.k, c.v, q_out=self._qr, pos_offset=off)
+        m = None if self.m is None else ctypes.byref(self.m)
+        hip._check(lib.ea_hip_attention_mods(ctypes.byref(self.gc), ctypes.byref(self.bufs), ctypes.byref(self.o), m,
+                                             self.ws.data_ptr(), self.ws_bytes, st), "ea_hip_attention")
 
     def _plan(self) -> int:
         """Host half of a step: one key per slot appended (pages allocated as needed) into the
@@ -772,8 +951,9 @@ class DecodeGraph:
         """After the latest step: flag-1 rows finished by the host exact tier, flag 2 raises."""
         st = ctypes.c_void_p(self.torch.cuda.current_stream(self.c.dev).cuda_stream)
         if bool((self.flags == 1).any().item()):
-            hip._check(hip.load().ea_hip_exact_rows(ctypes.byref(self.gc), ctypes.byref(self.bufs),
-                                                    ctypes.byref(self.o), st), "ea_hip_exact_rows")
+            hip._check(hip.load().ea_hip_exact_rows_mods(ctypes.byref(self.gc), ctypes.byref(self.bufs), ctypes.byref(self.o),
+                                                         None if self.m is None else ctypes.byref(self.m), st),
+                       "ea_hip_exact_rows")
         if bool((self.flags == 2).any().item()):
             raise ExactAttentionDomainError("non-finite input or fp32 logit overflow")
 
@@ -795,7 +975,8 @@ def hf_attention(module, query, key, value, attention_mask=None, scaling=None, d
     query (B, H, ql, D), key/value (B, Hkv, kl, D) bf16 CUDA tensors holding the whole cache,
     causal with the queries at the end of the key range (query t attends keys 0 .. kl-ql+t);
     `attention_mask` is not read, as in the reference (batches without padding). alpha =
-    RN_fp32(scaling / ln 2), scaling defaulting to `module.scaling`. One ea_hip_attention launch
+    RN_fp32(scaling / ln 2), scaling defaulting to `module.scaling`; `softcap`, which transformers passes
+    for models that cap their scores, caps them (c = RN_fp32(softcap / ln 2)). One ea_hip_attention launch
     straight on the tensors' strides (no copies); returns (out (B, ql, H, D) bf16, None). Rows the
     device tiers leave uncertified are finished by the host exact tier (ea_hip_exact_rows); raises
     on non-finite input or fp32 logit overflow, like the reference's kernels (this waits for the
@@ -805,6 +986,8 @@ def hf_attention(module, query, key, value, attention_mask=None, scaling=None, d
         raise ValueError("dropout is not part of ExactAttention")
     if kwargs.get("sliding_window"):
         raise ValueError("sliding-window attention is not supported")
+    cap = kwargs.get("softcap")
+    m = ctypes.byref(hip.ScoreModsArgs(softcap_bits=alpha_bits_for(float(cap)))) if cap else None
     B, H, ql, D = query.shape
     Hkv, kl = key.shape[1], key.shape[2]
     if key.shape != value.shape[:3] + (D,) or key.shape[0] != B or key.shape[3] != D:
@@ -831,7 +1014,7 @@ def hf_attention(module, query, key, value, attention_mask=None, scaling=None, d
     o = hip.Options(alpha_bits=ab, out_fp32=0, splits=0, tier2=1)
     lib = hip.load()
     nb, ns = ctypes.c_size_t(0), ctypes.c_int32(0)
-    hip._check(lib.ea_hip_workspace_size(ctypes.byref(g), ctypes.byref(o), ctypes.byref(nb), ctypes.byref(ns)),
+    hip._check(lib.ea_hip_mods_workspace_size(ctypes.byref(g), ctypes.byref(o), m, ctypes.byref(nb), ctypes.byref(ns)),
                "ea_hip_workspace_size")
     ws = _HF_WS.get(dev)
     if ws is None or ws.numel() < int(nb.value):
@@ -839,13 +1022,13 @@ def hf_attention(module, query, key, value, attention_mask=None, scaling=None, d
     b = hip.Buffers(q=query.data_ptr(), k=key.data_ptr(), v=value.data_ptr(), seq_len=lens.data_ptr(),
                     kv_len=kvl.data_ptr(), block_table=None, block_table_offset=None, tree_mask=None, tree_base=None,
                     out=out.data_ptr(), flags=flags.data_ptr())
-    hip._check(lib.ea_hip_attention(ctypes.byref(g), ctypes.byref(b), ctypes.byref(o), ws.data_ptr(), int(nb.value),
-                                    hip._stream_ptr(torch)), "ea_hip_attention")
+    hip._check(lib.ea_hip_attention_mods(ctypes.byref(g), ctypes.byref(b), ctypes.byref(o), m, ws.data_ptr(), int(nb.value),
+                                         hip._stream_ptr(torch)), "ea_hip_attention")
     if not bool(flags.any().item()):  # the usual case: one wait for the launch
         return out, None
     if bool((flags == 1).any().item()):
         # rows the device tiers left uncertified: the host exact tier, in place
-        hip._check(lib.ea_hip_exact_rows(ctypes.byref(g), ctypes.byref(b), ctypes.byref(o), hip._stream_ptr(torch)),
+        hip._check(lib.ea_hip_exact_rows_mods(ctypes.byref(g), ctypes.byref(b), ctypes.byref(o), m, hip._stream_ptr(torch)),
                    "ea_hip_exact_rows")
     if bool((flags == 2).any().item()):
         raise ExactAttentionDomainError("non-finite input or fp32 logit overflow")
