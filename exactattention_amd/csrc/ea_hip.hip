@@ -1406,6 +1406,43 @@ struct Plan {
 
 size_t align_up(size_t x) { return (x + 255) & ~(size_t)255; }
 
+// Key splits of the prefill kernel over nt tiles, while the (segment, row block) grid alone leaves CUs idle (one
+// block fills a CU's LDS): doubled while the grid is under 256 blocks and every split keeps at least 16
+// tiles; a caller's split count is taken as given.
+int prefill_splits(int64_t blocks, int nt, int splits) {
+    if (splits > 0) return splits;
+    int ns = 1;
+    while (blocks * ns < 256 && nt / (2 * ns) >= 16) ns *= 2;
+    return ns;
+}
+
+// Whether a step with score modifications takes the prefill kernel, which then pads heads below 128 dims
+// (a caller's digit tiles are of whole ones). It has a higher rate than the multi-row kernel and a
+// longer chain: 16 us a block and 3.3 a tile, behind slicing 0.4 us per 1000 keys of a segment, against 16 us
+// per million pairs, so the shorter of the two estimates (us) decides. On 189 steps of 16 to 2500 tokens, 1 to 4
+// sequences, 2 to 32 heads, 16 to 12000 keys, d = 96 and 128, with and without a cap, on normal values, the
+// choice was within 12% of the faster kernel in all but one (19% there). Scores twice as wide move the bases
+// more often: 10 to 40% more here, 0 to 8% there, and the choice within 32%. Prefill against multi-row
+// kernel, us: 16/8 heads, 64 x 64 keys 41 / 20, 256 x 256 54 / 41, 700 x 700 83 / 161, 128 x 3000 122 / 117, 256
+// x 3000 128 / 191, 2500 x 2500 426 / 932; 8/2 heads, 64 x 12000 127 / 125, 256 x 12000 202 / 332; d = 96, 4/4
+// heads, 256 x 4000 139 / 75. An fp32 output under a bias: the int32 sums' last bits, which the far keys' small
+// weights lose, then flag one row in 8 for tier 2, and the fp64 sums of the other kernel one in 40 to 350: 16/8
+// heads, 700 x 700 364 / 193, 2500 x 2500 2456 / 1387, within a window of 100 562 / 282. (Without a bias 127 /
+// 226 and 639 / 2516, one row in 250 against one in 13.)
+bool prefill_mods(const ea_geometry* g, const ea_options* o, const ea_score_mods* m, int span, int* ntiles, int* nrb) {
+    const int grp = g->num_q_heads / g->num_kv_heads;
+    if (!ea_prefill_eligible(*g, grp, o->kernel, ntiles, nrb, !o->kv_digits)) return false;
+    if (o->kernel == EA_KERNEL_PREFILL || o->timers) return true;
+    if (o->out_fp32 && m->slopes) return false;
+    const int64_t nseg = (int64_t)g->num_seqs * g->num_kv_heads;
+    const int nt = (span + 63) / 64, ns = prefill_splits(nseg * *nrb, nt, o->splits);
+    const double rounds = std::max(1.0, (double)(nseg * *nrb * ns) / 256);
+    const double slicing = o->kv_digits ? 0.0 : 0.4e-3 * (double)nseg * g->max_seq_len;
+    const double prefill = 20 + slicing + rounds * (16 + 3.3 * nt / ns) + (ns > 1 ? 15 : 0);
+    const double pairs = (double)g->num_seqs * g->num_tokens * g->num_q_heads * span;
+    return prefill <= 15 + 16e-6 * pairs;
+}
+
 // Rows per block of the multi-row kernel for this geometry, 0 where another kernel takes the step.
 // d = dv = 128: from 3 rows per segment on, up to where the int8 prefill kernel starts. With 1 or 2
 // rows ea_decode (whose 2-row blocks read at the rate of a large copy) takes the steps of 4096 or more
@@ -1427,10 +1464,6 @@ int mrow_rows(const ea_geometry* g, const ea_options* o, int r_seg, bool mods) {
         if ((r_seg <= 2 && tiles >= 4096) ||
             ea_prefill_eligible(*g, g->num_q_heads / g->num_kv_heads, o->kernel, &nt, &nr))
             return 0;
-    }
-    if (mods) {
-        int nt = 0, nr = 0;
-        if (ea_prefill_eligible(*g, g->num_q_heads / g->num_kv_heads, o->kernel, &nt, &nr)) return 0;
     }
     return r_seg <= 4 ? 4 : (r_seg <= 8 ? 8 : 16);
 }
@@ -1591,20 +1624,13 @@ int make_plan(const ea_geometry* g, const ea_options* o, Plan* pl, const ea_scor
     const int span = m ? mod_span(g, m, maxlen) : maxlen;
     pl->dq_max_tiles = (int)max_tiles;
     pl->t2_keys = maxlen;  // a row's visible keys are distinct and below max_seq_len
-    pl->prefill = ea_prefill_eligible(*g, pl->grp, o->kernel, &pl->pf_ntiles, &pl->pf_nrb) ? 1 : 0;
+    pl->prefill = (m ? prefill_mods(g, o, m, span, &pl->pf_ntiles, &pl->pf_nrb)
+                     : ea_prefill_eligible(*g, pl->grp, o->kernel, &pl->pf_ntiles, &pl->pf_nrb) != 0) ? 1 : 0;
     pl->pf_nsplit = pl->pf_tps = 1;
     if (pl->prefill) {
         if (o->kv_digits && o->kv_digits_tiles < pl->pf_ntiles) return -1;
-        // key splits when the (segment, row block) grid alone leaves CUs idle (one prefill block
-        // fills a CU's LDS): double the splits while the grid is under 256 blocks and every split
-        // keeps at least 16 tiles; a caller's split count is taken as given
-        int ns = 1;
         const int nt = (span + 63) / 64;
-        if (o->splits > 0) {
-            ns = o->splits;
-        } else {
-            while ((int64_t)pl->nseg * pl->pf_nrb * ns < 256 && nt / (2 * ns) >= 16) ns *= 2;
-        }
+        const int ns = prefill_splits((int64_t)pl->nseg * pl->pf_nrb, nt, o->splits);
         pl->pf_tps = (nt + ns - 1) / ns;
         if (pl->pf_tps < 1) pl->pf_tps = 1;
         pl->pf_nsplit = (nt + pl->pf_tps - 1) / pl->pf_tps;
@@ -1628,7 +1654,7 @@ int make_plan(const ea_geometry* g, const ea_options* o, Plan* pl, const ea_scor
     choose_splits(pl->nseg * (int64_t)gen.nrb, span, o->splits, &gen.nsplit, &gen.split_len);
     gen.dq = d128 && !m && dq_fits(gen.nrb);
     Tier1& mr = pl->mr;
-    mr.rb = mrow_rows(g, o, pl->r_seg, m != nullptr);
+    mr.rb = m && pl->prefill ? 0 : mrow_rows(g, o, pl->r_seg, m != nullptr);
     pl->mrow = mr.rb > 0;
     const size_t without = lay_out(pl, g, o, false);
     if (!pl->mrow) return 0;
@@ -1753,8 +1779,8 @@ int list_all(const Params& P, const ea_options* o, unsigned blocks, hipStream_t 
 
 // tier 2 on the listed rows
 void tier2(const Params& P, const ea_options* o, hipStream_t st) {
-    // 512 blocks cost an empty list 2 us, and one of many rows takes a sixteenth of the time on them: steps
-    // that may list many (2500 capped rows of 16 heads with large scores, 826 listed: 3040 -> 250 us)
+    // 512 blocks cost an empty list 2 us, and a long one is shorter by the CUs it fills: steps that may list many
+    // rows (2500 capped tokens of 16 heads, the step: 827 rows listed 3411 -> 995 us)
     const dim3 grid(o->force_tier2 ? EA_T2_BLOCKS : EA_DD_BLOCKS(P.out_fp32 || P.rows >= 8192)), blk(EA_T2_THREADS);
     if (o->force_tier2) {
         if (P.mods) hipLaunchKernelGGL(ea_tier2_wide<true>, grid, blk, 0, st, P);

@@ -366,8 +366,9 @@ struct PfPart {
     double pad2;
 };
 // Returns 1 when the prefill path handles this geometry (and sets the tile and block counts),
-// 0 otherwise. kernel: the ea_options.kernel choice (EA_KERNEL_*).
-int ea_prefill_eligible(const ea_geometry& g, int grp, int kernel, int* ntiles, int* nrb);
+// 0 otherwise. kernel: the ea_options.kernel choice (EA_KERNEL_*). padded: the kernel is its MOD variant,
+// which takes smaller heads than 128.
+int ea_prefill_eligible(const ea_geometry& g, int grp, int kernel, int* ntiles, int* nrb, bool padded = false);
 // Enqueue the slicing kernels (q rows, K/V tiles), then the prefill kernel; 0 or -100 - e.
 int ea_launch_prefill(const Params& P, hipStream_t st);
 int ea_launch_prefill_main(const Params& P, hipStream_t st);

@@ -69,13 +69,13 @@ __device__ __forceinline__ bool table_weight(uint32_t tbits, const double* T1s, 
 // elements at a time in 16-byte loads when both are 16-byte aligned (one memory round trip per
 // batch instead of one per element); mode 2: q holds NaN/inf (no score). Returns (status, M, E):
 // 0 w = M 2^E, 2 domain error, 3 score not certified, 4 weight not certified. MOD: with the cap C and
-// the bias of slope m at distance dist.
+// the bias of slope m at distance dist. d: the rows' elements, a multiple of 8.
 // ------------------------------------------------------------------------------------------------
 template <int MOD = 0>
 __device__ __forceinline__ int3 pf_cold_pair(int mode, const uint8_t* qrow, int qsw, const uint8_t* krow, int ksw,
                                           const uint16_t* qr, const uint16_t* kr, int32_t am, int eS, double alpha,
                                           const double* T1s, const double* T2, const ModCap& C = ModCap{}, float m = 0.0f,
-                                          int dist = 0) {
+                                          int dist = 0, int d = 128) {
     uint32_t tbits = 0;
     int ls = 3;
     bool zero = false;
@@ -126,12 +126,13 @@ __device__ __forceinline__ int3 pf_cold_pair(int mode, const uint8_t* qrow, int 
         };
         if ((((uintptr_t)qr | (uintptr_t)kr) & 15) == 0) {
 #pragma unroll 1
-            for (int c0 = 0; c0 < 128; c0 += 32) {
+            for (int c0 = 0; c0 < d; c0 += 32) {
                 uint4 qv[4], kv[4];
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    qv[u] = *(const uint4*)(qr + c0 + 8 * u);
-                    kv[u] = *(const uint4*)(kr + c0 + 8 * u);
+                    const bool in = c0 + 8 * u < d;  // d is a multiple of 8
+                    qv[u] = in ? *(const uint4*)(qr + c0 + 8 * u) : make_uint4(0, 0, 0, 0);
+                    kv[u] = in ? *(const uint4*)(kr + c0 + 8 * u) : make_uint4(0, 0, 0, 0);
                 }
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
@@ -143,7 +144,7 @@ __device__ __forceinline__ int3 pf_cold_pair(int mode, const uint8_t* qrow, int 
             }
         } else {
 #pragma unroll 1
-            for (int c = 0; c < 128; ++c) {
+            for (int c = 0; c < d; ++c) {
                 double e0;
                 ss = two_sum(ss, (double)__uint_as_float((uint32_t)qr[c] << 16) * (double)__uint_as_float((uint32_t)kr[c] << 16),
                              &e0);
@@ -258,6 +259,20 @@ __device__ __forceinline__ void score_mfma(const uint8_t* const (&kb)[2], const 
 #pragma unroll
             for (int s = (WIDE ? 0 : 1); s < 4; ++s)
                 acc[s + t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A, Bq[s], acc[s + t], 0, 0, 0);
+        }
+    }
+}
+
+// The q digit of weight 256^-1 (plane 4), of elements rounded at slicing, against K digits 1 to 3, beside
+// score_mfma: at most 4 digit pairs then share an accumulator, and 3 share acc_1.
+__device__ __forceinline__ void score_rest(const uint8_t* const (&kb)[2], const uint8_t* const (&qb)[2], int kt, v4i (&acc)[7]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const v4i Bq = *(const v4i*)(qb[h] + 512);
+#pragma unroll
+        for (int t = 1; t < 4; ++t) {
+            const v4i A = *(const v4i*)(kb[h] + t * 8192 + kt * 2048);
+            acc[t - 1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A, Bq, acc[t - 1], 0, 0, 0);
         }
     }
 }

@@ -159,9 +159,10 @@ __device__ __forceinline__ double quad_sumd(double x) {
 }
 
 // src: NE bf16 values (any alignment of 2 bytes); valid = false gives an all-zero vector.
-// lost[c] (optional) receives 1 for each element that is not exact in 30 bits.
+// lost[c] (optional) receives 1 for each element that is not exact in 30 bits. have: the elements there
+// are, a multiple of 8 (negative: none); the others are zeros.
 template <int NE>
-__device__ __forceinline__ void slice_n(const uint16_t* src, bool valid, SliceN<NE>& S, int* lost = nullptr) {
+__device__ __forceinline__ void slice_n(const uint16_t* src, bool valid, SliceN<NE>& S, int* lost = nullptr, int have = NE) {
     constexpr int G = 128 / NE;
     int m[NE], e[NE];
     int bad = 0, lead = INT_MIN;
@@ -171,7 +172,7 @@ __device__ __forceinline__ void slice_n(const uint16_t* src, bool valid, SliceN<
     if (valid && ((uintptr_t)src & 15) == 0) {
 #pragma unroll
         for (int i = 0; i < NE / 8; ++i) {
-            const uint4 v = ((const uint4*)src)[i];
+            const uint4 v = 8 * i < have ? ((const uint4*)src)[i] : make_uint4(0, 0, 0, 0);
             raw[4 * i] = v.x;
             raw[4 * i + 1] = v.y;
             raw[4 * i + 2] = v.z;
@@ -180,7 +181,7 @@ __device__ __forceinline__ void slice_n(const uint16_t* src, bool valid, SliceN<
     } else {
 #pragma unroll
         for (int i = 0; i < NE / 2; ++i)
-            raw[i] = valid ? ((uint32_t)src[2 * i] | ((uint32_t)src[2 * i + 1] << 16)) : 0u;
+            raw[i] = valid && 2 * i < have ? ((uint32_t)src[2 * i] | ((uint32_t)src[2 * i + 1] << 16)) : 0u;
     }
 #pragma unroll
     for (int k = 0; k < NE; ++k) {
@@ -228,8 +229,8 @@ __device__ __forceinline__ void slice_n(const uint16_t* src, bool valid, SliceN<
     S.amax = grp_maxd<G>(amax);
     S.asum = grp_sumd<G>(asum);  // integers below 2^41: exact in any order
 }
-__device__ __forceinline__ void slice32(const uint16_t* src, bool valid, Slice32& S, int* lost = nullptr) {
-    slice_n<32>(src, valid, S, lost);
+__device__ __forceinline__ void slice32(const uint16_t* src, bool valid, Slice32& S, int* lost = nullptr, int have = 32) {
+    slice_n<32>(src, valid, S, lost, have);
 }
 
 }  // namespace
@@ -249,7 +250,7 @@ __global__ void __launch_bounds__(256) ea_pf_qslice(Params P) {
     const int t = (int)((row / Hq) % T), hq = (int)(row % Hq);
     const uint16_t* qr = P.q + b * P.g.q_seq_stride + (int64_t)t * P.g.q_tok_stride + (int64_t)hq * P.g.q_head_stride;
     SliceN<8> S;
-    slice_n<8>(qr + 8 * q16, true, S);
+    slice_n<8>(qr + 8 * q16, 8 * q16 < P.g.head_dim, S);  // dims past the head's are zeros
     uint8_t* dst = P.pfq + row * 512 + 8 * q16;
 #pragma unroll
     for (int sp = 0; sp < 4; ++sp) *(uint2*)(dst + 128 * sp) = make_uint2(S.dig[sp][0], S.dig[sp][1]);
@@ -263,6 +264,22 @@ __global__ void __launch_bounds__(256) ea_pf_qslice(Params P) {
     }
 }
 
+// The next digit, of weight 256^-1, of 16 q elements: the signed byte nearest 256 (q 2^-lsb - X). planes: the
+// elements' bytes of digit plane 0; the first `have` of them exist, the others are zeros.
+__device__ __forceinline__ uint4 rest_digits(const uint16_t* q, const uint8_t* planes, int lsb, int have) {
+    uint64_t lo = 0, hi = 0;
+#pragma unroll 1
+    for (int k = 0; k < min(have, 16); ++k) {
+        int X = 0;
+        for (int sp = 3; sp >= 0; --sp) X = X * 256 + (int)(int8_t)planes[128 * sp + k];
+        const double r = ldexp((double)__uint_as_float((uint32_t)q[k] << 16), -lsb) - (double)X;
+        const uint64_t d = (uint64_t)(min((int)rint(r * 256.0), 127) & 0xFF) << (8 * (k & 7));
+        if (k < 8) lo |= d;
+        else hi |= d;
+    }
+    return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
+}
+
 // ------------------------------------------------------------------------------------------------
 // K/V pages -> one 64-key digit tile per block (segment-major), in the LDS layout of ea_pf_main.
 // Lane quad (key = tid / 4) covers the key's 128 dims and 128 channels. K planes are written
@@ -270,7 +287,7 @@ __global__ void __launch_bounds__(256) ea_pf_qslice(Params P) {
 // assembled in LDS and copied out in 16-byte chunks.
 // ------------------------------------------------------------------------------------------------
 // MOD (score modifications): tiles wholly before the first key that a token of the sequence sees are left
-// out; no row of ea_pf_main reads them.
+// out; no row of ea_pf_main reads them. Heads of fewer dims or channels than 128 are padded with zeros.
 template <bool MOD>
 __global__ void __launch_bounds__(256) ea_pf_kvslice(Params P) {
     __shared__ __align__(16) uint8_t s_v[32768];
@@ -315,7 +332,7 @@ __global__ void __launch_bounds__(256) ea_pf_kvslice(Params P) {
     int bad;
     {
         Slice32 S;
-        slice32(kr, valid, S);
+        slice32(kr, valid, S, nullptr, MOD ? P.g.head_dim - 32 * q4 : 32);
 #pragma unroll
         for (int sp = 0; sp < 4; ++sp) {
 #pragma unroll
@@ -340,7 +357,7 @@ __global__ void __launch_bounds__(256) ea_pf_kvslice(Params P) {
     {
         Slice32 S;
         int lost[32];
-        slice32(vr, valid, S, lost);
+        slice32(vr, valid, S, lost, MOD ? P.g.head_dim_v - 32 * q4 : 32);
         const int gq = (key >> 2) & 3, kt = key >> 4, ii = key & 3;
 #pragma unroll
         for (int sp = 0; sp < 4; ++sp)
@@ -411,7 +428,7 @@ constexpr int PF_OFF_V0 = 32768;
 constexpr int PF_OFF_V1 = 65536;
 constexpr int PF_OFF_M0 = 98304;
 constexpr int PF_OFF_M1 = PF_OFF_M0 + 4096;
-constexpr int PF_QROW = 528;                 // q digit row stride in LDS: 512 bytes + 16 of padding
+constexpr int PF_QROW = 656;                 // q digit row stride in LDS: 640 bytes + 16 of padding
 constexpr int PF_OFF_Q = PF_OFF_M1 + 4096;  // 32 rows x PF_QROW bytes
 constexpr int PF_OFF_T = PF_OFF_Q + 32 * PF_QROW;
 constexpr int PF_OFF_WD = PF_OFF_T + 4096;  // 5 planes x 4 key groups x 2 row groups x 64 lanes x 4 B
@@ -421,8 +438,8 @@ constexpr int PF_LDS = PF_OFF_KEND + 16;
 
 // MOD: a row's base leaves its largest weight at 2^23 to 2^24 times 2^PF_MOD_TOP0 of 2^38, with room for
 // larger ones to come; one that has to move shows scores of a wide spread, whose many small weights lose
-// bits below the base, and leaves it at PF_MOD_TOP.
-constexpr int PF_MOD_TOP0 = 11, PF_MOD_TOP = 13;
+// bits below the base, and leaves it at PF_MOD_TOP. fp32 outputs need every bit there is: PF_MOD_TOP32.
+constexpr int PF_MOD_TOP0 = 11, PF_MOD_TOP = 13, PF_MOD_TOP32 = 14;
 
 template <int N>
 struct PfPar {
@@ -546,15 +563,25 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
             if (lane == 0) atomicMin(&s_kbeg, kb0);
         }
     }
-    // q digits of the block's rows into LDS: [row][plane 4][128 bytes] with rows PF_QROW = 528
-    // bytes apart, so the 16 rows a 16-lane group reads start 4 banks apart (132 dwords = 4 mod 64)
-    // and a 16-byte read per lane touches every bank once; rows past the segment repeat its last row
+    // q digits of the block's rows into LDS: [row][plane 5][128 bytes] with rows PF_QROW = 656
+    // bytes apart, so the 16 rows a 16-lane group reads start 4 banks apart (164 dwords = 36 mod 64)
+    // and a 16-byte read per lane touches every bank once; rows past the segment repeat its last row.
+    // The last plane is read for rows with elements rounded at slicing alone (score_rest)
     for (int c = tid; c < RPB * 32; c += 64 * NWB) {
         const int r = c >> 5, q16 = c & 31;
         const int lrr = min(rbk * RPB + r, P.r_seg - 1);
         int tt;
         const int64_t gr = seg_row(P, b, hk, lrr, &tt);
         *(uint4*)(sQ + r * PF_QROW + q16 * 16) = *(const uint4*)(P.pfq + gr * 512 + q16 * 16);
+        if (q16 < 8) {
+            uint4 rest = make_uint4(0, 0, 0, 0);
+            const PfQMeta& m = ((const PfQMeta*)P.pfqm)[gr];
+            if ((m.flags >> 8) & 0xFF)
+                rest = rest_digits(P.q + b * P.g.q_seq_stride + (int64_t)tt * P.g.q_tok_stride +
+                                       (int64_t)(hk * P.grp + lrr % P.grp) * P.g.q_head_stride + 16 * q16,
+                                   P.pfq + gr * 512 + 16 * q16, m.lsb, P.g.head_dim - 16 * q16);
+            *(uint4*)(sQ + r * PF_QROW + 512 + q16 * 16) = rest;
+        }
     }
     // this lane's q digits (B operand of the score MFMA): row j, dims 64 h + 16 g .. + 15, plane s:
     // chunk 8 s + 4 h + g of the row
@@ -567,7 +594,12 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
     // the score bound per pair is adq * kA 2^lk: |a| times the fold error factor 6.01 u times
     // sum_i A_q,i, with 2^-48 of slack for the roundings of this product and of adq * kAs
     const double adq = fabs(qm.a) * (6.01 * 0x1p-53) * qm.qA * (1.0 + 0x1p-48);
-    const double aqL = fabs(qm.a) * 0.5 * (double)((qm.flags >> 8) & 0xFF);
+    // Elements of q rounded at slicing: each is within half a unit of 2^lsbq, and with its next digit, which
+    // such rows' scores take in (score_rest), within 1/256, times a K element of at most kX; K's lowest digit,
+    // which that product leaves out, is below 64 units, 2^-23 kX. With half a unit 6% of such a row's pairs
+    // (normal values: one row of 128 dims in some 5000) took the cold path one after another, and its block
+    // 4 times the others' time: 10000 rows of up to 2500 keys 505 us, 175 with the digit.
+    const double aqL = fabs(qm.a) * 0x1.01p-8 * (double)((qm.flags >> 8) & 0xFF);
     const double aqX = fabs(qm.a) * 0.5 * (qm.qX + 1.0);
     const bool lossy_q = __ballot(rvalid && ((qm.flags >> 8) & 0xFF)) != 0;
     const bool qbad = (qm.flags & 2) != 0;
@@ -810,7 +842,7 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
         }
         // the base moves when a weight would exceed 2^38 (G - base > 14 for G = E + vlsb)
         const bool need_rb = gm != INT_MIN && (base == INT_MIN || gm > base + 14);
-        int nb = need_rb ? gm - (!MOD ? 10 : (base == INT_MIN ? PF_MOD_TOP0 : PF_MOD_TOP)) : base;
+        int nb = need_rb ? gm - (!MOD ? 10 : (P.out_fp32 ? PF_MOD_TOP32 : (base == INT_MIN ? PF_MOD_TOP0 : PF_MOD_TOP))) : base;
         if constexpr (MOD) {
             if (++since > 4096 && base != INT_MIN) nb = max(nb, base + 8);
             if (ep_tiles > 0 && (__ballot(nb != base) != 0 || ep_tiles >= 256)) refold(ds_pair, nb);
@@ -887,6 +919,10 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
             for (int k = 0; k < 7; ++k) sacc[kk][k] = (v4i){0, 0, 0, 0};
         const bool wide = needq || ((tfl >> (NKT * hh)) & ((1 << NKT) - 1));
         auto scores = [&]() __attribute__((always_inline)) {
+            if (lossy_q) {
+#pragma unroll
+                for (int kk = 0; kk < NKT; ++kk) score_rest(kb, qb, NKT * hh + kk, sacc[kk]);
+            }
             if (wide) {
 #pragma unroll
                 for (int kk = 0; kk < NKT; ++kk) score_mfma<true>(kb, qb, NKT * hh + kk, sacc[kk]);
@@ -931,7 +967,7 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
             adel[kk][3] = adq * kA23.y;
         }
         if (lossy_q || (tfl & 32)) {
-            // elements rounded at slicing: |q_i - Q_i| <= 2^lsbq / 2 and the same for k
+            // elements rounded at slicing: |k_i - K_i| <= 2^lsbk / 2, and q's as aqL has them
 #pragma unroll
             for (int kk = 0; kk < NKT; ++kk)
 #pragma unroll
@@ -1025,7 +1061,8 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
                     kr = P.k + kv_off(P, b, n, hk, 0);
                 }
                 const int3 cw = pf_cold_pair<(MOD >= 2)>(mode, qlds, 0, (const uint8_t*)Kg + key * 128, key & 7, qr, kr, P.am,
-                                                  P.ae + qm.lsb + TMc->lsbk[key], P.alpha, T1s, T2, P.cap, mslope, n - mpos);
+                                                  P.ae + qm.lsb + TMc->lsbk[key], P.alpha, T1s, T2, P.cap, mslope, n - mpos,
+                                                  MOD ? P.g.head_dim : 128);
                 const bool live = cw.x == 0;
                 const int32_t M = cw.y, E = cw.z;
                 if (cw.x == 2) dom = 1;
@@ -1223,6 +1260,7 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
             orow[i] = b * P.g.o_seq_stride + (int64_t)(lrv / P.grp) * P.g.o_tok_stride +
                       (int64_t)hq * P.g.o_head_stride + 16 * NCT * hh + j;
         }
+        const int nch = MOD ? P.g.head_dim_v - 16 * NCT * hh - j : 128;  // channel 16 cc of this lane is there below it
         auto store_out = [&](int i, int cc, uint32_t bits) __attribute__((always_inline)) {
             if (P.out_fp32) ((uint32_t*)P.out)[orow[i] + 16 * cc] = bits;
             else ((uint16_t*)P.out)[orow[i] + 16 * cc] = (uint16_t)bits;
@@ -1248,8 +1286,9 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
                 if (!isfinite(q) || !isfinite(delta) || !live[i]) delta = __builtin_inf();
                 uint32_t bits = 0;
                 const bool ok = !skip[i] && certify_round_normal(q, delta, P.out_fp32, &bits);
-                if (ok && ovalid[i]) store_out(i, cc, bits);
-                if (!skip[i] && !ok) {
+                const bool there = !MOD || 16 * cc < nch;
+                if (ok && ovalid[i] && there) store_out(i, cc, bits);
+                if (!skip[i] && !ok && there) {
                     slow |= 1u << (4 * cc + i);
                     qd[64 * NWB * (4 * cc + i)] = make_double2(q, delta);
                 }
@@ -1317,6 +1356,7 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params P) {
                               (int64_t)hq * P.g.o_head_stride + 16 * NCT * hh + j;
 #pragma unroll
             for (int cc = 0; cc < NCT; ++cc) {
+                if (MOD && 16 * (NCT * hh + cc) + j >= P.g.head_dim_v) continue;
                 if (P.out_fp32) ((uint32_t*)P.out)[o + 16 * cc] = 0u;
                 else ((uint16_t*)P.out)[o + 16 * cc] = 0;
             }
@@ -1403,7 +1443,7 @@ __global__ void __launch_bounds__(128) ea_pf_combine(Params P) {
         const double q = nn * rz;
         double delta = (en * (1.0 + 0x1p-40) + fabs(q) * eZ) * rze * (1.0 + 0x1p-40) + fabs(q) * 0x1p-51 + 0x1p-1070;
         if (!isfinite(q) || !isfinite(delta) || !zok) delta = __builtin_inf();
-        fin = !certify_round(q, delta, P.out_fp32, &bits);
+        fin = c < P.g.head_dim_v && !certify_round(q, delta, P.out_fp32, &bits);
         if (fin) bits = 0;
     }
     const bool anyfin = __syncthreads_or(fin) != 0;  // every thread reaches this barrier
@@ -1437,10 +1477,13 @@ namespace {
 constexpr int PF_RPB = 32;
 }  // namespace
 
-int ea::ea_prefill_eligible(const ea_geometry& g, int grp, int kernel, int* ntiles, int* nrb) {
+int ea::ea_prefill_eligible(const ea_geometry& g, int grp, int kernel, int* ntiles, int* nrb, bool padded) {
     if (kernel == EA_KERNEL_DECODE || kernel == EA_KERNEL_GENERAL) return 0;
     const bool force = kernel == EA_KERNEL_PREFILL;
-    if (g.head_dim != 128 || g.head_dim_v != 128) return 0;
+    if (g.head_dim != 128 || g.head_dim_v != 128) {
+        // heads of 65 to 127 dims padded, as the multi-row kernel does; that one has a form of its own up to 64
+        if (!padded || (g.head_dim_v & 7) || (!force && g.head_dim <= 64 && g.head_dim_v <= 64)) return 0;
+    }
     const int64_t r_seg = (int64_t)g.num_tokens * grp;
     // Rows of one (sequence, KV head) that fill a 32-row block (64 tokens, or fewer tokens with a
     // wider GQA group: speculative trees, chunked prefill) read each K/V tile once here, against

@@ -114,6 +114,8 @@ SHAPES = [
     (2, 8, 4, 2, 64, 100, 16, ("auto", "general")),
     (1, 5, 8, 1, 96, 70, 8, ("auto",)),          # pages under 16 keys: the general kernel
     (1, 34, 2, 2, 128, 129, 32, ("auto", "prefill")),
+    (1, 33, 4, 2, 96, 100, 16, ("auto", "general")),  # padded to 128 dims in the prefill kernel
+    (2, 2, 4, 2, 72, 90, 16, ("auto", "prefill")),
 ]
 
 
@@ -144,6 +146,77 @@ def test_definition(gpu, shape, name):
 
 def _run_plain(p, ab, out):
     return hip.attention_problem(p, None, out, alpha_bits=ab)[0]
+
+
+@pytest.mark.parametrize("kernel", ["auto", "prefill", "general"])
+def test_head_sizes_and_strides(gpu, kernel):
+    """K and V of different head sizes, rows that start on 4-byte boundaries with other data between them, a
+    head size the prefill kernel pads: what lies past a row's end stays out."""
+    rng = np.random.default_rng(77)
+    B, T, Hq, Hkv, d, dv, S = 1, 40, 4, 2, 80, 104, 150
+    q, k, v = bf16(rng, (B, T, Hq, d)), bf16(rng, (B, Hkv, S, d)), bf16(rng, (B, Hkv, S, dv))
+    kv = S - T + 1 + np.arange(T)[None]
+    p = problem.contiguous(q, k, v, kv)
+    want, fl, _ = _run(p, default_alpha_bits(128), hip.ScoreMods(window=60, softcap=10.0), kernel="general")
+    g = p["geom"]
+    for x, w in (("k", d), ("v", dv)):
+        wide = np.full((B, S, Hkv, w + 10), 0x7FC0, np.uint16)
+        wide[..., :w] = p[x].transpose(0, 2, 1, 3)
+        p[x] = wide
+        g[x + "_page_stride"], g[x + "_slot_stride"], g[x + "_head_stride"] = S * Hkv * (w + 10), Hkv * (w + 10), w + 10
+    got, f2, st = _run(p, default_alpha_bits(128), hip.ScoreMods(window=60, softcap=10.0), kernel=kernel)
+    assert (fl == 0).all() and (f2 == 0).all()
+    assert np.array_equal(got, want)
+    assert st["prefill_kernel_rows"] == (T * Hq if kernel == "prefill" else 0)
+    some = mo.row(p, default_alpha_bits(128), 5, window=60, cap=10.0)
+    assert np.array_equal(got.reshape(-1, dv)[5], some)
+
+
+@pytest.mark.parametrize("name", ["plain", "none", "all"])
+@pytest.mark.parametrize("d", [128, 104])
+def test_elements_rounded_at_slicing(gpu, d, name):
+    """Rows of q with elements far below their largest: the prefill kernel takes their next 8 bits in, and
+    decides their scores as it does the others'."""
+    rng = np.random.default_rng(d)
+    B, T, Hq, Hkv, S = 1, 64, 4, 2, 700
+    p = _prob(rng, B, T, Hq, Hkv, d, S)
+    q = (p["q"].astype(np.uint32) << 16).view(np.float32).reshape(T * Hq, d).copy()
+    for r, (n, k) in enumerate([(1, 22), (1, 24), (1, 27), (1, 30), (1, 33), (3, 24), (3, 30), (40, 23), (d - 1, 25), (d - 1, 60)]):
+        q[20 * r, rng.permutation(d)[:n]] *= 2.0 ** -k
+    for r, x in ((210, 0.5), (211, -0.5), (212, 1.5), (213, -1.5), (214, 0.25)):
+        q[r, np.abs(q[r]) > 1.9] = 1.0
+        q[r, 0] = 1.0
+        q[r, d - 1] = x * 2.0 ** -29  # of a largest element of 1 to 2: half steps and their neighbours
+    bits = q.view(np.uint32) >> 16
+    assert (bits << 16 == q.view(np.uint32)).all()
+    p["q"] = bits.astype(np.uint16).reshape(p["q"].shape)
+    ab = default_alpha_bits(d)
+    m = None if name == "plain" else hip.ScoreMods(**_mods_of(name, rng, p))
+    got, fl, st = _run(p, ab, m, "fp32", "prefill")
+    want, f2, _ = _run(p, ab, m, "fp32", "general")
+    assert (fl == 0).all() and (f2 == 0).all()
+    assert np.array_equal(got, want)
+    if st["prefill_kernel_rows"] == 0:  # heads below 128 dims without modifications are another kernel's
+        assert name == "plain" and d != 128
+        return
+    # A score known to within e is undecided with probability 2 e / step, step = ulp of its fp32 value. e: n
+    # rounded elements of q within 2^-8 units each of K's largest, n of k within half a unit of q's largest.
+    k = (p["k"].astype(np.uint32) << 16).view(np.float32).reshape(Hkv, S, d).astype(np.float64)
+    q = q.reshape(T, Hkv, Hq // Hkv, d).astype(np.float64)
+
+    def unit(x):
+        u = 2.0 ** (np.floor(np.log2(np.abs(x).max(-1))) - 29)
+        return u, (np.rint(x / u[..., None]) != x / u[..., None]).sum(-1)
+
+    (uq, nq), (uk, nk) = unit(q), unit(k)
+    alpha = float(np.uint32(ab).view(np.float32))
+    expect = 0.0
+    for h in range(Hkv):
+        t = alpha * (q[:, h] @ k[h].T)
+        e = alpha * ((nq * uq * 1.01 * 2.0 ** -8)[:, h, :, None] * np.abs(k[h]).max(-1) +
+                     np.abs(q[:, h]).max(-1)[..., None] * (0.5 * nk * uk)[h])
+        expect += np.minimum(1.0, 2 * e / np.spacing(np.abs(t).astype(np.float32))).sum()
+    assert st["prefill_kernel_rows"] == T * Hq and st["slow_path_scores"] <= expect + 6 * expect ** 0.5 + 10, expect
 
 
 @pytest.mark.parametrize("name", ["docs", "steep", "cap", "all"])
