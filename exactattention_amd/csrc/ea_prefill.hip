@@ -1480,10 +1480,7 @@ constexpr int PF_RPB = 32;
 int ea::ea_prefill_eligible(const ea_geometry& g, int grp, int kernel, int* ntiles, int* nrb, bool padded) {
     if (kernel == EA_KERNEL_DECODE || kernel == EA_KERNEL_GENERAL) return 0;
     const bool force = kernel == EA_KERNEL_PREFILL;
-    if (g.head_dim != 128 || g.head_dim_v != 128) {
-        // heads of 65 to 127 dims padded, as the multi-row kernel does; that one has a form of its own up to 64
-        if (!padded || (g.head_dim_v & 7) || (!force && g.head_dim <= 64 && g.head_dim_v <= 64)) return 0;
-    }
+    if ((g.head_dim != 128 || g.head_dim_v != 128) && (!padded || (g.head_dim_v & 7))) return 0;
     const int64_t r_seg = (int64_t)g.num_tokens * grp;
     // Rows of one (sequence, KV head) that fill a 32-row block (64 tokens, or fewer tokens with a
     // wider GQA group: speculative trees, chunked prefill) read each K/V tile once here, against

@@ -116,6 +116,8 @@ SHAPES = [
     (1, 34, 2, 2, 128, 129, 32, ("auto", "prefill")),
     (1, 33, 4, 2, 96, 100, 16, ("auto", "general")),  # padded to 128 dims in the prefill kernel
     (2, 2, 4, 2, 72, 90, 16, ("auto", "prefill")),
+    (1, 40, 4, 2, 64, 150, 16, ("prefill",)),
+    (1, 33, 2, 1, 8, 90, 0, ("auto", "prefill")),
 ]
 
 
