@@ -425,6 +425,7 @@ int ea_hip_rotary(const ea_rotary* a, ea_stream_t stream) {
     const int tpb = a->num_tokens >= 4096 ? 4 : 1, v = wide ? 8 : (a->adjacent ? 2 : 1);
     const int64_t units = (int64_t)(a->num_q_heads + a->num_kv_heads) * ((a->adjacent ? R : h) + d - R) / v +
                           (a->v ? (int64_t)a->num_kv_heads * d / v : 0);
+    if (units * tpb >= (int64_t)1 << 30) return -1;  // the kernel counts them in 32 bits
     const int64_t slices = a->num_tokens < 256 ? std::min<int64_t>((units + RT_THREADS - 1) / RT_THREADS, 64) : 1;
     const dim3 grid((unsigned)(((int64_t)a->num_tokens + tpb - 1) / tpb), (unsigned)slices);
     const size_t lds = (size_t)tpb * h * 16;

@@ -196,7 +196,7 @@ class ScoreMods:
       softcap    scores s become c tanh(s / c), c in base-2 logits as alpha is (a cap C in natural units:
                  C / ln 2); 0: none
       slopes     (Hq,) fp32: each key's score falls by slope * |key - q_pos|, in base-2 logits; q_pos
-                 defaults to the end of the token's prefix (kv_len - 1)
+                 defaults to the end of the token's prefix (kv_len - 1); the distances must be below 2^31
       max_span   a bound of the keys between the first and the last that the tokens of one sequence see,
                  where it is far below the sequence's length (it sizes the grid, never the result)
     """
@@ -223,6 +223,10 @@ class ScoreMods:
                 raise ValueError(f"{name} must have {n} entries, got {t.numel()}")
             if t.is_floating_point() != (dt == torch.float32) or t.is_complex() or t.dtype == torch.bool:
                 raise ValueError(f"{name} must hold {'floats' if dt == torch.float32 else 'whole numbers'}")
+            if dt == torch.int32 and n and not t.is_cuda:  # a device array is the caller's word
+                least = int(geom["max_seq_len"]) - (1 << 31) + 1 if name == "q_pos" else -1 << 31
+                if int(t.min()) < least or int(t.max()) >= 1 << 31:
+                    raise ValueError(f"{name} must fit 32 bits" + (", as the distances do" if name == "q_pos" else ""))
             return t.to(device=dev, dtype=dt).contiguous()
 
         keep = (put(self.kv_begin, "kv_begin", tok, torch.int32), put(self.q_pos, "q_pos", tok, torch.int32),

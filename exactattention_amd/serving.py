@@ -24,12 +24,13 @@ from __future__ import annotations
 
 import ctypes
 import operator
+from types import SimpleNamespace
 
 import numpy as np
 
 from . import hip
 from .formats import ExactAttentionDomainError, ExactAttentionUncertifiedError, alpha_bits_for, alpha_fp32_bits
-from .step import Rotary, StepPlan  # noqa: F401
+from .step import PLAN_ROWS, PLAN_SEQS, Rotary, StepPlan  # noqa: F401
 
 TILE = 64  # keys per digit tile
 
@@ -193,9 +194,15 @@ class PagedKVCache:
 
     def _plan_general(self, seqs, counts, k_new, v_new):
         """_plan_append after its checks, for any counts (at least one key in all)."""
-        sa = np.asarray(seqs, dtype=np.int64)
         L, cnt, have, _ = self._grow(seqs, counts)
-        bt_pos, bt_val = [], []  # block-table entries of the new pages
+        idx, bt_pos, bt_val = self._slots(seqs, L, cnt, have)
+        arrays = [idx] + ([bt_pos, bt_val] if bt_pos.size else [])
+        return {"k": k_new.contiguous(), "v": v_new.contiguous(), "grown": bool(bt_pos.size), "arrays": arrays}
+
+    def _slots(self, seqs, L, cnt, have):
+        """After _grow: the pool rows of the new keys, and the new pages' block-table entries."""
+        sa = np.asarray(seqs, dtype=np.int64)
+        bt_pos, bt_val = [], []
         for s, h in zip(seqs, have.tolist()):
             for p in range(h, len(self.pages[s])):
                 bt_pos.append(s * self.max_pages + p)
@@ -203,10 +210,7 @@ class PagedKVCache:
         b_of = np.repeat(np.arange(len(seqs)), cnt)
         pos = np.arange(int(cnt.sum())) - np.repeat(np.cumsum(cnt) - cnt - L, cnt)
         idx = self.bt_host[sa[b_of], pos // self.P].astype(np.int64) * self.P + pos % self.P
-        arrays = [idx]
-        if bt_pos:
-            arrays += [np.asarray(bt_pos, dtype=np.int64), np.asarray(bt_val, dtype=np.int32)]
-        return {"k": k_new.contiguous(), "v": v_new.contiguous(), "grown": bool(bt_pos), "arrays": arrays}
+        return idx, np.asarray(bt_pos, dtype=np.int64), np.asarray(bt_val, dtype=np.int32)
 
     def _grow(self, seqs, counts):
         """The bookkeeping of an append of counts[i] keys to slot seqs[i]: pages taken, lengths, stale
@@ -239,14 +243,32 @@ class PagedKVCache:
         pages are taken here, and one launch on torch's current stream writes their block-table entries and
         the tokens' slots, positions, padded rows and visible lengths. Returns the StepPlan and device copies
         of the arrays `extra`, uploaded with the plan's."""
-        L, cnt, _, taken = self._grow(seqs, counts)
+        L, cnt, have, taken = self._grow(seqs, counts)
+        B, T = len(seqs), max(1, int(cnt.max()))
+        if B > PLAN_SEQS or self.max_seqs > PLAN_ROWS or B * T >= 1 << 31:
+            return self._host_plan(seqs, L, cnt, have, extra, stream)
         # the plan takes pages off the top of a stack: the last entry first
         up = self.stage.put(L.astype(np.int32), cnt.astype(np.int32), np.asarray(seqs, dtype=np.int32),
                             np.asarray(taken[::-1], dtype=np.int32), np.asarray([len(taken)], dtype=np.int32), *extra,
                             stream=stream)
-        plan = StepPlan(len(seqs), int(cnt.sum()), max(1, int(cnt.max())), device=self.dev)
+        plan = StepPlan(B, int(cnt.sum()), T, device=self.dev)
         plan.build(up[0], up[1], self.block_table, up[3], up[4], self.P, slots=up[2], max_seq_len=self.max_seq_len)
         return plan, up[5:]
+
+    def _host_plan(self, seqs, L, cnt, have, extra, stream):
+        """_step_plan's tensors made here, for more sequences or table rows than a StepPlan takes."""
+        B, T = len(seqs), max(1, int(cnt.max()))
+        idx, bt_pos, bt_val = self._slots(seqs, L, cnt, have)
+        b_of = np.repeat(np.arange(B), cnt)
+        j_of = np.arange(len(b_of)) - np.repeat(np.cumsum(cnt) - cnt, cnt)
+        pos = (L[b_of] + j_of).astype(np.int32)
+        kv = np.zeros((B, T), dtype=np.int32)
+        kv[b_of, j_of] = pos + 1
+        up = self.stage.put(idx, pos, b_of * T + j_of, kv, (L + cnt).astype(np.int32), bt_pos, bt_val, *extra, stream=stream)
+        if bt_pos.size:
+            self.block_table.view(-1).index_copy_(0, up[5], up[6])
+        plan = SimpleNamespace(dst_rows=up[0], positions=up[1], q_rows=up[2], kv_len=up[3], seq_len=up[4])
+        return plan, up[7:]
 
     def _plan_one_each(self, seqs, k_new, v_new):
         """_plan_append for one key per sequence (a decode step), in plain integer arithmetic: the

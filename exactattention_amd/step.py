@@ -21,6 +21,8 @@ import numpy as np
 
 from . import hip
 
+PLAN_SEQS, PLAN_ROWS = 8192, 65536  # sequences of a plan, rows of its block table
+
 PLAN_STATUS = {1: "out of pages", 2: "a sequence longer than its table row or max_seq_len",
                4: "more tokens than max_tokens or than pad_tokens of a sequence",
                8: "a negative length or count, or a table row outside the table or used twice"}
@@ -65,8 +67,8 @@ class StepPlan:
         import torch
         if num_seqs < 0 or max_tokens < 0 or pad_tokens <= 0:
             raise ValueError("num_seqs and max_tokens must not be negative, pad_tokens positive")
-        if num_seqs > 8192 or num_seqs * pad_tokens >= 1 << 31 or max_tokens >= 1 << 31:
-            raise ValueError("at most 8192 sequences, and fewer than 2^31 tokens and padded rows")
+        if num_seqs > PLAN_SEQS or num_seqs * pad_tokens >= 1 << 31 or max_tokens >= 1 << 31:
+            raise ValueError(f"at most {PLAN_SEQS} sequences, and fewer than 2^31 tokens and padded rows")
         dev = torch.empty(0, device=device).device
         if dev.type != "cuda":
             raise ValueError("the step plan runs on the GPU")
@@ -99,8 +101,8 @@ class StepPlan:
         rows, width = block_table.shape
         if page_size <= 0 or page_size & (page_size - 1):
             raise ValueError("page_size must be a power of two")
-        if rows > 65536:
-            raise ValueError("at most 65536 block table rows")
+        if rows > PLAN_ROWS:
+            raise ValueError(f"at most {PLAN_ROWS} block table rows")
         B, i32, at = self.num_seqs, self._i32, self.dev.index
         a = hip.StepPlanArgs.from_buffer_copy(self._fixed)
         a.page_size, a.table_rows, a.table_width = page_size, rows, width
@@ -176,6 +178,17 @@ class Rotary:
             raise ValueError(f"{name} needs a contiguous last dimension")
         return m, h, wide, st
 
+    def _target(self, x, name):
+        """_tokens of a tensor to be written, whose rows must not share memory."""
+        m, h, wide, st = self._tokens(x, name)
+        end = self.head_dim
+        for stride, size in sorted(((st[0], m), (st[1], h))):
+            if size > 1:
+                if stride < end:
+                    raise ValueError(f"{name} has rows that share memory")
+                end += stride * (size - 1)
+        return m, h, wide, st
+
     def _args(self, q, k, v, positions):
         """The arguments that the inputs give, checked; (arguments, fp32, tokens, Hq, Hkv)."""
         import torch
@@ -217,7 +230,7 @@ class Rotary:
             k_out = torch.empty((n, hk, self.head_dim), dtype=k.dtype, device=self.dev)
         elif k_out.shape != k.shape or k_out.dtype != k.dtype:
             raise ValueError("k_out must have k's shape and type")
-        so, ko = self._tokens(q_out, "q_out")[3], self._tokens(k_out, "k_out")[3]
+        so, ko = self._target(q_out, "q_out")[3], self._target(k_out, "k_out")[3]
         a.inverse, a.out_fp32, a.q_out_rows, a.pool_rows = bool(inverse), wide, n, n
         a.q_out, a.qo_tok_stride, a.qo_head_stride = q_out.data_ptr(), so[0], so[1]
         a.k_out, a.ko_tok_stride, a.ko_head_stride = k_out.data_ptr(), ko[0], ko[1]
@@ -232,6 +245,8 @@ class Rotary:
         head_dim). Returns it. Rows that no token names are not written; a row may be named once."""
         import torch
         a, _, n, hq, hk = self._args(q, k, v, positions)
+        if not -1 << 31 <= pos_offset < 1 << 31:
+            raise ValueError("pos_offset must fit 32 bits")
         at, d, i64 = self.dev.index, self.head_dim, torch.int64
         shape = k_pool.shape
         for pool, name in ((k_pool, "k_pool"), (v_pool, "v_pool")):
@@ -247,7 +262,9 @@ class Rotary:
             q_out = torch.empty((n, hq, d), dtype=torch.bfloat16, device=self.dev)
             rows, so = n, (hq * d, d)
         else:
-            rows, ho, wide, so = self._tokens(q_out, "q_out")
+            rows, ho, wide, so = self._target(q_out, "q_out")
+            if q_rows is not None and q_out.data_ptr() == q.data_ptr():
+                raise ValueError("q_out must not be q when q_rows moves its rows")
             if wide or ho != hq or (q_rows is None and rows < n):
                 raise ValueError("q_out must be (rows, Hq, head_dim) bf16 (or int16), a row per token without q_rows")
         a.dst_rows = _vec(dst_rows, "dst_rows", at, i64, n)

@@ -223,7 +223,8 @@ int ea_hip_exact_rows(const ea_geometry* g, const ea_buffers* b, const ea_option
  * not read: their pages may hold other sequences' keys by then. */
 typedef struct ea_score_mods {
     const int32_t* kv_begin; /* optional device array, per token; below 0 counts as 0 */
-    const int32_t* q_pos;    /* optional device array, per token; NULL: kv_len - 1 */
+    const int32_t* q_pos;    /* optional device array, per token; NULL: kv_len - 1. |n - q_pos| below 2^31 for
+                                every key n under max_seq_len */
     const float* slopes;     /* optional device array, per query head, in base-2 logits per key */
     uint32_t softcap_bits;   /* fp32 bits of c, positive; 0: none */
     int32_t window;          /* > 0: keys of the prefix a token sees at most; 0: all */

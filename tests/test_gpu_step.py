@@ -380,7 +380,11 @@ def test_rotary_refuses_on_the_device(gpu):
            lambda: r.rotate(q, k, pos, q_out=k), lambda: r.append(q, k, v, pos, dst.int(), pool, pool),
            lambda: r.append(q, k, v, pos, dst[:3], pool, pool), lambda: r.append(q, k, v, pos, dst, pool.float(), pool),
            lambda: r.append(q, k, v, pos, dst, pool, pool.expand(2, -1, -1, -1)), lambda: r.append(q, k, v, pos, dst, pool, pool, q_rows=dst),
-           lambda: r.append(q, k, v, pos, dst, pool, pool, q_out=q[:2]), lambda: r.append(q, k, v[:, :0], pos, dst, pool, pool)]
+           lambda: r.append(q, k, v, pos, dst, pool, pool, q_out=q[:2]), lambda: r.append(q, k, v[:, :0], pos, dst, pool, pool),
+           lambda: r.append(q, k, v, pos, dst, pool, pool, pos_offset=1 << 31),
+           lambda: r.append(q, k, v, pos, dst, pool, pool, q_rows=dst, q_out=q),  # rows that others read first
+           lambda: r.rotate(q, k, pos, q_out=q[:1].expand(4, -1, -1)),
+           lambda: r.rotate(q, k, pos, q_out=q.as_strided(q.shape, (32, 64, 1)))]
     for f in bad:
         with pytest.raises(ValueError):
             f()

@@ -100,6 +100,37 @@ def test_forward(gpu, name, d, page, rot):
         assert np.array_equal(cache.block_table.cpu().numpy()[x, :len(cache.pages[x])], cache.pages[x])
 
 
+@pytest.mark.parametrize("turned", [False, True])
+@pytest.mark.parametrize("B, slots", [(8200, 8200), (3, 65540)])
+def test_batches_past_a_plan(gpu, B, slots, turned):
+    """More sequences, or table rows, than a StepPlan takes: the step's vectors are made on the host, and the
+    batch's parts, each small enough for a plan, give the same."""
+    from exactattention_amd.serving import ExactAttentionBackend, PagedKVCache, Rotary
+    rng = np.random.default_rng(B)
+    r = Rotary(16) if turned else None
+    got = []
+    ql = [3] + [1, 2] * (B // 2)
+    ql = ql[:B]
+    steps = [[bf16(rng, (sum(ql), h, 16)) for h in (2, 1, 1)] for _ in range(2)]
+    for whole in (True, False):
+        cache = PagedKVCache(2 * B, 4, 1, 16, slots if whole else B, 8, digits=False)
+        be = ExactAttentionBackend(cache, 2, alpha_bits=default_alpha_bits(16), rotary=r)
+        s = [cache.add_sequence() for _ in range(B)] if whole is False or slots == B else list(range(slots - B, slots))
+        if whole and slots != B:
+            for x in s:
+                cache.live[x] = True
+        for q, k, v in steps:  # up to 6 keys, two pages
+            outs, cut, t0 = [], (B if whole else B // 2 + 1), 0
+            for i in range(0, B, cut):
+                n = sum(ql[i:i + cut])
+                o, f = be.forward(*(_dev(x[t0:t0 + n]) for x in (q, k, v)), s[i:i + cut], ql[i:i + cut])
+                be.check_flags(f)
+                outs.append(_bits(o))
+                t0 += n
+            got.append(np.concatenate(outs))
+    assert np.array_equal(got[0], got[2]) and np.array_equal(got[1], got[3])
+
+
 def test_forward_positions(gpu):
     """Three position axes, fp32 projections as parts of one row, and given positions for one axis."""
     import torch

@@ -52,7 +52,8 @@ def test_spec_refused(kw):
 
 @pytest.mark.parametrize("kw", [dict(kv_begin=np.zeros(3, np.int32)), dict(q_pos=np.zeros(1, np.int32)),
                                 dict(slopes=np.zeros(2, np.float32)), dict(slopes=np.zeros(4, np.int32)),
-                                dict(kv_begin=np.zeros(2, np.float32)), dict(q_pos=np.zeros(2, bool))])
+                                dict(kv_begin=np.zeros(2, np.float32)), dict(q_pos=np.zeros(2, bool)),
+                                dict(kv_begin=np.array([0, 1 << 31])), dict(q_pos=np.array([0, -(1 << 31) + 131072]))])
 def test_arrays_refused(kw):
     with pytest.raises(ValueError):
         hip.ScoreMods(**kw).bind(GEOM, "cpu")
@@ -62,6 +63,11 @@ def test_arrays_bound():
     a, keep = hip.ScoreMods(kv_begin=np.array([3, 4]), slopes=np.ones(4), window=7, softcap=2.0).bind(GEOM, "cpu")
     assert a.kv_begin == keep[0].data_ptr() and a.q_pos is None and a.window == 7 and a.softcap_bits == 0x40000000
     assert keep[0].dtype.itemsize == 4 and keep[2].dtype.is_floating_point
+
+
+def test_farthest_positions():
+    """Positions whose distance to every key still fits 32 bits."""
+    hip.ScoreMods(q_pos=np.array([(1 << 31) - 1, -(1 << 31) + 131073])).bind(GEOM, "cpu")
 
 
 def test_window_sizes_the_grid():

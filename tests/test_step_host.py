@@ -50,7 +50,7 @@ def _rotary(**kw):
     (-1, dict(num_axes=2, axis_of_pair=None)), (-2, dict(in_fp32=2)), (-2, dict(out_fp32=1)), (-2, dict(scale=float("nan"))),
     (-2, dict(scale=float("inf"))), (-1, dict(q=None)), (-1, dict(k=None)), (-1, dict(q_out=None)), (-1, dict(k_out=None)),
     (-1, dict(v_out=None)), (-1, dict(positions=None)), (-1, dict(half_turns=None)), (-1, dict(pool_rows=-1)),
-    (-1, dict(head_dim=63, rot_dim=62, adjacent=1)),
+    (-1, dict(head_dim=63, rot_dim=62, adjacent=1)), (-1, dict(num_q_heads=1 << 28)),
 ])
 def test_rotary_refuses(rc, kw):
     assert _rotary(**kw) == rc
