@@ -337,3 +337,65 @@ def test_hf_softcap(gpu):
         assert np.array_equal(_bits(out), want)
     with pytest.raises(ValueError):
         hf_attention(None, f(q).transpose(1, 2), f(k), f(v), scaling=1.0, softcap=-2.0)
+
+
+def test_far_pages(gpu):
+    """Pools of more than 2^31 elements: the last pages are written and read."""
+    import torch
+    from exactattention_amd.step import Rotary
+    rng = np.random.default_rng(5)
+    P, Hq, Hkv, d, n = 16, 4, 2, 128, 75
+    pages = (1 << 31) // (P * Hkv * d) + 8
+    q, k, v = (_dev(bf16(rng, (n, h, d))) for h in (Hq, Hkv, Hkv))
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    r, m = Rotary(d), _mods("all", Hq)
+    last = np.arange(-(-n // P))[::-1] + pages - 6
+    far = [torch.empty((pages, P, Hkv, d), dtype=torch.int16, device="cuda") for _ in range(2)]
+    near = [torch.zeros((8, P, Hkv, d), dtype=torch.int16, device="cuda") for _ in range(2)]
+    outs = []
+    for (kp, vp), pg in ((far, last), (near, last - (pages - 8))):
+        rows = torch.from_numpy(pg[np.arange(n) // P] * P + np.arange(n) % P).cuda()
+        qr = r.append(q, k, v, pos, rows, kp, vp)
+        for T in (1, 40):
+            g = dict(num_seqs=1, num_tokens=T, num_q_heads=Hq, num_kv_heads=Hkv, head_dim=d, head_dim_v=d, q_seq_stride=T * Hq * d,
+                     q_tok_stride=Hq * d, q_head_stride=d, o_seq_stride=T * Hq * d, o_tok_stride=Hq * d, o_head_stride=d,
+                     k_page_stride=P * Hkv * d, k_slot_stride=Hkv * d, k_head_stride=d, v_page_stride=P * Hkv * d,
+                     v_slot_stride=Hkv * d, v_head_stride=d, page_size=P, block_table_stride=len(pg), max_seq_len=n)
+            p = dict(geom=g, q=qr[n - T:], k=kp, v=vp, seq_len=np.array([n], np.int32),
+                     kv_len=(n - T + 1 + np.arange(T)).astype(np.int32), block_table=pg[None].astype(np.int32), out_shape=(1, T, Hq, d))
+            for kernel in ("auto", "general") if T == 1 else ("auto", "prefill"):
+                res, fl, _ = hip.attention_problem(p, None, alpha_bits=default_alpha_bits(d), kernel=kernel, mods=m)
+                outs.append(res)
+    for a, b in zip(outs[:4], outs[4:]):
+        assert np.array_equal(a, b)
+    assert np.array_equal(outs[2], outs[3])
+
+
+def test_two_streams(gpu):
+    """Steps in flight on two streams, each with its workspace: the outputs of each alone."""
+    import torch
+    rng = np.random.default_rng(6)
+    ab = default_alpha_bits(128)
+
+    def problem_of(B, T, S):
+        q, k, v = bf16(rng, (B, T, 4, 128), "normal", 2.0), bf16(rng, (B, 2, S, 128)), bf16(rng, (B, 2, S, 128))
+        return problem.contiguous(q, k, v, np.tile(S - T + 1 + np.arange(T), (B, 1)))
+
+    a = hip.DeviceProblem(problem_of(6, 1, 900), mods=_mods("all", 4))
+    b = hip.DeviceProblem(problem_of(1, 300, 700), kernel="prefill", mods=_mods("cap", 4))
+    c = hip.DeviceProblem(problem_of(2, 9, 1300), "fp32", mods=_mods("window", 4))
+    want = []
+    for dp in (a, b, c):
+        hip.launch_hip(dp, ab)
+        torch.cuda.synchronize()
+        want.append((dp.out.clone(), dp.flags.clone()))
+        dp.out.fill_(-1)
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(3):
+        for dp, s in ((b, s1), (a, s2), (c, s1), (a, s2), (a, s2)):
+            with torch.cuda.stream(s):
+                hip.launch_hip(dp, ab)
+    torch.cuda.synchronize()
+    for dp, (o, f) in zip((a, b, c), want):
+        assert torch.equal(dp.out, o) and torch.equal(dp.flags, f)
