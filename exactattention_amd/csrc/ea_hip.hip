@@ -1418,17 +1418,21 @@ int prefill_splits(int64_t blocks, int nt, int splits) {
 
 // Whether a step with score modifications takes the prefill kernel, which then pads heads below 128 dims
 // (a caller's digit tiles are of whole ones). It has a higher rate than the multi-row kernel and a
-// longer chain: 16 us a block and 3.3 a tile, behind slicing 0.4 us per 1000 keys of a segment, against 16 us
-// per million pairs (10 with heads of up to 64 dims), so the shorter of the two estimates (us) decides. On 189 steps of 16 to 2500 tokens, 1 to 4
-// sequences, 2 to 32 heads, 16 to 12000 keys, d = 96 and 128, with and without a cap, on normal values, the
-// choice was within 12% of the faster kernel in all but one (19% there). Scores twice as wide move the bases
-// more often: 10 to 40% more here, 0 to 8% there, and the choice within 32%. Prefill against multi-row
-// kernel, us: 16/8 heads, 64 x 64 keys 41 / 20, 256 x 256 54 / 41, 700 x 700 83 / 161, 128 x 3000 122 / 117, 256
-// x 3000 128 / 191, 2500 x 2500 426 / 932; 8/2 heads, 64 x 12000 127 / 125, 256 x 12000 202 / 332; d = 96, 4/4
-// heads, 256 x 4000 139 / 75; d = 64, 16/8 heads, 256 x 256 55 / 34, 256 x 4000 149 / 152, 2500 x 2500 430 / 576. An fp32 output under a bias: the int32 sums' last bits, which the far keys' small
-// weights lose, then flag one row in 8 for tier 2, and the fp64 sums of the other kernel one in 40 to 350: 16/8
-// heads, 700 x 700 364 / 193, 2500 x 2500 2456 / 1387, within a window of 100 562 / 282. (Without a bias 127 /
-// 226 and 639 / 2516, one row in 250 against one in 13.)
+// longer chain: 16 us a block and 3.3 a tile (4.5 with a bias, which raises the bases tile by tile), behind
+// slicing 0.4 us per 1000 keys of a segment, against 16 us per million pairs (10 with heads of up to 64
+// dims). The shorter of the two estimates (us) decides.
+// On 189 steps of 16 to 2500 tokens, 1 to 4 sequences, 2 to 32 heads, 16 to 12000 keys, d = 96 and 128, with and
+// without a cap, on normal values, the choice was within 12% of the faster kernel in all but one (19%
+// there). Scores twice as wide move the bases more often: 10 to 40% more here, 0 to 8% there, and the
+// choice within 32%. Prefill against multi-row kernel, us: 16/8 heads, 64 x 64 keys 41 / 20, 256 x 256 54 / 41,
+// 700 x 700 83 / 161, 128 x 3000 122 / 117, 256 x 3000 128 / 191, 2500 x 2500 426 / 932; 8/2 heads, 64 x 12000
+// 127 / 125, 256 x 12000 202 / 332; d = 96, 4/4 heads, 256 x 4000 139 / 75; d = 64, 16/8 heads, 256 x 256 55 / 34,
+// 256 x 4000 149 / 152, 2500 x 2500 430 / 576; with a bias 16/8 heads 2500 x 2500 674 / 967, d = 64, 16/4 heads, two
+// sequences of 777 x 777 265 / 165.
+// An fp32 output under a bias: the int32 sums' last bits, which the far keys' small weights lose, then
+// flag one row in 8 for tier 2, and the fp64 sums of the other kernel one in 40 to 350: 16/8 heads, 700 x 700
+// 364 / 193, 2500 x 2500 2456 / 1387, within a window of 100 562 / 282. (Without a bias 127 / 226 and 639 / 2516,
+// one row in 250 against one in 13.)
 bool prefill_mods(const ea_geometry* g, const ea_options* o, const ea_score_mods* m, int span, int* ntiles, int* nrb) {
     const int grp = g->num_q_heads / g->num_kv_heads;
     if (!ea_prefill_eligible(*g, grp, o->kernel, ntiles, nrb, !o->kv_digits)) return false;
@@ -1438,7 +1442,7 @@ bool prefill_mods(const ea_geometry* g, const ea_options* o, const ea_score_mods
     const int nt = (span + 63) / 64, ns = prefill_splits(nseg * *nrb, nt, o->splits);
     const double rounds = std::max(1.0, (double)(nseg * *nrb * ns) / 256);
     const double slicing = o->kv_digits ? 0.0 : 0.4e-3 * (double)nseg * g->max_seq_len;
-    const double prefill = 20 + slicing + rounds * (16 + 3.3 * nt / ns) + (ns > 1 ? 15 : 0);
+    const double prefill = 20 + slicing + rounds * (16 + (m->slopes ? 4.5 : 3.3) * nt / ns) + (ns > 1 ? 15 : 0);
     const double pairs = (double)g->num_seqs * g->num_tokens * g->num_q_heads * span;
     return prefill <= 15 + (std::max(g->head_dim, g->head_dim_v) > 64 ? 16e-6 : 10e-6) * pairs;
 }

@@ -221,6 +221,29 @@ def test_elements_rounded_at_slicing(gpu, d, name):
     assert st["prefill_kernel_rows"] == T * Hq and st["slow_path_scores"] <= expect + 6 * expect ** 0.5 + 10, expect
 
 
+@pytest.mark.parametrize("T", [1, 3, 34])
+@pytest.mark.parametrize("slope", [0.9, 7.0, 16.0, 40.0])
+def test_channels_of_far_keys_alone(gpu, T, slope):
+    """Channels whose values are zero but for keys of weights down to 2^-9000 of the row's largest."""
+    rng = np.random.default_rng(T)
+    S, Hq, d = 230, 2, 128
+    p = _prob(rng, 1, T, Hq, 1, d, S)
+    pos = (S - T + np.arange(T)).astype(np.int32)
+    sl = np.full(Hq, slope, np.float32)
+    ab = default_alpha_bits(d)
+    for far in (0x3F80, 0xBF80):
+        v = np.zeros((1, 1, S, d), np.uint16)
+        v[:, :, :100], v[:, :, 100:150, ::2], v[:, :, 150:, 5] = far, far, 0x4000
+        p["v"] = v
+        want = {r: mo.row(p, ab, r, slopes=sl, q_pos=pos[None]) for r in (0, T * Hq - 1)}
+        for kernel in ("auto", "general") + (("prefill",) if T == 34 else ()):
+            for force in (False, True):
+                res, fl, _ = _run(p, ab, hip.ScoreMods(slopes=sl, q_pos=pos), kernel=kernel, force=force)
+                assert (fl == 0).all()
+                for r, w in want.items():
+                    assert np.array_equal(res.reshape(-1, d)[r], w), (kernel, force, far)
+
+
 @pytest.mark.parametrize("name", ["docs", "steep", "cap", "all"])
 def test_host_exact_tier(gpu, name):
     """Rows left at flag 1 finished by the host tier: the same bits."""
