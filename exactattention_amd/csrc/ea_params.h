@@ -23,7 +23,8 @@ namespace ea {
 #define EA_T2_DONE (2 + EA_T2_ROWS)
 #define EA_T2_NEXT (3 + EA_T2_ROWS)
 #define EA_T2_CHUNKS (4 + EA_T2_ROWS)
-#define EA_T2_CNT (EA_T2_CHUNKS + EA_T2_BLOCKS)
+#define EA_PF_NEXT (EA_T2_CHUNKS + EA_T2_BLOCKS)  // ea_pf_main: items taken past the first blocks', per XCD
+#define EA_T2_CNT (EA_PF_NEXT + 8)
 #define EA_DD_BLOCKS(many) ((many) ? 512 : 32)  // of the double-double pass: two per CU where many rows are listed
 
 // ------------------------------------------------------------------------------------------------
@@ -371,6 +372,8 @@ struct PfPart {
 int ea_prefill_eligible(const ea_geometry& g, int grp, int kernel, int* ntiles, int* nrb, bool padded = false);
 // Enqueue the slicing kernels (q rows, K/V tiles), then the prefill kernel; 0 or -100 - e.
 int ea_launch_prefill(const Params& P, hipStream_t st);
+// ea_pf_main with score modifications (Params::mods), its own file
+const void* ea_pf_mod_fn(int mods);
 int ea_launch_prefill_main(const Params& P, hipStream_t st);
 // With key splits (P.pf_nsplit > 1): the merge of the splits' partials and the rounding.
 int ea_launch_prefill_combine(const Params& P, hipStream_t st);
