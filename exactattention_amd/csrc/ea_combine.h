@@ -132,8 +132,8 @@ __device__ inline int combine_row(const Params& P, int64_t row, int lane) {
         const double zs = n > 0 ? ldexp(z, max(dsh, -1000)) : 0.0;
         Z += zs;
         if constexpr (MOD) {
-            const int64_t cap = MR ? 16 * (((int64_t)n + 63) >> 6) + 6 : INT64_MAX;
-            A += zs * (double)(min((int64_t)n + 4, cap) + nsb + 1);
+            const int64_t most = (int64_t)n + 4, steps = 16 * (((int64_t)n + 63) >> 6) + 6;
+            A += zs * (double)((MR && steps < most ? steps : most) + nsb + 1);
         } else {
             A += zs * (double)(min((int64_t)n + 4, dcap) + nsb);
         }

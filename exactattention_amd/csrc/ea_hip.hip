@@ -49,20 +49,17 @@ using namespace ea;
 // the pieces it may have, instead of dq_min_share: the host knows no more than a hint of the span.
 template <int NT, bool MOD = false>
 __device__ void dq_plan_block(const Params& P) {
-    __shared__ int s_scan[2][NT];
-    __shared__ int s_share, s_most;
+    constexpr int NW = NT / 64;
+    __shared__ int s_sum[NW], s_most[NW];
     const int tid = threadIdx.x, U = P.dq_units, G = P.dq_blocks;
     int32_t* plan = P.dq_plan;
     int32_t* Su = plan + 2;
     int4* brec = (int4*)(plan + P.dq_rec_off);
     const int per = (U + NT - 1) / NT;
     const int u0 = min(tid * per, U), u1 = min(u0 + per, U);
-    // each thread's units twice: their tile counts, kept in Su, and then the prefix sums over them
-    int sum = 0, most = 0;
-    if constexpr (MOD) {
-        if (tid == 0) s_most = 0;
-        __syncthreads();
-    }
+    // each thread's units twice: their tile counts, kept in Su (the first in a register), and then the prefix
+    // sums over them: within the wave in registers, across the waves by way of LDS, one barrier in all
+    int sum = 0, most = 0, first = 0;
     for (int u = u0; u < u1; ++u) {
         int t;
         if constexpr (MOD) {
@@ -72,36 +69,36 @@ __device__ void dq_plan_block(const Params& P) {
         } else {
             t = min((unit_kend(P, u / P.nrb, u % P.nrb) + 63) >> 6, P.dq_max_tiles);
         }
-        Su[u] = t;
+        if (u == u0) first = t;
+        else Su[u] = t;
         sum += t;
     }
-    if constexpr (MOD) atomicMax(&s_most, most);
-    // inclusive scan of the chunk sums (Hillis-Steele, ping-pong)
-    int cur = 0;
-    s_scan[0][tid] = sum;
-    __syncthreads();
-    for (int o = 1; o < NT; o <<= 1) {
-        const int x = s_scan[cur][tid] + (tid >= o ? s_scan[cur][tid - o] : 0);
-        s_scan[cur ^ 1][tid] = x;
-        cur ^= 1;
-        __syncthreads();
+    int run = wave_scan_dpp(sum);
+    if constexpr (MOD) most = wave_max_dpp(most);
+    if ((tid & 63) == 63) {
+        s_sum[tid >> 6] = run;
+        if constexpr (MOD) s_most[tid >> 6] = most;
     }
-    const int W = s_scan[cur][NT - 1];
+    run -= sum;  // exclusive prefix of this thread's chunk, below
+    __syncthreads();
+    int W = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+        run += i < tid >> 6 ? s_sum[i] : 0;
+        W += s_sum[i];
+        if constexpr (MOD) most = max(most, s_most[i]);
+    }
+    // (nsplit slots hold the pieces of a unit: one more than the whole shares it spans)
+    const int least = MOD ? (most + P.nsplit - 2) / (P.nsplit - 1) : P.dq_min_share;
+    const int share = max(max((W + G - 1) / G, least), 1);
     if (tid == 0) {
-        // (nsplit slots hold the pieces of a unit: one more than the whole shares it spans)
-        const int least = MOD ? (s_most + P.nsplit - 2) / (P.nsplit - 1) : P.dq_min_share;
-        const int share = max(max((W + G - 1) / G, least), 1);
-        s_share = share;
         plan[0] = W;
         plan[1] = share;
         Su[U] = W;
         if (P.stats) atomicAdd((unsigned long long*)&P.stats[15], 1ull);
     }
-    __syncthreads();
-    const int share = s_share;
-    int run = s_scan[cur][tid] - sum;  // exclusive prefix of this thread's chunk
     for (int u = u0; u < u1; ++u) {
-        const int t = Su[u];
+        const int t = u == u0 ? first : Su[u];
         Su[u] = run;
         for (int g = (run + share - 1) / share; g * share < run + t && g < G; ++g)
             brec[g] = make_int4(u, run, run + t, share);

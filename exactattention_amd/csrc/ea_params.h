@@ -287,6 +287,17 @@ __device__ __forceinline__ int wave_max_dpp(int x) {
     return __builtin_amdgcn_readlane(x, 63);
 }
 
+// inclusive sum over the wave (every lane active): within each 16 lanes, then across by row broadcasts
+__device__ __forceinline__ int wave_scan_dpp(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
+    return x;
+}
+
 // Max within each 16-lane DPP row (lanes 16r .. 16r+15); every lane of the row receives it.
 __device__ __forceinline__ int row16_max(int x) {
     x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x111, 0xF, 0xF, false));

@@ -8,6 +8,7 @@
 #include <algorithm>
 
 #include "../../include/exactattn_hip.h"
+#include "ea_params.h"
 
 namespace {
 
@@ -30,17 +31,6 @@ int herr(hipError_t e) { return e == hipSuccess ? 0 : -100 - (int)e; }
 constexpr int SP_THREADS = 1024;
 constexpr int SP_MAX_SEQS = 8192;
 constexpr int SP_MAX_ROWS = 65536;
-
-// inclusive sum over the wave: within each 16 lanes, then across (row broadcasts)
-__device__ __forceinline__ int wave_scan(int x) {
-    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
-    return x;
-}
 
 __global__ void __launch_bounds__(SP_THREADS) ea_step_plan_kernel(ea_step_plan A, int pshift) {
     extern __shared__ __align__(16) int smem[];
@@ -83,7 +73,7 @@ __global__ void __launch_bounds__(SP_THREADS) ea_step_plan_kernel(ea_step_plan A
         st += (int)c;
         sp += need_of(L, c);
     }
-    int at = wave_scan(st), ap = wave_scan(sp);
+    int at = ea::wave_scan_dpp(st), ap = ea::wave_scan_dpp(sp);
     if ((tid & 63) == 63) {
         part[0][tid >> 6] = at;
         part[1][tid >> 6] = ap;
