@@ -85,31 +85,21 @@ __device__ __forceinline__ int to_fixed(int m, int e, int lsb, int* inexact) {
     return m < 0 ? -r : r;
 }
 
-// biased digit bytes of X (|X| < 2^30): byte s of the result, xor 0x80, is digit s
-__device__ __forceinline__ uint32_t digits_u(int X) { return (uint32_t)X + 0x80808080u; }
-__device__ __forceinline__ int digit(uint32_t u, int s) { return (int)(int8_t)(((u >> (8 * s)) & 0xFF) ^ 0x80); }
-// sum_s |d_s| 256^s
-__device__ __forceinline__ double digit_abs(uint32_t u) {
-    double a = 0.0;
-#pragma unroll
-    for (int s = 3; s >= 0; --s) {
-        int d = digit(u, s);
-        a = a * 256.0 + (double)(d < 0 ? -d : d);
-    }
-    return a;
+// digit bytes of X (|X| < 2^30): byte s is digit s, in two's complement
+__device__ __forceinline__ uint32_t digits_of(int X) { return ((uint32_t)X + 0x80808080u) ^ 0x80808080u; }
+// sum_s |d_s| 256^s: every byte's magnitude (at most 128) in place, below 2^32
+__device__ __forceinline__ uint32_t digit_abs(uint32_t v) {
+    const uint32_t neg = (v >> 7) & 0x01010101u;
+    return (v ^ (neg * 255u)) + neg;
 }
-
-__device__ __forceinline__ double wave_max_d(double x) {
-    for (int o = 32; o > 0; o >>= 1) x = fmax(x, __shfl_xor(x, o, 64));
-    return x;
-}
-
 
 // ------------------------------------------------------------------------------------------------
 // Digits of NE consecutive bf16 elements held by one lane; the G = 128 / NE adjacent lanes of a
 // group (lane & (G - 1)) cover a 128-element vector. Returns the vector's lsb (group-uniform) and
 // the digit bytes (4 planes x NE bytes, as NE / 4 dwords per plane). K/V rows take NE = 32 (a quad
-// per key); q rows NE = 8 (16 lanes per row: four times the lanes, a quarter of the chain).
+// per key); q rows NE = 8 (16 lanes per row: four times the lanes, a quarter of the chain). All of it in integers:
+// with magnitudes as fp64 sums, digits picked byte by byte and shuffles through LDS 65536 q rows took 20.9
+// us (now 17 to 19) and the K and V of 8 x 4096 keys 30.3 (25.9).
 // ------------------------------------------------------------------------------------------------
 template <int NE>
 struct SliceN {
@@ -119,46 +109,28 @@ struct SliceN {
 };
 using Slice32 = SliceN<32>;
 
+// over the group's G lanes, in every one of them: rotations within a row of 16 lanes, or permutations within a
+// quad
+template <int G, typename F>
+__device__ __forceinline__ int grp_all(int x, F f) {
+    static_assert(G == 16 || G == 4, "a DPP row or quad");
+    if constexpr (G == 16) {
+        x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x128, 0xF, 0xF, false));  // row_ror 8, 4, 2, 1
+        x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x124, 0xF, 0xF, false));
+        x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x122, 0xF, 0xF, false));
+        return f(x, __builtin_amdgcn_update_dpp(0, x, 0x121, 0xF, 0xF, false));
+    } else {
+        x = f(x, __builtin_amdgcn_update_dpp(0, x, 0xB1, 0xF, 0xF, false));  // quad_perm 1 0 3 2, 2 3 0 1
+        return f(x, __builtin_amdgcn_update_dpp(0, x, 0x4E, 0xF, 0xF, false));
+    }
+}
 template <int G>
 __device__ __forceinline__ int grp_max(int x) {
-#pragma unroll
-    for (int o = 1; o < G; o <<= 1) x = max(x, __shfl_xor(x, o, 64));
-    return x;
+    return grp_all<G>(x, [](int a, int b) { return max(a, b); });
 }
 template <int G>
 __device__ __forceinline__ int grp_sum(int x) {
-#pragma unroll
-    for (int o = 1; o < G; o <<= 1) x += __shfl_xor(x, o, 64);
-    return x;
-}
-template <int G>
-__device__ __forceinline__ double grp_maxd(double x) {
-#pragma unroll
-    for (int o = 1; o < G; o <<= 1) x = fmax(x, __shfl_xor(x, o, 64));
-    return x;
-}
-template <int G>
-__device__ __forceinline__ double grp_sumd(double x) {
-#pragma unroll
-    for (int o = 1; o < G; o <<= 1) x += __shfl_xor(x, o, 64);
-    return x;
-}
-
-__device__ __forceinline__ int quad_max(int x) {
-    x = max(x, __shfl_xor(x, 1, 64));
-    return max(x, __shfl_xor(x, 2, 64));
-}
-__device__ __forceinline__ int quad_sum(int x) {
-    x += __shfl_xor(x, 1, 64);
-    return x + __shfl_xor(x, 2, 64);
-}
-__device__ __forceinline__ double quad_maxd(double x) {
-    x = fmax(x, __shfl_xor(x, 1, 64));
-    return fmax(x, __shfl_xor(x, 2, 64));
-}
-__device__ __forceinline__ double quad_sumd(double x) {
-    x += __shfl_xor(x, 1, 64);
-    return x + __shfl_xor(x, 2, 64);
+    return grp_all<G>(x, [](int a, int b) { return a + b; });
 }
 
 // src: NE bf16 values (any alignment of 2 bytes); valid = false gives an all-zero vector.
@@ -196,11 +168,12 @@ __device__ __forceinline__ void slice_n(const uint16_t* src, bool valid, SliceN<
     lead = grp_max<G>(lead);
     bad = grp_max<G>(bad);
     const int lsb = (lead == INT_MIN) ? 0 : lead - 29;
-    int inex = 0, need4 = 0, xmax = 0;
-    double amax = 0.0, asum = 0.0;
+    int inex = 0, xmax = 0;
+    uint32_t amax = 0, low = 0;
+    uint64_t asum = 0;
 #pragma unroll
     for (int w4 = 0; w4 < NE / 4; ++w4) {
-        uint32_t u[4];
+        uint32_t v[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int kk = 4 * w4 + k;
@@ -208,29 +181,29 @@ __device__ __forceinline__ void slice_n(const uint16_t* src, bool valid, SliceN<
             const int X = (bad || m[kk] == 0) ? 0 : to_fixed(m[kk], e[kk], lsb, &ie);
             inex += ie;
             if (lost) lost[kk] = ie;
-            u[k] = digits_u(X);
-            need4 |= digit(u[k], 0) != 0;
-            const double a = digit_abs(u[k]);
-            amax = fmax(amax, a);
+            v[k] = digits_of(X);
+            low |= v[k] & 0xFFu;
+            const uint32_t a = digit_abs(v[k]);
+            amax = max(amax, a);
             asum += a;
             xmax = max(xmax, X < 0 ? -X : X);
         }
-        // plane s: byte k of dword w4 = digit s of element 4 w4 + k
-#pragma unroll
-        for (int sp = 0; sp < 4; ++sp) {
-            uint32_t d = 0;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) d |= (((u[k] >> (8 * sp)) & 0xFFu) ^ 0x80u) << (8 * k);
-            S.dig[sp][w4] = d;
-        }
+        // plane s: byte k of dword w4 = digit s of element 4 w4 + k, a transposition of 4 x 4 bytes
+        const uint32_t lo01 = __builtin_amdgcn_perm(v[1], v[0], 0x05010400u), hi01 = __builtin_amdgcn_perm(v[1], v[0], 0x07030602u);
+        const uint32_t lo23 = __builtin_amdgcn_perm(v[3], v[2], 0x05010400u), hi23 = __builtin_amdgcn_perm(v[3], v[2], 0x07030602u);
+        S.dig[0][w4] = __builtin_amdgcn_perm(lo23, lo01, 0x05040100u);
+        S.dig[1][w4] = __builtin_amdgcn_perm(lo23, lo01, 0x07060302u);
+        S.dig[2][w4] = __builtin_amdgcn_perm(hi23, hi01, 0x05040100u);
+        S.dig[3][w4] = __builtin_amdgcn_perm(hi23, hi01, 0x07060302u);
     }
     S.lsb = lsb;
     S.bad = bad;
     S.inex = grp_sum<G>(inex);
-    S.need4 = grp_max<G>(need4);
+    S.need4 = grp_max<G>(low != 0);
     S.xmax = grp_max<G>(xmax);
-    S.amax = grp_maxd<G>(amax);
-    S.asum = grp_sumd<G>(asum);  // integers below 2^41: exact in any order
+    S.amax = (double)(uint32_t)grp_all<G>((int)amax, [](int a, int b) { return (int)max((uint32_t)a, (uint32_t)b); });
+    const int hi = grp_sum<G>((int)(asum >> 20)), lo = grp_sum<G>((int)(asum & 0xFFFFF));
+    S.asum = (double)hi * 0x1p20 + (double)lo;  // exact: integers below 2^41
 }
 __device__ __forceinline__ void slice32(const uint16_t* src, bool valid, Slice32& S, int* lost = nullptr, int have = 32) {
     slice_n<32>(src, valid, S, lost, have);
@@ -359,7 +332,7 @@ __global__ void __launch_bounds__(256) ea_pf_kvslice(Params P) {
             for (int k = 0; k < 32; ++k)
                 if (lost[k]) atomicAdd(&s_lc[32 * q4 + k], 1);
         }
-        bad = quad_max(bad | S.bad);
+        bad = grp_max<4>(bad | S.bad);
         if (q4 == 0) {
             TM->vlsb[key] = S.lsb;
             if (bad) {
@@ -374,9 +347,8 @@ __global__ void __launch_bounds__(256) ea_pf_kvslice(Params P) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) dv4[tid + 256 * i] = sv4[tid + 256 * i];
     if (tid < 128) TM->EV[tid] = 0.5 * (0x1p38 + 1.0) * (double)s_lc[tid];
-    if (tid == 0) {
-        int tot = 0;
-        for (int c = 0; c < 128; ++c) tot += s_lc[c];
+    const int tot = tid < 64 ? wave_scan_dpp(s_lc[tid] + s_lc[tid + 64]) : 0;
+    if (tid == 63) {
         TM->tfl = s_tfl;
         TM->pad = 0;
         TM->EVt = 0.5 * (0x1p38 + 1.0) * (double)tot;
