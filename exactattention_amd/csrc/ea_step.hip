@@ -23,7 +23,8 @@ int herr(hipError_t e) { return e == hipSuccess ? 0 : -100 - (int)e; }
 // What bounds it is latency: 24 bytes a token leave it, and a step of 125,000 tokens writes 5 MB. So it
 // is one launch of a short chain: every block reads the sequences (12 bytes each), sums them up in LDS by
 // itself, and takes its share of the padded rows (b, j), whose sequence is a division away, without a
-// search. A row with a token writes all that belongs to it, and the table entry too where it opens a
+// search (with searches 5.6, 8.3 and 9.0 us for 33 sequences of 1 token, 256 of up to 300 and 1000 of up to 500;
+// 3.1, 5.0 and 6.3 so). A row with a token writes all that belongs to it, and the table entry too where it opens a
 // page. No block reads what another one writes (new pages come from the stack, not from the table), so
 // none waits for another. Every input is checked by each block alike: a step that does not fit leaves
 // the table alone and reports why.
@@ -148,7 +149,8 @@ __global__ void __launch_bounds__(SP_THREADS) ea_step_plan_kernel(ea_step_plan A
 // less than the pair's 8 bytes of traffic, so the exact form is free here.
 // What bounds it is memory: every element is read once and written once. A block takes whole tokens, so
 // the sines of a token are computed once for all its heads (LDS), and q, k and v of a token go in one
-// launch, k and v straight to their pool rows.
+// launch, k and v straight to their pool rows. 16,384 tokens of 32 q, 8 k and 8 v heads of 128 dims: 87 us, 4.6
+// TB/s of the 4.78 that a large copy reaches; 33 tokens 4.6 us, of which a launch alone is about 2.
 // ------------------------------------------------------------------------------------------------
 constexpr int RT_THREADS = 256;
 constexpr int RT_MAX_PAIRS = 128;  // rot_dim at most 256
@@ -410,13 +412,15 @@ int ea_hip_rotary(const ea_rotary* a, ea_stream_t stream) {
     }
     const bool wide = !(ptr & 15) && !(si & (in - 1)) && !(so & (out - 1)) && !(d & 7) && !((a->adjacent ? R : h) & 7);
     if (!wide && a->adjacent && (d & 1)) return -1;  // the narrow form of adjacent pairs takes two elements at a time
-    // four tokens a block where there are many (fewer sines waited for), and a block for every 256 units of a
-    // token where they alone would leave CUs idle
-    const int tpb = a->num_tokens >= 4096 ? 4 : 1, v = wide ? 8 : (a->adjacent ? 2 : 1);
+    // Four tokens a block where there are many (fewer sines waited for; 48 heads of 128 dims, 4 -> 1 a block: 8192
+    // tokens 43.2 -> 44.4 us, 16384 95.1 -> 97.2, but 4096 25.6 -> 25.1 and 1000 13.4 -> 9.8), and a block for every
+    // 256 units of a token where they alone would leave CUs idle (33 tokens 5.9 -> 4.2, 500 7.5 -> 6.4, but 1000
+    // 9.9 -> 10.2 and 16384 95 -> 100)
+    const int tpb = a->num_tokens >= 8192 ? 4 : 1, v = wide ? 8 : (a->adjacent ? 2 : 1);
     const int64_t units = (int64_t)(a->num_q_heads + a->num_kv_heads) * ((a->adjacent ? R : h) + d - R) / v +
                           (a->v ? (int64_t)a->num_kv_heads * d / v : 0);
     if (units * tpb >= (int64_t)1 << 30) return -1;  // the kernel counts them in 32 bits
-    const int64_t slices = a->num_tokens < 256 ? std::min<int64_t>((units + RT_THREADS - 1) / RT_THREADS, 64) : 1;
+    const int64_t slices = a->num_tokens < 768 ? std::min<int64_t>((units + RT_THREADS - 1) / RT_THREADS, 64) : 1;
     const dim3 grid((unsigned)(((int64_t)a->num_tokens + tpb - 1) / tpb), (unsigned)slices);
     const size_t lds = (size_t)tpb * h * 16;
     const hipStream_t st = (hipStream_t)stream;
