@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import numpy as np
 
@@ -28,22 +29,40 @@ PLAN_STATUS = {1: "out of pages", 2: "a sequence longer than its table row or ma
                8: "a negative length or count, or a table row outside the table or used twice"}
 
 
-def _call(fn, args, index: int, what: str) -> None:
-    """One launch on torch's current stream of device `index`, made current when it is not."""
+# ea_step_plan and ea_rotary as struct formats: a call packs its arguments in one go, where setting the fields of a
+# ctypes structure one by one costs about 70 ns each
+_PLAN, _ROTARY = struct.Struct("8i14Q"), struct.Struct("11if15q11Q")
+assert _PLAN.size == ctypes.sizeof(hip.StepPlanArgs) and _ROTARY.size == ctypes.sizeof(hip.RotaryArgs)
+
+
+_C = None  # torch's, once a plan or a rotation exists
+
+
+def _entry(name: str):
+    """The C entry point, taking its arguments packed."""
+    global _C
     import torch
-    C = torch._C
-    if C._cuda_getDevice() == index:
-        rc = fn(ctypes.byref(args), C._cuda_getCurrentRawStream(index))
+    _C = torch._C
+    fn = hip.load()[name]  # a function object of its own
+    fn.argtypes, fn.restype = [ctypes.c_char_p, ctypes.c_void_p], ctypes.c_int
+    return fn
+
+
+def _call(fn, args: bytes, index: int, what: str) -> None:
+    """One launch on torch's current stream of device `index`, made current when it is not."""
+    if _C._cuda_getDevice() == index:
+        rc = fn(args, _C._cuda_getCurrentRawStream(index))
     else:
+        import torch
         with torch.cuda.device(index):
-            rc = fn(ctypes.byref(args), C._cuda_getCurrentRawStream(index))
+            rc = fn(args, _C._cuda_getCurrentRawStream(index))
     if rc:
         raise ValueError(f"{what}: error code {rc}")
 
 
 def _vec(t, name, index, dtype, n=None):
     """The address of a contiguous tensor of this type on this device (of n entries)."""
-    if t.dtype is not dtype or not t.is_cuda or t.get_device() != index or not t.is_contiguous():
+    if t.dtype is not dtype or t.get_device() != index or not t.is_contiguous():  # -1 on the host
         raise ValueError(f"{name} must be a contiguous {dtype} tensor on cuda:{index}")
     if n is not None and t.numel() != n:
         raise ValueError(f"{name} must have {n} entries, got {t.numel()}")
@@ -82,12 +101,9 @@ class StepPlan:
         self.seq_len = torch.empty(num_seqs, dtype=i32, device=dev)
         self.num_free = torch.empty(1, dtype=i32, device=dev)
         self.status = torch.empty(1, dtype=i32, device=dev)
-        self._lib, self._i32 = hip.load().ea_hip_step_plan, i32
-        self._fixed = bytes(hip.StepPlanArgs(
-            num_seqs=num_seqs, max_tokens=max_tokens, pad_tokens=pad_tokens, dst_rows=self.dst_rows.data_ptr(),
-            positions=self.positions.data_ptr(), seq_of=self.seq_of.data_ptr(), q_rows=self.q_rows.data_ptr(),
-            kv_len=self.kv_len.data_ptr(), new_seq_len=self.seq_len.data_ptr(), new_num_free=self.num_free.data_ptr(),
-            status=self.status.data_ptr()))
+        self._fn, self._i32, self._at = _entry("ea_hip_step_plan"), i32, dev.index
+        self._out = tuple(t.data_ptr() for t in (self.dst_rows, self.positions, self.seq_of, self.q_rows, self.kv_len,
+                                                 self.seq_len, self.num_free, self.status))
 
     def build(self, seq_len, counts, block_table, free_pages, num_free, page_size: int, *, slots=None,
               max_seq_len: int | None = None) -> None:
@@ -103,19 +119,16 @@ class StepPlan:
             raise ValueError("page_size must be a power of two")
         if rows > PLAN_ROWS:
             raise ValueError(f"at most {PLAN_ROWS} block table rows")
-        B, i32, at = self.num_seqs, self._i32, self.dev.index
-        a = hip.StepPlanArgs.from_buffer_copy(self._fixed)
-        a.page_size, a.table_rows, a.table_width = page_size, rows, width
-        a.max_seq_len = 0x7FFFFFFF if max_seq_len is None else int(max_seq_len)
-        a.free_capacity = free_pages.numel()
-        a.seq_len = _vec(seq_len, "seq_len", at, i32, B)
-        a.counts = _vec(counts, "counts", at, i32, B)
-        if slots is not None:
-            a.slots = _vec(slots, "slots", at, i32, B)
-        a.free_pages = _vec(free_pages, "free_pages", at, i32)
-        a.num_free = _vec(num_free, "num_free", at, i32, 1)
-        a.block_table = _vec(block_table, "block_table", at, i32)
-        _call(self._lib, a, at, "ea_hip_step_plan")
+        B, i32, at = self.num_seqs, self._i32, self._at
+        longest = 0x7FFFFFFF if max_seq_len is None else int(max_seq_len)
+        if not 0 <= longest < 1 << 31:
+            raise ValueError("max_seq_len must fit 31 bits")
+        _call(self._fn, _PLAN.pack(
+            B, page_size, rows, width, self.max_tokens, self.pad_tokens, longest, free_pages.numel(),
+            _vec(seq_len, "seq_len", at, i32, B), _vec(counts, "counts", at, i32, B),
+            0 if slots is None else _vec(slots, "slots", at, i32, B), _vec(free_pages, "free_pages", at, i32),
+            _vec(num_free, "num_free", at, i32, 1), _vec(block_table, "block_table", at, i32), *self._out),
+            at, "ea_hip_step_plan")
 
     def check(self) -> None:
         """Waits for the plan and raises when the step did not fit."""
@@ -157,22 +170,20 @@ class Rotary:
         self.axes = len(sections) if sections is not None else int(ax.max()) + 1
         self.half_turns = torch.from_numpy(f / math.pi).to(self.dev)
         self.axis_of_pair = torch.from_numpy(ax.astype(np.uint8)).to(self.dev)
-        self._lib = hip.load().ea_hip_rotary
-        self._bits, self._f32 = (torch.bfloat16, torch.int16), torch.float32
-        self._fixed = bytes(hip.RotaryArgs(head_dim=head_dim, rot_dim=rot, num_axes=self.axes, adjacent=self.adjacent,
-                                           scale=self.scale, half_turns=self.half_turns.data_ptr(),
-                                           axis_of_pair=self.axis_of_pair.data_ptr()))
+        self._fn, self._at = _entry("ea_hip_rotary"), self.dev.index
+        self._bits, self._f32, self._i32, self._i64 = (torch.bfloat16, torch.int16), torch.float32, torch.int32, torch.int64
+        self._half, self._axis = self.half_turns.data_ptr(), self.axis_of_pair.data_ptr()
 
-    def _tokens(self, x, name, n=None, dtypes=None):
+    def _tokens(self, x, name, n=None):
         """Checks a (tokens, heads, head_dim) tensor, int16 standing for bf16 bits: (tokens, heads, fp32, strides)."""
-        if x.dim() != 3:
+        shape, st = x.shape, x.stride()
+        if len(shape) != 3:
             raise ValueError(f"{name} must be (tokens, heads, {self.head_dim})")
-        m, h, d = x.shape
-        st = x.stride()
+        m, h, d = shape
         if d != self.head_dim or (n is not None and m != n):
             raise ValueError(f"{name} must be (tokens, heads, {self.head_dim}), one row per token")
         wide = x.dtype is self._f32
-        if not (wide or x.dtype in self._bits) or not x.is_cuda or x.get_device() != self.dev.index:
+        if not (wide or x.dtype in self._bits) or x.get_device() != self._at:  # -1 on the host
             raise ValueError(f"{name} must be bf16 (or int16 bit patterns) or fp32 on {self.dev}")
         if st[2] != 1 and m * h:
             raise ValueError(f"{name} needs a contiguous last dimension")
@@ -190,51 +201,54 @@ class Rotary:
         return m, h, wide, st
 
     def _args(self, q, k, v, positions):
-        """The arguments that the inputs give, checked; (arguments, fp32, tokens, Hq, Hkv)."""
-        import torch
+        """The inputs, checked: (tokens, Hq, Hkv, fp32, strides of q, k and v in order, the positions' axis stride)."""
         n, hq, wide, sq = self._tokens(q, "q")
         _, hk, wk, sk = self._tokens(k, "k", n)
-        a = hip.RotaryArgs.from_buffer_copy(self._fixed)
+        sv = (0, 0)
         if v is not None:
             _, hv, wv, sv = self._tokens(v, "v", n)
             if hv != hk:
                 raise ValueError("k and v must have the same heads")
             wk = wk if wv == wk else None
-            a.v, a.v_tok_stride, a.v_head_stride = v.data_ptr(), sv[0], sv[1]
         if wk is not wide:
             raise ValueError("q, k and v must have one type")
-        if positions.dtype is not torch.int32 or not positions.is_cuda or positions.get_device() != self.dev.index:
+        if positions.dtype is not self._i32 or positions.get_device() != self._at:
             raise ValueError(f"positions must be int32 on {self.dev}")
-        shape, sp = tuple(positions.shape), positions.stride()
+        shape, sp = positions.shape, positions.stride()
         if shape != (n,) if len(shape) == 1 else (len(shape) != 2 or shape[1] != n or shape[0] < self.axes):
             raise ValueError(f"positions must be ({self.axes}, {n}) or, for one axis, ({n},)")
         if (len(shape) == 1 and self.axes > 1) or (n > 1 and sp[-1] != 1):
             raise ValueError(f"positions must be ({self.axes}, {n}), each axis contiguous")
-        a.num_tokens, a.num_q_heads, a.num_kv_heads, a.in_fp32 = n, hq, hk, wide
-        a.q_tok_stride, a.q_head_stride, a.k_tok_stride, a.k_head_stride = sq[0], sq[1], sk[0], sk[1]
-        a.pos_axis_stride = sp[0] if len(shape) == 2 else 0
-        a.q, a.k, a.positions = q.data_ptr(), k.data_ptr(), positions.data_ptr()
-        return a, wide, n, hq, hk
+        return n, hq, hk, wide, (sq[0], sq[1], sk[0], sk[1], sv[0], sv[1]), sp[0] if len(shape) == 2 else 0
+
+    def _launch(self, n, hq, hk, wide, strides, axis_stride, inverse, offset, so, sk, sv, rows, pool, inputs, outputs):
+        """strides: the inputs'; so, sk, sv: of q's, k's and v's output; rows, pool: theirs; inputs: addresses of q, k,
+        v and positions, outputs: of q_rows, dst_rows and the outputs."""
+        _call(self._fn, _ROTARY.pack(n, hq, hk, self.head_dim, self.rot_dim, self.axes, self.adjacent, inverse, wide,
+                                     wide and not sv, offset, self.scale, *strides, so[0], so[1], sk[0], sk[1],
+                                     *(sv or (0, 0)), axis_stride, rows, pool, *inputs, self._half, self._axis, *outputs),
+              self._at, "ea_hip_rotary")
 
     def rotate(self, q, k, positions, *, inverse: bool = False, q_out=None, k_out=None):
         """q (tokens, Hq, head_dim) and k (tokens, Hkv, head_dim) turned by positions ((tokens,) or (axes,
         tokens) int32), into new tensors of their type or into q_out and k_out (which may be q and k
         themselves). inverse turns back: the gradient of the rotation. Returns (q_out, k_out)."""
-        import torch
-        a, wide, n, hq, hk = self._args(q, k, None, positions)
+        n, hq, hk, wide, strides, axis_stride = self._args(q, k, None, positions)
+        d = self.head_dim
         if q_out is None:
-            q_out = torch.empty((n, hq, self.head_dim), dtype=q.dtype, device=self.dev)
+            q_out, so = q.new_empty((n, hq, d)), (hq * d, d)
         elif q_out.shape != q.shape or q_out.dtype != q.dtype:
             raise ValueError("q_out must have q's shape and type")
+        else:
+            so = self._target(q_out, "q_out")[3]
         if k_out is None:
-            k_out = torch.empty((n, hk, self.head_dim), dtype=k.dtype, device=self.dev)
+            k_out, sk = k.new_empty((n, hk, d)), (hk * d, d)
         elif k_out.shape != k.shape or k_out.dtype != k.dtype:
             raise ValueError("k_out must have k's shape and type")
-        so, ko = self._target(q_out, "q_out")[3], self._target(k_out, "k_out")[3]
-        a.inverse, a.out_fp32, a.q_out_rows, a.pool_rows = bool(inverse), wide, n, n
-        a.q_out, a.qo_tok_stride, a.qo_head_stride = q_out.data_ptr(), so[0], so[1]
-        a.k_out, a.ko_tok_stride, a.ko_head_stride = k_out.data_ptr(), ko[0], ko[1]
-        _call(self._lib, a, self.dev.index, "ea_hip_rotary")
+        else:
+            sk = self._target(k_out, "k_out")[3]
+        self._launch(n, hq, hk, wide, strides, axis_stride, bool(inverse), 0, so, sk, None, n, n,
+                     (q.data_ptr(), k.data_ptr(), 0, positions.data_ptr()), (0, 0, q_out.data_ptr(), k_out.data_ptr(), 0))
         return q_out, k_out
 
     def append(self, q, k, v, positions, dst_rows, k_pool, v_pool, *, q_rows=None, q_out=None, pos_offset: int = 0):
@@ -243,39 +257,34 @@ class Rotary:
         skipped) of the pools [pages, page_size, Hkv, head_dim], bf16. The rotated q goes to a new bf16
         tensor of q's shape, or to rows q_rows (int64; rows outside are skipped) of q_out (rows, Hq,
         head_dim). Returns it. Rows that no token names are not written; a row may be named once."""
-        import torch
-        a, _, n, hq, hk = self._args(q, k, v, positions)
+        n, hq, hk, wide, strides, axis_stride = self._args(q, k, v, positions)
         if not -1 << 31 <= pos_offset < 1 << 31:
             raise ValueError("pos_offset must fit 32 bits")
-        at, d, i64 = self.dev.index, self.head_dim, torch.int64
+        at, d, i64 = self._at, self.head_dim, self._i64
         shape = k_pool.shape
         for pool, name in ((k_pool, "k_pool"), (v_pool, "v_pool")):
-            if pool.dtype not in self._bits or not pool.is_cuda or pool.get_device() != at or not pool.is_contiguous():
+            if pool.dtype not in self._bits or pool.get_device() != at or not pool.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous bf16 (or int16) tensor on {self.dev}")
-            if pool.shape != shape:
-                raise ValueError("k_pool and v_pool must have one shape")
+        if v_pool.shape != shape:
+            raise ValueError("k_pool and v_pool must have one shape")
         if len(shape) != 4 or shape[2] != hk or shape[3] != d:
             raise ValueError(f"the pools must be (pages, page_size, {hk}, {d})")
         if q_out is None:
             if q_rows is not None:
                 raise ValueError("q_rows needs q_out")
-            q_out = torch.empty((n, hq, d), dtype=torch.bfloat16, device=self.dev)
+            q_out = q.new_empty((n, hq, d), dtype=self._bits[0])
             rows, so = n, (hq * d, d)
         else:
-            rows, ho, wide, so = self._target(q_out, "q_out")
+            rows, ho, w, so = self._target(q_out, "q_out")
             if q_rows is not None and q_out.data_ptr() == q.data_ptr():
                 raise ValueError("q_out must not be q when q_rows moves its rows")
-            if wide or ho != hq or (q_rows is None and rows < n):
+            if w or ho != hq or (q_rows is None and rows < n):
                 raise ValueError("q_out must be (rows, Hq, head_dim) bf16 (or int16), a row per token without q_rows")
-        a.dst_rows = _vec(dst_rows, "dst_rows", at, i64, n)
-        if q_rows is not None:
-            a.q_rows = _vec(q_rows, "q_rows", at, i64, n)
-        row = hk * d
-        a.pos_offset, a.q_out_rows, a.pool_rows = pos_offset, rows, shape[0] * shape[1]
-        a.q_out, a.qo_tok_stride, a.qo_head_stride = q_out.data_ptr(), so[0], so[1]
-        a.k_out, a.ko_tok_stride, a.ko_head_stride = k_pool.data_ptr(), row, d
-        a.v_out, a.vo_tok_stride, a.vo_head_stride = v_pool.data_ptr(), row, d
-        _call(self._lib, a, at, "ea_hip_rotary")
+        to = _vec(dst_rows, "dst_rows", at, i64, n)
+        self._launch(n, hq, hk, wide, strides, axis_stride, False, pos_offset, so, (hk * d, d), (hk * d, d), rows,
+                     shape[0] * shape[1], (q.data_ptr(), k.data_ptr(), v.data_ptr(), positions.data_ptr()),
+                     (0 if q_rows is None else _vec(q_rows, "q_rows", at, i64, n), to, q_out.data_ptr(), k_pool.data_ptr(),
+                      v_pool.data_ptr()))
         return q_out
 
 
