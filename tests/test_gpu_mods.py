@@ -467,3 +467,42 @@ def test_graph_replays(gpu):
         want, fl, _ = _run(dict(p, kv_len=kv), ab, mods)
         assert (fl == 0).all() and np.array_equal(got, want), i
     g.close()
+
+
+@pytest.mark.parametrize("name", ["docs", "alibi", "cap"])
+def test_more_items_than_blocks(gpu, name):
+    """Prefill steps whose row blocks outnumber the CUs: blocks take several, and the fp64 kernel's bits come
+    out, also from two steps in flight at once and from a captured step replayed after others."""
+    import torch
+    from exactattention_amd.graph import HipGraph
+    rng = np.random.default_rng(31)
+    p = _prob(rng, 1, 1300, 8, 8, 128, 1300, qscale=2.0)  # 8 x 41 row blocks
+    ab = default_alpha_bits(128)
+    m = _mods_of(name, rng, p)
+    want, fl, st = _run(p, ab, hip.ScoreMods(**m), kernel="decode")
+    assert (fl == 0).all() and st["mrow_kernel_rows"] == 8 * 1300
+    dps = [hip.DeviceProblem(p, "bf16", 0, "cuda:0", "prefill", mods=hip.ScoreMods(**m)) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in dps]
+    torch.cuda.synchronize()
+    for _ in range(2):
+        for dp, s in zip(dps, streams):
+            with torch.cuda.stream(s):
+                dp.out.fill_(-1)
+                hip.launch_hip(dp, ab)
+    torch.cuda.synchronize()
+    for dp in dps:
+        assert np.array_equal(dp.out.cpu().numpy().view(np.uint16), want) and not bool(dp.flags.any())
+        assert dp.stats.tolist()[10] == 2 * 8 * 1300
+    dp, g = dps[0], HipGraph()
+    with torch.cuda.stream(streams[0]):
+        g.capture(streams[0], lambda: hip.launch_hip(dp, ab))
+    for _ in range(3):
+        dp.out.fill_(-1)
+        dp.flags.fill_(9)
+        hip.launch_hip(dps[1], ab)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(streams[0]):
+            g.replay(streams[0])
+        torch.cuda.synchronize()
+        assert np.array_equal(dp.out.cpu().numpy().view(np.uint16), want) and not bool(dp.flags.any())
+    g.close()
