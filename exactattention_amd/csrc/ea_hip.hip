@@ -1419,16 +1419,15 @@ int prefill_splits(int64_t blocks, int nt, int splits) {
 // slicing 0.4 us per 1000 keys of a segment, against 16 us per million pairs (10 with heads of up to 64
 // dims). The shorter of the two estimates (us) decides.
 // On 189 steps of 16 to 2500 tokens, 1 to 4 sequences, 2 to 32 heads, 16 to 12000 keys, d = 96 and 128, with and
-// without a cap, on normal values, the choice was within 12% of the faster kernel in all but one (19%
-// there). Scores twice as wide move the bases more often: 10 to 40% more here, 0 to 8% there, and the
-// choice within 32%. Prefill against multi-row kernel, us: 16/8 heads, 64 x 64 keys 41 / 20, 256 x 256 54 / 41,
-// 700 x 700 83 / 161, 128 x 3000 122 / 117, 256 x 3000 128 / 191, 2500 x 2500 426 / 932; 8/2 heads, 64 x 12000
-// 127 / 125, 256 x 12000 202 / 332; d = 96, 4/4 heads, 256 x 4000 139 / 75; d = 64, 16/8 heads, 256 x 256 55 / 34,
-// 256 x 4000 149 / 152, 2500 x 2500 430 / 576; with a bias 16/8 heads 2500 x 2500 674 / 967, d = 64, 16/4 heads, two
-// sequences of 777 x 777 265 / 165.
+// without a cap, on normal values, the choice was within 12% of the faster kernel in all. Scores twice
+// as wide move the bases more often: 10 to 40% more here, 0 to 8% there, and the choice within 28%. Prefill
+// against multi-row kernel, us: 16/8 heads, 64 x 64 keys 38 / 21, 256 x 256 50 / 41, 700 x 700 77 / 157, 128 x 3000 119 /
+// 116, 256 x 3000 123 / 187, 2500 x 2500 411 / 930; 8/2 heads, 64 x 12000 124 / 123, 256 x 12000 200 / 330; d = 96, 4/4
+// heads, 256 x 4000 138 / 76; d = 64, 16/8 heads, 256 x 256 51 / 33, 256 x 4000 145 / 149, 2500 x 2500 407 / 573; with a
+// bias 16/8 heads 2500 x 2500 648 / 962, d = 64, 16/4 heads, two sequences of 777 x 777 257 / 167.
 // An fp32 output under a bias: the int32 sums' last bits, which the far keys' small weights lose, then
 // flag one row in 8 for tier 2, and the fp64 sums of the other kernel one in 40 to 350: 16/8 heads, 700 x 700
-// 364 / 193, 2500 x 2500 2456 / 1387, within a window of 100 562 / 282. (Without a bias 127 / 226 and 639 / 2516,
+// 361 / 191, 2500 x 2500 2422 / 1382, within a window of 100 560 / 278. (Without a bias 127 / 226 and 639 / 2516,
 // one row in 250 against one in 13.)
 bool prefill_mods(const ea_geometry* g, const ea_options* o, const ea_score_mods* m, int span, int* ntiles, int* nrb) {
     const int grp = g->num_q_heads / g->num_kv_heads;
