@@ -192,12 +192,9 @@ __global__ void __launch_bounds__(MR_THREADS, (mr_waves<RS, DK>())) ea_mrow(Para
             if constexpr (MOD) {
                 const int kvb = vis_begin(P, tok, kvl);
                 kbmax = kvb;
-                if (kvb < min(kvl, slen)) kbeg = kvb;
-                else kend = 0;
-                if (tmk) {
-                    kbeg = min(kbeg, tb + (int)__builtin_ctzll(tmk));
-                    kend = max(kend, tb + 64 - (int)__clzll(tmk));
-                }
+                const KeySpan ks = key_span(kvb, kvl, slen, tmk, tb);
+                kbeg = ks.beg;
+                kend = ks.end;
                 if (w == 0 && lane < RS) {
                     S.kvb[r] = kvb;
                     S.pos[r] = mod_pos(P, tok, kvl);

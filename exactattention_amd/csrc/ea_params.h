@@ -5,6 +5,7 @@
 
 #include "../../include/exactattn_hip.h"
 #include "ea_device.h"
+#include "ea_keys.h"
 #include "ea_mod.h"
 
 namespace ea {
@@ -176,16 +177,10 @@ __device__ inline int2 unit_keys(const Params& P, int seg, int rbk) {
     const int t1 = (row0 + nrow - 1) / P.grp;
     for (int t = row0 / P.grp; t <= t1; ++t) {
         const int64_t tok = (int64_t)b * P.g.num_tokens + t;
-        const int e = min(P.kv_len[tok], slen), g = vis_begin(P, tok, P.kv_len[tok]);
-        if (g < e) {
-            kbeg = min(kbeg, g);
-            kend = max(kend, e);
-        }
-        const uint64_t m = P.tree_mask ? P.tree_mask[tok] : 0ull;
-        if (m && tb + (int)__builtin_ctzll(m) < slen) {
-            kbeg = min(kbeg, tb + (int)__builtin_ctzll(m));
-            kend = max(kend, min(tb + 64 - (int)__clzll(m), slen));
-        }
+        const int kvl = P.kv_len[tok];
+        const KeySpan k = key_span(vis_begin(P, tok, kvl), kvl, slen, P.tree_mask ? P.tree_mask[tok] : 0ull, tb);
+        kbeg = min(kbeg, k.beg);
+        kend = max(kend, k.end);
     }
     return kend > 0 ? make_int2(kbeg, kend) : make_int2(0, 0);
 }
@@ -212,53 +207,6 @@ __device__ __forceinline__ bool visible(const Params& P, int64_t tok, int64_t b,
         if (i >= 0 && i < 64) return (P.tree_mask[tok] >> i) & 1;
     }
     return false;
-}
-
-// The visible keys of a query token, the set every tier attends: the prefix n < Lc with
-// Lc = min(kv_len, seq_len) (0 when kv_len < 0), and the tree keys tree_base + i (bit i of the tree
-// mask) at or past Lc and below seq_len, so a key in both counts once. vis_tree_bits keeps those
-// tree bits; the prefix clip is the caller's. Host and device.
-__host__ __device__ inline uint64_t vis_tree_bits(uint64_t mask, int64_t tb, int64_t Lc, int64_t slen) {
-    int64_t lo = Lc - tb, hi = slen - tb;  // keep bits i with lo <= i < hi
-    lo = lo < 0 ? 0 : (lo > 64 ? 64 : lo);
-    hi = hi < 0 ? 0 : (hi > 64 ? 64 : hi);
-    if (hi <= lo) return 0;
-    const uint64_t below_hi = hi >= 64 ? ~0ull : ((1ull << hi) - 1);
-    const uint64_t below_lo = lo >= 64 ? ~0ull : ((1ull << lo) - 1);
-    return mask & below_hi & ~below_lo;
-}
-__host__ __device__ inline int64_t vis_prefix(int64_t kv_len, int64_t slen) {
-    return kv_len < 0 ? 0 : (kv_len < slen ? kv_len : slen);
-}
-
-// A row's visible keys, listed: the prefix [begin, begin + npre), then the tree keys outside it in
-// bit order. With MOD false begin is 0.
-struct RowKeys {
-    int64_t begin, npre, tb;
-    uint64_t mask;
-    __host__ __device__ int64_t count() const { return npre + __builtin_popcountll(mask); }
-    __host__ __device__ int64_t key(int64_t j) const {
-        if (j < npre) return begin + j;
-        uint64_t m = mask;
-        for (int64_t c = j - npre; c > 0; --c) m &= m - 1;
-        return tb + __builtin_ctzll(m);
-    }
-};
-// kv_begin: the row's first prefix key (vis_begin). Tree keys below it count as tree keys.
-__host__ __device__ inline RowKeys row_keys(int64_t kv_begin, int64_t kv_len, int64_t slen, uint64_t mask, int64_t tb) {
-    RowKeys r;
-    const int64_t L = vis_prefix(kv_len, slen);
-    r.begin = kv_begin < L ? kv_begin : L;
-    r.npre = L - r.begin;
-    r.tb = tb;
-    r.mask = vis_tree_bits(mask, tb, r.begin == 0 || r.npre > 0 ? L : 0, slen);
-    if (r.begin > 0 && r.npre > 0) {
-        // the bits below the prefix too: those of keys under begin
-        const int64_t hi = r.begin - tb;
-        const uint64_t below = hi <= 0 ? 0ull : (hi >= 64 ? ~0ull : ((1ull << hi) - 1));
-        r.mask |= vis_tree_bits(mask, tb, 0, slen) & below;
-    }
-    return r;
 }
 
 // end of the visible key range of a query token

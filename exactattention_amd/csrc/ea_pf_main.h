@@ -197,12 +197,9 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params A) {
         mpos = mod_pos(P, tok, kvl);
         mslope = mod_slope(P, hk * P.grp + lrc % P.grp);
         kbmax = wave_max_i(rvalid ? kvb : 0);
-        if (kvb < min(kvl, slen)) vb = kvb;
-        else ve = 0;
-        if (tmk) {
-            vb = min(vb, tbase + (int)__builtin_ctzll(tmk));
-            ve = max(ve, min(tbase + 64 - (int)__clzll(tmk), slen));
-        }
+        const KeySpan ks = key_span(kvb, kvl, slen, tmk, tbase);
+        vb = ks.beg;
+        ve = ks.end;
     }
     __syncthreads();  // s_kend initialised
     {

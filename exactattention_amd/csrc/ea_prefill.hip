@@ -273,10 +273,9 @@ __global__ void __launch_bounds__(256) ea_pf_kvslice(Params P) {
         int first = INT_MAX;
         for (int t = tid; t < P.g.num_tokens; t += 256) {
             const int64_t tok = b * P.g.num_tokens + t;
-            const int g = vis_begin(P, tok, P.kv_len[tok]);
-            if (g < min(P.kv_len[tok], P.seq_len[b])) first = min(first, g);
-            const uint64_t m = P.tree_mask ? P.tree_mask[tok] : 0ull;
-            if (m) first = min(first, P.tree_base[b] + (int)__builtin_ctzll(m));
+            const int kvl = P.kv_len[tok];
+            first = min(first, key_span(vis_begin(P, tok, kvl), kvl, P.seq_len[b], P.tree_mask ? P.tree_mask[tok] : 0ull,
+                                        P.tree_mask ? P.tree_base[b] : 0).beg);
         }
         if (!__syncthreads_or(first < 64 * (tile + 1))) return;
     }
