@@ -1827,12 +1827,16 @@ int ea_hip_step_route(const ea_geometry* g, const ea_buffers* bf, const ea_optio
     return 0;
 }
 
-int ea_hip_reads_kv_digits(const ea_geometry* g, const ea_options* o, int32_t* reads) {
+int ea_hip_mods_reads_kv_digits(const ea_geometry* g, const ea_options* o, const ea_score_mods* m, int32_t* reads) {
     Plan pl;
-    int rc = make_plan(g, o, &pl);
+    int rc = make_plan(g, o, &pl, m);
     if (rc) return rc;
-    if (reads) *reads = (pl.prefill && o->kv_digits) ? 1 : 0;  // the test ea_hip_attention makes
+    if (reads) *reads = (pl.prefill && o->kv_digits) ? 1 : 0;  // the test attention_impl makes
     return 0;
+}
+
+int ea_hip_reads_kv_digits(const ea_geometry* g, const ea_options* o, int32_t* reads) {
+    return ea_hip_mods_reads_kv_digits(g, o, nullptr, reads);
 }
 
 static int attention_impl(const ea_geometry* g, const ea_buffers* bf, const ea_options* o, const ea_score_mods* m,

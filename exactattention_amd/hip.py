@@ -139,7 +139,9 @@ def load():
         lib.ea_hip_attention_mods.argtypes = [G, B, O, M, P, ctypes.c_size_t, P]
         lib.ea_hip_exact_rows_mods.argtypes = [G, B, O, M, P]
         lib.ea_hip_kat_mod_logit.argtypes = [ctypes.c_int64, P, P, P, ctypes.c_float, P, P, P]
-        for f in (lib.ea_hip_mods_workspace_size, lib.ea_hip_attention_mods, lib.ea_hip_exact_rows_mods, lib.ea_hip_kat_mod_logit):
+        lib.ea_hip_mods_reads_kv_digits.argtypes = [G, O, M, ctypes.POINTER(ctypes.c_int32)]
+        for f in (lib.ea_hip_mods_workspace_size, lib.ea_hip_attention_mods, lib.ea_hip_exact_rows_mods, lib.ea_hip_kat_mod_logit,
+                  lib.ea_hip_mods_reads_kv_digits):
             f.restype = ctypes.c_int
         lib.ea_hip_step_plan.argtypes = [ctypes.POINTER(StepPlanArgs), P]
         lib.ea_hip_step_plan.restype = ctypes.c_int

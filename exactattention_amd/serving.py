@@ -14,7 +14,7 @@ management to that script. Here the cache lives on the device:
     instead of slicing the whole prefix again. They are re-sliced lazily: an append or a truncation
     only marks the slot's tiles stale from its first changed key, and the stale tiles of every slot
     are re-sliced in one update right before a call that reads the cache (the library says which
-    calls do: ea_hip_reads_kv_digits). Decode steps, which read the bf16 cache, slice nothing.
+    calls do: ea_hip_mods_reads_kv_digits). Decode steps, which read the bf16 cache, slice nothing.
 
 Every call enqueues on torch's current stream and copies its result to the host (the caller sees
 (out bits, flags) like the reference's backends).
@@ -475,6 +475,7 @@ class ExactAttentionBackend:
             if tree_mask is not None:
                 tm, tb = dv[2], dv[3]
         o = hip.Options(alpha_bits=self.alpha_bits, out_fp32=int(self.out == "fp32"), splits=0, tier2=1)
+        m = None if self.mods is None else self._step_mods(kv_begin)
         if digits_slot is not None and c.digits is not None:
             o.kv_digits = ctypes.c_void_p(c._digit_base(digits_slot))
             o.kv_digits_tiles = c.tiles
@@ -483,12 +484,11 @@ class ExactAttentionBackend:
                 o.kv_digits = ctypes.c_void_p(c.digits.data_ptr())
                 o.kv_digits_slot = staged[2].data_ptr()
             reads = ctypes.c_int32(0)
-            hip._check(lib.ea_hip_reads_kv_digits(ctypes.byref(gc), ctypes.byref(o), ctypes.byref(reads)),
-                       "ea_hip_reads_kv_digits")
+            hip._check(lib.ea_hip_mods_reads_kv_digits(ctypes.byref(gc), ctypes.byref(o), None if m is None else ctypes.byref(m),
+                                                       ctypes.byref(reads)), "ea_hip_mods_reads_kv_digits")
             if reads.value:
                 c.flush(stream)  # the stale tiles, re-sliced ahead of the call in stream order
         nb, ns = ctypes.c_size_t(0), ctypes.c_int32(0)
-        m = None if self.mods is None else self._step_mods(kv_begin)
         if m is None:
             hip._check(lib.ea_hip_workspace_size(ctypes.byref(gc), ctypes.byref(o), ctypes.byref(nb), ctypes.byref(ns)),
                        "ea_hip_workspace_size")

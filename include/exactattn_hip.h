@@ -236,10 +236,12 @@ typedef struct ea_score_mods {
     int32_t pad0;
 } ea_score_mods;
 
-/* ea_hip_attention, ea_hip_workspace_size and ea_hip_exact_rows with score modifications (m NULL: without).
- * Same buffers, options, workspace rules and return codes; -2 also for a negative window or max_span, a
- * softcap that is negative, subnormal or not finite, and o->timers. o->prefill_waves is not read: the
- * 8-wave block runs. Steps that ea_hip_attention gives the d = 128 decode kernel run on the multi-row kernel.
+/* ea_hip_attention, ea_hip_workspace_size, ea_hip_reads_kv_digits and ea_hip_exact_rows with score modifications
+ * (m NULL: without). Same buffers, options, workspace rules and return codes; -2 also for a negative window or
+ * max_span, a softcap that is negative, subnormal or not finite, and o->timers. o->prefill_waves is not read: the
+ * 8-wave block runs. Steps that ea_hip_attention gives the d = 128 decode kernel run on the multi-row kernel, and
+ * which steps take the int8 prefill path depends on the modifications and on o->kv_digits being set: ask for the
+ * workspace and for the reads with the options of the call.
  * Reference counterpart: none (the reference's masks are key lists, src/exactattn/cpu.py:70-109). */
 int ea_hip_mods_workspace_size(const ea_geometry* g, const ea_options* o, const ea_score_mods* m, size_t* bytes,
                                int32_t* nsplit);
@@ -247,6 +249,7 @@ int ea_hip_attention_mods(const ea_geometry* g, const ea_buffers* b, const ea_op
                           void* workspace, size_t workspace_bytes, ea_stream_t stream);
 int ea_hip_exact_rows_mods(const ea_geometry* g, const ea_buffers* b, const ea_options* o, const ea_score_mods* m,
                            ea_stream_t stream);
+int ea_hip_mods_reads_kv_digits(const ea_geometry* g, const ea_options* o, const ea_score_mods* m, int32_t* reads);
 
 /* The host exact tier on one row of host arrays: q (d), k (n x d), v (n x dv) bf16 bits, alpha as
  * fp32 bits -> out (dv bf16 or fp32 bits). t_bits, w_m, w_e (optional, n entries each) receive
