@@ -176,10 +176,14 @@ def _stream_ptr(torch):
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-def workspace_size(g: dict, splits: int = 0, out_fp32: bool = False, kernel: int = 0, mods=None) -> tuple[int, int]:
-    """Bytes and splits of a step; mods: the ScoreModsArgs of one with score modifications."""
+def workspace_size(g: dict, splits: int = 0, out_fp32: bool = False, kernel: int = 0, mods=None,
+                   kv_digits: bool = False) -> tuple[int, int]:
+    """Bytes and splits of a step; mods: the ScoreModsArgs of one with score modifications; kv_digits: of a
+    step that is given a digit-tile cache."""
     lib = load()
     o = Options(splits=splits, out_fp32=int(out_fp32), tier2=1, kernel=kernel)
+    if kv_digits:  # set, and large enough: the size depends on nothing else of it
+        o.kv_digits, o.kv_digits_tiles = 1, 0x7FFFFFFF
     nb, ns = ctypes.c_size_t(0), ctypes.c_int32(0)
     if mods is None:
         _check(lib.ea_hip_workspace_size(ctypes.byref(geometry(g)), ctypes.byref(o), ctypes.byref(nb), ctypes.byref(ns)),
@@ -289,6 +293,9 @@ class DeviceProblem:
         self.flags = torch.empty(rows, dtype=torch.uint8, device=dev)
         self.mods, self._mods_keep = (None, None) if mods is None else mods.bind(self.geom, dev)
         nb, self.nsplit = workspace_size(self.geom, splits, self.out_fp32, self.kernel, self.mods)
+        if self.mods is not None and self.geom["head_dim"] == self.geom["head_dim_v"] == 128:
+            # a launch with a digit-tile cache may take another kernel
+            nb = max(nb, workspace_size(self.geom, splits, self.out_fp32, self.kernel, self.mods, True)[0])
         self.workspace = torch.empty(max(nb, 256), dtype=torch.uint8, device=dev)
         self.ws_bytes = nb
         self.stats = torch.zeros(len(STATS), dtype=torch.int64, device=dev)

@@ -46,3 +46,28 @@ def test_tiles_are_sliced_for_the_steps_that_read_them(gpu):
     be.check_flags(fl)
     assert c.stale[s] == 0
     assert np.array_equal(out.cpu().numpy().view(np.uint32), _general(q, k, v, 1 + np.arange(S), mods, "fp32"))
+
+
+def test_problem_with_a_digit_cache_and_modifications(gpu):
+    """A problem whose launch with a digit cache takes the int8 kernel and without one the multi-row kernel:
+    both run, and the bits are the same."""
+    import torch
+    rng = np.random.default_rng(2)
+    B, T, Hq, Hkv, d, S = 2, 96, 16, 8, 128, 2000
+    ab = default_alpha_bits(d)
+    p = problem.contiguous(bf16(rng, (B, T, Hq, d), "normal", 2.0), bf16(rng, (B, Hkv, S, d)), bf16(rng, (B, Hkv, S, d)),
+                           np.broadcast_to(S - T + 1 + np.arange(T), (B, T)))
+    dp = hip.DeviceProblem(p, mods=hip.ScoreMods(softcap=20.0))
+    dig = hip.KVDigits(dp, (S + 63) // 64)
+    at = [torch.full((B,), n, dtype=torch.int32, device="cuda") for n in (0, S)]
+    dig.update(dp, *at, S)
+    got = []
+    for kw in ({}, {"kv_digits": dig}):
+        dp.out.fill_(-1)
+        dp.stats.zero_()
+        hip.launch_hip(dp, ab, **kw)
+        torch.cuda.synchronize()
+        got.append((dp.out.cpu().numpy(), dict(zip(hip.STATS, dp.stats.tolist()))))
+        assert not bool(dp.flags.any())
+    assert got[0][1]["mrow_kernel_rows"] == got[1][1]["prefill_kernel_rows"] == B * T * Hq
+    assert np.array_equal(got[0][0], got[1][0])

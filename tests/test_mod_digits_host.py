@@ -56,3 +56,19 @@ def test_reads_without_modifications():
 def test_reads_refused():
     assert _reads(_geom(64, 64), hip.ScoreModsArgs(window=-1))[0] == -2
     assert _reads(_geom(64, 64), hip.ScoreModsArgs(), splits=-1)[0] == -2
+
+
+@pytest.mark.parametrize("geom", [(96, 2000, 2, 16, 8), (33, 16000, 2, 16, 8)])
+def test_workspace_holds_a_step_with_digits(geom):
+    """The estimate that picks the kernel leaves slicing out where a digit cache is given: a problem's workspace
+    is enough for its launches with one and without."""
+    T, S, B, Hq, Hkv = geom
+    g = _geom(T, S, B, Hq, Hkv)
+    spec = hip.ScoreMods(softcap=20.0)
+    a, _ = spec.bind(g, "cpu")
+    without, with_ = (hip.workspace_size(g, mods=a, kv_digits=x)[0] for x in (False, True))
+    assert _reads(g, a) == (0, 1) and with_ > without  # the choice differs here
+    prob = dict(geom=g, out_shape=(B, T, Hq, 128), q=np.zeros((B, T, Hq, 128), np.uint16))
+    dp = hip.DeviceProblem(prob, device="cpu", mods=spec)
+    assert dp.ws_bytes >= max(without, with_) and dp.workspace.numel() >= dp.ws_bytes
+    assert hip.DeviceProblem(prob, device="cpu").ws_bytes == hip.workspace_size(g)[0]
