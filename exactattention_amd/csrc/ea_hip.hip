@@ -1530,7 +1530,7 @@ void choose_splits_mrow(const Plan& pl, Tier1& mr, int maxlen, int dv, int split
 // path's, the prefill path's. When tier 2 runs, tier 1 and the prefill path are done with theirs, so
 // its double-double pass keeps the list of the rows it leaves (Params::t2left) and its chunk partials
 // there. The partials may reach into the 128-bit path's arrays: that path starts after the pass.
-size_t lay_out(Plan* pl, const ea_geometry* g, const ea_options* o, bool mrow) {
+size_t lay_out(Plan* pl, const ea_geometry* g, const ea_options* o, bool mrow, bool mods) {
     const int64_t R = pl->rows;
     const int dv = g->head_dim_v;
     size_t off = 0;
@@ -1570,7 +1570,8 @@ size_t lay_out(Plan* pl, const ea_geometry* g, const ea_options* o, bool mrow) {
         pl->off_pfqm = take((size_t)R * sizeof(PfQMeta));
         // with a digit cache of the caller's there is nothing to slice into the workspace
         if (!o->kv_digits) pl->off_pfkv = take((size_t)pl->nseg * pl->pf_ntiles * EA_PF_TILE_BYTES);
-        pl->off_pfscr = take((size_t)pl->nseg * pl->pf_nrb * pl->pf_nsplit * 512 * 32 * 8);
+        // modified steps keep the sums of their epochs in registers
+        pl->off_pfscr = take(mods ? 0 : (size_t)pl->nseg * pl->pf_nrb * pl->pf_nsplit * 512 * 32 * 8);
         pl->off_pfpart = take(pl->pf_nsplit > 1 ? (size_t)pl->pf_nsplit * R * (sizeof(PfPart) + 128 * 16) : 0);
     }
     pl->off_dd = align_up(pl->off_front + (size_t)R * 4);  // past Params::t2left
@@ -1656,7 +1657,7 @@ int make_plan(const ea_geometry* g, const ea_options* o, Plan* pl, const ea_scor
     Tier1& mr = pl->mr;
     mr.rb = m && pl->prefill ? 0 : mrow_rows(g, o, pl->r_seg, m != nullptr);
     pl->mrow = mr.rb > 0;
-    const size_t without = lay_out(pl, g, o, false);
+    const size_t without = lay_out(pl, g, o, false, m != nullptr);
     if (!pl->mrow) return 0;
     mr.nrb = (pl->r_seg + mr.rb - 1) / mr.rb;
     choose_splits_mrow(*pl, mr, span, g->head_dim_v, o->splits);
@@ -1679,7 +1680,7 @@ int make_plan(const ea_geometry* g, const ea_options* o, Plan* pl, const ea_scor
     // equal-share plan. With as many partials as the other kernel and no plan it needs less: no q.
     const size_t cap = EA_NOALLOC_SCRATCH_BYTES;
     const Tier1 first = mr;
-    while (lay_out(pl, g, o, true) > cap && without <= cap) {
+    while (lay_out(pl, g, o, true, m != nullptr) > cap && without <= cap) {
         if (o->splits == 0 && mr.nsplit > 1) {
             split_tiles(span, mr.nsplit / 2, &mr.nsplit, &mr.split_len);
         } else if (mr.dq) {

@@ -77,7 +77,8 @@ struct Params {
     uint8_t* pfq;     // rows * 512: q digit planes
     void* pfqm;       // rows * sizeof(PfQMeta)
     uint8_t* pfkv;    // nseg * pf_ntiles * EA_PF_TILE_BYTES: K/V digit tiles and tile metadata
-    double* pfscr;    // nseg * pf_nrb * 512 lanes * 32: per-lane sums of completed epochs
+    // nseg * pf_nrb * pf_nsplit * 512 lanes * 32: per-lane sums of completed epochs (not of modified steps)
+    double* pfscr;
     int32_t pf_ntiles;  // 64-key tiles per segment
     int32_t pf_nrb;     // 32-row blocks per segment
     // digit-tile cache (ea_hip_kv_digits_update): with kvd_begin set, ea_pf_kvslice re-slices the

@@ -72,3 +72,16 @@ def test_workspace_holds_a_step_with_digits(geom):
     dp = hip.DeviceProblem(prob, device="cpu", mods=spec)
     assert dp.ws_bytes >= max(without, with_) and dp.workspace.numel() >= dp.ws_bytes
     assert hip.DeviceProblem(prob, device="cpu").ws_bytes == hip.workspace_size(g)[0]
+
+
+def test_modified_prompts_keep_no_epoch_sums():
+    """A plain int8 step keeps 128 KB of epoch sums per row block and key split; a modified one keeps its own in
+    registers and asks for that much less."""
+    for T, S, B in ((4096, 4096, 1), (2500, 2500, 1), (700, 700, 3)):
+        g = _geom(T, S, B)
+        m = hip.ScoreModsArgs(softcap_bits=0x41A00000)
+        assert _reads(g, m) == (0, 1)
+        plain, splits = hip.workspace_size(g)
+        mods, other = hip.workspace_size(g, mods=m)
+        blocks = B * 8 * ((2 * T + 31) // 32)
+        assert splits == other and plain - mods >= blocks * splits * 512 * 32 * 8
