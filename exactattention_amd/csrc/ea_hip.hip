@@ -1170,7 +1170,7 @@ __device__ __forceinline__ int t2_left(const Params& P, int nact, int* slot_id) 
 // rows are listed; then the rows that stay undecided in 128-bit arithmetic. Measured: the 70 rows
 // that a 2048-row causal head in fp32 leaves, 840 -> 66 us; one
 // 4096-key bf16 row after a prefill step 116 -> 35 us; an empty list 4.6 us (3.8 at least)
-// in the trace, as without the pass; 512 blocks cost a C2 step 1.8 us, so bf16 steps, which list few rows,
+// in the trace, as without the pass; 512 blocks cost a C2 step 1.8 us, so bf16 steps of few rows, which list few,
 // launch 32. The pass itself is 1.5 us slower (64.8 -> 66.3) for the 128-bit path's registers beside it.
 template <bool MOD>
 __global__ void __launch_bounds__(EA_T2_THREADS) ea_tier2(Params P) {
@@ -1780,8 +1780,11 @@ int list_all(const Params& P, const ea_options* o, unsigned blocks, hipStream_t 
 
 // tier 2 on the listed rows
 void tier2(const Params& P, const ea_options* o, hipStream_t st) {
-    // 512 blocks cost an empty list 2 us, and a long one is shorter by the CUs it fills: steps that may list many
-    // rows (2500 capped tokens of 16 heads, the step: 827 rows listed 3411 -> 995 us)
+    // A long list is shorter by the CUs that 512 blocks fill, and an empty one costs a step 0.3 to 0.5 us more (8192
+    // rows: 256 sequences of 32 heads on 128 keys 82.1 -> 82.5 us a step, 500 keys 152.4 -> 152.9): steps that may
+    // list many rows take them, with modifications or without. 32 -> 512 blocks, us a step: 512 tokens of 16 heads,
+    // scores four times as wide, 72 rows listed 183 -> 137; 2500 such tokens, 1095 listed 4264 -> 1099; 2500
+    // capped ones, 827 listed 3411 -> 995.
     const dim3 grid(o->force_tier2 ? EA_T2_BLOCKS : EA_DD_BLOCKS(P.out_fp32 || P.rows >= 8192)), blk(EA_T2_THREADS);
     if (o->force_tier2) {
         if (P.mods) hipLaunchKernelGGL(ea_tier2_wide<true>, grid, blk, 0, st, P);
