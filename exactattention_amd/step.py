@@ -60,6 +60,39 @@ def _call(fn, args: bytes, index: int, what: str) -> None:
         raise ValueError(f"{what}: error code {rc}")
 
 
+_TURN = None
+
+
+def _turn():
+    """The rotation as a differentiable function: its gradient is the rotation back (one launch)."""
+    global _TURN
+    if _TURN is None:
+        import torch
+
+        class Turn(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, q, k, positions, rotary, inverse):
+                ctx.save_for_backward(positions)
+                ctx.rotary, ctx.inverse = rotary, inverse
+                ctx.set_materialize_grads(False)
+                out = rotary.rotate(q, k, positions, inverse=inverse)
+                ctx.mark_non_differentiable(*(o for o, need in zip(out, ctx.needs_input_grad) if not need))
+                return out
+
+            @staticmethod
+            def backward(ctx, *grads):
+                have = [g is not None and need for g, need in zip(grads, ctx.needs_input_grad)]
+                if not any(have):
+                    return (None,) * 5
+                none = grads[have.index(True)][:, :0]  # no heads
+                gs = [(g if g.stride(2) == 1 else g.contiguous()) if h else none for g, h in zip(grads, have)]
+                out = ctx.rotary.rotate(*gs, *ctx.saved_tensors, inverse=not ctx.inverse)
+                return tuple(g if h else None for g, h in zip(out, have)) + (None,) * 3
+
+        _TURN = Turn.apply
+    return _TURN
+
+
 def _vec(t, name, index, dtype, n=None):
     """The address of a contiguous tensor of this type on this device (of n entries)."""
     if t.dtype is not dtype or t.get_device() != index or not t.is_contiguous():  # -1 on the host
@@ -232,7 +265,12 @@ class Rotary:
     def rotate(self, q, k, positions, *, inverse: bool = False, q_out=None, k_out=None):
         """q (tokens, Hq, head_dim) and k (tokens, Hkv, head_dim) turned by positions ((tokens,) or (axes,
         tokens) int32), into new tensors of their type or into q_out and k_out (which may be q and k
-        themselves). inverse turns back: the gradient of the rotation. Returns (q_out, k_out)."""
+        themselves). inverse turns back: the gradient of the rotation. Returns (q_out, k_out). Gradients of q
+        and k pass through, with q_out and k_out not given."""
+        if (q.requires_grad or k.requires_grad) and _C.is_grad_enabled():
+            if q_out is not None or k_out is not None:
+                raise ValueError("q_out and k_out take no part in gradients: leave them out, or call under no_grad")
+            return _turn()(q, k, positions, self, bool(inverse))
         n, hq, hk, wide, strides, axis_stride = self._args(q, k, None, positions)
         d = self.head_dim
         if q_out is None:
@@ -256,7 +294,8 @@ class Rotary:
         head_dim) to rows dst_rows (int64, page * page_size + slot; rows outside the pool, such as -1, are
         skipped) of the pools [pages, page_size, Hkv, head_dim], bf16. The rotated q goes to a new bf16
         tensor of q's shape, or to rows q_rows (int64; rows outside are skipped) of q_out (rows, Hq,
-        head_dim). Returns it. Rows that no token names are not written; a row may be named once."""
+        head_dim). Returns it, without a gradient. Rows that no token names are not written; a row may be named
+        once."""
         n, hq, hk, wide, strides, axis_stride = self._args(q, k, v, positions)
         if not -1 << 31 <= pos_offset < 1 << 31:
             raise ValueError("pos_offset must fit 32 bits")
