@@ -93,6 +93,41 @@ def _turn():
     return _TURN
 
 
+class _At:
+    """Rows of memory as numpy sees an array, for its test of shared memory alone: nothing is read."""
+
+    def __init__(self, x, d):
+        ptr, n, h, st, sh, e = x
+        self.__array_interface__ = dict(data=(ptr, True), shape=(n, h, d * e), strides=(st * e, sh * e, 1), typestr="|u1", version=3)
+
+
+def _apart(x, y, d: int) -> bool:
+    """Whether two sets of rows of d elements, each (address, tokens, heads, their strides in elements, bytes an
+    element), have no byte in common."""
+    px, n, h, sx, hx, ex = x
+    py, m, g, sy, hy, ey = y
+    sx, sy, wx, wy = sx * ex, sy * ey, ((h - 1) * hx + d) * ex, ((g - 1) * hy + d) * ey
+    if px + (n - 1) * sx + wx <= py or py + (m - 1) * sy + wy <= px:
+        return True
+    if not (n and h and m and g):
+        return True
+    # views of one tensor, such as a fused projection: side by side within a token, or within a head's row
+    if sx == sy > 0 and wx <= (py - px) % sx <= sx - wy:
+        return True
+    hx, hy = hx * ex, hy * ey
+    if hx == hy > 0 and sx % hx == 0 == sy % hx and d * ex <= (py - px) % hx <= hx - d * ey:
+        return True
+    try:
+        return not np.shares_memory(np.asarray(_At(x, d)), np.asarray(_At(y, d)), max_work=1 << 20)
+    except np.exceptions.TooHardError:
+        return False
+
+
+def _same(x, y) -> bool:
+    """Whether they are the same rows: the rotation may then be done in place."""
+    return x[0] == y[0] and x[5] == y[5] and (x[1] == 1 or x[3] == y[3]) and (x[2] == 1 or x[4] == y[4])
+
+
 def _vec(t, name, index, dtype, n=None):
     """The address of a contiguous tensor of this type on this device (of n entries)."""
     if t.dtype is not dtype or t.get_device() != index or not t.is_contiguous():  # -1 on the host
@@ -262,6 +297,16 @@ class Rotary:
                                      *(sv or (0, 0)), axis_stride, rows, pool, *inputs, self._half, self._axis, *outputs),
               self._at, "ea_hip_rotary")
 
+    def _check_memory(self, q, k, q_out, k_out):
+        """rotate's outputs (None: a new one) are their own input, or share no memory with the inputs and each other."""
+        d = self.head_dim
+        q_in, k_in = q_out is not None and _same(q_out, q), k_out is not None and _same(k_out, k)
+        if q_out and not ((q_in or _apart(q_out, q, d)) and _apart(q_out, k, d)):
+            raise ValueError("q_out shares memory with k, or with q without being q")
+        if k_out and not ((k_in or _apart(k_out, k, d)) and (q_in or _apart(k_out, q, d)) and
+                          (k_in or not q_out or _apart(q_out, k_out, d))):
+            raise ValueError("k_out shares memory with q or q_out, or with k without being k")
+
     def rotate(self, q, k, positions, *, inverse: bool = False, q_out=None, k_out=None):
         """q (tokens, Hq, head_dim) and k (tokens, Hkv, head_dim) turned by positions ((tokens,) or (axes,
         tokens) int32), into new tensors of their type or into q_out and k_out (which may be q and k
@@ -273,21 +318,42 @@ class Rotary:
             return _turn()(q, k, positions, self, bool(inverse))
         n, hq, hk, wide, strides, axis_stride = self._args(q, k, None, positions)
         d = self.head_dim
-        if q_out is None:
+        given = q_out is not None, k_out is not None
+        if not given[0]:
             q_out, so = q.new_empty((n, hq, d)), (hq * d, d)
         elif q_out.shape != q.shape or q_out.dtype != q.dtype:
             raise ValueError("q_out must have q's shape and type")
         else:
             so = self._target(q_out, "q_out")[3]
-        if k_out is None:
+        if not given[1]:
             k_out, sk = k.new_empty((n, hk, d)), (hk * d, d)
         elif k_out.shape != k.shape or k_out.dtype != k.dtype:
             raise ValueError("k_out must have k's shape and type")
         else:
             sk = self._target(k_out, "k_out")[3]
+        qp, kp, to_q, to_k = q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr()
+        if True in given:
+            e = 4 if wide else 2
+            self._check_memory((qp, n, hq, strides[0], strides[1], e), (kp, n, hk, strides[2], strides[3], e),
+                               (to_q, n, hq, so[0], so[1], e) if given[0] else None,
+                               (to_k, n, hk, sk[0], sk[1], e) if given[1] else None)
         self._launch(n, hq, hk, wide, strides, axis_stride, bool(inverse), 0, so, sk, None, n, n,
-                     (q.data_ptr(), k.data_ptr(), 0, positions.data_ptr()), (0, 0, q_out.data_ptr(), k_out.data_ptr(), 0))
+                     (qp, kp, 0, positions.data_ptr()), (0, 0, to_q, to_k, 0))
         return q_out, k_out
+
+    def _check_target(self, out, at, n, hk, e, st, in_place, pools, size):
+        """append's q_out is q (in_place: rows in q's order), or shares no memory with the inputs (at addresses `at`,
+        their strides one after another) and the pools of `size` bytes."""
+        d, lo, h = self.head_dim, out[0], out[2]
+        hi = lo + 2 * ((out[1] - 1) * out[3] + (h - 1) * out[4] + d)
+        for p in pools:
+            if p < hi and lo < p + size and out[1] and h:
+                raise ValueError("q_out shares memory with a pool")
+        for i, p in enumerate(at):
+            if p < hi:  # else past its end
+                x = (p, n, hk if i else h, st[2 * i], st[2 * i + 1], e)
+                if not _apart(out, x, d) and not (i == 0 and in_place and _same(out, x)):
+                    raise ValueError("q_out shares memory with k or v, or with q without being q in its own rows")
 
     def append(self, q, k, v, positions, dst_rows, k_pool, v_pool, *, q_rows=None, q_out=None, pos_offset: int = 0):
         """A step's tokens into the cache: q and k turned by positions (+ pos_offset), k and v (tokens, Hkv,
@@ -308,6 +374,10 @@ class Rotary:
             raise ValueError("k_pool and v_pool must have one shape")
         if len(shape) != 4 or shape[2] != hk or shape[3] != d:
             raise ValueError(f"the pools must be (pages, page_size, {hk}, {d})")
+        slots = shape[0] * shape[1]
+        qp, kp, vp, to_k, to_v = q.data_ptr(), k.data_ptr(), v.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr()
+        if abs(to_k - to_v) < 2 * slots * hk * d:
+            raise ValueError("k_pool and v_pool share memory")
         if q_out is None:
             if q_rows is not None:
                 raise ValueError("q_rows needs q_out")
@@ -315,15 +385,14 @@ class Rotary:
             rows, so = n, (hq * d, d)
         else:
             rows, ho, w, so = self._target(q_out, "q_out")
-            if q_rows is not None and q_out.data_ptr() == q.data_ptr():
-                raise ValueError("q_out must not be q when q_rows moves its rows")
             if w or ho != hq or (q_rows is None and rows < n):
                 raise ValueError("q_out must be (rows, Hq, head_dim) bf16 (or int16), a row per token without q_rows")
+            self._check_target((q_out.data_ptr(), n if q_rows is None else rows, hq, so[0], so[1], 2), (qp, kp, vp), n, hk,
+                               4 if wide else 2, strides, q_rows is None, (to_k, to_v), 2 * slots * hk * d)
         to = _vec(dst_rows, "dst_rows", at, i64, n)
-        self._launch(n, hq, hk, wide, strides, axis_stride, False, pos_offset, so, (hk * d, d), (hk * d, d), rows,
-                     shape[0] * shape[1], (q.data_ptr(), k.data_ptr(), v.data_ptr(), positions.data_ptr()),
-                     (0 if q_rows is None else _vec(q_rows, "q_rows", at, i64, n), to, q_out.data_ptr(), k_pool.data_ptr(),
-                      v_pool.data_ptr()))
+        self._launch(n, hq, hk, wide, strides, axis_stride, False, pos_offset, so, (hk * d, d), (hk * d, d), rows, slots,
+                     (qp, kp, vp, positions.data_ptr()),
+                     (0 if q_rows is None else _vec(q_rows, "q_rows", at, i64, n), to, q_out.data_ptr(), to_k, to_v))
         return q_out
 
 

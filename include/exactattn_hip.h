@@ -436,7 +436,8 @@ int ea_hip_step_plan(const ea_step_plan* p, ea_stream_t stream);
  *   element c of head g of token t:  q + t q_tok_stride + g q_head_stride + c, k and v alike
  *   outputs: row r of q_out is q_rows[t] (NULL: t), row r of k_out and v_out is dst_rows[t] (NULL: t);
  *   rows outside [0, q_out_rows) or [0, pool_rows) are skipped
- * v may be NULL (k alone). q_out may be q and k_out k where their strides and rows are the same.
+ * v may be NULL (k alone). q_out may be q and k_out k where their strides and rows are the same; otherwise the
+ * rows written share no memory with the inputs or each other.
  * half_turns: num pairs fp64, the frequencies divided by pi. head_dim up to 256, rot_dim even. All
  * pointers are device memory. Enqueue only, capturable. Returns 0, -1 on bad arguments, -2 on a bad type
  * or scale, -100 - e on a HIP error. No reference counterpart. */
