@@ -795,16 +795,22 @@ class ExactAttentionBackend:
         """Keep the accepted draft nodes `path` (node indices in draft order) after the prefix:
         the cache is cut back to the prefix and the path's K/V appended in order (with rotary positions k as
         verify_tree took it: it is turned again)."""
-        self.cache.truncate(s, prefix_len)
-        if len(path):
-            idx = np.asarray(path)
-            if self.rotary is None:
-                self.cache.append(s, np.asarray(k)[idx], np.asarray(v)[idx])
-            else:
-                torch = self.cache.torch
-                at = torch.from_numpy(idx.astype(np.int64)).to(self.cache.dev)
-                kk, vv = (_dev16(torch, x, self.cache.dev).index_select(0, at) for x in (k, v))
-                self._append([s], [len(idx)], None, kk, vv)
+        c = self.cache
+        idx = np.asarray(path, dtype=np.int64)
+        if not len(idx):
+            c.truncate(s, prefix_len)
+            return
+        n = min(len(k), len(v))
+        if idx.ndim != 1 or idx.min() < -n or idx.max() >= n:
+            raise IndexError(f"path must hold indices of the {n} nodes of k and v")
+        if self.rotary is None:
+            kk, vv = np.asarray(k)[idx], np.asarray(v)[idx]
+        else:
+            # a gather on the GPU does not check its indices, nor count back from the end
+            self._positions(None, len(idx))
+            kk, vv = (_dev16(c.torch, x, c.dev).index_select(0, c.torch.from_numpy(idx % len(x)).to(c.dev)) for x in (k, v))
+        c.truncate(s, prefix_len)
+        self._append([s], [len(idx)], None, kk, vv)
 
 
 def _batch(q, axis: int):
