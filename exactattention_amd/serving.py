@@ -771,6 +771,8 @@ class ExactAttentionBackend:
             raise ValueError("at most 64 draft nodes")
         if self.mods is not None and self.mods.slopes is not None:
             raise ValueError("tree verification has no distance bias")
+        if any(parents[i] >= i for i in range(N)):
+            raise ValueError("a node's parent comes before it")
         L = c.length[s]
         depth = np.zeros(N, dtype=np.int64)
         for i in range(N):
