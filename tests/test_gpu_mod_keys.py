@@ -100,3 +100,43 @@ def test_bits_that_name_no_key_in_shares(gpu):
     assert (fl == 0).all() and np.array_equal(res, other)
     for r in (0, B * Hq - 1):
         assert np.array_equal(res.reshape(-1, d)[r], _want(p, m, r))
+
+
+@pytest.mark.parametrize("d", [128, 72])
+def test_trees_and_intervals_on_the_prefill_kernel(gpu, d):
+    """Tree keys past the interval, inside it and before its first key, on the int8 kernel, against the definition."""
+    B, T, Hq, Hkv, S = 2, 34, 2, 1, 330
+    rng, p = _prob(9, B, T, Hq, Hkv, d, S, 16)
+    kv = rng.integers(0, S, (B, T)).astype(np.int32)
+    begin = np.maximum(kv - rng.integers(0, 150, (B, T)), 0).astype(np.int32)
+    begin[:, ::7] = S  # no prefix key: the tree's alone
+    p["kv_len"] = kv.reshape(-1)
+    p["tree_mask"] = rng.integers(1, 1 << 62, B * T, dtype=np.int64).astype(np.uint64)
+    p["tree_mask"][::6] = 0
+    p["tree_base"] = np.array([70, 250], np.int32)
+    m = dict(kv_begin=begin, slopes=np.array([0.5, 0.02], np.float32), q_pos=kv + 3, softcap=12.0)
+    for out in ("bf16", "fp32"):
+        dp, res, fl = _run(p, m, "prefill", out=out)
+        assert (fl == 0).all() and _stats(dp)["prefill_kernel_rows"] == B * T * Hq
+        for r in rng.permutation(B * T * Hq)[:30].tolist() + [0, 1, B * T * Hq - 1]:
+            assert np.array_equal(res.reshape(-1, d)[r], _want(p, m, r, out)), (out, r)
+
+
+@pytest.mark.parametrize("base", [3, 700, 1180])
+def test_tiles_between_a_tree_and_the_intervals(gpu, base):
+    """One token's tree far before, or past, the intervals of the others: its tiles count as seen, the slicing
+    leaves out those before every token's first key and no others."""
+    B, T, Hq, Hkv, d, S = 2, 200, 4, 2, 128, 1300
+    rng, p = _prob(base, B, T, Hq, Hkv, d, S, 16)
+    kv = np.asarray(p["kv_len"]).reshape(B, T)
+    p["tree_mask"] = np.zeros(B * T, np.uint64)
+    p["tree_mask"][[5, T + 199]] = np.array([1 << 63 | 1, 1 << 40], np.uint64)
+    p["tree_base"] = np.full(B, base, np.int32)
+    m = dict(kv_begin=np.maximum(kv - 90, 0).astype(np.int32), softcap=9.0)
+    dp, res, fl = _run(p, m, "prefill")
+    assert (fl == 0).all() and _stats(dp)["prefill_kernel_rows"] == B * T * Hq
+    for kernel in ("general", "decode"):
+        _, other, f2 = _run(p, m, kernel)
+        assert (f2 == 0).all() and np.array_equal(res, other), kernel
+    for r in (5 * Hq, 6 * Hq, B * T * Hq - 1):
+        assert np.array_equal(res.reshape(-1, d)[r], _want(p, m, r))
