@@ -621,20 +621,25 @@ class ExactAttentionBackend:
         if self.rotary is not None or positions is not None:
             return self._forward_planned(query, key, value, list(seqs), ql, self._positions(positions, ntok))
         prefix = [c.length[s] for s in seqs]
+        plan = c._plan_append(seqs, ql, key, value, checked=True)
+        lens = np.asarray([c.length[s] for s in seqs], dtype=np.int32)
+        mine = [lens, np.asarray(seqs, dtype=np.int64) * c.max_pages, np.asarray(seqs, dtype=np.int32)]
         runs = None
         if T > 1:
             if query.dim() == 3 and query.element_size() == 2 and query.device == c.k.device:
                 runs = _equal_runs(ql, Hq, d, max(prefix))
-            if runs is None:
-                return self._forward_planned(query, key, value, list(seqs), ql, None)
-        plan = c._plan_append(seqs, ql, key, value, checked=True)
-        lens = np.asarray([c.length[s] for s in seqs], dtype=np.int32)
-        mine = [lens, np.asarray(seqs, dtype=np.int64) * c.max_pages, np.asarray(seqs, dtype=np.int32)]
-        if T > 1:
             start = np.concatenate([[0], np.cumsum(ql)])
             b_of = np.repeat(np.arange(B), ql)
             j_of = np.arange(ntok) - start[b_of]
-            mine.append((np.asarray(prefix, dtype=np.int32)[b_of] + j_of + 1).astype(np.int32))
+            seen = np.asarray(prefix, dtype=np.int32)[b_of] + j_of + 1
+            if runs is not None:
+                mine.append(seen.astype(np.int32))
+            else:
+                # Planned here: the append's launch writes the block table too. On the device (_forward_planned) it
+                # is one launch more: 3 sequences of 2 and 3 tokens 159 -> 169 us a call, 12 of 1 to 64 239 -> 245
+                kvl_h = np.zeros(B * T, dtype=np.int32)
+                kvl_h[b_of * T + j_of] = seen
+                mine += [kvl_h, (b_of * T + j_of).astype(np.int64)]
         n_app = len(plan["arrays"])
         ts = torch.cuda.current_stream(c.dev)
         st = ctypes.c_void_p(ts.cuda_stream)
@@ -644,27 +649,33 @@ class ExactAttentionBackend:
         if runs is not None:
             return self._forward_runs(query, list(seqs), ql, runs, staged, dev[n_app + 3], st)
         # one token per sequence sees the whole sequence: its visible length is the sequence's
+        kvl = dev[n_app + 3] if T > 1 else dev[n_app]
+        row = dev[n_app + 4] if T > 1 else None
         q16 = query.view(torch.int16) if query.dtype != torch.int16 else query
-        qd = q16.reshape(B, 1, Hq, d).contiguous()
+        if T == 1:
+            qd = q16.reshape(B, 1, Hq, d).contiguous()
+        else:
+            qd = torch.zeros((B * T, Hq, d), dtype=torch.int16, device=c.dev)
+            qd.index_copy_(0, row, q16)
+            qd = qd.view(B, T, Hq, d)
         slots = list(seqs)
-        out, flags = self._launch(slots, qd, dev[n_app], digits_slot=slots[0], staged=staged, stream=st)
-        self._last["keep"] += (q16,)
-        ret = (out.view(B, Hq, -1), flags.view(B, Hq))
-        self._last["ret"] = (ret, None, 1)
+        out, flags = self._launch(slots, qd, kvl, digits_slot=slots[0], staged=staged, stream=st)
+        self._last["keep"] += (q16, row)
+        if T == 1:
+            ret = (out.view(B, Hq, -1), flags.view(B, Hq))
+        else:
+            ret = (out.view(B * T, Hq, -1).index_select(0, row), flags.view(B * T, Hq).index_select(0, row))
+        self._last["ret"] = (ret, row, T)
         return ret
 
     def _forward_planned(self, query, key, value, seqs, ql, pos):
-        """forward() on rows padded to the longest chunk, the step planned on the device: the new tokens'
-        slots, rows and visible lengths come from one launch (PagedKVCache._step_plan), and with rotary
-        positions a second one turns q and k and writes q to its padded rows, k and v to the cache."""
+        """forward() with rotary positions, on rows padded to the longest chunk, the step planned on the device: one
+        launch gives the new tokens' slots, positions, rows and visible lengths (PagedKVCache._step_plan), a second
+        one turns q and k and writes q to its padded rows, k and v to the cache."""
         c, r = self.cache, self.rotary
         torch = c.torch
         B, T, Hq, d = len(ql), max(ql), query.shape[1], query.shape[2]
-        if r is None:
-            k16, v16 = _dev16(torch, key, c.dev).contiguous(), _dev16(torch, value, c.dev).contiguous()
-            q16 = query.view(torch.int16) if query.dtype != torch.int16 else query
-        else:
-            self._check_turn(query, key, value, pos)
+        self._check_turn(query, key, value, pos)
         ts = torch.cuda.current_stream(c.dev)
         st = ctypes.c_void_p(ts.cuda_stream)
         plan, (off, slot) = c._step_plan(seqs, ql, np.asarray(seqs, dtype=np.int64) * c.max_pages,
@@ -672,11 +683,7 @@ class ExactAttentionBackend:
         staged = (plan.seq_len, off, slot)
         ragged = B * T != sum(ql)
         qd = (torch.zeros if ragged else torch.empty)((B * T, Hq, d), dtype=torch.int16, device=c.dev)
-        if r is None:
-            c._kv_append(k16, v16, plan.dst_rows, sum(ql), None, None, 0, st)
-            qd.index_copy_(0, plan.q_rows, q16)
-        else:
-            r.append(query, key, value, plan.positions if pos is None else pos, plan.dst_rows, c.k, c.v, q_rows=plan.q_rows, q_out=qd)
+        r.append(query, key, value, plan.positions if pos is None else pos, plan.dst_rows, c.k, c.v, q_rows=plan.q_rows, q_out=qd)
         out, flags = self._launch(seqs, qd.view(B, T, Hq, d), plan.kv_len.view(-1), digits_slot=seqs[0], staged=staged, stream=st)
         self._last["keep"] += (plan,)
         if ragged:
