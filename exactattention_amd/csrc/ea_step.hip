@@ -341,6 +341,28 @@ __global__ void __launch_bounds__(RT_THREADS) ea_rotary_kernel(ea_rotary A, int 
     }
 }
 
+// Whether an array that the plan writes lies in another of its arrays: its blocks read the inputs while others
+// write, and no block waits for another
+bool plan_shares_memory(const ea_step_plan& p) {
+    struct Range {
+        const void* at;
+        int64_t bytes;
+    };
+    const int64_t B = p.num_seqs, N = p.max_tokens, table = (int64_t)p.table_rows * p.table_width;
+    const Range r[] = {{p.block_table, 4 * table},  {p.dst_rows, 8 * N},    {p.positions, 4 * N},    {p.seq_of, 4 * N},
+                       {p.q_rows, 8 * N},           {p.kv_len, 4 * B * p.pad_tokens}, {p.new_seq_len, 4 * B}, {p.new_num_free, 4},
+                       {p.status, 4},  // written up to here
+                       {p.seq_len, 4 * B},          {p.counts, 4 * B},      {p.slots, 4 * B},
+                       {p.free_pages, 4 * (int64_t)p.free_capacity},        {p.num_free, 4}};
+    constexpr int n = sizeof(r) / sizeof(r[0]), written = 9;
+    for (int i = 0; i < written; ++i)
+        for (int j = i + 1; j < n; ++j) {
+            const uintptr_t a = (uintptr_t)r[i].at, b = (uintptr_t)r[j].at;
+            if (a && b && r[i].bytes > 0 && r[j].bytes > 0 && a < b + r[j].bytes && b < a + r[i].bytes) return true;
+        }
+    return false;
+}
+
 template <int V, bool ADJ>
 void rotary_launch(const ea_rotary& A, dim3 grid, size_t lds, int tpb, hipStream_t st) {
     if (!A.in_fp32) hipLaunchKernelGGL((ea_rotary_kernel<V, false, false, ADJ>), grid, dim3(RT_THREADS), lds, st, A, tpb);
@@ -363,8 +385,7 @@ int ea_hip_step_plan(const ea_step_plan* p, ea_stream_t stream) {
     if (p->max_tokens > 0 && !p->dst_rows) return -1;
     if (p->free_capacity > 0 && !p->free_pages) return -1;
     if (p->num_seqs > 0 && (p->pad_tokens == 0 || (int64_t)p->num_seqs * p->pad_tokens >= (int64_t)1 << 31)) return -1;
-    // the blocks read these while others write those
-    if ((p->num_seqs > 0 && p->new_seq_len == p->seq_len) || p->new_num_free == p->num_free) return -1;
+    if (plan_shares_memory(*p)) return -1;
     int ps = 0;
     while ((1 << ps) < p->page_size) ++ps;
     // two rows a thread, up to two blocks a CU

@@ -178,8 +178,8 @@ class StepPlan:
         """seq_len, counts: (num_seqs,) int32; block_table: (rows, width) int32, its rows those of `slots`
         (int32; None: row b) grown in place; free_pages: the stack's int32 array, num_free its height (a
         one-entry int32 tensor). max_seq_len: bound of the lengths (None: what a table row holds). The
-        outputs must not be passed in as the inputs of the same build: copy them (or use two plans in
-        turn)."""
+        outputs must not be passed in as the inputs of the same build (it is refused, as any array written that
+        shares memory with another one): copy them, or use two plans in turn."""
         if block_table.dim() != 2:
             raise ValueError("block_table must be (rows, width)")
         rows, width = block_table.shape

@@ -395,7 +395,7 @@ int ea_hip_kv_digits_update(const ea_geometry* g, const ea_buffers* b, const int
  *   status        0, or why the step does not fit (EA_PLAN_* bits); then no entry of the table is
  *                 written, lengths and stack are reported as they were, dst_rows, positions, seq_of and
  *                 q_rows are -1 and kv_len is 0
- * All pointers are device memory; new_seq_len and new_num_free must not be seq_len and num_free. Up to
+ * All pointers are device memory, and no array that is written shares memory with another one. Up to
  * 8192 sequences and 65536 table rows, num_seqs * pad_tokens below 2^31; a row may appear once. Entries of the first pages and of
  * free_pages are taken as they are. Enqueue only, capturable. Returns 0, -1 on bad arguments,
  * -100 - e on a HIP error. No reference counterpart. */
