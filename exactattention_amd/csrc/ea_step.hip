@@ -149,8 +149,9 @@ __global__ void __launch_bounds__(SP_THREADS) ea_step_plan_kernel(ea_step_plan A
 // less than the pair's 8 bytes of traffic, so the exact form is free here.
 // What bounds it is memory: every element is read once and written once. A block takes whole tokens, so
 // the sines of a token are computed once for all its heads (LDS), and q, k and v of a token go in one
-// launch, k and v straight to their pool rows. 16,384 tokens of 32 q, 8 k and 8 v heads of 128 dims: 87 us, 4.6
-// TB/s of the 4.78 that a large copy reaches; 33 tokens 4.6 us, of which a launch alone is about 2.
+// launch, k and v straight to their pool rows. 16,384 tokens of 32 q, 8 k and 8 v heads of 128 dims: 88 us, 4.6
+// TB/s of the 4.78 that a large copy reaches; 33 tokens 4.2 us, of which a launch alone is about 2 (of a graph of
+// 24 launches each).
 // ------------------------------------------------------------------------------------------------
 constexpr int RT_THREADS = 256;
 constexpr int RT_MAX_PAIRS = 128;  // rot_dim at most 256
@@ -433,13 +434,21 @@ int ea_hip_rotary(const ea_rotary* a, ea_stream_t stream) {
     }
     const bool wide = !(ptr & 15) && !(si & (in - 1)) && !(so & (out - 1)) && !(d & 7) && !((a->adjacent ? R : h) & 7);
     if (!wide && a->adjacent && (d & 1)) return -1;  // the narrow form of adjacent pairs takes two elements at a time
-    // Four tokens a block where there are many (fewer sines waited for; 48 heads of 128 dims, 4 -> 1 a block: 8192
-    // tokens 43.2 -> 44.4 us, 16384 95.1 -> 97.2, but 4096 25.6 -> 25.1 and 1000 13.4 -> 9.8), and a block for every
-    // 256 units of a token where they alone would leave CUs idle (33 tokens 5.9 -> 4.2, 500 7.5 -> 6.4, but 1000
-    // 9.9 -> 10.2 and 16384 95 -> 100)
-    const int tpb = a->num_tokens >= 8192 ? 4 : 1, v = wide ? 8 : (a->adjacent ? 2 : 1);
+    // A unit is a thread's work, and a block takes whole tokens: where a token has fewer units than the block threads, it
+    // takes as many tokens as fill them (1 -> 2 -> 4 a block: 40 units a token, 2000 tokens 6.7 -> 4.8 -> 5.2 us, 4096 10.7 ->
+    // 7.4 -> 6.5; 88 units, 4096 tokens 14.3 -> 10.4 -> 11.8), from where there are blocks enough (1000 tokens 4.6 either
+    // way). Many tokens take two at least, whose sines are then waited for once (8192 tokens of 256 units 28.5 -> 28.1
+    // -> 29.4, 448 50.0 -> 49.3 -> 49.9, 704 75.5 -> 76.0 -> 82.3; 4096 of 448 29.3 -> 30.2), and very many of few units four
+    // (16384 of 448 92.6 -> 89.1 -> 87.7, of 704 143.6 -> 141.7 -> 144.2). Few tokens of many units are cut into a block for
+    // every 256 units (whole -> cut: 33 tokens of 448 5.8 -> 4.2, 500 7.7 -> 6.5, of 704 10.3 -> 8.7, of 2048 21.5 -> 16.2; but
+    // 1000 of 448 10.0 -> 10.5, of 704 14.7 -> 14.4, of 2048 29.3 -> 29.2, and 4096 of 2048 88 -> 101). Times are those of 24
+    // launches in a graph, over buffers past the caches' size where they are large.
+    const int v = wide ? 8 : (a->adjacent ? 2 : 1);
     const int64_t units = (int64_t)(a->num_q_heads + a->num_kv_heads) * ((a->adjacent ? R : h) + d - R) / v +
                           (a->v ? (int64_t)a->num_kv_heads * d / v : 0);
+    int tpb = 1;
+    while (a->num_tokens >= 1536 && tpb < 4 && 2 * tpb * units <= RT_THREADS) tpb *= 2;
+    if (a->num_tokens >= 8192) tpb = std::max(tpb, a->num_tokens >= 16384 && units <= 512 ? 4 : 2);
     if (units * tpb >= (int64_t)1 << 30) return -1;  // the kernel counts them in 32 bits
     const int64_t slices = a->num_tokens < 768 ? std::min<int64_t>((units + RT_THREADS - 1) / RT_THREADS, 64) : 1;
     const dim3 grid((unsigned)(((int64_t)a->num_tokens + tpb - 1) / tpb), (unsigned)slices);
