@@ -565,9 +565,12 @@ class ExactAttentionBackend:
         if r is None:
             raise ValueError("positions need rotary=")
         if not hasattr(positions, "data_ptr"):
-            positions = self.cache.torch.from_numpy(np.ascontiguousarray(positions, dtype=np.int32))
+            a = np.asarray(positions)
+            if a.size and (a.dtype.kind not in "iu" or a.min() < -(1 << 31) or a.max() >= 1 << 31):
+                raise ValueError("positions must be whole numbers of 32 bits")
+            positions = self.cache.torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32))
         p = positions.to(self.cache.dev)
-        if p.shape[-1] != n:
+        if not p.dim() or p.shape[-1] != n:
             raise ValueError("one position per token and axis")
         return p
 
