@@ -160,3 +160,36 @@ def test_outputs_given_are_refused(gpu):
     with torch.no_grad():
         rot.rotate(q, k, pos, q_out=torch.empty_like(q))
     rot.rotate(q.detach(), k.detach(), pos, q_out=torch.empty_like(q), k_out=torch.empty_like(k))
+
+
+def test_on_a_stream_and_in_a_graph(gpu):
+    """Forward and backward on another stream than the default, and captured and replayed on new values."""
+    import torch
+    rot, q, k, gq, gk, pos = _inputs((50, 4, 2, 64, {}), torch.float32, 9)
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def step():
+        yq, yk = rot.rotate(q, k, pos)
+        return (yq, yk, *torch.autograd.grad((yq, yk), (q, k), (gq, gk)))
+
+    def want():
+        with torch.no_grad():
+            return (*rot.rotate(q, k, pos), *rot.rotate(gq, gk, pos, inverse=True))
+
+    with torch.cuda.stream(st):
+        for _ in range(3):
+            got = step()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want()))
+    del got  # no eager graph of these leaves lives while the capture runs
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        got = step()
+    for i in range(4):
+        with torch.no_grad():
+            for x in (q, k, gq, gk):
+                x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(i)))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want())), i
