@@ -8,8 +8,8 @@ import sys
 import tempfile
 from concurrent.futures import ThreadPoolExecutor
 
-SOURCES = ["ea_hip.hip", "ea_decode.hip", "ea_mrow.hip", "ea_prefill.hip", "ea_prefill_mod.hip",
-           "ea_step.hip", "ea_exact_host.cpp", "ea_csr.cpp"]
+SOURCES = ["ea_hip.hip", "ea_decode.hip", "ea_mrow.hip", "ea_mrow4.hip", "ea_prefill.hip", "ea_prefill_mod.hip",
+           "ea_step.hip", "ea_norm.hip", "ea_draft.hip", "ea_exact_host.cpp", "ea_csr.cpp"]
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libexactattn_hip.so")
@@ -36,7 +36,7 @@ def build(verbose: bool = False) -> str:
             return subprocess.run([hipcc, *cmd], capture_output=True, text=True)
 
         out = [os.path.join(objs, f + ".o") for f in SOURCES]
-        with ThreadPoolExecutor(4) as pool:
+        with ThreadPoolExecutor(8) as pool:
             done = list(pool.map(lambda x: run([*HIPCC_FLAGS, *FILE_FLAGS.get(x[0], []), "-c", os.path.join(CSRC, x[0]), "-o", x[1]]),
                                  zip(SOURCES, out)))
         if all(r.returncode == 0 for r in done):

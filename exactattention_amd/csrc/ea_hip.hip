@@ -797,10 +797,18 @@ __device__ __forceinline__ void t2_rows(const Params& P, T2Smem& S, int& s_last,
         const bool k16 = (((uintptr_t)P.k | (uintptr_t)(P.g.k_page_stride * 2) | (uintptr_t)(P.g.k_slot_stride * 2) |
                            (uintptr_t)(P.g.k_head_stride * 2)) & 15) == 0 && d == 128;
         for (int64_t jr = tid; jr < nkc && !myflag && S.flag < 2; jr += EA_T2_THREADS) {
-            const uint16_t* kr = P.k + kv_off(P, b, key_n(jc0 + jr), hk, 0);
+            const int64_t ko = kv_off(P, b, key_n(jc0 + jr), hk, 0);
+            const uint16_t* kr = P.k + ko;
             // 16 dims (8 dwords) at a time, read twice: the lead exponent, then the window sum
             auto kchunk = [&](int c16, uint32_t (&kw)[8]) __attribute__((always_inline)) {
-                if (k16) {
+                if (P.ks) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int i = 16 * c16 + 8 * h;  // d is a multiple of 8
+                        const uint4 u = i < d ? kv4_load8(P.k, P.ks, ko + i) : make_uint4(0, 0, 0, 0);
+                        kw[4 * h] = u.x; kw[4 * h + 1] = u.y; kw[4 * h + 2] = u.z; kw[4 * h + 3] = u.w;
+                    }
+                } else if (k16) {
                     const uint4 u0 = ((const uint4*)kr)[2 * c16], u1 = ((const uint4*)kr)[2 * c16 + 1];
                     kw[0] = u0.x; kw[1] = u0.y; kw[2] = u0.z; kw[3] = u0.w;
                     kw[4] = u1.x; kw[5] = u1.y; kw[6] = u1.z; kw[7] = u1.w;
@@ -922,6 +930,12 @@ __device__ __forceinline__ void t2_rows(const Params& P, T2Smem& S, int& s_last,
 #pragma unroll
                 for (int kk = 0; kk < 16; ++kk) {
                     const int64_t o = __shfl(myoff, kk, 64);
+                    if (P.vs) {
+                        const uint32_t two = kk < nk && 2 * ln < dv ? kv4_load2(P.v, P.vs, o + 2 * ln) : 0u;
+                        vx[kk][0] = two & 0xFFFFu;
+                        vx[kk][1] = two >> 16;
+                        continue;
+                    }
 #pragma unroll
                     for (int h = 0; h < 2; ++h) vx[kk][h] = (kk < nk && 2 * ln + h < dv) ? (uint32_t)P.v[o + 2 * ln + h] : 0u;
                 }
@@ -1236,7 +1250,9 @@ __global__ void __launch_bounds__(256) ea_gather_row(Params P, int64_t row, int6
         const int wdt = isv ? dv : d;
         const int64_t j = r / wdt;
         const int e = (int)(r % wdt);
-        dst[i] = (isv ? P.v : P.k)[kv_off(P, b, keys.key(j), hk, isv) + e];
+        const int64_t o = kv_off(P, b, keys.key(j), hk, isv) + e;
+        if (P.ks) dst[i] = (uint16_t)(kv4_load2(isv ? P.v : P.k, isv ? P.vs : P.ks, o & ~(int64_t)1) >> (16 * (o & 1)));
+        else dst[i] = (isv ? P.v : P.k)[o];
     }
 }
 
@@ -1597,7 +1613,16 @@ int check_mods(const ea_options* o, const ea_score_mods* m) {
     return c == 0 || (f > 0 && f < 255) ? 0 : -2;
 }
 
-int make_plan(const ea_geometry* g, const ea_options* o, Plan* pl, const ea_score_mods* m = nullptr) {
+// 0, or the code that the 4-bit entry points return: rows of whole groups, and what reads bf16 rows is no choice
+int check_kv4(const ea_geometry* g, const ea_options* o) {
+    const int64_t st[6] = {g->k_page_stride, g->k_slot_stride, g->k_head_stride, g->v_page_stride, g->v_slot_stride, g->v_head_stride};
+    for (int64_t x : st)
+        if (x & 31) return -1;
+    if (g->head_dim_v & 7) return -1;
+    return o->kv_digits || o->timers || o->kernel == EA_KERNEL_DECODE || o->kernel == EA_KERNEL_GENERAL ? -2 : 0;
+}
+
+int make_plan(const ea_geometry* g, const ea_options* o, Plan* pl, const ea_score_mods* m = nullptr, bool kv4 = false) {
     if (!g || !o) return -1;
     if (g->num_seqs < 0 || g->num_tokens <= 0 || g->num_q_heads <= 0 || g->num_kv_heads <= 0) return -1;
     if (g->num_q_heads % g->num_kv_heads) return -1;
@@ -1610,6 +1635,8 @@ int make_plan(const ea_geometry* g, const ea_options* o, Plan* pl, const ea_scor
     if (o->prefill_waves != 0 && o->prefill_waves != 4 && o->prefill_waves != 8) return -2;
     const int mrc = check_mods(o, m);
     if (mrc) return mrc;
+    const int krc = kv4 ? check_kv4(g, o) : 0;
+    if (krc) return krc;
     pl->grp = g->num_q_heads / g->num_kv_heads;
     pl->r_seg = g->num_tokens * pl->grp;
     pl->nseg = g->num_seqs * g->num_kv_heads;
@@ -1655,7 +1682,8 @@ int make_plan(const ea_geometry* g, const ea_options* o, Plan* pl, const ea_scor
     choose_splits(pl->nseg * (int64_t)gen.nrb, span, o->splits, &gen.nsplit, &gen.split_len);
     gen.dq = d128 && !m && dq_fits(gen.nrb);
     Tier1& mr = pl->mr;
-    mr.rb = m && pl->prefill ? 0 : mrow_rows(g, o, pl->r_seg, m != nullptr);
+    // ea_decode reads neither modifications nor 4-bit caches
+    mr.rb = (m || kv4) && pl->prefill ? 0 : mrow_rows(g, o, pl->r_seg, m != nullptr || kv4);
     pl->mrow = mr.rb > 0;
     const size_t without = lay_out(pl, g, o, false, m != nullptr);
     if (!pl->mrow) return 0;
@@ -1699,7 +1727,12 @@ int herr(hipError_t e) { return e == hipSuccess ? 0 : -100 - (int)e; }
 int reported_nsplit(const Plan& pl) { return pl.prefill ? pl.pf_nsplit : (pl.mrow ? pl.mr.nsplit : pl.gen.nsplit); }
 
 // The caller's arrays and strides, as far as the choice of kernel and the split kernels read them
-void set_inputs(Params& P, const Plan& pl, const ea_geometry* g, const ea_buffers* bf, const ea_score_mods* m = nullptr) {
+void set_inputs(Params& P, const Plan& pl, const ea_geometry* g, const ea_buffers* bf, const ea_score_mods* m = nullptr,
+                const ea_kv4* x = nullptr) {
+    if (x) {
+        P.ks = x->k_scales;
+        P.vs = x->v_scales;
+    }
     if (m) {
         float c;
         memcpy(&c, &m->softcap_bits, 4);
@@ -1843,21 +1876,28 @@ int ea_hip_reads_kv_digits(const ea_geometry* g, const ea_options* o, int32_t* r
     return ea_hip_mods_reads_kv_digits(g, o, nullptr, reads);
 }
 
+// The scales of a 4-bit cache and what its kernels need of the pointers and pages
+static int check_kv4_buffers(const ea_geometry* g, const ea_buffers* bf, const ea_kv4* x) {
+    if (!x->k_scales || !x->v_scales || (((uintptr_t)bf->k | (uintptr_t)bf->v) & 15)) return -1;
+    return bf->block_table && g->page_size < 16 ? -1 : 0;
+}
+
 static int attention_impl(const ea_geometry* g, const ea_buffers* bf, const ea_options* o, const ea_score_mods* m,
-                          void* workspace, size_t workspace_bytes, ea_stream_t stream) {
+                          const ea_kv4* x4, void* workspace, size_t workspace_bytes, ea_stream_t stream) {
     Plan pl;
-    int rc = make_plan(g, o, &pl, m);
+    int rc = make_plan(g, o, &pl, m, x4 != nullptr);
     if (rc) return rc;
     uint32_t ab = o->alpha_bits;
     // an empty batch reads and writes nothing: no buffer or workspace is needed for it
     if (pl.rows == 0) return ((ab >> 23) & 0xFF) == 0xFF ? -3 : 0;
     if (!bf || !bf->q || !bf->k || !bf->v || !bf->seq_len || !bf->kv_len || !bf->out || !bf->flags) return -1;
     if (bf->tree_mask && !bf->tree_base) return -1;
+    if (x4 && (rc = check_kv4_buffers(g, bf, x4))) return rc;
     if (workspace_bytes < pl.total || (!workspace && pl.total)) return -2;
     if (((ab >> 23) & 0xFF) == 0xFF) return -3;
     Params P;
     memset(&P, 0, sizeof(P));
-    set_inputs(P, pl, g, bf, m);
+    set_inputs(P, pl, g, bf, m, x4);
     P.out = bf->out; P.flags = bf->flags; P.stats = o->stats;
     P.stats_x = o->stats && o->stats_entries == EA_STATS ? o->stats + 16 : nullptr;
     P.timers = o->timers;
@@ -1904,6 +1944,7 @@ static int attention_impl(const ea_geometry* g, const ea_buffers* bf, const ea_o
     if (!pl.prefill) {
         int slots = 0, cus = 0;
         use_decode = choose_split_kernel(P, pl);
+        if (x4 && !P.mrow) return -1;  // strides past the kernel's 32-bit offsets
         if (P.mrow && (rc = ea_mrow_slots(P, &slots))) return rc;
         if (use_decode && (rc = ea_decode_slots(P, &slots, &cus))) return rc;
         const int nsplit = P.nsplit;
@@ -2040,12 +2081,28 @@ static int attention_impl(const ea_geometry* g, const ea_buffers* bf, const ea_o
 
 int ea_hip_attention(const ea_geometry* g, const ea_buffers* bf, const ea_options* o, void* workspace,
                      size_t workspace_bytes, ea_stream_t stream) {
-    return attention_impl(g, bf, o, nullptr, workspace, workspace_bytes, stream);
+    return attention_impl(g, bf, o, nullptr, nullptr, workspace, workspace_bytes, stream);
 }
 
 int ea_hip_attention_mods(const ea_geometry* g, const ea_buffers* bf, const ea_options* o, const ea_score_mods* m,
                           void* workspace, size_t workspace_bytes, ea_stream_t stream) {
-    return attention_impl(g, bf, o, m, workspace, workspace_bytes, stream);
+    return attention_impl(g, bf, o, m, nullptr, workspace, workspace_bytes, stream);
+}
+
+int ea_hip_attention_kv4(const ea_geometry* g, const ea_buffers* bf, const ea_options* o, const ea_score_mods* m,
+                         const ea_kv4* x, void* workspace, size_t workspace_bytes, ea_stream_t stream) {
+    if (!x) return -1;
+    return attention_impl(g, bf, o, m, x, workspace, workspace_bytes, stream);
+}
+
+int ea_hip_kv4_workspace_size(const ea_geometry* g, const ea_options* o, const ea_score_mods* m, size_t* bytes,
+                              int32_t* nsplit) {
+    Plan pl;
+    int rc = make_plan(g, o, &pl, m, true);
+    if (rc) return rc;
+    if (bytes) *bytes = pl.total;
+    if (nsplit) *nsplit = reported_nsplit(pl);
+    return 0;
 }
 
 int ea_hip_mods_workspace_size(const ea_geometry* g, const ea_options* o, const ea_score_mods* m, size_t* bytes,
@@ -2070,13 +2127,14 @@ int ea_hip_attention_noalloc(const ea_geometry* g, const ea_buffers* bf, const e
 }
 
 static int exact_rows_impl(const ea_geometry* g, const ea_buffers* bf, const ea_options* o, const ea_score_mods* m,
-                           ea_stream_t stream) {
+                           const ea_kv4* x4, ea_stream_t stream) {
     Plan pl;
-    int rc = make_plan(g, o, &pl, m);
+    int rc = make_plan(g, o, &pl, m, x4 != nullptr);
     if (rc) return rc;
     if (pl.rows == 0) return ((o->alpha_bits >> 23) & 0xFF) == 0xFF ? -3 : 0;  // an empty batch
     if (!bf || !bf->q || !bf->k || !bf->v || !bf->seq_len || !bf->kv_len || !bf->out || !bf->flags) return -1;
     if (bf->tree_mask && !bf->tree_base) return -1;
+    if (x4 && (rc = check_kv4_buffers(g, bf, x4))) return rc;
     if (((o->alpha_bits >> 23) & 0xFF) == 0xFF) return -3;
     hipStream_t st = (hipStream_t)stream;
     hipError_t e = hipStreamSynchronize(st);
@@ -2089,7 +2147,7 @@ static int exact_rows_impl(const ea_geometry* g, const ea_buffers* bf, const ea_
     if (todo.empty()) return 0;
     Params P;
     memset(&P, 0, sizeof(P));
-    set_inputs(P, pl, g, bf, m);
+    set_inputs(P, pl, g, bf, m, x4);
     const int d = g->head_dim, dv = g->head_dim_v, T = g->num_tokens, Hq = g->num_q_heads;
     // each listed row's visible keys, and with modifications its slope and position
     struct Listed {
@@ -2175,13 +2233,18 @@ static int exact_rows_impl(const ea_geometry* g, const ea_buffers* bf, const ea_
     return 0;
 }
 
-int ea_hip_exact_rows_mods(const ea_geometry* g, const ea_buffers* bf, const ea_options* o, const ea_score_mods* m,
-                           ea_stream_t stream) {
+int ea_hip_exact_rows_kv4(const ea_geometry* g, const ea_buffers* bf, const ea_options* o, const ea_score_mods* m,
+                          const ea_kv4* x, ea_stream_t stream) {
     try {
-        return exact_rows_impl(g, bf, o, m, stream);
+        return exact_rows_impl(g, bf, o, m, x, stream);
     } catch (...) {  // host vectors: only an exhausted heap throws
         return EA_ERR_HOST_MEMORY;
     }
+}
+
+int ea_hip_exact_rows_mods(const ea_geometry* g, const ea_buffers* bf, const ea_options* o, const ea_score_mods* m,
+                           ea_stream_t stream) {
+    return ea_hip_exact_rows_kv4(g, bf, o, m, nullptr, stream);
 }
 
 int ea_hip_exact_rows(const ea_geometry* g, const ea_buffers* bf, const ea_options* o, ea_stream_t stream) {

@@ -34,8 +34,10 @@ namespace ea {
 struct Params {
     ea_geometry g;
     const uint16_t* q;
-    const uint16_t* k;
+    const uint16_t* k;   // of a 4-bit cache (ks, vs set): its codes, as v
     const uint16_t* v;
+    const uint8_t* ks;   // scales of a cache held in 4 bits (ea_kv4.h); NULL: bf16
+    const uint8_t* vs;
     const int32_t* seq_len;
     const int32_t* kv_len;
     const int32_t* bt;
@@ -286,6 +288,8 @@ int ea_launch_decode(const Params& P, hipStream_t st);
 // same three questions as for the decode kernel.
 int ea_mrow_eligible(const Params& P);
 int ea_mrow_slots(const Params& P, int* slots);
+// its variants for 4-bit caches, their own file
+const void* ea_mrow_kv4_fn(int rb, bool small, int mods);
 int ea_launch_mrow(const Params& P, hipStream_t st);
 
 // int8-MFMA prefill path (ea_prefill.hip). A tile holds 64 keys of one segment:

@@ -13,6 +13,7 @@
 // wave v the V rows of keys 16 v .. 16 v + 15, two channels per lane; about 950 VALU instructions per
 // wave and pass. The figures are at ea_tier2 (ea_hip.hip).
 #pragma once
+#include "ea_kv4.h"
 #include "ea_params.h"
 #include "ea_pf_common.h"
 
@@ -201,7 +202,8 @@ __device__ inline void dd_rows(const Params& P, DDSmem& S, int cnt, int C, DDPar
                 vx[kk] = 0;
                 if (kk < nk && 2 * lane < dv) {
                     const uint16_t* vp = P.v + o + 2 * lane;
-                    vx[kk] = v4 ? *(const uint32_t*)vp : ((uint32_t)vp[0] | ((uint32_t)vp[1] << 16));
+                    if (P.vs) vx[kk] = kv4_load2(P.v, P.vs, o + 2 * lane);
+                    else vx[kk] = v4 ? *(const uint32_t*)vp : ((uint32_t)vp[0] | ((uint32_t)vp[1] << 16));
                 }
             }
             // ---- scores and weights: 4 lanes per key
@@ -211,14 +213,17 @@ __device__ inline void dd_rows(const Params& P, DDSmem& S, int cnt, int C, DDPar
             double s = 0.0, es = 0.0, ea = 0.0;
             bool bad = false;
             if (have) {
-                const uint16_t* kr = P.k + kv_off(P, b, key_n(j), hk, 0);
+                const int64_t ko = kv_off(P, b, key_n(j), hk, 0);
+                const uint16_t* kr = P.k + ko;
                 uint4 kv[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int c0 = 8 * (4 * i + part);
                     kv[i] = make_uint4(0, 0, 0, 0);
                     if (c0 >= d) continue;  // d is a multiple of 8
-                    if (k16) {
+                    if (P.ks) {
+                        kv[i] = kv4_load8(P.k, P.ks, ko + c0);
+                    } else if (k16) {
                         kv[i] = *(const uint4*)(kr + c0);
                     } else {
                         uint32_t* kw = (uint32_t*)&kv[i];

@@ -70,6 +70,30 @@ class RotaryArgs(ctypes.Structure):
                                     "k_out", "v_out")])
 
 
+class KV4Args(ctypes.Structure):
+    _fields_ = [("k_scales", P), ("v_scales", P)]
+
+
+class NormRotaryArgs(ctypes.Structure):
+    _fields_ = ([("r", RotaryArgs)] + [(n, P) for n in ("q_weight", "k_weight", "k_scales", "v_scales")]
+                + [("k_page_stride", ctypes.c_int64), ("v_page_stride", ctypes.c_int64), ("page_size", ctypes.c_int32),
+                   ("weights_fp32", ctypes.c_int32), ("eps", ctypes.c_float), ("pad0", ctypes.c_int32)])
+
+
+class NormRotaryGradArgs(ctypes.Structure):
+    _fields_ = ([("r", RotaryArgs), ("gq", P), ("gk", P)]
+                + [(n, ctypes.c_int64) for n in ("gq_tok_stride", "gq_head_stride", "gk_tok_stride", "gk_head_stride")]
+                + [(n, P) for n in ("q_weight", "k_weight", "dq_weight", "dk_weight", "partial")]
+                + [("weights_fp32", ctypes.c_int32), ("eps", ctypes.c_float)])
+
+
+class DraftCheckArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("num_seqs", "num_drafts", "vocab", "pad0")]
+                + [(n, ctypes.c_int64) for n in ("p_seq_stride", "p_row_stride", "q_seq_stride", "q_row_stride")]
+                + [(n, P) for n in ("probs", "draft_probs", "drafted", "uniforms", "parents", "counts", "accepted", "path", "tokens",
+                                    "work")])
+
+
 # ea_options.kernel (include/exactattn_hip.h EA_KERNEL_*)
 KERNELS = {"auto": 0, "prefill": 1, "decode": 2, "general": 3}
 
@@ -147,6 +171,20 @@ def load():
         lib.ea_hip_step_plan.restype = ctypes.c_int
         lib.ea_hip_rotary.argtypes = [ctypes.POINTER(RotaryArgs), P]
         lib.ea_hip_rotary.restype = ctypes.c_int
+        X = ctypes.POINTER(KV4Args)
+        lib.ea_hip_attention_kv4.argtypes = [G, B, O, M, X, P, ctypes.c_size_t, P]
+        lib.ea_hip_kv4_workspace_size.argtypes = [G, O, M, ctypes.POINTER(ctypes.c_size_t), ctypes.POINTER(ctypes.c_int32)]
+        lib.ea_hip_exact_rows_kv4.argtypes = [G, B, O, M, X, P]
+        lib.ea_hip_kv4_values.argtypes = [ctypes.c_int64, ctypes.c_int32, P, P, P, P]
+        lib.ea_hip_norm_rotary.argtypes = [ctypes.POINTER(NormRotaryArgs), P]
+        lib.ea_hip_norm_rotary_grad.argtypes = [ctypes.POINTER(NormRotaryGradArgs), P]
+        lib.ea_hip_draft_check.argtypes = [ctypes.POINTER(DraftCheckArgs), P]
+        for f in (lib.ea_hip_attention_kv4, lib.ea_hip_kv4_workspace_size, lib.ea_hip_exact_rows_kv4, lib.ea_hip_kv4_values,
+                  lib.ea_hip_norm_rotary, lib.ea_hip_norm_rotary_grad, lib.ea_hip_draft_check):
+            f.restype = ctypes.c_int
+        lib.ea_hip_norm_rotary_grad_size.argtypes = [ctypes.POINTER(NormRotaryGradArgs)]
+        lib.ea_hip_draft_check_size.argtypes = [ctypes.POINTER(DraftCheckArgs)]
+        lib.ea_hip_norm_rotary_grad_size.restype = lib.ea_hip_draft_check_size.restype = ctypes.c_size_t
         lib.ea_hip_kv_digits_bytes.argtypes = [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]
         lib.ea_hip_kv_digits_bytes.restype = ctypes.c_size_t
         lib.ea_hip_kv_digits_update.argtypes = [ctypes.POINTER(Geometry), ctypes.POINTER(Buffers), P, P,
@@ -177,15 +215,18 @@ def _stream_ptr(torch):
 
 
 def workspace_size(g: dict, splits: int = 0, out_fp32: bool = False, kernel: int = 0, mods=None,
-                   kv_digits: bool = False) -> tuple[int, int]:
+                   kv_digits: bool = False, kv4: bool = False) -> tuple[int, int]:
     """Bytes and splits of a step; mods: the ScoreModsArgs of one with score modifications; kv_digits: of a
-    step that is given a digit-tile cache."""
+    step that is given a digit-tile cache; kv4: of one over a 4-bit cache."""
     lib = load()
     o = Options(splits=splits, out_fp32=int(out_fp32), tier2=1, kernel=kernel)
     if kv_digits:  # set, and large enough: the size depends on nothing else of it
         o.kv_digits, o.kv_digits_tiles = 1, 0x7FFFFFFF
     nb, ns = ctypes.c_size_t(0), ctypes.c_int32(0)
-    if mods is None:
+    if kv4:
+        _check(lib.ea_hip_kv4_workspace_size(ctypes.byref(geometry(g)), ctypes.byref(o), None if mods is None else ctypes.byref(mods),
+                                             ctypes.byref(nb), ctypes.byref(ns)), "ea_hip_kv4_workspace_size")
+    elif mods is None:
         _check(lib.ea_hip_workspace_size(ctypes.byref(geometry(g)), ctypes.byref(o), ctypes.byref(nb), ctypes.byref(ns)),
                "ea_hip_workspace_size")
     else:
@@ -257,7 +298,8 @@ def step_route(g: dict, ptrs: dict, **opt) -> tuple[str, int, bool, int]:
 
 class DeviceProblem:
     """A problem's arrays resident on the GPU, plus output, flags, workspace and stats buffers.
-    Built once; `launch_hip` then runs steps on it with no allocation."""
+    Built once; `launch_hip` then runs steps on it with no allocation. prob["kv4"], a KV4Pool, in place of "k" and
+    "v": a cache held in 4 bits, whose geometry() the problem's holds."""
 
     def __init__(self, prob: dict, out: str = "bf16", splits: int = 0, device: str = "cuda", kernel: str = "auto",
                  prefill_waves: int = 0, mods: ScoreMods | None = None):
@@ -285,6 +327,14 @@ class DeviceProblem:
                 a = a.view(np.int64)
             return torch.from_numpy(a).to(dev)
 
+        self.kv4 = prob.get("kv4")
+        self._kv4_args = None if self.kv4 is None else self.kv4.args()
+        if self.kv4 is not None:
+            if self.kv4.dev != torch.empty(0, device=dev).device:
+                raise ValueError(f"the 4-bit cache must be on {dev}")
+            if any(self.geom.get(f) != x for f, x in self.kv4.geometry().items()):
+                raise ValueError("the geometry is not the 4-bit cache's (KV4Pool.geometry)")
+            prob = {**prob, "k": self.kv4.k, "v": self.kv4.v}
         self.t = {k: t(prob.get(k)) for k in ("q", "k", "v", "seq_len", "kv_len", "block_table",
                                                "block_table_offset", "tree_mask", "tree_base")}
         rows = int(np.prod(prob["out_shape"][:3]))
@@ -292,8 +342,8 @@ class DeviceProblem:
         self.out = torch.empty(prob["out_shape"], dtype=torch.int32 if self.out_fp32 else torch.int16, device=dev)
         self.flags = torch.empty(rows, dtype=torch.uint8, device=dev)
         self.mods, self._mods_keep = (None, None) if mods is None else mods.bind(self.geom, dev)
-        nb, self.nsplit = workspace_size(self.geom, splits, self.out_fp32, self.kernel, self.mods)
-        if self.mods is not None and self.geom["head_dim"] == self.geom["head_dim_v"] == 128:
+        nb, self.nsplit = workspace_size(self.geom, splits, self.out_fp32, self.kernel, self.mods, kv4=self.kv4 is not None)
+        if self.kv4 is None and self.mods is not None and self.geom["head_dim"] == self.geom["head_dim_v"] == 128:
             # a launch with a digit-tile cache may take another kernel
             nb = max(nb, workspace_size(self.geom, splits, self.out_fp32, self.kernel, self.mods, True)[0])
         self.workspace = torch.empty(max(nb, 256), dtype=torch.uint8, device=dev)
@@ -332,6 +382,11 @@ def launch_hip(dp: DeviceProblem, alpha_bits: int, merge_order=None, tier2: bool
     lib = load()
     o = options(dp, alpha_bits, merge_order, tier2, events, timers, kv_digits, force_tier2)
     b = dp.buffers()
+    if dp.kv4 is not None:
+        _check(lib.ea_hip_attention_kv4(ctypes.byref(dp._geom_c), ctypes.byref(b), ctypes.byref(o),
+                                        None if dp.mods is None else ctypes.byref(dp.mods), ctypes.byref(dp._kv4_args),
+                                        dp.workspace.data_ptr(), dp.ws_bytes, _stream_ptr(dp.torch)), "ea_hip_attention_kv4")
+        return
     if dp.mods is not None:
         _check(lib.ea_hip_attention_mods(ctypes.byref(dp._geom_c), ctypes.byref(b), ctypes.byref(o), ctypes.byref(dp.mods),
                                          dp.workspace.data_ptr(), dp.ws_bytes, _stream_ptr(dp.torch)), "ea_hip_attention_mods")
@@ -347,7 +402,8 @@ def exact_rows(dp: DeviceProblem, alpha_bits: int) -> None:
     o = options(dp, alpha_bits)
     b = dp.buffers()
     m = None if dp.mods is None else ctypes.byref(dp.mods)
-    _check(lib.ea_hip_exact_rows_mods(ctypes.byref(dp._geom_c), ctypes.byref(b), ctypes.byref(o), m, _stream_ptr(dp.torch)),
+    x = None if dp.kv4 is None else ctypes.byref(dp._kv4_args)
+    _check(lib.ea_hip_exact_rows_kv4(ctypes.byref(dp._geom_c), ctypes.byref(b), ctypes.byref(o), m, x, _stream_ptr(dp.torch)),
            "ea_hip_exact_rows")
 
 

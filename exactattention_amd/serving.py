@@ -14,7 +14,9 @@ management to that script. Here the cache lives on the device:
     instead of slicing the whole prefix again. They are re-sliced lazily: an append or a truncation
     only marks the slot's tiles stale from its first changed key, and the stale tiles of every slot
     are re-sliced in one update right before a call that reads the cache (the library says which
-    calls do: ea_hip_mods_reads_kv_digits). Decode steps, which read the bf16 cache, slice nothing.
+    calls do: ea_hip_mods_reads_kv_digits). Decode steps, which read the bf16 cache, slice nothing;
+  * or, with bits=4, a KV4Pool in place of the bf16 pools, a quarter of their size and a bit: keys and values are rounded to it
+    as they are written, and attention reads it. Digit tiles, seven times its size, are not kept with it.
 
 Every call enqueues on torch's current stream and copies its result to the host (the caller sees
 (out bits, flags) like the reference's backends).
@@ -30,7 +32,8 @@ import numpy as np
 
 from . import hip
 from .formats import ExactAttentionDomainError, ExactAttentionUncertifiedError, alpha_bits_for, alpha_fp32_bits
-from .step import PLAN_ROWS, PLAN_SEQS, Rotary, StepPlan  # noqa: F401
+from .kv4 import KV4Pool
+from .step import PLAN_ROWS, PLAN_SEQS, DraftCheck, HeadNorm, Rotary, StepPlan  # noqa: F401
 
 TILE = 64  # keys per digit tile
 
@@ -91,17 +94,30 @@ def _torch_dtypes(torch):
 
 class PagedKVCache:
     def __init__(self, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, max_seqs: int,
-                 max_seq_len: int, digits: bool = True, device: str = "cuda"):
+                 max_seq_len: int, digits: bool = True, device: str = "cuda", bits: int = 16):
         import torch
         if page_size <= 0 or page_size & (page_size - 1):
             raise ValueError("page_size must be a power of two")
+        if bits not in (16, 4):
+            raise ValueError("bits must be 16 or 4")
         self.torch = torch
         self.dev = torch.device(device)
         self.P, self.Hkv, self.d = page_size, num_kv_heads, head_dim
         self.max_seqs, self.max_seq_len = max_seqs, max_seq_len
         self.max_pages = (max_seq_len + page_size - 1) // page_size
-        self.k = torch.zeros((num_pages, page_size, num_kv_heads, head_dim), dtype=torch.int16, device=self.dev)
-        self.v = torch.zeros_like(self.k)
+        self.pool4 = None
+        if bits == 4:
+            if self.dev.type != "cuda":
+                raise ValueError("a cache in 4 bits lives on the GPU")
+            self.pool4 = KV4Pool(num_pages, page_size, num_kv_heads, head_dim, self.dev)
+            self.k, self.v = self.pool4.k, self.pool4.v
+            digits = False
+        else:
+            self.k = torch.zeros((num_pages, page_size, num_kv_heads, head_dim), dtype=torch.int16, device=self.dev)
+            self.v = torch.zeros_like(self.k)
+        # what Rotary.append writes to, and the scales of an attention call
+        self.pools = (self.k, self.v) if self.pool4 is None else (self.pool4, None)
+        self._kv4 = None if self.pool4 is None else self.pool4.args()
         self.block_table = torch.zeros((max_seqs, self.max_pages), dtype=torch.int32, device=self.dev)
         self.bt_host = np.zeros((max_seqs, self.max_pages), dtype=np.int32)
         _torch_dtypes(torch)
@@ -150,12 +166,12 @@ class PagedKVCache:
     def _geom1(self, s: int, T: int, Hq: int, seq_len: int) -> dict:
         """Serving geometry of one sequence slot (b = 0) over the shared pools."""
         P, Hkv, d = self.P, self.Hkv, self.d
-        return dict(num_seqs=1, num_tokens=T, num_q_heads=Hq, num_kv_heads=Hkv, head_dim=d, head_dim_v=d,
+        pages = dict(k_page_stride=P * Hkv * d, k_slot_stride=Hkv * d, k_head_stride=d,
+                     v_page_stride=P * Hkv * d, v_slot_stride=Hkv * d, v_head_stride=d) if self.pool4 is None else self.pool4.geometry()
+        return dict(dict(num_seqs=1, num_tokens=T, num_q_heads=Hq, num_kv_heads=Hkv, head_dim=d, head_dim_v=d,
                     q_seq_stride=T * Hq * d, q_tok_stride=Hq * d, q_head_stride=d,
                     o_seq_stride=T * Hq * d, o_tok_stride=Hq * d, o_head_stride=d,
-                    k_page_stride=P * Hkv * d, k_slot_stride=Hkv * d, k_head_stride=d,
-                    v_page_stride=P * Hkv * d, v_slot_stride=Hkv * d, v_head_stride=d,
-                    page_size=P, block_table_stride=self.max_pages, max_seq_len=max(1, seq_len))
+                    page_size=P, block_table_stride=self.max_pages, max_seq_len=max(1, seq_len)), **pages)
 
     # ---- writes
     def append(self, s: int, k_bits, v_bits) -> None:
@@ -317,6 +333,13 @@ class PagedKVCache:
             self.v.view(-1, H, d).index_copy_(0, dst, v_new.reshape(-1, H, d))
             return
         rows = self.k.shape[0] * self.P
+        if self.pool4 is not None and n:
+            H, d = self.Hkv, self.d
+            with self.torch.cuda.device(self.dev):
+                self.pool4.append(k_new.reshape(-1, H, d)[:n], v_new.reshape(-1, H, d)[:n], dst)
+            n = 0
+        if n == 0 and n_bt == 0:
+            return
         hip._check(hip.load().ea_hip_kv_append(
             self.k.data_ptr(), self.v.data_ptr(), rows, self.Hkv * self.d, k_new.data_ptr(), v_new.data_ptr(),
             dst.data_ptr(), n, self.block_table.data_ptr(), self.block_table.numel(),
@@ -410,17 +433,24 @@ class ExactAttentionBackend:
     mods: score modifications of every call (hip.ScoreMods with a window, slopes or a softcap; its
     per-token arrays are the calls' own). A token's distance counts from its own position, the end of
     its prefix. rotary: rotary positions (Rotary): the calls then take q and k as the projections leave them,
-    turn both by the tokens' positions and write k to the cache on the way."""
+    turn both by the tokens' positions and write k to the cache on the way. norm: a norm of every query and key head in
+    front of the rotation (HeadNorm)."""
 
     def __init__(self, cache: PagedKVCache, num_q_heads: int, alpha=None, out: str = "bf16", *, alpha_bits=None,
-                 mods: "hip.ScoreMods | None" = None, rotary: Rotary | None = None):
+                 mods: "hip.ScoreMods | None" = None, rotary: Rotary | None = None, norm: HeadNorm | None = None):
         self.cache, self.Hq, self.out = cache, num_q_heads, out
         self.alpha_bits = alpha_fp32_bits(alpha, alpha_bits)
         if mods is not None and (mods.kv_begin is not None or mods.q_pos is not None):
             raise ValueError("kv_begin and q_pos are per token: the backend's calls set them")
         if rotary is not None and rotary.head_dim != cache.d:
             raise ValueError("the rotary positions are of another head size")
-        self.mods, self.rotary = mods, rotary
+        if norm is not None:
+            if rotary is None:
+                raise ValueError("norm needs rotary=")
+            norm._weights(rotary)  # of its head size, type and device
+        if rotary is not None and cache.pool4 is not None and rotary.rot_dim % 4:
+            raise ValueError("rot_dim must be a multiple of 4 with a cache in 4 bits")
+        self.mods, self.rotary, self.norm = mods, rotary, norm
         self._mods_keep = None
         if mods is not None:
             g = dict(num_seqs=0, num_tokens=0, num_q_heads=num_q_heads)
@@ -489,7 +519,10 @@ class ExactAttentionBackend:
             if reads.value:
                 c.flush(stream)  # the stale tiles, re-sliced ahead of the call in stream order
         nb, ns = ctypes.c_size_t(0), ctypes.c_int32(0)
-        if m is None:
+        if c.pool4 is not None:
+            hip._check(lib.ea_hip_kv4_workspace_size(ctypes.byref(gc), ctypes.byref(o), None if m is None else ctypes.byref(m),
+                                                     ctypes.byref(nb), ctypes.byref(ns)), "ea_hip_kv4_workspace_size")
+        elif m is None:
             hip._check(lib.ea_hip_workspace_size(ctypes.byref(gc), ctypes.byref(o), ctypes.byref(nb), ctypes.byref(ns)),
                        "ea_hip_workspace_size")
         else:
@@ -503,7 +536,11 @@ class ExactAttentionBackend:
                         tree_mask=None if tm is None else tm.data_ptr(), tree_base=None if tb is None else tb.data_ptr(),
                         out=out.data_ptr(), flags=flags.data_ptr())
         st = stream if stream is not None else hip._stream_ptr(torch)
-        if m is None:
+        if c.pool4 is not None:
+            hip._check(lib.ea_hip_attention_kv4(ctypes.byref(gc), ctypes.byref(b), ctypes.byref(o),
+                                                None if m is None else ctypes.byref(m), ctypes.byref(c._kv4), ws.data_ptr(),
+                                                int(nb.value), st), "ea_hip_attention_kv4")
+        elif m is None:
             hip._check(lib.ea_hip_attention(ctypes.byref(gc), ctypes.byref(b), ctypes.byref(o), ws.data_ptr(), int(nb.value),
                                             st), "ea_hip_attention")
         else:
@@ -519,8 +556,9 @@ class ExactAttentionBackend:
         c = self.cache
         m = self._last["mods"]
         for gc, b, o in self._last["before"] + [self._last["args"]]:
-            hip._check(hip.load().ea_hip_exact_rows_mods(ctypes.byref(gc), ctypes.byref(b), ctypes.byref(o),
-                                                         None if m is None else ctypes.byref(m), hip._stream_ptr(c.torch)),
+            hip._check(hip.load().ea_hip_exact_rows_kv4(ctypes.byref(gc), ctypes.byref(b), ctypes.byref(o),
+                                                        None if m is None else ctypes.byref(m),
+                                                        None if c._kv4 is None else ctypes.byref(c._kv4), hip._stream_ptr(c.torch)),
                        "ea_hip_exact_rows")
 
     def _append(self, seqs, counts, q, k, v, positions=None):
@@ -543,7 +581,7 @@ class ExactAttentionBackend:
         pos = self._positions(positions, n)
         self._check_turn(qd, kd, vd, pos)
         plan, _ = c._step_plan(seqs, counts)
-        return self.rotary.append(qd, kd, vd, plan.positions if pos is None else pos, plan.dst_rows, c.k, c.v)
+        return self.rotary.append(qd, kd, vd, plan.positions if pos is None else pos, plan.dst_rows, *c.pools, norm=self.norm)
 
     def _check_turn(self, q, k, v, pos) -> None:
         """What Rotary.append would refuse, before the cache's bookkeeping changes."""
@@ -686,7 +724,8 @@ class ExactAttentionBackend:
         staged = (plan.seq_len, off, slot)
         ragged = B * T != sum(ql)
         qd = (torch.zeros if ragged else torch.empty)((B * T, Hq, d), dtype=torch.int16, device=c.dev)
-        r.append(query, key, value, plan.positions if pos is None else pos, plan.dst_rows, c.k, c.v, q_rows=plan.q_rows, q_out=qd)
+        r.append(query, key, value, plan.positions if pos is None else pos, plan.dst_rows, *c.pools, q_rows=plan.q_rows, q_out=qd,
+                 norm=self.norm)
         out, flags = self._launch(seqs, qd.view(B, T, Hq, d), plan.kv_len.view(-1), digits_slot=seqs[0], staged=staged, stream=st)
         self._last["keep"] += (plan,)
         if ragged:
@@ -769,7 +808,7 @@ class ExactAttentionBackend:
         return res[:, 0], fl
 
     def verify_tree(self, s: int, q, k, v, parents):
-        """Speculative verification: N <= 64 draft nodes, parents[i] < i (-1: the prefix), appended
+        """Speculative verification's attention (DraftCheck then says which nodes stand): N <= 64 draft nodes, parents[i] < i (-1: the prefix), appended
         after the prefix; node i attends the prefix and its root-to-node path. q (N, Hq, d), k/v
         (N, Hkv, d). Returns (out (N, Hq, d), flags); keep the accepted path with accept().
         A node's position is the prefix's length plus its depth (rotary positions; a window counts the
@@ -842,7 +881,7 @@ class DecodeGraph:
 
     The caller writes the step's inputs into the static tensors `q` (B, 1, Hq, d), `k` and `v`
     (B, Hkv, d) (int16 views of bf16) before calling step(); the outputs land in `out` and `flags`.
-    The backend's score modifications and rotary positions are part of the graph: q and k are then given
+    The backend's score modifications, rotary positions and head norms are part of the graph: q and k are then given
     unturned, and with several position axes the caller also writes `positions` (axes, B), int32.
     `max_len` bounds every sequence's length while the graph lives: it sizes the split grid (the
     kernel skips the splits past a sequence's end), so a tight bound keeps the grid dense."""
@@ -905,9 +944,9 @@ class DecodeGraph:
         self.o = hip.Options(alpha_bits=backend.alpha_bits, out_fp32=int(fp32), splits=0, tier2=1)
         nb, ns = ctypes.c_size_t(0), ctypes.c_int32(0)
         self.m = None if backend.mods is None else backend._step_mods()
-        hip._check(lib.ea_hip_mods_workspace_size(ctypes.byref(self.gc), ctypes.byref(self.o),
-                                                  None if self.m is None else ctypes.byref(self.m), ctypes.byref(nb),
-                                                  ctypes.byref(ns)), "ea_hip_workspace_size")
+        size = lib.ea_hip_mods_workspace_size if c.pool4 is None else lib.ea_hip_kv4_workspace_size
+        hip._check(size(ctypes.byref(self.gc), ctypes.byref(self.o), None if self.m is None else ctypes.byref(self.m),
+                        ctypes.byref(nb), ctypes.byref(ns)), "ea_hip_workspace_size")
         self.ws_bytes = int(nb.value)
         self.ws = torch.empty(max(self.ws_bytes, 256), dtype=torch.uint8, device=dev)
         rot = backend.rotary
@@ -935,8 +974,12 @@ class DecodeGraph:
         c._kv_append(self.k, self.v, d["idx"], self.B if rot is None else 0, d["bt_pos"], d["bt_val"], self.B, st)
         if rot is not None:
             pos, off = (d["kvl"], -1) if self.positions is None else (self.positions, 0)
-            rot.append(self.q[:, 0], self.k, self.v, pos, d["idx"], c.k, c.v, q_out=self._qr, pos_offset=off)
+            rot.append(self.q[:, 0], self.k, self.v, pos, d["idx"], *c.pools, q_out=self._qr, pos_offset=off, norm=self.be.norm)
         m = None if self.m is None else ctypes.byref(self.m)
+        if c.pool4 is not None:
+            hip._check(lib.ea_hip_attention_kv4(ctypes.byref(self.gc), ctypes.byref(self.bufs), ctypes.byref(self.o), m,
+                                                ctypes.byref(c._kv4), self.ws.data_ptr(), self.ws_bytes, st), "ea_hip_attention_kv4")
+            return
         hip._check(lib.ea_hip_attention_mods(ctypes.byref(self.gc), ctypes.byref(self.bufs), ctypes.byref(self.o), m,
                                              self.ws.data_ptr(), self.ws_bytes, st), "ea_hip_attention")
 
@@ -991,8 +1034,10 @@ class DecodeGraph:
         """After the latest step: flag-1 rows finished by the host exact tier, flag 2 raises."""
         st = ctypes.c_void_p(self.torch.cuda.current_stream(self.c.dev).cuda_stream)
         if bool((self.flags == 1).any().item()):
-            hip._check(hip.load().ea_hip_exact_rows_mods(ctypes.byref(self.gc), ctypes.byref(self.bufs), ctypes.byref(self.o),
-                                                         None if self.m is None else ctypes.byref(self.m), st),
+            x = self.c._kv4
+            hip._check(hip.load().ea_hip_exact_rows_kv4(ctypes.byref(self.gc), ctypes.byref(self.bufs), ctypes.byref(self.o),
+                                                        None if self.m is None else ctypes.byref(self.m),
+                                                        None if x is None else ctypes.byref(x), st),
                        "ea_hip_exact_rows")
         if bool((self.flags == 2).any().item()):
             raise ExactAttentionDomainError("non-finite input or fp32 logit overflow")

@@ -1,13 +1,18 @@
-"""What a serving step does before its attention call: the step plan and the rotary positions.
+"""What a serving step does around its attention call: the step plan, the rotary positions with the norms of query and
+key heads, and the check of drafted tokens.
 
   StepPlan  where the new tokens go, from lengths that are on the device: block-table growth from a
             stack of free pages, each token's slot in the pool, its position and its visible length
             (ea_hip_step_plan). Lengths and the stack's height go in and come out as device tensors,
             so a loop that keeps them there, or a captured graph, needs no host between its steps.
   Rotary    q and k turned by positions of one or several axes, k and v written into a paged cache in
-            the same launch, or the rotation and its inverse alone (ea_hip_rotary).
+            the same launch, or the rotation and its inverse alone (ea_hip_rotary). With a HeadNorm every query
+            and key head is normed in the same pass (ea_hip_norm_rotary, and its gradient), and the cache may be
+            one held in 4 bits (KV4Pool).
+  DraftCheck  which drafted tokens stand, from the target's probabilities and given random numbers, and the token
+            after them (ea_hip_draft_check).
 
-Both enqueue on torch's current stream of the tensors' device and do not wait. No reference
+All enqueue on torch's current stream of the tensors' device and do not wait. No reference
 counterpart: the reference's demo leaves its cache and positions to transformers
 (scripts/spec_decode_demo.py:116-125).
 """
@@ -21,6 +26,7 @@ import struct
 import numpy as np
 
 from . import hip
+from .kv4 import KV4Pool
 
 PLAN_SEQS, PLAN_ROWS = 8192, 65536  # sequences of a plan, rows of its block table
 
@@ -32,7 +38,11 @@ PLAN_STATUS = {1: "out of pages", 2: "a sequence longer than its table row or ma
 # ea_step_plan and ea_rotary as struct formats: a call packs its arguments in one go, where setting the fields of a
 # ctypes structure one by one costs about 70 ns each
 _PLAN, _ROTARY = struct.Struct("8i14Q"), struct.Struct("11if15q11Q")
+_NORM, _GRAD = struct.Struct("11if15q11Q4Q2q2ifi"), struct.Struct("11if15q11Q2Q4q5Qif")
+_DRAFT = struct.Struct("4i4q10Q")
 assert _PLAN.size == ctypes.sizeof(hip.StepPlanArgs) and _ROTARY.size == ctypes.sizeof(hip.RotaryArgs)
+assert _NORM.size == ctypes.sizeof(hip.NormRotaryArgs) and _GRAD.size == ctypes.sizeof(hip.NormRotaryGradArgs)
+assert _DRAFT.size == ctypes.sizeof(hip.DraftCheckArgs)
 
 
 _C = None  # torch's, once a plan or a rotation exists
@@ -91,6 +101,38 @@ def _turn():
 
         _TURN = Turn.apply
     return _TURN
+
+
+_NORM_TURN = None
+
+
+def _norm_turn():
+    """The norm and the rotation as a differentiable function of q, k and the weights."""
+    global _NORM_TURN
+    if _NORM_TURN is None:
+        import torch
+
+        class NormTurn(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, q, k, qw, kw, positions, rotary, eps):
+                ctx.save_for_backward(q, k, qw, kw, positions)
+                ctx.rotary, ctx.eps = rotary, eps
+                ctx.set_materialize_grads(False)
+                out = rotary.rotate(q, k, positions, norm=HeadNorm(qw, kw, eps))
+                need = ctx.needs_input_grad
+                ctx.mark_non_differentiable(*(o for i, o in enumerate(out) if not (need[i] or need[i + 2])))
+                return out
+
+            @staticmethod
+            @torch.autograd.function.once_differentiable
+            def backward(ctx, gq, gk):
+                q, k, qw, kw, positions = ctx.saved_tensors
+                need = ctx.needs_input_grad
+                out = ctx.rotary._norm_grad(q, k, qw, kw, ctx.eps, positions, gq, gk, need[2], need[3])
+                return tuple(g if n else None for g, n in zip(out, need)) + (None,) * 3
+
+        _NORM_TURN = NormTurn.apply
+    return _NORM_TURN
 
 
 class _At:
@@ -205,6 +247,29 @@ class StepPlan:
             raise RuntimeError("step plan: " + "; ".join(m for b, m in PLAN_STATUS.items() if st & b))
 
 
+class HeadNorm:
+    """A norm of every query and key head in front of the rotation: x / sqrt(mean x^2 + eps) * weight over the head's
+    elements. q_weight, k_weight: (head_dim,) bf16 or fp32, both of one type (parameters get their gradients)."""
+
+    def __init__(self, q_weight, k_weight, eps: float = 1e-6):
+        if not (math.isfinite(eps) and eps >= 0):
+            raise ValueError("eps must be finite and not negative")
+        if q_weight.dtype != k_weight.dtype or q_weight.dim() != 1 or q_weight.shape != k_weight.shape:
+            raise ValueError("q_weight and k_weight must be (head_dim,) tensors of one type")
+        self.q_weight, self.k_weight, self.eps = q_weight, k_weight, float(eps)
+
+    def _weights(self, r):
+        """(address of q's, of k's, whether they are fp32), checked for the rotation r."""
+        out = []
+        for name, w in (("q_weight", self.q_weight), ("k_weight", self.k_weight)):
+            if w.shape[0] != r.head_dim or not (w.dtype is r._f32 or w.dtype is r._bits[0]) or w.get_device() != r._at:
+                raise ValueError(f"{name} must be ({r.head_dim},) bf16 or fp32 on {r.dev}")
+            if w.shape[0] > 1 and w.stride(0) != 1:
+                raise ValueError(f"{name} must be contiguous")
+            out.append(w.data_ptr())
+        return out[0], out[1], self.q_weight.dtype is r._f32
+
+
 class Rotary:
     """Rotary positions of heads of head_dim elements, the first rot_dim of them in pairs: (i, i +
     rot_dim / 2), or (2i, 2i + 1) with `adjacent`. Pair i turns by position * inv_freq[i] (default
@@ -241,6 +306,7 @@ class Rotary:
         self._fn, self._at = _entry("ea_hip_rotary"), self.dev.index
         self._bits, self._f32, self._i32, self._i64 = (torch.bfloat16, torch.int16), torch.float32, torch.int32, torch.int64
         self._half, self._axis = self.half_turns.data_ptr(), self.axis_of_pair.data_ptr()
+        self._norm_fn = self._grad_fn = None
 
     def _tokens(self, x, name, n=None):
         """Checks a (tokens, heads, head_dim) tensor, int16 standing for bf16 bits: (tokens, heads, fp32, strides)."""
@@ -289,9 +355,22 @@ class Rotary:
             raise ValueError(f"positions must be ({self.axes}, {n}), each axis contiguous")
         return n, hq, hk, wide, (sq[0], sq[1], sk[0], sk[1], sv[0], sv[1]), sp[0] if len(shape) == 2 else 0
 
-    def _launch(self, n, hq, hk, wide, strides, axis_stride, inverse, offset, so, sk, sv, rows, pool, inputs, outputs):
+    def _launch(self, n, hq, hk, wide, strides, axis_stride, inverse, offset, so, sk, sv, rows, pool, inputs, outputs, norm=None,
+                kv4=None):
         """strides: the inputs'; so, sk, sv: of q's, k's and v's output; rows, pool: theirs; inputs: addresses of q, k,
-        v and positions, outputs: of q_rows, dst_rows and the outputs."""
+        v and positions, outputs: of q_rows, dst_rows and the outputs; norm: HeadNorm; kv4: the KV4Pool written to."""
+        if norm is not None or kv4 is not None:
+            if self._norm_fn is None:
+                self._norm_fn = _entry("ea_hip_norm_rotary")
+            qw, kw, w32 = (0, 0, 0) if norm is None else norm._weights(self)
+            page = 0 if kv4 is None else kv4.Hkv * kv4.page_size * kv4.width
+            scales = (0, 0) if kv4 is None else (kv4.k_scales.data_ptr(), kv4.v_scales.data_ptr())
+            _call(self._norm_fn, _NORM.pack(
+                n, hq, hk, self.head_dim, self.rot_dim, self.axes, self.adjacent, inverse, wide, wide and not sv, offset, self.scale,
+                *strides, so[0], so[1], sk[0], sk[1], *(sv or (0, 0)), axis_stride, rows, pool, *inputs, self._half, self._axis,
+                *outputs, qw, kw, *scales, page, page, 0 if kv4 is None else kv4.page_size, w32, 0.0 if norm is None else norm.eps, 0),
+                self._at, "ea_hip_norm_rotary")
+            return
         _call(self._fn, _ROTARY.pack(n, hq, hk, self.head_dim, self.rot_dim, self.axes, self.adjacent, inverse, wide,
                                      wide and not sv, offset, self.scale, *strides, so[0], so[1], sk[0], sk[1],
                                      *(sv or (0, 0)), axis_stride, rows, pool, *inputs, self._half, self._axis, *outputs),
@@ -307,11 +386,21 @@ class Rotary:
                           (k_in or not q_out or _apart(q_out, k_out, d))):
             raise ValueError("k_out shares memory with q or q_out, or with k without being k")
 
-    def rotate(self, q, k, positions, *, inverse: bool = False, q_out=None, k_out=None):
+    def rotate(self, q, k, positions, *, inverse: bool = False, q_out=None, k_out=None, norm: HeadNorm | None = None):
         """q (tokens, Hq, head_dim) and k (tokens, Hkv, head_dim) turned by positions ((tokens,) or (axes,
         tokens) int32), into new tensors of their type or into q_out and k_out (which may be q and k
-        themselves). inverse turns back: the gradient of the rotation. Returns (q_out, k_out). Gradients of q
-        and k pass through, with q_out and k_out not given."""
+        themselves). inverse turns back: the gradient of the rotation. norm: every head is normed first (not with
+        inverse). Returns (q_out, k_out). Gradients of q, k and the norm's weights pass through, with q_out and k_out not
+        given."""
+        if norm is not None:
+            if inverse:
+                raise ValueError("the norm has no inverse")
+            if _C.is_grad_enabled() and any(x.requires_grad for x in (q, k, norm.q_weight, norm.k_weight)):
+                if q_out is not None or k_out is not None:
+                    raise ValueError("q_out and k_out take no part in gradients: leave them out, or call under no_grad")
+                if not (q.is_floating_point() and k.is_floating_point()):
+                    raise ValueError("bit patterns have no gradients: give bf16 or fp32")
+                return _norm_turn()(q, k, norm.q_weight, norm.k_weight, positions, self, norm.eps)
         if (q.requires_grad or k.requires_grad) and _C.is_grad_enabled():
             if q_out is not None or k_out is not None:
                 raise ValueError("q_out and k_out take no part in gradients: leave them out, or call under no_grad")
@@ -338,8 +427,42 @@ class Rotary:
                                (to_q, n, hq, so[0], so[1], e) if given[0] else None,
                                (to_k, n, hk, sk[0], sk[1], e) if given[1] else None)
         self._launch(n, hq, hk, wide, strides, axis_stride, bool(inverse), 0, so, sk, None, n, n,
-                     (qp, kp, 0, positions.data_ptr()), (0, 0, to_q, to_k, 0))
+                     (qp, kp, 0, positions.data_ptr()), (0, 0, to_q, to_k, 0), norm)
         return q_out, k_out
+
+    def _norm_grad(self, q, k, qw, kw, eps, positions, gq, gk, want_qw, want_kw):
+        """The gradients (q, k, q_weight, k_weight) of rotate(norm=) for those of its outputs (None: of an output that
+        nothing depends on, whose inputs get None)."""
+        import torch
+        have = gq is not None, gk is not None
+        if not any(have):
+            return (None,) * 4
+        xs = [x if h else x[:, :0] for x, h in zip((q, k), have)]
+        gs = [(g if g.stride(2) == 1 else g.contiguous()) if h else x for g, x, h in zip((gq, gk), xs, have)]
+        n, hq, hk, wide, strides, axis_stride = self._args(*xs, None, positions)
+        sg = [self._tokens(g, "the gradient", n)[3] for g in gs]
+        d = self.head_dim
+        out = [x.new_empty(x.shape) for x in xs]
+        want = want_qw and have[0], want_kw and have[1]
+        dw = [torch.empty_like(w) if y else None for w, y in zip((qw, kw), want)]
+        wq, wk, w32 = HeadNorm(qw, kw, eps)._weights(self)
+        if self._grad_fn is None:
+            self._grad_fn = _entry("ea_hip_norm_rotary_grad")
+
+        def pack(partial):
+            return _GRAD.pack(n, hq, hk, d, self.rot_dim, self.axes, self.adjacent, 0, wide, wide, 0, self.scale, *strides, hq * d, d,
+                              hk * d, d, 0, 0, axis_stride, n, n, xs[0].data_ptr(), xs[1].data_ptr(), 0, positions.data_ptr(),
+                              self._half, self._axis, 0, 0, out[0].data_ptr(), out[1].data_ptr(), 0, gs[0].data_ptr(),
+                              gs[1].data_ptr(), sg[0][0], sg[0][1], sg[1][0], sg[1][1], wq, wk,
+                              *(0 if w is None else w.data_ptr() for w in dw), partial, w32, eps)
+
+        args, partial = pack(0), None
+        if any(want):
+            size = hip.load().ea_hip_norm_rotary_grad_size(hip.NormRotaryGradArgs.from_buffer_copy(args))
+            partial = torch.empty(size // 8, dtype=torch.float64, device=self.dev)
+            args = pack(partial.data_ptr())
+        _call(self._grad_fn, args, self._at, "ea_hip_norm_rotary_grad")
+        return (out[0] if have[0] else None, out[1] if have[1] else None, *dw)
 
     def _check_target(self, out, at, n, hk, e, st, in_place, pools, size):
         """append's q_out is q (in_place: rows in q's order), or shares no memory with the inputs (at addresses `at`,
@@ -355,13 +478,18 @@ class Rotary:
                 if not _apart(out, x, d) and not (i == 0 and in_place and _same(out, x)):
                     raise ValueError("q_out shares memory with k or v, or with q without being q in its own rows")
 
-    def append(self, q, k, v, positions, dst_rows, k_pool, v_pool, *, q_rows=None, q_out=None, pos_offset: int = 0):
+    def append(self, q, k, v, positions, dst_rows, k_pool, v_pool=None, *, q_rows=None, q_out=None, pos_offset: int = 0,
+               norm: HeadNorm | None = None):
         """A step's tokens into the cache: q and k turned by positions (+ pos_offset), k and v (tokens, Hkv,
         head_dim) to rows dst_rows (int64, page * page_size + slot; rows outside the pool, such as -1, are
         skipped) of the pools [pages, page_size, Hkv, head_dim], bf16. The rotated q goes to a new bf16
         tensor of q's shape, or to rows q_rows (int64; rows outside are skipped) of q_out (rows, Hq,
         head_dim). Returns it, without a gradient. Rows that no token names are not written; a row may be named
-        once."""
+        once. With a KV4Pool as k_pool (and no v_pool) k and v are written in 4 bits. norm: the heads of q and k are
+        normed first."""
+        four = isinstance(k_pool, KV4Pool)
+        if four:
+            return self._append4(q, k, v, positions, dst_rows, k_pool, v_pool, q_rows, q_out, pos_offset, norm)
         n, hq, hk, wide, strides, axis_stride = self._args(q, k, v, positions)
         if not -1 << 31 <= pos_offset < 1 << 31:
             raise ValueError("pos_offset must fit 32 bits")
@@ -392,8 +520,125 @@ class Rotary:
         to = _vec(dst_rows, "dst_rows", at, i64, n)
         self._launch(n, hq, hk, wide, strides, axis_stride, False, pos_offset, so, (hk * d, d), (hk * d, d), rows, slots,
                      (qp, kp, vp, positions.data_ptr()),
-                     (0 if q_rows is None else _vec(q_rows, "q_rows", at, i64, n), to, q_out.data_ptr(), to_k, to_v))
+                     (0 if q_rows is None else _vec(q_rows, "q_rows", at, i64, n), to, q_out.data_ptr(), to_k, to_v), norm)
         return q_out
+
+    def _append4(self, q, k, v, positions, dst_rows, pool, v_pool, q_rows, q_out, pos_offset, norm):
+        """append into a KV4Pool."""
+        n, hq, hk, wide, strides, axis_stride = self._args(q, k, v, positions)
+        if v_pool is not None:
+            raise ValueError("a KV4Pool holds both k and v")
+        if not -1 << 31 <= pos_offset < 1 << 31:
+            raise ValueError("pos_offset must fit 32 bits")
+        at, d, i64 = self._at, self.head_dim, self._i64
+        if pool.dev != self.dev or pool.Hkv != hk or pool.head_dim != d:
+            raise ValueError(f"the pool must hold {hk} heads of {d} on {self.dev}")
+        if self.rot_dim % 4:
+            raise ValueError("rot_dim must be a multiple of 4 with a cache in 4 bits")
+        qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
+        mine = (pool.k, pool.k_scales, pool.v, pool.v_scales)
+        if q_out is None:
+            if q_rows is not None:
+                raise ValueError("q_rows needs q_out")
+            q_out = q.new_empty((n, hq, d), dtype=self._bits[0])
+            rows, so = n, (hq * d, d)
+        else:
+            rows, ho, w, so = self._target(q_out, "q_out")
+            if w or ho != hq or (q_rows is None and rows < n):
+                raise ValueError("q_out must be (rows, Hq, head_dim) bf16 (or int16), a row per token without q_rows")
+            for t in mine:
+                self._check_target((q_out.data_ptr(), n if q_rows is None else rows, hq, so[0], so[1], 2), (qp, kp, vp), n, hk,
+                                   4 if wide else 2, strides, q_rows is None, (t.data_ptr(),), t.numel())
+        to = _vec(dst_rows, "dst_rows", at, i64, n)
+        slot, head = pool.width, pool.page_size * pool.width
+        self._launch(n, hq, hk, wide, strides, axis_stride, False, pos_offset, so, (slot, head), (slot, head), rows,
+                     pool.num_pages * pool.page_size, (qp, kp, vp, positions.data_ptr()),
+                     (0 if q_rows is None else _vec(q_rows, "q_rows", at, i64, n), to, q_out.data_ptr(), pool.k.data_ptr(),
+                      pool.v.data_ptr()), norm, pool)
+        return q_out
+
+
+def append_kv4(pool: KV4Pool, k, v, dst_rows) -> None:
+    """KV4Pool.append: the norm and rotation's kernel with neither."""
+    import torch
+    d = pool.head_dim
+    for name, x in (("k", k), ("v", v)):
+        if x.dim() != 3 or tuple(x.shape) != (k.shape[0], pool.Hkv, d) or x.device != pool.dev or x.dtype != k.dtype:
+            raise ValueError(f"{name} must be (tokens, {pool.Hkv}, {d}) on {pool.dev}, both of one type")
+        if x.dtype not in (torch.bfloat16, torch.int16, torch.float32) or (x.numel() and x.stride(2) != 1):
+            raise ValueError(f"{name} must be bf16 (or int16) or fp32 with a contiguous last dimension")
+    n, slot, head = k.shape[0], pool.width, pool.page_size * pool.width
+    to = _vec(dst_rows, "dst_rows", pool.dev.index, torch.int64, n)
+    page = pool.Hkv * head
+    _call(_entry("ea_hip_norm_rotary"), _NORM.pack(
+        n, 0, pool.Hkv, d, 0, 1, 0, 0, k.dtype == torch.float32, 0, 0, 1.0, 0, 0, k.stride(0), k.stride(1), v.stride(0), v.stride(1), 0, 0,
+        slot, head, slot, head, 0, 0, pool.num_pages * pool.page_size, 0, k.data_ptr(), v.data_ptr(), 0, 0, 0, 0, to, 0,
+        pool.k.data_ptr(), pool.v.data_ptr(), 0, 0, pool.k_scales.data_ptr(), pool.v_scales.data_ptr(), page, page, pool.page_size, 0,
+        0.0, 0), pool.dev.index, "ea_hip_norm_rotary")
+
+
+class DraftCheck:
+    """Which drafted tokens of num_seqs sequences stand, num_drafts nodes of each at most, over `vocab` tokens. verify()
+    writes these int32 tensors, made once here (a captured graph can hold them; one object's calls must not overlap):
+
+      accepted (num_seqs,)                how many nodes stand
+      path (num_seqs, num_drafts)         they, in order; -1 past them. What ExactAttentionBackend.accept takes
+      tokens (num_seqs, num_drafts + 1)   their tokens, then the new one; -1 past it
+    """
+
+    def __init__(self, num_seqs: int, num_drafts: int, vocab: int, device="cuda"):
+        import torch
+        if not 0 <= num_seqs <= 65535 or not 0 <= num_drafts <= 64 or not 0 < vocab <= 1 << 19:
+            raise ValueError("at most 65535 sequences, 64 drafted nodes and 2^19 tokens")
+        self.dev = torch.empty(0, device=device).device
+        if self.dev.type != "cuda":
+            raise ValueError("the check of drafted tokens runs on the GPU")
+        self.num_seqs, self.num_drafts, self.vocab = num_seqs, num_drafts, vocab
+        self._fn, self._at, self._i32, self._f32 = _entry("ea_hip_draft_check"), self.dev.index, torch.int32, torch.float32
+        i32 = dict(dtype=torch.int32, device=self.dev)
+        self.accepted = torch.empty(num_seqs, **i32)
+        self.path = torch.empty((num_seqs, num_drafts), **i32)
+        self.tokens = torch.empty((num_seqs, num_drafts + 1), **i32)
+        size = hip.load().ea_hip_draft_check_size(hip.DraftCheckArgs(num_seqs=num_seqs))
+        self._work = torch.zeros(size // 8, dtype=torch.int64, device=self.dev)
+        self._out = tuple(t.data_ptr() for t in (self.accepted, self.path, self.tokens, self._work))
+
+    def _rows(self, x, name, n):
+        B, V = self.num_seqs, self.vocab
+        if tuple(x.shape) != (B, n, V) or x.dtype is not self._f32 or x.get_device() != self._at:
+            raise ValueError(f"{name} must be ({B}, {n}, {V}) fp32 on {self.dev}")
+        st = x.stride()
+        if V > 1 and st[2] != 1 and B * n:
+            raise ValueError(f"{name} needs a contiguous last dimension")
+        return x.data_ptr(), st[0], st[1]
+
+    def verify(self, probs, drafted, uniforms, *, draft_probs=None, parents=None, counts=None) -> None:
+        """probs (num_seqs, num_drafts + 1, vocab) fp32: the target's probabilities after the prefix and after each node (rows
+        may lie apart); drafted (num_seqs, num_drafts) int32: the nodes' tokens; uniforms (num_seqs, num_drafts + 1)
+        fp32: random numbers in [0, 1), a node's each and the new token's; counts (num_seqs,) int32: nodes of each
+        sequence (None: all).
+
+        draft_probs (num_seqs, num_drafts, vocab) fp32: the distributions that the nodes of a chain were drawn from; without
+        them the tokens are taken as given, and parents (num_seqs, num_drafts) int32 (a node's parent comes before it, -1: the
+        prefix) may make them a tree, as verify_tree takes it. Either way the tokens follow the target's distribution."""
+        B, N, at = self.num_seqs, self.num_drafts, self._at
+        if draft_probs is not None and parents is not None:
+            raise ValueError("trees are of given tokens: draft_probs are of a chain")
+        p, ps, pr = self._rows(probs, "probs", N + 1)
+        q, qs, qr = (0, 0, 0) if draft_probs is None else self._rows(draft_probs, "draft_probs", N)
+        ints = [0 if x is None else _vec(x, name, at, self._i32, n)
+                for x, name, n in ((drafted, "drafted", B * N), (parents, "parents", B * N), (counts, "counts", B))]
+        u = _vec(uniforms, "uniforms", at, self._f32, B * (N + 1))
+        for x, n in zip(ints, (B * N, B * N, B)):
+            for out in (self.accepted, self.path, self.tokens):
+                if x and n and out.numel() and x < out.data_ptr() + 4 * out.numel() and out.data_ptr() < x + 4 * n:
+                    raise ValueError("an input is one of the check's own outputs: copy it")
+        _call(self._fn, _DRAFT.pack(B, N, self.vocab, 0, ps, pr, qs, qr, p, q, ints[0], u, ints[1], ints[2], *self._out),
+              at, "ea_hip_draft_check")
+
+    def paths(self) -> list:
+        """Waits for the check: the nodes that stand, a list for each sequence (accept's path)."""
+        return [[i for i in p if i >= 0] for p in self.path.tolist()]
 
 
 def _deal(sections, half: int, interleaved: bool):

@@ -462,6 +462,112 @@ typedef struct ea_rotary {
 } ea_rotary;
 int ea_hip_rotary(const ea_rotary* a, ea_stream_t stream);
 
+/* Caches held in 4 bits, in the microscaling format of 4-bit floats: an element is a sign, 2 bits of exponent and 1 of
+ * mantissa (0, 0.5, 1, 1.5, 2, 3, 4, 6), element 2 i of a row in the low half of byte i, and a byte b scales 32
+ * consecutive ones by 2^(b - 127) (255: NaN). Every value is a bf16, so attention over such a cache is defined as, and
+ * equals to the bit, attention over the bf16 cache of its values; values past the largest bf16 are infinities.
+ * ea_hip_attention_kv4 is ea_hip_attention_mods (m may be NULL) with b->k and b->v pointing at codes and x at the scales.
+ * The geometry's strides count elements and are multiples of 32: an element at offset e has its code in byte e / 2 and its
+ * scale in byte e / 32, so a row of d elements takes whole groups, (d + 31) / 32 scales. head_dim and head_dim_v are multiples
+ * of 8, pages (with a block table) hold 16 slots or more, codes start on 16 bytes. Refused: digit-tile caches, phase
+ * timers, EA_KERNEL_DECODE and EA_KERNEL_GENERAL (-2), strides, pages and pointers other than these, or so large that 32
+ * slots span 2^29 elements (-1).
+ * ea_hip_kv4_workspace_size, ea_hip_exact_rows_kv4: the workspace and the host's exact tier of such a step.
+ * ea_hip_kv4_values: rows of whole groups (codes, scales) -> rows of head_dim bf16, both dense. No reference
+ * counterpart. */
+typedef struct ea_kv4 {
+    const uint8_t* k_scales;
+    const uint8_t* v_scales;
+} ea_kv4;
+int ea_hip_attention_kv4(const ea_geometry* g, const ea_buffers* b, const ea_options* o, const ea_score_mods* m, const ea_kv4* x,
+                         void* workspace, size_t workspace_bytes, ea_stream_t stream);
+int ea_hip_kv4_workspace_size(const ea_geometry* g, const ea_options* o, const ea_score_mods* m, size_t* bytes, int32_t* nsplit);
+int ea_hip_exact_rows_kv4(const ea_geometry* g, const ea_buffers* b, const ea_options* o, const ea_score_mods* m, const ea_kv4* x,
+                          ea_stream_t stream);
+int ea_hip_kv4_values(int64_t rows, int32_t head_dim, const uint8_t* codes, const uint8_t* scales, uint16_t* values,
+                      ea_stream_t stream);
+
+/* ea_hip_rotary with a norm of every query and key head in front, into a bf16 or a 4-bit cache.
+ *   norm   x -> x rsqrt(mean x^2 + eps) w over the head's elements, w = q_weight or k_weight (head_dim entries, bf16, or fp32
+ *          with weights_fp32); both NULL: none
+ *   turn   as ea_rotary says; half_turns NULL (with rot_dim 0): none
+ *   4 bit  with k_scales and v_scales set, k_out and v_out are codes. Row r of dst_rows is slot r % page_size of page
+ *          r / page_size, at element (r / page_size) page_stride + (r % page_size) ko_tok_stride + head ko_head_stride (vo alike; multiples
+ *          of 32). A group's scale is the smallest 2^e with max|x| < 7 2^e, e in [-125, 125], so that no element
+ *          below 7 2^125 is off by more than half a step; elements go to the nearest, ties to the even code, larger ones to 6 2^125. A group
+ *          with a NaN, an infinity or a value past fp32's becomes scale 255. Codes past head_dim are left alone.
+ * Everything is computed in fp64 and rounded once. head_dim is even or at most 128. r.inverse is refused with a norm. In
+ * 4 bits head_dim is a multiple of 8 and rot_dim of 4. r.q_out may be r.q and r.k_out r.k (bf16 or fp32) as with
+ * ea_hip_rotary. Returns as ea_hip_rotary. */
+typedef struct ea_norm_rotary {
+    ea_rotary r;
+    const void* q_weight;
+    const void* k_weight;
+    uint8_t* k_scales;
+    uint8_t* v_scales;
+    int64_t k_page_stride, v_page_stride;
+    int32_t page_size, weights_fp32;
+    float eps;
+    int32_t pad0;
+} ea_norm_rotary;
+int ea_hip_norm_rotary(const ea_norm_rotary* a, ea_stream_t stream);
+
+/* Its gradient (without v, rows or a 4-bit cache): r.q and r.k are the inputs of the forward call, gq and gk the gradients of
+ * its outputs (the inputs' type), r.q_out and r.k_out take those of q and k, dq_weight and dk_weight those of the weights, in
+ * their type (NULL: not wanted). With g = R^T gout, xh = x rsqrt(mean x^2 + eps):
+ *   dx = rsqrt(mean x^2 + eps) (g w - xh mean(g w xh)),   dw = sum over tokens and heads of g xh
+ * in fp64, the sums in an order that the sizes alone decide. partial: a workspace of ea_hip_norm_rotary_grad_size(a) bytes.
+ * r.q_out may not be r.q. */
+typedef struct ea_norm_rotary_grad {
+    ea_rotary r;
+    const void* gq;
+    const void* gk;
+    int64_t gq_tok_stride, gq_head_stride, gk_tok_stride, gk_head_stride;
+    const void* q_weight;
+    const void* k_weight;
+    void* dq_weight;
+    void* dk_weight;
+    double* partial;
+    int32_t weights_fp32;
+    float eps;
+} ea_norm_rotary_grad;
+size_t ea_hip_norm_rotary_grad_size(const ea_norm_rotary_grad* a);
+int ea_hip_norm_rotary_grad(const ea_norm_rotary_grad* a, ea_stream_t stream);
+
+/* Which drafted tokens stand. Sequence b has counts[b] (NULL: num_drafts) drafted nodes, node i after node parents[b][i] < i
+ * (-1: the prefix; parents NULL: a chain, node i after node i - 1). probs[b][0] holds the target's probabilities after the prefix,
+ * probs[b][1 + i] those after node i; uniforms[b][i] is node i's random number in [0, 1) and uniforms[b][num_drafts] the new token's.
+ *   with draft_probs[b][i], the distribution that chain node i was drawn from: it stands where those before it do and
+ *     u_i q(x_i) < p(x_i); after the first that does not, the new token comes from max(p - q, 0), after the last one from p
+ *   without: a node's children are tried in order, child i standing where u_i (1 - m) < p(x_i), m the mass of the siblings that
+ *     did not (a token counts once: a second node of it does not stand); after the last node that stands the new token comes from p without
+ *     the tokens of its children
+ * Both leave the target's distribution as it is. Tests are made in fp64. The new token is the first whose running sum of
+ * weights floor(2^44 w) exceeds u times their total (products in fp64, sums in integers: no order of summation changes it); probabilities are
+ * clipped to [0, 1], NaN is 0. Where no weight is left, p itself is taken, and without any the token is -1.
+ *   accepted[b]: nodes that stand;  path[b][..]: they, in order, then -1;  tokens[b][0 .. num_drafts]: their tokens, the new
+ *   one, then -1
+ * A node with a token outside the vocabulary or a parent at or past it does not stand. num_drafts <= 64, vocab <= 2^19; rows of
+ * probs and draft_probs dense, their strides in elements. work: ea_hip_draft_check_size(a) bytes, zero before the first call and left
+ * so; calls that share it must not overlap. All pointers are device memory. Enqueue only, capturable. Returns 0, -1 on bad arguments,
+ * -100 - e on a HIP error. No reference counterpart. */
+typedef struct ea_draft_check {
+    int32_t num_seqs, num_drafts, vocab, pad0;
+    int64_t p_seq_stride, p_row_stride, q_seq_stride, q_row_stride;
+    const float* probs;
+    const float* draft_probs;
+    const int32_t* drafted;  /* [num_seqs][num_drafts] */
+    const float* uniforms;   /* [num_seqs][num_drafts + 1] */
+    const int32_t* parents;
+    const int32_t* counts;
+    int32_t* accepted;
+    int32_t* path;
+    int32_t* tokens;
+    uint64_t* work;
+} ea_draft_check;
+size_t ea_hip_draft_check_size(const ea_draft_check* a);
+int ea_hip_draft_check(const ea_draft_check* a, ea_stream_t stream);
+
 /* Library version string. */
 const char* ea_hip_version(void);
 
