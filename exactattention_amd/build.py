@@ -8,7 +8,7 @@ import sys
 import tempfile
 from concurrent.futures import ThreadPoolExecutor
 
-SOURCES = ["ea_hip.hip", "ea_decode.hip", "ea_mrow.hip", "ea_mrow4.hip", "ea_prefill.hip", "ea_prefill_mod.hip",
+SOURCES = ["ea_hip.hip", "ea_decode.hip", "ea_mrow.hip", "ea_four.hip", "ea_prefill.hip", "ea_prefill_mod.hip",
            "ea_step.hip", "ea_norm.hip", "ea_draft.hip", "ea_exact_host.cpp", "ea_csr.cpp"]
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -23,7 +23,7 @@ HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
                "-fno-gpu-flush-denormals-to-zero", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
                "-mllvm", "-amdgpu-mfma-vgpr-form=1", "-Wall", "-Wno-unused-function"]
 # and for one source alone; the reason stands there
-FILE_FLAGS = {"ea_prefill_mod.hip": ["-mllvm", "-disable-machine-licm=1"]}
+FILE_FLAGS = {f: ["-mllvm", "-disable-machine-licm=1"] for f in ("ea_prefill_mod.hip", "ea_four.hip")}
 
 
 def build(verbose: bool = False) -> str:

@@ -137,7 +137,7 @@ __device__ inline int combine_row(const Params& P, int64_t row, int lane) {
         } else {
             A += zs * (double)(min((int64_t)n + 4, dcap) + nsb);
         }
-        nterm += n > 0 ? n : 0;
+        nterm += n > 0 ? (P.ks ? (n >> 10) + 1 : n) : 0;  // the 4-bit kernel's counts hold its own error too
     };
     add_z(n0, r0, z0);
     for (int j = 1; j < J; ++j) {
@@ -153,7 +153,7 @@ __device__ inline int combine_row(const Params& P, int64_t row, int lane) {
         A += __shfl_xor(A, o, 64);
         nterm += __shfl_xor(nterm, o, 64);
     }
-    const double tiny = (double)(nterm + 64 * nsb + 64) * 0x1p-1074;
+    const double tiny = ((double)nterm * (P.ks ? 1024.0 : 1.0) + (double)(64 * nsb + 64)) * 0x1p-1074;
     const double eZ = A * up + tiny;
     if (!(Z > 2.0 * eZ) || !isfinite(Z)) flag = 1;
     bool ok = !flag;

@@ -1,0 +1,956 @@
+// Tier-1 split kernel for caches held in 4 bits (ea_kv4.h) on the low-precision matrix instructions (gfx950): certified sums, as
+// the other split kernels', whose partials the same combine merges.
+//
+// What a 4-bit cache changes: a key's element is a 4-bit float under a power of two, which v_mfma_scale_f32_16x16x128_f8f6f4
+// multiplies as it stands, scale included. The fp64 kernels convert every element and pay 16 MACs a cycle and SIMD; here a key's 128
+// elements are one instruction of 16 cycles for 16 columns.
+//
+//   scores   q is cut once into 6 balanced digits of 5 bits, -16 .. 15, each a 6-bit float (3 of mantissa: the code of a
+//            magnitude is the magnitude). A product of a digit and an element is a whole number of halves, at most 192; 128 of
+//            them, and scales up to 2^9 apart, are below 2^24 units: the instruction's fp32 sum is exact, in any order. The 6 sums join
+//            in fp64 exactly, 49 bits, so the score of a pair is exact, and the certified logit almost always decided. What elements
+//            far below the row's top leave (one of a row's 128 is 2^-20 of the largest in some rows of every step) takes 6 digits
+//            more, in blocks of rows that have any; what those leave is counted and bounded. Keys whose scales lie further apart are
+//            left to the exact path.
+//   weights  w = RN24(2^t) = M 2^E (cert_pairs), their exponents against a base per row
+//   P.V      V's scale belongs to its key, a summand: it moves into the weight. For each group of 32 channels the weight
+//            W = RN(M 2^(E + b - G - base)) <= 2^46 (b the scale's byte, G the group's largest) becomes 6 balanced digits of 8 bits,
+//            read out of an fp64 sum with 2^52, and v_mfma_i32_16x16x64_i8 sums them over 64 keys with the elements as
+//            whole numbers (-12 .. 12, byte lookups). int32 sums are exact; a base that must move folds them into fp64.
+//            The rounding of W is the one error: half a unit of 2^(base + G) a key.
+//
+// What bounds it is the VALU, with 2 waves a SIMD (the int32 sums alone are 64 registers of 4 rows, 96 of 8): of a tile of 64 keys and 4
+// rows 48 instructions for the scores, 200 for the certified weights, 88 a group of 32 channels, half of them for V's bytes. A step of 32
+// ragged sequences to 4096 keys, 32/8 heads: 65 us, 69 on the fp64 matrix instructions; 8 of 30000 to 131072, 16/8 heads: 249, 437.
+//
+// Layout. A block is 4 waves over one (segment, block of RS = 4 or 8 rows, key range); wave w takes 64-key tiles w, w + 4, .. and
+// meets the others in the epilogue only. Lane l: g = l / 16, n = l % 16; its pairs are those of its rows, RS / 4 from (RS / 4) g, with
+// the keys 4 n + u (u = 0..3) of the tile.
+//   q     digits in registers, the A operand (M = a row's digit, K = dim): with M = 4 g + i in the order of the rows, the 4 sums of
+//         D that a lane gets are digits of its own rows: 2 instructions a key of 4 rows, 3 of 8, and nothing passes between lanes
+//   K     lane loads dims 32 g .. + 31 of the keys 4 n + u (16 bytes and a scale each): the B operand (K = dim, N = key)
+//   W     digits to LDS, [plane][row][64 keys]; A operand (M = plane and row, K = key): 4 rows: planes 0, 1 and 2..5; 8 rows:
+//         planes 0, 1 and 2, 3 and 4, 5, the rows in an order that leaves a lane the sums of its own rows
+//   V     l = 0..3: lane loads channels 32 l + 2 n and + 1 of keys 16 g .. + 15 (16 bytes): two B operands (K = key, N = channel)
+//   O     fp64 sums, in LDS: they change only where int32 sums are folded into them
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "ea_kv4.h"
+#include "ea_params.h"
+#include "ea_pf_common.h"
+
+using namespace ea;
+
+namespace {
+
+constexpr int F4_THREADS = 256;
+constexpr int F4_NONE = -1200000000;  // base of a row without a visible key so far
+constexpr int F4_BITS = 22;           // a weight's exponent E may exceed the base by this: M < 2^24 then gives 46 bits
+constexpr int F4_HEAD = 2;            // room left when the base moves
+constexpr int F4_SPREAD = 9;          // of a key's scales, for exact sums
+constexpr int F4_LIST = 64;
+constexpr int F4_EPOCH = 16384;       // tiles between folds at most: 2^14 x 64 keys x 128 x 12 < 2^31
+constexpr int F4_WROW = 20;           // dwords a row of 64 digits takes (16 and 4 that spread the rows over the banks)
+typedef int f4_i8 __attribute__((ext_vector_type(8)));
+typedef int f4_i4 __attribute__((ext_vector_type(4)));
+typedef float f4_f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t f4_u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t f4_u2 __attribute__((ext_vector_type(2)));
+typedef unsigned short f4_h2 __attribute__((ext_vector_type(2)));
+
+template <int RS, int NG>
+struct FourSmem {
+    uint32_t q6[2][RS * 6 * 24];  // q's digits [row][digit][32-dim block][6 dwords], and those of what they leave
+    uint32_t zero[8];
+    double T1[256], T2[256];  // exp2 tables, T1 times 2^23
+    double rq[RS], rqe[RS];   // 2^(lsb + 3); |alpha| times the sum of |q| that both rounds lost
+    int bad[RS], more[RS], kvl[RS];
+    uint64_t tmk[RS];
+    int kvb[RS], pos[RS];  // with score modifications
+    float slope[RS];
+    double wZ[4][RS], we[4][RS];
+    int wR[4][RS], wf[4][RS], wn[4];
+    uint32_t wv[4][4];  // per wave and group: the largest scale
+    uint32_t list[4][F4_LIST + 64 * RS];
+    double O[4][RS][32 * NG];  // per wave: of channel 32 l + 2 n + h at 32 l + 16 h + n
+    union alignas(16) {
+        uint32_t W[4][6 * RS * F4_WROW];
+        uint8_t dig[2][RS * 6 * 128];
+    };
+};
+
+// x of the lane 16 (32) lanes away
+__device__ __forceinline__ double xor16(double x) { return __shfl_xor(x, 16, 64); }
+__device__ __forceinline__ double xor32(double x) { return __shfl_xor(x, 32, 64); }
+__device__ __forceinline__ f4_h2 pk_max(f4_h2 a, f4_h2 b) { return __builtin_elementwise_max(a, b); }
+
+// The bytes of 4 elements, whole numbers of halves, from the low (HI = false) or high halves of 4 bytes: 0, 1, 2, 3, 4, 6, 8, 12 and
+// their negatives. A byte permutation looks up 8 entries; selectors 8 to 11 give the signs of the table's odd entries (0 or 0xFF), 12
+// gives 0 and 13 to 15 0xFF. So P[x] ^ N[x ^ 8] has both halves of the code in one place, each table holding its entries XORed with what the
+// other one gives there:
+//   P[i] = v_i ^ b_i, b_0..3 the signs of N[1], N[3], N[5], N[7], b_4 = 0, b_5..7 = 0xFF; N[i] = -v_i ^ a_i, a from P's signs alike
+//   P[5] = ~6 and P[7] = ~12 are negative, N[5] = ~-6 = 5 and N[7] = ~-12 = 11 positive: b_2 = b_3 = 0, so P[3] = 3, a_1 = 0 and
+//   N[1] = -1: b_0 = 0xFF; a_3 = 0xFF makes N[3] = ~-3 = 2 positive: b_1 = 0 and P[1] = 1, a_0 = 0; a_2 = 0xFF
+template <bool HI>
+__device__ __forceinline__ uint32_t four_bytes(uint32_t w) {
+    constexpr uint32_t M = 0x0F0F0F0Fu;
+    constexpr uint32_t p[8] = {0, 1, 2, 3, 4, 6, 8, 12};
+    constexpr auto neg = [](uint32_t x) { return (0u - x) & 0xFFu; };
+    constexpr uint32_t P0 = (p[0] ^ 0xFFu) | p[1] << 8 | p[2] << 16 | p[3] << 24;
+    constexpr uint32_t P1 = p[4] | (p[5] ^ 0xFFu) << 8 | (p[6] ^ 0xFFu) << 16 | (p[7] ^ 0xFFu) << 24;
+    constexpr uint32_t N0 = neg(p[0]) | neg(p[1]) << 8 | (neg(p[2]) ^ 0xFFu) << 16 | (neg(p[3]) ^ 0xFFu) << 24;
+    constexpr uint32_t N1 = neg(p[4]) | (neg(p[5]) ^ 0xFFu) << 8 | (neg(p[6]) ^ 0xFFu) << 16 | (neg(p[7]) ^ 0xFFu) << 24;
+    const uint32_t s = HI ? w >> 4 : w;
+    const uint32_t x = s & M, y = (s & M) ^ 0x08080808u;
+    return __builtin_amdgcn_perm(P1, P0, x) ^ __builtin_amdgcn_perm(N1, N0, y);
+}
+
+}  // namespace
+
+// MOD: with score modifications (ea_mod.h): 1 key ranges alone, 2 with a bias, 3 with a cap; a unit's key range is then counted from its
+// rows' first visible key, down to a whole tile, and on uniform splits the last split takes every key past the others.
+template <int RS, int NG, int MOD>
+__global__ void __launch_bounds__(F4_THREADS, 2) ea_four(Params P) {
+    constexpr int RL = RS / 4;            // rows of a lane
+    constexpr int NMF = RS == 4 ? 2 : 3;  // matrix instructions for 6 digits of the rows
+    typedef FourSmem<RS, NG> Smem;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    Smem& S = *reinterpret_cast<Smem*>(smem_raw);
+    const int tid = (int)threadIdx.x;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int d = P.g.head_dim, dv = P.g.head_dim_v;
+    const int wid = kv4_width(dv), ng = wid >> 5;  // V's channels in whole groups
+
+    S.T1[tid] = u64_as_f64(EA_T1_BITS[tid]) * 8388608.0;  // 2^23: exact
+    S.T2[tid] = u64_as_f64(EA_T2_BITS[tid]);
+    if (tid < 8) S.zero[tid] = 0;
+    if (blockIdx.x == 0 && blockIdx.y == 0) {
+        // on uniform splits the step's first kernel clears the tier-2 work list and chunk counts
+        if (!P.dq_stream && tid < EA_T2_CNT) P.wl_cnt[tid] = 0;
+        if (tid == 0 && P.stats) atomicAdd((unsigned long long*)&P.stats[9], (unsigned long long)P.rows);
+        if (tid == 0 && P.stats_x) atomicAdd((unsigned long long*)&P.stats_x[0], (unsigned long long)P.rows);
+    }
+
+    // One piece: keys [kA, kB) of unit `item` (segment, row block), clipped to the unit's visible end, as partial slot `split`.
+    auto piece = [&](const int item, const int split, int kA, int kB) __attribute__((always_inline)) {
+        const int lane = tid & 63;
+        const int g = lane >> 4, n = lane & 15;
+        const int seg = item / P.nrb, rbk = item % P.nrb;
+        const int Hkv = P.g.num_kv_heads;
+        const int b = seg / Hkv, hk = seg % Hkv;
+        const int row0 = rbk * RS;
+        const int nrow = min(RS, P.r_seg - row0);
+        auto q_row = [&](int r) __attribute__((always_inline)) {
+            const int lr = row0 + r, t = lr / P.grp, gi = lr % P.grp;
+            return P.q + (int64_t)b * P.g.q_seq_stride + (int64_t)t * P.g.q_tok_stride + (int64_t)(hk * P.grp + gi) * P.g.q_head_stride;
+        };
+        // ---- q's digits: X = q / 2^lsb, |X| < 2^28, in 6 digits of 5 bits
+        for (int r = w; r < RS; r += 4) {
+            int m[2] = {0, 0}, e[2] = {0, 0}, bad = 0, lead = INT_MIN;
+            if (r < nrow) {
+                const uint16_t* qr = q_row(r);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int i = 2 * lane + h;
+                    const uint32_t x = i < d ? qr[i] : 0u;
+                    const int f = (x >> 7) & 0xFF;
+                    bad |= f == 0xFF;
+                    m[h] = (int)(x & 0x7F) | (f ? 0x80 : 0);
+                    e[h] = (f ? f : 1) - 134;
+                    if (m[h]) lead = max(lead, e[h] + 31 - __clz(m[h]));
+                    if (x & 0x8000) m[h] = -m[h];
+                }
+            }
+            lead = wave_max_dpp(lead);
+            bad = wave_max_dpp(bad);
+            const int lsb = lead == INT_MIN ? 0 : lead - 27;
+            // two rounds: q in units of 2^lsb, then what that leaves in units of 2^(lsb - 28): half a unit of the first at most,
+            // and nothing in most rows (with one round, a row whose smallest element is 20 binades below its largest leaves an
+            // eighth of its pairs to the exact path)
+            int lost = 0, more = 0;
+#pragma unroll
+            for (int k2 = 0; k2 < 2; ++k2) {
+                uint32_t y[2];
+                lost = 0;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int a = m[h] < 0 ? -m[h] : m[h], sh = e[h] - lsb + 28 * k2;
+                    int X = 0, rest = 0;
+                    if (a && !bad) {
+                        if (sh >= 0) {
+                            X = a << sh;
+                        } else {
+                            X = sh >= -10 ? (a + (1 << (-sh - 1))) >> -sh : 0;
+                            rest = sh >= -10 ? a - (X << -sh) : a;
+                        }
+                    }
+                    y[h] = (uint32_t)(m[h] < 0 ? -X : X) + 0x21084210u;
+                    m[h] = m[h] < 0 ? -rest : rest;
+                    lost += rest != 0;
+                }
+#pragma unroll
+                for (int k = 0; k < 6; ++k) {
+                    uint32_t c2 = 0;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int dk = (int)((y[h] >> (5 * k)) & 31u) - 16;
+                        c2 |= (dk < 0 ? 32u | (uint32_t)-dk : (uint32_t)dk) << (8 * h);
+                    }
+                    *(uint16_t*)&S.dig[k2][(r * 6 + k) * 128 + 2 * lane] = (uint16_t)c2;
+                }
+                if (k2 == 0) more = __ballot(lost != 0) != 0;
+            }
+            lost = wave_sum_i(lost);
+            if (lane == 0) {
+                S.bad[r] = bad;
+                S.more[r] = more;
+                S.rq[r] = ldexp(1.0, lsb + 3);
+                S.rqe[r] = fabs(P.alpha) * (double)lost * ldexp(0.5 * (1.0 + 0x1p-20), lsb - 28);
+            }
+        }
+        // ---- the rows' visible keys: prefix and tree mask in LDS (tiles inside every prefix do not read them), the last
+        // visible key and the shortest prefix of the block
+        const int slen = P.seq_len[b];
+        const int tb = P.tree_mask ? P.tree_base[b] : 0;
+        int kend = 0, kvmin = INT_MAX;
+        int kbeg = INT_MAX, kbmax = 0;  // MOD: the rows' first visible key, their last prefix start
+        {
+            const int r = lane & (RS - 1);
+            const int tok = b * P.g.num_tokens + (row0 + min(r, nrow - 1)) / P.grp;
+            const int kvl = P.kv_len[tok];
+            const uint64_t tmk = P.tree_mask ? P.tree_mask[tok] : 0ull;
+            kend = tmk ? max(kvl, tb + 64 - (int)__clzll(tmk)) : kvl;
+            kvmin = kvl;
+            if constexpr (MOD) {
+                const int kvb = vis_begin(P, tok, kvl);
+                kbmax = kvb;
+                const KeySpan ks = key_span(kvb, kvl, slen, tmk, tb);
+                kbeg = ks.beg;
+                kend = ks.end;
+                if (w == 0 && lane < RS) {
+                    S.kvb[r] = kvb;
+                    S.pos[r] = mod_pos(P, tok, kvl);
+                    const int lr = row0 + min(r, nrow - 1);
+                    S.slope[r] = mod_slope(P, hk * P.grp + lr % P.grp);
+                }
+            }
+            if (w == 0 && lane < RS) {
+                S.kvl[r] = r < nrow ? kvl : INT_MIN;
+                S.tmk[r] = r < nrow ? tmk : 0ull;
+            }
+        }
+        kend = min(wave_max_dpp(kend), slen);
+        kvmin = min(-wave_max_dpp(-kvmin), slen);
+        if constexpr (MOD) {
+            kbeg = -wave_max_dpp(-kbeg);
+            kbmax = wave_max_dpp(kbmax);
+            const int k0 = kend > 0 ? tile_floor(kbeg) : 0;
+            kA += k0;
+            kB += k0;
+        }
+        const int k1 = min(kB, kend);
+        const int k0w = kA + 64 * w;  // this wave's tiles: k0w + 256 it
+        const int nst = k1 > k0w ? (k1 - k0w + 255) >> 8 : 0;
+        __syncthreads();  // the digits are in LDS: 32 of a block to 24 bytes
+        int two = 0;  // does a row of the block need the second round?
+#pragma unroll
+        for (int r = 0; r < RS; ++r) two |= S.more[r];
+        two = __builtin_amdgcn_readfirstlane(two);
+        for (int x0 = tid; x0 < RS * 24 * (1 + two); x0 += F4_THREADS) {
+            const int k2 = x0 >= RS * 24, x = x0 - (k2 ? RS * 24 : 0);
+            const uint32_t* src = (const uint32_t*)&S.dig[k2][(x >> 2) * 128 + 32 * (x & 3)];
+            uint32_t c[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t y = src[j];  // 4 codes of 6 bits in bytes
+                c[j] = (y & 0x3Fu) | (y >> 2 & 0xFC0u) | (y >> 4 & 0x3F000u) | (y >> 6 & 0xFC0000u);
+            }
+            f4_u2* const o = (f4_u2*)&S.q6[k2][x * 6];
+            o[0] = (f4_u2){c[0] | c[1] << 24, c[1] >> 8 | c[2] << 16};
+            o[1] = (f4_u2){c[2] >> 16 | c[3] << 8, c[4] | c[5] << 24};
+            o[2] = (f4_u2){c[5] >> 8 | c[6] << 16, c[6] >> 16 | c[7] << 8};
+        }
+        __syncthreads();
+        // the lane's part of a row block's digits, instruction j: M = n is digit 4 j + n % 4 of the digits of the rows of n / 4
+        auto q_part = [&](int k2, int j) __attribute__((always_inline)) {
+            const int c = 4 * j + (n & 3), qr = RL * (n >> 2) + (c >= 6 ? 1 : 0), qk = c >= 6 ? c - 6 : c;
+            const uint32_t* const p = RS == 4 && c >= 6 ? S.zero : &S.q6[k2][((qr * 6 + qk) * 4 + g) * 6];
+            const f4_u2 x = *(const f4_u2*)p, y = *(const f4_u2*)(p + 2), t = *(const f4_u2*)(p + 4);
+            return (f4_i8){(int)x.x, (int)x.y, (int)y.x, (int)y.y, (int)t.x, (int)t.y, 0, 0};
+        };
+        f4_i8 qd[NMF];
+#pragma unroll
+        for (int j = 0; j < NMF; ++j) qd[j] = q_part(0, j);
+        const int row = RL * g;  // the lane's rows: row + j
+        cint_t* btb = (cint_t*)P.bt + (P.bt ? (P.bt_off ? P.bt_off[b] : (int64_t)b * P.g.block_table_stride) : 0);
+        const int pshift = P.pshift, pmask = (1 << pshift) - 1;
+        // 16 consecutive keys from a multiple of 16 (a run) lie in one page (page size >= 16) and are one tile of V. Runs past the
+        // last key (or, MOD, before the first) read the last one's again, as keys past the last one do within theirs, and weigh
+        // nothing. Offsets count 32 elements: 16 bytes, or one scale.
+        auto run_of = [&](int n0, int at) __attribute__((always_inline)) {
+            int m = min(n0 + 16 * at, k1 - 1);
+            if constexpr (MOD) m = max(m, kbeg);
+            return m & ~15;
+        };
+        struct Pages {
+            int k, v;
+        };
+        auto pages_of = [&](int n0) __attribute__((always_inline)) {
+            Pages p = {b, b};
+            if (P.bt) {
+                p.k = btb[run_of(n0, n >> 2) >> pshift];
+                p.v = btb[run_of(n0, g) >> pshift];
+            }
+            return p;
+        };
+        auto times = [](int x, int64_t stride) __attribute__((always_inline)) {  // x >= 0
+            return (uint64_t)(uint32_t)x * (uint32_t)stride + ((uint64_t)((uint32_t)x * (uint32_t)(stride >> 32)) << 32);
+        };
+        struct KR {
+            f4_u4 k[4];
+            uint32_t s[4];
+        };
+        struct VR {
+            f4_u4 v[NG];
+            uint32_t s[NG];
+        };
+        const int64_t kps = P.g.k_page_stride >> 5, kss = P.g.k_slot_stride >> 5, vps = P.g.v_page_stride >> 5;
+        const int gk = min(g, (d - 1) >> 5);  // blocks past the head: q's digits are zeros there
+        const char* const kbase = (const char*)P.k + (((int64_t)hk * P.g.k_head_stride) >> 1) + 16 * gk;
+        const uint8_t* const ksbase = P.ks + (((int64_t)hk * P.g.k_head_stride) >> 5) + gk;
+        const char* const vbase = (const char*)P.v + (((int64_t)hk * P.g.v_head_stride) >> 1) + 16 * n;
+        const uint8_t* const vsbase = P.vs + (((int64_t)hk * P.g.v_head_stride) >> 5) + 4 * (n & 3);
+        auto issue_k = [&](int n0, const Pages& p, KR& x) __attribute__((always_inline)) {
+            const int run = run_of(n0, n >> 2), lim = k1 - 1 - run;
+            const uint64_t at = times(p.k, kps) + times(P.bt ? run & pmask : run, kss);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const uint64_t to = at + (uint64_t)((uint32_t)min(4 * (n & 3) + u, lim) * (uint32_t)kss);
+                x.k[u] = *(const f4_u4*)(kbase + (to << 4));
+                x.s[u] = ksbase[to];
+            }
+        };
+        auto issue_v = [&](int n0, const Pages& p, VR& x) __attribute__((always_inline)) {
+            const int rv = run_of(n0, g), rs = run_of(n0, n >> 2);
+            const uint64_t at = times(p.v, vps) + times((P.bt ? rv & pmask : rv) >> 4, wid >> 1);
+            const uint64_t as = times(p.k, vps) + times((P.bt ? rs & pmask : rs) >> 4, wid >> 1);
+            const char* const vc = vbase + (at << 4);
+            const uint8_t* const vs = vsbase + as;
+#pragma unroll
+            for (int l = 0; l < NG; ++l) {
+                x.v[l] = l < ng ? *(const f4_u4*)(vc + 256 * l) : (f4_u4){0u, 0u, 0u, 0u};
+                x.s[l] = l < ng ? *(const uint32_t*)(vs + 16 * l) : 0u;
+            }
+        };
+
+        const double alpha = P.alpha;
+        double rq[RL], rqe[RL];
+        int rfl[RL];   // the row is left to tier 2
+        int base[RL];  // of the row
+        double z[RL], lostw[RL];  // the weights' sum, and what rounding took from their whole numbers
+#pragma unroll
+        for (int j = 0; j < RL; ++j) {
+            rq[j] = S.rq[row + j];
+            rqe[j] = S.rqe[row + j];
+            rfl[j] = S.bad[row + j];
+            base[j] = F4_NONE;
+            z[j] = lostw[j] = 0.0;
+        }
+        int G[NG];             // the groups' references, uniform
+        f4_h2 vm[NG];          // the largest scales the lane saw, of even and odd keys
+#pragma unroll
+        for (int l = 0; l < NG; ++l) {
+            G[l] = 0;
+            vm[l] = (f4_h2){0, 0};
+        }
+        int lo = -100000;      // scales of keys in [lo, lo + F4_SPREAD] need no closer look
+        double kbnd = 0.0;     // an upper bound of |k| for such keys
+        f4_i4 acc[NMF][2 * NG];
+        double* const O = &S.O[w][row][n];  // [j][c]: the lane's own
+#pragma unroll
+        for (int c = 0; c < 2 * NG; ++c) {
+#pragma unroll
+            for (int j = 0; j < NMF; ++j) acc[j][c] = (f4_i4){0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < RL; ++j) O[j * 32 * NG + 16 * c] = 0.0;
+        }
+        int since = 0, folds = 0;
+        int n5 = 0, n6 = 0, n8 = 0, cnt = 0;  // wave-uniform
+        const double gw = RS == 4 ? (g == 0 ? 1.0 : (g == 1 ? 0x1p8 : (g == 2 ? 0x1p16 : 0x1p24))) : (g < 2 ? 1.0 : 0x1p8);
+
+        // the int32 sums into the fp64 ones: digits joined, the lanes' parts added up, each lane left with its own rows
+        auto fold = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int l = 0; l < NG; ++l) {
+                const double unit = ldexp(gw, G[l] - 128);  // in halves of 2^(G - 127)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int c = 2 * l + h;
+                    double t[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        double x = (double)acc[NMF - 1][c][i];
+#pragma unroll
+                        for (int j = NMF - 2; j >= 0; --j) x = __fma_rn(x, 65536.0, (double)acc[j][c][i]);
+                        t[i] = x * unit;
+                    }
+                    const bool up = g >= 2;
+                    double a = up ? t[2] : t[0], e = up ? t[3] : t[1];
+                    a += xor32(up ? t[0] : t[2]);
+                    e += xor32(up ? t[1] : t[3]);
+                    if constexpr (RS == 4) {
+                        const bool odd = g & 1;
+                        O[16 * c] += (odd ? e : a) + xor16(odd ? a : e);
+                    } else {
+                        O[16 * c] += a;
+                        O[32 * NG + 16 * c] += e;
+                    }
+#pragma unroll
+                    for (int j = 0; j < NMF; ++j) acc[j][c] = (f4_i4){0, 0, 0, 0};
+                }
+            }
+            ++folds;
+            since = 0;
+        };
+        // a row's base to nb (the same in every lane of the row), after a fold
+        auto rebase = [&](int j, int nb) __attribute__((always_inline)) {
+            double f = 1.0;
+            if (nb != base[j]) {
+                if (base[j] != F4_NONE) {
+                    if (!MOD && base[j] - nb < -900) rfl[j] = 1;
+                    f = ldexp(1.0, max(base[j] - nb, -1000));
+                    z[j] *= f;
+                    lostw[j] *= f;
+                }
+                base[j] = nb;
+            }
+#pragma unroll
+            for (int c = 0; c < 2 * NG; ++c) O[j * 32 * NG + 16 * c] *= f;
+        };
+
+        auto tile = [&](int n0, bool more, KR& kr, VR& vr) __attribute__((always_inline)) {
+            Pages nx = {0, 0};
+            if (more) nx = pages_of(n0 + 256);
+            // ---- are the scales near enough to each other for exact sums?
+            uint32_t wide = 0;  // bit u: key 4 n + u is left to the exact path
+            {
+                uint32_t far = 0;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) far |= (uint32_t)((int)kr.s[u] - lo) > F4_SPREAD ? 1u : 0u;
+                if (__builtin_expect(__ballot(far != 0) != 0, 0)) {
+                    int top = 0;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const uint32_t any = (kr.k[u].x | kr.k[u].y | kr.k[u].z | kr.k[u].w) & 0x77777777u;
+                        const bool has = any != 0 || kr.s[u] == 255;  // groups of zeros take any scale
+                        int mx = has ? (int)kr.s[u] : 0, mn = has ? (int)kr.s[u] : 1000;
+                        mx = max(mx, __shfl_xor(mx, 16, 64));
+                        mn = min(mn, __shfl_xor(mn, 16, 64));
+                        mx = max(mx, __shfl_xor(mx, 32, 64));
+                        mn = min(mn, __shfl_xor(mn, 32, 64));
+                        // sums far from fp32's ends, too
+                        const bool off = mn != 1000 && (mx - mn > F4_SPREAD || mn < 40 || mx > 230);
+                        if (!has) kr.s[u] = 127;
+                        if (off) {
+                            wide |= 1u << u;
+                        } else if (mn != 1000) {
+                            top = max(top, mx);
+                        }
+                    }
+                    top = wave_max_dpp(top);
+                    if (top > 0) lo = max(top - (F4_SPREAD - 1), 40);
+                    kbnd = max(kbnd, 6.0 * ldexp(1.0, max(top, lo + F4_SPREAD) - 127));
+                }
+            }
+            const bool edge = n0 + 64 > min(kvmin, k1) || (MOD && n0 < kbmax);
+            const bool cut = n0 + 64 > k1 || (MOD && n0 < kbeg);
+            const int kn = n0 + 4 * n;  // the first of the lane's keys
+            // ---- scores: 6 exact sums for every pair
+            double sc[RL][4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const f4_i8 B = {(int)kr.k[u].x, (int)kr.k[u].y, (int)kr.k[u].z, (int)kr.k[u].w, 0, 0, 0, 0};
+                f4_f4 D[NMF];
+#pragma unroll
+                for (int j = 0; j < NMF; ++j)
+                    D[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(qd[j], B, (f4_f4){0.0f, 0.0f, 0.0f, 0.0f}, 2, 4, 0, 127, 0,
+                                                                            (int)kr.s[u]);
+#pragma unroll
+                for (int j = 0; j < RL; ++j) {
+                    double x = (double)D[(6 * j + 5) >> 2][(6 * j + 5) & 3];
+#pragma unroll
+                    for (int k = 4; k >= 0; --k) x = __fma_rn(x, 32.0, (double)D[(6 * j + k) >> 2][(6 * j + k) & 3]);
+                    sc[j][u] = x;
+                }
+            }
+            if (__builtin_expect(two, 0)) {
+                f4_i8 q2[NMF];
+#pragma unroll
+                for (int j = 0; j < NMF; ++j) q2[j] = q_part(1, j);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const f4_i8 B = {(int)kr.k[u].x, (int)kr.k[u].y, (int)kr.k[u].z, (int)kr.k[u].w, 0, 0, 0, 0};
+                    f4_f4 D[NMF];
+#pragma unroll
+                    for (int j = 0; j < NMF; ++j)
+                        D[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(q2[j], B, (f4_f4){0.0f, 0.0f, 0.0f, 0.0f}, 2, 4, 0, 127,
+                                                                                0, (int)kr.s[u]);
+#pragma unroll
+                    for (int j = 0; j < RL; ++j) {
+                        double x = (double)D[(6 * j + 5) >> 2][(6 * j + 5) & 3];
+#pragma unroll
+                        for (int k = 4; k >= 0; --k) x = __fma_rn(x, 32.0, (double)D[(6 * j + k) >> 2][(6 * j + k) & 3]);
+                        sc[j][u] = __fma_rn(x, 0x1p-28, sc[j][u]);  // one rounding, in ad below
+                    }
+                }
+            }
+            if (more) issue_k(n0 + 256, nx, kr);
+            int M[RL][4], E[RL][4];
+            uint32_t good = 0;  // bit 4 j + i
+#pragma unroll
+            for (int j = 0; j < RL; ++j) {
+                // ---- which of the pairs are visible
+                uint32_t vis = row + j < nrow ? 15u : 0u;
+                if (edge) {
+                    vis = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = kn + i, ti = key - tb;
+                        const bool in = ((unsigned)ti < 64u) & (((S.tmk[row + j] >> (ti & 63)) & 1ull) != 0);
+                        bool pre = key < S.kvl[row + j];
+                        if constexpr (MOD) pre = pre & (key >= S.kvb[row + j]);
+                        vis |= ((key < k1) & (pre | in)) ? (1u << i) : 0u;
+                    }
+                }
+                // ---- certified weights
+                const double adel = rqe[j] * kbnd;
+                double s[4], ad[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[i] = sc[j][i] * rq[j];
+                    ad[i] = two ? __fma_rn(fabs(s[i] * alpha), 0x1p-52, adel) : adel;
+                }
+                int Mi[4], Ei[4];
+                bool ok[4];
+                if constexpr (MOD >= 2) {
+                    float sl[4];
+                    int dist[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        sl[i] = S.slope[row + j];
+                        dist[i] = kn + i - S.pos[row + j];
+                    }
+                    pf::cert_pairs<4, MOD>(s, ad, alpha, S.T1, S.T2, Mi, Ei, ok, P.cap, sl, dist);
+                } else {
+                    pf::cert_pairs<4>(s, ad, alpha, S.T1, S.T2, Mi, Ei, ok);
+                }
+                uint32_t gd = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) gd |= ok[i] ? (1u << i) : 0u;
+                gd &= ~wide;
+                const uint32_t slow = vis & ~gd;
+                gd &= vis;
+                if (__builtin_expect(__ballot(slow != 0) != 0, 0)) {
+                    // undecided pairs wait in the wave's list for flush(); a row that is flagged already needs no more of them
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const bool put = ((slow >> i) & 1) && !rfl[j];
+                        const uint64_t m = __ballot(put);
+                        if (put)
+                            S.list[w][cnt + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0))] =
+                                (uint32_t)(row + j) << 29 | (uint32_t)(kn + i - kA);
+                        cnt += (int)__popcll(m);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool y = (gd >> i) & 1;
+                    M[j][i] = y ? Mi[i] : 0;
+                    E[j][i] = y ? Ei[i] : 0;
+                }
+                good |= gd << (4 * j);
+            }
+            // ---- bases and references move when a weight or a scale passes them
+            if (cut) {  // scales of slots past the last key (or before the first) may be anything
+                uint32_t keep = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) keep |= (kn + i < k1 && (!MOD || kn + i >= kbeg)) ? 0xFFu << (8 * i) : 0u;
+#pragma unroll
+                for (int l = 0; l < NG; ++l) vr.s[l] &= keep;
+            }
+            bool move = false;
+#pragma unroll
+            for (int j = 0; j < RL; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) move |= ((good >> (4 * j + i)) & 1) && E[j][i] > base[j] + F4_BITS;
+            uint32_t past = 0;
+#pragma unroll
+            for (int l = 0; l < NG; ++l) {
+                const uint32_t x = vr.s[l];
+                vm[l] = pk_max(vm[l], pk_max(__builtin_bit_cast(f4_h2, x & 0x00FF00FFu), __builtin_bit_cast(f4_h2, x >> 8 & 0x00FF00FFu)));
+                const f4_h2 ref = __builtin_bit_cast(f4_h2, (uint32_t)G[l] * 0x10001u);
+                past |= __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(vm[l], ref));
+            }
+            if (__ballot(move || past != 0) != 0 || since >= F4_EPOCH) {
+                if (since) fold();
+#pragma unroll
+                for (int l = 0; l < NG; ++l) {
+                    const int top = wave_max_dpp((int)max(vm[l].x, vm[l].y));
+                    G[l] = max(G[l], top >= G[l] ? top + 1 : 0);  // one binade of room
+                }
+#pragma unroll
+                for (int j = 0; j < RL; ++j) {
+                    int m = F4_NONE;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) m = (good >> (4 * j + i)) & 1 ? max(m, E[j][i]) : m;
+                    for (int o = 1; o < 16; o <<= 1) m = max(m, __shfl_xor(m, o, 64));
+                    const int nb = m > base[j] + F4_BITS ? m - (F4_BITS - F4_HEAD) : base[j];
+                    if (folds) {
+                        rebase(j, nb);
+                    } else {
+                        base[j] = nb;  // nothing summed yet
+                    }
+                }
+            }
+            ++since;
+            double md[RL][4];
+#pragma unroll
+            for (int j = 0; j < RL; ++j) {
+                const int bs = base[j] == F4_NONE ? 0 : base[j];  // without a visible key so far every weight is 0
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    md[j][i] = (double)M[j][i];
+                    E[j][i] = (good >> (4 * j + i)) & 1 ? max(E[j][i] - bs, -1000) : 32;  // pairs that weigh nothing are exact
+                    z[j] += ldexp(md[j][i], E[j][i]);
+                }
+            }
+            // ---- P.V
+#pragma unroll
+            for (int l = 0; l < NG; ++l) {
+                if (l >= ng) break;
+                uint32_t* const W = S.W[w];  // read before it is written again: a wave's LDS accesses keep their order
+                constexpr double BIG = 0x1.8p52 + 141289400074368.0;  // and 0x808080808080
+#pragma unroll
+                for (int j = 0; j < RL; ++j) {
+                    uint32_t L[4], H[4];
+                    double xw[4], y[4];
+                    int least = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int sh = E[j][i] + (int)(vr.s[l] >> (8 * i) & 0xFFu) - G[l];
+                        least = min(least, sh);
+                        xw[i] = ldexp(md[j][i], sh);
+                        y[i] = xw[i] + BIG;
+                        L[i] = (uint32_t)__double2loint(y[i]);
+                        H[i] = (uint32_t)__double2hiint(y[i]);
+                    }
+                    if (__builtin_expect(__ballot(least < 0) != 0, 0)) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) lostw[j] += fabs(xw[i] - (y[i] - BIG));
+                    }
+                    // byte p of the four sums is plane p: transpositions of 4 x 4 and 4 x 2 bytes
+                    const uint32_t l01 = __builtin_amdgcn_perm(L[1], L[0], 0x05010400u), h01 = __builtin_amdgcn_perm(L[1], L[0], 0x07030602u);
+                    const uint32_t l23 = __builtin_amdgcn_perm(L[3], L[2], 0x05010400u), h23 = __builtin_amdgcn_perm(L[3], L[2], 0x07030602u);
+                    const uint32_t t01 = __builtin_amdgcn_perm(H[1], H[0], 0x05010400u), t23 = __builtin_amdgcn_perm(H[3], H[2], 0x05010400u);
+                    const uint32_t pl[6] = {__builtin_amdgcn_perm(l23, l01, 0x05040100u), __builtin_amdgcn_perm(l23, l01, 0x07060302u),
+                                            __builtin_amdgcn_perm(h23, h01, 0x05040100u), __builtin_amdgcn_perm(h23, h01, 0x07060302u),
+                                            __builtin_amdgcn_perm(t23, t01, 0x05040100u), __builtin_amdgcn_perm(t23, t01, 0x07060302u)};
+                    const int at = (RS == 4 ? g : 4 * (g & 1) + 2 * (g >> 1) + j) * F4_WROW + n;
+#pragma unroll
+                    for (int p = 0; p < 6; ++p) W[p * RS * F4_WROW + at] = pl[p] ^ 0x80808080u;
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                f4_i4 A[NMF];
+                if constexpr (RS == 4) {
+                    const uint32_t* const a0 = n < 8 ? &W[n * F4_WROW + 4 * g] : S.zero;
+                    A[0] = __builtin_bit_cast(f4_i4, *(const f4_u4*)a0);
+                    A[1] = __builtin_bit_cast(f4_i4, *(const f4_u4*)&W[(8 + n) * F4_WROW + 4 * g]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < NMF; ++j) A[j] = __builtin_bit_cast(f4_i4, *(const f4_u4*)&W[(16 * j + n) * F4_WROW + 4 * g]);
+                }
+                f4_i4 B0, B1;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    B0[x] = (int)four_bytes<false>(vr.v[l][x]);
+                    B1[x] = (int)four_bytes<true>(vr.v[l][x]);
+                }
+#pragma unroll
+                for (int j = 0; j < NMF; ++j) {
+                    acc[j][2 * l] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[j], B0, acc[j][2 * l], 0, 0, 0);
+                    acc[j][2 * l + 1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[j], B1, acc[j][2 * l + 1], 0, 0, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (more) issue_v(n0 + 256, nx, vr);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+
+        // ---- the pairs waiting in the list, 4 at a time and 16 lanes a pair: every product of the score separately,
+        // TwoSum-accumulated, the certified weight, then one pair after another into the row's fp64 sums. (A lane a pair took 8 us of a
+        // step with one such pair, most of it waiting for 16 loads in turn.)
+        auto flush = [&]() __attribute__((always_inline)) {
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+            for (int at = 0; at < cnt; at += 4) {
+                const bool have = at + g < cnt;
+                const uint32_t en = have ? S.list[w][at + g] : 0u;
+                const int er = (int)(en >> 29), ek = kA + (int)(en & 0x1FFFFFFFu);
+                double ss = 0.0, es = 0.0, ea = 0.0;
+                if (have && 8 * n < d) {
+                    const uint16_t* qr = q_row(er) + 8 * n;
+                    const uint4 kv = kv4_load8(P.k, P.ks, kv_off(P, b, ek, hk, 0) + 8 * n);
+                    const uint32_t wd[4] = {kv.x, kv.y, kv.z, kv.w};
+                    uint32_t qw[8];
+#pragma unroll
+                    for (int h = 0; h < 8; ++h) qw[h] = qr[h];
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        double e0, e1;
+                        ss = two_sum(ss, (double)__uint_as_float(qw[2 * h] << 16) * bf16lo_f64(wd[h]), &e0);
+                        ss = two_sum(ss, (double)__uint_as_float(qw[2 * h + 1] << 16) * bf16hi_f64(wd[h]), &e1);
+                        es += e0 + e1;
+                        ea += fabs(e0) + fabs(e1);
+                    }
+                }
+#pragma unroll
+                for (int o = 1; o < 16; o <<= 1) {  // alike in both lanes: a sum and its error do not depend on the order
+                    double e;
+                    ss = two_sum(ss, __shfl_xor(ss, o, 64), &e);
+                    es = (es + __shfl_xor(es, o, 64)) + e;
+                    ea = (ea + __shfl_xor(ea, o, 64)) + fabs(e);
+                }
+                int32_t Mi = 0, Ei = 0;
+                bool live = false;
+                int why = 0;  // 1 score not certified, 2 weight not certified
+                const bool fin = have && isfinite(ss);
+                if (have) {
+                    uint32_t tbits = 0;
+                    int ls = 3;
+                    if (fin) {
+                        const bool zero = ss == 0.0 && es == 0.0 && ea == 0.0;
+                        ls = zero ? 1 : logit_cert(alpha, ss, es, ea * 0x1p-44, &tbits);
+                        if (ls == 1) tbits = 0;
+                        if constexpr (MOD >= 2) ls = mod_logit(ls, zero, P.cap, S.slope[er], ek - S.pos[er], S.T1, 23, &tbits);
+                    }
+                    if (ls == 2 || ls == 3) {
+                        why = 1;  // undecided, or an overflow (tier 2 reports the domain error)
+                    } else if (pf::table_weight(tbits, S.T1, S.T2, &Mi, &Ei)) {
+                        live = true;
+                    } else {
+                        int64_t E2 = 0;
+                        live = weight_wide(tbits, &Mi, &E2) == 0 && E2 > -(1LL << 30) && E2 < (1LL << 30);
+                        if (!live) why = 2;
+                        Ei = (int32_t)E2;
+                    }
+                }
+                const uint64_t first = 0x0001000100010001ull;  // a lane of each pair
+                n5 += (int)__popcll(__ballot(why == 1) & first);
+                n6 += (int)__popcll(__ballot(why == 2) & first);
+                n8 += (int)__popcll(__ballot(fin) & first);
+                for (uint64_t m = __ballot(have && !live) & first; m; m &= m - 1) {
+                    const int r = __builtin_amdgcn_readlane(er, __builtin_ctzll(m));
+#pragma unroll
+                    for (int j = 0; j < RL; ++j)
+                        if (row + j == r) rfl[j] = 1;
+                }
+                for (uint64_t lv = __ballot(live) & first; lv; lv &= lv - 1) {
+                    const int ln = __builtin_ctzll(lv);
+                    const int r = __builtin_amdgcn_readlane(er, ln), key = __builtin_amdgcn_readlane(ek, ln);
+                    const int Mr = __builtin_amdgcn_readlane(Mi, ln), Er = __builtin_amdgcn_readlane(Ei, ln);
+                    const int64_t vc = kv4_v(P, b, key, hk);
+                    uint32_t v2[NG];
+#pragma unroll
+                    for (int l = 0; l < NG; ++l) {
+                        v2[l] = l < ng ? kv4_vload2(P.v, P.vs, vc, 32 * l + 2 * n) : 0u;
+                        // the scales that these sums met belong to the bound on |v|
+                        if (l < ng) vm[l] = pk_max(vm[l], (f4_h2){(P.vs + kv4_vscale(vc))[16 * l], 0});
+                    }
+#pragma unroll
+                    for (int j = 0; j < RL; ++j) {
+                        if (row + j != r) continue;
+                        if (Er > base[j] + F4_BITS) rebase(j, Er - (F4_BITS - F4_HEAD));
+                        const int de = Er - base[j];
+                        if (!MOD && de < -1000) rfl[j] = 1;
+                        const double om = de < -1000 ? 0.0 : ldexp((double)Mr, de);
+                        z[j] += n == 0 ? om : 0.0;
+#pragma unroll
+                        for (int l = 0; l < NG; ++l) {
+                            if (l >= ng) break;
+                            double* const o = &O[j * 32 * NG + 32 * l];
+                            o[0] = __fma_rn(om, bf16lo_f64(v2[l]), o[0]);
+                            o[16] = __fma_rn(om, bf16hi_f64(v2[l]), o[16]);
+                        }
+                    }
+                    ++folds;
+                }
+            }
+            cnt = 0;
+        };
+
+        // ---- the wave's tiles: K of the next one is requested once the scores have read this one's registers, V once P.V has;
+        // pages are looked up a tile ahead. A flush (rare) drops the loads in flight and starts over
+        for (int it = 0; it < nst;) {
+            KR kr;
+            VR vr;
+            {
+                const Pages p0 = pages_of(k0w + 256 * it);
+                issue_k(k0w + 256 * it, p0, kr);
+                issue_v(k0w + 256 * it, p0, vr);
+            }
+#pragma unroll 1
+            for (; it < nst && cnt < F4_LIST; ++it) tile(k0w + 256 * it, it + 1 < nst, kr, vr);
+            if (since) fold();
+            if (cnt > 0) flush();
+        }
+
+        // ---- epilogue: row totals of the wave, then the 4 waves' partials at the rows' largest base (exact powers of two), two
+        // additions deep
+        {
+#pragma unroll
+            for (int j = 0; j < RL; ++j) {
+                double zs = z[j], ls = lostw[j];
+                int fl = rfl[j];
+                for (int o = 1; o < 16; o <<= 1) {
+                    zs += __shfl_xor(zs, o, 64);
+                    ls += __shfl_xor(ls, o, 64);
+                    fl |= __shfl_xor(fl, o, 64);
+                }
+                if (n == 0) {
+                    S.wR[w][row + j] = base[j];
+                    S.wZ[w][row + j] = zs;
+                    S.we[w][row + j] = ls;
+                    S.wf[w][row + j] = fl;
+                }
+            }
+            if (lane == 0) S.wn[w] = folds;
+#pragma unroll
+            for (int l = 0; l < NG; ++l) {
+                const int top = wave_max_dpp((int)max(vm[l].x, vm[l].y));
+                if (lane == 0) S.wv[w][l] = (uint32_t)top;
+            }
+        }
+        __syncthreads();
+        const int64_t pbase = (int64_t)split * P.rows;
+        auto sums_at = [&](int r, double (&f)[4]) __attribute__((always_inline)) {  // the waves' factors to the largest base
+            int Rm = F4_NONE, far = 0;
+            for (int ww = 0; ww < 4; ++ww) Rm = max(Rm, S.wR[ww][r]);
+#pragma unroll
+            for (int ww = 0; ww < 4; ++ww) {
+                const bool any = S.wR[ww][r] != F4_NONE;
+                const int sh = any ? S.wR[ww][r] - Rm : 0;
+                far |= !MOD && sh < -900;
+                f[ww] = any ? ldexp(1.0, max(sh, -1000)) : 0.0;
+            }
+            return far ? INT_MIN : Rm;
+        };
+        // a thread 2 channels of a row at a time
+        for (int x = tid; x < nrow * 16 * NG; x += F4_THREADS) {
+            const int r = x / (16 * NG), p = x % (16 * NG), l = p >> 4, c = p & 15;
+            if (2 * p >= dv) continue;
+            double f[4], o[2];
+            sums_at(r, f);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int at = 32 * l + 16 * h + c;
+                o[h] = (f[0] * S.O[0][r][at] + f[2] * S.O[2][r][at]) + (f[1] * S.O[1][r][at] + f[3] * S.O[3][r][at]);
+            }
+            const int lr = row0 + r;
+            const int64_t gr = row_index(P, b, lr / P.grp, hk * P.grp + lr % P.grp);
+            *(double2*)(P.pN + (pbase + gr) * dv + 2 * p) = make_double2(o[0], o[1]);
+        }
+        if (w == 3 && lane < nrow) {
+            const int r = lane;
+            double f[4], lost = 0.0;
+            const int Rm = sums_at(r, f);
+            int fl = Rm == INT_MIN, fo = 0;
+            for (int ww = 0; ww < 4; ++ww) {
+                fl |= S.wf[ww][r];
+                fo += S.wn[ww];
+                lost += f[ww] * S.we[ww][r];
+            }
+            // keys of the piece up to the row's last visible one: at least the keys summed
+            const uint64_t tm = S.tmk[r];
+            const int ke = min(tm ? max(S.kvl[r], tb + 64 - (int)__clzll(tm)) : S.kvl[r], k1);
+            const int nk = Rm == F4_NONE ? 0 : ke - kA;
+            const double Z = (f[0] * S.wZ[0][r] + f[2] * S.wZ[2][r]) + (f[1] * S.wZ[1][r] + f[3] * S.wZ[3][r]);
+            // The depth that the combine multiplies by u Z max|v|: fp64 roundings (a key each, folds of 5, joins), and what the
+            // weights lost, at most 12 units of 2^(base + G) for each of theirs: max|v| is 12 units of the largest scale and G at
+            // most a binade above it, so 2 lost / Z, in units of u
+            const double depth = (double)nk + 16.0 + 8.0 * (double)fo + (lost / Z) * (0x1p54 * (1.0 + 0x1p-20)) + 1.0;
+            int most = nk;
+            if (nk > 0) {
+                if (!(depth < 0x1p28)) fl = 1;
+                most = fl ? nk : (int)depth * (MOD ? 4 : 1);  // the modified steps' combine counts a quarter
+            }
+            const int lr = row0 + r;
+            const int64_t o = pbase + row_index(P, b, lr / P.grp, hk * P.grp + lr % P.grp);
+            P.pR[o] = Rm == F4_NONE ? INT_MIN : Rm;
+            P.pZ[o] = Z;
+            P.pn[o] = fl ? -1 : most;
+        } else if (w == 2) {
+            for (int ch = lane; ch < dv; ch += 64) {
+                const int l = ch >> 5;
+                const uint32_t top = max(max(S.wv[0][l], S.wv[1][l]), max(S.wv[2][l], S.wv[3][l]));
+                P.pV[(((int64_t)split * P.nseg + seg) * P.nrb + rbk) * dv + ch] = kv4_bound(top);
+            }
+        }
+        if (P.stats && lane == 0) {
+            if (n5) atomicAdd((unsigned long long*)&P.stats[5], (unsigned long long)n5);
+            if (n6) atomicAdd((unsigned long long*)&P.stats[6], (unsigned long long)n6);
+            if (n8) atomicAdd((unsigned long long*)&P.stats[8], (unsigned long long)n8);
+        }
+    };
+
+    // One piece per block on uniform splits; on the equal-share plan (Params::dq_*) one per unit its share reaches, read as the
+    // decode kernel reads it. A segment's row blocks go to one XCD (ea_decode.hip has both placements and their reasons).
+    int u, start, end, share = 1, gb = 0;
+    const int32_t* Su = P.dq_plan + 2;
+    if (P.dq_stream) {
+        gb = (int)blockIdx.x;
+        if (P.nrb > 1 && (P.dq_blocks & 7) == 0 && (int64_t)P.dq_units * 8 > P.dq_blocks)
+            gb = (gb & 7) * (P.dq_blocks >> 3) + (gb >> 3);
+        const int4 rec = ((const int4*)(P.dq_plan + P.dq_rec_off))[gb];
+        u = rec.x;
+        share = rec.w;
+        if (u >= P.dq_units || share <= 0) return;  // past the last share: no tile
+        start = gb * share;
+        end = min(start + share, P.dq_plan[0]);
+    } else {
+        u = (int)blockIdx.x;
+        if (P.nrb > 1 && (P.nseg & 7) == 0) {
+            const int lo = u & 7, hi = u >> 3;
+            u = ((hi / P.nrb) * 8 + lo) * P.nrb + hi % P.nrb;
+        }
+        start = (int)blockIdx.y * (P.split_len >> 6);
+        end = start + (P.split_len >> 6);
+        if (MOD && blockIdx.y == gridDim.y - 1) end = 1 << 23;  // keys are below 2^29
+    }
+    for (bool first = true;; first = false) {
+        int t0 = start, t1 = end, slot = (int)blockIdx.y;
+        if (P.dq_stream) {
+            if (start >= end || u >= P.dq_units) break;
+            const int su = Su[u], eu = Su[u + 1];
+            if (eu <= start) {
+                ++u;
+                continue;
+            }
+            slot = gb - su / share;
+            t0 = start - su;
+            t1 = min(end, eu) - su;
+            start = min(end, eu);
+            if (slot >= P.nsplit) break;  // share >= dq_min_share keeps every unit within nsplit slots
+        }
+        if (!first) __syncthreads();  // the previous piece's LDS reads are done
+        piece(u, slot, t0 * 64, t1 * 64);
+        if (!P.dq_stream) break;
+        ++u;
+    }
+}

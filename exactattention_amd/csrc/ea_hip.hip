@@ -926,12 +926,12 @@ __device__ __forceinline__ void t2_rows(const Params& P, T2Smem& S, int& s_last,
             // broadcast and the batch's V elements loaded together (independent loads in flight)
             uint32_t vx[16][2];
             auto load_batch = [&](int64_t jb, int nk) __attribute__((always_inline)) {
-                const int64_t myoff = ln < nk ? kv_off(P, b, key_n(jc0 + jb + ln), hk, 1) : 0;
+                const int64_t myoff = ln >= nk ? 0 : (P.vs ? kv4_v(P, b, key_n(jc0 + jb + ln), hk) : kv_off(P, b, key_n(jc0 + jb + ln), hk, 1));
 #pragma unroll
                 for (int kk = 0; kk < 16; ++kk) {
                     const int64_t o = __shfl(myoff, kk, 64);
                     if (P.vs) {
-                        const uint32_t two = kk < nk && 2 * ln < dv ? kv4_load2(P.v, P.vs, o + 2 * ln) : 0u;
+                        const uint32_t two = kk < nk && 2 * ln < dv ? kv4_vload2(P.v, P.vs, o, 2 * ln) : 0u;
                         vx[kk][0] = two & 0xFFFFu;
                         vx[kk][1] = two >> 16;
                         continue;
@@ -1250,9 +1250,13 @@ __global__ void __launch_bounds__(256) ea_gather_row(Params P, int64_t row, int6
         const int wdt = isv ? dv : d;
         const int64_t j = r / wdt;
         const int e = (int)(r % wdt);
-        const int64_t o = kv_off(P, b, keys.key(j), hk, isv) + e;
-        if (P.ks) dst[i] = (uint16_t)(kv4_load2(isv ? P.v : P.k, isv ? P.vs : P.ks, o & ~(int64_t)1) >> (16 * (o & 1)));
-        else dst[i] = (isv ? P.v : P.k)[o];
+        if (P.ks) {
+            const uint32_t two = isv ? kv4_vload2(P.v, P.vs, kv4_v(P, b, keys.key(j), hk), e & ~1)
+                                     : kv4_load2(P.k, P.ks, kv_off(P, b, keys.key(j), hk, 0) + (e & ~1));
+            dst[i] = (uint16_t)(two >> (16 * (e & 1)));
+        } else {
+            dst[i] = (isv ? P.v : P.k)[kv_off(P, b, keys.key(j), hk, isv) + e];
+        }
     }
 }
 
@@ -1613,13 +1617,13 @@ int check_mods(const ea_options* o, const ea_score_mods* m) {
     return c == 0 || (f > 0 && f < 255) ? 0 : -2;
 }
 
-// 0, or the code that the 4-bit entry points return: rows of whole groups, and what reads bf16 rows is no choice
+// 0, or the code that the 4-bit entry points return: K rows of whole groups, V tiles of 16 slots that start on 64 bytes of codes,
+// and no choice of the other caches' kernels
 int check_kv4(const ea_geometry* g, const ea_options* o) {
-    const int64_t st[6] = {g->k_page_stride, g->k_slot_stride, g->k_head_stride, g->v_page_stride, g->v_slot_stride, g->v_head_stride};
-    for (int64_t x : st)
-        if (x & 31) return -1;
+    if ((g->k_page_stride | g->k_slot_stride | g->k_head_stride) & 31) return -1;
+    if (g->v_slot_stride != ((g->head_dim_v + 31) & ~31) || ((g->v_page_stride | g->v_head_stride) & 127)) return -1;
     if (g->head_dim_v & 7) return -1;
-    return o->kv_digits || o->timers || o->kernel == EA_KERNEL_DECODE || o->kernel == EA_KERNEL_GENERAL ? -2 : 0;
+    return o->kv_digits || o->timers || o->kernel != EA_KERNEL_AUTO ? -2 : 0;
 }
 
 int make_plan(const ea_geometry* g, const ea_options* o, Plan* pl, const ea_score_mods* m = nullptr, bool kv4 = false) {
@@ -1652,8 +1656,8 @@ int make_plan(const ea_geometry* g, const ea_options* o, Plan* pl, const ea_scor
     const int span = m ? mod_span(g, m, maxlen) : maxlen;
     pl->dq_max_tiles = (int)max_tiles;
     pl->t2_keys = maxlen;  // a row's visible keys are distinct and below max_seq_len
-    pl->prefill = (m ? prefill_mods(g, o, m, span, &pl->pf_ntiles, &pl->pf_nrb)
-                     : ea_prefill_eligible(*g, pl->grp, o->kernel, &pl->pf_ntiles, &pl->pf_nrb) != 0) ? 1 : 0;
+    pl->prefill = !kv4 && (m ? prefill_mods(g, o, m, span, &pl->pf_ntiles, &pl->pf_nrb)
+                             : ea_prefill_eligible(*g, pl->grp, o->kernel, &pl->pf_ntiles, &pl->pf_nrb) != 0) ? 1 : 0;
     pl->pf_nsplit = pl->pf_tps = 1;
     if (pl->prefill) {
         if (o->kv_digits && o->kv_digits_tiles < pl->pf_ntiles) return -1;
@@ -1682,8 +1686,8 @@ int make_plan(const ea_geometry* g, const ea_options* o, Plan* pl, const ea_scor
     choose_splits(pl->nseg * (int64_t)gen.nrb, span, o->splits, &gen.nsplit, &gen.split_len);
     gen.dq = d128 && !m && dq_fits(gen.nrb);
     Tier1& mr = pl->mr;
-    // ea_decode reads neither modifications nor 4-bit caches
-    mr.rb = (m || kv4) && pl->prefill ? 0 : mrow_rows(g, o, pl->r_seg, m != nullptr || kv4);
+    mr.rb = m && pl->prefill ? 0 : mrow_rows(g, o, pl->r_seg, m != nullptr || kv4);
+    if (kv4) mr.rb = std::min(mr.rb, 8);  // ea_four's row blocks
     pl->mrow = mr.rb > 0;
     const size_t without = lay_out(pl, g, o, false, m != nullptr);
     if (!pl->mrow) return 0;
@@ -1754,7 +1758,7 @@ void set_inputs(Params& P, const Plan& pl, const ea_geometry* g, const ea_buffer
 // The fp64 kernel of a step that does not take the prefill path (host logic): sets P.mrow, its row
 // blocks and its uniform splits. Returns whether it is ea_decode (false: ea_mrow or ea_split).
 bool choose_split_kernel(Params& P, const Plan& pl) {
-    P.mrow = pl.mrow && pl.nseg > 0 && ea_mrow_eligible(P);
+    P.mrow = pl.mrow && pl.nseg > 0 && (P.ks ? ea_four_eligible(P) : ea_mrow_eligible(P));
     const Tier1& t = P.mrow ? pl.mr : pl.gen;
     P.rb = t.rb;
     P.nrb = t.nrb;
@@ -1878,7 +1882,7 @@ int ea_hip_reads_kv_digits(const ea_geometry* g, const ea_options* o, int32_t* r
 
 // The scales of a 4-bit cache and what its kernels need of the pointers and pages
 static int check_kv4_buffers(const ea_geometry* g, const ea_buffers* bf, const ea_kv4* x) {
-    if (!x->k_scales || !x->v_scales || (((uintptr_t)bf->k | (uintptr_t)bf->v) & 15)) return -1;
+    if (!x->k_scales || !x->v_scales || (((uintptr_t)bf->k | (uintptr_t)bf->v) & 15) || ((uintptr_t)x->v_scales & 3)) return -1;
     return bf->block_table && g->page_size < 16 ? -1 : 0;
 }
 
@@ -1945,14 +1949,15 @@ static int attention_impl(const ea_geometry* g, const ea_buffers* bf, const ea_o
         int slots = 0, cus = 0;
         use_decode = choose_split_kernel(P, pl);
         if (x4 && !P.mrow) return -1;  // strides past the kernel's 32-bit offsets
-        if (P.mrow && (rc = ea_mrow_slots(P, &slots))) return rc;
+        if (P.mrow && (rc = P.ks ? ea_four_slots(P, &slots) : ea_mrow_slots(P, &slots))) return rc;
         if (use_decode && (rc = ea_decode_slots(P, &slots, &cus))) return rc;
         const int nsplit = P.nsplit;
         const int64_t units = (int64_t)P.nseg * P.nrb;
         // the equal-share plan when the uniform split grid would take more than one round of
         // resident blocks (long or ragged contexts); otherwise one block per (unit, split)
         P.dq_lead = 0;
-        if (use_decode || P.mrow) P.pv_tiles = P.split_len / EA_TILE;
+        // (the 4-bit kernel's partials say their depth themselves)
+        if (use_decode || (P.mrow && !x4)) P.pv_tiles = P.split_len / EA_TILE;
         if (use_decode && nsplit >= 2 && units * nsplit == slots && slots > cus) {
             // exactly one round: the first wave's splits are weighted 5 against 4 (the decode
             // kernel's uniform path); the longest is at most 5 / (5 + 4 (n - 1)) of the unit's
@@ -2039,7 +2044,7 @@ static int attention_impl(const ea_geometry* g, const ea_buffers* bf, const ea_o
         const dim3 blk(EA_THREADS);
         const size_t lds = sizeof(SplitSmem);
         if (P.mrow) {
-            if ((rc = ea_launch_mrow(P, st))) return rc;
+            if ((rc = P.ks ? ea_launch_four(P, st) : ea_launch_mrow(P, st))) return rc;
         } else if (use_decode) {
             if ((rc = ea_launch_decode(P, st))) return rc;
         } else if (P.mods) {

@@ -166,8 +166,9 @@ __global__ void __launch_bounds__(NR_THREADS) ea_norm_rotary_kernel(ea_norm_rota
         const int64_t ts = v ? A.vo_tok_stride : A.ko_tok_stride, hs = v ? A.vo_head_stride : A.ko_head_stride;
         if constexpr (KV4) {
             x.scales = v ? N.v_scales : N.k_scales;
-            const int64_t page = r / N.page_size;
-            x.o = page * (v ? N.v_page_stride : N.k_page_stride) + (r - page * N.page_size) * ts + g * hs;
+            const int64_t page = r / N.page_size, slot = r - page * N.page_size;
+            if (v) x.o = kv4_v_at(page * N.v_page_stride + g * hs, slot, kv4_width(d));
+            else x.o = page * N.k_page_stride + slot * ts + g * hs;
         } else {
             x.o = r * ts + g * hs;
         }
@@ -242,7 +243,6 @@ __global__ void __launch_bounds__(NR_THREADS) ea_norm_rotary_kernel(ea_norm_rota
                     const int fld = (int)(top >> 23);
                     const int sc = fld == 255 ? 255 : min(max(fld - ((top & 0x7FFFFFu) < 0x600000u ? 2 : 1), 2), 252);
                     const float by = __uint_as_float((uint32_t)sc << 23);
-                    const int64_t at = x.row.o + H.e[k];
                     uint32_t w = 0;
                     if (sc != 255) {
                         w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[k][0], f[k][1], by, 0);
@@ -252,9 +252,17 @@ __global__ void __launch_bounds__(NR_THREADS) ea_norm_rotary_kernel(ea_norm_rota
                             w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[k][6], f[k][7], by, 3);
                         }
                     }
-                    if constexpr (C == 8) *(uint32_t*)((uint8_t*)x.row.dst + (at >> 1)) = w;
-                    else ((uint8_t*)x.row.dst)[at >> 1] = (uint8_t)w;
-                    if ((H.e[k] & 31) == 0) x.row.scales[at >> 5] = (uint8_t)sc;
+                    uint8_t* const dst = (uint8_t*)x.row.dst;
+                    if (x.row.kind == 2) {  // a byte for each pair of channels, 16 apart
+#pragma unroll
+                        for (int i = 0; i < C; i += 2) dst[x.row.o + 8 * (H.e[k] + i)] = (uint8_t)(w >> (4 * i));
+                        if ((H.e[k] & 31) == 0) x.row.scales[kv4_vscale(x.row.o) + (H.e[k] >> 1)] = (uint8_t)sc;
+                    } else {
+                        const int64_t at = x.row.o + H.e[k];
+                        if constexpr (C == 8) *(uint32_t*)(dst + (at >> 1)) = w;
+                        else dst[at >> 1] = (uint8_t)w;
+                        if ((H.e[k] & 31) == 0) x.row.scales[at >> 5] = (uint8_t)sc;
+                    }
                 }
                 return;
             }
@@ -395,13 +403,22 @@ __global__ void __launch_bounds__(256) ea_norm_weights_kernel(const double* part
     else ((uint16_t*)out)[i] = (uint16_t)f64_bf16(s);
 }
 
-// rows of whole groups to bf16, 8 elements a thread
+// rows of K, or slots of V's tiles, to bf16, 8 elements a thread
+template <bool V>
 __global__ void __launch_bounds__(256) ea_kv4_values_kernel(int64_t n, int per, int groups, const uint8_t* codes, const uint8_t* scales,
                                                             uint16_t* out) {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
         const int64_t row = i / per;
         const int c = (int)(i - row * per);
-        *(uint4*)(out + row * per * 8 + 8 * c) = kv4_load8(codes, scales, row * groups * 32 + 8 * c);
+        uint4 x;
+        if constexpr (V) {
+            const int64_t at = kv4_v_at(0, row, 32 * groups);
+            x = make_uint4(kv4_vload2(codes, scales, at, 8 * c), kv4_vload2(codes, scales, at, 8 * c + 2),
+                           kv4_vload2(codes, scales, at, 8 * c + 4), kv4_vload2(codes, scales, at, 8 * c + 6));
+        } else {
+            x = kv4_load8(codes, scales, row * groups * 32 + 8 * c);
+        }
+        *(uint4*)(out + row * per * 8 + 8 * c) = x;
     }
 }
 
@@ -466,9 +483,9 @@ int ea_hip_norm_rotary(const ea_norm_rotary* a, ea_stream_t stream) {
     const int d = r.head_dim, R = r.rot_dim;
     if (four) {
         if ((d & 7) || (R & 3)) return -1;
-        if (((r.ko_tok_stride | r.ko_head_stride | r.vo_tok_stride | r.vo_head_stride | a->k_page_stride | a->v_page_stride) & 31) != 0)
-            return -1;
-        if (((uintptr_t)r.k_out | (uintptr_t)r.v_out) & 3) return -1;
+        if (((r.ko_tok_stride | r.ko_head_stride | a->k_page_stride) & 31) || ((r.vo_head_stride | a->v_page_stride) & 127)) return -1;
+        if (r.v && (r.vo_tok_stride != kv4_width(d) || (a->page_size & 15))) return -1;
+        if (((uintptr_t)r.k_out & 3) || (r.v && ((uintptr_t)r.v_out & 15))) return -1;
     }
     // 16-byte accesses: every row of every tensor starts on one (a 4-bit row's runs of 8 are 4 bytes)
     const int64_t in = r.in_fp32 ? 4 : 8, out = r.out_fp32 ? 4 : 8;
@@ -594,17 +611,17 @@ int ea_hip_norm_rotary_grad(const ea_norm_rotary_grad* a, ea_stream_t stream) {
     return 0;
 }
 
-int ea_hip_kv4_values(int64_t rows, int32_t head_dim, const uint8_t* codes, const uint8_t* scales, uint16_t* values,
+int ea_hip_kv4_values(int64_t rows, int32_t head_dim, int32_t is_v, const uint8_t* codes, const uint8_t* scales, uint16_t* values,
                       ea_stream_t stream) {
-    if (rows < 0 || head_dim <= 0 || (head_dim & 7)) return -1;
+    if (rows < 0 || head_dim <= 0 || (head_dim & 7) || (is_v && (rows & 15))) return -1;
     if (rows == 0) return 0;
     if (!codes || !scales || !values || ((uintptr_t)codes & 3) || ((uintptr_t)values & 15)) return -1;
     const int per = head_dim / 8;
     if (rows > (((int64_t)1 << 62) / head_dim)) return -1;
     const int64_t n = rows * per;
     const unsigned grid = (unsigned)std::min<int64_t>((n + 255) / 256, 8192);
-    hipLaunchKernelGGL(ea_kv4_values_kernel, dim3(grid), dim3(256), 0, (hipStream_t)stream, n, per, (head_dim + 31) / 32, codes,
-                       scales, values);
+    const auto fn = is_v ? ea_kv4_values_kernel<true> : ea_kv4_values_kernel<false>;
+    hipLaunchKernelGGL(fn, dim3(grid), dim3(256), 0, (hipStream_t)stream, n, per, (head_dim + 31) / 32, codes, scales, values);
     return herr(hipGetLastError());
 }
 

@@ -288,8 +288,10 @@ int ea_launch_decode(const Params& P, hipStream_t st);
 // same three questions as for the decode kernel.
 int ea_mrow_eligible(const Params& P);
 int ea_mrow_slots(const Params& P, int* slots);
-// its variants for 4-bit caches, their own file
-const void* ea_mrow_kv4_fn(int rb, bool small, int mods);
+// The split kernel of 4-bit caches (ea_four.h): row blocks of P.rb = 4 or 8. The same three questions.
+int ea_four_eligible(const Params& P);
+int ea_four_slots(const Params& P, int* slots);
+int ea_launch_four(const Params& P, hipStream_t st);
 int ea_launch_mrow(const Params& P, hipStream_t st);
 
 // int8-MFMA prefill path (ea_prefill.hip). A tile holds 64 keys of one segment:

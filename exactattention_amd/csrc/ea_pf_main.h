@@ -702,13 +702,12 @@ __global__ void __launch_bounds__(64 * NWB, 1) ea_pf_main(Params A) {
                 const int mode = qbad ? 2 : ((!((qm.flags >> 8) & 0xFF) && !(kf >> 8)) ? 0 : 1);
                 const uint16_t* qr = nullptr;
                 const uint16_t* kr = nullptr;
-                const bool four = mode == 1 && P.ks;  // a 4-bit cache has no bf16 row to read: tier 2's pair
-                if (mode == 1 && !four) {
+                if (mode == 1) {
                     qr = P.q + b * P.g.q_seq_stride + (int64_t)tq * P.g.q_tok_stride +
                          (int64_t)(hk * P.grp + lrc % P.grp) * P.g.q_head_stride;
                     kr = P.k + kv_off(P, b, n, hk, 0);
                 }
-                const int3 cw = four ? make_int3(3, 0, 0) : pf_cold_pair<(MOD >= 2)>(mode, qlds, 0, (const uint8_t*)Kg + key * 128, key & 7, qr, kr, P.am,
+                const int3 cw = pf_cold_pair<(MOD >= 2)>(mode, qlds, 0, (const uint8_t*)Kg + key * 128, key & 7, qr, kr, P.am,
                                                   P.ae + qm.lsb + TMc->lsbk[key], P.alpha, T1s, T2, P.cap, mslope, n - mpos,
                                                   MOD ? P.g.head_dim : 128);
                 const bool live = cw.x == 0;

@@ -41,7 +41,6 @@
 #include <atomic>
 #include <mutex>
 
-#include "ea_kv4.h"
 #include "ea_params.h"
 #include "ea_pf_common.h"
 #include "ea_pf_main.h"
@@ -138,9 +137,13 @@ __device__ __forceinline__ int grp_sum(int x) {
 // lost[c] (optional) receives 1 for each element that is not exact in 30 bits. have: the elements there
 // are, a multiple of 8 (negative: none); the others are zeros.
 template <int NE>
-__device__ __forceinline__ void load_words(const uint16_t* src, bool valid, uint32_t (&raw)[NE / 2], int have) {
+__device__ __forceinline__ void slice_n(const uint16_t* src, bool valid, SliceN<NE>& S, int* lost = nullptr, int have = NE) {
+    constexpr int G = 128 / NE;
+    int m[NE], e[NE];
+    int bad = 0, lead = INT_MIN;
     // the 2 NE bytes as 16-byte loads when they start on a 16-byte boundary (the usual cache
     // strides), else element by element
+    uint32_t raw[NE / 2];
     if (valid && ((uintptr_t)src & 15) == 0) {
 #pragma unroll
         for (int i = 0; i < NE / 8; ++i) {
@@ -155,13 +158,6 @@ __device__ __forceinline__ void load_words(const uint16_t* src, bool valid, uint
         for (int i = 0; i < NE / 2; ++i)
             raw[i] = valid && 2 * i < have ? ((uint32_t)src[2 * i] | ((uint32_t)src[2 * i + 1] << 16)) : 0u;
     }
-}
-// raw: NE bf16 values, two a word
-template <int NE>
-__device__ __forceinline__ void slice_words(const uint32_t (&raw)[NE / 2], SliceN<NE>& S, int* lost = nullptr) {
-    constexpr int G = 128 / NE;
-    int m[NE], e[NE];
-    int bad = 0, lead = INT_MIN;
 #pragma unroll
     for (int k = 0; k < NE; ++k) {
         int bk;
@@ -209,28 +205,8 @@ __device__ __forceinline__ void slice_words(const uint32_t (&raw)[NE / 2], Slice
     const int hi = grp_sum<G>((int)(asum >> 20)), lo = grp_sum<G>((int)(asum & 0xFFFFF));
     S.asum = (double)hi * 0x1p20 + (double)lo;  // exact: integers below 2^41
 }
-template <int NE>
-__device__ __forceinline__ void slice_n(const uint16_t* src, bool valid, SliceN<NE>& S, int* lost = nullptr, int have = NE) {
-    uint32_t raw[NE / 2];
-    load_words<NE>(src, valid, raw, have);
-    slice_words<NE>(raw, S, lost);
-}
-// 32 elements of a K or V row from element offset `off`; KV4: of a 4-bit cache
-template <bool KV4>
-__device__ __forceinline__ void slice32(const uint16_t* src, const uint8_t* scales, int64_t off, bool valid, Slice32& S,
-                                        int* lost = nullptr, int have = 32) {
-    if constexpr (KV4) {
-        uint32_t raw[16];
-        if (valid && have > 0) {
-            kv4_load32(src, scales, off, have, raw);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) raw[i] = 0;
-        }
-        slice_words<32>(raw, S, lost);
-    } else {
-        slice_n<32>(src + off, valid, S, lost, have);
-    }
+__device__ __forceinline__ void slice32(const uint16_t* src, bool valid, Slice32& S, int* lost = nullptr, int have = 32) {
+    slice_n<32>(src, valid, S, lost, have);
 }
 
 }  // namespace
@@ -272,7 +248,7 @@ __global__ void __launch_bounds__(256) ea_pf_qslice(Params P) {
 // ------------------------------------------------------------------------------------------------
 // MOD (score modifications): tiles wholly before the first key that a token of the sequence sees are left
 // out; no row of ea_pf_main reads them. Heads of fewer dims or channels than 128 are padded with zeros.
-template <bool MOD, bool KV4 = false>
+template <bool MOD>
 __global__ void __launch_bounds__(256) ea_pf_kvslice(Params P) {
     __shared__ __align__(16) uint8_t s_v[32768];
     __shared__ int s_lc[128];
@@ -310,11 +286,12 @@ __global__ void __launch_bounds__(256) ea_pf_kvslice(Params P) {
     __syncthreads();
     const int64_t n = (int64_t)tile * 64 + key;
     const bool valid = n < P.seq_len[b];
-    const int64_t ko = (valid ? kv_off(P, b, n, hk, 0) : 0) + 32 * q4, vo = (valid ? kv_off(P, b, n, hk, 1) : 0) + 32 * q4;
+    const uint16_t* kr = P.k + (valid ? kv_off(P, b, n, hk, 0) : 0) + 32 * q4;
+    const uint16_t* vr = P.v + (valid ? kv_off(P, b, n, hk, 1) : 0) + 32 * q4;
     int bad;
     {
         Slice32 S;
-        slice32<KV4>(P.k, P.ks, ko, valid, S, nullptr, MOD ? P.g.head_dim - 32 * q4 : 32);
+        slice32(kr, valid, S, nullptr, MOD ? P.g.head_dim - 32 * q4 : 32);
 #pragma unroll
         for (int sp = 0; sp < 4; ++sp) {
 #pragma unroll
@@ -339,7 +316,7 @@ __global__ void __launch_bounds__(256) ea_pf_kvslice(Params P) {
     {
         Slice32 S;
         int lost[32];
-        slice32<KV4>(P.v, P.vs, vo, valid, S, lost, MOD ? P.g.head_dim_v - 32 * q4 : 32);
+        slice32(vr, valid, S, lost, MOD ? P.g.head_dim_v - 32 * q4 : 32);
         const int gq = (key >> 2) & 3, kt = key >> 4, ii = key & 3;
 #pragma unroll
         for (int sp = 0; sp < 4; ++sp)
@@ -508,9 +485,7 @@ int ea::ea_launch_prefill(const Params& P, hipStream_t st) {
     if (e != hipSuccess) return -100 - (int)e;
     if (P.nseg > 0 && P.pf_ntiles > 0 && !P.pf_kv_cached) {
         const dim3 grid((unsigned)(P.nseg * P.pf_ntiles));
-        if (P.ks && P.mods) hipLaunchKernelGGL((ea_pf_kvslice<true, true>), grid, dim3(256), 0, st, Pc);
-        else if (P.ks) hipLaunchKernelGGL((ea_pf_kvslice<false, true>), grid, dim3(256), 0, st, Pc);
-        else if (P.mods) hipLaunchKernelGGL(ea_pf_kvslice<true>, grid, dim3(256), 0, st, Pc);
+        if (P.mods) hipLaunchKernelGGL(ea_pf_kvslice<true>, grid, dim3(256), 0, st, Pc);
         else hipLaunchKernelGGL(ea_pf_kvslice<false>, grid, dim3(256), 0, st, Pc);
         e = hipGetLastError();
         if (e != hipSuccess) return -100 - (int)e;

@@ -194,7 +194,7 @@ __device__ inline void dd_rows(const Params& P, DDSmem& S, int cnt, int C, DDPar
             // requested first, so that one memory latency covers K and V
             const int kb = 16 * wv;
             const int nk = (int)max((int64_t)0, min((int64_t)16, jc1 - j0 - kb));
-            const int64_t myoff = lane < nk ? kv_off(P, b, key_n(j0 + kb + lane), hk, 1) : 0;
+            const int64_t myoff = lane >= nk ? 0 : (P.vs ? kv4_v(P, b, key_n(j0 + kb + lane), hk) : kv_off(P, b, key_n(j0 + kb + lane), hk, 1));
             uint32_t vx[16];
 #pragma unroll
             for (int kk = 0; kk < 16; ++kk) {
@@ -202,7 +202,7 @@ __device__ inline void dd_rows(const Params& P, DDSmem& S, int cnt, int C, DDPar
                 vx[kk] = 0;
                 if (kk < nk && 2 * lane < dv) {
                     const uint16_t* vp = P.v + o + 2 * lane;
-                    if (P.vs) vx[kk] = kv4_load2(P.v, P.vs, o + 2 * lane);
+                    if (P.vs) vx[kk] = kv4_vload2(P.v, P.vs, o, 2 * lane);
                     else vx[kk] = v4 ? *(const uint32_t*)vp : ((uint32_t)vp[0] | ((uint32_t)vp[1] << 16));
                 }
             }

@@ -175,7 +175,7 @@ def load():
         lib.ea_hip_attention_kv4.argtypes = [G, B, O, M, X, P, ctypes.c_size_t, P]
         lib.ea_hip_kv4_workspace_size.argtypes = [G, O, M, ctypes.POINTER(ctypes.c_size_t), ctypes.POINTER(ctypes.c_int32)]
         lib.ea_hip_exact_rows_kv4.argtypes = [G, B, O, M, X, P]
-        lib.ea_hip_kv4_values.argtypes = [ctypes.c_int64, ctypes.c_int32, P, P, P, P]
+        lib.ea_hip_kv4_values.argtypes = [ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, P, P, P, P]
         lib.ea_hip_norm_rotary.argtypes = [ctypes.POINTER(NormRotaryArgs), P]
         lib.ea_hip_norm_rotary_grad.argtypes = [ctypes.POINTER(NormRotaryGradArgs), P]
         lib.ea_hip_draft_check.argtypes = [ctypes.POINTER(DraftCheckArgs), P]

@@ -16,11 +16,13 @@ GROUP = 32  # elements to a scale
 
 
 class KV4Pool:
-    """Pages of `page_size` slots, a head's slots one after another:
+    """Pages of `page_size` slots, a head's slots one after another; w is head_dim in whole groups of 32:
 
-      k, v                 (pages, Hkv, page_size, width / 2) uint8, element 2 i in the low half of byte i; width:
-                           head_dim in whole groups of 32
-      k_scales, v_scales   (pages, Hkv, page_size, width / 32) uint8, 2^(byte - 127), 255 NaN
+      k          (pages, Hkv, page_size, w / 2) uint8, element 2 i of a key in the low half of byte i
+      k_scales   (pages, Hkv, page_size, w / 32) uint8, 2^(byte - 127), 255 NaN
+      v          (pages, Hkv, page_size / 16, w / 2, 16) uint8: for 16 slots, channels 2 i and 2 i + 1 (its low half the first)
+                 of each slot, as the matrix instructions sum over keys
+      v_scales   (pages, Hkv, page_size / 16, w / 32, 16) uint8
 
     zero in a new pool (all values 0). `of` takes arrays that are there already."""
 
@@ -29,16 +31,22 @@ class KV4Pool:
         if num_pages < 0 or num_kv_heads <= 0 or head_dim <= 0:
             raise ValueError("num_pages must not be negative, num_kv_heads and head_dim positive")
         w = -(-head_dim // GROUP)
-        new = [torch.zeros((num_pages, num_kv_heads, page_size, n), dtype=torch.uint8, device=device)
-               for n in (16 * w, w, 16 * w, w)]
+        new = [torch.zeros((num_pages, num_kv_heads, page_size, n), dtype=torch.uint8, device=device) for n in (16 * w, w)]
+        new += [torch.zeros((num_pages, num_kv_heads, page_size // 16, n, 16), dtype=torch.uint8, device=device) for n in (16 * w, w)]
         self._take(*new, head_dim)
 
     @classmethod
     def of(cls, k, k_scales, v, v_scales, head_dim: int) -> "KV4Pool":
-        """A pool on these four tensors (in the layout above, contiguous)."""
+        """A pool on these four tensors (contiguous), v and v_scales in tiles as above, or, copied then, in rows as k and k_scales
+        are."""
         self = cls.__new__(cls)
-        self._take(k, k_scales, v, v_scales, head_dim)
+        tiles = [t.unflatten(2, (-1, 16)).transpose(3, 4).contiguous() if t.dim() == 4 and t.shape[2] % 16 == 0 else t for t in (v, v_scales)]
+        self._take(k, k_scales, *tiles, head_dim)
         return self
+
+    def rows(self):
+        """k, k_scales, v and v_scales, all in rows: what `of` takes (copies of v's)."""
+        return (self.k, self.k_scales, *(t.transpose(3, 4).flatten(2, 3).contiguous() for t in (self.v, self.v_scales)))
 
     def _take(self, k, ks, v, vs, d):
         import torch
@@ -46,15 +54,17 @@ class KV4Pool:
         if k.dim() != 4 or k.shape[3] != 16 * w:
             raise ValueError(f"k must be (pages, heads, page_size, {16 * w})")
         pages, heads, P, _ = k.shape
-        for name, t, n in (("k", k, 16 * w), ("k_scales", ks, w), ("v", v, 16 * w), ("v_scales", vs, w)):
-            if t.dtype != torch.uint8 or tuple(t.shape) != (pages, heads, P, n) or not t.is_contiguous() or t.device != k.device:
-                raise ValueError(f"{name} must be a contiguous uint8 tensor ({pages}, {heads}, {P}, {n}) on {k.device}")
-        if d <= 0 or d % 8:
-            raise ValueError("head_dim must be a multiple of 8")
         if P <= 0 or P & (P - 1) or P < 16:
             raise ValueError("page_size must be a power of two of 16 slots or more")
-        if k.data_ptr() % 16 or v.data_ptr() % 16:
-            raise ValueError("k and v must start on 16 bytes")
+        for name, t, shape in (("k", k, (P, 16 * w)), ("k_scales", ks, (P, w)), ("v", v, (P // 16, 16 * w, 16)),
+                               ("v_scales", vs, (P // 16, w, 16))):
+            shape = (pages, heads, *shape)
+            if t.dtype != torch.uint8 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != k.device:
+                raise ValueError(f"{name} must be a contiguous uint8 tensor {shape} on {k.device}")
+        if d <= 0 or d % 8:
+            raise ValueError("head_dim must be a multiple of 8")
+        if k.data_ptr() % 16 or v.data_ptr() % 16 or vs.data_ptr() % 4:
+            raise ValueError("k and v must start on 16 bytes, v_scales on 4")
         at = [(t.data_ptr(), t.data_ptr() + t.numel()) for t in (k, ks, v, vs)]
         if any(a[0] < b[1] and b[0] < a[1] for i, a in enumerate(at) for b in at[i + 1:]):
             raise ValueError("the pool's tensors share memory")
@@ -78,10 +88,10 @@ class KV4Pool:
         shape = (self.num_pages, self.Hkv, self.page_size, self.head_dim)
         out = []
         with torch.cuda.device(self.dev):
-            for codes, scales in ((self.k, self.k_scales), (self.v, self.v_scales)):
+            for is_v, codes, scales in ((0, self.k, self.k_scales), (1, self.v, self.v_scales)):
                 x = torch.empty(shape, dtype=torch.bfloat16, device=self.dev)
-                hip._check(hip.load().ea_hip_kv4_values(x.numel() // self.head_dim, self.head_dim, codes.data_ptr(), scales.data_ptr(),
-                                                        x.data_ptr(), hip._stream_ptr(torch)), "ea_hip_kv4_values")
+                hip._check(hip.load().ea_hip_kv4_values(x.numel() // self.head_dim, self.head_dim, is_v, codes.data_ptr(),
+                                                        scales.data_ptr(), x.data_ptr(), hip._stream_ptr(torch)), "ea_hip_kv4_values")
                 out.append(x)
         return tuple(out)
 

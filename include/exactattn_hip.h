@@ -463,18 +463,23 @@ typedef struct ea_rotary {
 int ea_hip_rotary(const ea_rotary* a, ea_stream_t stream);
 
 /* Caches held in 4 bits, in the microscaling format of 4-bit floats: an element is a sign, 2 bits of exponent and 1 of
- * mantissa (0, 0.5, 1, 1.5, 2, 3, 4, 6), element 2 i of a row in the low half of byte i, and a byte b scales 32
- * consecutive ones by 2^(b - 127) (255: NaN). Every value is a bf16, so attention over such a cache is defined as, and
- * equals to the bit, attention over the bf16 cache of its values; values past the largest bf16 are infinities.
- * ea_hip_attention_kv4 is ea_hip_attention_mods (m may be NULL) with b->k and b->v pointing at codes and x at the scales.
- * The geometry's strides count elements and are multiples of 32: an element at offset e has its code in byte e / 2 and its
- * scale in byte e / 32, so a row of d elements takes whole groups, (d + 31) / 32 scales. head_dim and head_dim_v are multiples
- * of 8, pages (with a block table) hold 16 slots or more, codes start on 16 bytes. Refused: digit-tile caches, phase
- * timers, EA_KERNEL_DECODE and EA_KERNEL_GENERAL (-2), strides, pages and pointers other than these, or so large that 32
- * slots span 2^29 elements (-1).
+ * mantissa (0, 0.5, 1, 1.5, 2, 3, 4, 6), and a byte b scales 32 consecutive ones of a row by 2^(b - 127) (255: NaN). Every value
+ * is a bf16, so attention over such a cache is defined as, and equals to the bit, attention over the bf16 cache of its values;
+ * values past the largest bf16 are infinities.
+ *   K   element 2 i of a row in the low half of byte i. The strides count elements and are multiples of 32: an element at offset
+ *       e has its code in byte e / 2 and its scale in byte e / 32
+ *   V   16 slots of a head are a tile: w / 2 pairs of channels (w: head_dim_v in whole groups of 32) by 16 slots, a byte for a pair
+ *       (the even channel in its low half) and slot; scales w / 32 groups by 16 slots. v_slot_stride is w, the other strides
+ *       multiples of 128 elements: with at = page v_page_stride + head v_head_stride, channel c of slot s has its code in byte
+ *       at / 2 + 8 w (s / 16) + 16 (c / 2) + s % 16 and its scale in at / 32 + (w / 2) (s / 16) + 16 (c / 32) + s % 16. Tiles are there
+ *       whole, whatever the last slot in use
+ * ea_hip_attention_kv4 is ea_hip_attention_mods (m may be NULL) with b->k and b->v pointing at codes, which start on 16 bytes, and x at
+ * the scales, V's on 4. head_dim and head_dim_v are multiples of 8, pages (with a block table) hold 16 slots or more. Refused:
+ * digit-tile caches, phase timers, a choice of kernel (-2), other strides, pages and pointers than these, slots of K 2^24 elements
+ * apart, or sequences of 2^29 keys (-1).
  * ea_hip_kv4_workspace_size, ea_hip_exact_rows_kv4: the workspace and the host's exact tier of such a step.
- * ea_hip_kv4_values: rows of whole groups (codes, scales) -> rows of head_dim bf16, both dense. No reference
- * counterpart. */
+ * ea_hip_kv4_values: dense rows of K (is_v 0), or slots of dense tiles of V (a multiple of 16), to rows of head_dim bf16. No
+ * reference counterpart. */
 typedef struct ea_kv4 {
     const uint8_t* k_scales;
     const uint8_t* v_scales;
@@ -484,17 +489,18 @@ int ea_hip_attention_kv4(const ea_geometry* g, const ea_buffers* b, const ea_opt
 int ea_hip_kv4_workspace_size(const ea_geometry* g, const ea_options* o, const ea_score_mods* m, size_t* bytes, int32_t* nsplit);
 int ea_hip_exact_rows_kv4(const ea_geometry* g, const ea_buffers* b, const ea_options* o, const ea_score_mods* m, const ea_kv4* x,
                           ea_stream_t stream);
-int ea_hip_kv4_values(int64_t rows, int32_t head_dim, const uint8_t* codes, const uint8_t* scales, uint16_t* values,
+int ea_hip_kv4_values(int64_t rows, int32_t head_dim, int32_t is_v, const uint8_t* codes, const uint8_t* scales, uint16_t* values,
                       ea_stream_t stream);
 
 /* ea_hip_rotary with a norm of every query and key head in front, into a bf16 or a 4-bit cache.
  *   norm   x -> x rsqrt(mean x^2 + eps) w over the head's elements, w = q_weight or k_weight (head_dim entries, bf16, or fp32
  *          with weights_fp32); both NULL: none
  *   turn   as ea_rotary says; half_turns NULL (with rot_dim 0): none
- *   4 bit  with k_scales and v_scales set, k_out and v_out are codes. Row r of dst_rows is slot r % page_size of page
- *          r / page_size, at element (r / page_size) page_stride + (r % page_size) ko_tok_stride + head ko_head_stride (vo alike; multiples
- *          of 32). A group's scale is the smallest 2^e with max|x| < 7 2^e, e in [-125, 125], so that no element
- *          below 7 2^125 is off by more than half a step; elements go to the nearest, ties to the even code, larger ones to 6 2^125. A group
+ *   4 bit  with k_scales and v_scales set, k_out and v_out are a 4-bit cache's codes. Row r of dst_rows is slot r % page_size of
+ *          page r / page_size; K's strides are k_page_stride, ko_tok_stride and ko_head_stride, V's v_page_stride, vo_tok_stride (w) and
+ *          vo_head_stride, as ea_kv4 asks, page_size a multiple of 16. A group's scale is the smallest 2^e with max|x| < 7 2^e, e in
+ *          [-125, 125], so that no element below 7 2^125 is off by more than half a step; elements go to the nearest, ties to the even
+ *          code, larger ones to 6 2^125. A group
  *          with a NaN, an infinity or a value past fp32's becomes scale 255. Codes past head_dim are left alone.
  * Everything is computed in fp64 and rounded once. head_dim is even or at most 128. r.inverse is refused with a norm. In
  * 4 bits head_dim is a multiple of 8 and rot_dim of 4. r.q_out may be r.q and r.k_out r.k (bf16 or fp32) as with

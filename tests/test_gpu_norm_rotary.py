@@ -174,7 +174,7 @@ def test_append_in_4_bits(gpu, case, dtype, normed):
     page, slot = dst[live] // P, dst[live] % P
     y = _norm64(k, norm.k_weight, norm.eps) if normed else k.double().cpu().numpy()
     k64 = _turned(rot, y, pos)[live]
-    arrays = [a.cpu().numpy() for a in (pool.k, pool.k_scales, pool.v, pool.v_scales)]
+    arrays = [a.cpu().numpy() for a in pool.rows()]
     # elements that neither the norm nor the rotation changes are exact, ties among them
     slack = np.where(normed | (np.arange(d) < rot.rot_dim), 2.0 ** -36 * np.abs(y).max(), 0.0)
     _codes_match(arrays[0][page, :, slot], arrays[1][page, :, slot], k64, slack)
@@ -211,7 +211,8 @@ def test_pool_append(gpu, d, dtype):
     dst = r.permutation(7 * P)[:n].astype(np.int64)
     pool.append(x[0].transpose(0, 1).contiguous().transpose(0, 1), x[1], torch.from_numpy(dst).cuda())
     page, slot = dst // P, dst % P
-    for t, codes, scales in ((x[0], pool.k, pool.k_scales), (x[1], pool.v, pool.v_scales)):
+    rows = pool.rows()
+    for t, codes, scales in ((x[0], *rows[:2]), (x[1], *rows[2:])):
         c, s = f4.quantize(t.double().cpu().numpy())
         bad = np.repeat(s == 255, 16, -1)
         got = codes.cpu().numpy()[page, :, slot]
