@@ -49,6 +49,7 @@ using namespace ea;
 namespace {
 
 constexpr int F4_THREADS = 256;
+constexpr int F4_W2 = 2;
 constexpr int F4_NONE = -1200000000;  // base of a row without a visible key so far
 constexpr int F4_BITS = 22;           // a weight's exponent E may exceed the base by this: M < 2^24 then gives 46 bits
 constexpr int F4_HEAD = 2;            // room left when the base moves
@@ -78,8 +79,9 @@ struct FourSmem {
     uint32_t wv[4][4];  // per wave and group: the largest scale
     uint32_t list[4][F4_LIST + 64 * RS];
     double O[4][RS][32 * NG];  // per wave: of channel 32 l + 2 n + h at 32 l + 16 h + n
+    static constexpr int PG = RS == 8 ? 1 : NG;  // groups of channels whose digits lie here together
     union alignas(16) {
-        uint32_t W[4][6 * RS * F4_WROW];
+        uint32_t W[4][PG][6 * RS * F4_WROW];
         uint8_t dig[2][RS * 6 * 128];
     };
 };
@@ -115,20 +117,19 @@ __device__ __forceinline__ uint32_t four_bytes(uint32_t w) {
 // MOD: with score modifications (ea_mod.h): 1 key ranges alone, 2 with a bias, 3 with a cap; a unit's key range is then counted from its
 // rows' first visible key, down to a whole tile, and on uniform splits the last split takes every key past the others.
 template <int RS, int NG, int MOD>
-__global__ void __launch_bounds__(F4_THREADS, 2) ea_four(Params P) {
-    constexpr int RL = RS / 4;            // rows of a lane
-    constexpr int NMF = RS == 4 ? 2 : 3;  // matrix instructions for 6 digits of the rows
+__global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Params P) {
+    constexpr int RL = RS == 8 ? 2 : 1;                  // rows of a lane
+    constexpr int KL = RS == 2 ? 2 : 4;                  // keys of a lane
+    constexpr int NMF = RS == 2 ? 1 : (RS == 4 ? 2 : 3);  // matrix instructions for 6 digits of the rows
     typedef FourSmem<RS, NG> Smem;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     Smem& S = *reinterpret_cast<Smem*>(smem_raw);
     const int tid = (int)threadIdx.x;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int d = P.g.head_dim, dv = P.g.head_dim_v;
-    const int wid = kv4_width(dv), ng = wid >> 5;  // V's channels in whole groups
+    const int wid = kv4_width(dv), ng = NG == 2 ? wid >> 5 : NG;  // V's channels in whole groups: NG, or 1 with NG = 2
 
-    S.T1[tid] = u64_as_f64(EA_T1_BITS[tid]) * 8388608.0;  // 2^23: exact
-    S.T2[tid] = u64_as_f64(EA_T2_BITS[tid]);
-    if (tid < 8) S.zero[tid] = 0;
+    const double t1 = u64_as_f64(EA_T1_BITS[tid]) * 8388608.0, t2 = u64_as_f64(EA_T2_BITS[tid]);  // 2^23: exact
     if (blockIdx.x == 0 && blockIdx.y == 0) {
         // on uniform splits the step's first kernel clears the tier-2 work list and chunk counts
         if (!P.dq_stream && tid < EA_T2_CNT) P.wl_cnt[tid] = 0;
@@ -137,7 +138,7 @@ __global__ void __launch_bounds__(F4_THREADS, 2) ea_four(Params P) {
     }
 
     // One piece: keys [kA, kB) of unit `item` (segment, row block), clipped to the unit's visible end, as partial slot `split`.
-    auto piece = [&](const int item, const int split, int kA, int kB) __attribute__((always_inline)) {
+    auto piece = [&](const bool first, const int item, const int split, int kA, int kB) __attribute__((always_inline)) {
         const int lane = tid & 63;
         const int g = lane >> 4, n = lane & 15;
         const int seg = item / P.nrb, rbk = item % P.nrb;
@@ -149,15 +150,149 @@ __global__ void __launch_bounds__(F4_THREADS, 2) ea_four(Params P) {
             const int lr = row0 + r, t = lr / P.grp, gi = lr % P.grp;
             return P.q + (int64_t)b * P.g.q_seq_stride + (int64_t)t * P.g.q_tok_stride + (int64_t)(hk * P.grp + gi) * P.g.q_head_stride;
         };
+        // what the digits are cut from, requested before anything waits
+        uint32_t qv[(RS + 3) / 4][2];
+#pragma unroll
+        for (int r4 = 0; r4 < RS; r4 += 4)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int i = 2 * lane + h;
+                qv[r4 / 4][h] = r4 + w < nrow && i < d ? q_row(r4 + w)[i] : 0u;
+            }
+        // ---- the rows' visible keys: prefix and tree mask in LDS (tiles inside every prefix do not read them), the last
+        // visible key and the shortest prefix of the block
+        const int slen = P.seq_len[b];
+        const int tb = P.tree_mask ? P.tree_base[b] : 0;
+        int kend = 0, kvmin = INT_MAX;
+        int kbeg = INT_MAX, kbmax = 0;  // MOD: the rows' first visible key, their last prefix start
+        {
+            const int r = lane & (RS - 1);
+            const int tok = b * P.g.num_tokens + (row0 + min(r, nrow - 1)) / P.grp;
+            const int kvl = P.kv_len[tok];
+            const uint64_t tmk = P.tree_mask ? P.tree_mask[tok] : 0ull;
+            kend = tmk ? max(kvl, tb + 64 - (int)__clzll(tmk)) : kvl;
+            kvmin = kvl;
+            if constexpr (MOD) {
+                const int kvb = vis_begin(P, tok, kvl);
+                kbmax = kvb;
+                const KeySpan ks = key_span(kvb, kvl, slen, tmk, tb);
+                kbeg = ks.beg;
+                kend = ks.end;
+                if (w == 0 && lane < RS) {
+                    S.kvb[r] = kvb;
+                    S.pos[r] = mod_pos(P, tok, kvl);
+                    const int lr = row0 + min(r, nrow - 1);
+                    S.slope[r] = mod_slope(P, hk * P.grp + lr % P.grp);
+                }
+            }
+            if (w == 0 && lane < RS) {
+                S.kvl[r] = r < nrow ? kvl : INT_MIN;
+                S.tmk[r] = r < nrow ? tmk : 0ull;
+            }
+        }
+        kend = min(wave_max_dpp(kend), slen);
+        kvmin = min(-wave_max_dpp(-kvmin), slen);
+        if constexpr (MOD) {
+            kbeg = -wave_max_dpp(-kbeg);
+            kbmax = wave_max_dpp(kbmax);
+            const int k0 = kend > 0 ? tile_floor(kbeg) : 0;
+            kA += k0;
+            kB += k0;
+        }
+        const int k1 = min(kB, kend);
+        const int k0w = kA + 64 * w;  // this wave's tiles: k0w + 256 it
+        const int nst = k1 > k0w ? (k1 - k0w + 255) >> 8 : 0;
+        const int row = RS == 2 ? g >> 1 : RL * g;  // the lane's rows: row + j
+        const int sub = RS == 2 ? 2 * (g & 1) : 0;  // its keys of a tile: 4 n + sub + i
+        constexpr int RLANES = RS == 2 ? 32 : 16;   // lanes of a row
+        const bool head = n == 0 && sub == 0;       // the first of them
+        // Loads of a tile stand under no branch: one that waits for older loads could not tell how many younger ones there are, and
+        // would wait for all. So caches without pages look one up (and do not use it), and the last tile requests its last run again.
+        cint_t* btb = P.bt ? (cint_t*)P.bt + (P.bt_off ? P.bt_off[b] : (int64_t)b * P.g.block_table_stride) : (cint_t*)P.seq_len;
+        const int bmask = P.bt ? -1 : 0;
+        const int pshift = P.pshift, pmask = (1 << pshift) - 1;
+        // 16 consecutive keys from a multiple of 16 (a run) lie in one page (page size >= 16) and are one tile of V. Runs past the
+        // last key (or, MOD, before the first) read the last one's again, as keys past the last one do within theirs, and weigh
+        // nothing. Offsets count 32 elements: 16 bytes, or one scale.
+        auto run_of = [&](int n0, int at) __attribute__((always_inline)) {
+            int m = min(n0 + 16 * at, k1 - 1);
+            if constexpr (MOD) m = max(m, kbeg);
+            return m & ~15;
+        };
+        struct Pages {
+            int k, v;
+        };
+        auto pages_of = [&](int n0) __attribute__((always_inline)) {
+            const int pk = btb[(run_of(n0, n >> 2) >> pshift) & bmask], pv = btb[(run_of(n0, g) >> pshift) & bmask];
+            return (Pages){P.bt ? pk : b, P.bt ? pv : b};
+        };
+        auto times = [](int x, int64_t stride) __attribute__((always_inline)) {  // x >= 0
+            return (uint64_t)(uint32_t)x * (uint32_t)stride + ((uint64_t)((uint32_t)x * (uint32_t)(stride >> 32)) << 32);
+        };
+        struct KR {
+            f4_u4 k[4];
+            uint32_t s[4];
+        };
+        struct VR {
+            f4_u4 v[NG];
+            uint32_t s[NG];
+        };
+        const int64_t kps = P.g.k_page_stride >> 5, kss = P.g.k_slot_stride >> 5, vps = P.g.v_page_stride >> 5;
+        const int gk = min(g, (d - 1) >> 5);  // blocks past the head: q's digits are zeros there
+        const char* const kbase = (const char*)P.k + (((int64_t)hk * P.g.k_head_stride) >> 1) + 16 * gk;
+        const uint8_t* const ksbase = P.ks + (((int64_t)hk * P.g.k_head_stride) >> 5) + gk;
+        const char* const vbase = (const char*)P.v + (((int64_t)hk * P.g.v_head_stride) >> 1) + 16 * n;
+        const uint8_t* const vsbase = P.vs + (((int64_t)hk * P.g.v_head_stride) >> 5) + 4 * (n & 3) + sub;
+        auto issue_k = [&](int n0, const Pages& p, KR& x) __attribute__((always_inline)) {
+            const int run = run_of(n0, n >> 2), lim = k1 - 1 - run;
+            const uint64_t at = times(p.k, kps) + times(P.bt ? run & pmask : run, kss);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const uint64_t to = at + (uint64_t)((uint32_t)min(4 * (n & 3) + u, lim) * (uint32_t)kss);
+                x.k[u] = *(const f4_u4*)(kbase + (to << 4));
+                x.s[u] = ksbase[to];
+            }
+        };
+        auto issue_v = [&](int n0, const Pages& p, VR& x) __attribute__((always_inline)) {
+            const int rv = run_of(n0, g), rs = run_of(n0, n >> 2);
+            const uint64_t at = times(p.v, vps) + times((P.bt ? rv & pmask : rv) >> 4, wid >> 1);
+            const uint64_t as = times(p.k, vps) + times((P.bt ? rs & pmask : rs) >> 4, wid >> 1);
+            const char* const vc = vbase + (at << 4);
+            const uint8_t* const vs = vsbase + as;
+#pragma unroll
+            for (int l = 0; l < NG; ++l) {
+                const int lx = min(l, ng - 1);
+                x.v[l] = *(const f4_u4*)(vc + 256 * lx);
+                x.s[l] = KL == 4 ? *(const uint32_t*)(vs + 16 * lx) : *(const uint16_t*)(vs + 16 * lx);
+            }
+        };
+
+        // the first tile is requested before the digits are cut
+        KR kr;
+        VR vr;
+        Pages nx = {0, 0};  // of the next tile
+        auto begin = [&](int n0) __attribute__((always_inline)) {
+            const Pages p = pages_of(n0);
+            nx = pages_of(n0 + 256);
+            issue_k(n0, p, kr);
+            issue_v(n0, p, vr);
+        };
+        if (nst > 0) begin(k0w);
+        if (first) {
+            S.T1[tid] = t1;
+            S.T2[tid] = t2;
+            if (tid < 8) S.zero[tid] = 0;
+        }
         // ---- q's digits: X = q / 2^lsb, |X| < 2^28, in 6 digits of 5 bits
-        for (int r = w; r < RS; r += 4) {
+#pragma unroll
+        for (int r4 = 0; r4 < RS; r4 += 4) {
+            const int r = r4 + w;
+            if (r >= RS) break;
             int m[2] = {0, 0}, e[2] = {0, 0}, bad = 0, lead = INT_MIN;
             if (r < nrow) {
-                const uint16_t* qr = q_row(r);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int i = 2 * lane + h;
-                    const uint32_t x = i < d ? qr[i] : 0u;
+                    const uint32_t x = qv[r4 / 4][h];
                     const int f = (x >> 7) & 0xFF;
                     bad |= f == 0xFF;
                     m[h] = (int)(x & 0x7F) | (f ? 0x80 : 0);
@@ -213,49 +348,6 @@ __global__ void __launch_bounds__(F4_THREADS, 2) ea_four(Params P) {
                 S.rqe[r] = fabs(P.alpha) * (double)lost * ldexp(0.5 * (1.0 + 0x1p-20), lsb - 28);
             }
         }
-        // ---- the rows' visible keys: prefix and tree mask in LDS (tiles inside every prefix do not read them), the last
-        // visible key and the shortest prefix of the block
-        const int slen = P.seq_len[b];
-        const int tb = P.tree_mask ? P.tree_base[b] : 0;
-        int kend = 0, kvmin = INT_MAX;
-        int kbeg = INT_MAX, kbmax = 0;  // MOD: the rows' first visible key, their last prefix start
-        {
-            const int r = lane & (RS - 1);
-            const int tok = b * P.g.num_tokens + (row0 + min(r, nrow - 1)) / P.grp;
-            const int kvl = P.kv_len[tok];
-            const uint64_t tmk = P.tree_mask ? P.tree_mask[tok] : 0ull;
-            kend = tmk ? max(kvl, tb + 64 - (int)__clzll(tmk)) : kvl;
-            kvmin = kvl;
-            if constexpr (MOD) {
-                const int kvb = vis_begin(P, tok, kvl);
-                kbmax = kvb;
-                const KeySpan ks = key_span(kvb, kvl, slen, tmk, tb);
-                kbeg = ks.beg;
-                kend = ks.end;
-                if (w == 0 && lane < RS) {
-                    S.kvb[r] = kvb;
-                    S.pos[r] = mod_pos(P, tok, kvl);
-                    const int lr = row0 + min(r, nrow - 1);
-                    S.slope[r] = mod_slope(P, hk * P.grp + lr % P.grp);
-                }
-            }
-            if (w == 0 && lane < RS) {
-                S.kvl[r] = r < nrow ? kvl : INT_MIN;
-                S.tmk[r] = r < nrow ? tmk : 0ull;
-            }
-        }
-        kend = min(wave_max_dpp(kend), slen);
-        kvmin = min(-wave_max_dpp(-kvmin), slen);
-        if constexpr (MOD) {
-            kbeg = -wave_max_dpp(-kbeg);
-            kbmax = wave_max_dpp(kbmax);
-            const int k0 = kend > 0 ? tile_floor(kbeg) : 0;
-            kA += k0;
-            kB += k0;
-        }
-        const int k1 = min(kB, kend);
-        const int k0w = kA + 64 * w;  // this wave's tiles: k0w + 256 it
-        const int nst = k1 > k0w ? (k1 - k0w + 255) >> 8 : 0;
         __syncthreads();  // the digits are in LDS: 32 of a block to 24 bytes
         int two = 0;  // does a row of the block need the second round?
 #pragma unroll
@@ -278,85 +370,25 @@ __global__ void __launch_bounds__(F4_THREADS, 2) ea_four(Params P) {
         __syncthreads();
         // the lane's part of a row block's digits, instruction j: M = n is digit 4 j + n % 4 of the digits of the rows of n / 4
         auto q_part = [&](int k2, int j) __attribute__((always_inline)) {
-            const int c = 4 * j + (n & 3), qr = RL * (n >> 2) + (c >= 6 ? 1 : 0), qk = c >= 6 ? c - 6 : c;
-            const uint32_t* const p = RS == 4 && c >= 6 ? S.zero : &S.q6[k2][((qr * 6 + qk) * 4 + g) * 6];
+            int c = RS == 2 ? n & 7 : 4 * j + (n & 3);
+            asm volatile("" : "+v"(c));  // read where it is used
+            const int qr = RS == 2 ? n >> 3 : RL * (n >> 2) + (c >= 6 ? 1 : 0), qk = c >= 6 ? c - 6 : c;
+            const uint32_t* const p = RS != 8 && c >= 6 ? S.zero : &S.q6[k2][((qr * 6 + qk) * 4 + g) * 6];
             const f4_u2 x = *(const f4_u2*)p, y = *(const f4_u2*)(p + 2), t = *(const f4_u2*)(p + 4);
             return (f4_i8){(int)x.x, (int)x.y, (int)y.x, (int)y.y, (int)t.x, (int)t.y, 0, 0};
         };
+        // 8 rows leave no registers for what the tile needs once: q's digits are read again for every tile
+        constexpr bool AGAIN = RS == 8;
         f4_i8 qd[NMF];
 #pragma unroll
-        for (int j = 0; j < NMF; ++j) qd[j] = q_part(0, j);
-        const int row = RL * g;  // the lane's rows: row + j
-        cint_t* btb = (cint_t*)P.bt + (P.bt ? (P.bt_off ? P.bt_off[b] : (int64_t)b * P.g.block_table_stride) : 0);
-        const int pshift = P.pshift, pmask = (1 << pshift) - 1;
-        // 16 consecutive keys from a multiple of 16 (a run) lie in one page (page size >= 16) and are one tile of V. Runs past the
-        // last key (or, MOD, before the first) read the last one's again, as keys past the last one do within theirs, and weigh
-        // nothing. Offsets count 32 elements: 16 bytes, or one scale.
-        auto run_of = [&](int n0, int at) __attribute__((always_inline)) {
-            int m = min(n0 + 16 * at, k1 - 1);
-            if constexpr (MOD) m = max(m, kbeg);
-            return m & ~15;
-        };
-        struct Pages {
-            int k, v;
-        };
-        auto pages_of = [&](int n0) __attribute__((always_inline)) {
-            Pages p = {b, b};
-            if (P.bt) {
-                p.k = btb[run_of(n0, n >> 2) >> pshift];
-                p.v = btb[run_of(n0, g) >> pshift];
-            }
-            return p;
-        };
-        auto times = [](int x, int64_t stride) __attribute__((always_inline)) {  // x >= 0
-            return (uint64_t)(uint32_t)x * (uint32_t)stride + ((uint64_t)((uint32_t)x * (uint32_t)(stride >> 32)) << 32);
-        };
-        struct KR {
-            f4_u4 k[4];
-            uint32_t s[4];
-        };
-        struct VR {
-            f4_u4 v[NG];
-            uint32_t s[NG];
-        };
-        const int64_t kps = P.g.k_page_stride >> 5, kss = P.g.k_slot_stride >> 5, vps = P.g.v_page_stride >> 5;
-        const int gk = min(g, (d - 1) >> 5);  // blocks past the head: q's digits are zeros there
-        const char* const kbase = (const char*)P.k + (((int64_t)hk * P.g.k_head_stride) >> 1) + 16 * gk;
-        const uint8_t* const ksbase = P.ks + (((int64_t)hk * P.g.k_head_stride) >> 5) + gk;
-        const char* const vbase = (const char*)P.v + (((int64_t)hk * P.g.v_head_stride) >> 1) + 16 * n;
-        const uint8_t* const vsbase = P.vs + (((int64_t)hk * P.g.v_head_stride) >> 5) + 4 * (n & 3);
-        auto issue_k = [&](int n0, const Pages& p, KR& x) __attribute__((always_inline)) {
-            const int run = run_of(n0, n >> 2), lim = k1 - 1 - run;
-            const uint64_t at = times(p.k, kps) + times(P.bt ? run & pmask : run, kss);
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const uint64_t to = at + (uint64_t)((uint32_t)min(4 * (n & 3) + u, lim) * (uint32_t)kss);
-                x.k[u] = *(const f4_u4*)(kbase + (to << 4));
-                x.s[u] = ksbase[to];
-            }
-        };
-        auto issue_v = [&](int n0, const Pages& p, VR& x) __attribute__((always_inline)) {
-            const int rv = run_of(n0, g), rs = run_of(n0, n >> 2);
-            const uint64_t at = times(p.v, vps) + times((P.bt ? rv & pmask : rv) >> 4, wid >> 1);
-            const uint64_t as = times(p.k, vps) + times((P.bt ? rs & pmask : rs) >> 4, wid >> 1);
-            const char* const vc = vbase + (at << 4);
-            const uint8_t* const vs = vsbase + as;
-#pragma unroll
-            for (int l = 0; l < NG; ++l) {
-                x.v[l] = l < ng ? *(const f4_u4*)(vc + 256 * l) : (f4_u4){0u, 0u, 0u, 0u};
-                x.s[l] = l < ng ? *(const uint32_t*)(vs + 16 * l) : 0u;
-            }
-        };
-
+        for (int j = 0; j < NMF; ++j)
+            if (!AGAIN) qd[j] = q_part(0, j);
         const double alpha = P.alpha;
-        double rq[RL], rqe[RL];
         int rfl[RL];   // the row is left to tier 2
         int base[RL];  // of the row
         double z[RL], lostw[RL];  // the weights' sum, and what rounding took from their whole numbers
 #pragma unroll
         for (int j = 0; j < RL; ++j) {
-            rq[j] = S.rq[row + j];
-            rqe[j] = S.rqe[row + j];
             rfl[j] = S.bad[row + j];
             base[j] = F4_NONE;
             z[j] = lostw[j] = 0.0;
@@ -371,23 +403,38 @@ __global__ void __launch_bounds__(F4_THREADS, 2) ea_four(Params P) {
         int lo = -100000;      // scales of keys in [lo, lo + F4_SPREAD] need no closer look
         double kbnd = 0.0;     // an upper bound of |k| for such keys
         f4_i4 acc[NMF][2 * NG];
-        double* const O = &S.O[w][row][n];  // [j][c]: the lane's own
+        // the lane's own sums: [j][c], or with 2 rows those of c = 2 l + g % 2
+        constexpr int OC = RS == 2 ? NG : 2 * NG, OS = RS == 2 ? 32 : 16;
+        double* const O = &S.O[w][row][8 * sub + n];
 #pragma unroll
         for (int c = 0; c < 2 * NG; ++c) {
 #pragma unroll
             for (int j = 0; j < NMF; ++j) acc[j][c] = (f4_i4){0, 0, 0, 0};
 #pragma unroll
-            for (int j = 0; j < RL; ++j) O[j * 32 * NG + 16 * c] = 0.0;
+            for (int j = 0; j < RL; ++j)
+                if (c < OC) O[j * 32 * NG + OS * c] = 0.0;
         }
         int since = 0, folds = 0;
         int n5 = 0, n6 = 0, n8 = 0, cnt = 0;  // wave-uniform
-        const double gw = RS == 4 ? (g == 0 ? 1.0 : (g == 1 ? 0x1p8 : (g == 2 ? 0x1p16 : 0x1p24))) : (g < 2 ? 1.0 : 0x1p8);
+        const double gw = RS == 2 ? (g == 0 ? 1.0 : (g == 1 ? 0x1p16 : 0x1p32)) : RS == 4 ? (g == 0 ? 1.0 : (g == 1 ? 0x1p8 : (g == 2 ? 0x1p16 : 0x1p24))) : (g < 2 ? 1.0 : 0x1p8);
 
         // the int32 sums into the fp64 ones: digits joined, the lanes' parts added up, each lane left with its own rows
         auto fold = [&]() __attribute__((always_inline)) {
 #pragma unroll
             for (int l = 0; l < NG; ++l) {
                 const double unit = ldexp(gw, G[l] - 128);  // in halves of 2^(G - 127)
+                if constexpr (RS == 2) {
+                    double a[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const f4_i4 x = acc[0][2 * l + h];
+                        const double t0 = __fma_rn((double)x[2], 256.0, (double)x[0]) * unit, t1 = __fma_rn((double)x[3], 256.0, (double)x[1]) * unit;
+                        a[h] = (row ? t1 : t0) + xor32(row ? t0 : t1);
+                        acc[0][2 * l + h] = (f4_i4){0, 0, 0, 0};
+                    }
+                    O[32 * l] += (sub ? a[1] : a[0]) + xor16(sub ? a[0] : a[1]);
+                    continue;
+                }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int c = 2 * l + h;
@@ -403,7 +450,7 @@ __global__ void __launch_bounds__(F4_THREADS, 2) ea_four(Params P) {
                     double a = up ? t[2] : t[0], e = up ? t[3] : t[1];
                     a += xor32(up ? t[0] : t[2]);
                     e += xor32(up ? t[1] : t[3]);
-                    if constexpr (RS == 4) {
+                    if constexpr (RS != 8) {
                         const bool odd = g & 1;
                         O[16 * c] += (odd ? e : a) + xor16(odd ? a : e);
                     } else {
@@ -430,12 +477,11 @@ __global__ void __launch_bounds__(F4_THREADS, 2) ea_four(Params P) {
                 base[j] = nb;
             }
 #pragma unroll
-            for (int c = 0; c < 2 * NG; ++c) O[j * 32 * NG + 16 * c] *= f;
+            for (int c = 0; c < OC; ++c) O[j * 32 * NG + OS * c] *= f;
         };
 
-        auto tile = [&](int n0, bool more, KR& kr, VR& vr) __attribute__((always_inline)) {
-            Pages nx = {0, 0};
-            if (more) nx = pages_of(n0 + 256);
+        auto tile = [&](int n0) __attribute__((always_inline)) {
+            const Pages after = pages_of(n0 + 512);
             // ---- are the scales near enough to each other for exact sums?
             uint32_t wide = 0;  // bit u: key 4 n + u is left to the exact path
             {
@@ -469,57 +515,73 @@ __global__ void __launch_bounds__(F4_THREADS, 2) ea_four(Params P) {
             }
             const bool edge = n0 + 64 > min(kvmin, k1) || (MOD && n0 < kbmax);
             const bool cut = n0 + 64 > k1 || (MOD && n0 < kbeg);
-            const int kn = n0 + 4 * n;  // the first of the lane's keys
+            const int kn = n0 + 4 * n + sub;  // the first of the lane's keys
+            if constexpr (KL == 2) wide >>= sub;
             // ---- scores: 6 exact sums for every pair
             double sc[RL][4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const f4_i8 B = {(int)kr.k[u].x, (int)kr.k[u].y, (int)kr.k[u].z, (int)kr.k[u].w, 0, 0, 0, 0};
-                f4_f4 D[NMF];
-#pragma unroll
-                for (int j = 0; j < NMF; ++j)
-                    D[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(qd[j], B, (f4_f4){0.0f, 0.0f, 0.0f, 0.0f}, 2, 4, 0, 127, 0,
-                                                                            (int)kr.s[u]);
-#pragma unroll
-                for (int j = 0; j < RL; ++j) {
-                    double x = (double)D[(6 * j + 5) >> 2][(6 * j + 5) & 3];
-#pragma unroll
-                    for (int k = 4; k >= 0; --k) x = __fma_rn(x, 32.0, (double)D[(6 * j + k) >> 2][(6 * j + k) & 3]);
-                    sc[j][u] = x;
-                }
-            }
-            if (__builtin_expect(two, 0)) {
-                f4_i8 q2[NMF];
-#pragma unroll
-                for (int j = 0; j < NMF; ++j) q2[j] = q_part(1, j);
+            auto products = [&](const f4_i8 (&qa)[NMF], double (&x)[RL][4]) __attribute__((always_inline)) {
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     const f4_i8 B = {(int)kr.k[u].x, (int)kr.k[u].y, (int)kr.k[u].z, (int)kr.k[u].w, 0, 0, 0, 0};
                     f4_f4 D[NMF];
 #pragma unroll
                     for (int j = 0; j < NMF; ++j)
-                        D[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(q2[j], B, (f4_f4){0.0f, 0.0f, 0.0f, 0.0f}, 2, 4, 0, 127,
-                                                                                0, (int)kr.s[u]);
+                        D[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(qa[j], B, (f4_f4){0.0f, 0.0f, 0.0f, 0.0f}, 2, 4, 0, 127, 0,
+                                                                                (int)kr.s[u]);
+                    if constexpr (RS == 2) {
+                        x[0][u] = (double)D[0][3];
 #pragma unroll
-                    for (int j = 0; j < RL; ++j) {
-                        double x = (double)D[(6 * j + 5) >> 2][(6 * j + 5) & 3];
+                        for (int k = 2; k >= 0; --k) x[0][u] = __fma_rn(x[0][u], 32.0, (double)D[0][k]);
+                        x[0][u] *= sub ? 0x1p20 : 1.0;
+                    } else {
 #pragma unroll
-                        for (int k = 4; k >= 0; --k) x = __fma_rn(x, 32.0, (double)D[(6 * j + k) >> 2][(6 * j + k) & 3]);
-                        sc[j][u] = __fma_rn(x, 0x1p-28, sc[j][u]);  // one rounding, in ad below
+                        for (int j = 0; j < RL; ++j) {
+                            x[j][u] = (double)D[(6 * j + 5) >> 2][(6 * j + 5) & 3];
+#pragma unroll
+                            for (int k = 4; k >= 0; --k) x[j][u] = __fma_rn(x[j][u], 32.0, (double)D[(6 * j + k) >> 2][(6 * j + k) & 3]);
+                        }
                     }
                 }
+                if constexpr (RS == 2) {
+                    // digits 0..3 of a row's sums lie 16 lanes before digits 4 and 5: the first lane takes keys 0 and 1, the other 2 and 3
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const auto lo = __builtin_amdgcn_permlane16_swap(__double2loint(x[0][u]), __double2loint(x[0][u + 2]), false, false);
+                        const auto hi = __builtin_amdgcn_permlane16_swap(__double2hiint(x[0][u]), __double2hiint(x[0][u + 2]), false, false);
+                        x[0][u] = __hiloint2double((int)hi[0], (int)lo[0]) + __hiloint2double((int)hi[1], (int)lo[1]);
+                    }
+                }
+            };
+            if constexpr (AGAIN) {
+                f4_i8 qt[NMF];
+#pragma unroll
+                for (int j = 0; j < NMF; ++j) qt[j] = q_part(0, j);
+                products(qt, sc);
+            } else {
+                products(qd, sc);
             }
-            if (more) issue_k(n0 + 256, nx, kr);
-            int M[RL][4], E[RL][4];
+            if (__builtin_expect(two, 0)) {
+                f4_i8 q2[NMF];
+                double s2[RL][4];
+#pragma unroll
+                for (int j = 0; j < NMF; ++j) q2[j] = q_part(1, j);
+                products(q2, s2);
+#pragma unroll
+                for (int j = 0; j < RL; ++j)
+#pragma unroll
+                    for (int i = 0; i < KL; ++i) sc[j][i] = __fma_rn(s2[j][i], 0x1p-28, sc[j][i]);  // one rounding, in ad below
+            }
+            issue_k(n0 + 256, nx, kr);
+            int M[RL][KL], E[RL][KL];
             uint32_t good = 0;  // bit 4 j + i
 #pragma unroll
             for (int j = 0; j < RL; ++j) {
                 // ---- which of the pairs are visible
-                uint32_t vis = row + j < nrow ? 15u : 0u;
+                uint32_t vis = row + j < nrow ? (1u << KL) - 1u : 0u;
                 if (edge) {
                     vis = 0;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < KL; ++i) {
                         const int key = kn + i, ti = key - tb;
                         const bool in = ((unsigned)ti < 64u) & (((S.tmk[row + j] >> (ti & 63)) & 1ull) != 0);
                         bool pre = key < S.kvl[row + j];
@@ -528,37 +590,39 @@ __global__ void __launch_bounds__(F4_THREADS, 2) ea_four(Params P) {
                     }
                 }
                 // ---- certified weights
-                const double adel = rqe[j] * kbnd;
-                double s[4], ad[4];
+                int jr = row + j;
+                if constexpr (AGAIN) asm volatile("" : "+v"(jr));
+                const double adel = S.rqe[jr] * kbnd, rq = S.rq[jr];
+                double s[KL], ad[KL];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s[i] = sc[j][i] * rq[j];
+                for (int i = 0; i < KL; ++i) {
+                    s[i] = sc[j][i] * rq;
                     ad[i] = two ? __fma_rn(fabs(s[i] * alpha), 0x1p-52, adel) : adel;
                 }
-                int Mi[4], Ei[4];
-                bool ok[4];
+                int Mi[KL], Ei[KL];
+                bool ok[KL];
                 if constexpr (MOD >= 2) {
-                    float sl[4];
-                    int dist[4];
+                    float sl[KL];
+                    int dist[KL];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < KL; ++i) {
                         sl[i] = S.slope[row + j];
                         dist[i] = kn + i - S.pos[row + j];
                     }
-                    pf::cert_pairs<4, MOD>(s, ad, alpha, S.T1, S.T2, Mi, Ei, ok, P.cap, sl, dist);
+                    pf::cert_pairs<KL, MOD>(s, ad, alpha, S.T1, S.T2, Mi, Ei, ok, P.cap, sl, dist);
                 } else {
-                    pf::cert_pairs<4>(s, ad, alpha, S.T1, S.T2, Mi, Ei, ok);
+                    pf::cert_pairs<KL>(s, ad, alpha, S.T1, S.T2, Mi, Ei, ok);
                 }
                 uint32_t gd = 0;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) gd |= ok[i] ? (1u << i) : 0u;
+                for (int i = 0; i < KL; ++i) gd |= ok[i] ? (1u << i) : 0u;
                 gd &= ~wide;
                 const uint32_t slow = vis & ~gd;
                 gd &= vis;
                 if (__builtin_expect(__ballot(slow != 0) != 0, 0)) {
                     // undecided pairs wait in the wave's list for flush(); a row that is flagged already needs no more of them
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < KL; ++i) {
                         const bool put = ((slow >> i) & 1) && !rfl[j];
                         const uint64_t m = __ballot(put);
                         if (put)
@@ -568,7 +632,7 @@ __global__ void __launch_bounds__(F4_THREADS, 2) ea_four(Params P) {
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < KL; ++i) {
                     const bool y = (gd >> i) & 1;
                     M[j][i] = y ? Mi[i] : 0;
                     E[j][i] = y ? Ei[i] : 0;
@@ -579,7 +643,7 @@ __global__ void __launch_bounds__(F4_THREADS, 2) ea_four(Params P) {
             if (cut) {  // scales of slots past the last key (or before the first) may be anything
                 uint32_t keep = 0;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) keep |= (kn + i < k1 && (!MOD || kn + i >= kbeg)) ? 0xFFu << (8 * i) : 0u;
+                for (int i = 0; i < KL; ++i) keep |= (kn + i < k1 && (!MOD || kn + i >= kbeg)) ? 0xFFu << (8 * i) : 0u;
 #pragma unroll
                 for (int l = 0; l < NG; ++l) vr.s[l] &= keep;
             }
@@ -587,7 +651,7 @@ __global__ void __launch_bounds__(F4_THREADS, 2) ea_four(Params P) {
 #pragma unroll
             for (int j = 0; j < RL; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) move |= ((good >> (4 * j + i)) & 1) && E[j][i] > base[j] + F4_BITS;
+                for (int i = 0; i < KL; ++i) move |= ((good >> (4 * j + i)) & 1) && E[j][i] > base[j] + F4_BITS;
             uint32_t past = 0;
 #pragma unroll
             for (int l = 0; l < NG; ++l) {
@@ -607,8 +671,8 @@ __global__ void __launch_bounds__(F4_THREADS, 2) ea_four(Params P) {
                 for (int j = 0; j < RL; ++j) {
                     int m = F4_NONE;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) m = (good >> (4 * j + i)) & 1 ? max(m, E[j][i]) : m;
-                    for (int o = 1; o < 16; o <<= 1) m = max(m, __shfl_xor(m, o, 64));
+                    for (int i = 0; i < KL; ++i) m = (good >> (4 * j + i)) & 1 ? max(m, E[j][i]) : m;
+                    for (int o = 1; o < RLANES; o <<= 1) m = max(m, __shfl_xor(m, o, 64));
                     const int nb = m > base[j] + F4_BITS ? m - (F4_BITS - F4_HEAD) : base[j];
                     if (folds) {
                         rebase(j, nb);
@@ -618,30 +682,29 @@ __global__ void __launch_bounds__(F4_THREADS, 2) ea_four(Params P) {
                 }
             }
             ++since;
-            double md[RL][4];
+            double md[RL][KL];
 #pragma unroll
             for (int j = 0; j < RL; ++j) {
                 const int bs = base[j] == F4_NONE ? 0 : base[j];  // without a visible key so far every weight is 0
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < KL; ++i) {
                     md[j][i] = (double)M[j][i];
                     E[j][i] = (good >> (4 * j + i)) & 1 ? max(E[j][i] - bs, -1000) : 32;  // pairs that weigh nothing are exact
                     z[j] += ldexp(md[j][i], E[j][i]);
                 }
             }
-            // ---- P.V
-#pragma unroll
-            for (int l = 0; l < NG; ++l) {
-                if (l >= ng) break;
-                uint32_t* const W = S.W[w];  // read before it is written again: a wave's LDS accesses keep their order
+            // ---- P.V: a phase writes the digits of its groups and reads them back; the next one writes them anew (a wave's LDS
+            // accesses keep their order)
+            auto digits = [&](const int l) __attribute__((always_inline)) {
+                uint32_t* const W = S.W[w][l % Smem::PG];
                 constexpr double BIG = 0x1.8p52 + 141289400074368.0;  // and 0x808080808080
 #pragma unroll
                 for (int j = 0; j < RL; ++j) {
-                    uint32_t L[4], H[4];
-                    double xw[4], y[4];
+                    uint32_t L[KL], H[KL];
+                    double xw[KL], y[KL];
                     int least = 0;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < KL; ++i) {
                         const int sh = E[j][i] + (int)(vr.s[l] >> (8 * i) & 0xFFu) - G[l];
                         least = min(least, sh);
                         xw[i] = ldexp(md[j][i], sh);
@@ -651,26 +714,39 @@ __global__ void __launch_bounds__(F4_THREADS, 2) ea_four(Params P) {
                     }
                     if (__builtin_expect(__ballot(least < 0) != 0, 0)) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) lostw[j] += fabs(xw[i] - (y[i] - BIG));
+                        for (int i = 0; i < KL; ++i) lostw[j] += fabs(xw[i] - (y[i] - BIG));
                     }
-                    // byte p of the four sums is plane p: transpositions of 4 x 4 and 4 x 2 bytes
+                    // byte p of the sums is plane p: transpositions of 4 x 4 and 4 x 2 bytes, or 2 x 4 and 2 x 2
                     const uint32_t l01 = __builtin_amdgcn_perm(L[1], L[0], 0x05010400u), h01 = __builtin_amdgcn_perm(L[1], L[0], 0x07030602u);
-                    const uint32_t l23 = __builtin_amdgcn_perm(L[3], L[2], 0x05010400u), h23 = __builtin_amdgcn_perm(L[3], L[2], 0x07030602u);
-                    const uint32_t t01 = __builtin_amdgcn_perm(H[1], H[0], 0x05010400u), t23 = __builtin_amdgcn_perm(H[3], H[2], 0x05010400u);
-                    const uint32_t pl[6] = {__builtin_amdgcn_perm(l23, l01, 0x05040100u), __builtin_amdgcn_perm(l23, l01, 0x07060302u),
-                                            __builtin_amdgcn_perm(h23, h01, 0x05040100u), __builtin_amdgcn_perm(h23, h01, 0x07060302u),
-                                            __builtin_amdgcn_perm(t23, t01, 0x05040100u), __builtin_amdgcn_perm(t23, t01, 0x07060302u)};
-                    const int at = (RS == 4 ? g : 4 * (g & 1) + 2 * (g >> 1) + j) * F4_WROW + n;
+                    const uint32_t t01 = __builtin_amdgcn_perm(H[1], H[0], 0x05010400u);
+                    if constexpr (KL == 2) {
+                        const uint32_t pp[3] = {l01 ^ 0x80808080u, h01 ^ 0x80808080u, t01 ^ 0x80808080u};
+                        uint16_t* const at = (uint16_t*)&W[row * F4_WROW + n] + (sub >> 1);
 #pragma unroll
-                    for (int p = 0; p < 6; ++p) W[p * RS * F4_WROW + at] = pl[p] ^ 0x80808080u;
+                        for (int p = 0; p < 6; ++p) at[p * 2 * RS * F4_WROW] = (uint16_t)(pp[p >> 1] >> (16 * (p & 1)));
+                    } else {
+                        const uint32_t l23 = __builtin_amdgcn_perm(L[KL - 1], L[KL - 2], 0x05010400u);
+                        const uint32_t h23 = __builtin_amdgcn_perm(L[KL - 1], L[KL - 2], 0x07030602u);
+                        const uint32_t t23 = __builtin_amdgcn_perm(H[KL - 1], H[KL - 2], 0x05010400u);
+                        const uint32_t pl[6] = {__builtin_amdgcn_perm(l23, l01, 0x05040100u), __builtin_amdgcn_perm(l23, l01, 0x07060302u),
+                                                __builtin_amdgcn_perm(h23, h01, 0x05040100u), __builtin_amdgcn_perm(h23, h01, 0x07060302u),
+                                                __builtin_amdgcn_perm(t23, t01, 0x05040100u), __builtin_amdgcn_perm(t23, t01, 0x07060302u)};
+                        const int at = (RS == 4 ? g : 4 * (g & 1) + 2 * (g >> 1) + j) * F4_WROW + n;
+#pragma unroll
+                        for (int p = 0; p < 6; ++p) W[p * RS * F4_WROW + at] = pl[p] ^ 0x80808080u;
+                    }
                 }
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                __builtin_amdgcn_wave_barrier();
+            };
+            auto multiply = [&](const int l) __attribute__((always_inline)) {
+                const uint32_t* const W = S.W[w][l % Smem::PG];
                 f4_i4 A[NMF];
-                if constexpr (RS == 4) {
+                if constexpr (RS == 2) {
+                    const uint32_t* const a0 = n < 12 ? &W[n * F4_WROW + 4 * g] : S.zero;
+                    A[0] = __builtin_bit_cast(f4_i4, *(const f4_u4*)a0);
+                } else if constexpr (RS == 4) {
                     const uint32_t* const a0 = n < 8 ? &W[n * F4_WROW + 4 * g] : S.zero;
                     A[0] = __builtin_bit_cast(f4_i4, *(const f4_u4*)a0);
-                    A[1] = __builtin_bit_cast(f4_i4, *(const f4_u4*)&W[(8 + n) * F4_WROW + 4 * g]);
+                    A[NMF - 1] = __builtin_bit_cast(f4_i4, *(const f4_u4*)&W[(8 + n) * F4_WROW + 4 * g]);
                 } else {
 #pragma unroll
                     for (int j = 0; j < NMF; ++j) A[j] = __builtin_bit_cast(f4_i4, *(const f4_u4*)&W[(16 * j + n) * F4_WROW + 4 * g]);
@@ -686,9 +762,22 @@ __global__ void __launch_bounds__(F4_THREADS, 2) ea_four(Params P) {
                     acc[j][2 * l] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[j], B0, acc[j][2 * l], 0, 0, 0);
                     acc[j][2 * l + 1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[j], B1, acc[j][2 * l + 1], 0, 0, 0);
                 }
+            };
+#pragma unroll
+            for (int l0 = 0; l0 < NG; l0 += Smem::PG) {
+                if (l0 >= ng) break;
+#pragma unroll
+                for (int l = l0; l < l0 + Smem::PG; ++l)
+                    if (l < ng) digits(l);
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int l = l0; l < l0 + Smem::PG; ++l)
+                    if (l < ng) multiply(l);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if (more) issue_v(n0 + 256, nx, vr);
+            issue_v(n0 + 256, nx, vr);
+            nx = after;
             __builtin_amdgcn_sched_barrier(0);
         };
 
@@ -751,17 +840,17 @@ __global__ void __launch_bounds__(F4_THREADS, 2) ea_four(Params P) {
                         Ei = (int32_t)E2;
                     }
                 }
-                const uint64_t first = 0x0001000100010001ull;  // a lane of each pair
-                n5 += (int)__popcll(__ballot(why == 1) & first);
-                n6 += (int)__popcll(__ballot(why == 2) & first);
-                n8 += (int)__popcll(__ballot(fin) & first);
-                for (uint64_t m = __ballot(have && !live) & first; m; m &= m - 1) {
+                const uint64_t lead4 = 0x0001000100010001ull;  // a lane of each pair
+                n5 += (int)__popcll(__ballot(why == 1) & lead4);
+                n6 += (int)__popcll(__ballot(why == 2) & lead4);
+                n8 += (int)__popcll(__ballot(fin) & lead4);
+                for (uint64_t m = __ballot(have && !live) & lead4; m; m &= m - 1) {
                     const int r = __builtin_amdgcn_readlane(er, __builtin_ctzll(m));
 #pragma unroll
                     for (int j = 0; j < RL; ++j)
                         if (row + j == r) rfl[j] = 1;
                 }
-                for (uint64_t lv = __ballot(live) & first; lv; lv &= lv - 1) {
+                for (uint64_t lv = __ballot(live) & lead4; lv; lv &= lv - 1) {
                     const int ln = __builtin_ctzll(lv);
                     const int r = __builtin_amdgcn_readlane(er, ln), key = __builtin_amdgcn_readlane(ek, ln);
                     const int Mr = __builtin_amdgcn_readlane(Mi, ln), Er = __builtin_amdgcn_readlane(Ei, ln);
@@ -780,11 +869,15 @@ __global__ void __launch_bounds__(F4_THREADS, 2) ea_four(Params P) {
                         const int de = Er - base[j];
                         if (!MOD && de < -1000) rfl[j] = 1;
                         const double om = de < -1000 ? 0.0 : ldexp((double)Mr, de);
-                        z[j] += n == 0 ? om : 0.0;
+                        z[j] += head ? om : 0.0;
 #pragma unroll
                         for (int l = 0; l < NG; ++l) {
                             if (l >= ng) break;
                             double* const o = &O[j * 32 * NG + 32 * l];
+                            if constexpr (RS == 2) {
+                                o[0] = __fma_rn(om, sub ? bf16hi_f64(v2[l]) : bf16lo_f64(v2[l]), o[0]);
+                                continue;
+                            }
                             o[0] = __fma_rn(om, bf16lo_f64(v2[l]), o[0]);
                             o[16] = __fma_rn(om, bf16hi_f64(v2[l]), o[16]);
                         }
@@ -796,19 +889,15 @@ __global__ void __launch_bounds__(F4_THREADS, 2) ea_four(Params P) {
         };
 
         // ---- the wave's tiles: K of the next one is requested once the scores have read this one's registers, V once P.V has;
-        // pages are looked up a tile ahead. A flush (rare) drops the loads in flight and starts over
+        // pages are looked up a tile before that. A flush (rare) drops the loads in flight and starts over
         for (int it = 0; it < nst;) {
-            KR kr;
-            VR vr;
-            {
-                const Pages p0 = pages_of(k0w + 256 * it);
-                issue_k(k0w + 256 * it, p0, kr);
-                issue_v(k0w + 256 * it, p0, vr);
-            }
 #pragma unroll 1
-            for (; it < nst && cnt < F4_LIST; ++it) tile(k0w + 256 * it, it + 1 < nst, kr, vr);
+            for (; it < nst && cnt < F4_LIST; ++it) tile(k0w + 256 * it);
             if (since) fold();
-            if (cnt > 0) flush();
+            if (cnt > 0) {
+                flush();
+                if (it < nst) begin(k0w + 256 * it);
+            }
         }
 
         // ---- epilogue: row totals of the wave, then the 4 waves' partials at the rows' largest base (exact powers of two), two
@@ -818,12 +907,12 @@ __global__ void __launch_bounds__(F4_THREADS, 2) ea_four(Params P) {
             for (int j = 0; j < RL; ++j) {
                 double zs = z[j], ls = lostw[j];
                 int fl = rfl[j];
-                for (int o = 1; o < 16; o <<= 1) {
+                for (int o = 1; o < RLANES; o <<= 1) {
                     zs += __shfl_xor(zs, o, 64);
                     ls += __shfl_xor(ls, o, 64);
                     fl |= __shfl_xor(fl, o, 64);
                 }
-                if (n == 0) {
+                if (head) {
                     S.wR[w][row + j] = base[j];
                     S.wZ[w][row + j] = zs;
                     S.we[w][row + j] = ls;
@@ -934,7 +1023,7 @@ __global__ void __launch_bounds__(F4_THREADS, 2) ea_four(Params P) {
         if (MOD && blockIdx.y == gridDim.y - 1) end = 1 << 23;  // keys are below 2^29
     }
     for (bool first = true;; first = false) {
-        int t0 = start, t1 = end, slot = (int)blockIdx.y;
+        int t0 = start, te = end, slot = (int)blockIdx.y;
         if (P.dq_stream) {
             if (start >= end || u >= P.dq_units) break;
             const int su = Su[u], eu = Su[u + 1];
@@ -944,12 +1033,12 @@ __global__ void __launch_bounds__(F4_THREADS, 2) ea_four(Params P) {
             }
             slot = gb - su / share;
             t0 = start - su;
-            t1 = min(end, eu) - su;
+            te = min(end, eu) - su;
             start = min(end, eu);
             if (slot >= P.nsplit) break;  // share >= dq_min_share keeps every unit within nsplit slots
         }
         if (!first) __syncthreads();  // the previous piece's LDS reads are done
-        piece(u, slot, t0 * 64, t1 * 64);
+        piece(first, u, slot, t0 * 64, te * 64);
         if (!P.dq_stream) break;
         ++u;
     }

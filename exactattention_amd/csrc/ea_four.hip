@@ -1,36 +1,38 @@
 // The split kernel of 4-bit caches: its variants and its host side.
+#include <algorithm>
 #include <mutex>
 
 #include "ea_four.h"
 
 namespace {
 
-// MOD: Params::mods, 0 the plain kernel; 4 groups of channels a lane's loads, or 2 where V has no more
-template <int RS, int MOD>
-const void* four_fn(bool small) {
-    return small ? (const void*)ea_four<RS, 2, MOD> : (const void*)ea_four<RS, 4, MOD>;
+// MOD: Params::mods, 0 the plain kernel; NG: V's groups of 32 channels, 2 also for 1
+template <int RS, int NG>
+const void* four_fn(int mod) {
+    return mod == 3 ? (const void*)ea_four<RS, NG, 3> : (mod == 2 ? (const void*)ea_four<RS, NG, 2>
+                                                                  : (mod ? (const void*)ea_four<RS, NG, 1> : (const void*)ea_four<RS, NG, 0>));
 }
+struct Four {
+    const void* fn;
+    size_t lds;
+};
 template <int RS>
-const void* four_fn(bool small, int mod) {
-    return mod == 3 ? four_fn<RS, 3>(small) : (mod == 2 ? four_fn<RS, 2>(small) : (mod ? four_fn<RS, 1>(small) : four_fn<RS, 0>(small)));
+Four four_of(int ng, int mod) {
+    return ng == 4 ? Four{four_fn<RS, 4>(mod), sizeof(FourSmem<RS, 4>)}
+                   : (ng == 3 ? Four{four_fn<RS, 3>(mod), sizeof(FourSmem<RS, 3>)} : Four{four_fn<RS, 2>(mod), sizeof(FourSmem<RS, 2>)});
 }
-bool four_small(const Params& P) { return P.g.head_dim_v <= 64; }
-const void* four_fn_for(const Params& P) {
-    return P.rb == 4 ? four_fn<4>(four_small(P), P.mods) : four_fn<8>(four_small(P), P.mods);
-}
-size_t four_lds(const Params& P) {
-    const bool s = four_small(P);
-    return P.rb == 4 ? (s ? sizeof(FourSmem<4, 2>) : sizeof(FourSmem<4, 4>)) : (s ? sizeof(FourSmem<8, 2>) : sizeof(FourSmem<8, 4>));
-}
+Four four_of(int rs, int ng, int mod) { return rs == 2 ? four_of<2>(ng, mod) : (rs == 4 ? four_of<4>(ng, mod) : four_of<8>(ng, mod)); }
+int four_ng(const Params& P) { return std::max(2, (P.g.head_dim_v + 31) >> 5); }
+Four four_of(const Params& P) { return four_of(P.rb, four_ng(P), P.mods); }
 hipError_t four_attrs() {
     static std::once_flag once;
     static hipError_t err = hipSuccess;
     std::call_once(once, [] {
-        for (int mod = 0; mod < 4; ++mod)
-            for (int small = 0; small < 2; ++small)
-                for (const void* f : {four_fn<4>(small, mod), four_fn<8>(small, mod)}) {
-                    const hipError_t e =
-                        hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(FourSmem<8, 4>));
+        for (int rs = 2; rs <= 8; rs *= 2)
+            for (int ng = 2; ng <= 4; ++ng)
+                for (int mod = 0; mod < 4; ++mod) {
+                    const Four f = four_of(rs, ng, mod);
+                    const hipError_t e = hipFuncSetAttribute(f.fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)f.lds);
                     if (e != hipSuccess) err = e;
                 }
     });
@@ -49,18 +51,19 @@ int ea::ea_four_eligible(const Params& P) {
 int ea::ea_four_slots(const Params& P, int* slots) {
     // blocks resident on the current device at once, cached per device and kernel
     static std::mutex mu;
-    static int cache[64][16] = {};
+    static int cache[64][36] = {};
     hipError_t e = four_attrs();
     if (e != hipSuccess) return -100 - (int)e;
     int dev = 0;
     if ((e = hipGetDevice(&dev)) != hipSuccess) return -100 - (int)e;
-    const int ki = (P.rb == 4 ? 0 : 1) + (four_small(P) ? 2 : 0) + 4 * P.mods;
+    const Four f = four_of(P);
+    const int ki = (P.rb == 2 ? 0 : (P.rb == 4 ? 1 : 2)) + 3 * (four_ng(P) - 2) + 9 * P.mods;
     std::lock_guard<std::mutex> lk(mu);
     if (dev < 0 || dev >= 64) return -1;
     if (!cache[dev][ki]) {
         int cus = 0, per = 0;
         if ((e = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev)) != hipSuccess) return -100 - (int)e;
-        if ((e = hipOccupancyMaxActiveBlocksPerMultiprocessor(&per, four_fn_for(P), F4_THREADS, four_lds(P))) != hipSuccess)
+        if ((e = hipOccupancyMaxActiveBlocksPerMultiprocessor(&per, f.fn, F4_THREADS, f.lds)) != hipSuccess)
             return -100 - (int)e;
         cache[dev][ki] = (cus > 0 ? cus : 1) * (per > 0 ? per : 1);
     }
@@ -71,9 +74,10 @@ int ea::ea_four_slots(const Params& P, int* slots) {
 int ea::ea_launch_four(const Params& P, hipStream_t st) {
     hipError_t e = four_attrs();
     if (e != hipSuccess) return -100 - (int)e;
+    const Four f = four_of(P);
     Params Pc = P;
     void* args[] = {&Pc};
     const dim3 grid = P.dq_stream ? dim3((unsigned)P.dq_blocks) : dim3((unsigned)(P.nseg * P.nrb), (unsigned)P.nsplit);
-    e = hipLaunchKernel(four_fn_for(P), grid, dim3(F4_THREADS), args, four_lds(P), st);
+    e = hipLaunchKernel(f.fn, grid, dim3(F4_THREADS), args, f.lds, st);
     return e == hipSuccess ? 0 : -100 - (int)e;
 }
