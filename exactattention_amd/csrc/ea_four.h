@@ -19,18 +19,19 @@
 //            whole numbers (-12 .. 12, byte lookups). int32 sums are exact; a base that must move folds them into fp64.
 //            The rounding of W is the one error: half a unit of 2^(base + G) a key.
 //
-// What bounds it is the VALU, with 2 waves a SIMD (the int32 sums alone are 64 registers of 4 rows, 96 of 8): of a tile of 64 keys and 4
-// rows 48 instructions for the scores, 200 for the certified weights, 88 a group of 32 channels, half of them for V's bytes. A step of 32
-// ragged sequences to 4096 keys, 32/8 heads: 65 us, 69 on the fp64 matrix instructions; 8 of 30000 to 131072, 16/8 heads: 249, 437.
+// What bounds it is the VALU, and HBM where a block has 2 rows: of a tile of 64 keys and 4 rows 55 instructions for the scores, 135 for the
+// weights, 37 a group of 32 channels for their digits and 44 for V's bytes; 2 waves a SIMD (the int32 sums alone are 64 registers; 8 rows
+// took 96, spilled, and then waited for every load: a 1500-token chunk 770 us, 680 with 4). A step of 32 ragged sequences to 4096 keys,
+// 32/8 heads: 66 us, 69 on the fp64 matrix instructions; 8 of 30000 to 131072, 16/8 heads: 182 (4.5 TB/s), 437.
 //
-// Layout. A block is 4 waves over one (segment, block of RS = 4 or 8 rows, key range); wave w takes 64-key tiles w, w + 4, .. and
-// meets the others in the epilogue only. Lane l: g = l / 16, n = l % 16; its pairs are those of its rows, RS / 4 from (RS / 4) g, with
-// the keys 4 n + u (u = 0..3) of the tile.
+// Layout. A block is 4 waves over one (segment, block of RS = 2 or 4 rows, key range); wave w takes 64-key tiles w, w + 4, .. and
+// meets the others in the epilogue only. Lane l: g = l / 16, n = l % 16; its pairs are those of its row, with the keys 4 n + u (u =
+// 0..3) of the tile: row g, or of 2 rows row g / 2 and half of the keys.
 //   q     digits in registers, the A operand (M = a row's digit, K = dim): with M = 4 g + i in the order of the rows, the 4 sums of
-//         D that a lane gets are digits of its own rows: 2 instructions a key of 4 rows, 3 of 8, and nothing passes between lanes
+//         D that a lane gets are digits of its own row: 2 instructions a key of 4 rows, and nothing passes between lanes; 1 of 2
+//         rows, whose lanes swap halves
 //   K     lane loads dims 32 g .. + 31 of the keys 4 n + u (16 bytes and a scale each): the B operand (K = dim, N = key)
-//   W     digits to LDS, [plane][row][64 keys]; A operand (M = plane and row, K = key): 4 rows: planes 0, 1 and 2..5; 8 rows:
-//         planes 0, 1 and 2, 3 and 4, 5, the rows in an order that leaves a lane the sums of its own rows
+//   W     digits to LDS, [plane][row][64 keys]; A operand (M = plane and row, K = key): 4 rows: planes 0, 1 and 2..5
 //   V     l = 0..3: lane loads channels 32 l + 2 n and + 1 of keys 16 g .. + 15 (16 bytes): two B operands (K = key, N = channel)
 //   O     fp64 sums, in LDS: they change only where int32 sums are folded into them
 #pragma once
@@ -69,7 +70,7 @@ struct FourSmem {
     uint32_t q6[2][RS * 6 * 24];  // q's digits [row][digit][32-dim block][6 dwords], and those of what they leave
     uint32_t zero[8];
     double T1[256], T2[256];  // exp2 tables, T1 times 2^23
-    double rq[RS], rqe[RS];   // 2^(lsb + 3); |alpha| times the sum of |q| that both rounds lost
+    double rq[RS], rqe[RS];   // alpha 2^(lsb + 3); |alpha| times the sum of |q| that both rounds lost
     int bad[RS], more[RS], kvl[RS];
     uint64_t tmk[RS];
     int kvb[RS], pos[RS];  // with score modifications
@@ -79,9 +80,8 @@ struct FourSmem {
     uint32_t wv[4][4];  // per wave and group: the largest scale
     uint32_t list[4][F4_LIST + 64 * RS];
     double O[4][RS][32 * NG];  // per wave: of channel 32 l + 2 n + h at 32 l + 16 h + n
-    static constexpr int PG = RS == 8 ? 1 : NG;  // groups of channels whose digits lie here together
     union alignas(16) {
-        uint32_t W[4][PG][6 * RS * F4_WROW];
+        uint32_t W[4][NG][6 * RS * F4_WROW];
         uint8_t dig[2][RS * 6 * 128];
     };
 };
@@ -112,15 +112,44 @@ __device__ __forceinline__ uint32_t four_bytes(uint32_t w) {
     return __builtin_amdgcn_perm(P1, P0, x) ^ __builtin_amdgcn_perm(N1, N0, y);
 }
 
+// Certified weights of exact sums: w = RN24(2^t), t = RN32(x), x within p 2^-49 + adel of p = a xs: t is decided when both ends of
+// that interval round to it. |t| <= 2^-25 gives 1. 2^t from the tables and the cubic of pf::cert_pairs, with its bound: t is cut at
+// multiples of 2^-16 by an addition (of t - 2^-17, which is exact; a multiple may go down, and leaves r = 2^-16). w = Y 2^(fl - 23), Y in
+// 2^23 .. 2^24; not ok: left to the exact path.
+template <int NP>
+__device__ __forceinline__ void four_weights(const double (&xs)[NP], double a, double adel, const double* T1s, const double* T2, double (&Y)[NP],
+                                             int (&fl)[NP], bool (&ok)[NP]) {
+    const double c1 = u64_as_f64(EA_C_BITS[0]), c2 = u64_as_f64(EA_C_BITS[1]), c3 = u64_as_f64(EA_C_BITS[2]);
+    constexpr double CUT = 0x1.8p36;
+    double r[NP], aa[NP];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        const double p = a * xs[i], e = __fma_rn(fabs(p), 0x1p-49, adel);
+        const float lo = (float)(p - e), hi = (float)(p + e);
+        ok[i] = (lo == hi) & (fabsf(hi) < 0x1p29f);
+        const double t = (double)(fabsf(hi) <= 0x1p-25f ? 0.0f : hi);
+        const double X = (t - 0x1p-17) + CUT;
+        r[i] = t - (X - CUT);
+        const uint32_t k = (uint32_t)__double2loint(X);  // t in units of 2^-16, its low half the fraction
+        fl[i] = (int)__builtin_amdgcn_alignbit((uint32_t)__double2hiint(X), k, 16);
+        aa[i] = T1s[(k >> 8) & 255u] * T2[k & 255u];
+    }
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        const double y = __fma_rn(aa[i], r[i] * __fma_rn(r[i], __fma_rn(r[i], c3, c2), c1), aa[i]);
+        Y[i] = (y + 0x1.8p52) - 0x1.8p52;
+        ok[i] = ok[i] & (fabs(y - Y[i]) <= 0.5 - 0x1p-26);
+    }
+}
+
 }  // namespace
 
 // MOD: with score modifications (ea_mod.h): 1 key ranges alone, 2 with a bias, 3 with a cap; a unit's key range is then counted from its
 // rows' first visible key, down to a whole tile, and on uniform splits the last split takes every key past the others.
 template <int RS, int NG, int MOD>
 __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Params P) {
-    constexpr int RL = RS == 8 ? 2 : 1;                  // rows of a lane
-    constexpr int KL = RS == 2 ? 2 : 4;                  // keys of a lane
-    constexpr int NMF = RS == 2 ? 1 : (RS == 4 ? 2 : 3);  // matrix instructions for 6 digits of the rows
+    constexpr int KL = RS;               // keys of a lane
+    constexpr int NMF = RS == 2 ? 1 : 2;  // matrix instructions for 6 digits of the rows
     typedef FourSmem<RS, NG> Smem;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     Smem& S = *reinterpret_cast<Smem*>(smem_raw);
@@ -202,7 +231,7 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
         const int k1 = min(kB, kend);
         const int k0w = kA + 64 * w;  // this wave's tiles: k0w + 256 it
         const int nst = k1 > k0w ? (k1 - k0w + 255) >> 8 : 0;
-        const int row = RS == 2 ? g >> 1 : RL * g;  // the lane's rows: row + j
+        const int row = RS == 2 ? g >> 1 : g;       // the lane's row
         const int sub = RS == 2 ? 2 * (g & 1) : 0;  // its keys of a tile: 4 n + sub + i
         constexpr int RLANES = RS == 2 ? 32 : 16;   // lanes of a row
         const bool head = n == 0 && sub == 0;       // the first of them
@@ -344,7 +373,7 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
             if (lane == 0) {
                 S.bad[r] = bad;
                 S.more[r] = more;
-                S.rq[r] = ldexp(1.0, lsb + 3);
+                S.rq[r] = ldexp(P.alpha, lsb + 3);
                 S.rqe[r] = fabs(P.alpha) * (double)lost * ldexp(0.5 * (1.0 + 0x1p-20), lsb - 28);
             }
         }
@@ -370,29 +399,19 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
         __syncthreads();
         // the lane's part of a row block's digits, instruction j: M = n is digit 4 j + n % 4 of the digits of the rows of n / 4
         auto q_part = [&](int k2, int j) __attribute__((always_inline)) {
-            int c = RS == 2 ? n & 7 : 4 * j + (n & 3);
-            asm volatile("" : "+v"(c));  // read where it is used
-            const int qr = RS == 2 ? n >> 3 : RL * (n >> 2) + (c >= 6 ? 1 : 0), qk = c >= 6 ? c - 6 : c;
-            const uint32_t* const p = RS != 8 && c >= 6 ? S.zero : &S.q6[k2][((qr * 6 + qk) * 4 + g) * 6];
+            const int c = RS == 2 ? n & 7 : 4 * j + (n & 3);
+            const int qr = RS == 2 ? n >> 3 : n >> 2;
+            const uint32_t* const p = c >= 6 ? S.zero : &S.q6[k2][((qr * 6 + c) * 4 + g) * 6];
             const f4_u2 x = *(const f4_u2*)p, y = *(const f4_u2*)(p + 2), t = *(const f4_u2*)(p + 4);
             return (f4_i8){(int)x.x, (int)x.y, (int)y.x, (int)y.y, (int)t.x, (int)t.y, 0, 0};
         };
-        // 8 rows leave no registers for what the tile needs once: q's digits are read again for every tile
-        constexpr bool AGAIN = RS == 8;
         f4_i8 qd[NMF];
 #pragma unroll
-        for (int j = 0; j < NMF; ++j)
-            if (!AGAIN) qd[j] = q_part(0, j);
+        for (int j = 0; j < NMF; ++j) qd[j] = q_part(0, j);
         const double alpha = P.alpha;
-        int rfl[RL];   // the row is left to tier 2
-        int base[RL];  // of the row
-        double z[RL], lostw[RL];  // the weights' sum, and what rounding took from their whole numbers
-#pragma unroll
-        for (int j = 0; j < RL; ++j) {
-            rfl[j] = S.bad[row + j];
-            base[j] = F4_NONE;
-            z[j] = lostw[j] = 0.0;
-        }
+        int rfl = S.bad[row];  // the row is left to tier 2
+        int base = F4_NONE;    // of the row
+        double z = 0.0, lostw = 0.0;  // the weights' sum, and what rounding took from their whole numbers
         int G[NG];             // the groups' references, uniform
         f4_h2 vm[NG];          // the largest scales the lane saw, of even and odd keys
 #pragma unroll
@@ -400,23 +419,21 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
             G[l] = 0;
             vm[l] = (f4_h2){0, 0};
         }
-        int lo = -100000;      // scales of keys in [lo, lo + F4_SPREAD] need no closer look
-        double kbnd = 0.0;     // an upper bound of |k| for such keys
+        int lo = 120;          // scales of keys in [lo, lo + F4_SPREAD] need no closer look: at first 2^-7 .. 2^2
+        double kbnd = 6.0 * 0x1p2;  // an upper bound of |k| for such keys
         f4_i4 acc[NMF][2 * NG];
-        // the lane's own sums: [j][c], or with 2 rows those of c = 2 l + g % 2
+        // the lane's own sums: [c], or with 2 rows those of c = 2 l + g % 2
         constexpr int OC = RS == 2 ? NG : 2 * NG, OS = RS == 2 ? 32 : 16;
         double* const O = &S.O[w][row][8 * sub + n];
 #pragma unroll
         for (int c = 0; c < 2 * NG; ++c) {
 #pragma unroll
             for (int j = 0; j < NMF; ++j) acc[j][c] = (f4_i4){0, 0, 0, 0};
-#pragma unroll
-            for (int j = 0; j < RL; ++j)
-                if (c < OC) O[j * 32 * NG + OS * c] = 0.0;
+            if (c < OC) O[OS * c] = 0.0;
         }
         int since = 0, folds = 0;
         int n5 = 0, n6 = 0, n8 = 0, cnt = 0;  // wave-uniform
-        const double gw = RS == 2 ? (g == 0 ? 1.0 : (g == 1 ? 0x1p16 : 0x1p32)) : RS == 4 ? (g == 0 ? 1.0 : (g == 1 ? 0x1p8 : (g == 2 ? 0x1p16 : 0x1p24))) : (g < 2 ? 1.0 : 0x1p8);
+        const double gw = RS == 2 ? (g == 0 ? 1.0 : (g == 1 ? 0x1p16 : 0x1p32)) : (g == 0 ? 1.0 : (g == 1 ? 0x1p8 : (g == 2 ? 0x1p16 : 0x1p24)));
 
         // the int32 sums into the fp64 ones: digits joined, the lanes' parts added up, each lane left with its own rows
         auto fold = [&]() __attribute__((always_inline)) {
@@ -450,13 +467,8 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
                     double a = up ? t[2] : t[0], e = up ? t[3] : t[1];
                     a += xor32(up ? t[0] : t[2]);
                     e += xor32(up ? t[1] : t[3]);
-                    if constexpr (RS != 8) {
-                        const bool odd = g & 1;
-                        O[16 * c] += (odd ? e : a) + xor16(odd ? a : e);
-                    } else {
-                        O[16 * c] += a;
-                        O[32 * NG + 16 * c] += e;
-                    }
+                    const bool odd = g & 1;
+                    O[16 * c] += (odd ? e : a) + xor16(odd ? a : e);
 #pragma unroll
                     for (int j = 0; j < NMF; ++j) acc[j][c] = (f4_i4){0, 0, 0, 0};
                 }
@@ -465,19 +477,19 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
             since = 0;
         };
         // a row's base to nb (the same in every lane of the row), after a fold
-        auto rebase = [&](int j, int nb) __attribute__((always_inline)) {
+        auto rebase = [&](int nb) __attribute__((always_inline)) {
             double f = 1.0;
-            if (nb != base[j]) {
-                if (base[j] != F4_NONE) {
-                    if (!MOD && base[j] - nb < -900) rfl[j] = 1;
-                    f = ldexp(1.0, max(base[j] - nb, -1000));
-                    z[j] *= f;
-                    lostw[j] *= f;
+            if (nb != base) {
+                if (base != F4_NONE) {
+                    if (!MOD && base - nb < -900) rfl = 1;
+                    f = ldexp(1.0, max(base - nb, -1000));
+                    z *= f;
+                    lostw *= f;
                 }
-                base[j] = nb;
+                base = nb;
             }
 #pragma unroll
-            for (int c = 0; c < OC; ++c) O[j * 32 * NG + OS * c] *= f;
+            for (int c = 0; c < OC; ++c) O[OS * c] *= f;
         };
 
         auto tile = [&](int n0) __attribute__((always_inline)) {
@@ -518,8 +530,8 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
             const int kn = n0 + 4 * n + sub;  // the first of the lane's keys
             if constexpr (KL == 2) wide >>= sub;
             // ---- scores: 6 exact sums for every pair
-            double sc[RL][4];
-            auto products = [&](const f4_i8 (&qa)[NMF], double (&x)[RL][4]) __attribute__((always_inline)) {
+            double sc[4];
+            auto products = [&](const f4_i8 (&qa)[NMF], double (&x)[4]) __attribute__((always_inline)) {
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     const f4_i8 B = {(int)kr.k[u].x, (int)kr.k[u].y, (int)kr.k[u].z, (int)kr.k[u].w, 0, 0, 0, 0};
@@ -528,116 +540,105 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
                     for (int j = 0; j < NMF; ++j)
                         D[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(qa[j], B, (f4_f4){0.0f, 0.0f, 0.0f, 0.0f}, 2, 4, 0, 127, 0,
                                                                                 (int)kr.s[u]);
-                    if constexpr (RS == 2) {
-                        x[0][u] = (double)D[0][3];
+                    constexpr int LAST = RS == 2 ? 3 : 5;
+                    x[u] = (double)D[LAST >> 2][LAST & 3];
 #pragma unroll
-                        for (int k = 2; k >= 0; --k) x[0][u] = __fma_rn(x[0][u], 32.0, (double)D[0][k]);
-                        x[0][u] *= sub ? 0x1p20 : 1.0;
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < RL; ++j) {
-                            x[j][u] = (double)D[(6 * j + 5) >> 2][(6 * j + 5) & 3];
-#pragma unroll
-                            for (int k = 4; k >= 0; --k) x[j][u] = __fma_rn(x[j][u], 32.0, (double)D[(6 * j + k) >> 2][(6 * j + k) & 3]);
-                        }
-                    }
+                    for (int k = LAST - 1; k >= 0; --k) x[u] = __fma_rn(x[u], 32.0, (double)D[k >> 2][k & 3]);
+                    if constexpr (RS == 2) x[u] *= sub ? 0x1p20 : 1.0;
                 }
                 if constexpr (RS == 2) {
                     // digits 0..3 of a row's sums lie 16 lanes before digits 4 and 5: the first lane takes keys 0 and 1, the other 2 and 3
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        const auto lo = __builtin_amdgcn_permlane16_swap(__double2loint(x[0][u]), __double2loint(x[0][u + 2]), false, false);
-                        const auto hi = __builtin_amdgcn_permlane16_swap(__double2hiint(x[0][u]), __double2hiint(x[0][u + 2]), false, false);
-                        x[0][u] = __hiloint2double((int)hi[0], (int)lo[0]) + __hiloint2double((int)hi[1], (int)lo[1]);
+                        const auto lo = __builtin_amdgcn_permlane16_swap(__double2loint(x[u]), __double2loint(x[u + 2]), false, false);
+                        const auto hi = __builtin_amdgcn_permlane16_swap(__double2hiint(x[u]), __double2hiint(x[u + 2]), false, false);
+                        x[u] = __hiloint2double((int)hi[0], (int)lo[0]) + __hiloint2double((int)hi[1], (int)lo[1]);
                     }
                 }
             };
-            if constexpr (AGAIN) {
-                f4_i8 qt[NMF];
-#pragma unroll
-                for (int j = 0; j < NMF; ++j) qt[j] = q_part(0, j);
-                products(qt, sc);
-            } else {
-                products(qd, sc);
-            }
+            products(qd, sc);
             if (__builtin_expect(two, 0)) {
                 f4_i8 q2[NMF];
-                double s2[RL][4];
+                double s2[4];
 #pragma unroll
                 for (int j = 0; j < NMF; ++j) q2[j] = q_part(1, j);
                 products(q2, s2);
 #pragma unroll
-                for (int j = 0; j < RL; ++j)
-#pragma unroll
-                    for (int i = 0; i < KL; ++i) sc[j][i] = __fma_rn(s2[j][i], 0x1p-28, sc[j][i]);  // one rounding, in ad below
+                for (int i = 0; i < KL; ++i) sc[i] = __fma_rn(s2[i], 0x1p-28, sc[i]);  // one rounding, in the weights' bound
             }
             issue_k(n0 + 256, nx, kr);
-            int M[RL][KL], E[RL][KL];
-            uint32_t good = 0;  // bit 4 j + i
+            double md[KL];  // the weights: md 2^(base + ex)
+            int ex[KL];
+            constexpr uint32_t ALL = (1u << KL) - 1u;
+            // ---- certified weights
+            const double adel = S.rqe[row] * kbnd, rq = S.rq[row];
+            bool ok[KL];
+            double x[KL];
 #pragma unroll
-            for (int j = 0; j < RL; ++j) {
-                // ---- which of the pairs are visible
-                uint32_t vis = row + j < nrow ? (1u << KL) - 1u : 0u;
-                if (edge) {
-                    vis = 0;
-#pragma unroll
-                    for (int i = 0; i < KL; ++i) {
-                        const int key = kn + i, ti = key - tb;
-                        const bool in = ((unsigned)ti < 64u) & (((S.tmk[row + j] >> (ti & 63)) & 1ull) != 0);
-                        bool pre = key < S.kvl[row + j];
-                        if constexpr (MOD) pre = pre & (key >= S.kvb[row + j]);
-                        vis |= ((key < k1) & (pre | in)) ? (1u << i) : 0u;
-                    }
-                }
-                // ---- certified weights
-                int jr = row + j;
-                if constexpr (AGAIN) asm volatile("" : "+v"(jr));
-                const double adel = S.rqe[jr] * kbnd, rq = S.rq[jr];
-                double s[KL], ad[KL];
+            for (int i = 0; i < KL; ++i) x[i] = sc[i];
+            if constexpr (MOD >= 2) {
+                float sl[KL];
+                int dist[KL], Mi[KL];
+                double ad[KL];
 #pragma unroll
                 for (int i = 0; i < KL; ++i) {
-                    s[i] = sc[j][i] * rq;
-                    ad[i] = two ? __fma_rn(fabs(s[i] * alpha), 0x1p-52, adel) : adel;
+                    sl[i] = S.slope[row];
+                    dist[i] = kn + i - S.pos[row];
+                    ad[i] = __fma_rn(fabs(x[i] * rq), 0x1p-52, adel);
                 }
-                int Mi[KL], Ei[KL];
-                bool ok[KL];
-                if constexpr (MOD >= 2) {
-                    float sl[KL];
-                    int dist[KL];
+                pf::cert_pairs<KL, MOD>(x, ad, rq, S.T1, S.T2, Mi, ex, ok, P.cap, sl, dist);
 #pragma unroll
-                    for (int i = 0; i < KL; ++i) {
-                        sl[i] = S.slope[row + j];
-                        dist[i] = kn + i - S.pos[row + j];
-                    }
-                    pf::cert_pairs<KL, MOD>(s, ad, alpha, S.T1, S.T2, Mi, Ei, ok, P.cap, sl, dist);
-                } else {
-                    pf::cert_pairs<KL>(s, ad, alpha, S.T1, S.T2, Mi, Ei, ok);
+                for (int i = 0; i < KL; ++i) {
+                    md[i] = (double)Mi[i];
+                    ok[i] &= ex[i] < (1 << 29) && ex[i] > -(1 << 29) - 23;  // differences from a base fit an int
+                    ex[i] -= base;
                 }
+            } else {
+                four_weights<KL>(x, rq, adel, S.T1, S.T2, md, ex, ok);
+#pragma unroll
+                for (int i = 0; i < KL; ++i) ex[i] -= base + 23;
+            }
+            // ---- which of the pairs are visible (rows past the last one weigh what they like)
+            uint32_t vis = ALL;
+            if (edge) {
+                vis = 0;
+#pragma unroll
+                for (int i = 0; i < KL; ++i) {
+                    const int key = kn + i, ti = key - tb;
+                    const bool in = ((unsigned)ti < 64u) & (((S.tmk[row] >> (ti & 63)) & 1ull) != 0);
+                    bool pre = key < S.kvl[row];
+                    if constexpr (MOD) pre = pre & (key >= S.kvb[row]);
+                    vis |= ((key < k1) & (pre | in)) ? (1u << i) : 0u;
+                }
+            }
+            bool all = (vis == ALL) & (wide == 0);
+#pragma unroll
+            for (int i = 0; i < KL; ++i) all = all & ok[i];
+            if (__ballot(!all) != 0) {
                 uint32_t gd = 0;
 #pragma unroll
                 for (int i = 0; i < KL; ++i) gd |= ok[i] ? (1u << i) : 0u;
                 gd &= ~wide;
-                const uint32_t slow = vis & ~gd;
+                const uint32_t slow = row < nrow ? vis & ~gd : 0u;
                 gd &= vis;
                 if (__builtin_expect(__ballot(slow != 0) != 0, 0)) {
                     // undecided pairs wait in the wave's list for flush(); a row that is flagged already needs no more of them
 #pragma unroll
                     for (int i = 0; i < KL; ++i) {
-                        const bool put = ((slow >> i) & 1) && !rfl[j];
+                        const bool put = ((slow >> i) & 1) && !rfl;
                         const uint64_t m = __ballot(put);
                         if (put)
                             S.list[w][cnt + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0))] =
-                                (uint32_t)(row + j) << 29 | (uint32_t)(kn + i - kA);
+                                (uint32_t)(row) << 29 | (uint32_t)(kn + i - kA);
                         cnt += (int)__popcll(m);
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < KL; ++i) {
+                for (int i = 0; i < KL; ++i) {  // the others weigh nothing
                     const bool y = (gd >> i) & 1;
-                    M[j][i] = y ? Mi[i] : 0;
-                    E[j][i] = y ? Ei[i] : 0;
+                    md[i] = y ? md[i] : 0.0;
+                    ex[i] = y ? ex[i] : F4_BITS;
                 }
-                good |= gd << (4 * j);
             }
             // ---- bases and references move when a weight or a scale passes them
             if (cut) {  // scales of slots past the last key (or before the first) may be anything
@@ -647,11 +648,9 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
 #pragma unroll
                 for (int l = 0; l < NG; ++l) vr.s[l] &= keep;
             }
-            bool move = false;
+            int most = ex[0];
 #pragma unroll
-            for (int j = 0; j < RL; ++j)
-#pragma unroll
-                for (int i = 0; i < KL; ++i) move |= ((good >> (4 * j + i)) & 1) && E[j][i] > base[j] + F4_BITS;
+            for (int i = 1; i < KL; ++i) most = max(most, ex[i]);
             uint32_t past = 0;
 #pragma unroll
             for (int l = 0; l < NG; ++l) {
@@ -660,96 +659,81 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
                 const f4_h2 ref = __builtin_bit_cast(f4_h2, (uint32_t)G[l] * 0x10001u);
                 past |= __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(vm[l], ref));
             }
-            if (__ballot(move || past != 0) != 0 || since >= F4_EPOCH) {
+            if (__ballot(most > F4_BITS || past != 0) != 0 || since >= F4_EPOCH) {
                 if (since) fold();
 #pragma unroll
                 for (int l = 0; l < NG; ++l) {
                     const int top = wave_max_dpp((int)max(vm[l].x, vm[l].y));
-                    G[l] = max(G[l], top >= G[l] ? top + 1 : 0);  // one binade of room
+                    G[l] = max(G[l], top >= G[l] ? min(top + 1, 255) : 0);  // one binade of room
                 }
+                int m = 0;
 #pragma unroll
-                for (int j = 0; j < RL; ++j) {
-                    int m = F4_NONE;
+                for (int i = 0; i < KL; ++i) m = max(m, ex[i]);  // pairs that weigh nothing have F4_BITS
+                for (int o = 1; o < RLANES; o <<= 1) m = max(m, __shfl_xor(m, o, 64));
+                const int up = m > F4_BITS ? m - (F4_BITS - F4_HEAD) : 0;
 #pragma unroll
-                    for (int i = 0; i < KL; ++i) m = (good >> (4 * j + i)) & 1 ? max(m, E[j][i]) : m;
-                    for (int o = 1; o < RLANES; o <<= 1) m = max(m, __shfl_xor(m, o, 64));
-                    const int nb = m > base[j] + F4_BITS ? m - (F4_BITS - F4_HEAD) : base[j];
-                    if (folds) {
-                        rebase(j, nb);
-                    } else {
-                        base[j] = nb;  // nothing summed yet
-                    }
+                for (int i = 0; i < KL; ++i) ex[i] = md[i] != 0.0 ? ex[i] - up : F4_BITS;
+                if (folds) {
+                    rebase(base + up);
+                } else {
+                    base += up;  // nothing summed yet
                 }
             }
             ++since;
-            double md[RL][KL];
 #pragma unroll
-            for (int j = 0; j < RL; ++j) {
-                const int bs = base[j] == F4_NONE ? 0 : base[j];  // without a visible key so far every weight is 0
-#pragma unroll
-                for (int i = 0; i < KL; ++i) {
-                    md[j][i] = (double)M[j][i];
-                    E[j][i] = (good >> (4 * j + i)) & 1 ? max(E[j][i] - bs, -1000) : 32;  // pairs that weigh nothing are exact
-                    z[j] += ldexp(md[j][i], E[j][i]);
-                }
-            }
+            for (int i = 0; i < KL; ++i) z += ldexp(md[i], ex[i]);
             // ---- P.V: a phase writes the digits of its groups and reads them back; the next one writes them anew (a wave's LDS
             // accesses keep their order)
             auto digits = [&](const int l) __attribute__((always_inline)) {
-                uint32_t* const W = S.W[w][l % Smem::PG];
+                uint32_t* const W = S.W[w][l];
                 constexpr double BIG = 0x1.8p52 + 141289400074368.0;  // and 0x808080808080
+                const uint32_t below = (uint32_t)G[l] * (KL == 4 ? 0x01010101u : 0x0101u) - vr.s[l];  // bytes, none of them negative
+                uint32_t L[KL], H[KL];
+                double xw[KL], y[KL];
+                int least = 0;
 #pragma unroll
-                for (int j = 0; j < RL; ++j) {
-                    uint32_t L[KL], H[KL];
-                    double xw[KL], y[KL];
-                    int least = 0;
+                for (int i = 0; i < KL; ++i) {
+                    const int sh = ex[i] - (int)(below >> (8 * i) & 0xFFu);
+                    least = min(least, sh);
+                    xw[i] = ldexp(md[i], sh);
+                    y[i] = xw[i] + BIG;
+                    L[i] = (uint32_t)__double2loint(y[i]);
+                    H[i] = (uint32_t)__double2hiint(y[i]);
+                }
+                if (__builtin_expect(__ballot(least < 0) != 0, 0)) {
 #pragma unroll
-                    for (int i = 0; i < KL; ++i) {
-                        const int sh = E[j][i] + (int)(vr.s[l] >> (8 * i) & 0xFFu) - G[l];
-                        least = min(least, sh);
-                        xw[i] = ldexp(md[j][i], sh);
-                        y[i] = xw[i] + BIG;
-                        L[i] = (uint32_t)__double2loint(y[i]);
-                        H[i] = (uint32_t)__double2hiint(y[i]);
-                    }
-                    if (__builtin_expect(__ballot(least < 0) != 0, 0)) {
+                    for (int i = 0; i < KL; ++i) lostw += fabs(xw[i] - (y[i] - BIG));
+                }
+                // byte p of the sums is plane p: transpositions of 4 x 4 and 4 x 2 bytes, or 2 x 4 and 2 x 2
+                const uint32_t l01 = __builtin_amdgcn_perm(L[1], L[0], 0x05010400u), h01 = __builtin_amdgcn_perm(L[1], L[0], 0x07030602u);
+                const uint32_t t01 = __builtin_amdgcn_perm(H[1], H[0], 0x05010400u);
+                if constexpr (KL == 2) {
+                    const uint32_t pp[3] = {l01 ^ 0x80808080u, h01 ^ 0x80808080u, t01 ^ 0x80808080u};
+                    uint16_t* const at = (uint16_t*)&W[row * F4_WROW + n] + (sub >> 1);
 #pragma unroll
-                        for (int i = 0; i < KL; ++i) lostw[j] += fabs(xw[i] - (y[i] - BIG));
-                    }
-                    // byte p of the sums is plane p: transpositions of 4 x 4 and 4 x 2 bytes, or 2 x 4 and 2 x 2
-                    const uint32_t l01 = __builtin_amdgcn_perm(L[1], L[0], 0x05010400u), h01 = __builtin_amdgcn_perm(L[1], L[0], 0x07030602u);
-                    const uint32_t t01 = __builtin_amdgcn_perm(H[1], H[0], 0x05010400u);
-                    if constexpr (KL == 2) {
-                        const uint32_t pp[3] = {l01 ^ 0x80808080u, h01 ^ 0x80808080u, t01 ^ 0x80808080u};
-                        uint16_t* const at = (uint16_t*)&W[row * F4_WROW + n] + (sub >> 1);
+                    for (int p = 0; p < 6; ++p) at[p * 2 * RS * F4_WROW] = (uint16_t)(pp[p >> 1] >> (16 * (p & 1)));
+                } else {
+                    const uint32_t l23 = __builtin_amdgcn_perm(L[KL - 1], L[KL - 2], 0x05010400u);
+                    const uint32_t h23 = __builtin_amdgcn_perm(L[KL - 1], L[KL - 2], 0x07030602u);
+                    const uint32_t t23 = __builtin_amdgcn_perm(H[KL - 1], H[KL - 2], 0x05010400u);
+                    const uint32_t pl[6] = {__builtin_amdgcn_perm(l23, l01, 0x05040100u), __builtin_amdgcn_perm(l23, l01, 0x07060302u),
+                                            __builtin_amdgcn_perm(h23, h01, 0x05040100u), __builtin_amdgcn_perm(h23, h01, 0x07060302u),
+                                            __builtin_amdgcn_perm(t23, t01, 0x05040100u), __builtin_amdgcn_perm(t23, t01, 0x07060302u)};
+                    const int at = row * F4_WROW + n;
 #pragma unroll
-                        for (int p = 0; p < 6; ++p) at[p * 2 * RS * F4_WROW] = (uint16_t)(pp[p >> 1] >> (16 * (p & 1)));
-                    } else {
-                        const uint32_t l23 = __builtin_amdgcn_perm(L[KL - 1], L[KL - 2], 0x05010400u);
-                        const uint32_t h23 = __builtin_amdgcn_perm(L[KL - 1], L[KL - 2], 0x07030602u);
-                        const uint32_t t23 = __builtin_amdgcn_perm(H[KL - 1], H[KL - 2], 0x05010400u);
-                        const uint32_t pl[6] = {__builtin_amdgcn_perm(l23, l01, 0x05040100u), __builtin_amdgcn_perm(l23, l01, 0x07060302u),
-                                                __builtin_amdgcn_perm(h23, h01, 0x05040100u), __builtin_amdgcn_perm(h23, h01, 0x07060302u),
-                                                __builtin_amdgcn_perm(t23, t01, 0x05040100u), __builtin_amdgcn_perm(t23, t01, 0x07060302u)};
-                        const int at = (RS == 4 ? g : 4 * (g & 1) + 2 * (g >> 1) + j) * F4_WROW + n;
-#pragma unroll
-                        for (int p = 0; p < 6; ++p) W[p * RS * F4_WROW + at] = pl[p] ^ 0x80808080u;
-                    }
+                    for (int p = 0; p < 6; ++p) W[p * RS * F4_WROW + at] = pl[p] ^ 0x80808080u;
                 }
             };
             auto multiply = [&](const int l) __attribute__((always_inline)) {
-                const uint32_t* const W = S.W[w][l % Smem::PG];
+                const uint32_t* const W = S.W[w][l];
                 f4_i4 A[NMF];
                 if constexpr (RS == 2) {
                     const uint32_t* const a0 = n < 12 ? &W[n * F4_WROW + 4 * g] : S.zero;
                     A[0] = __builtin_bit_cast(f4_i4, *(const f4_u4*)a0);
-                } else if constexpr (RS == 4) {
+                } else {
                     const uint32_t* const a0 = n < 8 ? &W[n * F4_WROW + 4 * g] : S.zero;
                     A[0] = __builtin_bit_cast(f4_i4, *(const f4_u4*)a0);
                     A[NMF - 1] = __builtin_bit_cast(f4_i4, *(const f4_u4*)&W[(8 + n) * F4_WROW + 4 * g]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < NMF; ++j) A[j] = __builtin_bit_cast(f4_i4, *(const f4_u4*)&W[(16 * j + n) * F4_WROW + 4 * g]);
                 }
                 f4_i4 B0, B1;
 #pragma unroll
@@ -764,18 +748,14 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
                 }
             };
 #pragma unroll
-            for (int l0 = 0; l0 < NG; l0 += Smem::PG) {
-                if (l0 >= ng) break;
+            for (int l = 0; l < NG; ++l)
+                if (l < ng) digits(l);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
 #pragma unroll
-                for (int l = l0; l < l0 + Smem::PG; ++l)
-                    if (l < ng) digits(l);
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                __builtin_amdgcn_wave_barrier();
-#pragma unroll
-                for (int l = l0; l < l0 + Smem::PG; ++l)
-                    if (l < ng) multiply(l);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+            for (int l = 0; l < NG; ++l)
+                if (l < ng) multiply(l);
+            __builtin_amdgcn_sched_barrier(0);
             issue_v(n0 + 256, nx, vr);
             nx = after;
             __builtin_amdgcn_sched_barrier(0);
@@ -846,9 +826,7 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
                 n8 += (int)__popcll(__ballot(fin) & lead4);
                 for (uint64_t m = __ballot(have && !live) & lead4; m; m &= m - 1) {
                     const int r = __builtin_amdgcn_readlane(er, __builtin_ctzll(m));
-#pragma unroll
-                    for (int j = 0; j < RL; ++j)
-                        if (row + j == r) rfl[j] = 1;
+                    if (row == r) rfl = 1;
                 }
                 for (uint64_t lv = __ballot(live) & lead4; lv; lv &= lv - 1) {
                     const int ln = __builtin_ctzll(lv);
@@ -862,18 +840,16 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
                         // the scales that these sums met belong to the bound on |v|
                         if (l < ng) vm[l] = pk_max(vm[l], (f4_h2){(P.vs + kv4_vscale(vc))[16 * l], 0});
                     }
-#pragma unroll
-                    for (int j = 0; j < RL; ++j) {
-                        if (row + j != r) continue;
-                        if (Er > base[j] + F4_BITS) rebase(j, Er - (F4_BITS - F4_HEAD));
-                        const int de = Er - base[j];
-                        if (!MOD && de < -1000) rfl[j] = 1;
+                    if (row == r) {
+                        if (Er > base + F4_BITS) rebase(Er - (F4_BITS - F4_HEAD));
+                        const int de = Er - base;
+                        if (!MOD && de < -1000) rfl = 1;
                         const double om = de < -1000 ? 0.0 : ldexp((double)Mr, de);
-                        z[j] += head ? om : 0.0;
+                        z += head ? om : 0.0;
 #pragma unroll
                         for (int l = 0; l < NG; ++l) {
                             if (l >= ng) break;
-                            double* const o = &O[j * 32 * NG + 32 * l];
+                            double* const o = &O[32 * l];
                             if constexpr (RS == 2) {
                                 o[0] = __fma_rn(om, sub ? bf16hi_f64(v2[l]) : bf16lo_f64(v2[l]), o[0]);
                                 continue;
@@ -903,21 +879,18 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
         // ---- epilogue: row totals of the wave, then the 4 waves' partials at the rows' largest base (exact powers of two), two
         // additions deep
         {
-#pragma unroll
-            for (int j = 0; j < RL; ++j) {
-                double zs = z[j], ls = lostw[j];
-                int fl = rfl[j];
-                for (int o = 1; o < RLANES; o <<= 1) {
-                    zs += __shfl_xor(zs, o, 64);
-                    ls += __shfl_xor(ls, o, 64);
-                    fl |= __shfl_xor(fl, o, 64);
-                }
-                if (head) {
-                    S.wR[w][row + j] = base[j];
-                    S.wZ[w][row + j] = zs;
-                    S.we[w][row + j] = ls;
-                    S.wf[w][row + j] = fl;
-                }
+            double zs = z, ls = lostw;
+            int fl = rfl;
+            for (int o = 1; o < RLANES; o <<= 1) {
+                zs += __shfl_xor(zs, o, 64);
+                ls += __shfl_xor(ls, o, 64);
+                fl |= __shfl_xor(fl, o, 64);
+            }
+            if (head) {
+                S.wR[w][row] = base;
+                S.wZ[w][row] = zs;
+                S.we[w][row] = ls;
+                S.wf[w][row] = fl;
             }
             if (lane == 0) S.wn[w] = folds;
 #pragma unroll

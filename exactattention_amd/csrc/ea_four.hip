@@ -21,14 +21,14 @@ Four four_of(int ng, int mod) {
     return ng == 4 ? Four{four_fn<RS, 4>(mod), sizeof(FourSmem<RS, 4>)}
                    : (ng == 3 ? Four{four_fn<RS, 3>(mod), sizeof(FourSmem<RS, 3>)} : Four{four_fn<RS, 2>(mod), sizeof(FourSmem<RS, 2>)});
 }
-Four four_of(int rs, int ng, int mod) { return rs == 2 ? four_of<2>(ng, mod) : (rs == 4 ? four_of<4>(ng, mod) : four_of<8>(ng, mod)); }
+Four four_of(int rs, int ng, int mod) { return rs == 2 ? four_of<2>(ng, mod) : four_of<4>(ng, mod); }
 int four_ng(const Params& P) { return std::max(2, (P.g.head_dim_v + 31) >> 5); }
 Four four_of(const Params& P) { return four_of(P.rb, four_ng(P), P.mods); }
 hipError_t four_attrs() {
     static std::once_flag once;
     static hipError_t err = hipSuccess;
     std::call_once(once, [] {
-        for (int rs = 2; rs <= 8; rs *= 2)
+        for (int rs = 2; rs <= 4; rs *= 2)
             for (int ng = 2; ng <= 4; ++ng)
                 for (int mod = 0; mod < 4; ++mod) {
                     const Four f = four_of(rs, ng, mod);
@@ -51,13 +51,13 @@ int ea::ea_four_eligible(const Params& P) {
 int ea::ea_four_slots(const Params& P, int* slots) {
     // blocks resident on the current device at once, cached per device and kernel
     static std::mutex mu;
-    static int cache[64][36] = {};
+    static int cache[64][24] = {};
     hipError_t e = four_attrs();
     if (e != hipSuccess) return -100 - (int)e;
     int dev = 0;
     if ((e = hipGetDevice(&dev)) != hipSuccess) return -100 - (int)e;
     const Four f = four_of(P);
-    const int ki = (P.rb == 2 ? 0 : (P.rb == 4 ? 1 : 2)) + 3 * (four_ng(P) - 2) + 9 * P.mods;
+    const int ki = (P.rb == 2 ? 0 : 1) + 2 * (four_ng(P) - 2) + 6 * P.mods;
     std::lock_guard<std::mutex> lk(mu);
     if (dev < 0 || dev >= 64) return -1;
     if (!cache[dev][ki]) {

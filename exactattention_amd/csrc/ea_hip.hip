@@ -1687,7 +1687,7 @@ int make_plan(const ea_geometry* g, const ea_options* o, Plan* pl, const ea_scor
     gen.dq = d128 && !m && dq_fits(gen.nrb);
     Tier1& mr = pl->mr;
     mr.rb = m && pl->prefill ? 0 : mrow_rows(g, o, pl->r_seg, m != nullptr || kv4);
-    if (kv4 && mr.rb) mr.rb = pl->r_seg <= 2 ? 2 : std::min(mr.rb, 8);  // ea_four's row blocks
+    if (kv4 && mr.rb) mr.rb = pl->r_seg <= 2 ? 2 : 4;  // ea_four's row blocks
     pl->mrow = mr.rb > 0;
     const size_t without = lay_out(pl, g, o, false, m != nullptr);
     if (!pl->mrow) return 0;
