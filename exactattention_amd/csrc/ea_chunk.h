@@ -18,6 +18,26 @@ __device__ __forceinline__ uint32_t f64_bf16(double x) {
     }
     return (b + 0x7FFFu + ((b >> 16) & 1u)) >> 16;
 }
+// The same of N values, two to a word. Rounded to fp32 first, which only a value next to a tie of bf16 can tell: where one looks like a tie
+// (2^-16 of them do) all are rounded singly. 3 instructions a value; f64_bf16 takes two branches.
+template <int N>
+__device__ __forceinline__ void f64_bf16_all(const double (&x)[N], uint32_t* out) {
+    typedef float two_f __attribute__((ext_vector_type(2)));
+    typedef __bf16 two_b __attribute__((ext_vector_type(2)));
+    typedef unsigned short two_h __attribute__((ext_vector_type(2)));
+    two_h tie = {0xFFFF, 0xFFFF};
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        const two_f f = {(float)x[i], (float)x[i + 1]};
+        out[i / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f, two_b));
+        const uint32_t low = __builtin_amdgcn_perm(__float_as_uint(f.y), __float_as_uint(f.x), 0x05040100u) ^ 0x80008000u;
+        tie = __builtin_elementwise_min(tie, __builtin_bit_cast(two_h, low));
+    }
+    if (__builtin_expect(tie.x == 0 || tie.y == 0, 0)) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) out[i / 2] = f64_bf16(x[i]) | f64_bf16(x[i + 1]) << 16;
+    }
+}
 __device__ __forceinline__ uint32_t f32_bf16(float f) {
     const uint32_t b = __float_as_uint(f);
     if ((b & 0x7FFFFFFFu) > 0x7F800000u) return (b >> 16) | 0x40u;
@@ -56,6 +76,14 @@ struct Chunk {
         if constexpr (FP32) r[i] = __float_as_uint((float)x);
         else if (i & 1) r[i >> 1] |= f64_bf16(x) << 16;
         else r[i >> 1] = f64_bf16(x);
+    }
+    __device__ __forceinline__ void put_all(const double (&x)[V]) {
+        if constexpr (FP32 || V < 2) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) put(i, x[i]);
+        } else {
+            f64_bf16_all<V>(x, r);
+        }
     }
     __device__ __forceinline__ void store(void* p, int64_t at) const {
         if constexpr (V == 8) {

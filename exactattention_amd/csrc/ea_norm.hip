@@ -127,10 +127,11 @@ struct Row {
     bool live;
 };
 
-template <int C, bool IN32, bool OUT32, bool KV4, bool ADJ>
+// FULL: every lane holds two whole runs, and 32 elements lie with 4 lanes from a multiple of 4 (full_lanes)
+template <int C, bool IN32, bool OUT32, bool KV4, bool ADJ, bool FULL>
 __global__ void __launch_bounds__(NR_THREADS) ea_norm_rotary_kernel(ea_norm_rotary N, int tpb, int L) {
     extern __shared__ __align__(16) double2 cs[];  // tpb x pairs, then the weights of q and k (d each)
-    __shared__ uint32_t s_max[NR_THREADS];         // of a head's groups, at its lanes' places
+    __shared__ uint32_t s_max[FULL ? 1 : NR_THREADS];  // of a head's groups, at its lanes' places
     const ea_rotary& A = N.r;
     const int d = A.head_dim, R = A.rot_dim, h = R / 2, tid = threadIdx.x;
     const int64_t t0 = (int64_t)blockIdx.x * tpb;
@@ -139,10 +140,11 @@ __global__ void __launch_bounds__(NR_THREADS) ea_norm_rotary_kernel(ea_norm_rota
     double* const wt = (double*)(cs + tpb * h);
     const int Hq = A.num_q_heads, Hk = A.num_kv_heads, I = Hq + Hk + (A.v ? Hk : 0);
     const int u = tid & (L - 1), base = tid & ~(L - 1);
+    const int shift = KV4 && !(N.page_size & (N.page_size - 1)) ? __builtin_ctz(N.page_size) : -1;  // -1: a division
     auto row_of = [&](int it) __attribute__((always_inline)) {
         Row x;
-        x.tk = it / I;
-        int g = it - x.tk * I;
+        int g = it;
+        for (x.tk = 0; g >= I; ++x.tk) g -= I;  // a few tokens
         const int64_t t = t0 + x.tk;
         x.scales = nullptr;
         if (g < Hq) {
@@ -166,7 +168,7 @@ __global__ void __launch_bounds__(NR_THREADS) ea_norm_rotary_kernel(ea_norm_rota
         const int64_t ts = v ? A.vo_tok_stride : A.ko_tok_stride, hs = v ? A.vo_head_stride : A.ko_head_stride;
         if constexpr (KV4) {
             x.scales = v ? N.v_scales : N.k_scales;
-            const int64_t page = r / N.page_size, slot = r - page * N.page_size;
+            const int64_t page = shift >= 0 ? r >> shift : r / N.page_size, slot = r - page * N.page_size;
             if (v) x.o = kv4_v_at(page * N.v_page_stride + g * hs, slot, kv4_width(d));
             else x.o = page * N.k_page_stride + slot * ts + g * hs;
         } else {
@@ -184,13 +186,13 @@ __global__ void __launch_bounds__(NR_THREADS) ea_norm_rotary_kernel(ea_norm_rota
         x.row = row_of(it);
         x.H = held_by<C, ADJ>(u, d, R, x.row.kind == 2);
         if (!x.row.live) return;
-        if (x.H.e[0] >= 0) x.a.load(x.row.src, x.row.s + x.H.e[0]);
-        if (x.H.e[1] >= 0) x.b.load(x.row.src, x.row.s + x.H.e[1]);
+        if (FULL || x.H.e[0] >= 0) x.a.load(x.row.src, x.row.s + x.H.e[0]);
+        if (FULL || x.H.e[1] >= 0) x.b.load(x.row.src, x.row.s + x.H.e[1]);
     };
     auto finish = [&](Work& x) __attribute__((always_inline)) {
         if (!x.row.live) return;
         const Held& H = x.H;
-        const bool has[2] = {H.e[0] >= 0, H.e[1] >= 0};
+        const bool has[2] = {FULL || H.e[0] >= 0, FULL || H.e[1] >= 0};
         const bool four = KV4 && x.row.kind != 0;
         if (!four && (x.row.kind == 2 || !(norm || H.turn[0] || H.turn[1]))) {  // as it is
             if (has[0]) store_as<C, IN32, OUT32>(x.a, x.row.dst, x.row.o + H.e[0]);
@@ -227,19 +229,31 @@ __global__ void __launch_bounds__(NR_THREADS) ea_norm_rotary_kernel(ea_norm_rota
                     m[0] = max(m[0], __float_as_uint(f[0][i]) & 0x7FFFFFFFu);  // magnitudes order as whole numbers, NaN last
                     m[1] = max(m[1], __float_as_uint(f[1][i]) & 0x7FFFFFFFu);
                 }
-                // a head has at most as many groups as lanes, which all lie in one wave
-                s_max[tid] = 0;
-                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-                __builtin_amdgcn_wave_barrier();
+                if constexpr (FULL) {
 #pragma unroll
-                for (int k = 0; k < 2; ++k)
-                    if (has[k]) atomicMax(&s_max[base + (H.e[k] >> 5)], m[k]);
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                __builtin_amdgcn_wave_barrier();
+                    for (int k = 0; k < 2; ++k) {
+                        m[k] = max(m[k], (uint32_t)__builtin_amdgcn_mov_dpp((int)m[k], 0xB1, 0xF, 0xF, true));
+                        m[k] = max(m[k], (uint32_t)__builtin_amdgcn_mov_dpp((int)m[k], 0x4E, 0xF, 0xF, true));
+                    }
+                } else {
+                    // a head has at most as many groups as lanes, which all lie in one wave
+                    s_max[tid] = 0;
+                    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        if (has[k]) atomicMax(&s_max[base + (H.e[k] >> 5)], m[k]);
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        if (has[k])
+                            m[k] = __hip_atomic_load(&s_max[base + (H.e[k] >> 5)], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+                }
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     if (!has[k]) continue;
-                    const uint32_t top = __hip_atomic_load(&s_max[base + (H.e[k] >> 5)], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+                    const uint32_t top = m[k];
                     const int fld = (int)(top >> 23);
                     const int sc = fld == 255 ? 255 : min(max(fld - ((top & 0x7FFFFFu) < 0x600000u ? 2 : 1), 2), 252);
                     const float by = __uint_as_float((uint32_t)sc << 23);
@@ -269,13 +283,11 @@ __global__ void __launch_bounds__(NR_THREADS) ea_norm_rotary_kernel(ea_norm_rota
         }
         Chunk<C, OUT32> y;
         if (has[0]) {
-#pragma unroll
-            for (int i = 0; i < C; ++i) y.put(i, a[i]);
+            y.put_all(a);
             y.store(x.row.dst, x.row.o + H.e[0]);
         }
         if (has[1]) {
-#pragma unroll
-            for (int i = 0; i < C; ++i) y.put(i, b[i]);
+            y.put_all(b);
             y.store(x.row.dst, x.row.o + H.e[1]);
         }
     };
@@ -287,16 +299,16 @@ __global__ void __launch_bounds__(NR_THREADS) ea_norm_rotary_kernel(ea_norm_rota
         for (int i = tid; i < 2 * d; i += NR_THREADS)
             wt[i] = i < d ? weight_at(N.q_weight, N.weights_fp32, i) : weight_at(N.k_weight, N.weights_fp32, i - d);
     __syncthreads();
-    if (it < total) finish(x);
-    for (it += step; it < total; it += step) {
-        fetch(it, x);
+    while (it < total) {
         finish(x);
+        it += step;
+        if (it < total) fetch(it, x);
     }
 }
 
 // The gradient. A block takes the q heads or the k heads (the first qblocks blocks those of q) of every so many tokens and keeps
 // its sums of g xh, each lane those of its own elements; the lanes that held the same elements meet in LDS at the end.
-template <int C, bool F32, bool ADJ>
+template <int C, bool F32, bool ADJ, bool FULL>
 __global__ void __launch_bounds__(NR_THREADS) ea_norm_rotary_grad_kernel(ea_norm_rotary_grad G, int tpb, int L, int qblocks) {
     extern __shared__ __align__(16) double2 cs[];  // tpb x pairs, the weight (d), and the lanes' sums (256 x 2 C) at the end
     const ea_rotary& A = G.r;
@@ -307,7 +319,7 @@ __global__ void __launch_bounds__(NR_THREADS) ea_norm_rotary_grad_kernel(ea_norm
     double* const wt = (double*)(cs + tpb * h);
     const int u = tid & (L - 1);
     const Held H = held_by<C, ADJ>(u, d, R, false);
-    const bool has[2] = {H.e[0] >= 0, H.e[1] >= 0};
+    const bool has[2] = {FULL || H.e[0] >= 0, FULL || H.e[1] >= 0};
     const void* const xs = isk ? A.k : A.q;
     const void* const gs = isk ? G.gk : G.gq;
     void* const os = isk ? A.k_out : A.q_out;
@@ -357,12 +369,14 @@ __global__ void __launch_bounds__(NR_THREADS) ea_norm_rotary_grad_kernel(ea_norm
             for (int k = 0; k < 2; ++k) {
                 if (!has[k]) continue;
                 Chunk<C, F32> o;
+                double y[C];
 #pragma unroll
                 for (int i = 0; i < C; ++i) {
                     const double gi = k ? b[i] : a[i], xi = (double)x[k].get(i);
                     acc[k][i] = __fma_rn(gi, xi * r, acc[k][i]);
-                    o.put(i, r * __fma_rn(-xi, m, gi * wt[H.e[k] + i]));
+                    y[i] = r * __fma_rn(-xi, m, gi * wt[H.e[k] + i]);
                 }
+                o.put_all(y);
                 o.store(os, t * ot + hd * oh + H.e[k]);
             }
         }
@@ -382,43 +396,60 @@ __global__ void __launch_bounds__(NR_THREADS) ea_norm_rotary_grad_kernel(ea_norm
     }
 }
 
-// the blocks' partial sums to the weights' gradients: 32 elements a block, 8 threads each, in a fixed order
-__global__ void __launch_bounds__(256) ea_norm_weights_kernel(const double* partial, int d, int qblocks, int kblocks, void* dq,
-                                                              void* dk, int fp32) {
-    __shared__ double part[8][32];
+// the blocks' partial sums to the weights' gradients: 32 elements a block, 32 threads each, in a fixed order
+__global__ void __launch_bounds__(1024) ea_norm_weights_kernel(const double* partial, int d, int qblocks, int kblocks, void* dq,
+                                                               void* dk, int fp32) {
+    __shared__ double part[32][33];
     const int per = (d + 31) / 32;
     const bool isk = (int)blockIdx.x >= per;
-    const int i = ((int)blockIdx.x - (isk ? per : 0)) * 32 + (threadIdx.x & 31), y = threadIdx.x >> 5;
+    const int x = threadIdx.x & 31, i = ((int)blockIdx.x - (isk ? per : 0)) * 32 + x, y = threadIdx.x >> 5;
     void* const out = isk ? dk : dq;
     if (!out) return;
     const int b0 = isk ? qblocks : 0, n = isk ? kblocks : qblocks;
-    double s = 0.0;
+    double s[4] = {0.0, 0.0, 0.0, 0.0};
     if (i < d)
-        for (int b = y; b < n; b += 8) s += partial[(int64_t)(b0 + b) * d + i];
-    part[y][threadIdx.x & 31] = s;
-    __syncthreads();
+        for (int b = y; b < n; b += 128)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (b + 32 * k < n) s[k] += partial[(int64_t)(b0 + b + 32 * k) * d + i];
+    part[y][x] = (s[0] + s[1]) + (s[2] + s[3]);
+    for (int o = 16; o > 0; o >>= 1) {
+        __syncthreads();
+        if (y < o) part[y][x] += part[y + o][x];
+    }
     if (y || i >= d) return;
-    for (int k = 1; k < 8; ++k) s += part[k][threadIdx.x];
-    if (fp32) ((float*)out)[i] = (float)s;
-    else ((uint16_t*)out)[i] = (uint16_t)f64_bf16(s);
+    if (fp32) ((float*)out)[i] = (float)part[0][x];
+    else ((uint16_t*)out)[i] = (uint16_t)f64_bf16(part[0][x]);
 }
 
-// rows of K, or slots of V's tiles, to bf16, 8 elements a thread
-template <bool V>
-__global__ void __launch_bounds__(256) ea_kv4_values_kernel(int64_t n, int per, int groups, const uint8_t* codes, const uint8_t* scales,
-                                                            uint16_t* out) {
+// rows of K to bf16, 8 elements a thread
+__global__ void __launch_bounds__(256) ea_kv4_keys_kernel(int64_t n, int per, int groups, const uint8_t* codes, const uint8_t* scales,
+                                                          uint16_t* out) {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
         const int64_t row = i / per;
         const int c = (int)(i - row * per);
-        uint4 x;
-        if constexpr (V) {
-            const int64_t at = kv4_v_at(0, row, 32 * groups);
-            x = make_uint4(kv4_vload2(codes, scales, at, 8 * c), kv4_vload2(codes, scales, at, 8 * c + 2),
-                           kv4_vload2(codes, scales, at, 8 * c + 4), kv4_vload2(codes, scales, at, 8 * c + 6));
-        } else {
-            x = kv4_load8(codes, scales, row * groups * 32 + 8 * c);
+        *(uint4*)(out + row * per * 8 + 8 * c) = kv4_load8(codes, scales, row * groups * 32 + 8 * c);
+    }
+}
+
+// tiles of V to rows of bf16, 8 channels of a tile's 16 slots a thread: 16-byte reads, and writes that are whole rows over the lanes
+// (a thread for 8 channels of one slot gathers bytes: 131072 slots of 128 channels 20 us, here 9)
+__global__ void __launch_bounds__(256) ea_kv4_tiles_kernel(int64_t n, int per, int groups, const uint8_t* codes, const uint8_t* scales,
+                                                           uint16_t* out) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int64_t tile = i / per;
+        const int c = (int)(i - tile * per);
+        const uint8_t* const p = codes + tile * groups * 256 + 64 * c;
+        const uint4 w[4] = {*(const uint4*)p, *(const uint4*)(p + 16), *(const uint4*)(p + 32), *(const uint4*)(p + 48)};
+        const uint4 s = *(const uint4*)(scales + tile * groups * 16 + 16 * (c >> 2));
+        uint16_t* o = out + tile * 16 * per * 8 + 8 * c;
+#pragma unroll
+        for (int k = 0; k < 16; ++k, o += per * 8) {
+            auto byte = [&](const uint4& x) { return ((k < 4 ? x.x : (k < 8 ? x.y : (k < 12 ? x.z : x.w))) >> (8 * (k & 3))) & 0xFFu; };
+            const uint32_t sc = byte(s);
+            *(uint4*)o = make_uint4(kv4_bf16x2<0>(byte(w[0]), sc), kv4_bf16x2<0>(byte(w[1]), sc), kv4_bf16x2<0>(byte(w[2]), sc),
+                                    kv4_bf16x2<0>(byte(w[3]), sc));
         }
-        *(uint4*)(out + row * per * 8 + 8 * c) = x;
     }
 }
 
@@ -435,19 +466,22 @@ int lanes_of(int d, int C) {
     return L;
 }
 
-template <int C, bool ADJ>
+// every lane holds two whole runs of 8, 4 lanes 32 elements
+bool full_lanes(int d, int R, bool adjacent, int C, int L) { return C == 8 && d == 16 * L && d % 64 == 0 && (adjacent || R % 64 == 0); }
+
+template <int C, bool ADJ, bool FULL>
 void launch(const ea_norm_rotary& a, dim3 grid, size_t lds, int tpb, int L, hipStream_t st) {
     const bool four = a.k_scales != nullptr;
     auto go = [&](auto* fn) { hipLaunchKernelGGL(fn, grid, dim3(NR_THREADS), lds, st, a, tpb, L); };
     if (!a.r.in_fp32) {
-        if (four) go(ea_norm_rotary_kernel<C, false, false, true, ADJ>);
-        else go(ea_norm_rotary_kernel<C, false, false, false, ADJ>);
+        if (four) go(ea_norm_rotary_kernel<C, false, false, true, ADJ, FULL>);
+        else go(ea_norm_rotary_kernel<C, false, false, false, ADJ, FULL>);
     } else if (four) {
-        go(ea_norm_rotary_kernel<C, true, false, true, ADJ>);
+        go(ea_norm_rotary_kernel<C, true, false, true, ADJ, FULL>);
     } else if (a.r.out_fp32) {
-        go(ea_norm_rotary_kernel<C, true, true, false, ADJ>);
+        go(ea_norm_rotary_kernel<C, true, true, false, ADJ, FULL>);
     } else {
-        go(ea_norm_rotary_kernel<C, true, false, false, ADJ>);
+        go(ea_norm_rotary_kernel<C, true, false, false, ADJ, FULL>);
     }
 }
 
@@ -518,13 +552,16 @@ int ea_hip_norm_rotary(const ea_norm_rotary* a, ea_stream_t stream) {
     const dim3 grid((unsigned)(((int64_t)r.num_tokens + tpb - 1) / tpb), (unsigned)slices);
     const size_t lds = (size_t)tpb * (R / 2) * 16 + (size_t)2 * d * 8;
     const hipStream_t st = (hipStream_t)stream;
+    const bool full = full_lanes(d, R, r.adjacent != 0, C, L);
     if (r.adjacent) {
-        if (C == 8) launch<8, true>(*a, grid, lds, tpb, L, st);
-        else launch<2, true>(*a, grid, lds, tpb, L, st);
+        if (full) launch<8, true, true>(*a, grid, lds, tpb, L, st);
+        else if (C == 8) launch<8, true, false>(*a, grid, lds, tpb, L, st);
+        else launch<2, true, false>(*a, grid, lds, tpb, L, st);
     } else {
-        if (C == 8) launch<8, false>(*a, grid, lds, tpb, L, st);
-        else if (C == 2) launch<2, false>(*a, grid, lds, tpb, L, st);
-        else launch<1, false>(*a, grid, lds, tpb, L, st);
+        if (full) launch<8, false, true>(*a, grid, lds, tpb, L, st);
+        else if (C == 8) launch<8, false, false>(*a, grid, lds, tpb, L, st);
+        else if (C == 2) launch<2, false, false>(*a, grid, lds, tpb, L, st);
+        else launch<1, false, false>(*a, grid, lds, tpb, L, st);
     }
     return herr(hipGetLastError());
 }
@@ -590,21 +627,26 @@ int ea_hip_norm_rotary_grad(const ea_norm_rotary_grad* a, ea_stream_t stream) {
             hipLaunchKernelGGL(fn, dim3((unsigned)(qb + kb)), dim3(NR_THREADS), lds, st, *a, tpb, L, qb);
             return herr(hipGetLastError());
         };
+        auto both = [&](auto* wide, auto* narrow) -> int { return r.in_fp32 ? go(wide) : go(narrow); };
+        const bool full = full_lanes(d, R, r.adjacent != 0, C, L);
         int e;
         if (r.adjacent) {
-            if (C == 8) e = r.in_fp32 ? go(ea_norm_rotary_grad_kernel<8, true, true>) : go(ea_norm_rotary_grad_kernel<8, false, true>);
-            else e = r.in_fp32 ? go(ea_norm_rotary_grad_kernel<2, true, true>) : go(ea_norm_rotary_grad_kernel<2, false, true>);
+            if (full) e = both(ea_norm_rotary_grad_kernel<8, true, true, true>, ea_norm_rotary_grad_kernel<8, false, true, true>);
+            else if (C == 8) e = both(ea_norm_rotary_grad_kernel<8, true, true, false>, ea_norm_rotary_grad_kernel<8, false, true, false>);
+            else e = both(ea_norm_rotary_grad_kernel<2, true, true, false>, ea_norm_rotary_grad_kernel<2, false, true, false>);
+        } else if (full) {
+            e = both(ea_norm_rotary_grad_kernel<8, true, false, true>, ea_norm_rotary_grad_kernel<8, false, false, true>);
         } else if (C == 8) {
-            e = r.in_fp32 ? go(ea_norm_rotary_grad_kernel<8, true, false>) : go(ea_norm_rotary_grad_kernel<8, false, false>);
+            e = both(ea_norm_rotary_grad_kernel<8, true, false, false>, ea_norm_rotary_grad_kernel<8, false, false, false>);
         } else if (C == 2) {
-            e = r.in_fp32 ? go(ea_norm_rotary_grad_kernel<2, true, false>) : go(ea_norm_rotary_grad_kernel<2, false, false>);
+            e = both(ea_norm_rotary_grad_kernel<2, true, false, false>, ea_norm_rotary_grad_kernel<2, false, false, false>);
         } else {
-            e = r.in_fp32 ? go(ea_norm_rotary_grad_kernel<1, true, false>) : go(ea_norm_rotary_grad_kernel<1, false, false>);
+            e = both(ea_norm_rotary_grad_kernel<1, true, false, false>, ea_norm_rotary_grad_kernel<1, false, false, false>);
         }
         if (e) return e;
     }
     if (sums) {
-        hipLaunchKernelGGL(ea_norm_weights_kernel, dim3((unsigned)(2 * ((d + 31) / 32))), dim3(256), 0, st, a->partial, d, qb, kb,
+        hipLaunchKernelGGL(ea_norm_weights_kernel, dim3((unsigned)(2 * ((d + 31) / 32))), dim3(1024), 0, st, a->partial, d, qb, kb,
                            a->dq_weight, a->dk_weight, a->weights_fp32);
         return herr(hipGetLastError());
     }
@@ -618,9 +660,9 @@ int ea_hip_kv4_values(int64_t rows, int32_t head_dim, int32_t is_v, const uint8_
     if (!codes || !scales || !values || ((uintptr_t)codes & 3) || ((uintptr_t)values & 15)) return -1;
     const int per = head_dim / 8;
     if (rows > (((int64_t)1 << 62) / head_dim)) return -1;
-    const int64_t n = rows * per;
+    const int64_t n = (is_v ? rows / 16 : rows) * per;
     const unsigned grid = (unsigned)std::min<int64_t>((n + 255) / 256, 8192);
-    const auto fn = is_v ? ea_kv4_values_kernel<true> : ea_kv4_values_kernel<false>;
+    const auto fn = is_v ? ea_kv4_tiles_kernel : ea_kv4_keys_kernel;
     hipLaunchKernelGGL(fn, dim3(grid), dim3(256), 0, (hipStream_t)stream, n, per, (head_dim + 31) / 32, codes, scales, values);
     return herr(hipGetLastError());
 }

@@ -85,15 +85,23 @@ class KV4Pool:
     def values(self):
         """The cache's values: k, v (pages, Hkv, page_size, head_dim) bf16, new tensors."""
         import torch
-        shape = (self.num_pages, self.Hkv, self.page_size, self.head_dim)
-        out = []
-        with torch.cuda.device(self.dev):
-            for is_v, codes, scales in ((0, self.k, self.k_scales), (1, self.v, self.v_scales)):
-                x = torch.empty(shape, dtype=torch.bfloat16, device=self.dev)
-                hip._check(hip.load().ea_hip_kv4_values(x.numel() // self.head_dim, self.head_dim, is_v, codes.data_ptr(),
-                                                        scales.data_ptr(), x.data_ptr(), hip._stream_ptr(torch)), "ea_hip_kv4_values")
-                out.append(x)
-        return tuple(out)
+        C = torch._C
+        x = self.k.new_empty((2, self.num_pages, self.Hkv, self.page_size, self.head_dim), dtype=torch.bfloat16)
+        index, rows = self.dev.index, self.num_pages * self.Hkv * self.page_size
+        fn, at = hip.load().ea_hip_kv4_values, x.data_ptr()
+
+        def launch():
+            st = C._cuda_getCurrentRawStream(index)
+            hip._check(fn(rows, self.head_dim, 0, self.k.data_ptr(), self.k_scales.data_ptr(), at, st), "ea_hip_kv4_values")
+            hip._check(fn(rows, self.head_dim, 1, self.v.data_ptr(), self.v_scales.data_ptr(), at + 2 * rows * self.head_dim, st),
+                       "ea_hip_kv4_values")
+
+        if C._cuda_getDevice() == index:
+            launch()
+        else:
+            with torch.cuda.device(index):
+                launch()
+        return x.unbind(0)
 
     def append(self, k, v, dst_rows) -> None:
         """k and v (tokens, Hkv, head_dim), bf16 (or int16) or fp32 with any strides over tokens and heads, to rows

@@ -33,7 +33,7 @@ import numpy as np
 from . import hip
 from .formats import ExactAttentionDomainError, ExactAttentionUncertifiedError, alpha_bits_for, alpha_fp32_bits
 from .kv4 import KV4Pool
-from .step import PLAN_ROWS, PLAN_SEQS, DraftCheck, HeadNorm, Rotary, StepPlan  # noqa: F401
+from .step import PLAN_ROWS, PLAN_SEQS, DraftCheck, HeadNorm, Rotary, StepPlan, _weights  # noqa: F401
 
 TILE = 64  # keys per digit tile
 
@@ -447,7 +447,7 @@ class ExactAttentionBackend:
         if norm is not None:
             if rotary is None:
                 raise ValueError("norm needs rotary=")
-            norm._weights(rotary)  # of its head size, type and device
+            _weights(rotary, norm.q_weight, norm.k_weight)  # of its head size, type and device
         if rotary is not None and cache.pool4 is not None and rotary.rot_dim % 4:
             raise ValueError("rot_dim must be a multiple of 4 with a cache in 4 bits")
         self.mods, self.rotary, self.norm = mods, rotary, norm

@@ -114,13 +114,14 @@ def _norm_turn():
 
         class NormTurn(torch.autograd.Function):
             @staticmethod
-            def forward(ctx, q, k, qw, kw, positions, rotary, eps):
+            def forward(ctx, q, k, qw, kw, positions, rotary, norm):
                 ctx.save_for_backward(q, k, qw, kw, positions)
-                ctx.rotary, ctx.eps = rotary, eps
                 ctx.set_materialize_grads(False)
-                out = rotary.rotate(q, k, positions, norm=HeadNorm(qw, kw, eps))
-                need = ctx.needs_input_grad
-                ctx.mark_non_differentiable(*(o for i, o in enumerate(out) if not (need[i] or need[i + 2])))
+                out = rotary.rotate(q, k, positions, norm=norm)
+                ctx.rotary, ctx.eps = rotary, norm.eps
+                a, b, c, d = ctx.needs_input_grad[:4]
+                if not ((a or c) and (b or d)):
+                    ctx.mark_non_differentiable(out[1] if a or c else out[0])
                 return out
 
             @staticmethod
@@ -258,16 +259,16 @@ class HeadNorm:
             raise ValueError("q_weight and k_weight must be (head_dim,) tensors of one type")
         self.q_weight, self.k_weight, self.eps = q_weight, k_weight, float(eps)
 
-    def _weights(self, r):
-        """(address of q's, of k's, whether they are fp32), checked for the rotation r."""
-        out = []
-        for name, w in (("q_weight", self.q_weight), ("k_weight", self.k_weight)):
-            if w.shape[0] != r.head_dim or not (w.dtype is r._f32 or w.dtype is r._bits[0]) or w.get_device() != r._at:
-                raise ValueError(f"{name} must be ({r.head_dim},) bf16 or fp32 on {r.dev}")
-            if w.shape[0] > 1 and w.stride(0) != 1:
-                raise ValueError(f"{name} must be contiguous")
-            out.append(w.data_ptr())
-        return out[0], out[1], self.q_weight.dtype is r._f32
+
+def _weights(r, q_weight, k_weight):
+    """The addresses of the norms' weights, checked for the rotation r."""
+    f32, bits, at = r._f32, r._bits[0], r._at
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w.shape[0] != r.head_dim or not (w.dtype is f32 or w.dtype is bits) or w.get_device() != at:
+            raise ValueError(f"{name} must be ({r.head_dim},) bf16 or fp32 on {r.dev}")
+        if w.shape[0] > 1 and w.stride(0) != 1:
+            raise ValueError(f"{name} must be contiguous")
+    return q_weight.data_ptr(), k_weight.data_ptr()
 
 
 class Rotary:
@@ -307,6 +308,7 @@ class Rotary:
         self._bits, self._f32, self._i32, self._i64 = (torch.bfloat16, torch.int16), torch.float32, torch.int32, torch.int64
         self._half, self._axis = self.half_turns.data_ptr(), self.axis_of_pair.data_ptr()
         self._norm_fn = self._grad_fn = None
+        self._partial = {}  # bytes that the weights' gradients are summed in, by heads
 
     def _tokens(self, x, name, n=None):
         """Checks a (tokens, heads, head_dim) tensor, int16 standing for bf16 bits: (tokens, heads, fp32, strides)."""
@@ -362,7 +364,7 @@ class Rotary:
         if norm is not None or kv4 is not None:
             if self._norm_fn is None:
                 self._norm_fn = _entry("ea_hip_norm_rotary")
-            qw, kw, w32 = (0, 0, 0) if norm is None else norm._weights(self)
+            qw, kw, w32 = (0, 0, 0) if norm is None else (*_weights(self, norm.q_weight, norm.k_weight), norm.q_weight.dtype is self._f32)
             page = 0 if kv4 is None else kv4.Hkv * kv4.page_size * kv4.width
             scales = (0, 0) if kv4 is None else (kv4.k_scales.data_ptr(), kv4.v_scales.data_ptr())
             _call(self._norm_fn, _NORM.pack(
@@ -395,12 +397,12 @@ class Rotary:
         if norm is not None:
             if inverse:
                 raise ValueError("the norm has no inverse")
-            if _C.is_grad_enabled() and any(x.requires_grad for x in (q, k, norm.q_weight, norm.k_weight)):
+            if _C.is_grad_enabled() and (q.requires_grad or k.requires_grad or norm.q_weight.requires_grad or norm.k_weight.requires_grad):
                 if q_out is not None or k_out is not None:
                     raise ValueError("q_out and k_out take no part in gradients: leave them out, or call under no_grad")
                 if not (q.is_floating_point() and k.is_floating_point()):
                     raise ValueError("bit patterns have no gradients: give bf16 or fp32")
-                return _norm_turn()(q, k, norm.q_weight, norm.k_weight, positions, self, norm.eps)
+                return _norm_turn()(q, k, norm.q_weight, norm.k_weight, positions, self, norm)
         if (q.requires_grad or k.requires_grad) and _C.is_grad_enabled():
             if q_out is not None or k_out is not None:
                 raise ValueError("q_out and k_out take no part in gradients: leave them out, or call under no_grad")
@@ -433,36 +435,40 @@ class Rotary:
     def _norm_grad(self, q, k, qw, kw, eps, positions, gq, gk, want_qw, want_kw):
         """The gradients (q, k, q_weight, k_weight) of rotate(norm=) for those of its outputs (None: of an output that
         nothing depends on, whose inputs get None)."""
-        import torch
-        have = gq is not None, gk is not None
-        if not any(have):
+        have_q, have_k = gq is not None, gk is not None
+        if not (have_q or have_k):
             return (None,) * 4
-        xs = [x if h else x[:, :0] for x, h in zip((q, k), have)]
-        gs = [(g if g.stride(2) == 1 else g.contiguous()) if h else x for g, x, h in zip((gq, gk), xs, have)]
-        n, hq, hk, wide, strides, axis_stride = self._args(*xs, None, positions)
-        sg = [self._tokens(g, "the gradient", n)[3] for g in gs]
+        if not have_q:
+            q = gq = q[:, :0]
+        if not have_k:
+            k = gk = k[:, :0]
+        if gq.stride(2) != 1:
+            gq = gq.contiguous()
+        if gk.stride(2) != 1:
+            gk = gk.contiguous()
+        n, hq, hk, wide, strides, axis_stride = self._args(q, k, None, positions)
+        sq, sk = self._tokens(gq, "the gradient", n)[3], self._tokens(gk, "the gradient", n)[3]
         d = self.head_dim
-        out = [x.new_empty(x.shape) for x in xs]
-        want = want_qw and have[0], want_kw and have[1]
-        dw = [torch.empty_like(w) if y else None for w, y in zip((qw, kw), want)]
-        wq, wk, w32 = HeadNorm(qw, kw, eps)._weights(self)
+        dq, dk = q.new_empty((n, hq, d)), k.new_empty((n, hk, d))
+        dqw = qw.new_empty(d) if want_qw and have_q else None
+        dkw = kw.new_empty(d) if want_kw and have_k else None
         if self._grad_fn is None:
             self._grad_fn = _entry("ea_hip_norm_rotary_grad")
-
-        def pack(partial):
-            return _GRAD.pack(n, hq, hk, d, self.rot_dim, self.axes, self.adjacent, 0, wide, wide, 0, self.scale, *strides, hq * d, d,
-                              hk * d, d, 0, 0, axis_stride, n, n, xs[0].data_ptr(), xs[1].data_ptr(), 0, positions.data_ptr(),
-                              self._half, self._axis, 0, 0, out[0].data_ptr(), out[1].data_ptr(), 0, gs[0].data_ptr(),
-                              gs[1].data_ptr(), sg[0][0], sg[0][1], sg[1][0], sg[1][1], wq, wk,
-                              *(0 if w is None else w.data_ptr() for w in dw), partial, w32, eps)
-
-        args, partial = pack(0), None
-        if any(want):
-            size = hip.load().ea_hip_norm_rotary_grad_size(hip.NormRotaryGradArgs.from_buffer_copy(args))
-            partial = torch.empty(size // 8, dtype=torch.float64, device=self.dev)
-            args = pack(partial.data_ptr())
-        _call(self._grad_fn, args, self._at, "ea_hip_norm_rotary_grad")
-        return (out[0] if have[0] else None, out[1] if have[1] else None, *dw)
+        partial = None
+        if dqw is not None or dkw is not None:
+            size = self._partial.get((hq, hk))
+            if size is None:  # as much as any number of tokens takes
+                most = hip.NormRotaryGradArgs()
+                most.r.num_tokens, most.r.num_q_heads, most.r.num_kv_heads, most.r.head_dim = (1 << 31) - 1, hq, hk, d
+                size = self._partial[hq, hk] = hip.load().ea_hip_norm_rotary_grad_size(most)
+            partial = self.half_turns.new_empty(size // 8)
+        _call(self._grad_fn, _GRAD.pack(
+            n, hq, hk, d, self.rot_dim, self.axes, self.adjacent, 0, wide, wide, 0, self.scale, *strides, hq * d, d, hk * d, d, 0, 0,
+            axis_stride, n, n, q.data_ptr(), k.data_ptr(), 0, positions.data_ptr(), self._half, self._axis, 0, 0, dq.data_ptr(),
+            dk.data_ptr(), 0, gq.data_ptr(), gk.data_ptr(), sq[0], sq[1], sk[0], sk[1], *_weights(self, qw, kw),
+            0 if dqw is None else dqw.data_ptr(), 0 if dkw is None else dkw.data_ptr(), 0 if partial is None else partial.data_ptr(),
+            qw.dtype is self._f32, eps), self._at, "ea_hip_norm_rotary_grad")
+        return dq if have_q else None, dk if have_k else None, dqw, dkw
 
     def _check_target(self, out, at, n, hk, e, st, in_place, pools, size):
         """append's q_out is q (in_place: rows in q's order), or shares no memory with the inputs (at addresses `at`,
