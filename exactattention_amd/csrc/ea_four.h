@@ -158,7 +158,9 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
     const int d = P.g.head_dim, dv = P.g.head_dim_v;
     const int wid = kv4_width(dv), ng = NG == 2 ? wid >> 5 : NG;  // V's channels in whole groups: NG, or 1 with NG = 2
 
-    const double t1 = u64_as_f64(EA_T1_BITS[tid]) * 8388608.0, t2 = u64_as_f64(EA_T2_BITS[tid]);  // 2^23: exact
+    S.T1[tid] = u64_as_f64(EA_T1_BITS[tid]) * 8388608.0;  // 2^23: exact
+    S.T2[tid] = u64_as_f64(EA_T2_BITS[tid]);
+    if (tid < 8) S.zero[tid] = 0;
     if (blockIdx.x == 0 && blockIdx.y == 0) {
         // on uniform splits the step's first kernel clears the tier-2 work list and chunk counts
         if (!P.dq_stream && tid < EA_T2_CNT) P.wl_cnt[tid] = 0;
@@ -168,7 +170,10 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
 
     // One piece: keys [kA, kB) of unit `item` (segment, row block), clipped to the unit's visible end, as partial slot `split`.
     auto piece = [&](const bool first, const int item, const int split, int kA, int kB) __attribute__((always_inline)) {
-        const int lane = tid & 63;
+        // what follows from the lane is found anew for every piece: kept over the pieces it spills, and a reload waits for the loads of
+        // the first tile
+        int lane = tid & 63;
+        asm volatile("" : "+v"(lane));
         const int g = lane >> 4, n = lane & 15;
         const int seg = item / P.nrb, rbk = item % P.nrb;
         const int Hkv = P.g.num_kv_heads;
@@ -307,11 +312,6 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
             issue_v(n0, p, vr);
         };
         if (nst > 0) begin(k0w);
-        if (first) {
-            S.T1[tid] = t1;
-            S.T2[tid] = t2;
-            if (tid < 8) S.zero[tid] = 0;
-        }
         // ---- q's digits: X = q / 2^lsb, |X| < 2^28, in 6 digits of 5 bits
 #pragma unroll
         for (int r4 = 0; r4 < RS; r4 += 4) {
@@ -943,10 +943,11 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
             const int ke = min(tm ? max(S.kvl[r], tb + 64 - (int)__clzll(tm)) : S.kvl[r], k1);
             const int nk = Rm == F4_NONE ? 0 : ke - kA;
             const double Z = (f[0] * S.wZ[0][r] + f[2] * S.wZ[2][r]) + (f[1] * S.wZ[1][r] + f[3] * S.wZ[3][r]);
-            // The depth that the combine multiplies by u Z max|v|: fp64 roundings (a key each, folds of 5, joins), and what the
+            // The depth that the combine multiplies by u Z max|v|. P.V: int32 sums are exact, a fold adds 4 numbers up, a pair of the
+            // exact path one (8 each), 16 for the joins. Z: 4 keys of every 256 are added up in a lane, 16 for the joins. What the
             // weights lost, at most 12 units of 2^(base + G) for each of theirs: max|v| is 12 units of the largest scale and G at
             // most a binade above it, so 2 lost / Z, in units of u
-            const double depth = (double)nk + 16.0 + 8.0 * (double)fo + (lost / Z) * (0x1p54 * (1.0 + 0x1p-20)) + 1.0;
+            const double depth = (double)(nk >> 6) + 40.0 + 8.0 * (double)fo + (lost / Z) * (0x1p54 * (1.0 + 0x1p-20)) + 1.0;
             int most = nk;
             if (nk > 0) {
                 if (!(depth < 0x1p28)) fl = 1;

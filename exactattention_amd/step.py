@@ -112,6 +112,14 @@ def _norm_turn():
     if _NORM_TURN is None:
         import torch
 
+        def gradient(ctx, gq, gk):
+            q, k, qw, kw, positions = ctx.saved_tensors
+            a, b, c, d = ctx.needs_input_grad[:4]
+            dq, dk, dqw, dkw = ctx.rotary._norm_grad(q, k, qw, kw, ctx.eps, positions, gq, gk, c, d)
+            return dq if a else None, dk if b else None, dqw, dkw, None, None, None
+
+        once = torch.autograd.function.once_differentiable(gradient)  # under create_graph
+
         class NormTurn(torch.autograd.Function):
             @staticmethod
             def forward(ctx, q, k, qw, kw, positions, rotary, norm):
@@ -125,12 +133,8 @@ def _norm_turn():
                 return out
 
             @staticmethod
-            @torch.autograd.function.once_differentiable
             def backward(ctx, gq, gk):
-                q, k, qw, kw, positions = ctx.saved_tensors
-                need = ctx.needs_input_grad
-                out = ctx.rotary._norm_grad(q, k, qw, kw, ctx.eps, positions, gq, gk, need[2], need[3])
-                return tuple(g if n else None for g, n in zip(out, need)) + (None,) * 3
+                return once(ctx, gq, gk) if _C.is_grad_enabled() else gradient(ctx, gq, gk)
 
         _NORM_TURN = NormTurn.apply
     return _NORM_TURN
