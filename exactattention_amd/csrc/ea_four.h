@@ -112,19 +112,19 @@ __device__ __forceinline__ uint32_t four_bytes(uint32_t w) {
     return __builtin_amdgcn_perm(P1, P0, x) ^ __builtin_amdgcn_perm(N1, N0, y);
 }
 
-// Certified weights of exact sums: w = RN24(2^t), t = RN32(x), x within p 2^-49 + adel of p = a xs: t is decided when both ends of
+// Certified weights of exact sums: w = RN24(2^t), t = RN32(x), x within |p| rel + adel of p = a xs: t is decided when both ends of
 // that interval round to it. |t| <= 2^-25 gives 1. 2^t from the tables and the cubic of pf::cert_pairs, with its bound: t is cut at
 // multiples of 2^-16 by an addition (of t - 2^-17, which is exact; a multiple may go down, and leaves r = 2^-16). w = Y 2^(fl - 23), Y in
 // 2^23 .. 2^24; not ok: left to the exact path.
 template <int NP>
-__device__ __forceinline__ void four_weights(const double (&xs)[NP], double a, double adel, const double* T1s, const double* T2, double (&Y)[NP],
+__device__ __forceinline__ void four_weights(const double (&xs)[NP], double a, double rel, double adel, const double* T1s, const double* T2, double (&Y)[NP],
                                              int (&fl)[NP], bool (&ok)[NP]) {
     const double c1 = u64_as_f64(EA_C_BITS[0]), c2 = u64_as_f64(EA_C_BITS[1]), c3 = u64_as_f64(EA_C_BITS[2]);
     constexpr double CUT = 0x1.8p36;
     double r[NP], aa[NP];
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-        const double p = a * xs[i], e = __fma_rn(fabs(p), 0x1p-49, adel);
+        const double p = a * xs[i], e = __fma_rn(fabs(p), rel, adel);
         const float lo = (float)(p - e), hi = (float)(p + e);
         ok[i] = (lo == hi) & (fabsf(hi) < 0x1p29f);
         const double t = (double)(fabsf(hi) <= 0x1p-25f ? 0.0f : hi);
@@ -594,7 +594,7 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
                     ex[i] -= base;
                 }
             } else {
-                four_weights<KL>(x, rq, adel, S.T1, S.T2, md, ex, ok);
+                four_weights<KL>(x, rq, 0x1p-49, adel, S.T1, S.T2, md, ex, ok);
 #pragma unroll
                 for (int i = 0; i < KL; ++i) ex[i] -= base + 23;
             }
@@ -615,6 +615,26 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
 #pragma unroll
             for (int i = 0; i < KL; ++i) all = all & ok[i];
             if (__ballot(!all) != 0) {
+                if constexpr (MOD < 2) {
+                    // A score of few bits may lie on a tie of t: 1 pair in 2^14 of normal q and K. Where the product is exact, too, it
+                    // rounds to even like any other
+#pragma unroll
+                    for (int i = 0; i < KL; ++i) {
+                        const bool tie = !two && !ok[i] && adel == 0.0 && __fma_rn(rq, x[i], -(rq * x[i])) == 0.0;
+                        if (__ballot(tie) != 0) {
+                            const double xt[1] = {x[i]};
+                            double yt[1];
+                            int ft[1];
+                            bool okt[1];
+                            four_weights<1>(xt, rq, 0.0, 0.0, S.T1, S.T2, yt, ft, okt);
+                            const bool take = tie && okt[0];
+                            ok[i] = ok[i] | take;
+                            md[i] = take ? yt[0] : md[i];
+                            ex[i] = take ? ft[0] - (base + 23) : ex[i];
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
                 uint32_t gd = 0;
 #pragma unroll
                 for (int i = 0; i < KL; ++i) gd |= ok[i] ? (1u << i) : 0u;
