@@ -77,7 +77,7 @@ struct FourSmem {
     float slope[RS];
     double wZ[4][RS], we[4][RS];
     int wR[4][RS], wf[4][RS], wn[4];
-    uint32_t wv[4][4];  // per wave and group: the largest scale
+    uint32_t wv[4][4];  // per wave and group: the reference, no key's scale is larger
     uint32_t list[4][F4_LIST + 64 * RS];
     double O[4][RS][32 * NG];  // per wave: of channel 32 l + 2 n + h at 32 l + 16 h + n
     union alignas(16) {
@@ -413,14 +413,10 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
         int base = F4_NONE;    // of the row
         double z = 0.0, lostw = 0.0;  // the weights' sum, and what rounding took from their whole numbers
         int G[NG];             // the groups' references, uniform
-        f4_h2 vm[NG];          // the largest scales the lane saw, of even and odd keys
 #pragma unroll
-        for (int l = 0; l < NG; ++l) {
-            G[l] = 0;
-            vm[l] = (f4_h2){0, 0};
-        }
+        for (int l = 0; l < NG; ++l) G[l] = 0;
         int lo = 120;          // scales of keys in [lo, lo + F4_SPREAD] need no closer look: at first 2^-7 .. 2^2
-        double kbnd = 6.0 * 0x1p2;  // an upper bound of |k| for such keys
+        int kexp = 2;          // 6 2^kexp bounds |k| of such keys
         f4_i4 acc[NMF][2 * NG];
         // the lane's own sums: [c], or with 2 rows those of c = 2 l + g % 2
         constexpr int OC = RS == 2 ? NG : 2 * NG, OS = RS == 2 ? 32 : 16;
@@ -521,8 +517,8 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
                         }
                     }
                     top = wave_max_dpp(top);
-                    if (top > 0) lo = max(top - (F4_SPREAD - 1), 40);
-                    kbnd = max(kbnd, 6.0 * ldexp(1.0, max(top, lo + F4_SPREAD) - 127));
+                    if (top > 0) lo = __builtin_amdgcn_readfirstlane(max(top - (F4_SPREAD - 1), 40));
+                    kexp = max(kexp, __builtin_amdgcn_readfirstlane(max(top, lo + F4_SPREAD)) - 127);
                 }
             }
             const bool edge = n0 + 64 > min(kvmin, k1) || (MOD && n0 < kbmax);
@@ -571,7 +567,7 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
             int ex[KL];
             constexpr uint32_t ALL = (1u << KL) - 1u;
             // ---- certified weights
-            const double adel = S.rqe[row] * kbnd, rq = S.rq[row];
+            const double adel = S.rqe[row] * ldexp(6.0, kexp), rq = S.rq[row];
             bool ok[KL];
             double x[KL];
 #pragma unroll
@@ -671,20 +667,21 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
             int most = ex[0];
 #pragma unroll
             for (int i = 1; i < KL; ++i) most = max(most, ex[i]);
+            f4_h2 top[NG];  // of the scales of even and odd keys
             uint32_t past = 0;
 #pragma unroll
             for (int l = 0; l < NG; ++l) {
                 const uint32_t x = vr.s[l];
-                vm[l] = pk_max(vm[l], pk_max(__builtin_bit_cast(f4_h2, x & 0x00FF00FFu), __builtin_bit_cast(f4_h2, x >> 8 & 0x00FF00FFu)));
+                top[l] = pk_max(__builtin_bit_cast(f4_h2, x & 0x00FF00FFu), __builtin_bit_cast(f4_h2, x >> 8 & 0x00FF00FFu));
                 const f4_h2 ref = __builtin_bit_cast(f4_h2, (uint32_t)G[l] * 0x10001u);
-                past |= __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(vm[l], ref));
+                past |= __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(top[l], ref));
             }
             if (__ballot(most > F4_BITS || past != 0) != 0 || since >= F4_EPOCH) {
                 if (since) fold();
 #pragma unroll
                 for (int l = 0; l < NG; ++l) {
-                    const int top = wave_max_dpp((int)max(vm[l].x, vm[l].y));
-                    G[l] = max(G[l], top >= G[l] ? min(top + 1, 255) : 0);  // one binade of room
+                    const int m = wave_max_dpp((int)max(top[l].x, top[l].y));
+                    G[l] = max(G[l], m >= G[l] ? min(m + 1, 255) : 0);  // one binade of room
                 }
                 int m = 0;
 #pragma unroll
@@ -855,11 +852,7 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
                     const int64_t vc = kv4_v(P, b, key, hk);
                     uint32_t v2[NG];
 #pragma unroll
-                    for (int l = 0; l < NG; ++l) {
-                        v2[l] = l < ng ? kv4_vload2(P.v, P.vs, vc, 32 * l + 2 * n) : 0u;
-                        // the scales that these sums met belong to the bound on |v|
-                        if (l < ng) vm[l] = pk_max(vm[l], (f4_h2){(P.vs + kv4_vscale(vc))[16 * l], 0});
-                    }
+                    for (int l = 0; l < NG; ++l) v2[l] = l < ng ? kv4_vload2(P.v, P.vs, vc, 32 * l + 2 * n) : 0u;
                     if (row == r) {
                         if (Er > base + F4_BITS) rebase(Er - (F4_BITS - F4_HEAD));
                         const int de = Er - base;
@@ -914,10 +907,8 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
             }
             if (lane == 0) S.wn[w] = folds;
 #pragma unroll
-            for (int l = 0; l < NG; ++l) {
-                const int top = wave_max_dpp((int)max(vm[l].x, vm[l].y));
-                if (lane == 0) S.wv[w][l] = (uint32_t)top;
-            }
+            for (int l = 0; l < NG; ++l)
+                if (lane == 0) S.wv[w][l] = (uint32_t)G[l];
         }
         __syncthreads();
         const int64_t pbase = (int64_t)split * P.rows;
@@ -965,9 +956,9 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
             const double Z = (f[0] * S.wZ[0][r] + f[2] * S.wZ[2][r]) + (f[1] * S.wZ[1][r] + f[3] * S.wZ[3][r]);
             // The depth that the combine multiplies by u Z max|v|. P.V: int32 sums are exact, a fold adds 4 numbers up, a pair of the
             // exact path one (8 each), 16 for the joins. Z: 4 keys of every 256 are added up in a lane, 16 for the joins. What the
-            // weights lost, at most 12 units of 2^(base + G) for each of theirs: max|v| is 12 units of the largest scale and G at
-            // most a binade above it, so 2 lost / Z, in units of u
-            const double depth = (double)(nk >> 6) + 40.0 + 8.0 * (double)fo + (lost / Z) * (0x1p54 * (1.0 + 0x1p-20)) + 1.0;
+            // weights lost, at most 12 units of 2^(base + G) for each of theirs, which the combine takes for max|v|: lost / Z, in
+            // units of u
+            const double depth = (double)(nk >> 6) + 40.0 + 8.0 * (double)fo + (lost / Z) * (0x1p53 * (1.0 + 0x1p-20)) + 1.0;
             int most = nk;
             if (nk > 0) {
                 if (!(depth < 0x1p28)) fl = 1;
