@@ -198,6 +198,28 @@ def test_streams_graphs_and_reuse(gpu):
         assert torch.equal(a.tokens, b.tokens) and torch.equal(a.path, b.path) and torch.equal(a.accepted, b.accepted)
 
 
+def test_calls_in_a_row(gpu):
+    """Many blocks a sequence, whose last one joins the sums, called again and again without a wait in between."""
+    import torch
+    rng = np.random.default_rng(11)
+    B, N, V = 48, 3, 40000
+    c = DraftCheck(B, N, V, "cuda:0")
+    sets, want = [], []
+    for _ in range(2):
+        p = oracle.softmax(rng, (B, N + 1, V), 2.5)
+        x = np.argsort(-p, -1)[:, :N, 0].copy()
+        u = rng.random((B, N + 1)).astype(np.float32)
+        want.append(_check(p, x, u))
+        sets.append((_cuda(p, np.float32), _cuda(x, np.int32), _cuda(u, np.float32)))
+    got = []
+    for i in range(200):
+        c.verify(*sets[i % 2])
+        got.append(torch.cat([c.accepted[:, None], c.path, c.tokens], 1))
+    for i, t in enumerate(got):
+        acc, path, tok = want[i % 2]
+        assert t.tolist() == [[a, *b, *d] for a, b, d in zip(acc, path, tok)], i
+
+
 def test_refusals(gpu):
     import torch
     for a in ((-1, 1, 5), (1, 65, 5), (1, 1, 0), (1, 1, (1 << 19) + 1), (65536, 1, 5)):

@@ -78,7 +78,7 @@ def test_rows_and_head_sizes(gpu, T, grp, d):
 @pytest.mark.parametrize("B,T,grp", [(70, 1, 8), (70, 9, 1), (40, 17, 1), (300, 1, 2)])
 @pytest.mark.parametrize("d", [64, 128])
 def test_wide_blocks_and_many_units(gpu, B, T, grp, d):
-    """Blocks of 8 and 16 rows, and grids past one round of blocks."""
+    """Segments of 8 to 17 rows, and grids past one round of blocks."""
     rng = np.random.default_rng(B + T + d)
     for S in (T, 65 + T, 200):
         _check(_problem(rng, B, T, 2 * grp, 2, S, d), "fp32" if S & 1 else "bf16")
@@ -315,3 +315,27 @@ def test_the_splits_do_not_change_a_bit(gpu):
         got, flags, _ = hip.attention_problem(pair[0], None, "fp32", splits, alpha_bits=default_alpha_bits(128), device="cuda:0")
         assert not flags.any() and (want is None or np.array_equal(got, want))
         want = got
+
+
+@pytest.mark.parametrize("T,grp", [(1, 2), (1, 4), (12, 2)])
+def test_logits_on_a_tie(gpu, T, grp):
+    """Scores of few bits: products with alpha that lie halfway between two fp32 numbers round to even, and no pair of them takes the
+    exact path."""
+    rng = np.random.default_rng(T + grp)
+    arrays = f4.random_pool(rng, 82, 2, 16, 128, 0, 0)
+    pair = _problem(rng, 2, T, 2 * grp, 2, 640, 128, arrays=arrays)
+    q = (rng.integers(-6, 7, pair[1]["q"].shape) / 4.0).astype(np.float32)
+    bits = (q.view(np.uint32) >> 16).astype(np.uint16)
+    for p in pair:
+        p["q"] = bits
+    ab = default_alpha_bits(128)
+    alpha = float(np.array([ab], np.uint32).view(np.float32)[0])
+    k = f4.values(arrays[0], arrays[1], 128)  # (pages, heads, slots, d)
+    s = np.einsum("bthd,phsd->bthps", q.reshape(2, T, 2, grp, 128)[:, :, :, 0], k)
+    p = alpha * s  # exact: 24 and 15 bits
+    f = p.astype(np.float32)
+    other = np.nextafter(f, np.where(p > f, np.inf, -np.inf).astype(np.float32))
+    ties = (p != f) & (p == (f.astype(np.float64) + other.astype(np.float64)) / 2)
+    assert ties.sum() > 50
+    st = _check(pair)
+    assert st["slow_path_scores"] == 0, st

@@ -395,3 +395,19 @@ def test_refusals(gpu):
     for bad in (dict(k=k[:, :, :32]), dict(v=v.bfloat16()), dict(k=k.double()), dict(k=k.cpu()), dict(dst_rows=dst[:3])):
         with pytest.raises(ValueError):
             pool.append(**{**dict(k=k, v=v, dst_rows=dst), **bad})
+
+
+def test_gradients_of_gradients_are_refused(gpu):
+    """create_graph gives the same first gradients; what would differentiate them raises."""
+    import torch
+    from exactattention_amd.step import HeadNorm, Rotary
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    q, k = (torch.randn((5, h, 64), device="cuda", generator=gen).requires_grad_() for h in (4, 2))
+    w = [(1 + 0.1 * torch.randn(64, device="cuda", generator=gen)).requires_grad_() for _ in range(2)]
+    rot, pos = Rotary(64), torch.arange(5, dtype=torch.int32, device="cuda")
+    loss = lambda: sum(x.square().sum() for x in rot.rotate(q, k, pos, norm=HeadNorm(*w, 1e-6)))  # noqa: E731
+    plain = torch.autograd.grad(loss(), (q, k, *w))
+    again = torch.autograd.grad(loss(), (q, k, *w), create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(plain, again))
+    with pytest.raises(RuntimeError):
+        again[0].sum().backward()
