@@ -21,12 +21,14 @@
 //
 // What bounds it is the VALU, and HBM where a block has 2 rows: of a tile of 64 keys and 4 rows 55 instructions for the scores, 135 for the
 // weights, 37 a group of 32 channels for their digits and 44 for V's bytes; 2 waves a SIMD (the int32 sums alone are 64 registers; 8 rows
-// took 96, spilled, and then waited for every load: a 1500-token chunk 770 us, 680 with 4). A step of 32 ragged sequences to 4096 keys,
-// 32/8 heads: 66 us, 69 on the fp64 matrix instructions; 8 of 30000 to 131072, 16/8 heads: 182 (4.5 TB/s), 437.
+// a wave took 96, spilled, and then waited for every load: a 1500-token chunk 770 us, 680 with 4). A step of 32 ragged sequences to
+// 4096 keys, 32/8 heads: 60 us, 69 on the fp64 matrix instructions; 8 of 30000 to 131072, 16/8 heads: 176 (4.6 TB/s), 437; a chunk of
+// 1500 tokens behind 2500, 16/8 heads: 580, 718.
 //
-// Layout. A block is 4 waves over one (segment, block of RS = 2 or 4 rows, key range); wave w takes 64-key tiles w, w + 4, .. and
-// meets the others in the epilogue only. Lane l: g = l / 16, n = l % 16; its pairs are those of its row, with the keys 4 n + u (u =
-// 0..3) of the tile: row g, or of 2 rows row g / 2 and half of the keys.
+// Layout. A block is 4 waves over one (segment, block of rows, key range). WR = 1: RS = 2 or 4 rows, wave w takes 64-key tiles w, w +
+// 4, .. and meets the others in the epilogue only. WR = 4: 16 rows, a wave takes 4 of them and every tile. Lane l: g = l / 16, n = l % 16;
+// its pairs are those of its row, with the keys 4 n + u (u = 0..3) of the tile: row g of the wave's, or of 2 rows row g / 2 and half of the
+// keys.
 //   q     digits in registers, the A operand (M = a row's digit, K = dim): with M = 4 g + i in the order of the rows, the 4 sums of
 //         D that a lane gets are digits of its own row: 2 instructions a key of 4 rows, and nothing passes between lanes; 1 of 2
 //         rows, whose lanes swap halves
@@ -65,16 +67,17 @@ typedef uint32_t f4_u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t f4_u2 __attribute__((ext_vector_type(2)));
 typedef unsigned short f4_h2 __attribute__((ext_vector_type(2)));
 
-template <int RS, int NG>
+template <int RS, int NG, int WR>
 struct FourSmem {
-    uint32_t q6[2][RS * 6 * 24];  // q's digits [row][digit][32-dim block][6 dwords], and those of what they leave
+    static constexpr int RB = RS * WR;  // rows of the block
+    uint32_t q6[2][RB * 6 * 24];  // q's digits [row][digit][32-dim block][6 dwords], and those of what they leave
     uint32_t zero[8];
     double T1[256], T2[256];  // exp2 tables, T1 times 2^23
-    double rq[RS], rqe[RS];   // alpha 2^(lsb + 3); |alpha| times the sum of |q| that both rounds lost
-    int bad[RS], more[RS], kvl[RS];
-    uint64_t tmk[RS];
-    int kvb[RS], pos[RS];  // with score modifications
-    float slope[RS];
+    double rq[RB], rqe[RB];   // alpha 2^(lsb + 3); |alpha| times the sum of |q| that both rounds lost
+    int bad[RB], more[RB], kvl[RB];
+    uint64_t tmk[RB];
+    int kvb[RB], pos[RB];  // with score modifications
+    float slope[RB];
     double wZ[4][RS], we[4][RS];
     int wR[4][RS], wf[4][RS], wn[4];
     uint32_t wv[4][4];  // per wave and group: the reference, no key's scale is larger
@@ -82,7 +85,7 @@ struct FourSmem {
     double O[4][RS][32 * NG];  // per wave: of channel 32 l + 2 n + h at 32 l + 16 h + n
     union alignas(16) {
         uint32_t W[4][NG][6 * RS * F4_WROW];
-        uint8_t dig[2][RS * 6 * 128];
+        uint8_t dig[2][RB * 6 * 128];
     };
 };
 
@@ -146,11 +149,13 @@ __device__ __forceinline__ void four_weights(const double (&xs)[NP], double a, d
 
 // MOD: with score modifications (ea_mod.h): 1 key ranges alone, 2 with a bias, 3 with a cap; a unit's key range is then counted from its
 // rows' first visible key, down to a whole tile, and on uniform splits the last split takes every key past the others.
-template <int RS, int NG, int MOD>
+template <int RS, int NG, int MOD, int WR>
 __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Params P) {
     constexpr int KL = RS;               // keys of a lane
     constexpr int NMF = RS == 2 ? 1 : 2;  // matrix instructions for 6 digits of the rows
-    typedef FourSmem<RS, NG> Smem;
+    constexpr int RB = RS * WR;           // rows of the block
+    constexpr int STEP = WR == 1 ? 256 : 64;  // from a wave's tile to its next
+    typedef FourSmem<RS, NG, WR> Smem;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     Smem& S = *reinterpret_cast<Smem*>(smem_raw);
     const int tid = (int)threadIdx.x;
@@ -178,16 +183,17 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
         const int seg = item / P.nrb, rbk = item % P.nrb;
         const int Hkv = P.g.num_kv_heads;
         const int b = seg / Hkv, hk = seg % Hkv;
-        const int row0 = rbk * RS;
-        const int nrow = min(RS, P.r_seg - row0);
+        const int row0 = rbk * RB;
+        const int nrow = min(RB, P.r_seg - row0);
+        const int wrow = WR == 1 ? 0 : RS * w;  // the first of the wave's rows
         auto q_row = [&](int r) __attribute__((always_inline)) {
             const int lr = row0 + r, t = lr / P.grp, gi = lr % P.grp;
             return P.q + (int64_t)b * P.g.q_seq_stride + (int64_t)t * P.g.q_tok_stride + (int64_t)(hk * P.grp + gi) * P.g.q_head_stride;
         };
         // what the digits are cut from, requested before anything waits
-        uint32_t qv[(RS + 3) / 4][2];
+        uint32_t qv[(RB + 3) / 4][2];
 #pragma unroll
-        for (int r4 = 0; r4 < RS; r4 += 4)
+        for (int r4 = 0; r4 < RB; r4 += 4)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int i = 2 * lane + h;
@@ -200,7 +206,7 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
         int kend = 0, kvmin = INT_MAX;
         int kbeg = INT_MAX, kbmax = 0;  // MOD: the rows' first visible key, their last prefix start
         {
-            const int r = lane & (RS - 1);
+            const int r = lane & (RB - 1);
             const int tok = b * P.g.num_tokens + (row0 + min(r, nrow - 1)) / P.grp;
             const int kvl = P.kv_len[tok];
             const uint64_t tmk = P.tree_mask ? P.tree_mask[tok] : 0ull;
@@ -212,14 +218,14 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
                 const KeySpan ks = key_span(kvb, kvl, slen, tmk, tb);
                 kbeg = ks.beg;
                 kend = ks.end;
-                if (w == 0 && lane < RS) {
+                if (w == 0 && lane < RB) {
                     S.kvb[r] = kvb;
                     S.pos[r] = mod_pos(P, tok, kvl);
                     const int lr = row0 + min(r, nrow - 1);
                     S.slope[r] = mod_slope(P, hk * P.grp + lr % P.grp);
                 }
             }
-            if (w == 0 && lane < RS) {
+            if (w == 0 && lane < RB) {
                 S.kvl[r] = r < nrow ? kvl : INT_MIN;
                 S.tmk[r] = r < nrow ? tmk : 0ull;
             }
@@ -234,8 +240,8 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
             kB += k0;
         }
         const int k1 = min(kB, kend);
-        const int k0w = kA + 64 * w;  // this wave's tiles: k0w + 256 it
-        const int nst = k1 > k0w ? (k1 - k0w + 255) >> 8 : 0;
+        const int k0w = WR == 1 ? kA + 64 * w : kA;  // this wave's tiles: k0w + STEP it
+        const int nst = k1 > k0w && wrow < nrow ? (k1 - k0w + STEP - 1) / STEP : 0;
         const int row = RS == 2 ? g >> 1 : g;       // the lane's row
         const int sub = RS == 2 ? 2 * (g & 1) : 0;  // its keys of a tile: 4 n + sub + i
         constexpr int RLANES = RS == 2 ? 32 : 16;   // lanes of a row
@@ -307,16 +313,16 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
         Pages nx = {0, 0};  // of the next tile
         auto begin = [&](int n0) __attribute__((always_inline)) {
             const Pages p = pages_of(n0);
-            nx = pages_of(n0 + 256);
+            nx = pages_of(n0 + STEP);
             issue_k(n0, p, kr);
             issue_v(n0, p, vr);
         };
         if (nst > 0) begin(k0w);
         // ---- q's digits: X = q / 2^lsb, |X| < 2^28, in 6 digits of 5 bits
 #pragma unroll
-        for (int r4 = 0; r4 < RS; r4 += 4) {
+        for (int r4 = 0; r4 < RB; r4 += 4) {
             const int r = r4 + w;
-            if (r >= RS) break;
+            if (r >= RB) break;
             int m[2] = {0, 0}, e[2] = {0, 0}, bad = 0, lead = INT_MIN;
             if (r < nrow) {
 #pragma unroll
@@ -378,12 +384,15 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
             }
         }
         __syncthreads();  // the digits are in LDS: 32 of a block to 24 bytes
-        int two = 0;  // does a row of the block need the second round?
+        int any = 0, two = 0;  // does a row of the block, of the wave, need the second round?
 #pragma unroll
-        for (int r = 0; r < RS; ++r) two |= S.more[r];
+        for (int r = 0; r < RB; ++r) any |= S.more[r];
+#pragma unroll
+        for (int r = 0; r < RS; ++r) two |= S.more[wrow + r];
+        any = __builtin_amdgcn_readfirstlane(any);
         two = __builtin_amdgcn_readfirstlane(two);
-        for (int x0 = tid; x0 < RS * 24 * (1 + two); x0 += F4_THREADS) {
-            const int k2 = x0 >= RS * 24, x = x0 - (k2 ? RS * 24 : 0);
+        for (int x0 = tid; x0 < RB * 24 * (1 + any); x0 += F4_THREADS) {
+            const int k2 = x0 >= RB * 24, x = x0 - (k2 ? RB * 24 : 0);
             const uint32_t* src = (const uint32_t*)&S.dig[k2][(x >> 2) * 128 + 32 * (x & 3)];
             uint32_t c[8];
 #pragma unroll
@@ -400,7 +409,7 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
         // the lane's part of a row block's digits, instruction j: M = n is digit 4 j + n % 4 of the digits of the rows of n / 4
         auto q_part = [&](int k2, int j) __attribute__((always_inline)) {
             const int c = RS == 2 ? n & 7 : 4 * j + (n & 3);
-            const int qr = RS == 2 ? n >> 3 : n >> 2;
+            const int qr = wrow + (RS == 2 ? n >> 3 : n >> 2);
             const uint32_t* const p = c >= 6 ? S.zero : &S.q6[k2][((qr * 6 + c) * 4 + g) * 6];
             const f4_u2 x = *(const f4_u2*)p, y = *(const f4_u2*)(p + 2), t = *(const f4_u2*)(p + 4);
             return (f4_i8){(int)x.x, (int)x.y, (int)y.x, (int)y.y, (int)t.x, (int)t.y, 0, 0};
@@ -409,7 +418,7 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
 #pragma unroll
         for (int j = 0; j < NMF; ++j) qd[j] = q_part(0, j);
         const double alpha = P.alpha;
-        int rfl = S.bad[row];  // the row is left to tier 2
+        int rfl = S.bad[wrow + row];  // the row is left to tier 2
         int base = F4_NONE;    // of the row
         double z = 0.0, lostw = 0.0;  // the weights' sum, and what rounding took from their whole numbers
         int G[NG];             // the groups' references, uniform
@@ -489,7 +498,7 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
         };
 
         auto tile = [&](int n0) __attribute__((always_inline)) {
-            const Pages after = pages_of(n0 + 512);
+            const Pages after = pages_of(n0 + 2 * STEP);
             // ---- are the scales near enough to each other for exact sums?
             uint32_t wide = 0;  // bit u: key 4 n + u is left to the exact path
             {
@@ -562,12 +571,12 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
 #pragma unroll
                 for (int i = 0; i < KL; ++i) sc[i] = __fma_rn(s2[i], 0x1p-28, sc[i]);  // one rounding, in the weights' bound
             }
-            issue_k(n0 + 256, nx, kr);
+            issue_k(n0 + STEP, nx, kr);
             double md[KL];  // the weights: md 2^(base + ex)
             int ex[KL];
             constexpr uint32_t ALL = (1u << KL) - 1u;
             // ---- certified weights
-            const double adel = S.rqe[row] * ldexp(6.0, kexp), rq = S.rq[row];
+            const double adel = S.rqe[wrow + row] * ldexp(6.0, kexp), rq = S.rq[wrow + row];
             bool ok[KL];
             double x[KL];
 #pragma unroll
@@ -578,8 +587,8 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
                 double ad[KL];
 #pragma unroll
                 for (int i = 0; i < KL; ++i) {
-                    sl[i] = S.slope[row];
-                    dist[i] = kn + i - S.pos[row];
+                    sl[i] = S.slope[wrow + row];
+                    dist[i] = kn + i - S.pos[wrow + row];
                     ad[i] = __fma_rn(fabs(x[i] * rq), 0x1p-52, adel);
                 }
                 pf::cert_pairs<KL, MOD>(x, ad, rq, S.T1, S.T2, Mi, ex, ok, P.cap, sl, dist);
@@ -601,9 +610,9 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
 #pragma unroll
                 for (int i = 0; i < KL; ++i) {
                     const int key = kn + i, ti = key - tb;
-                    const bool in = ((unsigned)ti < 64u) & (((S.tmk[row] >> (ti & 63)) & 1ull) != 0);
-                    bool pre = key < S.kvl[row];
-                    if constexpr (MOD) pre = pre & (key >= S.kvb[row]);
+                    const bool in = ((unsigned)ti < 64u) & (((S.tmk[wrow + row] >> (ti & 63)) & 1ull) != 0);
+                    bool pre = key < S.kvl[wrow + row];
+                    if constexpr (MOD) pre = pre & (key >= S.kvb[wrow + row]);
                     vis |= ((key < k1) & (pre | in)) ? (1u << i) : 0u;
                 }
             }
@@ -635,7 +644,7 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
 #pragma unroll
                 for (int i = 0; i < KL; ++i) gd |= ok[i] ? (1u << i) : 0u;
                 gd &= ~wide;
-                const uint32_t slow = row < nrow ? vis & ~gd : 0u;
+                const uint32_t slow = wrow + row < nrow ? vis & ~gd : 0u;
                 gd &= vis;
                 if (__builtin_expect(__ballot(slow != 0) != 0, 0)) {
                     // undecided pairs wait in the wave's list for flush(); a row that is flagged already needs no more of them
@@ -697,8 +706,8 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
                 }
             }
             ++since;
-#pragma unroll
-            for (int i = 0; i < KL; ++i) z += ldexp(md[i], ex[i]);
+            if constexpr (KL == 2) z += ldexp(md[0], ex[0]) + ldexp(md[1], ex[1]);
+            else z += (ldexp(md[0], ex[0]) + ldexp(md[1], ex[1])) + (ldexp(md[KL - 2], ex[KL - 2]) + ldexp(md[KL - 1], ex[KL - 1]));
             // ---- P.V: a phase writes the digits of its groups and reads them back; the next one writes them anew (a wave's LDS
             // accesses keep their order)
             auto digits = [&](const int l) __attribute__((always_inline)) {
@@ -773,7 +782,7 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
             for (int l = 0; l < NG; ++l)
                 if (l < ng) multiply(l);
             __builtin_amdgcn_sched_barrier(0);
-            issue_v(n0 + 256, nx, vr);
+            issue_v(n0 + STEP, nx, vr);
             nx = after;
             __builtin_amdgcn_sched_barrier(0);
         };
@@ -791,7 +800,7 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
                 const int er = (int)(en >> 29), ek = kA + (int)(en & 0x1FFFFFFFu);
                 double ss = 0.0, es = 0.0, ea = 0.0;
                 if (have && 8 * n < d) {
-                    const uint16_t* qr = q_row(er) + 8 * n;
+                    const uint16_t* qr = q_row(wrow + er) + 8 * n;
                     const uint4 kv = kv4_load8(P.k, P.ks, kv_off(P, b, ek, hk, 0) + 8 * n);
                     const uint32_t wd[4] = {kv.x, kv.y, kv.z, kv.w};
                     uint32_t qw[8];
@@ -824,7 +833,7 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
                         const bool zero = ss == 0.0 && es == 0.0 && ea == 0.0;
                         ls = zero ? 1 : logit_cert(alpha, ss, es, ea * 0x1p-44, &tbits);
                         if (ls == 1) tbits = 0;
-                        if constexpr (MOD >= 2) ls = mod_logit(ls, zero, P.cap, S.slope[er], ek - S.pos[er], S.T1, 23, &tbits);
+                        if constexpr (MOD >= 2) ls = mod_logit(ls, zero, P.cap, S.slope[wrow + er], ek - S.pos[wrow + er], S.T1, 23, &tbits);
                     }
                     if (ls == 2 || ls == 3) {
                         why = 1;  // undecided, or an overflow (tier 2 reports the domain error)
@@ -881,11 +890,11 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
         // pages are looked up a tile before that. A flush (rare) drops the loads in flight and starts over
         for (int it = 0; it < nst;) {
 #pragma unroll 1
-            for (; it < nst && cnt < F4_LIST; ++it) tile(k0w + 256 * it);
+            for (; it < nst && cnt < F4_LIST; ++it) tile(k0w + STEP * it);
             if (since) fold();
             if (cnt > 0) {
                 flush();
-                if (it < nst) begin(k0w + 256 * it);
+                if (it < nst) begin(k0w + STEP * it);
             }
         }
 
@@ -912,8 +921,10 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
         }
         __syncthreads();
         const int64_t pbase = (int64_t)split * P.rows;
-        auto sums_at = [&](int r, double (&f)[4]) __attribute__((always_inline)) {  // the waves' factors to the largest base
+        // WR = 1: the waves' factors to the row's largest base; otherwise one wave has it
+        auto sums_at = [&](int r, double (&f)[4]) __attribute__((always_inline)) {
             int Rm = F4_NONE, far = 0;
+            if constexpr (WR > 1) return S.wR[r / RS][r % RS];
             for (int ww = 0; ww < 4; ++ww) Rm = max(Rm, S.wR[ww][r]);
 #pragma unroll
             for (int ww = 0; ww < 4; ++ww) {
@@ -929,11 +940,12 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
             const int r = x / (16 * NG), p = x % (16 * NG), l = p >> 4, c = p & 15;
             if (2 * p >= dv) continue;
             double f[4], o[2];
-            sums_at(r, f);
+            if constexpr (WR == 1) sums_at(r, f);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int at = 32 * l + 16 * h + c;
-                o[h] = (f[0] * S.O[0][r][at] + f[2] * S.O[2][r][at]) + (f[1] * S.O[1][r][at] + f[3] * S.O[3][r][at]);
+                if constexpr (WR > 1) o[h] = S.O[r / RS][r % RS][at];
+                else o[h] = (f[0] * S.O[0][r][at] + f[2] * S.O[2][r][at]) + (f[1] * S.O[1][r][at] + f[3] * S.O[3][r][at]);
             }
             const int lr = row0 + r;
             const int64_t gr = row_index(P, b, lr / P.grp, hk * P.grp + lr % P.grp);
@@ -944,18 +956,26 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
             double f[4], lost = 0.0;
             const int Rm = sums_at(r, f);
             int fl = Rm == INT_MIN, fo = 0;
-            for (int ww = 0; ww < 4; ++ww) {
-                fl |= S.wf[ww][r];
-                fo += S.wn[ww];
-                lost += f[ww] * S.we[ww][r];
+            double Z = 0.0;
+            if constexpr (WR > 1) {
+                fl |= S.wf[r / RS][r % RS];
+                fo = S.wn[r / RS];
+                lost = S.we[r / RS][r % RS];
+                Z = S.wZ[r / RS][r % RS];
+            } else {
+                for (int ww = 0; ww < 4; ++ww) {
+                    fl |= S.wf[ww][r];
+                    fo += S.wn[ww];
+                    lost += f[ww] * S.we[ww][r];
+                }
+                Z = (f[0] * S.wZ[0][r] + f[2] * S.wZ[2][r]) + (f[1] * S.wZ[1][r] + f[3] * S.wZ[3][r]);
             }
             // keys of the piece up to the row's last visible one: at least the keys summed
             const uint64_t tm = S.tmk[r];
             const int ke = min(tm ? max(S.kvl[r], tb + 64 - (int)__clzll(tm)) : S.kvl[r], k1);
             const int nk = Rm == F4_NONE ? 0 : ke - kA;
-            const double Z = (f[0] * S.wZ[0][r] + f[2] * S.wZ[2][r]) + (f[1] * S.wZ[1][r] + f[3] * S.wZ[3][r]);
             // The depth that the combine multiplies by u Z max|v|. P.V: int32 sums are exact, a fold adds 4 numbers up, a pair of the
-            // exact path one (8 each), 16 for the joins. Z: 4 keys of every 256 are added up in a lane, 16 for the joins. What the
+            // exact path one (8 each), 16 for the joins. Z: one sum for every 64 keys in a lane at most, 16 for the joins. What the
             // weights lost, at most 12 units of 2^(base + G) for each of theirs, which the combine takes for max|v|: lost / Z, in
             // units of u
             const double depth = (double)(nk >> 6) + 40.0 + 8.0 * (double)fo + (lost / Z) * (0x1p53 * (1.0 + 0x1p-20)) + 1.0;

@@ -6,32 +6,33 @@
 
 namespace {
 
-// MOD: Params::mods, 0 the plain kernel; NG: V's groups of 32 channels, 2 also for 1
-template <int RS, int NG>
-const void* four_fn(int mod) {
-    return mod == 3 ? (const void*)ea_four<RS, NG, 3> : (mod == 2 ? (const void*)ea_four<RS, NG, 2>
-                                                                  : (mod ? (const void*)ea_four<RS, NG, 1> : (const void*)ea_four<RS, NG, 0>));
-}
+// MOD: Params::mods, 0 the plain kernel; NG: V's groups of 32 channels, 2 also for 1; WR: waves with rows of their own
 struct Four {
     const void* fn;
     size_t lds;
 };
-template <int RS>
-Four four_of(int ng, int mod) {
-    return ng == 4 ? Four{four_fn<RS, 4>(mod), sizeof(FourSmem<RS, 4>)}
-                   : (ng == 3 ? Four{four_fn<RS, 3>(mod), sizeof(FourSmem<RS, 3>)} : Four{four_fn<RS, 2>(mod), sizeof(FourSmem<RS, 2>)});
+template <int RS, int NG, int WR>
+Four four_of(int mod) {
+    const void* const fn[4] = {(const void*)ea_four<RS, NG, 0, WR>, (const void*)ea_four<RS, NG, 1, WR>, (const void*)ea_four<RS, NG, 2, WR>,
+                               (const void*)ea_four<RS, NG, 3, WR>};
+    return {fn[mod], sizeof(FourSmem<RS, NG, WR>)};
 }
-Four four_of(int rs, int ng, int mod) { return rs == 2 ? four_of<2>(ng, mod) : four_of<4>(ng, mod); }
+template <int RS, int WR>
+Four four_of(int ng, int mod) {
+    return ng == 4 ? four_of<RS, 4, WR>(mod) : (ng == 3 ? four_of<RS, 3, WR>(mod) : four_of<RS, 2, WR>(mod));
+}
+constexpr int FOUR_RB[3] = {2, 4, 16};  // row blocks
+Four four_of(int rb, int ng, int mod) { return rb == 2 ? four_of<2, 1>(ng, mod) : (rb == 4 ? four_of<4, 1>(ng, mod) : four_of<4, 4>(ng, mod)); }
 int four_ng(const Params& P) { return std::max(2, (P.g.head_dim_v + 31) >> 5); }
 Four four_of(const Params& P) { return four_of(P.rb, four_ng(P), P.mods); }
 hipError_t four_attrs() {
     static std::once_flag once;
     static hipError_t err = hipSuccess;
     std::call_once(once, [] {
-        for (int rs = 2; rs <= 4; rs *= 2)
+        for (int rb : FOUR_RB)
             for (int ng = 2; ng <= 4; ++ng)
                 for (int mod = 0; mod < 4; ++mod) {
-                    const Four f = four_of(rs, ng, mod);
+                    const Four f = four_of(rb, ng, mod);
                     const hipError_t e = hipFuncSetAttribute(f.fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)f.lds);
                     if (e != hipSuccess) err = e;
                 }
@@ -51,13 +52,13 @@ int ea::ea_four_eligible(const Params& P) {
 int ea::ea_four_slots(const Params& P, int* slots) {
     // blocks resident on the current device at once, cached per device and kernel
     static std::mutex mu;
-    static int cache[64][24] = {};
+    static int cache[64][36] = {};
     hipError_t e = four_attrs();
     if (e != hipSuccess) return -100 - (int)e;
     int dev = 0;
     if ((e = hipGetDevice(&dev)) != hipSuccess) return -100 - (int)e;
     const Four f = four_of(P);
-    const int ki = (P.rb == 2 ? 0 : 1) + 2 * (four_ng(P) - 2) + 6 * P.mods;
+    const int ki = (P.rb == 2 ? 0 : (P.rb == 4 ? 1 : 2)) + 3 * (four_ng(P) - 2) + 9 * P.mods;
     std::lock_guard<std::mutex> lk(mu);
     if (dev < 0 || dev >= 64) return -1;
     if (!cache[dev][ki]) {

@@ -1687,7 +1687,13 @@ int make_plan(const ea_geometry* g, const ea_options* o, Plan* pl, const ea_scor
     gen.dq = d128 && !m && dq_fits(gen.nrb);
     Tier1& mr = pl->mr;
     mr.rb = m && pl->prefill ? 0 : mrow_rows(g, o, pl->r_seg, m != nullptr || kv4);
-    if (kv4 && mr.rb) mr.rb = pl->r_seg <= 2 ? 2 : 4;  // ea_four's row blocks
+    // ea_four's row blocks: 16, a wave for every 4 rows, where they are three quarters full or more and fill a round of 2 a CU: fewer
+    // pieces, each read by one block (a 1500-token chunk of 16/8 heads, 1504 blocks: 660 us with 4 rows, 580 with 16). Fewer
+    // blocks split their keys more often (8 drafted tokens of 8 x 16K, 64 units: 118 and 130).
+    if (kv4 && mr.rb) {
+        const int nb = (pl->r_seg + 15) / 16;
+        mr.rb = pl->r_seg <= 2 ? 2 : (4 * pl->r_seg >= 48 * nb && (int64_t)pl->nseg * nb >= 512 ? 16 : 4);
+    }
     pl->mrow = mr.rb > 0;
     const size_t without = lay_out(pl, g, o, false, m != nullptr);
     if (!pl->mrow) return 0;
@@ -1698,7 +1704,7 @@ int make_plan(const ea_geometry* g, const ea_options* o, Plan* pl, const ea_scor
     // segments of 100 keys 32.7 -> 25.8 us a step (29.5 on ea_decode), of 1000 33.2 -> 27.0; one of 16K 58.7
     // -> 41.0 (56.4); 8 rows, 8 -> 4: 8 segments of 2000 keys 30.2 -> 28.3. Past it they only read K and V
     // more often: 8 segments of 16K keys 63 -> 74.
-    while (mr.rb > 4) {
+    while (mr.rb > 4 && !kv4) {
         Tier1 half = mr;
         half.rb = mr.rb / 2;
         half.nrb = (pl->r_seg + half.rb - 1) / half.rb;

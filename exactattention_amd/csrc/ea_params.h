@@ -288,7 +288,7 @@ int ea_launch_decode(const Params& P, hipStream_t st);
 // same three questions as for the decode kernel.
 int ea_mrow_eligible(const Params& P);
 int ea_mrow_slots(const Params& P, int* slots);
-// The split kernel of 4-bit caches (ea_four.h): row blocks of P.rb = 2 or 4. The same three questions.
+// The split kernel of 4-bit caches (ea_four.h): row blocks of P.rb = 2, 4 or 16. The same three questions.
 int ea_four_eligible(const Params& P);
 int ea_four_slots(const Params& P, int* slots);
 int ea_launch_four(const Params& P, hipStream_t st);

@@ -92,6 +92,17 @@ def test_prompt_chunks(gpu, T, d):
         _check(_problem(rng, 2, T, 4, 2, S, d))
 
 
+@pytest.mark.parametrize("B,T,Hkv,grp", [(32, 64, 8, 4), (64, 13, 8, 1), (130, 31, 4, 1)])
+@pytest.mark.parametrize("d", [64, 96, 128])
+def test_waves_with_rows_of_their_own(gpu, B, T, Hkv, grp, d):
+    """Blocks of 16 rows: full ones, ones of 13 rows whose last wave has one, a second one of 15; keys that end inside tiles, and
+    sequences that end inside the prompt."""
+    rng = np.random.default_rng(B + T + d)
+    S = T + 90
+    kv = np.minimum(np.broadcast_to(S - T + 1 + np.arange(T), (B, T)), rng.integers(0, S + 1, (B, 1)))
+    _check(_problem(rng, B, T, Hkv * grp, Hkv, S, d, 32, kv_len=kv))
+
+
 @pytest.mark.parametrize("T", [2, 64])
 def test_scales_far_apart(gpu, T):
     """Groups 2^60 apart, beyond what the sums hold exactly, subnormal values, and groups of zeros."""
