@@ -211,6 +211,21 @@ def test_score_modifications(gpu, name, T, d):
     assert not flags.any() and not wf.any() and np.array_equal(got, want)
 
 
+@pytest.mark.parametrize("name", sorted(MODS))
+@pytest.mark.parametrize("B,T,Hkv,grp,d", [(16, 64, 4, 2, 128), (80, 14, 8, 1, 64), (6, 90, 6, 4, 96)])
+def test_score_modifications_in_wide_blocks(gpu, name, B, T, Hkv, grp, d):
+    """Blocks of 16 rows, whose key range counts from their first visible key."""
+    rng = np.random.default_rng(B + T + d)
+    m = dict(MODS[name])
+    if m.get("slopes"):
+        m["slopes"] = (1.4426950408889634 * 2.0 ** (-2.0 * (np.arange(Hkv * grp) % 4 + 1))).astype(np.float32)
+    a, b = _problem(rng, B, T, Hkv * grp, Hkv, T + 170, d, qscale=2.0)
+    ab = default_alpha_bits(d)
+    want, wf, _ = hip.attention_problem(b, None, alpha_bits=ab, kernel="general", mods=hip.ScoreMods(**m), device="cuda:0")
+    got, flags, _ = hip.attention_problem(a, None, alpha_bits=ab, mods=hip.ScoreMods(**m), device="cuda:0")
+    assert not flags.any() and not wf.any() and np.array_equal(got, want)
+
+
 @pytest.mark.parametrize("T,d", [(1, 128), (4, 72), (64, 128)])
 def test_the_other_tiers(gpu, T, d):
     """Every row through the device's second tier, and through the host's exact one."""
