@@ -5,7 +5,7 @@
 // the one behind the last node that stands is read whole, with the draft's row at a rejection. What bounds it is latency: one launch,
 // gridDim.x blocks a sequence. Each of them walks the nodes by itself (one wave, a lane a node), sums the weights of its part of the
 // vocabulary and leaves the sum; the last one to do so finds the part that holds the new token, and the token in it.
-// A chain of 4 over 32000 tokens 7.4 us, 64 chains of 8 over 128000 23 (65 MB, 13 at the copy rate), 16 trees of 16 over 50021 9.
+// A chain of 4 over 32000 tokens 7.4 us, 64 chains of 8 over 128000 22 (65 MB, 13 at the copy rate), 16 trees of 16 over 50021 9.
 // Weights are whole numbers of 2^-44, so their sums are exact in any order and the token does not depend on the split.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(DC_THREADS) ea_draft_check_kernel(ea_draft_che
     __shared__ int s_len, s_out, s_last, s_pick;
     __shared__ int s_gone[DC_MAX_NODES], s_ngone;  // tokens that p has lost
     __shared__ uint32_t s_bits[DC_MAX_VOCAB / DC_MAX_PARTS / 32 + 1];
-    __shared__ uint64_t s_sum[2][DC_THREADS / 64];
+    __shared__ uint64_t s_sum[DC_THREADS / 64], s_part[DC_MAX_PARTS];
     __shared__ uint64_t s_goal;
     __shared__ int s_whole;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
@@ -155,67 +155,61 @@ __global__ void __launch_bounds__(DC_THREADS) ea_draft_check_kernel(ea_draft_che
         }
     };
     const float4 none = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    {
-        const int lo = (int)blockIdx.x * part, hi = min(lo + part, V);
-        mark((int)blockIdx.x);
-        double s = 0.0, s0 = 0.0;
+    // the block's sum over part k, in thread 0; all: of p itself
+    auto part_sum = [&](int k, bool all) -> uint64_t {
+        const int lo = k * part, hi = min(lo + part, V);
+        double s = 0.0;
         for (int i = lo + 4 * tid; i < hi; i += 2 * DC_TILE) {  // two tiles' loads at once
             const bool more = i + DC_TILE < hi;
             const float4 p[2] = {load4(pr, i, V, wide), more ? load4(pr, i + DC_TILE, V, wide) : none};
-            const float4 q[2] = {qr ? load4(qr, i, V, wide) : none, qr && more ? load4(qr, i + DC_TILE, V, wide) : none};
+            const float4 q[2] = {qr && !all ? load4(qr, i, V, wide) : none, qr && !all && more ? load4(qr, i + DC_TILE, V, wide) : none};
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                if (k && !more) break;
-                double x[4], y[4];
-                weights(lo, i + k * DC_TILE, p[k], q[k], false, x);
-                weights(lo, i + k * DC_TILE, p[k], none, true, y);
+            for (int e = 0; e < 2; ++e) {
+                if (e && !more) break;
+                double x[4];
+                weights(lo, i + e * DC_TILE, p[e], q[e], all, x);
                 s += (x[0] + x[1]) + (x[2] + x[3]);
-                s0 += (y[0] + y[1]) + (y[2] + y[3]);
             }
         }
-        uint64_t t = (uint64_t)s, t0 = (uint64_t)s0;
-        for (int o = 32; o > 0; o >>= 1) {
-            t += (uint64_t)__shfl_xor((unsigned long long)t, o, 64);
-            t0 += (uint64_t)__shfl_xor((unsigned long long)t0, o, 64);
-        }
-        if (lane == 0) {
-            s_sum[0][w] = t;
-            s_sum[1][w] = t0;
-        }
-    }
-    __syncthreads();
+        uint64_t t = (uint64_t)s;
+        for (int o = 32; o > 0; o >>= 1) t += (uint64_t)__shfl_xor((unsigned long long)t, o, 64);
+        if (lane == 0) s_sum[w] = t;
+        __syncthreads();
+        t = 0;
+        for (int e = 0; e < DC_THREADS / 64; ++e) t += s_sum[e];
+        return t;
+    };
+    mark((int)blockIdx.x);
+    const uint64_t own = part_sum((int)blockIdx.x, false);
     uint64_t* const sums = A.work + (int64_t)b * (2 * DC_MAX_PARTS + 1);
     uint64_t* const count = sums + 2 * DC_MAX_PARTS;
     if (tid == 0) {
-        uint64_t t = 0, t0 = 0;
-        for (int k = 0; k < DC_THREADS / 64; ++k) {
-            t += s_sum[0][k];
-            t0 += s_sum[1][k];
-        }
-        // Exchanges happen where all dies meet, and one that has returned has happened: the count moves after the sums without a
+        // An exchange happens where all dies meet, and one that has returned has happened: the count moves after the sum without a
         // release, which writes back a die's second-level cache for every block (64 sequences of 8 drafts over 128000 tokens, 1024
         // blocks: 50 us with it, 27 without, and 2048 blocks 75 and 24)
-        const uint64_t a = __hip_atomic_exchange(&sums[2 * blockIdx.x], t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        const uint64_t c = __hip_atomic_exchange(&sums[2 * blockIdx.x + 1], t0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        asm volatile("" ::"v"(a), "v"(c) : "memory");
+        const uint64_t was = __hip_atomic_exchange(&sums[blockIdx.x], own, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        asm volatile("" ::"v"(was) : "memory");
         s_last = __hip_atomic_fetch_add(count, (uint64_t)1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint64_t)(parts - 1);
     }
     __syncthreads();
     if (!s_last) return;
     if (w == 0) {
-        uint64_t t = 0, t0 = 0;
-        if (lane < parts) {
-            t = __hip_atomic_load(&sums[2 * lane], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            t0 = __hip_atomic_load(&sums[2 * lane + 1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const uint64_t t = lane < parts ? __hip_atomic_load(&sums[lane], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+        s_part[lane] = t;
+        const bool any = __ballot(t != 0) != 0;
+        if (lane == 0) s_whole = !any;  // nothing left of p: p itself
+    }
+    __syncthreads();
+    if (s_whole)
+        for (int k = 0; k < parts; ++k) {  // as good as never
+            const uint64_t t = part_sum(k, true);
+            if (tid == 0) s_part[k] = t;
+            __syncthreads();
         }
-        uint64_t upto = wave_scan64(t, lane);
-        uint64_t total = (uint64_t)__shfl((unsigned long long)upto, 63, 64);
-        const bool whole = total == 0;  // nothing left of p: p itself
-        if (whole) {
-            upto = wave_scan64(t0, lane);
-            t = t0;
-            total = (uint64_t)__shfl((unsigned long long)upto, 63, 64);
-        }
+    if (w == 0) {
+        const uint64_t t = s_part[lane];
+        const uint64_t upto = wave_scan64(t, lane);
+        const uint64_t total = (uint64_t)__shfl((unsigned long long)upto, 63, 64);
         const double u = (double)U[N];
         const double g = u > 0.0 ? u * (double)total : 0.0;  // NaN: 0
         uint64_t goal = g < (double)total ? (uint64_t)g : total;
@@ -224,7 +218,6 @@ __global__ void __launch_bounds__(DC_THREADS) ea_draft_check_kernel(ea_draft_che
         if (lane == 0) {
             __hip_atomic_store(count, (uint64_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             s_pick = total == 0 ? -1 : __builtin_ctzll(m);
-            s_whole = whole;
             s_out = -1;
         }
         if (total && lane == __builtin_ctzll(m)) s_goal = goal - (upto - t);
@@ -243,12 +236,12 @@ __global__ void __launch_bounds__(DC_THREADS) ea_draft_check_kernel(ea_draft_che
             if (i < hi) weights(lo, i, load4(pr, i, V, wide), qr && !all ? load4(qr, i, V, wide) : none, all, x);
             const uint64_t own = (uint64_t)((x[0] + x[1]) + (x[2] + x[3]));
             const uint64_t upto = wave_scan64(own, lane);
-            if (lane == 63) s_sum[0][w] = upto;
+            if (lane == 63) s_sum[w] = upto;
             __syncthreads();
             uint64_t base = before, all4 = 0;
             for (int j = 0; j < DC_THREADS / 64; ++j) {
-                if (j < w) base += s_sum[0][j];
-                all4 += s_sum[0][j];
+                if (j < w) base += s_sum[j];
+                all4 += s_sum[j];
             }
             base += upto - own;
             if (base <= goal && goal < base + own) {
