@@ -724,8 +724,8 @@ struct T2Part {
 // larger base by an arithmetic right shift: floor(a 2^-s) <= a 2^-s < floor(a 2^-s) + lost, so
 // the row's sums stay of the form [acc, acc + lost count] in units of the common base, the form
 // the final rounding takes. With C = 1 the block finishes the row itself. done: EA_T2_BLOCKS
-// counters, 0 at the start, of the rows' finished chunks. MOD: with score modifications.
-template <bool MOD>
+// counters, 0 at the start, of the rows' finished chunks. MOD: with score modifications. KV4: the cache is held in 4 bits.
+template <bool MOD, bool KV4>
 __device__ __forceinline__ void t2_rows(const Params& P, T2Smem& S, int& s_last, int32_t* list, int cnt, int slot_id,
                                         int32_t* done, int32_t* next) {
     const int tid = threadIdx.x;
@@ -801,7 +801,7 @@ __device__ __forceinline__ void t2_rows(const Params& P, T2Smem& S, int& s_last,
             const uint16_t* kr = P.k + ko;
             // 16 dims (8 dwords) at a time, read twice: the lead exponent, then the window sum
             auto kchunk = [&](int c16, uint32_t (&kw)[8]) __attribute__((always_inline)) {
-                if (P.ks) {
+                if constexpr (KV4) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const int i = 16 * c16 + 8 * h;  // d is a multiple of 8
@@ -926,11 +926,11 @@ __device__ __forceinline__ void t2_rows(const Params& P, T2Smem& S, int& s_last,
             // broadcast and the batch's V elements loaded together (independent loads in flight)
             uint32_t vx[16][2];
             auto load_batch = [&](int64_t jb, int nk) __attribute__((always_inline)) {
-                const int64_t myoff = ln >= nk ? 0 : (P.vs ? kv4_v(P, b, key_n(jc0 + jb + ln), hk) : kv_off(P, b, key_n(jc0 + jb + ln), hk, 1));
+                const int64_t myoff = ln >= nk ? 0 : (KV4 ? kv4_v(P, b, key_n(jc0 + jb + ln), hk) : kv_off(P, b, key_n(jc0 + jb + ln), hk, 1));
 #pragma unroll
                 for (int kk = 0; kk < 16; ++kk) {
                     const int64_t o = __shfl(myoff, kk, 64);
-                    if (P.vs) {
+                    if constexpr (KV4) {
                         const uint32_t two = kk < nk && 2 * ln < dv ? kv4_vload2(P.v, P.vs, o, 2 * ln) : 0u;
                         vx[kk][0] = two & 0xFFFFu;
                         vx[kk][1] = two >> 16;
@@ -1186,7 +1186,7 @@ __device__ __forceinline__ int t2_left(const Params& P, int nact, int* slot_id) 
 // 4096-key bf16 row after a prefill step 116 -> 35 us; an empty list 4.6 us (3.8 at least)
 // in the trace, as without the pass; 512 blocks cost a C2 step 1.8 us, so bf16 steps of few rows, which list few,
 // launch 32. The pass itself is 1.5 us slower (64.8 -> 66.3) for the 128-bit path's registers beside it.
-template <bool MOD>
+template <bool MOD, bool KV4>
 __global__ void __launch_bounds__(EA_T2_THREADS) ea_tier2(Params P) {
     __shared__ union {
         T2Smem t2;
@@ -1198,25 +1198,25 @@ __global__ void __launch_bounds__(EA_T2_THREADS) ea_tier2(Params P) {
     // every item of a split row is in flight at once (a block each, a partial each, a count per row)
     // and no chunk is shorter than a pass of 128 keys
     const int C = cnt <= EA_T2_ROWS ? min(min(EA_DD_PARTS, (int)gridDim.x) / cnt, (P.t2_keys + EA_DD_KEYS - 1) / EA_DD_KEYS) : 1;
-    dd_rows<MOD>(P, S.dd, cnt, max(C, 1), (DDPart*)P.ddpart);
+    dd_rows<MOD, KV4>(P, S.dd, cnt, max(C, 1), (DDPart*)P.ddpart);
     const int nact = (int)min((int64_t)cnt * max(C, 1), (int64_t)gridDim.x);
     if ((int)blockIdx.x >= nact) return;
     agent_done();  // the list of what is left, and the partials, whose memory the 128-bit path reuses
     __syncthreads();
     if (threadIdx.x == 0) s_left = t2_left(P, nact, &s_slot);
     __syncthreads();
-    if (s_left > 0) t2_rows<MOD>(P, S.t2, s_last, P.t2left, s_left, s_slot, &P.wl_cnt[EA_T2_CHUNKS], &P.wl_cnt[EA_T2_NEXT]);
+    if (s_left > 0) t2_rows<MOD, KV4>(P, S.t2, s_last, P.t2left, s_left, s_slot, &P.wl_cnt[EA_T2_CHUNKS], &P.wl_cnt[EA_T2_NEXT]);
 }
 
 // force_tier2: every row straight to the 128-bit path, over EA_T2_BLOCKS blocks. A kernel of its own:
 // beside the double-double pass the body spills 324 SGPRs instead of 176 (32 rows of 32K keys, that pass
 // included, 6.4 ms against 6.0).
-template <bool MOD>
+template <bool MOD, bool KV4>
 __global__ void __launch_bounds__(EA_T2_THREADS) ea_tier2_wide(Params P) {
     __shared__ T2Smem S;
     __shared__ int s_last;
     const int cnt = *P.wl_cnt;
-    if (cnt > 0) t2_rows<MOD>(P, S, s_last, P.wl, cnt, (int)blockIdx.x, &P.wl_cnt[EA_T2_CHUNKS], nullptr);
+    if (cnt > 0) t2_rows<MOD, KV4>(P, S, s_last, P.wl, cnt, (int)blockIdx.x, &P.wl_cnt[EA_T2_CHUNKS], nullptr);
 }
 
 // Lists every row for tier 2 (ea_options.force_tier2); runs after tier 1, so nothing else appends.
@@ -1830,11 +1830,12 @@ void tier2(const Params& P, const ea_options* o, hipStream_t st) {
     // capped ones, 827 listed 3411 -> 995.
     const dim3 grid(o->force_tier2 ? EA_T2_BLOCKS : EA_DD_BLOCKS(P.out_fp32 || P.rows >= 8192)), blk(EA_T2_THREADS);
     if (o->force_tier2) {
-        if (P.mods) hipLaunchKernelGGL(ea_tier2_wide<true>, grid, blk, 0, st, P);
-        else hipLaunchKernelGGL(ea_tier2_wide<false>, grid, blk, 0, st, P);
+        if (P.ks) hipLaunchKernelGGL((P.mods ? ea_tier2_wide<true, true> : ea_tier2_wide<false, true>), grid, blk, 0, st, P);
+        else hipLaunchKernelGGL((P.mods ? ea_tier2_wide<true, false> : ea_tier2_wide<false, false>), grid, blk, 0, st, P);
     } else {
-        if (P.mods) hipLaunchKernelGGL(ea_tier2<true>, grid, blk, 0, st, P);
-        else hipLaunchKernelGGL(ea_tier2<false>, grid, blk, 0, st, P);
+        // (a choice of format within the loads: 32 rows of 32K keys 6.9 -> 8.5 ms)
+        if (P.ks) hipLaunchKernelGGL((P.mods ? ea_tier2<true, true> : ea_tier2<false, true>), grid, blk, 0, st, P);
+        else hipLaunchKernelGGL((P.mods ? ea_tier2<true, false> : ea_tier2<false, false>), grid, blk, 0, st, P);
     }
 }
 

@@ -142,7 +142,8 @@ struct DDSmem {
 // rows with a domain error flag 2; the rest are listed in P.t2left, P.wl_cnt[EA_T2_LEFT] of them.
 // MOD: with score modifications; weights 2^-800 below the row's reference, which leave the row undecided
 // otherwise, then count as terms left out, at most 2^-770 each.
-template <bool MOD = false>
+// KV4: the cache is held in 4 bits.
+template <bool MOD = false, bool KV4 = false>
 __device__ inline void dd_rows(const Params& P, DDSmem& S, int cnt, int C, DDPart* parts) {
     const int tid = (int)threadIdx.x, lane = tid & 63, wv = tid >> 6;
     const int d = P.g.head_dim, dv = P.g.head_dim_v, Hq = P.g.num_q_heads, T = P.g.num_tokens;
@@ -194,7 +195,7 @@ __device__ inline void dd_rows(const Params& P, DDSmem& S, int cnt, int C, DDPar
             // requested first, so that one memory latency covers K and V
             const int kb = 16 * wv;
             const int nk = (int)max((int64_t)0, min((int64_t)16, jc1 - j0 - kb));
-            const int64_t myoff = lane >= nk ? 0 : (P.vs ? kv4_v(P, b, key_n(j0 + kb + lane), hk) : kv_off(P, b, key_n(j0 + kb + lane), hk, 1));
+            const int64_t myoff = lane >= nk ? 0 : (KV4 ? kv4_v(P, b, key_n(j0 + kb + lane), hk) : kv_off(P, b, key_n(j0 + kb + lane), hk, 1));
             uint32_t vx[16];
 #pragma unroll
             for (int kk = 0; kk < 16; ++kk) {
@@ -202,7 +203,7 @@ __device__ inline void dd_rows(const Params& P, DDSmem& S, int cnt, int C, DDPar
                 vx[kk] = 0;
                 if (kk < nk && 2 * lane < dv) {
                     const uint16_t* vp = P.v + o + 2 * lane;
-                    if (P.vs) vx[kk] = kv4_vload2(P.v, P.vs, o, 2 * lane);
+                    if (KV4) vx[kk] = kv4_vload2(P.v, P.vs, o, 2 * lane);
                     else vx[kk] = v4 ? *(const uint32_t*)vp : ((uint32_t)vp[0] | ((uint32_t)vp[1] << 16));
                 }
             }
@@ -221,7 +222,7 @@ __device__ inline void dd_rows(const Params& P, DDSmem& S, int cnt, int C, DDPar
                     const int c0 = 8 * (4 * i + part);
                     kv[i] = make_uint4(0, 0, 0, 0);
                     if (c0 >= d) continue;  // d is a multiple of 8
-                    if (P.ks) {
+                    if (KV4) {
                         kv[i] = kv4_load8(P.k, P.ks, ko + c0);
                     } else if (k16) {
                         kv[i] = *(const uint4*)(kr + c0);
