@@ -410,10 +410,18 @@ def exact_rows(dp: DeviceProblem, alpha_bits: int) -> None:
 class KVDigits:
     """A device digit-tile cache of a problem's K/V (the KV slice format kept across steps):
     `tiles` 64-key tiles per (sequence, KV head), EA_PF_TILE_BYTES each, laid out as
-    include/exactattn_hip.h describes for ea_hip_kv_digits_update."""
+    include/exactattn_hip.h describes for ea_hip_kv_digits_update. They are cut from a bf16 cache: a
+    problem over a 4-bit one is refused."""
+
+    @staticmethod
+    def _check(dp: DeviceProblem) -> None:
+        # the update reads K and V as rows of bf16, past the end of a 4-bit cache's codes
+        if dp.kv4 is not None:
+            raise ValueError("digit tiles are cut from a bf16 cache, not from one held in 4 bits")
 
     def __init__(self, dp: DeviceProblem, tiles: int):
         import torch
+        self._check(dp)
         lib = load()
         g = dp.geom
         n = lib.ea_hip_kv_digits_bytes(int(g["num_seqs"]), int(g["num_kv_heads"]), int(tiles))
@@ -425,6 +433,7 @@ class KVDigits:
     def update(self, dp: DeviceProblem, key_begin, key_end, max_new_keys: int) -> None:
         """Re-slice the tiles that hold keys key_begin[b] .. key_end[b] - 1 of each sequence
         (device int32 tensors), after they were written to dp's bf16 cache."""
+        self._check(dp)
         lib = load()
         b = dp.buffers()
         _check(lib.ea_hip_kv_digits_update(ctypes.byref(dp._geom_c), ctypes.byref(b), key_begin.data_ptr(),
