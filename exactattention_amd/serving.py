@@ -200,6 +200,8 @@ class PagedKVCache:
             raise ValueError("one count per sequence slot")
         if k_new.shape[0] != sum(counts) or v_new.shape[0] != sum(counts):
             raise ValueError("k/v must hold sum(counts) keys")
+        if not k_new.numel() == v_new.numel() == sum(counts) * self.Hkv * self.d:
+            raise ValueError(f"k/v must be ({sum(counts)}, {self.Hkv}, {self.d}) bf16 bits")
         if not checked:
             self._check_slots(seqs)
         if sum(counts) == 0:

@@ -2,9 +2,11 @@
 
 from types import SimpleNamespace
 
+import numpy as np
 import pytest
 
 from exactattention_amd import hip
+from exactattention_amd.serving import PagedKVCache
 
 
 def test_no_digit_tiles_of_a_4_bit_cache(monkeypatch):
@@ -20,3 +22,18 @@ def test_no_digit_tiles_of_a_4_bit_cache(monkeypatch):
     cache.tiles, cache.buf = 4, None
     with pytest.raises(ValueError, match="4 bits"):
         cache.update(dp, None, None, 64)
+
+
+@pytest.mark.parametrize("shape", [(3, 4, 64), (3, 1, 64), (3, 2, 32), (3, 2, 128)])
+def test_keys_of_other_heads_change_nothing(shape):
+    """Keys of other heads than the cache's are refused while lengths, pages and the table still are as they were (a 4-bit cache
+    took the first rows of what they reshape to, or raised with the pages taken)."""
+    c = PagedKVCache(4, 16, 2, 64, 2, 64, device="cpu")
+    s = c.add_sequence()
+    good, bad = np.zeros((3, 2, 64), np.uint16), np.zeros(shape, np.uint16)
+    for k, v in ((bad, good), (good, bad), (bad, bad)):
+        with pytest.raises(ValueError, match="bf16 bits"):
+            c.append(s, k, v)
+        assert c.length[s] == 0 and c.pages[s] == [] and len(c.free) == 4
+    c.append(s, good, good)
+    assert c.length[s] == 3 and len(c.free) == 3
