@@ -94,6 +94,8 @@ class DraftCheckArgs(ctypes.Structure):
                                     "work")])
 
 
+KV4_MAXD = 128  # head size that attention over a 4-bit cache takes (a pool by itself may hold larger ones)
+
 # ea_options.kernel (include/exactattn_hip.h EA_KERNEL_*)
 KERNELS = {"auto": 0, "prefill": 1, "decode": 2, "general": 3}
 
@@ -334,6 +336,8 @@ class DeviceProblem:
                 raise ValueError(f"the 4-bit cache must be on {dev}")
             if any(self.geom.get(f) != x for f, x in self.kv4.geometry().items()):
                 raise ValueError("the geometry is not the 4-bit cache's (KV4Pool.geometry)")
+            if self.kv4.head_dim > KV4_MAXD:
+                raise ValueError(f"attention over a cache in 4 bits takes heads of up to {KV4_MAXD}")
             prob = {**prob, "k": self.kv4.k, "v": self.kv4.v}
         self.t = {k: t(prob.get(k)) for k in ("q", "k", "v", "seq_len", "kv_len", "block_table",
                                                "block_table_offset", "tree_mask", "tree_base")}

@@ -109,6 +109,8 @@ class PagedKVCache:
         if bits == 4:
             if self.dev.type != "cuda":
                 raise ValueError("a cache in 4 bits lives on the GPU")
+            if head_dim > hip.KV4_MAXD:
+                raise ValueError(f"attention over a cache in 4 bits takes heads of up to {hip.KV4_MAXD}")
             self.pool4 = KV4Pool(num_pages, page_size, num_kv_heads, head_dim, self.dev)
             self.k, self.v = self.pool4.k, self.pool4.v
             digits = False

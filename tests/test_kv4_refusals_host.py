@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 
 from exactattention_amd import hip
+from exactattention_amd.kv4 import KV4Pool
 from exactattention_amd.serving import PagedKVCache
 
 
@@ -37,3 +38,17 @@ def test_keys_of_other_heads_change_nothing(shape):
         assert c.length[s] == 0 and c.pages[s] == [] and len(c.free) == 4
     c.append(s, good, good)
     assert c.length[s] == 3 and len(c.free) == 3
+
+
+def test_heads_that_attention_does_not_take():
+    """Heads past 128: a pool may hold them, but a cache to be served from, and a problem, say so when they are made, not by an
+    attention call's error code after the keys are in."""
+    for d in (136, 256):
+        with pytest.raises(ValueError, match="up to 128"):
+            PagedKVCache(4, 16, 2, d, 1, 64, bits=4)
+        pool = KV4Pool(1, 16, 1, d, device="cpu")
+        with pytest.raises(ValueError, match="up to 128"):
+            hip.DeviceProblem(dict(geom=dict(num_seqs=1, num_tokens=1, num_q_heads=1, max_seq_len=16, block_table_stride=1,
+                                             **pool.geometry()), kv4=pool, q=np.zeros((1, 1, 1, d), np.uint16),
+                                   seq_len=np.ones(1, np.int32), kv_len=np.ones(1, np.int32), block_table=np.zeros((1, 1), np.int32),
+                                   out_shape=(1, 1, 1, d)), device="cpu")
