@@ -301,7 +301,7 @@ def step_route(g: dict, ptrs: dict, **opt) -> tuple[str, int, bool, int]:
 class DeviceProblem:
     """A problem's arrays resident on the GPU, plus output, flags, workspace and stats buffers.
     Built once; `launch_hip` then runs steps on it with no allocation. prob["kv4"], a KV4Pool, in place of "k" and
-    "v": a cache held in 4 bits, whose geometry() the problem's holds."""
+    "v": a cache held in 4 bits, whose geometry() the problem's holds; without a block table its page b is sequence b."""
 
     def __init__(self, prob: dict, out: str = "bf16", splits: int = 0, device: str = "cuda", kernel: str = "auto",
                  prefill_waves: int = 0, mods: ScoreMods | None = None):
@@ -338,6 +338,11 @@ class DeviceProblem:
                 raise ValueError("the geometry is not the 4-bit cache's (KV4Pool.geometry)")
             if self.kv4.head_dim > KV4_MAXD:
                 raise ValueError(f"attention over a cache in 4 bits takes heads of up to {KV4_MAXD}")
+            if prob.get("block_table") is None:
+                lens = prob.get("seq_len")
+                host = lens is not None and not getattr(lens, "is_cuda", False)  # a device array is the caller's word
+                if self.geom["num_seqs"] > self.kv4.num_pages or (host and len(lens) and int(max(lens)) > self.kv4.page_size):
+                    raise ValueError("without a block table sequence b is page b of the 4-bit cache, and no longer than that")
             prob = {**prob, "k": self.kv4.k, "v": self.kv4.v}
         self.t = {k: t(prob.get(k)) for k in ("q", "k", "v", "seq_len", "kv_len", "block_table",
                                                "block_table_offset", "tree_mask", "tree_base")}

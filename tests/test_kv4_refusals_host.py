@@ -52,3 +52,16 @@ def test_heads_that_attention_does_not_take():
                                              **pool.geometry()), kv4=pool, q=np.zeros((1, 1, 1, d), np.uint16),
                                    seq_len=np.ones(1, np.int32), kv_len=np.ones(1, np.int32), block_table=np.zeros((1, 1), np.int32),
                                    out_shape=(1, 1, 1, d)), device="cpu")
+
+
+@pytest.mark.parametrize("seqs, keys", [(3, 16), (2, 17), (1, 64)])
+def test_no_block_table_and_no_page(seqs, keys):
+    """Without a block table the kernels read page b for sequence b: more sequences than pages, or longer ones, would be read from
+    behind the pool."""
+    pool = KV4Pool(2, 16, 1, 64, device="cpu")
+    with pytest.raises(ValueError, match="block table"):
+        hip.DeviceProblem(dict(geom=dict(num_seqs=seqs, num_tokens=1, num_q_heads=1, max_seq_len=keys, block_table_stride=0,
+                                         q_seq_stride=64, q_tok_stride=64, q_head_stride=64, o_seq_stride=64, o_tok_stride=64,
+                                         o_head_stride=64, **pool.geometry()), kv4=pool, q=np.zeros((seqs, 1, 1, 64), np.uint16),
+                               seq_len=np.full(seqs, keys, np.int32), kv_len=np.full(seqs, keys, np.int32),
+                               out_shape=(seqs, 1, 1, 64)), device="cpu")
