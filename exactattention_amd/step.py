@@ -636,9 +636,13 @@ class DraftCheck:
             raise ValueError("trees are of given tokens: draft_probs are of a chain")
         p, ps, pr = self._rows(probs, "probs", N + 1)
         q, qs, qr = (0, 0, 0) if draft_probs is None else self._rows(draft_probs, "draft_probs", N)
-        ints = [0 if x is None else _vec(x, name, at, self._i32, n)
-                for x, name, n in ((drafted, "drafted", B * N), (parents, "parents", B * N), (counts, "counts", B))]
-        u = _vec(uniforms, "uniforms", at, self._f32, B * (N + 1))
+        for x, name, shape in ((drafted, "drafted", (B, N)), (uniforms, "uniforms", (B, N + 1)), (parents, "parents", (B, N)),
+                               (counts, "counts", (B,))):
+            if x is not None and x.shape != shape:
+                raise ValueError(f"{name} must be {shape}, got {tuple(x.shape)}")
+        ints = [0 if x is None else _vec(x, name, at, self._i32)
+                for x, name in ((drafted, "drafted"), (parents, "parents"), (counts, "counts"))]
+        u = _vec(uniforms, "uniforms", at, self._f32)
         for x, n in zip(ints, (B * N, B * N, B)):
             for out in (self.accepted, self.path, self.tokens):
                 if x and n and out.numel() and x < out.data_ptr() + 4 * out.numel() and out.data_ptr() < x + 4 * n:
