@@ -500,6 +500,8 @@ class Rotary:
         four = isinstance(k_pool, KV4Pool)
         if four:
             return self._append4(q, k, v, positions, dst_rows, k_pool, v_pool, q_rows, q_out, pos_offset, norm)
+        if v_pool is None:
+            raise ValueError("v_pool is missing: only a KV4Pool holds both k and v")
         n, hq, hk, wide, strides, axis_stride = self._args(q, k, v, positions)
         if not -1 << 31 <= pos_offset < 1 << 31:
             raise ValueError("pos_offset must fit 32 bits")

@@ -37,3 +37,15 @@ def test_drafts_of_another_layout(calls):
     c.verify(**ok)
     c.verify(**ok, parents=ok["drafted"].clone(), counts=torch.zeros(B, dtype=torch.int32))
     assert len(calls) == 2
+
+
+def test_append_without_a_pool_for_v(calls, monkeypatch):
+    """A bf16 pool for k alone is an argument that is missing, not an attribute of None."""
+    r = step.Rotary.__new__(step.Rotary)
+    r.dev, r._at, r.head_dim, r._i64, r._bits = torch.device("cpu"), -1, 64, torch.int64, (torch.bfloat16, torch.int16)
+    monkeypatch.setattr(step.Rotary, "_args", lambda *a: (2, 1, 1, False, (64, 64) * 3, 0))
+    x, at = torch.zeros((2, 1, 64), dtype=torch.bfloat16), torch.zeros(2, dtype=torch.int64)
+    for v_pool in ((), (None,)):
+        with pytest.raises(ValueError, match="v_pool"):
+            r.append(x, x, x, at.int(), at, torch.zeros((1, 16, 1, 64), dtype=torch.bfloat16), *v_pool)
+    assert not calls
