@@ -45,14 +45,14 @@ assert _NORM.size == ctypes.sizeof(hip.NormRotaryArgs) and _GRAD.size == ctypes.
 assert _DRAFT.size == ctypes.sizeof(hip.DraftCheckArgs)
 
 
-_C = None  # torch's, once a plan or a rotation exists
+_C = _FORWARD = None  # torch's, and its forward-mode gradients, once a plan or a rotation exists
 
 
 def _entry(name: str):
     """The C entry point, taking its arguments packed."""
-    global _C
+    global _C, _FORWARD
     import torch
-    _C = torch._C
+    _C, _FORWARD = torch._C, torch.autograd.forward_ad
     fn = hip.load()[name]  # a function object of its own
     fn.argtypes, fn.restype = [ctypes.c_char_p, ctypes.c_void_p], ctypes.c_int
     return fn
@@ -68,6 +68,13 @@ def _call(fn, args: bytes, index: int, what: str) -> None:
             rc = fn(args, _C._cuda_getCurrentRawStream(index))
     if rc:
         raise ValueError(f"{what}: error code {rc}")
+
+
+def _no_tangents(*xs) -> None:
+    """Under a forward-mode level: inputs with a tangent, which the kernels would drop, are refused as those that need a
+    gradient are."""
+    if any(_FORWARD.unpack_dual(x).tangent is not None for x in xs):
+        raise NotImplementedError("the rotation has no forward-mode gradients")
 
 
 _TURN = None
@@ -397,7 +404,9 @@ class Rotary:
         tokens) int32), into new tensors of their type or into q_out and k_out (which may be q and k
         themselves). inverse turns back: the gradient of the rotation. norm: every head is normed first (not with
         inverse). Returns (q_out, k_out). Gradients of q, k and the norm's weights pass through, with q_out and k_out not
-        given."""
+        given; forward-mode ones are refused."""
+        if _FORWARD._current_level >= 0:
+            _no_tangents(q, k, *(() if norm is None else (norm.q_weight, norm.k_weight)))
         if norm is not None:
             if inverse:
                 raise ValueError("the norm has no inverse")

@@ -49,3 +49,26 @@ def test_append_without_a_pool_for_v(calls, monkeypatch):
         with pytest.raises(ValueError, match="v_pool"):
             r.append(x, x, x, at.int(), at, torch.zeros((1, 16, 1, 64), dtype=torch.bfloat16), *v_pool)
     assert not calls
+
+
+def test_forward_mode_tangents(calls, monkeypatch):
+    """A tangent of q, k or a weight is refused, whether or not anything needs a gradient: the kernels would drop it."""
+    import torch.autograd.forward_ad as fwd
+    monkeypatch.setattr(step, "_C", torch._C)
+    monkeypatch.setattr(step, "_FORWARD", fwd, raising=False)
+    r = step.Rotary.__new__(step.Rotary)
+    r.dev, r._at, r.head_dim, r._fn, r._norm_fn, r._half, r._axis = torch.device("cpu"), -1, 8, None, None, 0, 0
+    r.rot_dim, r.axes, r.adjacent, r.scale = 8, 1, False, 1.0
+    r._f32, r._i32, r._bits = torch.float32, torch.int32, (torch.bfloat16, torch.int16)
+    q, k, w, pos = torch.ones((2, 3, 8)), torch.ones((2, 1, 8)), torch.ones(8), torch.zeros(2, dtype=torch.int32)
+    with fwd.dual_level():
+        r.rotate(q, k, pos)
+        r.rotate(q, k, pos, norm=step.HeadNorm(w, w))
+        assert len(calls) == 2
+        for args, norm in (((fwd.make_dual(q, q), k), None), ((q, fwd.make_dual(k, k)), None),
+                           ((q, fwd.make_dual(k, k)), step.HeadNorm(w, w)), ((q, k), step.HeadNorm(fwd.make_dual(w, w), w)),
+                           ((q, k), step.HeadNorm(w, fwd.make_dual(w, w))), ((fwd.make_dual(q.clone().requires_grad_(), q), k), None)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                r.rotate(*args, pos, norm=norm)
+    r.rotate(q, k, pos)
+    assert len(calls) == 3
