@@ -28,6 +28,7 @@ import numpy as np
 from . import hip
 from .kv4 import KV4Pool
 
+_FP32_MAX = float(np.finfo(np.float32).max)
 PLAN_SEQS, PLAN_ROWS = 8192, 65536  # sequences of a plan, rows of its block table
 
 PLAN_STATUS = {1: "out of pages", 2: "a sequence longer than its table row or max_seq_len",
@@ -264,8 +265,8 @@ class HeadNorm:
     elements. q_weight, k_weight: (head_dim,) bf16 or fp32, both of one type (parameters get their gradients)."""
 
     def __init__(self, q_weight, k_weight, eps: float = 1e-6):
-        if not (math.isfinite(eps) and eps >= 0):
-            raise ValueError("eps must be finite and not negative")
+        if not 0 <= eps <= _FP32_MAX:  # the kernels take it as an fp32
+            raise ValueError("eps must be a finite fp32 number and not negative")
         if q_weight.dtype != k_weight.dtype or q_weight.dim() != 1 or q_weight.shape != k_weight.shape:
             raise ValueError("q_weight and k_weight must be (head_dim,) tensors of one type")
         self.q_weight, self.k_weight, self.eps = q_weight, k_weight, float(eps)

@@ -72,3 +72,12 @@ def test_forward_mode_tangents(calls, monkeypatch):
                 r.rotate(*args, pos, norm=norm)
     r.rotate(q, k, pos)
     assert len(calls) == 3
+
+
+@pytest.mark.parametrize("eps", [3.5e38, 1e300, -1e-9, float("inf"), float("nan")])
+def test_eps_that_is_no_fp32(eps):
+    """Refused where the norm is made, not while a step's arguments are packed, its tokens already counted in the cache."""
+    w = torch.ones(8)
+    with pytest.raises(ValueError, match="eps"):
+        step.HeadNorm(w, w, eps)
+    assert step.HeadNorm(w, w, 3e38).eps == 3e38 and step.HeadNorm(w, w, 0.0).eps == 0.0
