@@ -20,6 +20,7 @@ int herr(hipError_t e) { return e == hipSuccess ? 0 : -100 - (int)e; }
 
 constexpr int DC_THREADS = 256;
 constexpr int DC_MAX_PARTS = 64;
+constexpr int DC_WORK = DC_MAX_PARTS + 1;  // of the workspace, a sequence: a sum for each part, and their count
 constexpr int DC_MAX_NODES = 64;
 constexpr int DC_MAX_VOCAB = 1 << 19;
 // a part is whole tiles, 8 at most: a thread's sums of 32 whole numbers up to 2^44 are exact in fp64
@@ -181,8 +182,8 @@ __global__ void __launch_bounds__(DC_THREADS) ea_draft_check_kernel(ea_draft_che
     };
     mark((int)blockIdx.x);
     const uint64_t own = part_sum((int)blockIdx.x, false);
-    uint64_t* const sums = A.work + (int64_t)b * (2 * DC_MAX_PARTS + 1);
-    uint64_t* const count = sums + 2 * DC_MAX_PARTS;
+    uint64_t* const sums = A.work + (int64_t)b * DC_WORK;
+    uint64_t* const count = sums + DC_MAX_PARTS;
     if (tid == 0) {
         // An exchange happens where all dies meet, and one that has returned has happened: the count moves after the sum without a
         // release, which writes back a die's second-level cache for every block (64 sequences of 8 drafts over 128000 tokens, 1024
@@ -275,7 +276,7 @@ int parts_of(int B, int V, int* part) {
 extern "C" {
 
 size_t ea_hip_draft_check_size(const ea_draft_check* a) {
-    return a && a->num_seqs > 0 ? (size_t)a->num_seqs * (2 * DC_MAX_PARTS + 1) * 8 : 0;
+    return a && a->num_seqs > 0 ? (size_t)a->num_seqs * DC_WORK * 8 : 0;
 }
 
 int ea_hip_draft_check(const ea_draft_check* a, ea_stream_t stream) {

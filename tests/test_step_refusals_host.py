@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from exactattention_amd import step
+from exactattention_amd import hip, step
 
 
 @pytest.fixture
@@ -81,3 +81,9 @@ def test_eps_that_is_no_fp32(eps):
     with pytest.raises(ValueError, match="eps"):
         step.HeadNorm(w, w, eps)
     assert step.HeadNorm(w, w, 3e38).eps == 3e38 and step.HeadNorm(w, w, 0.0).eps == 0.0
+
+
+def test_draft_check_workspace():
+    """A sum for each of 64 parts of the vocabulary and their count, for each sequence."""
+    size = hip.load().ea_hip_draft_check_size
+    assert [size(hip.DraftCheckArgs(num_seqs=n)) for n in (0, 1, 7)] == [0, 65 * 8, 7 * 65 * 8]
