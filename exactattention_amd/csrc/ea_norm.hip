@@ -619,12 +619,9 @@ int ea_hip_norm_rotary_grad(const ea_norm_rotary_grad* a, ea_stream_t stream) {
         if (C == 0) return -1;
         const int L = lanes_of(d, C), tpb = NG_TOKENS;
         grad_blocks(*a, tpb, &qb, &kb);
+        // 42 KB at most: 4 turns of 128 pairs, 256 weights, and 256 / L rows of d <= 16 L sums
         const size_t lds = (size_t)tpb * (R / 2) * 16 + (size_t)d * 8 + (sums ? (size_t)(NR_THREADS / L) * d * 8 : 0);
         auto go = [&](auto* fn) -> int {
-            if (lds > 60 * 1024) {
-                const hipError_t e = hipFuncSetAttribute((const void*)fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-                if (e != hipSuccess) return herr(e);
-            }
             hipLaunchKernelGGL(fn, dim3((unsigned)(qb + kb)), dim3(NR_THREADS), lds, st, *a, tpb, L, qb);
             return herr(hipGetLastError());
         };
