@@ -52,7 +52,6 @@ using namespace ea;
 namespace {
 
 constexpr int F4_THREADS = 256;
-constexpr int F4_W2 = 2;
 constexpr int F4_NONE = -1200000000;  // base of a row without a visible key so far
 constexpr int F4_BITS = 22;           // a weight's exponent E may exceed the base by this: M < 2^24 then gives 46 bits
 constexpr int F4_HEAD = 2;            // room left when the base moves
@@ -150,7 +149,7 @@ __device__ __forceinline__ void four_weights(const double (&xs)[NP], double a, d
 // MOD: with score modifications (ea_mod.h): 1 key ranges alone, 2 with a bias, 3 with a cap; a unit's key range is then counted from its
 // rows' first visible key, down to a whole tile, and on uniform splits the last split takes every key past the others.
 template <int RS, int NG, int MOD, int WR>
-__global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Params P) {
+__global__ void __launch_bounds__(F4_THREADS, 2) ea_four(Params P) {
     constexpr int KL = RS;               // keys of a lane
     constexpr int NMF = RS == 2 ? 1 : 2;  // matrix instructions for 6 digits of the rows
     constexpr int RB = RS * WR;           // rows of the block
@@ -174,7 +173,7 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
     }
 
     // One piece: keys [kA, kB) of unit `item` (segment, row block), clipped to the unit's visible end, as partial slot `split`.
-    auto piece = [&](const bool first, const int item, const int split, int kA, int kB) __attribute__((always_inline)) {
+    auto piece = [&](const int item, const int split, int kA, int kB) __attribute__((always_inline)) {
         // what follows from the lane is found anew for every piece: kept over the pieces it spills, and a reload waits for the loads of
         // the first tile
         int lane = tid & 63;
@@ -1043,7 +1042,7 @@ __global__ void __launch_bounds__(F4_THREADS, RS == 2 ? F4_W2 : 2) ea_four(Param
             if (slot >= P.nsplit) break;  // share >= dq_min_share keeps every unit within nsplit slots
         }
         if (!first) __syncthreads();  // the previous piece's LDS reads are done
-        piece(first, u, slot, t0 * 64, te * 64);
+        piece(u, slot, t0 * 64, te * 64);
         if (!P.dq_stream) break;
         ++u;
     }
