@@ -22,8 +22,8 @@
 // What bounds it is the VALU, and HBM where a block has 2 rows: of a tile of 64 keys and 4 rows 55 instructions for the scores, 135 for the
 // weights, 37 a group of 32 channels for their digits and 44 for V's bytes; 2 waves a SIMD (the int32 sums alone are 64 registers; 8 rows
 // a wave took 96, spilled, and then waited for every load: a 1500-token chunk 770 us, 680 with 4). A step of 32 ragged sequences to
-// 4096 keys, 32/8 heads: 60 us, 69 on the fp64 matrix instructions; 8 of 30000 to 131072, 16/8 heads: 176 (4.6 TB/s), 437; a chunk of
-// 1500 tokens behind 2500, 16/8 heads: 580, 718.
+// 4096 keys, 32/8 heads: 59 us, 69 on the fp64 matrix instructions; 8 of 30000 to 131072, 16/8 heads: 172 (4.8 TB/s), 437; a chunk of
+// 1500 tokens behind 2500, 16/8 heads: 579, 718.
 //
 // Layout. A block is 4 waves over one (segment, block of rows, key range). WR = 1: RS = 2 or 4 rows, wave w takes 64-key tiles w, w +
 // 4, .. and meets the others in the epilogue only. WR = 4: 16 rows, a wave takes 4 of them and every tile. Lane l: g = l / 16, n = l % 16;

@@ -1527,6 +1527,9 @@ void choose_splits(int64_t items, int maxlen, int splits, int* nsplit, int* spli
 // its share, and at most 10 (16/8 or 8/8 heads, one token, plan -> one round: 32 x 300 keys 42.3 ->
 // 31.0 us, 32 x 700 50.0 -> 41.2, 64 x 300 46.5 -> 40.6, ragged to 900 keys 49.6 -> 38.6; but 24 rows, 20
 // x 400 keys 100 -> 112).
+// The split kernel of 4-bit caches takes the same counts, which were not fitted to it. On 11 steps, one sequence of 900 keys to 32 of
+// 4096, they are within 17% of the best of 2, 4, .. 128 splits (16/8 heads, 8 x 16K keys 51.7 us at 32, 44.2 at 8; one of 64K 43.5 at 64,
+// 38.9 at 32; 8 tokens on 16K 44.4 at 32, 39.2 at 16; 32/8 heads, 32 x 4096 62.6 at 8, 56.3 at 2; the others within 5%).
 void choose_splits_mrow(const Plan& pl, Tier1& mr, int maxlen, int dv, int splits) {
     int ns = splits;
     if (ns == 0) {
@@ -1688,8 +1691,10 @@ int make_plan(const ea_geometry* g, const ea_options* o, Plan* pl, const ea_scor
     Tier1& mr = pl->mr;
     mr.rb = m && pl->prefill ? 0 : mrow_rows(g, o, pl->r_seg, m != nullptr || kv4);
     // ea_four's row blocks: 16, a wave for every 4 rows, where they are three quarters full or more and fill a round of 2 a CU: fewer
-    // pieces, each read by one block (a 1500-token chunk of 16/8 heads, 1504 blocks: 660 us with 4 rows, 580 with 16). Fewer
-    // blocks split their keys more often (8 drafted tokens of 8 x 16K, 64 units: 118 and 130).
+    // pieces, each read by one block. Fewer blocks split their keys more often. 16/8 heads, tokens x keys, 4 rows -> 16: 1504
+    // blocks, 1500 x 4000 651 -> 565 us; 752, 750 x 4000 368 -> 337; 512, 512 x 4000 299 -> 272, 64 sequences of 8 x 2048 174 -> 140;
+    // 256, 256 x 4000 154 -> 153, 32 of 8 x 4096 157 -> 143; 128, 128 x 4000 91 -> 101, 16 of 8 x 8192 186 -> 181; 64, 8 of ragged
+    // 8 x 16K 118 -> 130.
     if (kv4 && mr.rb) {
         const int nb = (pl->r_seg + 15) / 16;
         mr.rb = pl->r_seg <= 2 ? 2 : (4 * pl->r_seg >= 48 * nb && (int64_t)pl->nseg * nb >= 512 ? 16 : 4);

@@ -7,9 +7,11 @@
 //   4 bits    a scale for 32 elements: the smallest 2^e with max|y| < 7 2^e, elements to the nearest of 0, 0.5, 1,
 //             1.5, 2, 3, 4, 6 times it
 //
-// All of it runs in fp64 and is rounded once, as the rotation by itself does. What bounds it is the VALU, 16 to 30 instructions an element
-// at a rate where memory would take 5 to 8: 16384 tokens of 32/8 heads of 128 bf16 into a 4-bit cache 116 us (353 MB, 68 us at the copy
-// rate); 4096 tokens of 16/8 heads forward 20 (50 MB, 10), gradient 30 (75 MB, 15), which 232 registers keep at 2 waves a SIMD.
+// All of it runs in fp64 and is rounded once, as the rotation by itself does. 16384 tokens of 32/8 heads of 128 bf16 into a 4-bit cache
+// 116 us (353 MB, 68 us at the copy rate); 4096 tokens of 16/8 heads forward 20 (50 MB, 10), gradient 31 (75 MB, 15), which 232
+// registers keep at 2 waves a SIMD. No one unit bounds it. In those three the VALU issues 64, 61 and 50% of the CUs' busy cycles (16 to
+// 30 instructions an element) and conflicts on LDS banks take 38, 39 and 27%: the lanes of a head read turns 128 and weights 64 bytes
+// apart. Waves wait for 61, 53 and 41% of their time.
 // Layout: L lanes hold a head, 2 C elements each: the two halves of C rotated pairs, or two runs of C others. So a head's sums
 // are log2 L shuffles, the rotation needs no other lane's elements, and with C = 8 every access has 16 bytes. C = 2 and 1
 // take what is not aligned so, or whose halves are not whole runs.

@@ -415,7 +415,8 @@ def _equal_runs(ql, heads=None, head_dim=128, longest=0):
     others, padded -> three runs): 64 tokens between 5 and 5 decode tokens, 16 heads, 300 keys 236 ->
     257, 3000 keys 243 -> 264 (but alone 413 -> 359), 5000 keys 0.83 times, 9000 keys 0.60; 4 heads
     9000 keys 287 -> 310; 100 tokens between 12 and 12, 32 heads, 300 keys 259 -> 275, 1000 keys 0.90
-    times, 2000 keys 0.64; 64 heads, 300 keys 0.96, 1000 keys 0.69."""
+    times, 2000 keys 0.64; 64 heads, 300 keys 0.96, 1000 keys 0.69. The times are those of 16-bit caches; a batch over
+    a 4-bit one is cut alike."""
     n = 1 + sum(map(operator.ne, ql, ql[1:]))
     if n == 1:
         return [(0, len(ql))]
@@ -812,8 +813,8 @@ class ExactAttentionBackend:
         return res[:, 0], fl
 
     def verify_tree(self, s: int, q, k, v, parents):
-        """Speculative verification's attention (DraftCheck then says which nodes stand): N <= 64 draft nodes, parents[i] < i (-1: the prefix), appended
-        after the prefix; node i attends the prefix and its root-to-node path. q (N, Hq, d), k/v
+        """Speculative verification's attention (DraftCheck then says which nodes stand): N <= 64 draft nodes,
+        parents[i] < i (-1: the prefix), appended after the prefix; node i attends the prefix and its root-to-node path. q (N, Hq, d), k/v
         (N, Hkv, d). Returns (out (N, Hq, d), flags); keep the accepted path with accept().
         A node's position is the prefix's length plus its depth (rotary positions; a window counts the
         prefix's last keys and the path's). Slopes are refused: distances are between cache slots, which
